@@ -380,6 +380,105 @@ int h3b_attention(const void* q, const void* q_scale, int q_gran, int q_block, i
                   const void* v_scale, int64_t H, const void* bitmap, float sm_scale, void* out,
                   int64_t out_row_stride, void* stream);
 
+/* ---------------------------------------------------------------- streaming attention
+ *
+ * Attention of new tokens over the keys before them, for video generated chunk by chunk
+ * and for the language models around it.  In a sequence of Lk keys the Lq queries are
+ * the last Lq tokens: query i stands at p = Lk - Lq + i and sees key j when p >= 0,
+ * j < Lk, j <= last(p), and last(p) - j < window or j < sinks.  last(p) = p for chunk 1;
+ * otherwise the end of p's chunk of `chunk` tokens (a latent frame), chunks counted from
+ * the end of the `sinks` first tokens (the packed prefix), which form one of their own.
+ * A query that sees no key gives 0.  Query head h reads kv head h / (Hq / Hkv).
+ * fp16 or bf16 (dtype 1 or 2) rows of heads of 128 channels, fp32 softmax and sums. */
+
+/* A paged K/V cache: pools [layers, pages, kv_heads, page_tokens, 128] that share one
+ * page table.  dtype: 1 fp16, 2 bf16, 3 e4m3 with k_scale / v_scale f32 [layers,
+ * kv_heads] (value = code * scale).  table int32 [table_rows, table_width]: the pages of
+ * each sequence in order, -1 where there is none; lens int32 [table_rows]: its tokens;
+ * refs int32 [pages]: table entries naming the page (0: free).  status int32 [1]: 0, or
+ * the reason why a call below could not be done.  Such a call changes nothing, and so do
+ * all h3b_pages_* calls after it until the caller clears the word.
+ * page_tokens: 16, 32, 64 or 128; table_rows <= 262144. */
+typedef struct h3b_page_cache {
+  void* k;
+  void* v;
+  int64_t layers, pages, kv_heads, page_tokens;
+  int dtype;
+  const float* k_scale;
+  const float* v_scale;
+  int32_t* table;
+  int64_t table_rows, table_width;
+  int32_t* lens;
+  int32_t* refs;
+  int32_t* status;
+} h3b_page_cache;
+/* values of the status word */
+#define H3B_PAGES_EXHAUSTED 1 /* not enough free pages */
+#define H3B_PAGES_TOO_LONG 2  /* a sequence would outgrow its row of the table */
+#define H3B_PAGES_BAD_SLOT 3  /* a slot outside the table, or named twice */
+#define H3B_PAGES_OCCUPIED 4  /* fork into a slot that holds tokens */
+#define H3B_PAGES_BAD_COUNT 5 /* token counts negative, unordered or beyond the length */
+#define H3B_PAGES_BAD_PAGE 6  /* a page outside the pool */
+
+/* Window attention over contiguous K/V.  q, out: rows [Tq, Hq * 128] with their strides;
+ * k, v: rows [Tk, Hkv * 128].  query_starts / key_starts: device int32 [seqs + 1], the
+ * first row of each sequence (ascending from 0 to Tq / Tk), both or neither (one
+ * sequence).  Query rows outside every sequence are not written. */
+int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                         int64_t v_row_stride, int dtype, int64_t Tq, int64_t Tk, const int32_t* query_starts,
+                         const int32_t* key_starts, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t window,
+                         int64_t sinks, int64_t chunk, float sm_scale, void* out, int64_t out_row_stride,
+                         void* stream);
+
+/* The same over one layer of a 16-bit paged cache of the queries' type: sequence i is
+ * table row slots[i] (NULL: row i), its queries the last tokens that the row holds. */
+int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, int64_t Tq, const int32_t* query_starts,
+                               const int32_t* slots, int64_t seqs, int64_t Hq, const h3b_page_cache* cache,
+                               int64_t layer, int64_t window, int64_t sinks, int64_t chunk, float sm_scale, void* out,
+                               int64_t out_row_stride, void* stream);
+
+/* Attention of one new token per sequence, the last of table row slots[i] (NULL: row i),
+ * over a 16-bit cache of the queries' type or an e4m3 cache.  q, out: rows [seqs,
+ * Hq * 128]; seqs <= 4096.  workspace: h3b_decode_workspace_bytes() bytes, 16-byte
+ * aligned, not shared by calls on different streams. */
+int64_t h3b_decode_workspace_bytes(void);
+int h3b_decode_attention(const void* q, int64_t q_row_stride, int dtype, const int32_t* slots, int64_t seqs, int64_t Hq,
+                         const h3b_page_cache* cache, int64_t layer, int64_t window, int64_t sinks, float sm_scale,
+                         void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Room for starts[i + 1] - starts[i] more tokens (starts NULL: one) in each of the n
+ * distinct slots: pages are taken lowest index first in the order of the slots, lengths
+ * grow.  A partly filled last page that other sequences share is replaced by a copy of
+ * its rows in every layer (the copy is the first page that its sequence takes).
+ * workspace: h3b_pages_workspace_bytes(n, pages) bytes. */
+int64_t h3b_pages_workspace_bytes(int64_t n, int64_t pages);
+int h3b_pages_extend(const h3b_page_cache* cache, const int32_t* slots, int64_t n, const int32_t* starts,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* K/V rows [tokens, kv_heads * 128] (fp16 or bf16, row strides) into the last
+ * starts[i + 1] - starts[i] tokens (NULL: one) of each slot, in one layer.  An e4m3
+ * pool holds x / scale, rounded to nearest even, saturated at +-448. */
+int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
+                    const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
+                    int64_t tokens, void* stream);
+
+/* Slots dst[i] (empty, distinct, none of them a source) become sequences that share the
+ * pages of src[i]. */
+int h3b_pages_fork(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* Each of the n distinct slots keeps its first keep[i] tokens (NULL: none); pages that
+ * no sequence names any more are free. */
+int h3b_pages_truncate(const h3b_page_cache* cache, const int32_t* slots, const int32_t* keep, int64_t n, void* stream);
+
+/* Moves the pages in use to the front of the pool, in every layer: of u pages in use the
+ * i-th at or after page u goes to the i-th free one before it.  workspace:
+ * h3b_pages_workspace_bytes(0, pages) bytes. */
+int h3b_pages_compact(const h3b_page_cache* cache, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Pages src[i] over pages dst[i] in every layer; no page both source and target.  The
+ * tables stay as they are. */
+int h3b_pages_copy(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

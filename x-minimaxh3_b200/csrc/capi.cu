@@ -7,6 +7,7 @@
 #include <string>
 
 #include "h3b_kernels.cuh"
+#include "streaming.cuh"
 
 namespace {
 
@@ -540,6 +541,270 @@ int h3b_attention(const void* q, const void* q_scale, int q_gran, int q_block, i
   if (r == 1) return fail(H3B_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
   if (r == 3) return fail(H3B_ERR_UNSUPPORTED, "attention: kernel register count differs from the planned split");
   return cuda_status(e, "attention");
+}
+
+// ---- streaming attention and its paged cache
+
+namespace {
+
+// Everything about a cache that can be checked on the host; 0 or the failure's status.
+int check_cache(const h3b_page_cache* c, int64_t layer, const char* what) {
+  const std::string w(what);
+  if (!c) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null cache");
+  if (!c->k || !c->v || !c->table || !c->lens || !c->refs || !c->status)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null pointer in the cache");
+  if (c->layers <= 0 || c->pages <= 0 || c->kv_heads <= 0 || c->table_rows <= 0 || c->table_width <= 0)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": cache sizes must be positive");
+  if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128)
+    return fail(H3B_ERR_UNSUPPORTED, w + ": page_tokens must be 16, 32, 64 or 128");
+  if (c->dtype < 1 || c->dtype > 3) return fail(H3B_ERR_UNSUPPORTED, w + ": cache dtype must be fp16, bf16 or e4m3");
+  if (c->dtype == 3 && (!c->k_scale || !c->v_scale))
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": an e4m3 cache needs k_scale and v_scale");
+  if (layer < 0 || layer >= c->layers) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": no such layer");
+  if (c->pages > (1 << 28) || c->table_rows > h3b::kPagesMaxRows || c->table_width * c->page_tokens > (1 << 30) ||
+      c->pages * c->kv_heads > INT_MAX || c->kv_heads > 65535)
+    return fail(H3B_ERR_UNSUPPORTED, w + ": cache too large");
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(H3B_ERR_UNSUPPORTED, w + ": pools must be 16-byte aligned");
+  return H3B_OK;
+}
+int elem_bytes(const h3b_page_cache* c) { return c->dtype == 3 ? 1 : 2; }
+h3b::PagedArgs paged_args(const h3b_page_cache* c, int64_t layer, const int32_t* slots) {
+  const int64_t at = layer * c->pages * c->kv_heads * c->page_tokens * 128 * elem_bytes(c);
+  h3b::PagedArgs p{};
+  p.k = static_cast<const char*>(c->k) + at;
+  p.v = static_cast<const char*>(c->v) + at;
+  p.pages = c->pages;
+  p.page = (int)c->page_tokens;
+  p.table = c->table;
+  p.width = (int)c->table_width;
+  p.rows = (int)c->table_rows;
+  p.lens = c->lens;
+  p.slots = slots;
+  return p;
+}
+h3b::PageTables page_tables(const h3b_page_cache* c) {
+  return {c->table, (int)c->table_rows, (int)c->table_width, c->lens, c->refs, (int)c->pages, (int)c->page_tokens,
+          c->status};
+}
+h3b::PagePools page_pools(const h3b_page_cache* c) {
+  return {static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->layers, (int)c->kv_heads, elem_bytes(c)};
+}
+// Shared checks of the attention entries: rows of Hq heads in q and out, the window rule.
+int check_rows(const void* q, int64_t q_stride, int dtype, int64_t rows, int64_t Hq, int64_t Hkv, int64_t window,
+               int64_t sinks, int64_t chunk, const void* out, int64_t out_stride, const char* what) {
+  const std::string w(what);
+  if (!q || !out) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null pointer");
+  if (rows < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": the query heads must be a multiple of the kv heads");
+  if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, w + ": dtype must be fp16 or bf16");
+  if (window < 0 || sinks < 0 || chunk < 1)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": need window >= 0, sinks >= 0 and chunk >= 1");
+  if (rows > (1 << 30) || Hq > 65535) return fail(H3B_ERR_UNSUPPORTED, w + ": too many rows or heads");
+  if (q_stride < Hq * 128 || q_stride % 8 || out_stride < Hq * 128 || out_stride % 8)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": bad row stride");
+  if (!aligned16(q) || !aligned16(out)) return fail(H3B_ERR_UNSUPPORTED, w + ": rows must be 16-byte aligned");
+  return H3B_OK;
+}
+int clip(int64_t x) { return x > (1 << 30) ? 1 << 30 : (int)x; }
+int window_status(int r, cudaError_t e, const char* what) {
+  if (r == 1) return fail(H3B_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed");
+  if (r == 3) return fail(H3B_ERR_UNSUPPORTED, std::string(what) + ": kernel register count differs from the planned split");
+  return cuda_status(e, what);
+}
+
+}  // namespace
+
+int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                         int64_t v_row_stride, int dtype, int64_t Tq, int64_t Tk, const int32_t* query_starts,
+                         const int32_t* key_starts, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t window,
+                         int64_t sinks, int64_t chunk, float sm_scale, void* out, int64_t out_row_stride,
+                         void* stream) {
+  if (Tq == 0) return ok();
+  int r = check_rows(q, q_row_stride, dtype, Tq, Hq, Hkv, window, sinks, chunk, out, out_row_stride, "window_attention");
+  if (r) return r;
+  if (Tk < 0 || Tk > (1 << 30) || seqs < 1 || seqs > (1 << 24)) return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: bad sizes");
+  if (Tk > 0 && (!k || !v)) return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: null pointer");
+  if ((query_starts == nullptr) != (key_starts == nullptr) || (!query_starts && seqs != 1))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: query_starts and key_starts come together");
+  if (Tk > 0 && (k_row_stride < Hkv * 128 || k_row_stride % 8 || v_row_stride < Hkv * 128 || v_row_stride % 8))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: bad K/V row stride");
+  if (!aligned16(k) || !aligned16(v)) return fail(H3B_ERR_UNSUPPORTED, "window_attention: K and V must be 16-byte aligned");
+  h3b::WindowArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_stride = q_row_stride;
+  a.k = static_cast<const uint16_t*>(k);
+  a.k_stride = k_row_stride;
+  a.v = static_cast<const uint16_t*>(v);
+  a.v_stride = v_row_stride;
+  a.Tq = (int)Tq;
+  a.Tk = (int)Tk;
+  a.seqs = (int)seqs;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.q_starts = query_starts;
+  a.k_starts = key_starts;
+  a.rule = {clip(window), clip(sinks), clip(chunk)};
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride = out_row_stride;
+  cudaError_t e = cudaSuccess;
+  r = h3b::launch_window_attention(a, dtype == 2, st(stream), &e);
+  return window_status(r, e, "window_attention");
+}
+
+int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, int64_t Tq, const int32_t* query_starts,
+                               const int32_t* slots, int64_t seqs, int64_t Hq, const h3b_page_cache* cache,
+                               int64_t layer, int64_t window, int64_t sinks, int64_t chunk, float sm_scale, void* out,
+                               int64_t out_row_stride, void* stream) {
+  if (Tq == 0) return ok();
+  int r = check_cache(cache, layer, "paged_window_attention");
+  if (r) return r;
+  r = check_rows(q, q_row_stride, dtype, Tq, Hq, cache->kv_heads, window, sinks, chunk, out, out_row_stride,
+                 "paged_window_attention");
+  if (r) return r;
+  if (cache->dtype != dtype)
+    return fail(H3B_ERR_UNSUPPORTED, "paged_window_attention: the cache must hold the queries' 16-bit type");
+  if (seqs < 1 || seqs > (1 << 24)) return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: bad sizes");
+  if (!query_starts && seqs != 1)
+    return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: several sequences need query_starts");
+  h3b::WindowArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_stride = q_row_stride;
+  a.Tq = (int)Tq;
+  a.seqs = (int)seqs;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)cache->kv_heads;
+  a.q_starts = query_starts;
+  a.rule = {clip(window), clip(sinks), clip(chunk)};
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride = out_row_stride;
+  a.paged = paged_args(cache, layer, slots);
+  cudaError_t e = cudaSuccess;
+  r = h3b::launch_window_attention(a, dtype == 2, st(stream), &e);
+  return window_status(r, e, "paged_window_attention");
+}
+
+int64_t h3b_decode_workspace_bytes(void) { return h3b::decode_workspace_bytes(); }
+
+int h3b_decode_attention(const void* q, int64_t q_row_stride, int dtype, const int32_t* slots, int64_t seqs, int64_t Hq,
+                         const h3b_page_cache* cache, int64_t layer, int64_t window, int64_t sinks, float sm_scale,
+                         void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (seqs == 0) return ok();
+  int r = check_cache(cache, layer, "decode_attention");
+  if (r) return r;
+  r = check_rows(q, q_row_stride, dtype, seqs, Hq, cache->kv_heads, window, sinks, 1, out, out_row_stride,
+                 "decode_attention");
+  if (r) return r;
+  if (cache->dtype != 3 && cache->dtype != dtype)
+    return fail(H3B_ERR_UNSUPPORTED, "decode_attention: the cache must hold the queries' type or e4m3");
+  if (seqs > h3b::kDecodeMaxSeqs) return fail(H3B_ERR_UNSUPPORTED, "decode_attention: more than 4096 sequences in a call");
+  if (seqs * Hq > INT_MAX) return fail(H3B_ERR_UNSUPPORTED, "decode_attention: too many heads");
+  if (!workspace || workspace_bytes < h3b::decode_workspace_bytes())
+    return fail(H3B_ERR_INVALID_ARGUMENT, "decode_attention: workspace too small");
+  if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "decode_attention: workspace must be 16-byte aligned");
+  h3b::DecodeArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_stride = q_row_stride;
+  a.seqs = (int)seqs;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)cache->kv_heads;
+  a.paged = paged_args(cache, layer, slots);
+  const bool e4m3 = cache->dtype == 3;
+  a.k_scale = e4m3 ? cache->k_scale + layer * cache->kv_heads : nullptr;
+  a.v_scale = e4m3 ? cache->v_scale + layer * cache->kv_heads : nullptr;
+  a.rule = {clip(window), clip(sinks), 1};
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride = out_row_stride;
+  a.partial = static_cast<float*>(workspace);
+  const int kind = e4m3 ? (dtype == 2 ? 2 : 3) : (dtype == 2 ? 0 : 1);
+  return cuda_status(h3b::launch_decode_attention(a, kind, st(stream)), "decode_attention");
+}
+
+int64_t h3b_pages_workspace_bytes(int64_t n, int64_t pages) { return h3b::pages_workspace_bytes(n, pages); }
+
+int h3b_pages_extend(const h3b_page_cache* cache, const int32_t* slots, int64_t n, const int32_t* starts,
+                     void* workspace, int64_t workspace_bytes, void* stream) {
+  if (n == 0) return ok();
+  const int r = check_cache(cache, 0, "pages_extend");
+  if (r) return r;
+  if (!slots) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_extend: null pointer");
+  if (n < 0 || n > cache->table_rows) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_extend: more sequences than table rows");
+  if (!workspace || workspace_bytes < h3b::pages_workspace_bytes(n, cache->pages))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_extend: workspace too small");
+  return cuda_status(h3b::launch_pages_extend(page_tables(cache), page_pools(cache), slots, (int)n, starts,
+                                              static_cast<int32_t*>(workspace), st(stream)), "pages_extend");
+}
+
+int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
+                    const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
+                    int64_t tokens, void* stream) {
+  if (n == 0 || tokens == 0) return ok();
+  const int r = check_cache(cache, layer, "pages_write");
+  if (r) return r;
+  if (!slots || !k || !v) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_write: null pointer");
+  if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, "pages_write: dtype must be fp16 or bf16");
+  if (cache->dtype != 3 && cache->dtype != dtype)
+    return fail(H3B_ERR_UNSUPPORTED, "pages_write: the cache must hold the rows' type or e4m3");
+  if (n < 0 || n > cache->table_rows || tokens < 0 || tokens > (1 << 30) || (!starts && tokens != n))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_write: bad sizes");
+  if (k_row_stride < cache->kv_heads * 128 || k_row_stride % 8 || v_row_stride < cache->kv_heads * 128 || v_row_stride % 8)
+    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_write: bad row stride");
+  if (!aligned16(k) || !aligned16(v)) return fail(H3B_ERR_UNSUPPORTED, "pages_write: rows must be 16-byte aligned");
+  h3b::PageWriteArgs w{};
+  w.k = static_cast<const uint16_t*>(k);
+  w.k_stride = k_row_stride;
+  w.v = static_cast<const uint16_t*>(v);
+  w.v_stride = v_row_stride;
+  w.tokens = tokens;
+  w.slots = slots;
+  w.n = (int)n;
+  w.starts = starts;
+  if (cache->dtype == 3) {
+    w.k_scale = cache->k_scale + layer * cache->kv_heads;
+    w.v_scale = cache->v_scale + layer * cache->kv_heads;
+  }
+  w.src_bf16 = dtype == 2;
+  return cuda_status(h3b::launch_pages_write(page_tables(cache), page_pools(cache), layer, w, st(stream)), "pages_write");
+}
+
+int h3b_pages_fork(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
+  if (n == 0) return ok();
+  const int r = check_cache(cache, 0, "pages_fork");
+  if (r) return r;
+  if (!src || !dst) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_fork: null pointer");
+  if (n < 0 || n > cache->table_rows) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_fork: more sequences than table rows");
+  return cuda_status(h3b::launch_pages_fork(page_tables(cache), src, dst, (int)n, st(stream)), "pages_fork");
+}
+
+int h3b_pages_truncate(const h3b_page_cache* cache, const int32_t* slots, const int32_t* keep, int64_t n, void* stream) {
+  if (n == 0) return ok();
+  const int r = check_cache(cache, 0, "pages_truncate");
+  if (r) return r;
+  if (!slots) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_truncate: null pointer");
+  if (n < 0 || n > cache->table_rows)
+    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_truncate: more sequences than table rows");
+  return cuda_status(h3b::launch_pages_truncate(page_tables(cache), slots, keep, (int)n, st(stream)), "pages_truncate");
+}
+
+int h3b_pages_compact(const h3b_page_cache* cache, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int r = check_cache(cache, 0, "pages_compact");
+  if (r) return r;
+  if (!workspace || workspace_bytes < h3b::pages_workspace_bytes(0, cache->pages))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_compact: workspace too small");
+  return cuda_status(h3b::launch_pages_compact(page_tables(cache), page_pools(cache), static_cast<int32_t*>(workspace),
+                                               st(stream)), "pages_compact");
+}
+
+int h3b_pages_copy(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
+  if (n == 0) return ok();
+  const int r = check_cache(cache, 0, "pages_copy");
+  if (r) return r;
+  if (!src || !dst) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_copy: null pointer");
+  if (n < 0 || n > cache->pages) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_copy: more pairs than pages");
+  return cuda_status(h3b::launch_pages_copy(page_pools(cache), (int)cache->pages, (int)cache->page_tokens, src, dst, (int)n,
+                                            cache->status, st(stream)), "pages_copy");
 }
 
 }  // extern "C"

@@ -1,0 +1,554 @@
+// decode_attn.cu -- attention of one new token per sequence over a paged K/V cache.
+//
+//   out[h] = sum_j softmax_j(scale * q[h] . k_j) v_j over the visible keys j
+//
+// Bound by reading K and V once.  The keys are cut into chunks of 16 (inside one page)
+// and the chunks of all (sequence, kv head) pairs into one list that every warp of a
+// persistent grid takes an equal, contiguous part of, so ragged lengths and few long
+// sequences load the card alike.  A pair whose chunks span several warps is joined by
+// a second kernel from fp32 partial sums with their softmax statistics.
+//
+// A warp keeps its chunk in registers, without shared memory:
+//   S^T = K . Q^T   m16n8k16, M = 16 keys, N = 8 heads of the group.  The products'
+//                   order over the 128 channels is free, so each thread loads 16
+//                   contiguous bytes of its key rows and the matching ones of Q.
+//   P^T             exp2 of S^T under the running maximum; the accumulator layout of
+//                   S^T becomes the B operand by one 8 x 8 transpose per 8 keys
+//   O^T += V^T . P^T  M = 16 channels, N = 8 heads, K = 16 keys: the A operand pairs
+//                   two keys of one channel, one byte permute per register
+// E4M3 caches are widened to fp16 (exact) with q in fp16 under a power of two per head.
+#include "streaming.cuh"
+
+namespace h3b {
+
+namespace {
+
+constexpr int kDecodeThreads = 128;
+constexpr int kChunk = 16;
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// streamed once: no place in L1
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two E4M3 bytes (low half of w, or high half) -> two fp16
+__device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) return bf16x2_bits(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// workspace: int64 prefix[kDecodeMaxSeqs + 1] (chunks before each sequence, one kv head
+// and row group), int64 share; then per (worker, slot) R rows of 128 sums and of (m, l)
+constexpr int64_t kDecodeHeader = (kDecodeMaxSeqs + 2) * 8;
+
+// The chunks of a sequence: those of the first tokens, then those of the window.
+struct ChunkList {
+  int first_n;  // chunks of the first tokens (0 when the window's chunks join them)
+  int win;      // first chunk of the window
+  int n;
+};
+__device__ __forceinline__ ChunkList chunk_list(const VisibleKeys& v) {
+  const int end = (v.end + kChunk - 1) / kChunk, firsts = (v.sinks + kChunk - 1) / kChunk, win = v.lo / kChunk;
+  if (v.lo >= v.end) return {firsts, end, firsts};  // no windowed key
+  if (v.sinks == 0) return {0, win, end - win};
+  if (firsts >= win) return {0, 0, end};
+  return {firsts, win, firsts + end - win};
+}
+
+template <int NT>
+__device__ __forceinline__ float* partial_rows(float* ws, int64_t worker, int slot) {
+  return ws + kDecodeHeader / 4 + (worker * 2 + slot) * (int64_t)(NT * 8) * 128;
+}
+template <int NT>
+__device__ __forceinline__ float* partial_stats(float* ws, int64_t workers, int64_t worker, int slot) {
+  return ws + kDecodeHeader / 4 + workers * 2 * (int64_t)(NT * 8) * 128 + (worker * 2 + slot) * (int64_t)(NT * 16);
+}
+
+// FP8: E4M3 cache; BF16: type of q and out (and of a 16-bit cache); NT: 8-head groups
+// a warp takes together.
+template <bool BF16, bool FP8, int NT, int MINB>
+__global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs a) {
+  extern __shared__ int64_t prefix[];  // [seqs + 1]
+  __shared__ int64_t carry;
+  __shared__ int64_t warp_sum[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int group = a.Hq / a.Hkv;
+  const int groups = (group + NT * 8 - 1) / (NT * 8);  // row groups of a kv head
+  const int heads = a.Hkv * groups;                    // (kv head, row group) pairs
+
+  if (threadIdx.x == 0) {
+    carry = 0;
+    prefix[0] = 0;
+  }
+  __syncthreads();
+  for (int base = 0; base < a.seqs; base += kDecodeThreads) {
+    const int i = base + threadIdx.x;
+    int64_t n = 0;
+    if (i < a.seqs) {
+      const int len = paged_len(a.paged, paged_slot(a.paged, i));
+      n = chunk_list(visible_keys(a.rule, len - 1, len)).n;
+    }
+    int64_t x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int64_t before = carry;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    if (i < a.seqs) prefix[i + 1] = before + x;
+    __syncthreads();
+    if (threadIdx.x == kDecodeThreads - 1) carry = before + x;
+    __syncthreads();
+  }
+  const int64_t total = prefix[a.seqs] * heads;
+  const int64_t share = (total + a.workers - 1) / a.workers;
+  if (blockIdx.x == 0) {
+    int64_t* head = reinterpret_cast<int64_t*>(a.partial);
+    for (int i = threadIdx.x; i <= a.seqs; i += kDecodeThreads) head[i] = prefix[i];
+    if (threadIdx.x == 0) head[kDecodeMaxSeqs + 1] = share;
+  }
+  const int64_t worker = (int64_t)blockIdx.x * (kDecodeThreads / 32) + warp;
+  int64_t at = worker * share;
+  const int64_t stop = min(at + share, total);
+  if (worker >= a.workers || at >= stop) return;
+
+  int b;
+  {
+    int lo = 0, hi = a.seqs - 1;  // the last sequence whose chunks begin at or before `at`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] * heads <= at) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+  }
+  bool first_piece = true;
+  while (at < stop) {
+    while (prefix[b + 1] * heads <= at) ++b;
+    const int64_t n_seq = prefix[b + 1] - prefix[b];
+    const int64_t in_seq = at - prefix[b] * heads;
+    const int hp = (int)(in_seq / n_seq);
+    const int c0 = (int)(in_seq - hp * n_seq);
+    const int c1 = (int)min(n_seq, (int64_t)c0 + (stop - at));
+    const int kh = hp / groups, r0 = (hp % groups) * NT * 8;
+    const int slot = paged_slot(a.paged, b);
+    const int len = paged_len(a.paged, slot);
+    const VisibleKeys see = visible_keys(a.rule, len - 1, len);
+    const ChunkList cl = chunk_list(see);
+
+    // Q of head r0 + 8 t + g: the channels this thread's K loads bring
+    uint32_t qf[NT][8][2];
+    float sc[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = r0 + t * 8 + g;
+      const uint16_t* qp = a.q + b * a.q_stride + ((int64_t)kh * group + r) * 128;
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // 16-bit: channels 32 i + 8 c + 0..7; E4M3: 64 (i / 2) + 16 c + 8 (i % 2) + 0..7
+        const int d = FP8 ? (i >> 1) * 64 + c * 16 + (i & 1) * 8 : i * 32 + c * 8;
+        w[i] = r < group ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
+      }
+      float up = 1.f;
+      if constexpr (FP8 && BF16) {
+        // bf16 q -> fp16 under a power of two: the head's largest |q| comes to [1, 2)
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(ws[e])), fabsf(bf16_hi(ws[e]))));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int ex = (int)(__float_as_uint(mx) >> 23) - 127;  // of a normal, finite maximum
+        float down = 1.f;
+        if (mx > 0.f && ex > -126 && ex < 127) {
+          up = __uint_as_float((uint32_t)(ex + 127) << 23);
+          down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t* ws = reinterpret_cast<uint32_t*>(&w[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ws[e] = pack16<false>(bf16_lo(ws[e]) * down, bf16_hi(ws[e]) * down);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qf[t][2 * i][0] = w[i].x;
+        qf[t][2 * i][1] = w[i].y;
+        qf[t][2 * i + 1][0] = w[i].z;
+        qf[t][2 * i + 1][1] = w[i].w;
+      }
+      const float s = a.scale_log2 * (FP8 ? a.k_scale[kh] : 1.f);
+      // the score columns of this thread are heads 2c and 2c + 1 of the tile
+      sc[t][0] = s * __shfl_sync(0xffffffffu, up, 8 * c);
+      sc[t][1] = s * __shfl_sync(0xffffffffu, up, 8 * c + 4);
+    }
+
+    float o[NT][8][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+    }
+
+    constexpr int kEB = FP8 ? 1 : 2;           // bytes per element
+    constexpr int kKL = FP8 ? 2 : 4;           // 16-byte loads of a key row per thread
+    constexpr int kVL = FP8 ? 1 : 2;
+    uint4 kr[2][kKL], vr[4][kVL];
+    int pgs = 0, pbase = c0 - 32;
+    auto chunk_of = [&](int ord) { return ord < cl.first_n ? ord : ord - cl.first_n + cl.win; };
+    // byte offset of key row 0 of chunk ordinal `ord`; page numbers come 32 chunks at a time
+    auto offset_of = [&](int ord) -> int64_t {
+      if (ord - pbase >= 32) {
+        pbase = ord;
+        const int o2 = min(ord + lane, c1 - 1);
+        pgs = (int)paged_page(a.paged, slot, chunk_of(o2) * kChunk / a.paged.page);
+      }
+      const int64_t pg = __shfl_sync(0xffffffffu, pgs, ord - pbase);
+      return ((pg * a.Hkv + kh) * a.paged.page + (chunk_of(ord) * kChunk & (a.paged.page - 1))) * (int64_t)(128 * kEB);
+    };
+    auto load_k = [&](int64_t off) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.paged.k) + off + g * (128 * kEB) + c * 16;
+#pragma unroll
+      for (int i = 0; i < kKL; ++i) {
+        kr[0][i] = ld_stream(p + i * 64);
+        kr[1][i] = ld_stream(p + i * 64 + 8 * 128 * kEB);
+      }
+    };
+    auto load_v = [&](int64_t off) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.paged.v) + off + 2 * c * (128 * kEB) + g * 16;
+#pragma unroll
+      for (int i = 0; i < kVL; ++i) {
+        vr[0][i] = ld_stream(p + i * 128);
+        vr[1][i] = ld_stream(p + i * 128 + 128 * kEB);
+        vr[2][i] = ld_stream(p + i * 128 + 8 * 128 * kEB);
+        vr[3][i] = ld_stream(p + i * 128 + 9 * 128 * kEB);
+      }
+    };
+    int64_t off = offset_of(c0);
+    load_k(off);
+    load_v(off);
+    for (int ord = c0; ord < c1; ++ord) {
+      const int j0 = chunk_of(ord) * kChunk;
+      float s[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+        if constexpr (FP8) {
+#pragma unroll
+          for (int i = 0; i < kKL; ++i) {
+            const uint32_t x[4] = {kr[0][i].x, kr[0][i].y, kr[0][i].z, kr[0][i].w};
+            const uint32_t y[4] = {kr[1][i].x, kr[1][i].y, kr[1][i].z, kr[1][i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mma16816<false>(s[t], widen_lo(x[e]), widen_lo(y[e]), widen_hi(x[e]), widen_hi(y[e]),
+                              qf[t][4 * i + e][0], qf[t][4 * i + e][1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kKL; ++i) {
+            mma16816<BF16>(s[t], kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y, qf[t][2 * i][0], qf[t][2 * i][1]);
+            mma16816<BF16>(s[t], kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w, qf[t][2 * i + 1][0],
+                           qf[t][2 * i + 1][1]);
+          }
+        }
+      }
+      int64_t next = 0;
+      if (ord + 1 < c1) {
+        next = offset_of(ord + 1);
+        load_k(next);
+      }
+      const bool whole = j0 + kChunk <= see.end && (j0 >= see.lo || j0 + kChunk <= see.sinks);
+      uint32_t hide = 0;  // bit 0: key j0 + g is invisible, bit 1: key j0 + g + 8
+      if (!whole) {
+        auto seen = [&](int j) { return j < see.end && (j >= see.lo || j < see.sinks); };
+        hide = (seen(j0 + g) ? 0u : 1u) | (seen(j0 + g + 8) ? 0u : 2u);
+        // what lies in invisible rows (stale or never written) must not meet P = 0
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (!seen(j0 + 2 * c + (kk & 1) + (kk >> 1) * 8)) {
+#pragma unroll
+            for (int i = 0; i < kVL; ++i) vr[kk][i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float x[4] = {s[t][0] * sc[t][0], s[t][1] * sc[t][1], s[t][2] * sc[t][0], s[t][3] * sc[t][1]};
+        if (hide & 1) x[0] = x[1] = -INFINITY;
+        if (hide & 2) x[2] = x[3] = -INFINITY;
+        float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+        }
+        const float n0 = fmaxf(m[t][0], mx0), n1 = fmaxf(m[t][1], mx1);
+        if (__any_sync(0xffffffffu, n0 != m[t][0] || n1 != m[t][1])) {
+          const float a0 = n0 == m[t][0] ? 1.f : exp2_fast(m[t][0] - n0);
+          const float a1 = n1 == m[t][1] ? 1.f : exp2_fast(m[t][1] - n1);
+          m[t][0] = n0;
+          m[t][1] = n1;
+          l[t][0] *= a0;
+          l[t][1] *= a1;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[t][i][0] *= a0;
+            o[t][i][1] *= a1;
+            o[t][i][2] *= a0;
+            o[t][i][3] *= a1;
+          }
+        }
+        // a maximum of -inf (nothing seen yet) subtracts as 0: exp2(-inf) = 0
+        const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;
+        const float p0 = exp2_fast(x[0] - f0), p1 = exp2_fast(x[1] - f1);
+        const float p2 = exp2_fast(x[2] - f0), p3 = exp2_fast(x[3] - f1);
+        l[t][0] += p0 + p2;
+        l[t][1] += p1 + p3;
+        // P rounds to the 16-bit type of the V product; its sum stays in fp32
+        pb[t][0] = transpose8x8(pack16<BF16 && !FP8>(p0, p1));
+        pb[t][1] = transpose8x8(pack16<BF16 && !FP8>(p2, p3));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if constexpr (FP8) {
+            const uint4& v = vr[kk][0];
+            const uint32_t word = (i >> 1) == 0 ? v.x : (i >> 1) == 1 ? v.y : (i >> 1) == 2 ? v.z : v.w;
+            w[kk] = (i & 1) ? widen_hi(word) : widen_lo(word);
+          } else {
+            const uint4& v = vr[kk][i >> 2];
+            w[kk] = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+          }
+        }
+        const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);
+        const uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816<BF16 && !FP8>(o[t][i], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+      }
+      if (ord + 1 < c1) load_v(next);
+    }
+
+    // channels of accumulator tile i, elements 0/1 (even) and 2/3 (odd): d, d + 1
+    auto channel = [&](int i) { return FP8 ? g * 16 + 2 * i : (i >> 2) * 64 + g * 8 + (i & 3) * 2; };
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[t][0] += __shfl_xor_sync(0xffffffffu, l[t][0], d);
+        l[t][1] += __shfl_xor_sync(0xffffffffu, l[t][1], d);
+      }
+    }
+    if (c0 == 0 && c1 == n_seq) {
+      const float vs = FP8 ? a.v_scale[kh] : 1.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = r0 + t * 8 + 2 * c + e;
+          if (r < group) {
+            const float inv = (l[t][e] == 0.f ? 0.f : 1.f / l[t][e]) * vs;
+            uint16_t* dst = a.out + b * a.out_stride + ((int64_t)kh * group + r) * 128;
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              uint4 w;
+              w.x = pack16<BF16>(o[t][i][e] * inv, o[t][i][2 + e] * inv);
+              w.y = pack16<BF16>(o[t][i + 1][e] * inv, o[t][i + 1][2 + e] * inv);
+              w.z = pack16<BF16>(o[t][i + 2][e] * inv, o[t][i + 2][2 + e] * inv);
+              w.w = pack16<BF16>(o[t][i + 3][e] * inv, o[t][i + 3][2 + e] * inv);
+              *reinterpret_cast<uint4*>(dst + channel(i)) = w;
+            }
+          }
+        }
+      }
+    } else {
+      const int ps = first_piece ? 0 : 1;
+      float* rows = partial_rows<NT>(a.partial, worker, ps);
+      float* stats = partial_stats<NT>(a.partial, a.workers, worker, ps);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = t * 8 + 2 * c + e;
+#pragma unroll
+          for (int i = 0; i < 8; i += 2)
+            *reinterpret_cast<float4*>(rows + r * 128 + channel(i)) =
+                make_float4(o[t][i][e], o[t][i][2 + e], o[t][i + 1][e], o[t][i + 1][2 + e]);
+          if (g == 0) *reinterpret_cast<float2*>(stats + r * 2) = make_float2(m[t][e], l[t][e]);
+        }
+      }
+    }
+    first_piece = false;
+    at += c1 - c0;
+  }
+}
+
+// Joins the partial sums of one head: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p,
+// in the order of the keys.  Heads that one warp finished are left alone; a head without
+// any visible key gives 0.
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(256) decode_join_kernel(DecodeArgs a) {
+  extern __shared__ float weight[];  // [workers]
+  __shared__ float red[8];
+  __shared__ float acc2[128];
+  const int group = a.Hq / a.Hkv, groups = (group + NT * 8 - 1) / (NT * 8), heads = a.Hkv * groups;
+  const int b = blockIdx.x / heads, hp = blockIdx.x % heads;
+  const int kh = hp / groups, r = blockIdx.y, head = (hp % groups) * NT * 8 + r;
+  if (head >= group) return;
+  const int64_t* prefix = reinterpret_cast<const int64_t*>(a.partial);
+  const int64_t share = prefix[kDecodeMaxSeqs + 1];
+  const int64_t n = prefix[b + 1] - prefix[b];
+  uint16_t* dst = a.out + b * a.out_stride + ((int64_t)kh * group + head) * 128;
+  const int tid = threadIdx.x, d = tid & 127, half = tid >> 7;
+  if (n == 0) {
+    if (tid < 64) reinterpret_cast<uint32_t*>(dst)[tid] = 0u;
+    return;
+  }
+  const int64_t s0 = prefix[b] * heads + hp * n, s1 = s0 + n;
+  const int64_t w0 = s0 / share, w1 = (s1 - 1) / share;
+  if (w0 == w1) return;
+  const int parts = (int)(w1 - w0 + 1);
+  auto slot_of = [&](int p) { return (w0 + p) * share >= s0 ? 0 : 1; };
+  float mx = -INFINITY;
+  for (int p = tid; p < parts; p += 256) {
+    const float v = partial_stats<NT>(a.partial, a.workers, w0 + p, slot_of(p))[r * 2];
+    weight[p] = v;
+    mx = fmaxf(mx, v);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if ((tid & 31) == 0) red[tid >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx = fmaxf(mx, red[i]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float total = 0.f;
+  for (int p = tid; p < parts; p += 256) {
+    const float w = exp2f(weight[p] - base);
+    weight[p] = w;
+    total = fmaf(w, partial_stats<NT>(a.partial, a.workers, w0 + p, slot_of(p))[r * 2 + 1], total);
+  }
+  __syncthreads();
+  total = warp_butterfly_sum(total);
+  if ((tid & 31) == 0) red[tid >> 5] = total;
+  __syncthreads();
+  total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total += red[i];
+  float acc = 0.f;
+#pragma unroll 8
+  for (int p = half; p < parts; p += 2)
+    acc = fmaf(weight[p], partial_rows<NT>(a.partial, w0 + p, slot_of(p))[r * 128 + d], acc);
+  if (half) acc2[d] = acc;
+  __syncthreads();
+  if (!half) {
+    const float inv = (total == 0.f ? 0.f : 1.f / total) * (a.v_scale ? a.v_scale[kh] : 1.f);
+    const float v = (acc + acc2[d]) * inv;
+    if constexpr (BF16)
+      dst[d] = f32_to_bf16_bits(v);
+    else
+      dst[d] = __half_as_ushort(__float2half_rn(v));
+  }
+}
+
+constexpr int kMinBlocks = 4;  // most blocks an SM runs in any variant (sizes the workspace)
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return n;
+}
+
+template <bool BF16, bool FP8, int NT, int MINB>
+cudaError_t launch_decode(DecodeArgs a, cudaStream_t s) {
+  const int sms = sm_count();
+  if (sms <= 0) return cudaErrorNoDevice;
+  const int group = a.Hq / a.Hkv;
+  const int64_t heads = (int64_t)a.Hkv * ((group + NT * 8 - 1) / (NT * 8));
+  const int64_t most = (int64_t)a.seqs * heads * (((int64_t)a.paged.width * a.paged.page + kChunk - 1) / kChunk);
+  constexpr int kWarps = kDecodeThreads / 32;
+  int64_t blocks = (most + kWarps - 1) / kWarps;
+  if (blocks > (int64_t)sms * MINB) blocks = (int64_t)sms * MINB;
+  if (blocks < 1) blocks = 1;
+  a.workers = (int)blocks * kWarps;
+  const size_t smem = (size_t)(a.seqs + 1) * 8;
+  decode_kernel<BF16, FP8, NT, MINB><<<(unsigned)blocks, kDecodeThreads, smem, s>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  dim3 grid((unsigned)(a.seqs * heads), (unsigned)(group < NT * 8 ? group : NT * 8));
+  decode_join_kernel<BF16, NT><<<grid, 256, (size_t)a.workers * 4, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int64_t decode_workspace_bytes() {
+  const int sms = sm_count();
+  // NT = 1 at kMinBlocks blocks per SM and NT = 2 at half of that need the same
+  return kDecodeHeader + (int64_t)sms * kMinBlocks * (kDecodeThreads / 32) * 2 * 8 * (128 + 2) * 4;
+}
+
+cudaError_t launch_decode_attention(DecodeArgs a, int kind, cudaStream_t s) {
+  const bool wide = a.Hq / a.Hkv > 8;
+  switch (kind) {
+    case 0: return wide ? launch_decode<true, false, 2, 2>(a, s) : launch_decode<true, false, 1, 3>(a, s);
+    case 1: return wide ? launch_decode<false, false, 2, 2>(a, s) : launch_decode<false, false, 1, 3>(a, s);
+    case 2: return wide ? launch_decode<true, true, 2, 2>(a, s) : launch_decode<true, true, 1, 4>(a, s);
+    default: return wide ? launch_decode<false, true, 2, 2>(a, s) : launch_decode<false, true, 1, 4>(a, s);
+  }
+}
+
+}  // namespace h3b

@@ -8,4 +8,7 @@
 #include "attn.cu"
 #include "ulysses.cu"
 #include "adaln.cu"
+#include "window_attn.cu"
+#include "decode_attn.cu"
+#include "kv_pages.cu"
 #include "capi.cu"

@@ -40,6 +40,30 @@ class MaskParams(ctypes.Structure):
     ]
 
 
+class PageCacheStruct(ctypes.Structure):
+    """h3b_page_cache (include/h3b.h)."""
+
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("layers", c_int64),
+        ("pages", c_int64),
+        ("kv_heads", c_int64),
+        ("page_tokens", c_int64),
+        ("dtype", c_int),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("table", c_void_p),
+        ("table_rows", c_int64),
+        ("table_width", c_int64),
+        ("lens", c_void_p),
+        ("refs", c_void_p),
+        ("status", c_void_p),
+    ]
+
+
+_cache_p = ctypes.POINTER(PageCacheStruct)
+
 # name -> argtypes (all return int status unless listed in _RESTYPES)
 _SIGNATURES = {
     "h3b_version": [],
@@ -89,9 +113,26 @@ _SIGNATURES = {
     "h3b_bitmap_to_lut": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
     "h3b_attention": [c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
                       c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p],
+    "h3b_window_attention": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p,
+                             c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
+                             c_int64, c_void_p],
+    "h3b_paged_window_attention": [c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, _cache_p,
+                                   c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p],
+    "h3b_decode_workspace_bytes": [],
+    "h3b_decode_attention": [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, _cache_p, c_int64, c_int64, c_int64,
+                             c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p],
+    "h3b_pages_workspace_bytes": [c_int64, c_int64],
+    "h3b_pages_extend": [_cache_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
+    "h3b_pages_write": [_cache_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                        c_int64, c_void_p],
+    "h3b_pages_fork": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "h3b_pages_truncate": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "h3b_pages_compact": [_cache_p, c_void_p, c_int64, c_void_p],
+    "h3b_pages_copy": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
 }
 _RESTYPES = {"h3b_version": ctypes.c_char_p, "h3b_last_error": ctypes.c_char_p,
-             "h3b_key_mean_workspace_bytes": c_int64}
+             "h3b_key_mean_workspace_bytes": c_int64, "h3b_decode_workspace_bytes": c_int64,
+             "h3b_pages_workspace_bytes": c_int64}
 
 EXPORTED = tuple(_SIGNATURES)
 
@@ -121,7 +162,8 @@ def lib():
 
 
 # kernels each entry launches (for the benchmark's launch count); default 1
-_KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2}
+_KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2, "decode_attention": 2, "pages_extend": 2,
+                     "pages_compact": 3}
 _launches = 0
 
 

@@ -1,0 +1,180 @@
+"""Streaming attention over libh3b.so: new tokens attend to the keys before them.
+
+Where the backends of `attention` take a whole sequence, bidirectionally and quantized,
+these take the tokens that come next -- a video chunk by chunk, a prompt, one decoded
+token -- in bf16 or fp16, with grouped heads and ragged batches:
+
+* window_attention        contiguous K/V
+* paged_window_attention  K/V of a 16-bit PagedKVCache
+* decode_attention        one new token per sequence, 16-bit or e4m3 cache
+* WindowAttentionB200     an AttentionBackend callable (q, k, v [L, H, 128]) over
+                          window_attention: sinks, chunk and window follow from the
+                          request's protected prefix and video layout
+
+Of a sequence's Lk keys the Lq queries are the last Lq tokens.  The query at position
+p = Lk - Lq + i sees key j when j <= last(p) and (last(p) - j < window or j < sinks).
+last(p) = p, or with chunk > 1 the end of p's chunk (a latent frame sees itself whole),
+chunks counted from the end of the `sinks` first tokens, which form one of their own.
+A query that sees nothing gives 0.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import context as _context
+from ._lib import check, lib
+from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _token_rows
+from .ops import _cuda, _p, _stream
+
+UNLIMITED = 1 << 30
+
+
+def _rule(window: int | None, sinks: int, chunk: int) -> tuple[int, int, int]:
+    window = UNLIMITED if window is None else int(window)
+    sinks, chunk = int(sinks), int(chunk)
+    if window < 0 or sinks < 0 or chunk < 1:
+        raise ValueError("need window >= 0, sinks >= 0 and chunk >= 1")
+    return window, sinks, chunk
+
+
+def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda:
+        raise ValueError("out must have q's shape and type")
+    st = out.stride()
+    if st[2] != 1 or st[1] != HEAD_DIM or st[0] % 8 or st[0] < q.shape[1] * HEAD_DIM or out.data_ptr() % 16:
+        raise ValueError("out must have contiguous heads and 16-byte aligned rows")
+    return out
+
+
+def _scale(scale: float | None) -> float:
+    return 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
+                     chunk: int = 1, scale: float | None = None, query_starts: torch.Tensor | None = None,
+                     key_starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """q [Tq, Hq, 128], k / v [Tk, Hkv, 128] -> [Tq, Hq, 128]; bf16 or fp16.
+
+    query_starts / key_starts: int32 [sequences + 1] first rows of each sequence of a
+    ragged batch (from 0 to Tq / Tk); None: one sequence."""
+    _cuda("window_attention", q, k, v)
+    q, k, v = _token_rows(q, None, "q"), _token_rows(k, None, "k"), _token_rows(v, None, "v")
+    if k.shape != v.shape or not q.dtype == k.dtype == v.dtype:
+        raise ValueError("k and v must have one shape, and q their type")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("the query heads must be a multiple of the kv heads")
+    window, sinks, chunk = _rule(window, sinks, chunk)
+    seqs = 1
+    if (query_starts is None) != (key_starts is None):
+        raise ValueError("query_starts and key_starts come together")
+    if query_starts is not None:
+        seqs = _index(query_starts, "query_starts").numel() - 1
+        _index(key_starts, "key_starts", seqs + 1)
+        if seqs < 1:
+            raise ValueError("query_starts needs at least two entries")
+    out = _output(out, q)
+    check(lib().h3b_window_attention(_p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0), DTYPE_CODES[q.dtype],
+                                     q.shape[0], k.shape[0], _p(query_starts), _p(key_starts), seqs, q.shape[1],
+                                     k.shape[1], window, sinks, chunk, _scale(scale), _p(out), out.stride(0),
+                                     _stream(q)), "window_attention")
+    return out
+
+
+def _cached_queries(q: torch.Tensor, cache: PagedKVCache, layer: int, what: str) -> torch.Tensor:
+    _cuda(what, q)
+    q = _token_rows(q, None, "q")
+    if q.shape[1] == 0 or q.shape[1] % cache.k.shape[2]:
+        raise ValueError("the query heads must be a multiple of the kv heads")
+    if not 0 <= layer < cache.k.shape[0]:
+        raise ValueError(f"the cache has no layer {layer}")
+    return q
+
+
+def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor | None = None, *,
+                           window: int | None = None, sinks: int = 0, chunk: int = 1, scale: float | None = None,
+                           query_starts: torch.Tensor | None = None, layer: int = 0,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """q [Tq, Hq, 128]: the last tokens of the cache's sequences `slots` (int32; None: slot 0, 1, ...),
+    already appended.  query_starts: int32 [sequences + 1]; None: one sequence."""
+    q = _cached_queries(q, cache, layer, "paged_window_attention")
+    if cache.k.dtype != q.dtype:
+        raise ValueError(f"a {cache.k.dtype} cache does not serve {q.dtype} queries of several tokens")
+    window, sinks, chunk = _rule(window, sinks, chunk)
+    seqs = 1 if query_starts is None else _index(query_starts, "query_starts").numel() - 1
+    if seqs < 1:
+        raise ValueError("query_starts needs at least two entries")
+    if slots is not None:
+        _index(slots, "slots", seqs)
+    elif seqs > cache.table.shape[0]:
+        raise ValueError("more sequences than the cache has slots")
+    out = _output(out, q)
+    check(lib().h3b_paged_window_attention(_p(q), q.stride(0), DTYPE_CODES[q.dtype], q.shape[0], _p(query_starts),
+                                           _p(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
+                                           _scale(scale), _p(out), out.stride(0), _stream(q)),
+          "paged_window_attention")
+    return out
+
+
+def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor | None = None, *,
+                     window: int | None = None, sinks: int = 0, scale: float | None = None, layer: int = 0,
+                     out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """q [n, Hq, 128]: the last token of each of the cache's sequences `slots` (int32 [n]; None: slots
+    0..n-1), already appended -> [n, Hq, 128].  workspace: uint8, reused by calls on one stream."""
+    q = _cached_queries(q, cache, layer, "decode_attention")
+    if cache.k.dtype not in (q.dtype, torch.float8_e4m3fn):
+        raise ValueError(f"a {cache.k.dtype} cache does not serve {q.dtype} queries")
+    window, sinks, _ = _rule(window, sinks, 1)
+    n = q.shape[0]
+    if slots is not None:
+        _index(slots, "slots", n)
+    elif n > cache.table.shape[0]:
+        raise ValueError("more sequences than the cache has slots")
+    need = lib().h3b_decode_workspace_bytes()
+    if workspace is None:
+        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+    elif workspace.numel() * workspace.element_size() < need or not workspace.is_cuda:
+        raise ValueError(f"the workspace must have {need} bytes on the device")
+    out = _output(out, q)
+    check(lib().h3b_decode_attention(_p(q), q.stride(0), DTYPE_CODES[q.dtype], _p(slots), n, q.shape[1], cache._ref,
+                                     layer, window, sinks, _scale(scale), _p(out), out.stride(0), _p(workspace), need,
+                                     _stream(q)), "decode_attention")
+    return out
+
+
+class WindowAttentionB200:
+    """Streaming backend (q, k, v: bf16 [L, H, 128]; fewer queries than keys for a next chunk).
+
+    The request's protected prefix stays visible (sinks) and its video layout sets the
+    chunk: every latent frame sees itself, the prefix and the `frames` - 1 frames before
+    it (all of them when `frames` is None).  Without a layout attention is causal with a
+    window of `tokens` (None: unlimited)."""
+
+    approximate = True
+
+    def __init__(self, frames: int | None = None, tokens: int | None = None, context=None) -> None:
+        if frames is not None and frames < 1 or tokens is not None and tokens < 1:
+            raise ValueError("a window holds at least one frame and one token")
+        self.frames, self.tokens = frames, tokens
+        self.context = context if context is not None else _context
+
+    def rule(self) -> dict:
+        """window, sinks and chunk of the current request."""
+        prefix = int(_context.source_getter(self.context, "current_attention_protected_prefix", 0))
+        layout = _context.source_getter(self.context, "current_attention_video_layout", None)
+        if layout is None:
+            return dict(window=self.tokens, sinks=prefix, chunk=1)
+        chunk = int(layout[1])
+        return dict(window=None if self.frames is None else self.frames * chunk, sinks=prefix, chunk=chunk)
+
+    def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        return window_attention(q, k, v, **self.rule())
+
+    def cached(self, q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor, layer: int = 0,
+               query_starts: torch.Tensor | None = None) -> torch.Tensor:
+        """The same over a paged cache that already holds the new tokens."""
+        return paged_window_attention(q, cache, slots, layer=layer, query_starts=query_starts, **self.rule())
