@@ -389,7 +389,8 @@ int h3b_attention(const void* q, const void* q_scale, int q_gran, int q_block, i
  * otherwise the end of p's chunk of `chunk` tokens (a latent frame), chunks counted from
  * the end of the `sinks` first tokens (the packed prefix), which form one of their own.
  * A query that sees no key gives 0.  Query head h reads kv head h / (Hq / Hkv).
- * fp16 or bf16 (dtype 1 or 2) rows of heads of 128 channels, fp32 softmax and sums. */
+ * fp16 or bf16 (dtype 1 or 2) rows of heads of 128 channels, fp32 softmax and sums;
+ * sm_scale positive and finite. */
 
 /* A paged K/V cache: pools [layers, pages, kv_heads, page_tokens, 128] that share one
  * page table.  dtype: 1 fp16, 2 bf16, 3 e4m3 with k_scale / v_scale f32 [layers,

@@ -591,7 +591,7 @@ h3b::PagePools page_pools(const h3b_page_cache* c) {
 }
 // Shared checks of the attention entries: rows of Hq heads in q and out, the window rule.
 int check_rows(const void* q, int64_t q_stride, int dtype, int64_t rows, int64_t Hq, int64_t Hkv, int64_t window,
-               int64_t sinks, int64_t chunk, const void* out, int64_t out_stride, const char* what) {
+               int64_t sinks, int64_t chunk, float sm_scale, const void* out, int64_t out_stride, const char* what) {
   const std::string w(what);
   if (!q || !out) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null pointer");
   if (rows < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv)
@@ -599,6 +599,8 @@ int check_rows(const void* q, int64_t q_stride, int dtype, int64_t rows, int64_t
   if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, w + ": dtype must be fp16 or bf16");
   if (window < 0 || sinks < 0 || chunk < 1)
     return fail(H3B_ERR_INVALID_ARGUMENT, w + ": need window >= 0, sinks >= 0 and chunk >= 1");
+  if (!(sm_scale > 0.f) || sm_scale > 3e38f)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": the softmax scale must be positive and finite");
   if (rows > (1 << 30) || Hq > 65535) return fail(H3B_ERR_UNSUPPORTED, w + ": too many rows or heads");
   if (q_stride < Hq * 128 || q_stride % 8 || out_stride < Hq * 128 || out_stride % 8)
     return fail(H3B_ERR_INVALID_ARGUMENT, w + ": bad row stride");
@@ -609,6 +611,7 @@ int clip(int64_t x) { return x > (1 << 30) ? 1 << 30 : (int)x; }
 int window_status(int r, cudaError_t e, const char* what) {
   if (r == 1) return fail(H3B_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed");
   if (r == 3) return fail(H3B_ERR_UNSUPPORTED, std::string(what) + ": kernel register count differs from the planned split");
+  if (r == 4) return fail(H3B_ERR_UNSUPPORTED, std::string(what) + ": too many tiles");
   return cuda_status(e, what);
 }
 
@@ -620,7 +623,7 @@ int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int
                          int64_t sinks, int64_t chunk, float sm_scale, void* out, int64_t out_row_stride,
                          void* stream) {
   if (Tq == 0) return ok();
-  int r = check_rows(q, q_row_stride, dtype, Tq, Hq, Hkv, window, sinks, chunk, out, out_row_stride, "window_attention");
+  int r = check_rows(q, q_row_stride, dtype, Tq, Hq, Hkv, window, sinks, chunk, sm_scale, out, out_row_stride, "window_attention");
   if (r) return r;
   if (Tk < 0 || Tk > (1 << 30) || seqs < 1 || seqs > (1 << 24)) return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: bad sizes");
   if (Tk > 0 && (!k || !v)) return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: null pointer");
@@ -659,7 +662,7 @@ int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, i
   if (Tq == 0) return ok();
   int r = check_cache(cache, layer, "paged_window_attention");
   if (r) return r;
-  r = check_rows(q, q_row_stride, dtype, Tq, Hq, cache->kv_heads, window, sinks, chunk, out, out_row_stride,
+  r = check_rows(q, q_row_stride, dtype, Tq, Hq, cache->kv_heads, window, sinks, chunk, sm_scale, out, out_row_stride,
                  "paged_window_attention");
   if (r) return r;
   if (cache->dtype != dtype)
@@ -693,7 +696,7 @@ int h3b_decode_attention(const void* q, int64_t q_row_stride, int dtype, const i
   if (seqs == 0) return ok();
   int r = check_cache(cache, layer, "decode_attention");
   if (r) return r;
-  r = check_rows(q, q_row_stride, dtype, seqs, Hq, cache->kv_heads, window, sinks, 1, out, out_row_stride,
+  r = check_rows(q, q_row_stride, dtype, seqs, Hq, cache->kv_heads, window, sinks, 1, sm_scale, out, out_row_stride,
                  "decode_attention");
   if (r) return r;
   if (cache->dtype != 3 && cache->dtype != dtype)

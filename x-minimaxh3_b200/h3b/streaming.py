@@ -52,7 +52,11 @@ def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
 
 
 def _scale(scale: float | None) -> float:
-    return 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    if scale is None:
+        return 1.0 / math.sqrt(HEAD_DIM)
+    if not 0.0 < float(scale) < math.inf:
+        raise ValueError("the softmax scale must be positive and finite")
+    return float(scale)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
