@@ -85,6 +85,30 @@ def test_window_attention(case, dtype):
         assert torch.equal(one, out)
 
 
+@pytest.mark.parametrize("heads", [(8, 4), (6, 2), (12, 12)], ids=str)
+@pytest.mark.parametrize("rule", [(None, 0, 1), (100, 3, 1), (1, 0, 700), (129, 260, 1)], ids=str)
+def test_window_more_work_than_multiprocessors(heads, rule):
+    """Many items per persistent block: ragged sequences, empty ones and gaps between first tokens and window."""
+    from h3b import window_attention
+
+    hq, hkv = heads
+    window, sinks, chunk = rule
+    rng = np.random.RandomState(hq)
+    lens = [int(x) for x in rng.choice([0, 1, 5, 127, 128, 129, 300, 700, 1100], 40)]
+    keys = [n + int(rng.choice([0, 0, 3, 400])) if i % 7 else n // 2 for i, n in enumerate(lens)]
+    g = _gen(hq)
+    q = _rand(g, sum(lens), hq, D, dtype=torch.bfloat16, scale=1.5)
+    k, v = (_rand(g, sum(keys), hkv, D, dtype=torch.bfloat16) for _ in range(2))
+    out = window_attention(q, k, v, window=window, sinks=sinks, chunk=chunk, query_starts=_starts(lens),
+                           key_starts=_starts(keys))
+    a = b = 0
+    for lq, lk in zip(lens, keys):
+        if lq:
+            ref, spread = attend(q[a:a + lq], k[b:b + lk], v[b:b + lk], visible(lq, lk, window, sinks, chunk, "cuda"))
+            assert_close(out[a:a + lq], ref, spread, lk, 6.0, f"sequence at {a}")
+        a, b = a + lq, b + lk
+
+
 def test_window_rows_that_see_nothing_give_zero():
     """More queries than keys, a window of nothing, and sequences without keys."""
     from h3b import window_attention

@@ -3,9 +3,9 @@
 //
 //   out_i = sum_j softmax_j(scale * q_i . k_j) v_j  over the keys j that query i sees
 //
-// One CTA per two 128-row query tiles A and B that read the same keys: two heads of one
-// kv head at the same rows (even groups), else two consecutive row tiles of one head.
-// It visits the 128-key tiles that any of its rows sees -- those of the first tokens,
+// A persistent CTA per SM works through items of two 128-row query tiles A and B that
+// read the same keys: two heads of one kv head at the same rows (even groups), else two
+// consecutive row tiles of one head.  An item visits the 128-key tiles that any of its rows sees -- those of the first tokens,
 // then those of the window -- in one pass with the running maximum and sum:
 //   S = Q . K^T     tcgen05 kind::f16, fp32 in tensor memory
 //   P = 2^(S c - m) the running maximum m moves only when a tile exceeds it by more than
@@ -19,11 +19,12 @@
 // with an infinity or NaN are cleared first, because P = 0 does not hide them from the
 // matrix product, and their rows' outputs get them added at the end (add_nonfinite).
 //
-// 384 threads: warp 0 loads (TMA; Q once, then K and V tiles through a ring of five
-// 32 KB slots), warp 1 allocates tensor memory and clears V, warps 2 and 3 issue the
-// MMAs of tile A and B, warps 4..7 and 8..11 are their softmax, one row per thread.
-// An issuer runs PV(n - 1) before S(n), whose columns hold P(n - 1); the two tiles
-// alternate on the tensor pipe and on the softmax units.
+// 384 threads: warp 0 plans the items and loads (TMA; Q once, then K and V tiles through
+// a ring of five 32 KB slots), warp 1 allocates tensor memory and clears V, warps 2 and 3
+// issue the MMAs of tile A and B, warps 4..7 and 8..11 are their softmax, one row per
+// thread.  S of a step's first 64 keys is issued as soon as the step before has been read
+// from tensor memory, S of the others after that step's PV, which reads P from their
+// columns; PV of 64 keys starts when half of P is written.  The two tiles take turns.
 // Tensor memory: S_A 0..127, S_B 128..255, O_A 256..383, O_B 384..511, P over S + 64.
 #include <climits>
 
@@ -99,10 +100,6 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
 struct TileKeys {
   int sn, w0, w1;
   int end, lo, sinks;  // what every row sees: keys below `sinks`, and [lo, end)
-  __device__ bool takes(int n) const { return n < sn || (n >= w0 && n < w1); }
-  __device__ bool whole(int n) const {
-    return n * 128 + 128 <= end && (n * 128 >= lo || n * 128 + 128 <= sinks);
-  }
 };
 __device__ TileKeys tile_keys(const WindowRule& r, int p0, int p1, int lk) {
   TileKeys t{0, 0, 0, 0, 0, 0};
@@ -121,17 +118,37 @@ __device__ TileKeys tile_keys(const WindowRule& r, int p0, int p1, int lk) {
   }
   return t;
 }
+// One work item of a CTA.  Its steps visit the union of both tiles' key tiles in order;
+// what a tile takes and what all its rows see whole are ranges of steps.
+struct StepRanges {
+  int head, from, to;     // a tile takes steps < head and [from, to)
+  int whole_head, whole_from, whole_to;  // steps without a mask
+  __device__ bool takes(int i) const { return i < head || (i >= from && i < to); }
+  __device__ bool whole(int i) const { return i < whole_head || (i >= whole_from && i < whole_to); }
+};
 struct WinPlan {
-  TileKeys tile[2];
+  StepRanges tile[2];
   int row[2], rows[2];  // first row (of q) and valid rows of each tile
-  int sn, w0, steps;    // the union's tiles, in the order visited
   int p0[2];            // position of the tile's first row
+  int sn, w0, steps;    // key tiles of the steps: [0, sn), then w0 and on; steps < 0: no more work
   int lk, k_row, slot;  // keys of the sequence, its first K row or its table row
+  int head0, kh;        // head of tile A, kv head
   __device__ int key_tile(int i) const { return i < sn ? i : w0 + (i - sn); }
-  __device__ bool masked(int n) const {
-    return (tile[0].takes(n) && !tile[0].whole(n)) || (tile[1].takes(n) && !tile[1].whole(n));
+  __device__ bool masked(int i) const {
+    return (tile[0].takes(i) && !tile[0].whole(i)) || (tile[1].takes(i) && !tile[1].whole(i));
   }
 };
+__device__ __forceinline__ StepRanges step_ranges(const TileKeys& t, int sn, int w0) {
+  auto step = [&](int n) { return n < sn ? n : sn + max(n - w0, 0); };  // first step at or after key tile n
+  StepRanges r;
+  r.head = t.sn;
+  r.from = step(t.w0);
+  r.to = max(step(t.w1), r.from);
+  r.whole_head = step(t.sinks / 128);
+  r.whole_from = step((t.lo + 127) / 128);
+  r.whole_to = step(t.end / 128);
+  return r;
+}
 
 // bits [a, b) of a word whose bit 0 stands for key `base`
 __device__ __forceinline__ uint32_t key_bits(int base, int a, int b) {
@@ -164,8 +181,10 @@ __device__ __forceinline__ void win_exp32(uint32_t* s, float2 c2, float2 o2, flo
 // One key tile for one query row.  cnt: tiles that the row's query tile has taken before
 // (their PV is complete: it was issued before this S).
 template <bool BF16, bool MASK>
-__device__ __forceinline__ void win_softmax(uint32_t s_addr, uint32_t o_addr, float c, const VisibleKeys& see, int j0,
-                                            int cnt, float& m, float& l) {
+__device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, float c, const VisibleKeys& see, int j0,
+                                            int cnt, float& m, float& l, uint64_t* s_free, uint64_t* p_half,
+                                            uint64_t* turn, uint32_t turn_parity, uint64_t* other_turn,
+                                            volatile int* abort_flag) {
   uint32_t s[128];
   __syncwarp();
   tmem_ld32(s_addr, H3B_S32(s, 0));
@@ -176,6 +195,9 @@ __device__ __forceinline__ void win_softmax(uint32_t s_addr, uint32_t o_addr, fl
   reg_barrier32(H3B_S32(s, 32));
   reg_barrier32(H3B_S32(s, 64));
   reg_barrier32(H3B_S32(s, 96));
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(s_free);
   if constexpr (MASK) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -219,44 +241,57 @@ __device__ __forceinline__ void win_softmax(uint32_t s_addr, uint32_t o_addr, fl
   // nothing seen so far: subtract 0, so that the -inf of unseen keys gives 0
   const float off = m == -__int_as_float(0x7f800000) ? 0.f : -m;
   const float2 c2 = make_float2(c, c), o2 = make_float2(off, off);
+  //TR3
+  if (!mbar_wait_warp(turn, turn_parity, abort_flag, H3B_STATUS_ATTN_TIMEOUT)) return false;
+  //TR4
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     win_exp32<MASK>(&s[h * 64], c2, o2, acc0, acc1);
     win_exp32<MASK>(&s[h * 64 + 32], c2, o2, acc0, acc1);
+    if (h == 1) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(other_turn);
+      //TR5
+    }
     uint32_t p[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e)
       p[e] = pack2<BF16>(__uint_as_float(s[h * 64 + 2 * e]), __uint_as_float(s[h * 64 + 2 * e + 1]));
     tmem_st32(s_addr + 64 + h * 32, p);
+    tmem_wait_st();
+    tc_fence_before();
+    if (h == 0) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(p_half);
+    }
   }
-  tmem_wait_st();
-  tc_fence_before();
   const float2 t = __fadd2_rn(acc0, acc1);
   l = l * alpha + (t.x + t.y);
+  return true;
 }
 
 // row of V (of the tile's kv head) of key j
 template <bool PAGED>
-__device__ __forceinline__ const uint16_t* value_row(const WindowArgs& a, const WinPlan& pl, int kh, int j) {
+__device__ __forceinline__ const uint16_t* value_row(const WindowArgs& a, const WinPlan& pl, int j) {
   if constexpr (PAGED)
     return static_cast<const uint16_t*>(a.paged.v) +
-           ((paged_page(a.paged, pl.slot, j / a.paged.page) * a.Hkv + kh) * a.paged.page + j % a.paged.page) * 128;
+           ((paged_page(a.paged, pl.slot, j / a.paged.page) * a.Hkv + pl.kh) * a.paged.page + j % a.paged.page) * 128;
   else
-    return a.v + (int64_t)(pl.k_row + j) * a.v_stride + kh * 128;
+    return a.v + (int64_t)(pl.k_row + j) * a.v_stride + pl.kh * 128;
 }
 
 // Adds to an output row the infinities and NaN of the V rows that it sees and that were
 // cleared from the masked tiles.  Only when there is such a row.
 template <bool BF16, bool PAGED>
-__device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& pl, int kh, const VisibleKeys& see,
+__device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& pl, const VisibleKeys& see,
                                            uint16_t* dst) {
   for (int i = 0; i < pl.steps; ++i) {
     const int n = pl.key_tile(i);
-    if (!pl.masked(n)) continue;
+    if (!pl.masked(i)) continue;
     for (int j = n * 128; j < min(n * 128 + 128, see.end); ++j) {
       if (j < see.lo && j >= see.sinks) continue;
-      const uint32_t* v = reinterpret_cast<const uint32_t*>(value_row<PAGED>(a, pl, kh, j));
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(value_row<PAGED>(a, pl, j));
       for (int e = 0; e < 64; ++e) {
         const uint32_t w = v[e], bad = nonfinite2<BF16>(w);
         if (!(bad & 0x80008000u)) continue;
@@ -271,329 +306,494 @@ __device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& p
   }
 }
 
+// Work item `item` for the whole warp: items number the heads of a tile first, tiles run
+// through the sequences from the last (with a causal mask the late tiles see most keys,
+// and go first).  Items beyond the last tile have steps -1.
+template <bool PAGED>
+__device__ void plan_item(const WindowArgs& a, int item, int items, int rows_per_cta, WinPlan* out) {
+  const int lane = threadIdx.x & 31;
+  const bool by_heads = rows_per_cta == 128;  // tiles A, B: two heads of a group; else two row tiles
+  const int columns = by_heads ? a.Hq / 2 : a.Hq;
+  int t = (items - 1 - item) / columns, seq = -1;
+  for (int base = 0; base < a.seqs; base += 32) {
+    int n = 0;
+    if (base + lane < a.seqs) {
+      const RowRange r = row_range(a.q_starts, base + lane, a.Tq);
+      n = (r.b - r.a + rows_per_cta - 1) / rows_per_cta;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, t < x);
+    if (hit) {
+      const int w = __ffs(hit) - 1;
+      seq = base + w;
+      t -= __shfl_sync(0xffffffffu, x - n, w);
+      break;
+    }
+    t -= __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) {
+    WinPlan p{};  // no sequence: nothing to visit, no row to write
+    if (seq >= 0) {
+      const RowRange qr = row_range(a.q_starts, seq, a.Tq);
+      if constexpr (PAGED) {
+        p.slot = paged_slot(a.paged, seq);
+        p.lk = paged_len(a.paged, p.slot);
+        p.k_row = 0;
+      } else {
+        const RowRange kr = row_range(a.k_starts, seq, a.Tk);
+        p.slot = 0;
+        p.lk = kr.b - kr.a;
+        p.k_row = kr.a;
+      }
+      p.head0 = (item % columns) * (by_heads ? 2 : 1);
+      p.kh = p.head0 / (a.Hq / a.Hkv);
+      const int lq = qr.b - qr.a;
+      TileKeys keys[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int first = t * rows_per_cta + (by_heads ? 0 : x * 128);
+        p.row[x] = qr.a + first;
+        p.rows[x] = max(0, min(128, lq - first));
+        p.p0[x] = p.lk - lq + first;
+        keys[x] = p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
+      }
+      p.sn = max(keys[0].sn, keys[1].sn);
+      int w0 = 1 << 30, w1 = 0;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (keys[x].w1 > keys[x].w0) {
+          w0 = min(w0, keys[x].w0);
+          w1 = max(w1, keys[x].w1);
+        }
+      }
+      p.w0 = max(w0, p.sn);
+      p.steps = p.sn + max(0, w1 - p.w0);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) p.tile[x] = step_ranges(keys[x], p.sn, p.w0);
+    }
+    *out = p;
+  }
+  __syncwarp();
+}
+
+// A counter through the phases of a ring of N barriers: slot and parity of its next use.
+template <int N>
+struct RingAt {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// 32 output rows of a warp (a row per lane, 8 pieces of 16 bytes of it) so that 8 lanes
+// store the 128 contiguous bytes of one row: an 8 x 8 transpose of pieces in each group
+// of 8 lanes.  A store of own rows would touch 32 lines for 512 bytes.
+__device__ __forceinline__ void transpose_pieces(uint4 (&u)[8]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int b = 1; b < 8; b <<= 1) {
+    const bool up = lane & b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i & b) continue;
+      uint4 &lo = u[i], &hi = u[i | b];
+      const uint4 give = up ? lo : hi;
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, give.x, b);
+      got.y = __shfl_xor_sync(0xffffffffu, give.y, b);
+      got.z = __shfl_xor_sync(0xffffffffu, give.z, b);
+      got.w = __shfl_xor_sync(0xffffffffu, give.w, b);
+      if (up)
+        lo = got;
+      else
+        hi = got;
+    }
+  }
+}
+
 template <bool BF16, bool PAGED>
 __global__ void __launch_bounds__(kWinThreads, 1)
     window_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WindowArgs a, int rows_per_cta) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WindowArgs a, int rows_per_cta,
+                  int items) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWinOffBar);
-  uint64_t* q_full = bars;              // 1
-  uint64_t* full = bars + 1;            // kWinSlots
-  uint64_t* empty = full + kWinSlots;   // kWinSlots
-  uint64_t* v_ok = empty + kWinSlots;   // 4: V of step i (mod 4) is free of what masking cannot hide
-  uint64_t* s_full = v_ok + 4;          // 2
-  uint64_t* p_full = s_full + 2;        // 2
-  uint64_t* o_full = p_full + 2;        // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* full = bars;                // kWinSlots
+  uint64_t* empty = full + kWinSlots;   // kWinSlots (a release per tile)
+  uint64_t* v_ok = empty + kWinSlots;   // 4: V of a step (mod 4) is free of what masking cannot hide
+  uint64_t* q_full = v_ok + 4;          // 1
+  uint64_t* q_empty = q_full + 1;       // 1 (per tile)
+  uint64_t* s_full = q_empty + 1;       // 2: S written
+  uint64_t* s_free = s_full + 2;        // 2: S read
+  uint64_t* p_half = s_free + 2;        // 2: P of the first 64 keys written
+  uint64_t* p_full = p_half + 2;        // 2
+  uint64_t* o_full = p_full + 2;        // 2: O of an item complete
+  uint64_t* o_free = o_full + 2;        // 2: O read
+  uint64_t* turns = o_free + 2;         // 2 x 4: whose exponentials run, per SM sub-partition
+  uint64_t* plan_full = turns + 8;      // 2
+  uint64_t* plan_free = plan_full + 2;  // 2
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(plan_free + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* cleared = abort_flag + 1;  // some seen V row was cleared
-  int* found = const_cast<int*>(abort_flag) + 2;  // sequence, tile of it
-  __shared__ WinPlan plan;
-
+  volatile int* cleared = abort_flag + 1;  // [2]: some seen V row of the item was cleared
+  __shared__ WinPlan plans[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.Hq / a.Hkv;
-  const bool by_heads = rows_per_cta == 128;  // A, B: two heads of a group; else two row tiles
-  const int columns = by_heads ? a.Hq / 2 : a.Hq;
-  const int head0 = (int)(blockIdx.x % columns) * (by_heads ? 2 : 1);
-  const int kh = head0 / group;
+  const bool by_heads = rows_per_cta == 128;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait_warp(bar, parity, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
+  };
 
-  // which sequence and rows: tiles are numbered through the sequences, the last first
-  // (with a causal mask they see most keys)
   if (warp == 0) {
-    int t = (int)((gridDim.x - 1 - blockIdx.x) / columns), seq = -1;
-    for (int base = 0; base < a.seqs; base += 32) {
-      int n = 0;
-      if (base + lane < a.seqs) {
-        const RowRange r = row_range(a.q_starts, base + lane, a.Tq);
-        n = (r.b - r.a + rows_per_cta - 1) / rows_per_cta;
-      }
-      int x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, t < x);
-      if (hit) {
-        const int w = __ffs(hit) - 1;
-        seq = base + w;
-        t -= __shfl_sync(0xffffffffu, x - n, w);
-        break;
-      }
-      t -= __shfl_sync(0xffffffffu, x, 31);
-    }
     if (lane == 0) {
-      found[0] = seq;
-      found[1] = t;
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
     }
-  }
-  __syncthreads();
-  if (found[0] < 0) return;  // the grid is an upper bound
-
-  if (threadIdx.x == 0) {
-    const int seq = found[0], t = found[1];
-    const RowRange qr = row_range(a.q_starts, seq, a.Tq);
-    WinPlan p;
-    if constexpr (PAGED) {
-      p.slot = paged_slot(a.paged, seq);
-      p.lk = paged_len(a.paged, p.slot);
-      p.k_row = 0;
-    } else {
-      const RowRange kr = row_range(a.k_starts, seq, a.Tk);
-      p.slot = 0;
-      p.lk = kr.b - kr.a;
-      p.k_row = kr.a;
-    }
-    const int lq = qr.b - qr.a;
-    for (int x = 0; x < 2; ++x) {
-      const int first = t * rows_per_cta + (by_heads ? 0 : x * 128);
-      p.row[x] = qr.a + first;
-      p.rows[x] = max(0, min(128, lq - first));
-      p.p0[x] = p.lk - lq + first;
-      p.tile[x] = p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
-    }
-    const TileKeys &ta = p.tile[0], &tb = p.tile[1];
-    p.sn = max(ta.sn, tb.sn);
-    int w0 = 1 << 30, w1 = 0;
-    if (ta.w1 > ta.w0) {
-      w0 = ta.w0;
-      w1 = ta.w1;
-    }
-    if (tb.w1 > tb.w0) {
-      w0 = min(w0, tb.w0);
-      w1 = max(w1, tb.w1);
-    }
-    p.w0 = max(w0, p.sn);
-    p.steps = p.sn + max(0, w1 - p.w0);
-    plan = p;
-
-    mbar_init(q_full, 1);
-    for (int s = 0; s < kWinSlots; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 2);  // one release per tile
-    }
-    for (int s = 0; s < 4; ++s) mbar_init(&v_ok[s], 1);
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 128);
-      mbar_init(&o_full[x], 1);
-    }
-    *abort_flag = 0;
-    *cleared = 0;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
+    plan_item<PAGED>(a, blockIdx.x, items, rows_per_cta, &plans[0]);
+  } else if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
+  } else if (warp == 2 && lane == 0) {
+    for (int s = 0; s < kWinSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 2);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(&v_ok[s], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&s_free[x], 4);  // a warp each
+      mbar_init(&p_half[x], 4);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&o_full[x], 1);
+      mbar_init(&o_free[x], 4);
+      mbar_init(&plan_full[x], 1);
+      mbar_init(&plan_free[x], 11);  // all warps but the planning one
+    }
+    for (int s = 0; s < 8; ++s) mbar_init(&turns[s], 1);
+    *abort_flag = 0;
+    cleared[0] = cleared[1] = 0;
+    fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int steps = plan.steps;
 
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWinCtrlRegs));
   if (warp == 0) {
-    if (elect_one()) {
-      mbar_arrive_expect_tx(q_full, 2 * kWinTile);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int h = by_heads ? head0 + x : head0;
-        uint8_t* dst = smem + x * kWinTile;
-        tma_load_3d(dst, &tmQ, q_full, 0, h, plan.row[x]);
-        tma_load_3d(dst + kWinTile / 2, &tmQ, q_full, 64, h, plan.row[x]);
-      }
-    }
-    __syncwarp();
-    int slot = 0;
-    uint32_t phase = 0;
-    const int box = PAGED ? min(a.paged.page, 128) : 128;
+    // plans the items and loads their tiles
+    RingAt<kWinSlots> at;
+    const int box = PAGED ? a.paged.page : 128;
     bool ok = true;
-    for (int i = 0; i < 2 * steps && ok; ++i) {
-      ok = mbar_wait_warp(&empty[slot], phase ^ 1, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
-      if (!ok) break;
-      const int j0 = plan.key_tile(i >> 1) * 128;
-      const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
-      uint8_t* dst = smem + kWinOffRing + slot * kWinTile;
-      if (lane == 0) mbar_arrive_expect_tx(&full[slot], kWinTile);
+    uint32_t q_parity = 1;
+    int k = 0;
+    for (int item = blockIdx.x;; item += gridDim.x, ++k) {
+      WinPlan* pl = &plans[k & 1];
+      if (k > 0) {
+        if (!wait(&plan_free[k & 1], (uint32_t)((k >> 1) & 1) ^ 1u)) break;
+        if (item < items)
+          plan_item<PAGED>(a, item, items, rows_per_cta, pl);
+        else if (lane == 0)
+          pl->steps = -1;
+        if (lane == 0) cleared[k & 1] = 0;
+        __syncwarp();
+      }
+      const int steps = pl->steps, sn = pl->sn, w0 = pl->w0, kh = pl->kh;
+      if (lane == 0) mbar_arrive(&plan_full[k & 1]);
+      if (steps < 0) break;
+      if (steps == 0) continue;
+      if (!(ok = wait(q_empty, q_parity))) break;
+      q_parity ^= 1u;
+      if (lane == 0) mbar_arrive_expect_tx(q_full, 2 * kWinTile);
       __syncwarp();
-      if constexpr (PAGED) {
-        // a copy per page and half of the channels; pages that no row needs, or that the
-        // table does not have, are read as zeros from outside the pool
-        const int boxes = 2 * (128 / box);
-        if (lane < boxes) {
-          const int half = lane & 1, j = j0 + (lane >> 1) * box, col = j / a.paged.page;
-          int64_t z = a.paged.pages * a.Hkv;
-          if (j < plan.lk && col < a.paged.width) {
-            const int pg = a.paged.table[(int64_t)plan.slot * a.paged.width + col];
-            if (pg >= 0 && pg < a.paged.pages) z = (int64_t)pg * a.Hkv + kh;
+      if (lane < 4)
+        tma_load_3d(smem + lane * (kWinTile / 2), &tmQ, q_full, (lane & 1) * 64,
+                    by_heads ? pl->head0 + (lane >> 1) : pl->head0, pl->row[lane >> 1]);
+      __syncwarp();
+      for (int i = 0; i < 2 * steps; ++i, at.next()) {
+        if (!(ok = wait(&empty[at.slot], at.parity ^ 1u))) break;
+        const int n = i >> 1, j0 = (n < sn ? n : w0 + (n - sn)) * 128;
+        const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
+        uint8_t* dst = smem + kWinOffRing + at.slot * kWinTile;
+        uint64_t* bar = &full[at.slot];
+        if (lane == 0) mbar_arrive_expect_tx(bar, kWinTile);
+        __syncwarp();
+        if constexpr (PAGED) {
+          // a copy per page and half of the channels; pages that no row needs, or that the
+          // table does not have, are read as zeros from outside the pool
+          if (lane < 256 / box) {
+            const int half = lane & 1, j = j0 + (lane >> 1) * box, col = j / box;
+            int64_t z = a.paged.pages * a.Hkv;
+            if (j < pl->lk && col < a.paged.width) {
+              const int pg = a.paged.table[(int64_t)pl->slot * a.paged.width + col];
+              if (pg >= 0 && pg < a.paged.pages) z = (int64_t)pg * a.Hkv + kh;
+            }
+            tma_load_3d(dst + half * (kWinTile / 2) + (lane >> 1) * box * 128, tm, bar, half * 64, 0, (int)z);
           }
-          tma_load_3d(dst + half * (kWinTile / 2) + (lane >> 1) * box * 128, tm, &full[slot], half * 64,
-                      j & (a.paged.page - 1), (int)z);
+        } else if (lane < 2) {
+          tma_load_3d(dst + lane * (kWinTile / 2), tm, bar, lane * 64, kh, pl->k_row + j0);
         }
-      } else if (lane < 2) {
-        tma_load_3d(dst + lane * (kWinTile / 2), tm, &full[slot], lane * 64, kh, plan.k_row + j0);
+        __syncwarp();
       }
-      __syncwarp();
-      if (++slot == kWinSlots) {
-        slot = 0;
-        phase ^= 1;
-      }
+      if (!ok) break;
     }
   } else if (warp == 1) {
     // V tiles, in order: those that are masked somewhere lose their non-finite elements
-    int item = 1;
-    for (int i = 0; i < steps; ++i, item += 2) {
-      const int slot = item % kWinSlots;
-      if (!mbar_wait_warp(&full[slot], (item / kWinSlots) & 1, abort_flag, H3B_STATUS_ATTN_TIMEOUT)) break;
-      const int n = plan.key_tile(i);
-      if (plan.masked(n)) {
-        uint4* v = reinterpret_cast<uint4*>(smem + kWinOffRing + slot * kWinTile);
-        uint32_t any = 0;
+    RingAt<kWinSlots> at;
+    RingAt<4> vo;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const WinPlan& pl = plans[k & 1];
+      if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
+      const int steps = pl.steps;
+      if (steps < 0) break;
+      for (int i = 0; i < steps; ++i) {
+        at.next();
+        if (!(ok = wait(&full[at.slot], at.parity))) break;
+        if (pl.masked(i)) {
+          uint4* v = reinterpret_cast<uint4*>(smem + kWinOffRing + at.slot * kWinTile);
+          uint32_t any = 0;
 #pragma unroll 8
-        for (int x = 0; x < kWinTile / 16 / 32; ++x) {
-          const uint4 w = v[x * 32 + lane];
-          any |= nonfinite2<BF16>(w.x) | nonfinite2<BF16>(w.y) | nonfinite2<BF16>(w.z) | nonfinite2<BF16>(w.w);
-        }
-        if (__any_sync(0xffffffffu, any & 0x80008000u)) {
-          for (int x = lane; x < kWinTile / 16; x += 32) {
-            uint4 w = v[x];
-            uint32_t* e = reinterpret_cast<uint32_t*>(&w);
-            bool hit = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t bad = nonfinite2<BF16>(e[k]);
-              if (bad & 0x8000u) e[k] &= 0xffff0000u;
-              if (bad & 0x80000000u) e[k] &= 0x0000ffffu;
-              hit |= (bad & 0x80008000u) != 0;
-            }
-            if (hit) {
-              v[x] = w;
-              const int j = n * 128 + (x / 8) % 128;  // 8 pieces of 16 bytes per row and half
-              if (j < plan.lk) *cleared = 1;
-            }
+          for (int x = 0; x < kWinTile / 16 / 32; ++x) {
+            const uint4 w = v[x * 32 + lane];
+            any |= nonfinite2<BF16>(w.x) | nonfinite2<BF16>(w.y) | nonfinite2<BF16>(w.z) | nonfinite2<BF16>(w.w);
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (__any_sync(0xffffffffu, any & 0x80008000u)) {
+            const int j0 = pl.key_tile(i) * 128;
+            for (int x = lane; x < kWinTile / 16; x += 32) {
+              uint4 w = v[x];
+              uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+              bool hit = false;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const uint32_t bad = nonfinite2<BF16>(e[c]);
+                if (bad & 0x8000u) e[c] &= 0xffff0000u;
+                if (bad & 0x80000000u) e[c] &= 0x0000ffffu;
+                hit |= (bad & 0x80008000u) != 0;
+              }
+              if (hit) {
+                v[x] = w;
+                if (j0 + (x / 8) % 128 < pl.lk) cleared[k & 1] = 1;  // 8 pieces per row and half
+              }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ok[vo.slot]);
+        vo.next();
+        at.next();
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ok[i & 3]);
+      if (lane == 0) mbar_arrive(&plan_free[k & 1]);
     }
   } else if (warp < 4) {
     // MMA issuer of tile x: the whole warp walks the steps, one elected lane issues
     const int x = warp - 2;
-    const TileKeys keys = plan.tile[x];
-    constexpr uint32_t idesc_s = idesc_f16<BF16>(128, 128, false);
+    constexpr uint32_t idesc_s = idesc_f16<BF16>(128, 128, false), idesc_half = idesc_f16<BF16>(128, 64, false);
     constexpr uint32_t idesc_pv = idesc_f16<BF16>(128, 128, true);
-    const uint32_t q_addr = smem_u32(smem + x * kWinTile), ring = smem_u32(smem + kWinOffRing);
+    const uint32_t ring = smem_u32(smem + kWinOffRing);
     const uint32_t s_tmem = tmem + (uint32_t)(x * 128), o_tmem = tmem + 256 + (uint32_t)(x * 128);
-    bool ok = mbar_wait_warp(q_full, 0, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
-    int pending = -1;  // step whose PV is to come
-    bool first = true;
-    uint32_t ppar = 0;
-    auto issue_pv = [&]() -> bool {
-      if (!mbar_wait_warp(&p_full[x], ppar, abort_flag, H3B_STATUS_ATTN_TIMEOUT)) return false;
-      ppar ^= 1u;
-      if (!mbar_wait_warp(&v_ok[pending & 3], (pending >> 2) & 1, abort_flag, H3B_STATUS_ATTN_TIMEOUT)) return false;
-      tc_fence_after();
-      const int slot = (2 * pending + 1) % kWinSlots;
-      const uint64_t vdesc = sdesc_mnmajor_sw128(ring + slot * kWinTile, kWinTile / 2);
-      if (elect_one()) {
+    const uint64_t qdesc = sdesc_kmajor_sw128(smem_u32(smem + x * kWinTile));
+    // S of 64 or 128 keys from row `row` of a K tile
+    auto issue_s = [&](int slot, int row, uint32_t idesc) {
+      const uint64_t kdesc = sdesc_kmajor_sw128(ring + slot * kWinTile + row * 128);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_f16_ts(o_tmem, s_tmem + 64 + 8 * k, vdesc + (uint64_t)(128 * k), idesc_pv, first && k == 0 ? 0u : 1u);
-        mma_commit(&empty[slot]);
+      for (int c = 0; c < 8; ++c) {
+        const uint64_t off = (uint64_t)((c & 3) * 2 + (c >> 2) * (kWinTile / 2 / 16));
+        mma_bf16_ss(s_tmem + row, qdesc + off, kdesc + off, idesc, c == 0 ? 0u : 1u);
       }
-      __syncwarp();
-      first = false;
-      pending = -1;
-      return true;
     };
-    for (int i = 0; i < steps && ok; ++i) {
-      const int ks = (2 * i) % kWinSlots, vs = (2 * i + 1) % kWinSlots;
-      ok = mbar_wait_warp(&full[ks], ((2 * i) / kWinSlots) & 1, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
-      if (!ok) break;
-      if (keys.takes(plan.key_tile(i))) {
-        if (pending >= 0 && !(ok = issue_pv())) break;
+    RingAt<kWinSlots> at;
+    RingAt<4> vo;
+    uint32_t q_parity = 0, o_parity = 1, step_parity = 0;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
+      const int steps = plans[k & 1].steps;
+      if (steps < 0) break;
+      const StepRanges r = plans[k & 1].tile[x];
+      const int last = r.to > r.from ? r.to - 1 : r.head - 1;  // last step taken (-1: none)
+      if (steps > 0) {
+        if (!(ok = wait(q_full, q_parity))) break;
+        q_parity ^= 1u;
+        if (last < 0 && lane == 0) mbar_arrive(q_empty);
+      }
+      bool first = true, issued = false;
+      for (int i = 0; i < steps; ++i) {
+        const RingAt<kWinSlots> kt = at;
+        at.next();
+        const RingAt<kWinSlots> vt = at;
+        at.next();
+        const RingAt<4> vs = vo;
+        vo.next();
+        if (!r.takes(i)) {
+          // V through its check, which must not fall behind the ring
+          if (!(ok = wait(&full[kt.slot], kt.parity) && wait(&v_ok[vs.slot], vs.parity))) break;
+          if (lane == 0) {
+            mbar_arrive(&empty[kt.slot]);
+            mbar_arrive(&empty[vt.slot]);
+          }
+          __syncwarp();
+          continue;
+        }
+        if (!issued) {
+          if (!(ok = wait(&full[kt.slot], kt.parity))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            issue_s(kt.slot, 0, idesc_s);
+            mma_commit(&empty[kt.slot]);
+            mma_commit(&s_full[x]);
+            if (i == last) mma_commit(q_empty);
+          }
+          __syncwarp();
+        }
+        issued = i < last && r.takes(i + 1);
+        if (issued) {
+          // the next S of the first 64 keys, over the columns that hold neither S nor P now
+          if (!(ok = wait(&full[at.slot], at.parity) && wait(&s_free[x], step_parity))) break;
+          tc_fence_after();
+          if (elect_one()) issue_s(at.slot, 0, idesc_half);
+          __syncwarp();
+        }
+        const uint64_t vdesc = sdesc_mnmajor_sw128(ring + vt.slot * kWinTile, kWinTile / 2);
+        if (first && !(ok = wait(&o_free[x], o_parity))) break;
+        if (!(ok = wait(&v_ok[vs.slot], vs.parity) && wait(&p_half[x], step_parity))) break;
         tc_fence_after();
-        const uint64_t qdesc = sdesc_kmajor_sw128(q_addr), kdesc = sdesc_kmajor_sw128(ring + ks * kWinTile);
+        //TM0 i
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t at = (uint64_t)((k & 3) * 2 + (k >> 2) * (kWinTile / 2 / 16));
-            mma_bf16_ss(s_tmem, qdesc + at, kdesc + at, idesc_s, k == 0 ? 0u : 1u);
-          }
-          mma_commit(&empty[ks]);
-          mma_commit(&s_full[x]);
+          for (int c = 0; c < 4; ++c)
+            mma_f16_ts(o_tmem, s_tmem + 64 + 8 * c, vdesc + (uint64_t)(128 * c), idesc_pv, first && c == 0 ? 0u : 1u);
         }
         __syncwarp();
-        pending = i;
-      } else {
-        // a PV left to come would hold its slot until the tile's next step
-        if (pending >= 0 && !(ok = issue_pv())) break;
-        ok = mbar_wait_warp(&full[vs], ((2 * i + 1) / kWinSlots) & 1, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
-        if (!ok) break;
+        first = false;
+        if (!(ok = wait(&p_full[x], step_parity))) break;
+        tc_fence_after();
+        //TM1 i
         if (elect_one()) {
-          mbar_arrive(&empty[ks]);
-          mbar_arrive(&empty[vs]);
+#pragma unroll
+          for (int c = 4; c < 8; ++c)
+            mma_f16_ts(o_tmem, s_tmem + 64 + 8 * c, vdesc + (uint64_t)(128 * c), idesc_pv, 1u);
+          mma_commit(&empty[vt.slot]);
+          if (issued) {
+            issue_s(at.slot, 64, idesc_half);  // its columns held P
+            mma_commit(&empty[at.slot]);
+            mma_commit(&s_full[x]);
+            if (i + 1 == last) mma_commit(q_empty);
+          } else if (i == last) {
+            mma_commit(&o_full[x]);
+          }
         }
         __syncwarp();
+        //TM2 i
+        step_parity ^= 1u;
       }
+      if (!ok) break;
+      if (last >= 0) o_parity ^= 1u;
+      if (lane == 0) mbar_arrive(&plan_free[k & 1]);
     }
-    if (ok && pending >= 0) ok = issue_pv();
-    if (ok && !first && elect_one()) mma_commit(&o_full[x]);
-    __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWinSoftRegs));
-    const int x = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
-    const bool row_ok = r < plan.rows[x];
-    const TileKeys keys = plan.tile[x];
-    const VisibleKeys see = visible_keys(a.rule, plan.p0[x] + r, plan.lk);
+    const int x = (warp - 4) >> 2, quad = warp & 3;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem + lane_off + (uint32_t)(x * 128);
     const uint32_t o_addr = tmem + lane_off + 256 + (uint32_t)(x * 128);
-    float m = -__int_as_float(0x7f800000), l = 0.f;
-    int cnt = 0;
+    // The two tiles' exponentials take turns in each SM sub-partition (warps q of A and B
+    // share one): otherwise both softmaxes run at the same time, and then both wait for
+    // the tensor pipe at the same time.
+    uint64_t *turn = &turns[x * 4 + quad], *other_turn = &turns[(x ^ 1) * 4 + quad];
+    uint32_t turn_parity = (uint32_t)(x ^ 1), step_parity = 0, o_parity = 0;
     bool ok = true;
-    for (int i = 0; i < steps; ++i) {
-      const int n = plan.key_tile(i);
-      if (!keys.takes(n)) continue;
-      ok = mbar_wait_warp(&s_full[x], (uint32_t)(cnt & 1), abort_flag, H3B_STATUS_ATTN_TIMEOUT);
-      if (!ok) break;
-      tc_fence_after();
-      if (keys.whole(n))
-        win_softmax<BF16, false>(s_addr, o_addr, a.scale_log2, see, n * 128, cnt, m, l);
-      else
-        win_softmax<BF16, true>(s_addr, o_addr, a.scale_log2, see, n * 128, cnt, m, l);
-      mbar_arrive(&p_full[x]);
-      ++cnt;
-    }
-    const int h = by_heads ? head0 + x : head0;
-    uint16_t* dst = a.out + (int64_t)(row_ok ? plan.row[x] + r : 0) * a.out_stride + (int64_t)h * 128;
-    if (ok && cnt > 0) {
-      if (mbar_wait_warp(&o_full[x], 0u, abort_flag, H3B_STATUS_ATTN_TIMEOUT)) {
+    for (int k = 0; ok; ++k) {
+      const WinPlan& pl = plans[k & 1];
+      if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
+      const int steps = pl.steps;
+      if (steps < 0) break;
+      const StepRanges r = pl.tile[x];
+      const VisibleKeys see = visible_keys(a.rule, pl.p0[x] + quad * 32 + lane, steps > 0 ? pl.lk : 0);
+      float m = -__int_as_float(0x7f800000), l = 0.f;
+      int cnt = 0;
+      for (int i = 0; i < steps; ++i, turn_parity ^= 1u) {
+        if (!r.takes(i)) {
+          if (!(ok = wait(turn, turn_parity))) break;
+          if (lane == 0) mbar_arrive(other_turn);
+          continue;
+        }
+        //TR0
+        if (!(ok = wait(&s_full[x], step_parity))) break;
         tc_fence_after();
+        //TR1
+        ok = r.whole(i) ? win_softmax<BF16, false>(s_addr, o_addr, a.scale_log2, see, 0, cnt, m, l, &s_free[x],
+                                                   &p_half[x], turn, turn_parity, other_turn, abort_flag)
+                        : win_softmax<BF16, true>(s_addr, o_addr, a.scale_log2, see, pl.key_tile(i) * 128, cnt, m, l,
+                                                  &s_free[x], &p_half[x], turn, turn_parity, other_turn, abort_flag);
+        if (!ok) break;
+        //TR2
         __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+        step_parity ^= 1u;
+        ++cnt;
+      }
+      if (!ok) break;
+      const int rows = pl.rows[x] - quad * 32;  // valid rows of this warp
+      const int64_t row0 = pl.row[x] + quad * 32;
+      uint16_t* dst = a.out + row0 * a.out_stride + (int64_t)(by_heads ? pl.head0 + x : pl.head0) * 128;
+      if (cnt > 0) {
+        if (!(ok = wait(&o_full[x], o_parity))) break;
+        o_parity ^= 1u;
+        tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 16) {
-          uint32_t o[16];
-          tmem_ld16(o_addr + c, o);
-          tmem_wait_ld();
-          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            w[e] = pack2<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-          if (row_ok) {
-            *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t o[64];
+          tmem_ld32(o_addr + half * 64, H3B_S32(o, 0));
+          tmem_ld32(o_addr + half * 64 + 32, H3B_S32(o, 32));
+          tmem_wait_ld_dep(H3B_S32(o, 0));
+          reg_barrier32(H3B_S32(o, 32));
+          if (half == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[x]);
+          }
+          uint4 u[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            u[e].x = pack2<BF16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+            u[e].y = pack2<BF16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+            u[e].z = pack2<BF16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+            u[e].w = pack2<BF16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+          }
+          transpose_pieces(u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int row = (lane & 24) + e;
+            if (row < rows)
+              *reinterpret_cast<uint4*>(dst + row * a.out_stride + half * 64 + (lane & 7) * 8) = u[e];
           }
         }
-        if (*cleared && row_ok) add_nonfinite<BF16, PAGED>(a, plan, kh, see, dst);
+        if (cleared[k & 1]) {
+          __syncwarp();
+          if (lane < rows) add_nonfinite<BF16, PAGED>(a, pl, see, dst + lane * a.out_stride);
+        }
+      } else {
+        for (int e = 0; e < min(rows, 32) * 16; e += 32) {
+          const int row = (e + lane) >> 4;
+          if (row < rows) *reinterpret_cast<uint4*>(dst + row * a.out_stride + ((e + lane) & 15) * 8) = make_uint4(0, 0, 0, 0);
+        }
       }
-    } else if (row_ok && cnt == 0) {
-      for (int c = 0; c < 128; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&plan_free[k & 1]);
     }
   }
 
@@ -642,9 +842,10 @@ int launch_window(const WindowArgs& a, cudaStream_t s, cudaError_t* err) {
   const bool by_heads = (a.Hq / a.Hkv) % 2 == 0;
   const int rows = by_heads ? 128 : 256;
   const int64_t tiles = (int64_t)a.Tq / rows + a.seqs;  // sum of ceil(len / rows) is at most this
-  const int64_t ctas = tiles * (by_heads ? a.Hq / 2 : a.Hq);
-  if (ctas > INT_MAX) return 4;
-  kern<<<(unsigned)ctas, kWinThreads, kWinSmem, s>>>(tq, tk, tv, a, rows);
+  const int64_t items = tiles * (by_heads ? a.Hq / 2 : a.Hq);
+  if (items > INT_MAX / 2) return 4;
+  const int64_t ctas = items < num_sms() ? items : num_sms();
+  kern<<<(unsigned)ctas, kWinThreads, kWinSmem, s>>>(tq, tk, tv, a, rows, (int)items);
   *err = cudaGetLastError();
   return *err == cudaSuccess ? 0 : 2;
 }
