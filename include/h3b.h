@@ -463,6 +463,11 @@ int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* s
                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
                     int64_t tokens, void* stream);
 
+/* h3b_pages_extend, then h3b_pages_write into `layer`, in two launches. */
+int h3b_pages_append(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
+                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
+                     int64_t tokens, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Slots dst[i] (empty, distinct, none of them a source) become sequences that share the
  * pages of src[i]. */
 int h3b_pages_fork(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);

@@ -737,39 +737,77 @@ int h3b_pages_extend(const h3b_page_cache* cache, const int32_t* slots, int64_t 
   if (!workspace || workspace_bytes < h3b::pages_workspace_bytes(n, cache->pages))
     return fail(H3B_ERR_INVALID_ARGUMENT, "pages_extend: workspace too small");
   return cuda_status(h3b::launch_pages_extend(page_tables(cache), page_pools(cache), slots, (int)n, starts,
-                                              static_cast<int32_t*>(workspace), st(stream)), "pages_extend");
+                                              static_cast<int32_t*>(workspace), true, st(stream)), "pages_extend");
 }
+
+}  // extern "C"
+
+namespace {
+
+// Checks the rows of a write and fills `w`; 0 or the failure's status.
+int write_args(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
+               const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype, int64_t tokens,
+               const char* what, h3b::PageWriteArgs* w) {
+  const std::string name(what);
+  const int r = check_cache(cache, layer, what);
+  if (r) return r;
+  if (!slots || (tokens > 0 && (!k || !v))) return fail(H3B_ERR_INVALID_ARGUMENT, name + ": null pointer");
+  if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, name + ": dtype must be fp16 or bf16");
+  if (cache->dtype != 3 && cache->dtype != dtype)
+    return fail(H3B_ERR_UNSUPPORTED, name + ": the cache must hold the rows' type or e4m3");
+  if (n < 0 || n > cache->table_rows || tokens < 0 || tokens > (1 << 30) || (!starts && tokens != n))
+    return fail(H3B_ERR_INVALID_ARGUMENT, name + ": bad sizes");
+  if (tokens > 0 && (k_row_stride < cache->kv_heads * 128 || k_row_stride % 8 || v_row_stride < cache->kv_heads * 128 ||
+                     v_row_stride % 8))
+    return fail(H3B_ERR_INVALID_ARGUMENT, name + ": bad row stride");
+  if (!aligned16(k) || !aligned16(v)) return fail(H3B_ERR_UNSUPPORTED, name + ": rows must be 16-byte aligned");
+  *w = {};
+  w->k = static_cast<const uint16_t*>(k);
+  w->k_stride = k_row_stride;
+  w->v = static_cast<const uint16_t*>(v);
+  w->v_stride = v_row_stride;
+  w->tokens = tokens;
+  w->slots = slots;
+  w->n = (int)n;
+  w->starts = starts;
+  if (cache->dtype == 3) {
+    w->k_scale = cache->k_scale + layer * cache->kv_heads;
+    w->v_scale = cache->v_scale + layer * cache->kv_heads;
+  }
+  w->src_bf16 = dtype == 2;
+  return H3B_OK;
+}
+
+}  // namespace
+
+extern "C" {
 
 int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
                     int64_t tokens, void* stream) {
   if (n == 0 || tokens == 0) return ok();
-  const int r = check_cache(cache, layer, "pages_write");
+  h3b::PageWriteArgs w;
+  const int r = write_args(cache, layer, slots, n, starts, k, k_row_stride, v, v_row_stride, dtype, tokens, "pages_write", &w);
   if (r) return r;
-  if (!slots || !k || !v) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_write: null pointer");
-  if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, "pages_write: dtype must be fp16 or bf16");
-  if (cache->dtype != 3 && cache->dtype != dtype)
-    return fail(H3B_ERR_UNSUPPORTED, "pages_write: the cache must hold the rows' type or e4m3");
-  if (n < 0 || n > cache->table_rows || tokens < 0 || tokens > (1 << 30) || (!starts && tokens != n))
-    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_write: bad sizes");
-  if (k_row_stride < cache->kv_heads * 128 || k_row_stride % 8 || v_row_stride < cache->kv_heads * 128 || v_row_stride % 8)
-    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_write: bad row stride");
-  if (!aligned16(k) || !aligned16(v)) return fail(H3B_ERR_UNSUPPORTED, "pages_write: rows must be 16-byte aligned");
-  h3b::PageWriteArgs w{};
-  w.k = static_cast<const uint16_t*>(k);
-  w.k_stride = k_row_stride;
-  w.v = static_cast<const uint16_t*>(v);
-  w.v_stride = v_row_stride;
-  w.tokens = tokens;
-  w.slots = slots;
-  w.n = (int)n;
-  w.starts = starts;
-  if (cache->dtype == 3) {
-    w.k_scale = cache->k_scale + layer * cache->kv_heads;
-    w.v_scale = cache->v_scale + layer * cache->kv_heads;
-  }
-  w.src_bf16 = dtype == 2;
-  return cuda_status(h3b::launch_pages_write(page_tables(cache), page_pools(cache), layer, w, st(stream)), "pages_write");
+  return cuda_status(h3b::launch_pages_write(page_tables(cache), page_pools(cache), layer, w, nullptr, st(stream)),
+                     "pages_write");
+}
+
+int h3b_pages_append(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
+                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
+                     int64_t tokens, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (n == 0) return ok();
+  h3b::PageWriteArgs w;
+  const int r = write_args(cache, layer, slots, n, starts, k, k_row_stride, v, v_row_stride, dtype, tokens, "pages_append", &w);
+  if (r) return r;
+  if (!workspace || workspace_bytes < h3b::pages_workspace_bytes(n, cache->pages))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "pages_append: workspace too small");
+  int32_t* ws = static_cast<int32_t*>(workspace);
+  const cudaError_t e = h3b::launch_pages_extend(page_tables(cache), page_pools(cache), slots, (int)n, starts, ws, false,
+                                                 st(stream));
+  if (e != cudaSuccess) return cuda_status(e, "pages_append");
+  return cuda_status(h3b::launch_pages_write(page_tables(cache), page_pools(cache), layer, w, ws, st(stream)),
+                     "pages_append");
 }
 
 int h3b_pages_fork(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {

@@ -121,6 +121,8 @@ __global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs
     carry = 0;
     prefix[0] = 0;
   }
+  chain_next();
+  chain_wait();
   __syncthreads();
   for (int base = 0; base < a.seqs; base += kDecodeThreads) {
     const int i = base + threadIdx.x;
@@ -445,8 +447,11 @@ __global__ void __launch_bounds__(256) decode_join_kernel(DecodeArgs a) {
   __shared__ float red[8];
   __shared__ float acc2[128];
   const int group = a.Hq / a.Hkv, groups = (group + NT * 8 - 1) / (NT * 8), heads = a.Hkv * groups;
-  const int b = blockIdx.x / heads, hp = blockIdx.x % heads;
-  const int kh = hp / groups, r = blockIdx.y, head = (hp % groups) * NT * 8 + r;
+  const int rows = min(group, NT * 8);
+  const int b = blockIdx.x / rows / heads, hp = blockIdx.x / rows % heads;
+  const int kh = hp / groups, r = blockIdx.x % rows, head = (hp % groups) * NT * 8 + r;
+  chain_next();
+  chain_wait();
   if (head >= group) return;
   const int64_t* prefix = reinterpret_cast<const int64_t*>(a.partial);
   const int64_t share = prefix[kDecodeMaxSeqs + 1];
@@ -525,12 +530,10 @@ cudaError_t launch_decode(DecodeArgs a, cudaStream_t s) {
   if (blocks < 1) blocks = 1;
   a.workers = (int)blocks * kWarps;
   const size_t smem = (size_t)(a.seqs + 1) * 8;
-  decode_kernel<BF16, FP8, NT, MINB><<<(unsigned)blocks, kDecodeThreads, smem, s>>>(a);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_chained(decode_kernel<BF16, FP8, NT, MINB>, blocks, kDecodeThreads, smem, s, a);
   if (e != cudaSuccess) return e;
-  dim3 grid((unsigned)(a.seqs * heads), (unsigned)(group < NT * 8 ? group : NT * 8));
-  decode_join_kernel<BF16, NT><<<grid, 256, (size_t)a.workers * 4, s>>>(a);
-  return cudaGetLastError();
+  const int64_t joins = a.seqs * heads * (group < NT * 8 ? group : NT * 8);
+  return launch_chained(decode_join_kernel<BF16, NT>, joins, 256, (size_t)a.workers * 4, s, a);
 }
 
 }  // namespace

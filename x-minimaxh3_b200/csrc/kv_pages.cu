@@ -71,6 +71,8 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t,
   __shared__ int warp_free[kPlanWarps];
   __shared__ int copies, fault;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  chain_next();
+  chain_wait();
   const ExtendPlan p = extend_plan(ws, n);
   if (tid == 0) {
     copies = 0;
@@ -184,11 +186,12 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t,
 }
 
 // The rows that shared last pages held, into their copies: a warp per (copy, layer, K/V, head).
-__global__ void __launch_bounds__(256) extend_copy_kernel(PagePools pool, int pages, int page, int n, const int32_t* ws) {
+__device__ __forceinline__ void copy_shared_rows(const PagePools& pool, int pages, int page, int n, const int32_t* ws,
+                                                 int64_t warp, int64_t warps) {
   const ExtendPlan p = extend_plan(const_cast<int32_t*>(ws), n);
   const int64_t units = (int64_t)*p.copies * pool.layers * 2 * pool.Hkv;
   const int lane = threadIdx.x & 31, row16 = 128 * pool.elem / 16;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
+  for (int64_t u = warp; u < units; u += warps) {
     const int h = (int)(u % pool.Hkv), kv = (int)(u / pool.Hkv & 1);
     const int64_t rest = u / (2 * pool.Hkv), layer = rest % pool.layers;
     const int i = (int)(rest / pool.layers);
@@ -196,8 +199,22 @@ __global__ void __launch_bounds__(256) extend_copy_kernel(PagePools pool, int pa
     const int64_t slab = (int64_t)page * row16;
     const uint4* src = base + ((layer * pages + p.src[i]) * pool.Hkv + h) * slab;
     uint4* dst = base + ((layer * pages + p.dst[i]) * pool.Hkv + h) * slab;
-    for (int x = lane; x < p.part[i] * row16; x += 32) dst[x] = src[x];
+    const int n16 = p.part[i] * row16;
+    int x = lane;
+    for (; x + 96 < n16; x += 128) {
+      const uint4 a = src[x], b = src[x + 32], c = src[x + 64], d = src[x + 96];
+      dst[x] = a;
+      dst[x + 32] = b;
+      dst[x + 64] = c;
+      dst[x + 96] = d;
+    }
+    for (; x < n16; x += 32) dst[x] = src[x];
   }
+}
+__global__ void __launch_bounds__(256) extend_copy_kernel(PagePools pool, int pages, int page, int n, const int32_t* ws) {
+  chain_next();
+  chain_wait();
+  copy_shared_rows(pool, pages, page, n, ws, (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), (int64_t)gridDim.x * 8);
 }
 
 // K/V rows of the last tokens of each sequence into their pages, a warp per token.
@@ -208,9 +225,17 @@ __device__ __forceinline__ uint32_t to_e4m3x4(const float* x, float scale) {
   return lo | (hi << 16);
 }
 template <bool FP8, bool BF16>
-__global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w) {
+__global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w,
+                                                    const int32_t* ws, int copy_blocks) {
   const int lane = threadIdx.x & 31;
-  const int64_t tok = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  chain_next();
+  chain_wait();
+  if ((int)blockIdx.x < copy_blocks) {  // rows of other places of the same pages
+    copy_shared_rows(pool, t.pages, t.page, w.n, ws, (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5),
+                     (int64_t)copy_blocks * 8);
+    return;
+  }
+  const int64_t tok = (int64_t)(blockIdx.x - copy_blocks) * 8 + (threadIdx.x >> 5);
   if (tok >= w.tokens || *t.status != kPagesOk) return;
   int i = (int)tok, back = 1;  // the token is the back-th last of sequence i
   if (w.starts) {
@@ -285,6 +310,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const 
   __shared__ int fault;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) fault = kPagesOk;
+  chain_next();
+  chain_wait();
   if (*t.status != kPagesOk) return;
   if (!slots_valid(dst, n, t.rows, seen)) {
     if (tid == 0) *t.status = kPagesBadSlot;
@@ -321,6 +348,8 @@ __global__ void __launch_bounds__(kPlanThreads) truncate_kernel(PageTables t, co
                                                                 int n) {
   extern __shared__ uint32_t seen[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  chain_next();
+  chain_wait();
   if (*t.status != kPagesOk) return;
   if (!slots_valid(slots, n, t.rows, seen)) {
     if (tid == 0) *t.status = kPagesBadSlot;
@@ -358,6 +387,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PageTables t
   __shared__ int count_a[kPlanWarps], count_b[kPlanWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const CompactPlan p = compact_plan(ws, t.pages);
+  chain_next();
+  chain_wait();
   if (*t.status != kPagesOk) {
     if (tid == 0) {
       *p.moves = 0;
@@ -426,6 +457,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PageTables t
 }
 __global__ void __launch_bounds__(256) compact_table_kernel(PageTables t, const int32_t* ws) {
   const CompactPlan p = compact_plan(const_cast<int32_t*>(ws), t.pages);
+  chain_next();
+  chain_wait();
   const int used = *p.used;
   const int64_t n = (int64_t)t.rows * t.width;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -437,6 +470,8 @@ __global__ void __launch_bounds__(256) compact_table_kernel(PageTables t, const 
 // value (compact) or null (n moves, whose pages are checked here).
 __global__ void __launch_bounds__(256) move_kernel(PagePools pool, int pages, int64_t bytes, const int32_t* src,
                                                    const int32_t* dst, const int32_t* count, int n, int32_t* status) {
+  chain_next();
+  chain_wait();
   const int64_t units = (int64_t)(count ? *count : n) * pool.layers * 2;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t layer = u / 2 % pool.layers;
@@ -471,54 +506,49 @@ int64_t pages_workspace_bytes(int64_t n, int64_t pages) {
   return 4 * (extend > compact ? extend : compact);
 }
 
+constexpr int kFullGrid = 1184;  // eight blocks for each of 148 multiprocessors
+
 cudaError_t launch_pages_extend(const PageTables& t, const PagePools& p, const int32_t* slots, int n,
-                                const int32_t* starts, int32_t* ws, cudaStream_t s) {
-  extend_plan_kernel<<<1, kPlanThreads, seen_bytes(t.rows), s>>>(t, slots, n, starts, ws);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+                                const int32_t* starts, int32_t* ws, bool copy, cudaStream_t s) {
+  const cudaError_t e = launch_chained(extend_plan_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, n, starts, ws);
+  if (e != cudaSuccess || !copy) return e;
   const int64_t most = ((int64_t)n * p.layers * 2 * p.Hkv + 7) / 8;
-  extend_copy_kernel<<<(unsigned)(most < 1184 ? most : 1184), 256, 0, s>>>(p, t.pages, t.page, n, ws);
-  return cudaGetLastError();
+  return launch_chained(extend_copy_kernel, most < kFullGrid ? most : kFullGrid, 256, 0, s, p, t.pages, t.page, n, ws);
 }
 
 cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t layer, const PageWriteArgs& w,
-                               cudaStream_t s) {
-  const unsigned blocks = (unsigned)((w.tokens + 7) / 8);
-  if (p.elem == 2)
-    write_kernel<false, true><<<blocks, 256, 0, s>>>(t, p, layer, w);
-  else if (w.src_bf16)
-    write_kernel<true, true><<<blocks, 256, 0, s>>>(t, p, layer, w);
-  else
-    write_kernel<true, false><<<blocks, 256, 0, s>>>(t, p, layer, w);
-  return cudaGetLastError();
+                               const int32_t* ws, cudaStream_t s) {
+  int64_t copies = 0;
+  if (ws) {
+    copies = ((int64_t)w.n * p.layers * 2 * p.Hkv + 7) / 8;
+    if (copies > kFullGrid / 2) copies = kFullGrid / 2;
+  }
+  auto kern = p.elem == 2 ? write_kernel<false, true> : w.src_bf16 ? write_kernel<true, true> : write_kernel<true, false>;
+  return launch_chained(kern, copies + (w.tokens + 7) / 8, 256, 0, s, t, p, layer, w, ws, (int)copies);
 }
 
 cudaError_t launch_pages_fork(const PageTables& t, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
-  fork_kernel<<<1, kPlanThreads, seen_bytes(t.rows), s>>>(t, src, dst, n);
-  return cudaGetLastError();
+  return launch_chained(fork_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n);
 }
 cudaError_t launch_pages_truncate(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
                                   cudaStream_t s) {
-  truncate_kernel<<<1, kPlanThreads, seen_bytes(t.rows), s>>>(t, slots, keep, n);
-  return cudaGetLastError();
+  return launch_chained(truncate_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n);
 }
 cudaError_t launch_pages_compact(const PageTables& t, const PagePools& p, int32_t* ws, cudaStream_t s) {
-  compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(t, ws);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_chained(compact_plan_kernel, 1, kPlanThreads, 0, s, t, ws);
   if (e != cudaSuccess) return e;
   const CompactPlan c = compact_plan(ws, t.pages);
   const int64_t entries = ((int64_t)t.rows * t.width + 255) / 256;
-  compact_table_kernel<<<(unsigned)(entries < 1184 ? entries : 1184), 256, 0, s>>>(t, ws);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  move_kernel<<<1184, 256, 0, s>>>(p, t.pages, (int64_t)p.Hkv * t.page * 128 * p.elem, c.src, c.dst, c.moves, 0, nullptr);
-  return cudaGetLastError();
+  e = launch_chained(compact_table_kernel, entries < kFullGrid ? entries : kFullGrid, 256, 0, s, t, ws);
+  if (e != cudaSuccess) return e;
+  return launch_chained(move_kernel, kFullGrid, 256, 0, s, p, t.pages, (int64_t)p.Hkv * t.page * 128 * p.elem, c.src,
+                        c.dst, c.moves, 0, nullptr);
 }
 cudaError_t launch_pages_copy(const PagePools& p, int pages, int page, const int32_t* src, const int32_t* dst, int n,
                               int32_t* status, cudaStream_t s) {
   const int64_t units = (int64_t)n * p.layers * 2;
-  move_kernel<<<(unsigned)(units < 1184 ? units : 1184), 256, 0, s>>>(p, pages, (int64_t)p.Hkv * page * 128 * p.elem, src,
-                                                                     dst, nullptr, n, status);
-  return cudaGetLastError();
+  return launch_chained(move_kernel, units < kFullGrid ? units : kFullGrid, 256, 0, s, p, pages,
+                        (int64_t)p.Hkv * page * 128 * p.elem, src, dst, nullptr, n, status);
 }
 
 }  // namespace h3b

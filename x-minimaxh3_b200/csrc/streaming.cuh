@@ -6,6 +6,27 @@
 
 namespace h3b {
 
+// Kernels of one step follow each other closely: each is launched to start while the one
+// before it in the stream ends (programmatic stream serialization), does what needs no
+// earlier result, and waits for that kernel's completion (chain_wait) before it touches
+// global memory; chain_next lets the kernel after it start that early in turn.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+cudaError_t launch_chained(void (*kernel)(P...), int64_t grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Which keys a query sees: key j of a sequence with lk keys is visible to the query at
 // position p >= 0 when  j < lk,  j <= last(p)  and  (last(p) - j < window or j < sinks).
 // last(p) = p for chunk 1; otherwise the end of p's chunk, chunks counted from the end
@@ -134,8 +155,9 @@ struct PagePools {
 };
 constexpr int kPagesMaxRows = 1 << 18;
 int64_t pages_workspace_bytes(int64_t n, int64_t pages);
+// copy: whether to make the planned copies too (launch_pages_write can)
 cudaError_t launch_pages_extend(const PageTables& t, const PagePools& p, const int32_t* slots, int n,
-                                const int32_t* starts, int32_t* ws, cudaStream_t s);
+                                const int32_t* starts, int32_t* ws, bool copy, cudaStream_t s);
 struct PageWriteArgs {
   const uint16_t* k;
   int64_t k_stride;
@@ -149,8 +171,9 @@ struct PageWriteArgs {
   const float* v_scale;
   int src_bf16;  // rows are bf16 (else fp16)
 };
+// ws: null, or the plan of launch_pages_extend whose copies are made by the same kernel
 cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t layer, const PageWriteArgs& w,
-                               cudaStream_t s);
+                               const int32_t* ws, cudaStream_t s);
 cudaError_t launch_pages_fork(const PageTables& t, const int32_t* src, const int32_t* dst, int n, cudaStream_t s);
 cudaError_t launch_pages_truncate(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
                                   cudaStream_t s);

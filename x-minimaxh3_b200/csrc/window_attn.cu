@@ -26,6 +26,7 @@
 // from tensor memory, S of the others after that step's PV, which reads P from their
 // columns; PV of 64 keys starts when half of P is written.  The two tiles take turns.
 // Tensor memory: S_A 0..127, S_B 128..255, O_A 256..383, O_B 384..511, P over S + 64.
+#include <atomic>
 #include <climits>
 
 #include "h3b_kernels.cuh"
@@ -458,6 +459,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
     }
+    chain_next();
+    chain_wait();
     plan_item<PAGED>(a, blockIdx.x, items, rows_per_cta, &plans[0]);
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -485,6 +488,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     cleared[0] = cleared[1] = 0;
     fence_mbar_init();
   }
+  if (warp != 0) chain_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -833,20 +837,26 @@ int launch_window(const WindowArgs& a, cudaStream_t s, cudaError_t* err) {
     if (!make_rows_tmap(&tv, a.v, BF16, (uint64_t)a.Hkv, (uint64_t)a.Tk, 256, (uint64_t)a.v_stride * 2, 1, 128)) return 1;
   }
   auto kern = window_kernel<BF16, PAGED>;
-  cudaFuncAttributes fa;
-  *err = cudaFuncGetAttributes(&fa, kern);
-  if (*err != cudaSuccess) return 2;
-  if (fa.numRegs != kWinRegs) return 3;  // the register split was planned for another count
-  *err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWinSmem);
-  if (*err != cudaSuccess) return 2;
+  // the kernel's attributes are checked and set once per device
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if ((*err = cudaGetDevice(&dev)) != cudaSuccess) return 2;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    cudaFuncAttributes fa;
+    if ((*err = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return 2;
+    if (fa.numRegs != kWinRegs) return 3;  // the register split was planned for another count
+    *err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWinSmem);
+    if (*err != cudaSuccess) return 2;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   const bool by_heads = (a.Hq / a.Hkv) % 2 == 0;
   const int rows = by_heads ? 128 : 256;
   const int64_t tiles = (int64_t)a.Tq / rows + a.seqs;  // sum of ceil(len / rows) is at most this
   const int64_t items = tiles * (by_heads ? a.Hq / 2 : a.Hq);
   if (items > INT_MAX / 2) return 4;
   const int64_t ctas = items < num_sms() ? items : num_sms();
-  kern<<<(unsigned)ctas, kWinThreads, kWinSmem, s>>>(tq, tk, tv, a, rows, (int)items);
-  *err = cudaGetLastError();
+  *err = launch_chained(kern, ctas, kWinThreads, kWinSmem, s, tq, tk, tv, a, rows, (int)items);
   return *err == cudaSuccess ? 0 : 2;
 }
 

@@ -125,6 +125,8 @@ _SIGNATURES = {
     "h3b_pages_extend": [_cache_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
     "h3b_pages_write": [_cache_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int,
                         c_int64, c_void_p],
+    "h3b_pages_append": [_cache_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                         c_int64, c_void_p, c_int64, c_void_p],
     "h3b_pages_fork": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
     "h3b_pages_truncate": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
     "h3b_pages_compact": [_cache_p, c_void_p, c_int64, c_void_p],
@@ -162,7 +164,7 @@ def lib():
 
 
 # kernels each entry launches (for the benchmark's launch count); default 1
-_KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2, "decode_attention": 2, "pages_extend": 2,
+_KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2, "decode_attention": 2, "pages_extend": 2, "pages_append": 2,
                      "pages_compact": 3}
 _launches = 0
 

@@ -25,7 +25,6 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import H3BError, PageCacheStruct, check, lib
-from .ops import _cuda, _p, _stream
 
 HEAD_DIM = 128
 PAGE_TOKENS = (16, 32, 64, 128)
@@ -40,22 +39,36 @@ STATUS_TEXT = {
 }
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _stream(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device, as the C entries take it (a token's worth of
+    calls is short enough for the stream object's construction to count)."""
+    return _raw_stream(t.get_device())
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _index(t: torch.Tensor, what: str, n: int | None = None) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.ndim != 1 or not t.is_cuda or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.ndim != 1 or not t.is_cuda or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 CUDA vector")
-    if n is not None and t.numel() != n:
+    if n is not None and t.shape[0] != n:
         raise ValueError(f"{what} must have {n} entries")
     return t
 
 
 def _token_rows(x: torch.Tensor, heads: int | None, what: str) -> torch.Tensor:
     """[T, H, 128] fp16 / bf16 with contiguous heads (any row stride that keeps 16-byte alignment)."""
-    if x.ndim != 3 or x.shape[2] != HEAD_DIM or (heads is not None and x.shape[1] != heads):
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {HEAD_DIM}]")
-    if x.dtype not in (torch.bfloat16, torch.float16):
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
         raise ValueError(f"{what} must be bfloat16 or float16")
-    st = x.stride()
-    if st[2] != 1 or st[1] != HEAD_DIM or st[0] % 8 or st[0] < x.shape[1] * HEAD_DIM or x.data_ptr() % 16:
+    row, head, channel = x.stride()
+    if channel != 1 or head != HEAD_DIM or row % 8 or row < shape[1] * HEAD_DIM or x.data_ptr() % 16:
         x = x.contiguous()
     return x
 
@@ -76,33 +89,36 @@ class PagedKVCache:
     v_scale: torch.Tensor | None = None
 
     def __post_init__(self) -> None:
-        k, v = self.k, self.v
-        _cuda("PagedKVCache", k, v, self.table, self.lens, self.refs, self.status, self.k_scale, self.v_scale)
-        if k.ndim != 5 or k.shape[4] != HEAD_DIM or k.shape != v.shape or k.dtype != v.dtype:
+        k, v, t, lens, refs, status = self.k, self.v, self.table, self.lens, self.refs, self.status
+        shape, dtype = k.shape, k.dtype
+        if not (k.is_cuda and v.is_cuda and t.is_cuda and lens.is_cuda and refs.is_cuda and status.is_cuda):
+            raise RuntimeError("PagedKVCache runs only on CUDA tensors (the B200 library has no CPU path)")
+        if len(shape) != 5 or shape[4] != HEAD_DIM or shape != v.shape or dtype is not v.dtype:
             raise ValueError("k and v must be [layers, pages, kv heads, page tokens, 128] of one type")
-        if k.dtype not in DTYPE_CODES:
+        if dtype not in DTYPE_CODES:
             raise ValueError("a cache holds float16, bfloat16 or float8_e4m3fn")
-        if k.shape[3] not in PAGE_TOKENS:
+        layers, pages, heads, page, _ = shape
+        if page not in PAGE_TOKENS:
             raise ValueError(f"page tokens must be one of {PAGE_TOKENS}")
-        layers, pages, heads, page, _ = k.shape
-        t = self.table
-        if t.ndim != 2 or self.lens.shape != (t.shape[0],) or self.refs.shape != (pages,) or self.status.numel() != 1:
+        rows, width = t.shape
+        if lens.shape != (rows,) or refs.shape != (pages,) or status.numel() != 1:
             raise ValueError("table [slots, width], lens [slots], refs [pages] and status [1] do not fit together")
-        for x in (t, self.lens, self.refs, self.status):
-            if x.dtype != torch.int32:
-                raise ValueError("table, lens, refs and status must be int32")
-        if k.dtype == torch.float8_e4m3fn:
+        if not t.dtype is lens.dtype is refs.dtype is status.dtype is torch.int32:
+            raise ValueError("table, lens, refs and status must be int32")
+        if not (k.is_contiguous() and v.is_contiguous() and t.is_contiguous() and lens.is_contiguous()
+                and refs.is_contiguous()):
+            raise ValueError("cache tensors must be contiguous")
+        k_scale = v_scale = None
+        if dtype is torch.float8_e4m3fn:
             for x in (self.k_scale, self.v_scale):
-                if x is None or x.dtype != torch.float32 or x.shape != (layers, heads) or not x.is_contiguous():
+                if (x is None or x.dtype is not torch.float32 or x.shape != (layers, heads) or not x.is_contiguous()
+                        or not x.is_cuda):
                     raise ValueError("an e4m3 cache needs float32 k_scale and v_scale [layers, kv heads]")
-        for x in (k, v, t, self.lens, self.refs):
-            if not x.is_contiguous():
-                raise ValueError("cache tensors must be contiguous")
-        scales = self.k_scale is not None and k.dtype == torch.float8_e4m3fn
+            k_scale, v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        self.page_tokens, self.kv_heads = page, heads
         self._ref = ctypes.byref(PageCacheStruct(
-            k.data_ptr(), v.data_ptr(), layers, pages, heads, page, DTYPE_CODES[k.dtype],
-            self.k_scale.data_ptr() if scales else None, self.v_scale.data_ptr() if scales else None, t.data_ptr(),
-            t.shape[0], t.shape[1], self.lens.data_ptr(), self.refs.data_ptr(), self.status.data_ptr()))
+            k.data_ptr(), v.data_ptr(), layers, pages, heads, page, DTYPE_CODES[dtype], k_scale, v_scale, t.data_ptr(),
+            rows, width, lens.data_ptr(), refs.data_ptr(), status.data_ptr()))
 
     @classmethod
     def create(cls, layers: int, pages: int, page_tokens: int, kv_heads: int, slots: int, max_tokens: int,
@@ -119,16 +135,8 @@ class PagedKVCache:
                    torch.full((slots, -(-max_tokens // page_tokens)), -1, **ints), torch.zeros(slots, **ints),
                    torch.zeros(pages, **ints), torch.zeros(1, **ints), k_scale, v_scale)
 
-    @property
-    def page_tokens(self) -> int:
-        return self.k.shape[3]
-
-    @property
-    def kv_heads(self) -> int:
-        return self.k.shape[2]
-
     def _workspace(self, n: int) -> torch.Tensor:
-        return torch.empty(lib().h3b_pages_workspace_bytes(n, self.k.shape[1]), device=self.k.device, dtype=torch.uint8)
+        return self.status.new_empty(lib().h3b_pages_workspace_bytes(n, self.k.shape[1]), dtype=torch.uint8)
 
     def extend(self, slots: torch.Tensor, starts: torch.Tensor | None = None) -> None:
         """Room for starts[i + 1] - starts[i] more tokens (None: one) of each of the distinct slots,
@@ -137,57 +145,64 @@ class PagedKVCache:
         if starts is not None:
             _index(starts, "starts", n + 1)
         ws = self._workspace(n)
-        check(lib().h3b_pages_extend(self._ref, _p(slots), n, _p(starts), _p(ws), ws.numel(), _stream(self.k)),
+        check(lib().h3b_pages_extend(self._ref, _ptr(slots), n, _ptr(starts), _ptr(ws), ws.numel(), _stream(self.k)),
               "pages_extend")
 
     def write(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | None = None,
               layer: int = 0) -> None:
         """K/V rows [tokens, kv heads, 128] into the last tokens of each slot, as `extend` made room for them."""
-        n = _index(slots, "slots").numel()
+        self._rows_into(lib().h3b_pages_write, "pages_write", slots, k, v, starts, layer)
+
+    def _rows_into(self, entry, what, slots, k, v, starts, layer, ws=None) -> None:
+        n = _index(slots, "slots").shape[0]
         if starts is not None:
             _index(starts, "starts", n + 1)
         k, v = _token_rows(k, self.kv_heads, "k"), _token_rows(v, self.kv_heads, "v")
-        _cuda("PagedKVCache.write", k, v)
-        if k.shape != v.shape or k.dtype != v.dtype:
+        if not (k.is_cuda and v.is_cuda):
+            raise RuntimeError("PagedKVCache takes only CUDA tensors (the B200 library has no CPU path)")
+        if k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError("k and v must have one shape and type")
         if starts is None and k.shape[0] != n:
             raise ValueError("without starts there is one token for each slot")
-        if self.k.dtype not in (k.dtype, torch.float8_e4m3fn):
+        if self.k.dtype is not k.dtype and self.k.dtype is not torch.float8_e4m3fn:
             raise ValueError(f"a {self.k.dtype} cache does not take {k.dtype} rows")
-        check(lib().h3b_pages_write(self._ref, int(layer), _p(slots), n, _p(starts), _p(k), k.stride(0), _p(v),
-                                    v.stride(0), DTYPE_CODES[k.dtype], k.shape[0], _stream(self.k)), "pages_write")
+        args = (self._ref, int(layer), slots.data_ptr(), n, _ptr(starts), k.data_ptr(), k.stride(0), v.data_ptr(),
+                v.stride(0), DTYPE_CODES[k.dtype], k.shape[0])
+        if ws is not None:
+            args += (ws.data_ptr(), ws.shape[0])
+        check(entry(*args, _stream(self.k)), what)
 
     def append(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | None = None,
                layer: int = 0) -> None:
         """extend, then write into `layer` (the other layers' rows are the caller's to write)."""
-        self.extend(slots, starts)
-        self.write(slots, k, v, starts, layer)
+        self._rows_into(lib().h3b_pages_append, "pages_append", slots, k, v, starts, layer,
+                        self._workspace(slots.shape[0]))
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Empty slots dst[i] become sequences that share the pages of src[i]."""
         n = _index(src, "src").numel()
-        check(lib().h3b_pages_fork(self._ref, _p(src), _p(_index(dst, "dst", n)), n, _stream(self.k)), "pages_fork")
+        check(lib().h3b_pages_fork(self._ref, _ptr(src), _ptr(_index(dst, "dst", n)), n, _stream(self.k)), "pages_fork")
 
     def truncate(self, slots: torch.Tensor, keep: torch.Tensor) -> None:
         """Each of the distinct slots keeps its first keep[i] tokens."""
         n = _index(slots, "slots").numel()
-        check(lib().h3b_pages_truncate(self._ref, _p(slots), _p(_index(keep, "keep", n)), n, _stream(self.k)),
+        check(lib().h3b_pages_truncate(self._ref, _ptr(slots), _ptr(_index(keep, "keep", n)), n, _stream(self.k)),
               "pages_truncate")
 
     def free(self, slots: torch.Tensor) -> None:
         """The distinct slots become empty; pages that no other sequence shares are free again."""
         n = _index(slots, "slots").numel()
-        check(lib().h3b_pages_truncate(self._ref, _p(slots), None, n, _stream(self.k)), "pages_truncate")
+        check(lib().h3b_pages_truncate(self._ref, _ptr(slots), None, n, _stream(self.k)), "pages_truncate")
 
     def compact(self) -> None:
         """Pages in use move to the front of the pool."""
         ws = self._workspace(0)
-        check(lib().h3b_pages_compact(self._ref, _p(ws), ws.numel(), _stream(self.k)), "pages_compact")
+        check(lib().h3b_pages_compact(self._ref, _ptr(ws), ws.numel(), _stream(self.k)), "pages_compact")
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Pages src[i] over pages dst[i] in every layer (no page may be both); the tables stay."""
         n = _index(src, "src").numel()
-        check(lib().h3b_pages_copy(self._ref, _p(src), _p(_index(dst, "dst", n)), n, _stream(self.k)), "pages_copy")
+        check(lib().h3b_pages_copy(self._ref, _ptr(src), _ptr(_index(dst, "dst", n)), n, _stream(self.k)), "pages_copy")
 
     def check(self) -> None:
         """Wait for the stream; raise, and clear the status word, if a call could not be done."""

@@ -26,8 +26,8 @@ import torch
 
 from . import context as _context
 from ._lib import check, lib
-from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _token_rows
-from .ops import _cuda, _p, _stream
+from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _ptr, _stream, _token_rows
+from .ops import _cuda
 
 UNLIMITED = 1 << 30
 
@@ -42,7 +42,7 @@ def _rule(window: int | None, sinks: int, chunk: int) -> tuple[int, int, int]:
 
 def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda:
         raise ValueError("out must have q's shape and type")
     st = out.stride()
@@ -68,7 +68,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     ragged batch (from 0 to Tq / Tk); None: one sequence."""
     _cuda("window_attention", q, k, v)
     q, k, v = _token_rows(q, None, "q"), _token_rows(k, None, "k"), _token_rows(v, None, "v")
-    if k.shape != v.shape or not q.dtype == k.dtype == v.dtype:
+    if k.shape != v.shape or not q.dtype is k.dtype is v.dtype:
         raise ValueError("k and v must have one shape, and q their type")
     if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError("the query heads must be a multiple of the kv heads")
@@ -82,9 +82,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         if seqs < 1:
             raise ValueError("query_starts needs at least two entries")
     out = _output(out, q)
-    check(lib().h3b_window_attention(_p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0), DTYPE_CODES[q.dtype],
-                                     q.shape[0], k.shape[0], _p(query_starts), _p(key_starts), seqs, q.shape[1],
-                                     k.shape[1], window, sinks, chunk, _scale(scale), _p(out), out.stride(0),
+    check(lib().h3b_window_attention(_ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), DTYPE_CODES[q.dtype],
+                                     q.shape[0], k.shape[0], _ptr(query_starts), _ptr(key_starts), seqs, q.shape[1],
+                                     k.shape[1], window, sinks, chunk, _scale(scale), _ptr(out), out.stride(0),
                                      _stream(q)), "window_attention")
     return out
 
@@ -117,9 +117,9 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
     elif seqs > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
     out = _output(out, q)
-    check(lib().h3b_paged_window_attention(_p(q), q.stride(0), DTYPE_CODES[q.dtype], q.shape[0], _p(query_starts),
-                                           _p(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
-                                           _scale(scale), _p(out), out.stride(0), _stream(q)),
+    check(lib().h3b_paged_window_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], q.shape[0], _ptr(query_starts),
+                                           _ptr(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
+                                           _scale(scale), _ptr(out), out.stride(0), _stream(q)),
           "paged_window_attention")
     return out
 
@@ -140,12 +140,12 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
         raise ValueError("more sequences than the cache has slots")
     need = lib().h3b_decode_workspace_bytes()
     if workspace is None:
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+        workspace = q.new_empty(need, dtype=torch.uint8)
     elif workspace.numel() * workspace.element_size() < need or not workspace.is_cuda:
         raise ValueError(f"the workspace must have {need} bytes on the device")
     out = _output(out, q)
-    check(lib().h3b_decode_attention(_p(q), q.stride(0), DTYPE_CODES[q.dtype], _p(slots), n, q.shape[1], cache._ref,
-                                     layer, window, sinks, _scale(scale), _p(out), out.stride(0), _p(workspace), need,
+    check(lib().h3b_decode_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], _ptr(slots), n, q.shape[1], cache._ref,
+                                     layer, window, sinks, _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), need,
                                      _stream(q)), "decode_attention")
     return out
 
