@@ -243,13 +243,15 @@ __global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs
       l[t][0] = l[t][1] = 0.f;
     }
 
-    constexpr int kEB = FP8 ? 1 : 2;           // bytes per element
-    constexpr int kKL = FP8 ? 2 : 4;           // 16-byte loads of a key row per thread
+    constexpr int kEB = FP8 ? 1 : 2;  // bytes per element
+    constexpr int kKL = FP8 ? 2 : 4;  // 16-byte loads of a key row per thread
     constexpr int kVL = FP8 ? 1 : 2;
-    uint4 kr[2][kKL], vr[4][kVL];
-    int pgs = 0, pbase = c0 - 32;
+    constexpr int CH = FP8 ? 2 : 1;   // chunks of a step: 8 KB of K and V under way per warp either way
+    uint4 kr[CH][2][kKL], vr[CH][4][kVL];
+    int pgs = 0, pbase = c0 - 64;
     auto chunk_of = [&](int ord) { return ord < cl.first_n ? ord : ord - cl.first_n + cl.win; };
-    // byte offset of key row 0 of chunk ordinal `ord`; page numbers come 32 chunks at a time
+    // byte offset of key row 0 of chunk ordinal `ord`; page numbers come 32 chunks at a
+    // time (an ordinal past the piece stands for its last)
     auto offset_of = [&](int ord) -> int64_t {
       if (ord - pbase >= 32) {
         pbase = ord;
@@ -257,80 +259,99 @@ __global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs
         pgs = (int)paged_page(a.paged, slot, chunk_of(o2) * kChunk / a.paged.page);
       }
       const int64_t pg = __shfl_sync(0xffffffffu, pgs, ord - pbase);
-      return ((pg * a.Hkv + kh) * a.paged.page + (chunk_of(ord) * kChunk & (a.paged.page - 1))) * (int64_t)(128 * kEB);
+      const int j = chunk_of(min(ord, c1 - 1)) * kChunk;
+      return ((pg * a.Hkv + kh) * a.paged.page + (j & (a.paged.page - 1))) * (int64_t)(128 * kEB);
     };
-    auto load_k = [&](int64_t off) {
-      const uint8_t* p = static_cast<const uint8_t*>(a.paged.k) + off + g * (128 * kEB) + c * 16;
+    auto load_k = [&](const int64_t (&off)[CH]) {
 #pragma unroll
-      for (int i = 0; i < kKL; ++i) {
-        kr[0][i] = ld_stream(p + i * 64);
-        kr[1][i] = ld_stream(p + i * 64 + 8 * 128 * kEB);
+      for (int u = 0; u < CH; ++u) {
+        const uint8_t* p = static_cast<const uint8_t*>(a.paged.k) + off[u] + g * (128 * kEB) + c * 16;
+#pragma unroll
+        for (int i = 0; i < kKL; ++i) {
+          kr[u][0][i] = ld_stream(p + i * 64);
+          kr[u][1][i] = ld_stream(p + i * 64 + 8 * 128 * kEB);
+        }
       }
     };
-    auto load_v = [&](int64_t off) {
-      const uint8_t* p = static_cast<const uint8_t*>(a.paged.v) + off + 2 * c * (128 * kEB) + g * 16;
+    auto load_v = [&](const int64_t (&off)[CH]) {
 #pragma unroll
-      for (int i = 0; i < kVL; ++i) {
-        vr[0][i] = ld_stream(p + i * 128);
-        vr[1][i] = ld_stream(p + i * 128 + 128 * kEB);
-        vr[2][i] = ld_stream(p + i * 128 + 8 * 128 * kEB);
-        vr[3][i] = ld_stream(p + i * 128 + 9 * 128 * kEB);
+      for (int u = 0; u < CH; ++u) {
+        const uint8_t* p = static_cast<const uint8_t*>(a.paged.v) + off[u] + 2 * c * (128 * kEB) + g * 16;
+#pragma unroll
+        for (int i = 0; i < kVL; ++i) {
+          vr[u][0][i] = ld_stream(p + i * 128);
+          vr[u][1][i] = ld_stream(p + i * 128 + 128 * kEB);
+          vr[u][2][i] = ld_stream(p + i * 128 + 8 * 128 * kEB);
+          vr[u][3][i] = ld_stream(p + i * 128 + 9 * 128 * kEB);
+        }
       }
     };
-    int64_t off = offset_of(c0);
+    int64_t off[CH];
+#pragma unroll
+    for (int u = 0; u < CH; ++u) off[u] = offset_of(c0 + u);
     load_k(off);
     load_v(off);
-    for (int ord = c0; ord < c1; ++ord) {
-      const int j0 = chunk_of(ord) * kChunk;
-      float s[NT][4];
+    for (int ord = c0; ord < c1; ord += CH) {
+      float s[CH][NT][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-        if constexpr (FP8) {
+      for (int u = 0; u < CH; ++u) {
 #pragma unroll
-          for (int i = 0; i < kKL; ++i) {
-            const uint32_t x[4] = {kr[0][i].x, kr[0][i].y, kr[0][i].z, kr[0][i].w};
-            const uint32_t y[4] = {kr[1][i].x, kr[1][i].y, kr[1][i].z, kr[1][i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              mma16816<false>(s[t], widen_lo(x[e]), widen_lo(y[e]), widen_hi(x[e]), widen_hi(y[e]),
-                              qf[t][4 * i + e][0], qf[t][4 * i + e][1]);
-          }
-        } else {
+        for (int t = 0; t < NT; ++t) {
+          float(&st)[4] = s[u][t];
+          st[0] = st[1] = st[2] = st[3] = 0.f;
 #pragma unroll
           for (int i = 0; i < kKL; ++i) {
-            mma16816<BF16>(s[t], kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y, qf[t][2 * i][0], qf[t][2 * i][1]);
-            mma16816<BF16>(s[t], kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w, qf[t][2 * i + 1][0],
-                           qf[t][2 * i + 1][1]);
+            const uint4 &x = kr[u][0][i], &y = kr[u][1][i];
+            if constexpr (FP8) {
+              const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                mma16816<false>(st, widen_lo(xs[e]), widen_lo(ys[e]), widen_hi(xs[e]), widen_hi(ys[e]),
+                                qf[t][4 * i + e][0], qf[t][4 * i + e][1]);
+            } else {
+              mma16816<BF16>(st, x.x, y.x, x.y, y.y, qf[t][2 * i][0], qf[t][2 * i][1]);
+              mma16816<BF16>(st, x.z, y.z, x.w, y.w, qf[t][2 * i + 1][0], qf[t][2 * i + 1][1]);
+            }
           }
         }
       }
-      int64_t next = 0;
-      if (ord + 1 < c1) {
-        next = offset_of(ord + 1);
-        load_k(next);
+      const bool more = ord + CH < c1;
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < CH; ++u) off[u] = offset_of(ord + CH + u);
+        load_k(off);
       }
-      const bool whole = j0 + kChunk <= see.end && (j0 >= see.lo || j0 + kChunk <= see.sinks);
-      uint32_t hide = 0;  // bit 0: key j0 + g is invisible, bit 1: key j0 + g + 8
-      if (!whole) {
-        auto seen = [&](int j) { return j < see.end && (j >= see.lo || j < see.sinks); };
-        hide = (seen(j0 + g) ? 0u : 1u) | (seen(j0 + g + 8) ? 0u : 2u);
-        // what lies in invisible rows (stale or never written) must not meet P = 0
+      uint32_t hide[CH];  // bit 0: key j0 + g of the chunk is invisible, bit 1: key j0 + g + 8
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if (!seen(j0 + 2 * c + (kk & 1) + (kk >> 1) * 8)) {
+      for (int u = 0; u < CH; ++u) {
+        const int j0 = chunk_of(ord + u) * kChunk;
+        const bool past = ord + u >= c1;
+        hide[u] = 0;
+        if (past || !(j0 + kChunk <= see.end && (j0 >= see.lo || j0 + kChunk <= see.sinks))) {
+          auto seen = [&](int j) { return !past && j < see.end && (j >= see.lo || j < see.sinks); };
+          hide[u] = (seen(j0 + g) ? 0u : 1u) | (seen(j0 + g + 8) ? 0u : 2u);
+          // what lies in invisible rows (stale or never written) must not meet P = 0
 #pragma unroll
-            for (int i = 0; i < kVL; ++i) vr[kk][i] = make_uint4(0, 0, 0, 0);
+          for (int kk = 0; kk < 4; ++kk) {
+            if (!seen(j0 + 2 * c + (kk & 1) + (kk >> 1) * 8)) {
+#pragma unroll
+              for (int i = 0; i < kVL; ++i) vr[u][kk][i] = make_uint4(0, 0, 0, 0);
+            }
           }
         }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[CH][NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float x[4] = {s[t][0] * sc[t][0], s[t][1] * sc[t][1], s[t][2] * sc[t][0], s[t][3] * sc[t][1]};
-        if (hide & 1) x[0] = x[1] = -INFINITY;
-        if (hide & 2) x[2] = x[3] = -INFINITY;
-        float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
+        float x[CH][4];
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < CH; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][e] = (hide[u] >> (e >> 1)) & 1u ? -INFINITY : s[u][t][e] * sc[t][e & 1];
+          mx0 = fmaxf(mx0, fmaxf(x[u][0], x[u][2]));
+          mx1 = fmaxf(mx1, fmaxf(x[u][1], x[u][3]));
+        }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
@@ -354,34 +375,40 @@ __global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs
         }
         // a maximum of -inf (nothing seen yet) subtracts as 0: exp2(-inf) = 0
         const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;
-        const float p0 = exp2_fast(x[0] - f0), p1 = exp2_fast(x[1] - f1);
-        const float p2 = exp2_fast(x[2] - f0), p3 = exp2_fast(x[3] - f1);
-        l[t][0] += p0 + p2;
-        l[t][1] += p1 + p3;
-        // P rounds to the 16-bit type of the V product; its sum stays in fp32
-        pb[t][0] = transpose8x8(pack16<BF16 && !FP8>(p0, p1));
-        pb[t][1] = transpose8x8(pack16<BF16 && !FP8>(p2, p3));
-      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t w[4];
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if constexpr (FP8) {
-            const uint4& v = vr[kk][0];
-            const uint32_t word = (i >> 1) == 0 ? v.x : (i >> 1) == 1 ? v.y : (i >> 1) == 2 ? v.z : v.w;
-            w[kk] = (i & 1) ? widen_hi(word) : widen_lo(word);
-          } else {
-            const uint4& v = vr[kk][i >> 2];
-            w[kk] = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
-          }
+        for (int u = 0; u < CH; ++u) {
+          const float p0 = exp2_fast(x[u][0] - f0), p1 = exp2_fast(x[u][1] - f1);
+          const float p2 = exp2_fast(x[u][2] - f0), p3 = exp2_fast(x[u][3] - f1);
+          l[t][0] += p0 + p2;
+          l[t][1] += p1 + p3;
+          // P rounds to the 16-bit type of the V product; its sum stays in fp32
+          pb[u][t][0] = transpose8x8(pack16<BF16 && !FP8>(p0, p1));
+          pb[u][t][1] = transpose8x8(pack16<BF16 && !FP8>(p2, p3));
         }
-        const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);
-        const uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) mma16816<BF16 && !FP8>(o[t][i], a0, a1, a2, a3, pb[t][0], pb[t][1]);
       }
-      if (ord + 1 < c1) load_v(next);
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            if constexpr (FP8) {
+              const uint4& v = vr[u][kk][0];
+              const uint32_t word = (i >> 1) == 0 ? v.x : (i >> 1) == 1 ? v.y : (i >> 1) == 2 ? v.z : v.w;
+              w[kk] = (i & 1) ? widen_hi(word) : widen_lo(word);
+            } else {
+              const uint4& v = vr[u][kk][i >> 2];
+              w[kk] = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+            }
+          }
+          const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);
+          const uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma16816<BF16 && !FP8>(o[t][i], a0, a1, a2, a3, pb[u][t][0], pb[u][t][1]);
+        }
+      }
+      if (more) load_v(off);
     }
 
     // channels of accumulator tile i, elements 0/1 (even) and 2/3 (odd): d, d + 1
@@ -438,75 +465,97 @@ __global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs
   }
 }
 
-// Joins the partial sums of one head: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p,
-// in the order of the keys.  Heads that one warp finished are left alone; a head without
-// any visible key gives 0.
+// Joins the partial sums of a (kv head, row group): out = sum_p 2^(m_p - M) O_p /
+// sum_p 2^(m_p - M) l_p.  A block per pair, its warps shared out over the rows and over
+// the parts of a row, four channels per lane; the order of the sums is that of the keys
+// for a given split.  Pairs that one warp finished are left alone; pairs without any
+// visible key give 0.
+constexpr int kJoinThreads = 512;
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(256) decode_join_kernel(DecodeArgs a) {
-  extern __shared__ float weight[];  // [workers]
-  __shared__ float red[8];
-  __shared__ float acc2[128];
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(DecodeArgs a) {
+  __shared__ float4 acc_s[kJoinThreads];
+  __shared__ float2 stat_s[kJoinThreads / 32];
   const int group = a.Hq / a.Hkv, groups = (group + NT * 8 - 1) / (NT * 8), heads = a.Hkv * groups;
-  const int rows = min(group, NT * 8);
-  const int b = blockIdx.x / rows / heads, hp = blockIdx.x / rows % heads;
-  const int kh = hp / groups, r = blockIdx.x % rows, head = (hp % groups) * NT * 8 + r;
+  const int b = blockIdx.x / heads, hp = blockIdx.x % heads;
+  const int kh = hp / groups, first = (hp % groups) * NT * 8, rows = min(group - first, NT * 8);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = (kJoinThreads / 32) / rows, r = warp % rows, split = warp / rows;
   chain_next();
   chain_wait();
-  if (head >= group) return;
   const int64_t* prefix = reinterpret_cast<const int64_t*>(a.partial);
-  const int64_t share = prefix[kDecodeMaxSeqs + 1];
-  const int64_t n = prefix[b + 1] - prefix[b];
-  uint16_t* dst = a.out + b * a.out_stride + ((int64_t)kh * group + head) * 128;
-  const int tid = threadIdx.x, d = tid & 127, half = tid >> 7;
+  const int64_t share = prefix[kDecodeMaxSeqs + 1], before = prefix[b];
+  const int64_t n = prefix[b + 1] - before;
+  uint16_t* dst = a.out + b * a.out_stride + ((int64_t)kh * group + first + r) * 128 + lane * 4;
   if (n == 0) {
-    if (tid < 64) reinterpret_cast<uint32_t*>(dst)[tid] = 0u;
+    if (split == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
     return;
   }
-  const int64_t s0 = prefix[b] * heads + hp * n, s1 = s0 + n;
+  const int64_t s0 = before * heads + hp * n, s1 = s0 + n;
   const int64_t w0 = s0 / share, w1 = (s1 - 1) / share;
   if (w0 == w1) return;
   const int parts = (int)(w1 - w0 + 1);
-  auto slot_of = [&](int p) { return (w0 + p) * share >= s0 ? 0 : 1; };
-  float mx = -INFINITY;
-  for (int p = tid; p < parts; p += 256) {
-    const float v = partial_stats<NT>(a.partial, a.workers, w0 + p, slot_of(p))[r * 2];
-    weight[p] = v;
-    mx = fmaxf(mx, v);
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (split < splits) {
+    // only the first part can lie in its worker's second slot: a later worker begins in the pair
+    const int head_slot = w0 * share >= s0 ? 0 : 1;
+    for (int p0 = split; p0 < parts; p0 += 8 * splits) {
+      float2 st[8];
+      float4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int p = p0 + u * splits;
+        const bool in = p < parts;
+        const int64_t w = w0 + (in ? p : 0);
+        const int slot = p == 0 ? head_slot : 0;
+        st[u] = in ? *reinterpret_cast<const float2*>(partial_stats<NT>(a.partial, a.workers, w, slot) + r * 2)
+                   : make_float2(-INFINITY, 0.f);
+        x[u] = in ? *reinterpret_cast<const float4*>(partial_rows<NT>(a.partial, w, slot) + r * 128 + lane * 4)
+                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mx = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) mx = fmaxf(mx, st[u].x);
+      const float base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base);
+      m = mx;
+      l *= keep;
+      acc.x *= keep;
+      acc.y *= keep;
+      acc.z *= keep;
+      acc.w *= keep;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = exp2f(st[u].x - base);
+        l = fmaf(w, st[u].y, l);
+        acc.x = fmaf(w, x[u].x, acc.x);
+        acc.y = fmaf(w, x[u].y, acc.y);
+        acc.z = fmaf(w, x[u].z, acc.z);
+        acc.w = fmaf(w, x[u].w, acc.w);
+      }
+    }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if ((tid & 31) == 0) red[tid >> 5] = mx;
+  acc_s[threadIdx.x] = acc;
+  if (lane == 0) stat_s[warp] = make_float2(m, l);
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) mx = fmaxf(mx, red[i]);
+  if (split > 0) return;
+  float mx = -INFINITY;
+  for (int i = 0; i < splits; ++i) mx = fmaxf(mx, stat_s[r + i * rows].x);
   const float base = mx == -INFINITY ? 0.f : mx;
   float total = 0.f;
-  for (int p = tid; p < parts; p += 256) {
-    const float w = exp2f(weight[p] - base);
-    weight[p] = w;
-    total = fmaf(w, partial_stats<NT>(a.partial, a.workers, w0 + p, slot_of(p))[r * 2 + 1], total);
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < splits; ++i) {
+    const float2 st = stat_s[r + i * rows];
+    const float4 x = acc_s[(r + i * rows) * 32 + lane];
+    const float w = exp2f(st.x - base);
+    total = fmaf(w, st.y, total);
+    acc.x = fmaf(w, x.x, acc.x);
+    acc.y = fmaf(w, x.y, acc.y);
+    acc.z = fmaf(w, x.z, acc.z);
+    acc.w = fmaf(w, x.w, acc.w);
   }
-  __syncthreads();
-  total = warp_butterfly_sum(total);
-  if ((tid & 31) == 0) red[tid >> 5] = total;
-  __syncthreads();
-  total = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) total += red[i];
-  float acc = 0.f;
-#pragma unroll 8
-  for (int p = half; p < parts; p += 2)
-    acc = fmaf(weight[p], partial_rows<NT>(a.partial, w0 + p, slot_of(p))[r * 128 + d], acc);
-  if (half) acc2[d] = acc;
-  __syncthreads();
-  if (!half) {
-    const float inv = (total == 0.f ? 0.f : 1.f / total) * (a.v_scale ? a.v_scale[kh] : 1.f);
-    const float v = (acc + acc2[d]) * inv;
-    if constexpr (BF16)
-      dst[d] = f32_to_bf16_bits(v);
-    else
-      dst[d] = __half_as_ushort(__float2half_rn(v));
-  }
+  const float inv = (total == 0.f ? 0.f : 1.f / total) * (a.v_scale ? a.v_scale[kh] : 1.f);
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
 }
 
 constexpr int kMinBlocks = 4;  // most blocks an SM runs in any variant (sizes the workspace)
@@ -532,8 +581,7 @@ cudaError_t launch_decode(DecodeArgs a, cudaStream_t s) {
   const size_t smem = (size_t)(a.seqs + 1) * 8;
   const cudaError_t e = launch_chained(decode_kernel<BF16, FP8, NT, MINB>, blocks, kDecodeThreads, smem, s, a);
   if (e != cudaSuccess) return e;
-  const int64_t joins = a.seqs * heads * (group < NT * 8 ? group : NT * 8);
-  return launch_chained(decode_join_kernel<BF16, NT>, joins, 256, (size_t)a.workers * 4, s, a);
+  return launch_chained(decode_join_kernel<BF16, NT>, a.seqs * heads, kJoinThreads, 0, s, a);
 }
 
 }  // namespace
@@ -549,8 +597,8 @@ cudaError_t launch_decode_attention(DecodeArgs a, int kind, cudaStream_t s) {
   switch (kind) {
     case 0: return wide ? launch_decode<true, false, 2, 2>(a, s) : launch_decode<true, false, 1, 3>(a, s);
     case 1: return wide ? launch_decode<false, false, 2, 2>(a, s) : launch_decode<false, false, 1, 3>(a, s);
-    case 2: return wide ? launch_decode<true, true, 2, 2>(a, s) : launch_decode<true, true, 1, 4>(a, s);
-    default: return wide ? launch_decode<false, true, 2, 2>(a, s) : launch_decode<false, true, 1, 4>(a, s);
+    case 2: return wide ? launch_decode<true, true, 2, 2>(a, s) : launch_decode<true, true, 1, 3>(a, s);
+    default: return wide ? launch_decode<false, true, 2, 2>(a, s) : launch_decode<false, true, 1, 3>(a, s);
   }
 }
 

@@ -39,20 +39,64 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* sum) {
   return v + before;
 }
 
+// apply(owner, r, load(owner, r)) for r < count of every thread's `count`, spread evenly
+// over the block, four at a time: owner is the thread whose count it is.  The loads of one
+// round are under way together, so apply must not change what load reads.
+// ends: [kPlanThreads] shared.
+template <typename L, typename A>
+__device__ __forceinline__ void block_expand(int count, int* red, int* ends, L load, A apply) {
+  int total;
+  ends[threadIdx.x] = block_scan(count, red, &total);
+  __syncthreads();
+  for (int e0 = threadIdx.x; e0 < total; e0 += 4 * kPlanThreads) {
+    int owner[4] = {0, 0, 0, 0}, r[4], value[4];
+#pragma unroll
+    for (int step = kPlanThreads / 2; step; step >>= 1) {  // the first owner whose end lies beyond e
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (ends[owner[u] + step - 1] <= e0 + u * kPlanThreads) owner[u] += step;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      owner[u] = min(owner[u], kPlanThreads - 1);
+      r[u] = e0 + u * kPlanThreads - (owner[u] ? ends[owner[u] - 1] : 0);
+      value[u] = e0 + u * kPlanThreads < total ? load(owner[u], r[u]) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (e0 + u * kPlanThreads < total) apply(owner[u], r[u], value[u]);
+  }
+  __syncthreads();
+}
+
 // Every slot named by slots[0, n) lies in the table and is named once.  seen: a bit per
-// row, zeroed here.  Returns false to every thread if not.
-__device__ bool slots_valid(const int32_t* slots, int n, int rows, uint32_t* seen) {
+// row, zeroed here.  Returns false to every thread if not.  mine: the thread's slots[tid],
+// loaded by the caller (n > tid).
+__device__ bool slots_valid(const int32_t* slots, int n, int rows, uint32_t* seen, int mine) {
   for (int i = threadIdx.x; i < (rows + 31) / 32; i += kPlanThreads) seen[i] = 0;
   __syncthreads();
   bool bad = false;
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-    const int s = slots[i];
+    const int s = i < kPlanThreads ? mine : slots[i];
     if (s < 0 || s >= rows)
       bad = true;
     else
       bad |= (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31)) & 1u;
   }
   return !__syncthreads_or(bad);
+}
+
+// Bit x of lane g's result: page `lo` + 32 g + x is free (a ballot per 32 pages).
+__device__ __forceinline__ uint32_t free_pages(const PageTables& t, int64_t lo) {
+  const int lane = threadIdx.x & 31;
+  uint32_t mask = 0;
+#pragma unroll 16
+  for (int g = 0; g < 32; ++g) {
+    const int64_t x = lo + g * 32 + lane;
+    const uint32_t m = __ballot_sync(0xffffffffu, x < t.pages && t.refs[x] == 0);
+    if (lane == g) mask = m;
+  }
+  return mask;
 }
 
 // workspace of extend: the copies' count (of 4 words), then first, asked, src, dst, part [n] each, given [pages]
@@ -67,25 +111,28 @@ __host__ __device__ __forceinline__ ExtendPlan extend_plan(int32_t* ws, int n) {
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t, const int32_t* slots, int n,
                                                                    const int32_t* starts, int32_t* ws) {
   extern __shared__ uint32_t seen[];
-  __shared__ int red[kPlanWarps];
-  __shared__ int warp_free[kPlanWarps];
+  __shared__ int red[kPlanWarps], ends[kPlanThreads], col[kPlanThreads], first_of[kPlanThreads];
   __shared__ int copies, fault;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   chain_next();
   chain_wait();
   const ExtendPlan p = extend_plan(ws, n);
+  // what does not depend on other loads is loaded together: each round trip counts here
+  const int status = *t.status;
+  const int mine = tid < n ? slots[tid] : 0;
+  uint32_t free_mask = free_pages(t, warp * 1024);
   if (tid == 0) {
     copies = 0;
     fault = kPagesOk;
     *p.copies = 0;
   }
-  if (*t.status != kPagesOk) return;
-  if (!slots_valid(slots, n, t.rows, seen)) {
+  if (status != kPagesOk) return;
+  if (!slots_valid(slots, n, t.rows, seen, mine)) {
     if (tid == 0) *t.status = kPagesBadSlot;
     return;
   }
   // pages asked for by each sequence, and where its share of them begins
-  int carry = 0, error = 0;
+  int carry = 0, error = 0, my_asked = 0, my_first = 0;
   for (int base = 0; base < n; base += kPlanThreads) {
     const int i = base + tid;
     int asked = 0;
@@ -107,13 +154,15 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t,
     }
     int sum;
     const int upto = block_scan(asked, red, &sum);
-    if (i < n) {
-      p.asked[i] = asked;
-      p.first[i] = carry + upto - asked;
+    my_asked = asked;
+    my_first = carry + upto - asked;
+    if (i < n && n > kPlanThreads) {
+      p.asked[i] = my_asked;
+      p.first[i] = my_first;
     }
     // a sum that passes 31 bits is more than any pool has
     if ((int64_t)carry + sum > t.pages) error = max(error, (int)kPagesExhausted);
-    carry = min(carry + sum, t.pages + 1);
+    carry = (int)min((int64_t)carry + sum, (int64_t)t.pages + 1);
   }
   if (error) atomicMax(&fault, error);
   __syncthreads();
@@ -122,64 +171,51 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t,
     return;
   }
   if (carry > 0) {
-    // the `carry` lowest free pages, in order: each warp counts the free pages of its
-    // part of refs, then lists those whose rank is asked for
-    const int per = ((t.pages + kPlanWarps - 1) / kPlanWarps + 31) & ~31;
-    const int lo = min(warp * per, t.pages), hi = min(lo + per, t.pages);
-    int count = 0;
-    for (int i = lo; i < hi; i += 128) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int x = i + u * 32 + lane;
-        count += x < hi && t.refs[x] == 0;
-      }
+    // The `carry` lowest free pages, in order: a warp looks at 1024 pages at a time, and
+    // the block's 32 x 1024 pages follow each other until enough are found.
+    int found = 0;
+    for (int64_t block = 0; block < t.pages && found < carry; block += kPlanWarps * 1024) {
+      if (block) free_mask = free_pages(t, block + warp * 1024);
+      int sum;
+      int rank = found + block_scan(__popc(free_mask), red, &sum) - __popc(free_mask);
+      const int64_t lo = block + warp * 1024 + lane * 32;
+      for (uint32_t m = free_mask; m && rank < carry; m &= m - 1, ++rank) p.given[rank] = (int)(lo + __ffs(m) - 1);
+      found += sum;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
-    if (lane == 0) warp_free[warp] = count;
-    __syncthreads();
-    int rank = 0, all = 0;
-    for (int w = 0; w < kPlanWarps; ++w) {
-      if (w < warp) rank += warp_free[w];
-      all += warp_free[w];
-    }
-    if (all < carry) {
+    if (found < carry) {
       if (tid == 0) *t.status = kPagesExhausted;
       return;
     }
-    for (int i = lo; i < hi && rank < carry; i += 32) {
-      const int x = i + lane;
-      const bool free_page = x < hi && t.refs[x] == 0;
-      const unsigned mask = __ballot_sync(0xffffffffu, free_page);
-      const int r = rank + __popc(mask & ((1u << lane) - 1));
-      if (free_page && r < carry) {
-        p.given[r] = x;
-        t.refs[x] = 1;
-      }
-      rank += __popc(mask);
-    }
     __syncthreads();
   }
-  // hand them out, a warp to a sequence
-  for (int i = warp; i < n; i += kPlanWarps) {
-    const int slot = slots[i], len = t.lens[slot], count = starts ? starts[i + 1] - starts[i] : 1;
-    const int have = pages_of(len, t.page), more = pages_of(len + count, t.page) - have;
-    const int asked = p.asked[i], first = p.first[i];
-    int32_t* row = t.table + (int64_t)slot * t.width;
-    const int copy = asked - more;
-    for (int r = lane; r < more; r += 32) row[have + r] = p.given[first + copy + r];
-    if (lane == 0) {
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + tid;
+    const bool kept = n <= kPlanThreads;
+    const int asked = i >= n ? 0 : kept ? my_asked : p.asked[i];
+    int slot = 0, grown = 0;
+    if (i < n) {
+      slot = slots[i];
+      const int len = t.lens[slot], first = kept ? my_first : p.first[i];
+      grown = len + (starts ? starts[i + 1] - starts[i] : 1);
+      const int have = pages_of(len, t.page), copy = asked - (pages_of(grown, t.page) - have);
       if (copy) {
-        const int old = row[have - 1], page = p.given[first];
-        const int at = atomicAdd(&copies, 1);
+        const int old = t.table[(int64_t)slot * t.width + have - 1], at = atomicAdd(&copies, 1);
         p.src[at] = old;
-        p.dst[at] = page;
+        p.dst[at] = p.given[first];
         p.part[at] = len % t.page;
-        row[have - 1] = page;
         atomicSub(&t.refs[old], 1);
       }
-      t.lens[slot] = len + count;
+      col[tid] = have - copy;
+      first_of[tid] = first;
     }
+    if (carry > 0)
+      block_expand(
+          asked, red, ends, [&](int owner, int r) { return p.given[first_of[owner] + r]; },
+          [&](int owner, int r, int page) {
+            t.table[(int64_t)slots[base + owner] * t.width + col[owner] + r] = page;
+            t.refs[page] = 1;
+          });
+    if (i < n) t.lens[slot] = grown;
   }
   __syncthreads();
   if (tid == 0) *p.copies = copies;
@@ -219,24 +255,39 @@ __global__ void __launch_bounds__(256) extend_copy_kernel(PagePools pool, int pa
 
 // K/V rows of the last tokens of each sequence into their pages, a warp per token.
 // E4M3 pools hold x / scale, rounded to nearest even and saturated at +-448.
-__device__ __forceinline__ uint32_t to_e4m3x4(const float* x, float scale) {
-  const uint32_t lo = f32x2_to_e4m3x2(__fdiv_rn(x[0], scale), __fdiv_rn(x[1], scale));
-  const uint32_t hi = f32x2_to_e4m3x2(__fdiv_rn(x[2], scale), __fdiv_rn(x[3], scale));
+// The quotient is the correctly rounded one (div_rn_by) wherever rounding it to E4M3 can
+// tell: above 1024 it saturates, and where the correction loses bits to underflow it is 0.
+// rb = 1 / scale; 0 where that is no normal number, which takes the plain division.
+__device__ __forceinline__ float over_scale(float x, float scale, float rb) {
+  if (rb == 0.f) return __fdiv_rn(x, scale);
+  const float q = __fmul_rn(x, rb);
+  return fabsf(q) > 1024.f ? q : div_rn_by(x, scale, rb);
+}
+__device__ __forceinline__ float scale_inverse(float scale) {
+  return scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : 0.f;
+}
+__device__ __forceinline__ uint32_t to_e4m3x4(float4 x, float scale, float rb) {
+  const uint32_t lo = f32x2_to_e4m3x2(over_scale(x.x, scale, rb), over_scale(x.y, scale, rb));
+  const uint32_t hi = f32x2_to_e4m3x2(over_scale(x.z, scale, rb), over_scale(x.w, scale, rb));
   return lo | (hi << 16);
 }
-template <bool FP8, bool BF16>
-__global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w,
-                                                    const int32_t* ws, int copy_blocks) {
-  const int lane = threadIdx.x & 31;
-  chain_next();
-  chain_wait();
-  if ((int)blockIdx.x < copy_blocks) {  // rows of other places of the same pages
-    copy_shared_rows(pool, t.pages, t.page, w.n, ws, (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5),
-                     (int64_t)copy_blocks * 8);
-    return;
-  }
-  const int64_t tok = (int64_t)(blockIdx.x - copy_blocks) * 8 + (threadIdx.x >> 5);
-  if (tok >= w.tokens || *t.status != kPagesOk) return;
+template <bool BF16>
+__device__ __forceinline__ float4 widen4(uint32_t w0, uint32_t w1) {
+  if constexpr (BF16)
+    return make_float4(__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16),
+                       __uint_as_float(w1 & 0xffff0000u));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w0));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w1));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 to_e4m3x16(const uint4& a, const uint4& b, float scale) {
+  const float rb = scale_inverse(scale);
+  return make_uint4(to_e4m3x4(widen4<BF16>(a.x, a.y), scale, rb), to_e4m3x4(widen4<BF16>(a.z, a.w), scale, rb),
+                    to_e4m3x4(widen4<BF16>(b.x, b.y), scale, rb), to_e4m3x4(widen4<BF16>(b.z, b.w), scale, rb));
+}
+// Element offset in a layer's pool of kv head 0 of row `tok` of the new rows; -1: nowhere.
+__device__ __forceinline__ int64_t row_place(const PageTables& t, const PageWriteArgs& w, int Hkv, int64_t tok) {
   int i = (int)tok, back = 1;  // the token is the back-th last of sequence i
   if (w.starts) {
     int lo = 0, hi = w.n - 1;  // the last sequence that begins at or before the token
@@ -245,75 +296,72 @@ __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool
       if (w.starts[mid] <= tok) lo = mid; else hi = mid - 1;
     }
     i = lo;
-    if (tok < w.starts[i] || tok >= w.starts[i + 1]) return;  // a row of no sequence
+    if (tok < w.starts[i] || tok >= w.starts[i + 1]) return -1;  // a row of no sequence
     back = (int)(w.starts[i + 1] - tok);
   }
   const int slot = w.slots[i];
-  if (slot < 0 || slot >= t.rows) return;
+  if (slot < 0 || slot >= t.rows) return -1;
   const int pos = t.lens[slot] - back;
-  if (pos < 0 || pos / t.page >= t.width) return;
+  if (pos < 0 || pos / t.page >= t.width) return -1;
   const int pg = t.table[(int64_t)slot * t.width + pos / t.page];
-  if (pg < 0 || pg >= t.pages) return;
-  const int64_t at = ((layer * t.pages + pg) * pool.Hkv * t.page + pos % t.page) * 128;
-  const int64_t head_step = (int64_t)t.page * 128;
-  const uint16_t* ks = w.k + tok * w.k_stride;
-  const uint16_t* vs = w.v + tok * w.v_stride;
-  // 16 channels of one head per lane and step
-  for (int x = lane; x < pool.Hkv * 8; x += 32) {
-    const int h = x >> 3, d = (x & 7) * 16;
-    uint4 a[4];
-    a[0] = *reinterpret_cast<const uint4*>(ks + h * 128 + d);
-    a[1] = *reinterpret_cast<const uint4*>(ks + h * 128 + d + 8);
-    a[2] = *reinterpret_cast<const uint4*>(vs + h * 128 + d);
-    a[3] = *reinterpret_cast<const uint4*>(vs + h * 128 + d + 8);
-    const int64_t o = at + h * head_step + d;
-    if constexpr (!FP8) {
+  if (pg < 0 || pg >= t.pages) return -1;
+  return ((int64_t)pg * Hkv * t.page + pos % t.page) * 128;
+}
+// A block writes `per` (1..8) tokens: their places are looked up side by side first, then
+// all their rows are under way together.
+template <bool FP8, bool BF16>
+__global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w,
+                                                    const int32_t* ws, int copy_blocks, int per) {
+  __shared__ int64_t place[8];
+  chain_next();
+  chain_wait();
+  if ((int)blockIdx.x < copy_blocks) {  // rows of other places of the same pages
+    copy_shared_rows(pool, t.pages, t.page, w.n, ws, (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5),
+                     (int64_t)copy_blocks * 8);
+    return;
+  }
+  const int64_t tok0 = (int64_t)(blockIdx.x - copy_blocks) * per;
+  const int some = (int)min((int64_t)per, w.tokens - tok0);
+  if ((int)threadIdx.x < some) place[threadIdx.x] = *t.status == kPagesOk ? row_place(t, w, pool.Hkv, tok0 + threadIdx.x) : -1;
+  __syncthreads();
+  const int64_t base = layer * t.pages * pool.Hkv * t.page * 128, head_step = (int64_t)t.page * 128;
+  // 16 channels of one head per thread and step
+  const int pieces = pool.Hkv * 8;
+#pragma unroll 2
+  for (int u = threadIdx.x; u < some * pieces; u += 256) {
+    const int j = u / pieces, x = u - j * pieces, h = x >> 3, d = (x & 7) * 16;
+    const uint4* ks = reinterpret_cast<const uint4*>(w.k + (tok0 + j) * w.k_stride + h * 128 + d);
+    const uint4* vs = reinterpret_cast<const uint4*>(w.v + (tok0 + j) * w.v_stride + h * 128 + d);
+    const uint4 k0 = __ldg(ks), k1 = __ldg(ks + 1), v0 = __ldg(vs), v1 = __ldg(vs + 1);
+    const int64_t at = place[j], o = base + at + h * head_step + d;
+    if (at < 0) continue;
+    if constexpr (FP8) {
+      *reinterpret_cast<uint4*>(pool.k + o) = to_e4m3x16<BF16>(k0, k1, w.k_scale[h]);
+      *reinterpret_cast<uint4*>(pool.v + o) = to_e4m3x16<BF16>(v0, v1, w.v_scale[h]);
+    } else {
       uint4* kd = reinterpret_cast<uint4*>(pool.k + o * 2);
       uint4* vd = reinterpret_cast<uint4*>(pool.v + o * 2);
-      kd[0] = a[0];
-      kd[1] = a[1];
-      vd[0] = a[2];
-      vd[1] = a[3];
-    } else {
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const float scale = (kv ? w.v_scale : w.k_scale)[h];
-        uint32_t r[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint4& src = a[kv * 2 + (q >> 1)];
-          const uint32_t w0 = q & 1 ? src.z : src.x, w1 = q & 1 ? src.w : src.y;
-          float f[4];
-          if constexpr (BF16) {
-            f[0] = __uint_as_float(w0 << 16);
-            f[1] = __uint_as_float(w0 & 0xffff0000u);
-            f[2] = __uint_as_float(w1 << 16);
-            f[3] = __uint_as_float(w1 & 0xffff0000u);
-          } else {
-            const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&w0));
-            const float2 x1 = __half22float2(*reinterpret_cast<const __half2*>(&w1));
-            f[0] = x0.x;
-            f[1] = x0.y;
-            f[2] = x1.x;
-            f[3] = x1.y;
-          }
-          r[q] = to_e4m3x4(f, scale);
-        }
-        *reinterpret_cast<uint4*>((kv ? pool.v : pool.k) + o) = make_uint4(r[0], r[1], r[2], r[3]);
-      }
+      kd[0] = k0;
+      kd[1] = k1;
+      vd[0] = v0;
+      vd[1] = v1;
     }
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const int32_t* src, const int32_t* dst, int n) {
+__global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const int32_t* src, const int32_t* dst, int n,
+                                                            bool apply) {
   extern __shared__ uint32_t seen[];
+  __shared__ int red[kPlanWarps], ends[kPlanThreads];
   __shared__ int fault;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x;
   if (tid == 0) fault = kPagesOk;
   chain_next();
   chain_wait();
-  if (*t.status != kPagesOk) return;
-  if (!slots_valid(dst, n, t.rows, seen)) {
+  const int status = *t.status;
+  const int mine = tid < n ? dst[tid] : 0;
+  if (status != kPagesOk) return;
+  if (!slots_valid(dst, n, t.rows, seen, mine)) {
     if (tid == 0) *t.status = kPagesBadSlot;
     return;
   }
@@ -329,29 +377,48 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const 
     if (tid == 0) *t.status = fault;
     return;
   }
-  for (int i = warp; i < n; i += kPlanWarps) {
-    const int len = t.lens[src[i]];
-    const int32_t* from = t.table + (int64_t)src[i] * t.width;
-    int32_t* to = t.table + (int64_t)dst[i] * t.width;
-    const int end = min(pages_of(max(len, 0), t.page), t.width);
-    for (int x = lane; x < end; x += 32) {
-      const int pg = from[x];
-      to[x] = pg;
-      if (pg >= 0 && pg < t.pages) atomicAdd(&t.refs[pg], 1);
-    }
-    if (lane == 0) t.lens[dst[i]] = len;
+  if (!apply) return;
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + tid;
+    const int len = i < n ? t.lens[src[i]] : 0;
+    block_expand(
+        min(pages_of(max(len, 0), t.page), t.width), red, ends,
+        [&](int owner, int x) { return t.table[(int64_t)src[base + owner] * t.width + x]; },
+        [&](int owner, int x, int pg) {
+          t.table[(int64_t)dst[base + owner] * t.width + x] = pg;
+          if (pg >= 0 && pg < t.pages) atomicAdd(&t.refs[pg], 1);
+        });
+    if (i < n) t.lens[dst[i]] = len;
   }
+}
+
+// The same without the checks, a block per pair.
+__global__ void __launch_bounds__(128) fork_rows_kernel(PageTables t, const int32_t* src, const int32_t* dst) {
+  chain_next();
+  chain_wait();
+  const int status = *t.status, s = src[blockIdx.x], d = dst[blockIdx.x];
+  if (status != kPagesOk) return;
+  const int len = t.lens[s], end = min(pages_of(max(len, 0), t.page), t.width);
+  for (int x = threadIdx.x; x < end; x += 128) {
+    const int pg = t.table[(int64_t)s * t.width + x];
+    t.table[(int64_t)d * t.width + x] = pg;
+    if (pg >= 0 && pg < t.pages) atomicAdd(&t.refs[pg], 1);
+  }
+  if (threadIdx.x == 0) t.lens[d] = len;
 }
 
 // keep[i] tokens of slots[i] stay (null: none); the pages behind them lose a reference.
 __global__ void __launch_bounds__(kPlanThreads) truncate_kernel(PageTables t, const int32_t* slots, const int32_t* keep,
-                                                                int n) {
+                                                                int n, bool apply) {
   extern __shared__ uint32_t seen[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int red[kPlanWarps], ends[kPlanThreads], from[kPlanThreads];
+  const int tid = threadIdx.x;
   chain_next();
   chain_wait();
-  if (*t.status != kPagesOk) return;
-  if (!slots_valid(slots, n, t.rows, seen)) {
+  const int status = *t.status;
+  const int mine = tid < n ? slots[tid] : 0;
+  if (status != kPagesOk) return;
+  if (!slots_valid(slots, n, t.rows, seen, mine)) {
     if (tid == 0) *t.status = kPagesBadSlot;
     return;
   }
@@ -362,18 +429,41 @@ __global__ void __launch_bounds__(kPlanThreads) truncate_kernel(PageTables t, co
     if (tid == 0) *t.status = kPagesBadCount;
     return;
   }
-  for (int i = warp; i < n; i += kPlanWarps) {
-    const int slot = slots[i], left = keep ? keep[i] : 0;
-    int32_t* row = t.table + (int64_t)slot * t.width;
-    const int end = min(pages_of(t.lens[slot], t.page), t.width);
-    for (int x = pages_of(left, t.page) + lane; x < end; x += 32) {
-      const int pg = row[x];
-      if (pg >= 0 && pg < t.pages) atomicSub(&t.refs[pg], 1);
-      row[x] = -1;
+  if (!apply) return;
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + tid;
+    int left = 0, drop = 0;
+    if (i < n) {
+      left = keep ? keep[i] : 0;
+      from[tid] = pages_of(left, t.page);
+      drop = min(pages_of(max(t.lens[slots[i]], 0), t.page), t.width) - from[tid];
     }
-    __syncwarp();
-    if (lane == 0) t.lens[slot] = left;
+    block_expand(
+        max(drop, 0), red, ends,
+        [&](int owner, int x) { return t.table[(int64_t)slots[base + owner] * t.width + from[owner] + x]; },
+        [&](int owner, int x, int pg) {
+          t.table[(int64_t)slots[base + owner] * t.width + from[owner] + x] = -1;
+          if (pg >= 0 && pg < t.pages) atomicSub(&t.refs[pg], 1);
+        });
+    if (i < n) t.lens[slots[i]] = left;
   }
+}
+
+// The same without the checks, a block per slot.
+__global__ void __launch_bounds__(128) truncate_rows_kernel(PageTables t, const int32_t* slots, const int32_t* keep) {
+  chain_next();
+  chain_wait();
+  const int status = *t.status, slot = slots[blockIdx.x], left = keep ? keep[blockIdx.x] : 0;
+  if (status != kPagesOk) return;
+  const int end = min(pages_of(max(t.lens[slot], 0), t.page), t.width);
+  __syncthreads();
+  for (int x = pages_of(left, t.page) + threadIdx.x; x < end; x += 128) {
+    int32_t* entry = t.table + (int64_t)slot * t.width + x;
+    const int pg = *entry;
+    *entry = -1;
+    if (pg >= 0 && pg < t.pages) atomicSub(&t.refs[pg], 1);
+  }
+  if (threadIdx.x == 0) t.lens[slot] = left;
 }
 
 // workspace of compact: moves, used, then src[pages], dst[pages], to[pages]
@@ -524,15 +614,29 @@ cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t 
     if (copies > kFullGrid / 2) copies = kFullGrid / 2;
   }
   auto kern = p.elem == 2 ? write_kernel<false, true> : w.src_bf16 ? write_kernel<true, true> : write_kernel<true, false>;
-  return launch_chained(kern, copies + (w.tokens + 7) / 8, 256, 0, s, t, p, layer, w, ws, (int)copies);
+  // two blocks for each multiprocessor first, then up to 8 tokens a block
+  int64_t per = w.tokens / (kFullGrid / 4);
+  per = per < 1 ? 1 : per > 8 ? 8 : per;
+  return launch_chained(kern, copies + (w.tokens + per - 1) / per, 256, 0, s, t, p, layer, w, ws, (int)copies, (int)per);
 }
 
+// Above this many table entries that a call may touch, a second launch with a block per
+// sequence changes them: one multiprocessor makes about a scattered reference update per
+// clock.  (128 sequences of 94 pages: XXX us in one launch, XXX us in two; 200 sequences of
+// which 12 lose a page: XXX and XXX us.)
+constexpr int64_t kOneBlockEntries = 16384;
 cudaError_t launch_pages_fork(const PageTables& t, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
-  return launch_chained(fork_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n);
+  const bool one = (int64_t)n * t.width <= kOneBlockEntries;
+  const cudaError_t e = launch_chained(fork_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n, one);
+  if (e != cudaSuccess || one) return e;
+  return launch_chained(fork_rows_kernel, n, 128, 0, s, t, src, dst);
 }
 cudaError_t launch_pages_truncate(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
                                   cudaStream_t s) {
-  return launch_chained(truncate_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n);
+  const bool one = (int64_t)n * t.width <= kOneBlockEntries;
+  const cudaError_t e = launch_chained(truncate_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n, one);
+  if (e != cudaSuccess || one) return e;
+  return launch_chained(truncate_rows_kernel, n, 128, 0, s, t, slots, keep);
 }
 cudaError_t launch_pages_compact(const PageTables& t, const PagePools& p, int32_t* ws, cudaStream_t s) {
   cudaError_t e = launch_chained(compact_plan_kernel, 1, kPlanThreads, 0, s, t, ws);
