@@ -424,19 +424,23 @@ typedef struct h3b_page_cache {
 /* Window attention over contiguous K/V.  q, out: rows [Tq, Hq * 128] with their strides;
  * k, v: rows [Tk, Hkv * 128].  query_starts / key_starts: device int32 [seqs + 1], the
  * first row of each sequence (ascending from 0 to Tq / Tk), both or neither (one
- * sequence).  Query rows outside every sequence are not written. */
+ * sequence).  Query rows outside every sequence are not written.
+ * workspace: NULL, or h3b_window_workspace_bytes() bytes, 16-byte aligned and not shared
+ * by calls on different streams, with which long rows of keys are divided over the
+ * multiprocessors (the results differ in the last bits of the fp32 sums). */
+int64_t h3b_window_workspace_bytes(void);
 int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                          int64_t v_row_stride, int dtype, int64_t Tq, int64_t Tk, const int32_t* query_starts,
                          const int32_t* key_starts, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t window,
                          int64_t sinks, int64_t chunk, float sm_scale, void* out, int64_t out_row_stride,
-                         void* stream);
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The same over one layer of a 16-bit paged cache of the queries' type: sequence i is
  * table row slots[i] (NULL: row i), its queries the last tokens that the row holds. */
 int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, int64_t Tq, const int32_t* query_starts,
                                const int32_t* slots, int64_t seqs, int64_t Hq, const h3b_page_cache* cache,
                                int64_t layer, int64_t window, int64_t sinks, int64_t chunk, float sm_scale, void* out,
-                               int64_t out_row_stride, void* stream);
+                               int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Attention of one new token per sequence, the last of table row slots[i] (NULL: row i),
  * over a 16-bit cache of the queries' type or an e4m3 cache.  q, out: rows [seqs,

@@ -109,6 +109,65 @@ def test_window_more_work_than_multiprocessors(heads, rule):
         a, b = a + lq, b + lk
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", [([200], 9000, 4, 2, None, 0, 1), ([5], 20000, 3, 1, None, 0, 1), ([1], 30011, 2, 2, 29000, 70, 1),
+                                  ([300, 1, 40], 7000, 6, 2, 5000, 300, 1), ([260], 6000, 5, 5, None, 100, 260),
+                                  ([1500], 0, 1, 1, None, 0, 1), ([2500], 0, 3, 3, 2000, 128, 1)],
+                         ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
+def test_window_few_rows_over_many_keys(case, dtype):
+    """Items cut along their keys and joined; twice the same bits."""
+    from h3b import window_attention
+
+    lens, past, hq, hkv, window, sinks, chunk = case
+    g = _gen(lens[0])
+    keys = [n + past for n in lens]
+    q = _rand(g, sum(lens), hq, D, dtype=dtype, scale=2.0)
+    k, v = (_rand(g, sum(keys), hkv, D, dtype=dtype) for _ in range(2))
+    kw = dict(window=window, sinks=sinks, chunk=chunk, query_starts=_starts(lens), key_starts=_starts(keys))
+    out = window_attention(q, k, v, **kw)
+    a = b = 0
+    for lq, lk in zip(lens, keys):
+        ref, spread = attend(q[a:a + lq], k[b:b + lk], v[b:b + lk], visible(lq, lk, window, sinks, chunk, "cuda"))
+        assert_close(out[a:a + lq], ref, spread, lk, 6.0, f"sequence at {a}")
+        a, b = a + lq, b + lk
+    assert torch.equal(window_attention(q, k, v, **kw), out)
+
+
+def test_window_cut_items_keep_unseen_rows_apart():
+    """Non-finite V and K rows inside and outside what the rows of cut items see."""
+    from h3b import window_attention
+
+    g = _gen(12)
+    n, past = 130, 8000
+    q = _rand(g, n, 2, D, dtype=torch.bfloat16)
+    k, v = (_rand(g, n + past, 1, D, dtype=torch.bfloat16) for _ in range(2))
+    kw = dict(window=7000, sinks=5)
+    see = visible(n, n + past, 7000, 5, 1, "cuda")
+    clean = window_attention(q, k, v, **kw)
+    for j in (6, 500, past + n - 7000 - 20, past + n - 7000 + 3, past + 10, past + 129):
+        dirty_k, dirty_v = k.clone(), v.clone()
+        dirty_v[j, 0, 3] = math.inf
+        got = window_attention(q, dirty_k, dirty_v, **kw)
+        hit = see[:, j]
+        assert torch.equal(got[~hit], clean[~hit]) and not torch.isfinite(got[hit][..., 3].float()).any()
+        keep = [c for c in range(D) if c != 3]
+        assert torch.equal(got[..., keep], clean[..., keep])
+        dirty_k[j] = math.nan
+        got = window_attention(q, dirty_k, v, **kw)
+        assert torch.equal(got[~hit], clean[~hit]) and torch.isnan(got[hit].float()).all()
+
+
+def test_window_overlapping_starts_stay_in_bounds():
+    """Starts that run backwards: rows may be anything, memory is not left."""
+    from h3b import window_attention
+
+    g = _gen(13)
+    q = _rand(g, 400, 2, D, dtype=torch.bfloat16)
+    k, v = (_rand(g, 400, 2, D, dtype=torch.bfloat16) for _ in range(2))
+    window_attention(q, k, v, query_starts=_i32([0, 400, 0, 400, -7, 900, 3]), key_starts=_i32([0, 400, 0, 400, -9, 4000, 1]))
+    torch.cuda.synchronize()
+
+
 def test_window_rows_that_see_nothing_give_zero():
     """More queries than keys, a window of nothing, and sequences without keys."""
     from h3b import window_attention

@@ -23,9 +23,9 @@ ODD = ctypes.c_void_p(24)
 
 
 def _window(q=D, qs=512, k=D, ks=256, v=D, vs=256, dtype=2, tq=8, tk=8, sq=None, sk=None, seqs=1, hq=4, hkv=2,
-            window=4, sinks=0, chunk=1, out=D, os=512):
+            window=4, sinks=0, chunk=1, out=D, os=512, ws=None, wsb=0):
     return lib().h3b_window_attention(q, qs, k, ks, v, vs, dtype, tq, tk, sq, sk, seqs, hq, hkv, window, sinks, chunk,
-                                      0.1, out, os, None)
+                                      0.1, out, os, ws, wsb, None)
 
 
 @pytest.mark.parametrize("status,kw", [
@@ -33,7 +33,7 @@ def _window(q=D, qs=512, k=D, ks=256, v=D, vs=256, dtype=2, tq=8, tk=8, sq=None,
     (-2, dict(dtype=3)), (-1, dict(window=-1)), (-1, dict(sinks=-1)), (-1, dict(chunk=0)), (-1, dict(qs=504)),
     (-1, dict(qs=516)), (-1, dict(os=128)), (-1, dict(ks=128)), (-1, dict(vs=260)), (-2, dict(q=ODD)), (-2, dict(v=ODD)),
     (-2, dict(tq=1 << 31)), (-1, dict(tk=-1)), (-1, dict(tq=-1)), (-1, dict(seqs=2)), (-1, dict(sq=D)), (-1, dict(seqs=0)),
-    (0, dict(tq=0, q=None)),
+    (-1, dict(ws=D, wsb=100)), (-2, dict(ws=ODD, wsb=1 << 40)), (0, dict(tq=0, q=None)),
 ])
 def test_window_entry_refuses(status, kw):
     assert _window(**kw) == status
@@ -41,7 +41,7 @@ def test_window_entry_refuses(status, kw):
 
 def _paged(q=D, dtype=2, tq=8, starts=None, seqs=1, hq=4, cache=None, layer=0):
     return lib().h3b_paged_window_attention(q, 512, dtype, tq, starts, None, seqs, hq, cache or _cache(), layer, 4, 0, 1,
-                                            0.1, D, 512, None)
+                                            0.1, D, 512, None, 0, None)
 
 
 @pytest.mark.parametrize("status,kw", [

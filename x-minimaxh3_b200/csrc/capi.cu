@@ -617,11 +617,13 @@ int window_status(int r, cudaError_t e, const char* what) {
 
 }  // namespace
 
+int64_t h3b_window_workspace_bytes(void) { return h3b::window_workspace_bytes(); }
+
 int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                          int64_t v_row_stride, int dtype, int64_t Tq, int64_t Tk, const int32_t* query_starts,
                          const int32_t* key_starts, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t window,
                          int64_t sinks, int64_t chunk, float sm_scale, void* out, int64_t out_row_stride,
-                         void* stream) {
+                         void* workspace, int64_t workspace_bytes, void* stream) {
   if (Tq == 0) return ok();
   int r = check_rows(q, q_row_stride, dtype, Tq, Hq, Hkv, window, sinks, chunk, sm_scale, out, out_row_stride, "window_attention");
   if (r) return r;
@@ -632,6 +634,9 @@ int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int
   if (Tk > 0 && (k_row_stride < Hkv * 128 || k_row_stride % 8 || v_row_stride < Hkv * 128 || v_row_stride % 8))
     return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: bad K/V row stride");
   if (!aligned16(k) || !aligned16(v)) return fail(H3B_ERR_UNSUPPORTED, "window_attention: K and V must be 16-byte aligned");
+  if (workspace && workspace_bytes < h3b::window_workspace_bytes())
+    return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: workspace too small");
+  if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "window_attention: workspace must be 16-byte aligned");
   h3b::WindowArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_row_stride;
@@ -651,14 +656,14 @@ int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int
   a.out = static_cast<uint16_t*>(out);
   a.out_stride = out_row_stride;
   cudaError_t e = cudaSuccess;
-  r = h3b::launch_window_attention(a, dtype == 2, st(stream), &e);
+  r = h3b::launch_window_attention(a, dtype == 2, workspace, st(stream), &e);
   return window_status(r, e, "window_attention");
 }
 
 int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, int64_t Tq, const int32_t* query_starts,
                                const int32_t* slots, int64_t seqs, int64_t Hq, const h3b_page_cache* cache,
                                int64_t layer, int64_t window, int64_t sinks, int64_t chunk, float sm_scale, void* out,
-                               int64_t out_row_stride, void* stream) {
+                               int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream) {
   if (Tq == 0) return ok();
   int r = check_cache(cache, layer, "paged_window_attention");
   if (r) return r;
@@ -670,6 +675,9 @@ int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, i
   if (seqs < 1 || seqs > (1 << 24)) return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: bad sizes");
   if (!query_starts && seqs != 1)
     return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: several sequences need query_starts");
+  if (workspace && workspace_bytes < h3b::window_workspace_bytes())
+    return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: workspace too small");
+  if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "paged_window_attention: workspace must be 16-byte aligned");
   h3b::WindowArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_row_stride;
@@ -684,7 +692,7 @@ int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, i
   a.out_stride = out_row_stride;
   a.paged = paged_args(cache, layer, slots);
   cudaError_t e = cudaSuccess;
-  r = h3b::launch_window_attention(a, dtype == 2, st(stream), &e);
+  r = h3b::launch_window_attention(a, dtype == 2, workspace, st(stream), &e);
   return window_status(r, e, "paged_window_attention");
 }
 

@@ -105,9 +105,14 @@ struct WindowArgs {
   uint16_t* out;
   int64_t out_stride;
   PagedArgs paged;  // paged.k set: keys come from the pages, k / v / k_starts unused
+  void* notes;      // of cut items and their pieces (set by the launcher; null: none is cut)
+  float* pieces;
 };
-// bf16: bfloat16, else float16.  0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err)
-int launch_window_attention(const WindowArgs& a, bool bf16, cudaStream_t s, cudaError_t* err);
+// bf16: bfloat16, else float16.  workspace: null, or window_workspace_bytes() with which
+// long items are cut.  0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err), 3 the
+// kernel's register count is not the planned one, 4 too many tiles
+int64_t window_workspace_bytes();
+int launch_window_attention(WindowArgs a, bool bf16, void* workspace, cudaStream_t s, cudaError_t* err);
 
 struct DecodeArgs {
   const uint16_t* q;

@@ -3,8 +3,8 @@
 //
 //   out_i = sum_j softmax_j(scale * q_i . k_j) v_j  over the keys j that query i sees
 //
-// A persistent CTA per SM works through items of two 128-row query tiles A and B that
-// read the same keys: two heads of one kv head at the same rows (even groups), else two
+// A persistent CTA per SM works through its share of the items, two 128-row query tiles
+// A and B that read the same keys: two heads of one kv head at the same rows (even groups), else two
 // consecutive row tiles of one head.  An item visits the 128-key tiles that any of its rows sees -- those of the first tokens,
 // then those of the window -- in one pass with the running maximum and sum:
 //   S = Q . K^T     tcgen05 kind::f16, fp32 in tensor memory
@@ -131,7 +131,9 @@ struct WinPlan {
   StepRanges tile[2];
   int row[2], rows[2];  // first row (of q) and valid rows of each tile
   int p0[2];            // position of the tile's first row
-  int sn, w0, steps;    // key tiles of the steps: [0, sn), then w0 and on; steps < 0: no more work
+  int sn, w0, steps;    // key tiles of the steps: [0, sn), then w0 and on
+  int from, to;         // the steps of this piece; from == to: no key to see; to < 0: no more work
+  int part;             // -1, or where the sums of a piece of an item go
   int lk, k_row, slot;  // keys of the sequence, its first K row or its table row
   int head0, kh;        // head of tile A, kv head
   __device__ int key_tile(int i) const { return i < sn ? i : w0 + (i - sn); }
@@ -158,18 +160,16 @@ __device__ __forceinline__ uint32_t key_bits(int base, int a, int b) {
   return below_y & ~below_x;
 }
 
-// 32 scores -> P, and their sum.  x = s c - m; one column pair in four takes the
-// polynomial on the FMA pipe, the others ex2.approx.  In masked tiles all take ex2, whose
-// exp2(-inf) is 0 (the polynomial ends at 2^-125, which would give a row that sees
-// nothing a sum).
-template <bool MASK>
+// 32 scores -> P = 2^(s c - m), and their sum.  All through ex2.approx: under the power
+// cap a polynomial on the FMA pipe for a share of them only adds instructions (8,192 x 32
+// heads, window 4,096: none 485 us, one in eight 494, one in four 492, one in two 533).
 __device__ __forceinline__ void win_exp32(uint32_t* s, float2 c2, float2 o2, float2& acc0, float2& acc1) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
     const float2 x0 = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, o2);
     const float2 x1 = __ffma2_rn(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), c2, o2);
     const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y));
-    const float2 p1 = !MASK && (c & 4) ? exp2_poly2(x1) : make_float2(ex2(x1.x), ex2(x1.y));
+    const float2 p1 = make_float2(ex2(x1.x), ex2(x1.y));
     acc0 = __fadd2_rn(acc0, p0);
     acc1 = __fadd2_rn(acc1, p1);
     s[c] = __float_as_uint(p0.x);
@@ -248,8 +248,8 @@ __device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, fl
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    win_exp32<MASK>(&s[h * 64], c2, o2, acc0, acc1);
-    win_exp32<MASK>(&s[h * 64 + 32], c2, o2, acc0, acc1);
+    win_exp32(&s[h * 64], c2, o2, acc0, acc1);
+    win_exp32(&s[h * 64 + 32], c2, o2, acc0, acc1);
     if (h == 1) {
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(other_turn);
@@ -282,14 +282,14 @@ __device__ __forceinline__ const uint16_t* value_row(const WindowArgs& a, const 
     return a.v + (int64_t)(pl.k_row + j) * a.v_stride + pl.kh * 128;
 }
 
-// Adds to an output row the infinities and NaN of the V rows that it sees and that were
-// cleared from the masked tiles.  Only when there is such a row.
+// Adds to an output row (or a piece's sums) the infinities and NaN of the V rows that it
+// sees and that were cleared from the masked tiles.  Only when there is such a row.
 template <bool BF16, bool PAGED>
 __device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& pl, const VisibleKeys& see,
-                                           uint16_t* dst) {
-  for (int i = 0; i < pl.steps; ++i) {
-    const int n = pl.key_tile(i);
+                                           uint16_t* dst, float* sums) {
+  for (int i = pl.from; i < pl.to; ++i) {
     if (!pl.masked(i)) continue;
+    const int n = pl.key_tile(i);
     for (int j = n * 128; j < min(n * 128 + 128, see.end); ++j) {
       if (j < see.lo && j >= see.sinks) continue;
       const uint32_t* v = reinterpret_cast<const uint32_t*>(value_row<PAGED>(a, pl, j));
@@ -298,30 +298,56 @@ __device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& p
         if (!(bad & 0x80008000u)) continue;
         for (int hi = 0; hi < 2; ++hi) {
           if (!((bad >> (hi ? 31 : 15)) & 1u)) continue;
-          uint16_t* o = dst + 2 * e + hi;
-          const float sum = unpack_half<BF16>(*o, 0) + unpack_half<BF16>(w, hi);
-          *o = (uint16_t)pack2<BF16>(sum, sum);
+          const int d = 2 * e + hi;
+          const float x = unpack_half<BF16>(w, hi);
+          if (sums) {
+            sums[d] += x;
+          } else {
+            const float sum = unpack_half<BF16>(dst[d], 0) + x;
+            dst[d] = (uint16_t)pack2<BF16>(sum, sum);
+          }
         }
       }
     }
   }
 }
 
-// Work item `item` for the whole warp: items number the heads of a tile first, tiles run
-// through the sequences from the last (with a causal mask the late tiles see most keys,
-// and go first).  Items beyond the last tile have steps -1.
-template <bool PAGED>
-__device__ void plan_item(const WindowArgs& a, int item, int items, int rows_per_cta, WinPlan* out) {
+// ---- the division of the work
+//
+// Items (a tile pair's rows and columns: head or head pair) are numbered tile by tile from
+// the last (with a causal mask the late tiles see most keys), columns first; an item is
+// worth its steps and kItemCost more.  Item c + r * CTAs goes to CTA c whole for the first
+// rounds r, so that CTAs that read the same keys read them at the same time, as long as no
+// CTA gets more than its equal share of all; what is left is dealt out along one list, to
+// each CTA what it lacks.  A boundary that falls into an item there cuts it, unless the
+// item is short (kCutFrom) or the piece would be (kLeastPiece): then it moves to the
+// item's nearer end.  The pieces of a cut item leave their sums, and window_join_kernel
+// puts them together.
+constexpr int kItemCost = 2;
+constexpr int kCutFrom = 9;
+constexpr int kLeastPiece = 3;
+constexpr int kPieceFloats = 2 * 128 * 130;  // O [2][128][128], then (m, l) [2][128]
+constexpr int kMaxTiles = kWinSlots * kWinTile / 12 - 16;  // prefix sums of tiles and sequences that fit the ring
+
+struct PieceNote {  // [CTA][2]: slot 1 a piece with the item's first step, slot 0 any other
+  int state;        // 0: none, 1: more pieces follow, 2: the last
+  int row[2], rows[2], head0, pad[2];
+};
+__host__ __device__ inline int64_t window_notes_bytes(int ctas) { return (int64_t)ctas * 2 * sizeof(PieceNote); }
+
+__device__ __forceinline__ int tiles_of(const WindowArgs& a, int seq, int rows_per_cta) {
+  const RowRange r = row_range(a.q_starts, seq, a.Tq);
+  return (r.b - r.a + rows_per_cta - 1) / rows_per_cta;
+}
+// A tile's sequence (-1: past the last tile) and its number in it.
+struct TileAt {
+  int seq, t;
+};
+// Tile t of all, found by the whole warp.
+__device__ TileAt find_tile(const WindowArgs& a, int t, int rows_per_cta) {
   const int lane = threadIdx.x & 31;
-  const bool by_heads = rows_per_cta == 128;  // tiles A, B: two heads of a group; else two row tiles
-  const int columns = by_heads ? a.Hq / 2 : a.Hq;
-  int t = (items - 1 - item) / columns, seq = -1;
   for (int base = 0; base < a.seqs; base += 32) {
-    int n = 0;
-    if (base + lane < a.seqs) {
-      const RowRange r = row_range(a.q_starts, base + lane, a.Tq);
-      n = (r.b - r.a + rows_per_cta - 1) / rows_per_cta;
-    }
+    const int n = base + lane < a.seqs ? tiles_of(a, base + lane, rows_per_cta) : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -331,56 +357,64 @@ __device__ void plan_item(const WindowArgs& a, int item, int items, int rows_per
     const unsigned hit = __ballot_sync(0xffffffffu, t < x);
     if (hit) {
       const int w = __ffs(hit) - 1;
-      seq = base + w;
-      t -= __shfl_sync(0xffffffffu, x - n, w);
-      break;
+      return {base + w, t - __shfl_sync(0xffffffffu, x - n, w)};
     }
     t -= __shfl_sync(0xffffffffu, x, 31);
   }
-  if (lane == 0) {
-    WinPlan p{};  // no sequence: nothing to visit, no row to write
-    if (seq >= 0) {
-      const RowRange qr = row_range(a.q_starts, seq, a.Tq);
-      if constexpr (PAGED) {
-        p.slot = paged_slot(a.paged, seq);
-        p.lk = paged_len(a.paged, p.slot);
-        p.k_row = 0;
-      } else {
-        const RowRange kr = row_range(a.k_starts, seq, a.Tk);
-        p.slot = 0;
-        p.lk = kr.b - kr.a;
-        p.k_row = kr.a;
-      }
-      p.head0 = (item % columns) * (by_heads ? 2 : 1);
-      p.kh = p.head0 / (a.Hq / a.Hkv);
-      const int lq = qr.b - qr.a;
-      TileKeys keys[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int first = t * rows_per_cta + (by_heads ? 0 : x * 128);
-        p.row[x] = qr.a + first;
-        p.rows[x] = max(0, min(128, lq - first));
-        p.p0[x] = p.lk - lq + first;
-        keys[x] = p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
-      }
-      p.sn = max(keys[0].sn, keys[1].sn);
-      int w0 = 1 << 30, w1 = 0;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (keys[x].w1 > keys[x].w0) {
-          w0 = min(w0, keys[x].w0);
-          w1 = max(w1, keys[x].w1);
-        }
-      }
-      p.w0 = max(w0, p.sn);
-      p.steps = p.sn + max(0, w1 - p.w0);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) p.tile[x] = step_ranges(keys[x], p.sn, p.w0);
-    }
-    *out = p;
-  }
-  __syncwarp();
+  return {-1, 0};
 }
+
+// Everything about a tile's item but its column: rows, key tiles, steps.
+template <bool PAGED>
+__device__ __forceinline__ void plan_tile(const WindowArgs& a, int seq, int t, int rows_per_cta, WinPlan& p) {
+  const bool by_heads = rows_per_cta == 128;  // tiles A, B: two heads of a group; else two row tiles
+  const RowRange qr = row_range(a.q_starts, seq, a.Tq);
+  if constexpr (PAGED) {
+    p.slot = paged_slot(a.paged, seq);
+    p.lk = paged_len(a.paged, p.slot);
+    p.k_row = 0;
+  } else {
+    const RowRange kr = row_range(a.k_starts, seq, a.Tk);
+    p.slot = 0;
+    p.lk = kr.b - kr.a;
+    p.k_row = kr.a;
+  }
+  const int lq = qr.b - qr.a;
+  TileKeys keys[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int first = t * rows_per_cta + (by_heads ? 0 : x * 128);
+    p.row[x] = qr.a + first;
+    p.rows[x] = max(0, min(128, lq - first));
+    p.p0[x] = p.lk - lq + first;
+    keys[x] = p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
+  }
+  p.sn = max(keys[0].sn, keys[1].sn);
+  int w0 = 1 << 30, w1 = 0;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (keys[x].w1 > keys[x].w0) {
+      w0 = min(w0, keys[x].w0);
+      w1 = max(w1, keys[x].w1);
+    }
+  }
+  p.w0 = max(w0, p.sn);
+  p.steps = p.sn + max(0, w1 - p.w0);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) p.tile[x] = step_ranges(keys[x], p.sn, p.w0);
+}
+
+// A place in the list that is dealt out: an item and a step of it.
+struct WorkAt {
+  int item, step;
+};
+// What a CTA does: `rounds` whole items, then from bounds[0] to bounds[1].
+constexpr int kListed = 60;
+struct WorkShare {
+  int valid, rounds;
+  WorkAt bounds[2];
+  TileAt tile[kListed];  // of the rounds' items, then of the dealt-out tiles in order
+};
 
 // A counter through the phases of a ring of N barriers: slot and parity of its next use.
 template <int N>
@@ -425,7 +459,7 @@ template <bool BF16, bool PAGED>
 __global__ void __launch_bounds__(kWinThreads, 1)
     window_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WindowArgs a, int rows_per_cta,
-                  int items) {
+                  int tiles) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWinOffBar);
@@ -447,6 +481,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* cleared = abort_flag + 1;  // [2]: some seen V row of the item was cleared
   __shared__ WinPlan plans[2];
+  __shared__ long long scan[kWinThreads / 32];
+  __shared__ WorkShare work;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool by_heads = rows_per_cta == 128;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -459,9 +495,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
     }
-    chain_next();
-    chain_wait();
-    plan_item<PAGED>(a, blockIdx.x, items, rows_per_cta, &plans[0]);
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -488,7 +521,122 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     cleared[0] = cleared[1] = 0;
     fence_mbar_init();
   }
-  if (warp != 0) chain_wait();
+  chain_next();
+  chain_wait();
+  const int columns = by_heads ? a.Hq / 2 : a.Hq;
+  {
+    // Costs of all tiles, as prefix sums in the ring's memory.  More than kMaxTiles do not
+    // fit: then all items are dealt whole, in rounds.
+    const bool fits = tiles <= kMaxTiles;
+    long long* upto = reinterpret_cast<long long*>(smem + kWinOffRing);  // [tiles] from the last tile, per column
+    int* seq_upto = reinterpret_cast<int*>(upto + (fits ? tiles : 0));   // [seqs]: tiles of 0..i
+    // inclusive prefix sums of n values over the block: value(i) -> put(i, sum)
+    auto prefix = [&](int n, auto value, auto put) {
+      const int per = (n + kWinThreads - 1) / kWinThreads, first = (int)threadIdx.x * per;
+      long long sum = 0;
+      for (int i = first; i < min(first + per, n); ++i) sum += value(i);
+      long long incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      long long run = incl - sum;
+      for (int w = 0; w < warp; ++w) run += scan[w];
+      for (int i = first; i < min(first + per, n); ++i) put(i, run += value(i));
+      __syncthreads();
+    };
+    const int ctas = (int)gridDim.x, me = (int)blockIdx.x;
+    if (!fits) {
+      if (threadIdx.x == 0) {
+        const int items = tiles * columns;
+        work.valid = tiles;
+        work.rounds = me < items ? (items - me + ctas - 1) / ctas : 0;
+        work.bounds[0] = work.bounds[1] = {items, 0};
+      }
+    } else {
+      prefix(a.seqs, [&](int i) { return (long long)tiles_of(a, i, rows_per_cta); },
+             [&](int i, long long x) { seq_upto[i] = (int)x; });
+      const int valid = min(seq_upto[a.seqs - 1], tiles);  // more only where the starts overlap
+      auto locate = [&](int tile) {
+        int lo = 0, hi = a.seqs - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (seq_upto[mid] > tile) hi = mid; else lo = mid + 1;
+        }
+        return TileAt{lo, tile - (lo ? seq_upto[lo - 1] : 0)};
+      };
+      for (int q = (int)threadIdx.x; q < valid; q += kWinThreads) {
+        const TileAt at = locate(valid - 1 - q);
+        WinPlan p;
+        plan_tile<PAGED>(a, at.seq, at.t, rows_per_cta, p);
+        upto[q] = p.steps + kItemCost;
+      }
+      __syncthreads();
+      prefix(valid, [&](int i) { return upto[i]; }, [&](int i, long long x) { upto[i] = x; });
+      const int items = valid * columns;
+      const long long all = valid ? upto[valid - 1] * columns : 0, share = (all + ctas - 1) / ctas;
+      auto cost = [&](int item) {
+        const int q = item / columns;
+        return upto[q] - (q ? upto[q - 1] : 0);
+      };
+      // whole rounds; a thread per CTA (the launch has at most kWinThreads)
+      int rounds = 0;
+      long long load = 0;
+      for (;; ++rounds) {
+        const int first = rounds * ctas;
+        const long long next = (int)threadIdx.x < ctas && first + ctas <= items ? load + cost(first + (int)threadIdx.x) : 0;
+        if (!__syncthreads_and(first + ctas <= items && next <= share)) break;
+        load = next;
+      }
+      const int dealt = rounds * ctas;  // first item of the list
+      const int q0 = dealt / columns;
+      const long long begin = dealt >= items ? all : (q0 ? upto[q0 - 1] : 0) * columns + (dealt - q0 * columns) * cost(dealt);
+      // what the CTAs before this one lack, and this one
+      auto place = [&](long long at, int which) {
+        WorkAt w{items, 0};
+        at += begin;
+        if (at < all) {
+          int lo = 0, hi = valid - 1;  // the first tile that ends beyond `at`
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (upto[mid] * columns > at) hi = mid; else lo = mid + 1;
+          }
+          const long long first = lo ? upto[lo - 1] : 0;
+          const int worth = (int)(upto[lo] - first), steps = worth - kItemCost;
+          const long long in = at - first * columns;
+          w.item = lo * columns + (int)(in / worth);
+          w.step = max((int)(in % worth) - kItemCost, 0);
+          const bool whole = !a.notes || steps < kCutFrom;  // the item may not be cut
+          if (w.step > 0 && (whole ? 2 * w.step >= steps : steps - w.step < kLeastPiece)) {
+            w.step = 0;
+            ++w.item;
+          } else if (whole || w.step < kLeastPiece) {
+            w.step = 0;
+          }
+        }
+        work.bounds[which] = w;
+      };
+      prefix(ctas, [&](int i) { return share - load; },  // thread i holds load i
+             [&](int i, long long x) {
+               if (i == me) place(x, 1);
+               if (i == me - 1) place(x, 0);
+               if (me == 0 && i == 0) place(0, 0);
+             });
+      const int sk = work.bounds[0].item / columns;
+      for (int e = (int)threadIdx.x; e < kListed; e += kWinThreads) {
+        const int q = e < rounds ? (me + e * ctas) / columns : sk + e - rounds;
+        work.tile[e] = q < valid ? locate(valid - 1 - q) : TileAt{-1, 0};
+      }
+      if (threadIdx.x == 0) {
+        work.valid = valid;
+        work.rounds = rounds;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring's loads come next
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -501,22 +649,57 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     const int box = PAGED ? a.paged.page : 128;
     bool ok = true;
     uint32_t q_parity = 1;
-    int k = 0;
-    for (int item = blockIdx.x;; item += gridDim.x, ++k) {
+    WorkAt w = work.bounds[0];
+    const WorkAt stop = work.bounds[1];
+    const int rounds = work.rounds, dealt_tile = w.item / columns;
+    PieceNote* notes = reinterpret_cast<PieceNote*>(a.notes) + 2 * blockIdx.x;
+    if (a.notes && lane < 2) notes[lane].state = 0;
+    __syncwarp();
+    for (int k = 0;; ++k) {
       WinPlan* pl = &plans[k & 1];
-      if (k > 0) {
-        if (!wait(&plan_free[k & 1], (uint32_t)((k >> 1) & 1) ^ 1u)) break;
-        if (item < items)
-          plan_item<PAGED>(a, item, items, rows_per_cta, pl);
-        else if (lane == 0)
-          pl->steps = -1;
-        if (lane == 0) cleared[k & 1] = 0;
-        __syncwarp();
+      if (k > 1 && !wait(&plan_free[k & 1], (uint32_t)((k >> 1) & 1) ^ 1u)) break;
+      const bool round = k < rounds;
+      if (round || w.item < stop.item || (w.item == stop.item && w.step < stop.step)) {
+        const int item = round ? (int)blockIdx.x + k * (int)gridDim.x : w.item, q = item / columns;
+        const int entry = round ? k : rounds + q - dealt_tile;
+        TileAt at;
+        if (entry < kListed && tiles <= kMaxTiles)
+          at = work.tile[entry];
+        else
+          at = find_tile(a, work.valid - 1 - q, rows_per_cta);
+        if (lane == 0) {
+          WinPlan p{};  // past the last tile: nothing to visit, no row to write
+          p.part = -1;
+          if (at.seq >= 0) plan_tile<PAGED>(a, at.seq, at.t, rows_per_cta, p);
+          p.head0 = (item - q * columns) * (by_heads ? 2 : 1);
+          p.kh = p.head0 / (a.Hq / a.Hkv);
+          p.from = round ? 0 : w.step;
+          p.to = !round && item == stop.item ? stop.step : p.steps;
+          if (p.from > 0 || p.to < p.steps) {
+            const int slot = p.from == 0 ? 1 : 0;
+            p.part = 2 * blockIdx.x + slot;
+            PieceNote n;
+            n.state = p.to == p.steps ? 2 : 1;
+            for (int x = 0; x < 2; ++x) {
+              n.row[x] = p.row[x];
+              n.rows[x] = p.rows[x];
+            }
+            n.head0 = p.head0;
+            n.pad[0] = n.pad[1] = 0;
+            notes[slot] = n;
+          }
+          *pl = p;
+          cleared[k & 1] = 0;
+        }
+        if (!round) w = {w.item + 1, 0};
+      } else if (lane == 0) {
+        pl->to = -1;
       }
-      const int steps = pl->steps, sn = pl->sn, w0 = pl->w0, kh = pl->kh;
+      __syncwarp();
+      const int from = pl->from, to = pl->to, sn = pl->sn, w0 = pl->w0, kh = pl->kh;
       if (lane == 0) mbar_arrive(&plan_full[k & 1]);
-      if (steps < 0) break;
-      if (steps == 0) continue;
+      if (to < 0) break;
+      if (from == to) continue;
       if (!(ok = wait(q_empty, q_parity))) break;
       q_parity ^= 1u;
       if (lane == 0) mbar_arrive_expect_tx(q_full, 2 * kWinTile);
@@ -525,7 +708,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         tma_load_3d(smem + lane * (kWinTile / 2), &tmQ, q_full, (lane & 1) * 64,
                     by_heads ? pl->head0 + (lane >> 1) : pl->head0, pl->row[lane >> 1]);
       __syncwarp();
-      for (int i = 0; i < 2 * steps; ++i, at.next()) {
+      for (int i = 2 * from; i < 2 * to; ++i, at.next()) {
         if (!(ok = wait(&empty[at.slot], at.parity ^ 1u))) break;
         const int n = i >> 1, j0 = (n < sn ? n : w0 + (n - sn)) * 128;
         const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
@@ -560,9 +743,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     for (int k = 0; ok; ++k) {
       const WinPlan& pl = plans[k & 1];
       if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
-      const int steps = pl.steps;
-      if (steps < 0) break;
-      for (int i = 0; i < steps; ++i) {
+      const int to = pl.to;
+      if (to < 0) break;
+      for (int i = pl.from; i < to; ++i) {
         at.next();
         if (!(ok = wait(&full[at.slot], at.parity))) break;
         if (pl.masked(i)) {
@@ -624,17 +807,20 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     bool ok = true;
     for (int k = 0; ok; ++k) {
       if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
-      const int steps = plans[k & 1].steps;
-      if (steps < 0) break;
+      const int from = plans[k & 1].from, to = plans[k & 1].to;
+      if (to < 0) break;
       const StepRanges r = plans[k & 1].tile[x];
-      const int last = r.to > r.from ? r.to - 1 : r.head - 1;  // last step taken (-1: none)
-      if (steps > 0) {
+      // last step taken (-1: none)
+      int last = min(r.to, to) - 1;
+      if (last < max(r.from, from)) last = min(r.head, to) - 1;
+      if (last < from) last = -1;
+      if (to > from) {
         if (!(ok = wait(q_full, q_parity))) break;
         q_parity ^= 1u;
         if (last < 0 && lane == 0) mbar_arrive(q_empty);
       }
       bool first = true, issued = false;
-      for (int i = 0; i < steps; ++i) {
+      for (int i = from; i < to; ++i) {
         const RingAt<kWinSlots> kt = at;
         at.next();
         const RingAt<kWinSlots> vt = at;
@@ -722,13 +908,13 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     for (int k = 0; ok; ++k) {
       const WinPlan& pl = plans[k & 1];
       if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
-      const int steps = pl.steps;
-      if (steps < 0) break;
+      const int to = pl.to;
+      if (to < 0) break;
       const StepRanges r = pl.tile[x];
-      const VisibleKeys see = visible_keys(a.rule, pl.p0[x] + quad * 32 + lane, steps > 0 ? pl.lk : 0);
+      const VisibleKeys see = visible_keys(a.rule, pl.p0[x] + quad * 32 + lane, to > pl.from ? pl.lk : 0);
       float m = -__int_as_float(0x7f800000), l = 0.f;
       int cnt = 0;
-      for (int i = 0; i < steps; ++i, turn_parity ^= 1u) {
+      for (int i = pl.from; i < to; ++i, turn_parity ^= 1u) {
         if (!r.takes(i)) {
           if (!(ok = wait(turn, turn_parity))) break;
           if (lane == 0) mbar_arrive(other_turn);
@@ -753,6 +939,13 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       const int rows = pl.rows[x] - quad * 32;  // valid rows of this warp
       const int64_t row0 = pl.row[x] + quad * 32;
       uint16_t* dst = a.out + row0 * a.out_stride + (int64_t)(by_heads ? pl.head0 + x : pl.head0) * 128;
+      const int part = pl.part;
+      float* sums = nullptr;  // this warp's rows of a piece: O [32][128]
+      if (part >= 0) {
+        float* piece = a.pieces + (int64_t)part * kPieceFloats;
+        sums = piece + (x * 128 + quad * 32) * 128;
+        *reinterpret_cast<float2*>(piece + 2 * 128 * 128 + (x * 128 + quad * 32 + lane) * 2) = make_float2(m, l);
+      }
       if (cnt > 0) {
         if (!(ok = wait(&o_full[x], o_parity))) break;
         o_parity ^= 1u;
@@ -771,6 +964,19 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             if (lane == 0) mbar_arrive(&o_free[x]);
           }
           uint4 u[8];
+          if (part >= 0) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                u[e] = make_uint4(o[q * 32 + 4 * e], o[q * 32 + 4 * e + 1], o[q * 32 + 4 * e + 2], o[q * 32 + 4 * e + 3]);
+              transpose_pieces(u);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<uint4*>(sums + ((lane & 24) + e) * 128 + half * 64 + q * 32 + (lane & 7) * 4) = u[e];
+            }
+            continue;
+          }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             u[e].x = pack2<BF16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
@@ -788,9 +994,10 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         }
         if (cleared[k & 1]) {
           __syncwarp();
-          if (lane < rows) add_nonfinite<BF16, PAGED>(a, pl, see, dst + lane * a.out_stride);
+          if (lane < rows)
+            add_nonfinite<BF16, PAGED>(a, pl, see, dst + lane * a.out_stride, part >= 0 ? sums + lane * 128 : nullptr);
         }
-      } else {
+      } else if (part < 0) {
         for (int e = 0; e < min(rows, 32) * 16; e += 32) {
           const int row = (e + lane) >> 4;
           if (row < rows) *reinterpret_cast<uint4*>(dst + row * a.out_stride + ((e + lane) & 15) * 8) = make_uint4(0, 0, 0, 0);
@@ -810,6 +1017,51 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   }
 }
 
+// Joins the pieces of cut items: a block per (CTA whose slot 1 begins a cut item, tile,
+// 32 rows), eight threads per row.  The pieces follow in slot 0 of the next CTAs.
+template <bool BF16>
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WindowArgs a, int ctas, int by_heads) {
+  chain_next();
+  chain_wait();
+  const PieceNote* notes = reinterpret_cast<const PieceNote*>(a.notes);
+  const int cta = blockIdx.x >> 3, x = (blockIdx.x >> 2) & 1, quad = blockIdx.x & 3;
+  const PieceNote first = notes[2 * cta + 1];
+  const int r = quad * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 4;
+  if (first.state != 1 || r >= first.rows[x]) return;
+  float m = -__int_as_float(0x7f800000), l = 0.f;
+  float4 acc[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = cta, more = 1; more && p < ctas; ++p) {
+    const int part = p == cta ? 2 * p + 1 : 2 * p;
+    if (p > cta) {
+      const int state = notes[part].state;
+      if (state == 0) continue;  // a CTA without a share
+      more = state == 1;
+    }
+    const float* piece = a.pieces + (int64_t)part * kPieceFloats;
+    const float2 st = *reinterpret_cast<const float2*>(piece + 2 * 128 * 128 + (x * 128 + r) * 2);
+    if (st.x == -__int_as_float(0x7f800000) && st.y == 0.f) continue;  // the row saw nothing there
+    const float m_new = st.x > m || m == -__int_as_float(0x7f800000) ? st.x : m;
+    const float keep = m == m_new ? 1.f : exp2f(m - m_new), w = st.x == m_new ? 1.f : exp2f(st.x - m_new);
+    m = m_new;
+    l = l * keep + st.y * w;
+    const float* o = piece + (x * 128 + r) * 128 + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 v = *reinterpret_cast<const float4*>(o + e * 32);
+      acc[e] = make_float4(fmaf(v.x, w, acc[e].x * keep), fmaf(v.y, w, acc[e].y * keep), fmaf(v.z, w, acc[e].z * keep),
+                           fmaf(v.w, w, acc[e].w * keep));
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* dst = a.out + (int64_t)(first.row[x] + r) * a.out_stride + (int64_t)(first.head0 + (by_heads ? x : 0)) * 128 + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    *reinterpret_cast<uint2*>(dst + e * 32) =
+        make_uint2(pack2<BF16>(acc[e].x * inv, acc[e].y * inv), pack2<BF16>(acc[e].z * inv, acc[e].w * inv));
+}
+
 // [d2][d1][128] 16-bit elements, 64-channel boxes of `box1` x `box2`
 bool make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, uint64_t d1, uint64_t d2, uint64_t stride1,
                     uint64_t stride2, uint32_t box1, uint32_t box2) {
@@ -824,8 +1076,16 @@ bool make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, uint64_t d1, ui
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// most key tiles that any item can visit
+int64_t window_most_steps(const WindowArgs& a, int rows) {
+  const int64_t keys = a.paged.k ? (int64_t)a.paged.width * a.paged.page : a.Tk;
+  const int64_t span = (int64_t)a.rule.window + rows + (a.rule.chunk > 1 ? 2 * (int64_t)a.rule.chunk : 0);
+  const int64_t window = span < keys ? span / 128 + 2 : keys / 128 + 1;
+  return window + (a.rule.sinks + 127) / 128;
+}
+
 template <bool BF16, bool PAGED>
-int launch_window(const WindowArgs& a, cudaStream_t s, cudaError_t* err) {
+int launch_window(WindowArgs a, cudaStream_t s, cudaError_t* err) {
   CUtensorMap tq, tk, tv;
   if (!make_rows_tmap(&tq, a.q, BF16, (uint64_t)a.Hq, (uint64_t)a.Tq, 256, (uint64_t)a.q_stride * 2, 1, 128)) return 1;
   if constexpr (PAGED) {
@@ -855,14 +1115,28 @@ int launch_window(const WindowArgs& a, cudaStream_t s, cudaError_t* err) {
   const int64_t tiles = (int64_t)a.Tq / rows + a.seqs;  // sum of ceil(len / rows) is at most this
   const int64_t items = tiles * (by_heads ? a.Hq / 2 : a.Hq);
   if (items > INT_MAX / 2) return 4;
-  const int64_t ctas = items < num_sms() ? items : num_sms();
-  *err = launch_chained(kern, ctas, kWinThreads, kWinSmem, s, tq, tk, tv, a, rows, (int)items);
+  // Pieces need room, a second launch and a pass over their sums: only where some item can
+  // be long enough to be cut (a bound from what the host knows).
+  const bool cuts = a.pieces && window_most_steps(a, rows) >= kCutFrom && tiles <= kMaxTiles;
+  if (!cuts) a.notes = nullptr;
+  const int sms = num_sms() < kWinThreads ? num_sms() : kWinThreads;
+  const int64_t ctas = !cuts && items < sms ? items : sms;
+  *err = launch_chained(kern, ctas, kWinThreads, kWinSmem, s, tq, tk, tv, a, rows, (int)tiles);
+  if (*err == cudaSuccess && cuts)
+    *err = launch_chained(window_join_kernel<BF16>, ctas * 8, 256, 0, s, a, (int)ctas, (int)by_heads);
   return *err == cudaSuccess ? 0 : 2;
 }
 
 }  // namespace
 
-int launch_window_attention(const WindowArgs& a, bool bf16, cudaStream_t s, cudaError_t* err) {
+int64_t window_workspace_bytes() {
+  const int sms = num_sms();
+  return window_notes_bytes(sms) + (int64_t)sms * 2 * kPieceFloats * 4;
+}
+
+int launch_window_attention(WindowArgs a, bool bf16, void* workspace, cudaStream_t s, cudaError_t* err) {
+  a.notes = workspace;
+  a.pieces = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + window_notes_bytes(num_sms())) : nullptr;
   if (!a.paged.k && a.Tk == 0) {  // no key anywhere
     *err = cudaMemset2DAsync(a.out, (size_t)a.out_stride * 2, 0, (size_t)a.Hq * 256, (size_t)a.Tq, s);
     return *err == cudaSuccess ? 0 : 2;

@@ -113,11 +113,13 @@ _SIGNATURES = {
     "h3b_bitmap_to_lut": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
     "h3b_attention": [c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
                       c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p],
+    "h3b_window_workspace_bytes": [],
     "h3b_window_attention": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p,
                              c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
-                             c_int64, c_void_p],
+                             c_int64, c_void_p, c_int64, c_void_p],
     "h3b_paged_window_attention": [c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, _cache_p,
-                                   c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p],
+                                   c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_int64,
+                                   c_void_p],
     "h3b_decode_workspace_bytes": [],
     "h3b_decode_attention": [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, _cache_p, c_int64, c_int64, c_int64,
                              c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p],
@@ -134,6 +136,7 @@ _SIGNATURES = {
 }
 _RESTYPES = {"h3b_version": ctypes.c_char_p, "h3b_last_error": ctypes.c_char_p,
              "h3b_key_mean_workspace_bytes": c_int64, "h3b_decode_workspace_bytes": c_int64,
+             "h3b_window_workspace_bytes": c_int64,
              "h3b_pages_workspace_bytes": c_int64}
 
 EXPORTED = tuple(_SIGNATURES)

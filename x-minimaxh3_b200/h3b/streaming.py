@@ -59,13 +59,28 @@ def _scale(scale: float | None) -> float:
     return float(scale)
 
 
+def _workspace(workspace: torch.Tensor | None, need: int, q: torch.Tensor) -> torch.Tensor:
+    if workspace is None:
+        return q.new_empty(need, dtype=torch.uint8)
+    if workspace.numel() * workspace.element_size() < need or not workspace.is_cuda or not workspace.is_contiguous():
+        raise ValueError(f"the workspace must have {need} contiguous bytes on the device")
+    return workspace
+
+
+def _window_workspace(workspace: torch.Tensor | None, q: torch.Tensor) -> tuple[torch.Tensor, int]:
+    need = lib().h3b_window_workspace_bytes()
+    return _workspace(workspace, need, q), need
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
                      chunk: int = 1, scale: float | None = None, query_starts: torch.Tensor | None = None,
-                     key_starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                     key_starts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q [Tq, Hq, 128], k / v [Tk, Hkv, 128] -> [Tq, Hq, 128]; bf16 or fp16.
 
     query_starts / key_starts: int32 [sequences + 1] first rows of each sequence of a
-    ragged batch (from 0 to Tq / Tk); None: one sequence."""
+    ragged batch (from 0 to Tq / Tk); None: one sequence.  workspace: uint8, reused by
+    calls on one stream."""
     _cuda("window_attention", q, k, v)
     q, k, v = _token_rows(q, None, "q"), _token_rows(k, None, "k"), _token_rows(v, None, "v")
     if k.shape != v.shape or not q.dtype is k.dtype is v.dtype:
@@ -82,10 +97,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         if seqs < 1:
             raise ValueError("query_starts needs at least two entries")
     out = _output(out, q)
+    workspace, size = _window_workspace(workspace, q)
     check(lib().h3b_window_attention(_ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), DTYPE_CODES[q.dtype],
                                      q.shape[0], k.shape[0], _ptr(query_starts), _ptr(key_starts), seqs, q.shape[1],
                                      k.shape[1], window, sinks, chunk, _scale(scale), _ptr(out), out.stride(0),
-                                     _stream(q)), "window_attention")
+                                     _ptr(workspace), size, _stream(q)), "window_attention")
     return out
 
 
@@ -101,8 +117,8 @@ def _cached_queries(q: torch.Tensor, cache: PagedKVCache, layer: int, what: str)
 
 def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor | None = None, *,
                            window: int | None = None, sinks: int = 0, chunk: int = 1, scale: float | None = None,
-                           query_starts: torch.Tensor | None = None, layer: int = 0,
-                           out: torch.Tensor | None = None) -> torch.Tensor:
+                           query_starts: torch.Tensor | None = None, layer: int = 0, out: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q [Tq, Hq, 128]: the last tokens of the cache's sequences `slots` (int32; None: slot 0, 1, ...),
     already appended.  query_starts: int32 [sequences + 1]; None: one sequence."""
     q = _cached_queries(q, cache, layer, "paged_window_attention")
@@ -117,9 +133,10 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
     elif seqs > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
     out = _output(out, q)
+    workspace, size = _window_workspace(workspace, q)
     check(lib().h3b_paged_window_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], q.shape[0], _ptr(query_starts),
                                            _ptr(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
-                                           _scale(scale), _ptr(out), out.stride(0), _stream(q)),
+                                           _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), size, _stream(q)),
           "paged_window_attention")
     return out
 
@@ -139,10 +156,7 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
     elif n > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
     need = lib().h3b_decode_workspace_bytes()
-    if workspace is None:
-        workspace = q.new_empty(need, dtype=torch.uint8)
-    elif workspace.numel() * workspace.element_size() < need or not workspace.is_cuda:
-        raise ValueError(f"the workspace must have {need} bytes on the device")
+    workspace = _workspace(workspace, need, q)
     out = _output(out, q)
     check(lib().h3b_decode_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], _ptr(slots), n, q.shape[1], cache._ref,
                                      layer, window, sinks, _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), need,
