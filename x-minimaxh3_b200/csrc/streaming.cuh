@@ -41,7 +41,7 @@ struct VisibleKeys {
 __host__ __device__ __forceinline__ VisibleKeys visible_keys(const WindowRule& r, int p, int lk) {
   if (p < 0) return {0, 0, 0};
   int64_t last = p;
-  if (r.chunk > 1) last = p < r.sinks ? r.sinks - 1 : r.sinks + ((int64_t)(p - r.sinks) / r.chunk + 1) * r.chunk - 1;
+  if (r.chunk > 1) last = p < r.sinks ? r.sinks - 1 : r.sinks + ((int64_t)((p - r.sinks) / r.chunk) + 1) * r.chunk - 1;
   const int end = last + 1 < lk ? (int)last + 1 : lk;
   int64_t lo = last - r.window + 1;
   lo = lo < 0 ? 0 : lo > end ? end : lo;

@@ -19,12 +19,13 @@
 // with an infinity or NaN are cleared first, because P = 0 does not hide them from the
 // matrix product, and their rows' outputs get them added at the end (add_nonfinite).
 //
-// 384 threads: warp 0 plans the items and loads (TMA; Q once, then K and V tiles through
+// 512 threads: warp 0 plans the items and loads (TMA; Q once, then K and V tiles through
 // a ring of five 32 KB slots), warp 1 allocates tensor memory and clears V, warps 2 and 3
 // issue the MMAs of tile A and B, warps 4..7 and 8..11 are their softmax, one row per
-// thread.  S of a step's first 64 keys is issued as soon as the step before has been read
-// from tensor memory, S of the others after that step's PV, which reads P from their
-// columns; PV of 64 keys starts when half of P is written.  The two tiles take turns.
+// thread, warps 12..15 write O of finished items while the next one runs.  S of a step's
+// first 64 keys is issued as soon as the step before has been read from their columns, S
+// of the others after that step's PV, which reads P from theirs; PV of 64 keys starts when
+// half of P is written.  The two tiles take turns.
 // Tensor memory: S_A 0..127, S_B 128..255, O_A 256..383, O_B 384..511, P over S + 64.
 #include <atomic>
 #include <climits>
@@ -36,19 +37,21 @@ namespace h3b {
 
 namespace {
 
-constexpr int kWinThreads = 384;
+constexpr int kWinThreads = 512;
 constexpr int kWinSlots = 5;
 constexpr int kWinTile = 128 * 128 * 2;  // bytes of a 128 x 128 16-bit tile
 constexpr int kWinOffRing = 2 * kWinTile;
-constexpr int kWinOffBar = kWinOffRing + kWinSlots * kWinTile;
-constexpr int kWinSmem = kWinOffBar + 512 + 1024;
-// Register split (setmaxnreg): every thread starts with kWinRegs, the control warpgroup
-// drops to kWinCtrlRegs, each softmax warpgroup rises to kWinSoftRegs; the shares may not
-// exceed the launch's total, or the rise would wait forever (the host checks kWinRegs).
-constexpr int kWinRegs = 168;
-constexpr int kWinCtrlRegs = 72;
-constexpr int kWinSoftRegs = 216;
-static_assert(128 * (kWinCtrlRegs + 2 * kWinSoftRegs) <= kWinThreads * kWinRegs, "register split too large");
+constexpr int kWinOffRest = kWinOffRing + kWinSlots * kWinTile;
+constexpr int kWinSmem = kWinOffRest + 3072;  // all of a block's 227 KB
+// Register split (setmaxnreg): every thread starts with kWinRegs, the control and output
+// warpgroups drop to kWinCtrlRegs and kWinOutRegs, each softmax warpgroup rises to
+// kWinSoftRegs; the shares may not exceed the launch's total, or the rise would wait
+// forever (the host checks kWinRegs).
+constexpr int kWinRegs = 128;
+constexpr int kWinCtrlRegs = 104;
+constexpr int kWinOutRegs = 104;
+constexpr int kWinSoftRegs = 152;
+static_assert(128 * (kWinCtrlRegs + kWinOutRegs + 2 * kWinSoftRegs) <= kWinThreads * kWinRegs, "register split too large");
 constexpr float kWinTau = 8.0f;
 
 // D(tmem) (+)= A(tmem) * B(smem), 16-bit x 16-bit -> fp32
@@ -67,6 +70,33 @@ __device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t smem_addr, uint
   return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(next_columns >> 4) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// Hand-over of tensor memory between warps: its order comes from tcgen05.wait and the
+// tcgen05 fences on both sides, so neither the arrival nor the wait orders other memory
+// (a releasing arrival costs about 150 cycles here, four of them a step).
+__device__ __forceinline__ void tmem_arrive(uint64_t* bar) {  // one arrival of the (converged) warp
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "@p mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool tmem_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool tmem_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  bool ok = tmem_try_wait(bar, parity);
+  if (!__all_sync(0xffffffffu, ok)) ok = mbar_wait_warp(bar, parity, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
+  return ok;
+}
+
 template <bool BF16>
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {
   return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
@@ -95,6 +125,17 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
   if constexpr (BF16) return (w & 0x7f807f80u) + 0x00800080u;
   return (w & 0x7c007c00u) + 0x04000400u;
+}
+
+// sum + 0 w, for both 16-bit values: stays 0 as long as they are finite
+template <bool BF16>
+__device__ __forceinline__ uint32_t zero_times2(uint32_t w, uint32_t sum) {
+  uint32_t r;
+  if constexpr (BF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(sum));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(sum));
+  return r;
 }
 
 // The 128-key tiles that rows [p0, p1] of a tile see: [0, sn) and [w0, w1), sn <= w0.
@@ -127,6 +168,18 @@ struct StepRanges {
   __device__ bool takes(int i) const { return i < head || (i >= from && i < to); }
   __device__ bool whole(int i) const { return i < whole_head || (i >= whole_from && i < whole_to); }
 };
+// The key tiles that rows [p0, p1] see, in the order of the steps: [0, sn), then w0 and on.
+struct UnionKeys {
+  int sn, w0, steps;
+};
+__device__ __forceinline__ UnionKeys union_keys(const WindowRule& r, int p0, int p1, int lk) {
+  if (p1 < 0) return {0, 0, 0};
+  const VisibleKeys a = visible_keys(r, p0 < 0 ? 0 : p0, lk), b = visible_keys(r, p1, lk);
+  const int sn = (b.sinks + 127) / 128;
+  if (a.lo >= b.end) return {sn, sn, sn};
+  const int w0 = max(a.lo / 128, sn);
+  return {sn, w0, sn + max((b.end + 127) / 128, w0) - w0};
+}
 struct WinPlan {
   StepRanges tile[2];
   int row[2], rows[2];  // first row (of q) and valid rows of each tile
@@ -179,53 +232,65 @@ __device__ __forceinline__ void win_exp32(uint32_t* s, float2 c2, float2 o2, flo
   }
 }
 
-// One key tile for one query row.  cnt: tiles that the row's query tile has taken before
-// (their PV is complete: it was issued before this S).
-template <bool BF16, bool MASK>
-__device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, float c, const VisibleKeys& see, int j0,
-                                            int cnt, float& m, float& l, uint64_t* s_free, uint64_t* p_half,
-                                            uint64_t* turn, uint32_t turn_parity, uint64_t* other_turn,
-                                            volatile int* abort_flag) {
-  uint32_t s[128];
+__device__ __forceinline__ void win_load64(uint32_t s_addr, uint32_t (&s)[64]) {
   __syncwarp();
   tmem_ld32(s_addr, H3B_S32(s, 0));
   tmem_ld32(s_addr + 32, H3B_S32(s, 32));
-  tmem_ld32(s_addr + 64, H3B_S32(s, 64));
-  tmem_ld32(s_addr + 96, H3B_S32(s, 96));
   tmem_wait_ld_dep(H3B_S32(s, 0));
   reg_barrier32(H3B_S32(s, 32));
-  reg_barrier32(H3B_S32(s, 64));
-  reg_barrier32(H3B_S32(s, 96));
-  tc_fence_before();
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(s_free);
-  if constexpr (MASK) {
+}
+
+// One key tile for one query row, in two passes over the scores: the maximum, then P.
+// Both are loops over halves of 64 keys, not unrolled: the softmax warps of both tiles run
+// through this code every step, and with all 128 columns unrolled (and masked tiles apart)
+// it did not stay in the instruction cache (11 prompts of about 500 tokens: 148 us with
+// masked tiles apart, 134 us as one, 116 us as loops).
+// The upper half goes first: its P lies over its own scores, and the lower half's columns
+// are free for the next S as soon as they are read.
+// cnt: tiles that the row's query tile has taken before (their PV is complete: it was
+// issued before this S).
+template <bool BF16>
+__device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, float c, const VisibleKeys& see,
+                                            bool whole, int j0, int cnt, float& m, float& l, uint64_t* s_free,
+                                            uint64_t* p_half, uint64_t* turn, uint32_t turn_parity,
+                                            uint64_t* other_turn, volatile int* abort_flag) {
+  uint32_t s[64];
+  float tmax = -__int_as_float(0x7f800000);
+#pragma unroll 1
+  for (int g = 0; g < 2; ++g) {
+    win_load64(s_addr + g * 64, s);
+    if (!whole) {  // scores of unseen keys become -inf, for the second pass too
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int base = j0 + w * 32;
-      const uint32_t bits = key_bits(base, see.lo, see.end) | key_bits(base, 0, see.sinks);
+      for (int w = 0; w < 2; ++w) {
+        const int base = j0 + g * 64 + w * 32;
+        const uint32_t bits = key_bits(base, see.lo, see.end) | key_bits(base, 0, see.sinks);
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (!((bits >> e) & 1u)) s[w * 32 + e] = 0xff800000u;
+        for (int e = 0; e < 32; ++e)
+          if (!((bits >> e) & 1u)) s[w * 32 + e] = 0xff800000u;
+        tmem_st32(s_addr + g * 64 + w * 32, H3B_S32(s, w * 32));
+      }
+      tmem_wait_st();
     }
-  }
-  float mx[4];
+    float mx[4];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    mx[w] = max3_nan(__uint_as_float(s[w * 32]), __uint_as_float(s[w * 32 + 1]), __uint_as_float(s[w * 32 + 2]));
+    for (int w = 0; w < 4; ++w)
+      mx[w] = max3_nan(__uint_as_float(s[w]), __uint_as_float(s[4 + w]), __uint_as_float(s[8 + w]));
 #pragma unroll
-    for (int e = 3; e < 31; e += 2)
-      mx[w] = max3_nan(mx[w], __uint_as_float(s[w * 32 + e]), __uint_as_float(s[w * 32 + e + 1]));
-    mx[w] = max3_nan(mx[w], __uint_as_float(s[w * 32 + 31]), __uint_as_float(s[w * 32 + 31]));
+    for (int e = 12; e < 60; e += 8)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx[w] = max3_nan(mx[w], __uint_as_float(s[e + w]), __uint_as_float(s[e + 4 + w]));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx[w] = max3_nan(mx[w], __uint_as_float(s[60 + w]), mx[w]);
+    tmax = max3_nan(tmax, max3_nan(mx[0], mx[1], mx[2]), mx[3]);
   }
-  const float tmax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * c;
+  tmax *= c;
   // a score of +inf or NaN: the row's result is not a number, whatever the rest does
   if (!(tmax < __int_as_float(0x7f800000))) l = __int_as_float(0x7fffffff);
   const float m_new = tmax > m + kWinTau || m == -__int_as_float(0x7f800000) ? tmax : m;
-  float alpha = 1.f;
   if (__any_sync(0xffffffffu, m_new != m)) {
-    alpha = m_new == m ? 1.f : ex2(m - m_new);
+    const float alpha = m_new == m ? 1.f : ex2(m - m_new);
     m = m_new;
+    l *= alpha;
     if (cnt > 0) {
       __syncwarp();
 #pragma unroll 1
@@ -243,32 +308,37 @@ __device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, fl
   const float off = m == -__int_as_float(0x7f800000) ? 0.f : -m;
   const float2 c2 = make_float2(c, c), o2 = make_float2(off, off);
   //TR3
-  if (!mbar_wait_warp(turn, turn_parity, abort_flag, H3B_STATUS_ATTN_TIMEOUT)) return false;
+  if (!tmem_wait(turn, turn_parity, abort_flag)) return false;
   //TR4
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    win_exp32(&s[h * 64], c2, o2, acc0, acc1);
-    win_exp32(&s[h * 64 + 32], c2, o2, acc0, acc1);
-    if (h == 1) {
+#pragma unroll 1
+  for (int g = 1; g >= 0; --g) {
+    win_load64(s_addr + g * 64, s);
+    if (g == 0) {
+      tc_fence_before();
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(other_turn);
+      tmem_arrive(s_free);
+    }
+    win_exp32(&s[0], c2, o2, acc0, acc1);
+    win_exp32(&s[32], c2, o2, acc0, acc1);
+    if (g == 0) {
+      __syncwarp();
+      tmem_arrive(other_turn);
       //TR5
     }
     uint32_t p[32];
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      p[e] = pack2<BF16>(__uint_as_float(s[h * 64 + 2 * e]), __uint_as_float(s[h * 64 + 2 * e + 1]));
-    tmem_st32(s_addr + 64 + h * 32, p);
+    for (int e = 0; e < 32; ++e) p[e] = pack2<BF16>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+    tmem_st32(s_addr + 64 + g * 32, p);
     tmem_wait_st();
     tc_fence_before();
-    if (h == 0) {
+    if (g == 1) {
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(p_half);
+      tmem_arrive(p_half);
     }
   }
   const float2 t = __fadd2_rn(acc0, acc1);
-  l = l * alpha + (t.x + t.y);
+  l += t.x + t.y;
   return true;
 }
 
@@ -323,8 +393,8 @@ __device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& p
 // item is short (kCutFrom) or the piece would be (kLeastPiece): then it moves to the
 // item's nearer end.  The pieces of a cut item leave their sums, and window_join_kernel
 // puts them together.
-constexpr int kItemCost = 2;
-constexpr int kCutFrom = 9;
+constexpr int kItemCost = 4;
+constexpr int kCutFrom = 8;
 constexpr int kLeastPiece = 3;
 constexpr int kPieceFloats = 2 * 128 * 130;  // O [2][128][128], then (m, l) [2][128]
 constexpr int kMaxTiles = kWinSlots * kWinTile / 12 - 16;  // prefix sums of tiles and sequences that fit the ring
@@ -380,28 +450,21 @@ __device__ __forceinline__ void plan_tile(const WindowArgs& a, int seq, int t, i
     p.k_row = kr.a;
   }
   const int lq = qr.b - qr.a;
-  TileKeys keys[2];
+  const int first = t * rows_per_cta;
+  const UnionKeys u = union_keys(a.rule, p.lk - lq + first, p.lk - lq + min(first + rows_per_cta, lq) - 1, p.lk);
+  p.sn = u.sn;
+  p.w0 = u.w0;
+  p.steps = u.steps;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const int first = t * rows_per_cta + (by_heads ? 0 : x * 128);
-    p.row[x] = qr.a + first;
-    p.rows[x] = max(0, min(128, lq - first));
-    p.p0[x] = p.lk - lq + first;
-    keys[x] = p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
+    const int from = first + (by_heads ? 0 : x * 128);
+    p.row[x] = qr.a + from;
+    p.rows[x] = max(0, min(128, lq - from));
+    p.p0[x] = p.lk - lq + from;
+    const TileKeys keys =
+        p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
+    p.tile[x] = step_ranges(keys, p.sn, p.w0);
   }
-  p.sn = max(keys[0].sn, keys[1].sn);
-  int w0 = 1 << 30, w1 = 0;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (keys[x].w1 > keys[x].w0) {
-      w0 = min(w0, keys[x].w0);
-      w1 = max(w1, keys[x].w1);
-    }
-  }
-  p.w0 = max(w0, p.sn);
-  p.steps = p.sn + max(0, w1 - p.w0);
-#pragma unroll
-  for (int x = 0; x < 2; ++x) p.tile[x] = step_ranges(keys[x], p.sn, p.w0);
 }
 
 // A place in the list that is dealt out: an item and a step of it.
@@ -409,7 +472,7 @@ struct WorkAt {
   int item, step;
 };
 // What a CTA does: `rounds` whole items, then from bounds[0] to bounds[1].
-constexpr int kListed = 60;
+constexpr int kListed = 48;
 struct WorkShare {
   int valid, rounds;
   WorkAt bounds[2];
@@ -429,16 +492,17 @@ struct RingAt {
   }
 };
 
-// 32 output rows of a warp (a row per lane, 8 pieces of 16 bytes of it) so that 8 lanes
-// store the 128 contiguous bytes of one row: an 8 x 8 transpose of pieces in each group
-// of 8 lanes.  A store of own rows would touch 32 lines for 512 bytes.
-__device__ __forceinline__ void transpose_pieces(uint4 (&u)[8]) {
+// 32 output rows of a warp (a row per lane, N pieces of 16 bytes of it) so that N lanes
+// store 16 N contiguous bytes of one row: an N x N transpose of pieces in each group of N
+// lanes.  A store of own rows would touch 32 lines for 512 bytes.
+template <int N>
+__device__ __forceinline__ void transpose_pieces(uint4 (&u)[N]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int b = 1; b < 8; b <<= 1) {
+  for (int b = 1; b < N; b <<= 1) {
     const bool up = lane & b;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (i & b) continue;
       uint4 &lo = u[i], &hi = u[i | b];
       const uint4 give = up ? lo : hi;
@@ -460,9 +524,25 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     window_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WindowArgs a, int rows_per_cta,
                   int tiles) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWinOffBar);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles and the room behind them count on it
+    if (threadIdx.x == 0) record_status(H3B_STATUS_ATTN_TIMEOUT);
+    return;
+  }
+  struct Rest {
+    uint64_t bars[46];
+    uint32_t words[8];
+    WinPlan plans[3];
+    WorkShare work;
+    long long scan[kWinThreads / 32];
+    float l[2][128];  // row sums of the item that warps 12..15 write
+  };
+  static_assert(sizeof(Rest) <= kWinSmem - kWinOffRest, "shared memory");
+  Rest& rest = *reinterpret_cast<Rest*>(smem + kWinOffRest);
+  WinPlan(&plans)[3] = rest.plans;
+  WorkShare& work = rest.work;
+  long long* scan = rest.scan;
+  uint64_t* bars = rest.bars;
   uint64_t* full = bars;                // kWinSlots
   uint64_t* empty = full + kWinSlots;   // kWinSlots (a release per tile)
   uint64_t* v_ok = empty + kWinSlots;   // 4: V of a step (mod 4) is free of what masking cannot hide
@@ -470,19 +550,18 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   uint64_t* q_empty = q_full + 1;       // 1 (per tile)
   uint64_t* s_full = q_empty + 1;       // 2: S written
   uint64_t* s_free = s_full + 2;        // 2: S read
-  uint64_t* p_half = s_free + 2;        // 2: P of the first 64 keys written
+  uint64_t* p_half = s_free + 2;        // 2: P of the last 64 keys written
   uint64_t* p_full = p_half + 2;        // 2
   uint64_t* o_full = p_full + 2;        // 2: O of an item complete
   uint64_t* o_free = o_full + 2;        // 2: O read
   uint64_t* turns = o_free + 2;         // 2 x 4: whose exponentials run, per SM sub-partition
-  uint64_t* plan_full = turns + 8;      // 2
-  uint64_t* plan_free = plan_full + 2;  // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(plan_free + 2);
+  uint64_t* plan_full = turns + 8;      // 3
+  uint64_t* plan_free = plan_full + 3;  // 3
+  uint64_t* l_full = plan_free + 3;     // 2: row sums of an item written
+  uint64_t* l_free = l_full + 2;        // 2: and read
+  uint32_t* tmem_slot = rest.words;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* cleared = abort_flag + 1;  // [2]: some seen V row of the item was cleared
-  __shared__ WinPlan plans[2];
-  __shared__ long long scan[kWinThreads / 32];
-  __shared__ WorkShare work;
+  volatile int* cleared = abort_flag + 1;  // [3]: some seen V row of the item was cleared
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool by_heads = rows_per_cta == 128;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -513,23 +592,27 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       mbar_init(&p_full[x], 4);
       mbar_init(&o_full[x], 1);
       mbar_init(&o_free[x], 4);
-      mbar_init(&plan_full[x], 1);
-      mbar_init(&plan_free[x], 11);  // all warps but the planning one
+      mbar_init(&l_full[x], 4);
+      mbar_init(&l_free[x], 4);
+    }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&plan_full[s], 1);
+      mbar_init(&plan_free[s], 15);  // all warps but the planning one
     }
     for (int s = 0; s < 8; ++s) mbar_init(&turns[s], 1);
     *abort_flag = 0;
-    cleared[0] = cleared[1] = 0;
+    cleared[0] = cleared[1] = cleared[2] = 0;
     fence_mbar_init();
   }
   chain_next();
   chain_wait();
   const int columns = by_heads ? a.Hq / 2 : a.Hq;
   {
-    // Costs of all tiles, as prefix sums in the ring's memory.  More than kMaxTiles do not
-    // fit: then all items are dealt whole, in rounds.
-    const bool fits = tiles <= kMaxTiles;
+    // Where no item is cut, all are dealt whole, in rounds.
+    const bool cuts = a.notes != nullptr;
+    // Else costs of all tiles, as prefix sums in the ring's memory.
     long long* upto = reinterpret_cast<long long*>(smem + kWinOffRing);  // [tiles] from the last tile, per column
-    int* seq_upto = reinterpret_cast<int*>(upto + (fits ? tiles : 0));   // [seqs]: tiles of 0..i
+    int* seq_upto = reinterpret_cast<int*>(upto + tiles);   // [seqs]: tiles of 0..i
     // inclusive prefix sums of n values over the block: value(i) -> put(i, sum)
     auto prefix = [&](int n, auto value, auto put) {
       const int per = (n + kWinThreads - 1) / kWinThreads, first = (int)threadIdx.x * per;
@@ -544,12 +627,13 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       if (lane == 31) scan[warp] = incl;
       __syncthreads();
       long long run = incl - sum;
-      for (int w = 0; w < warp; ++w) run += scan[w];
+#pragma unroll
+      for (int w = 0; w < kWinThreads / 32; ++w) run += w < warp ? scan[w] : 0;
       for (int i = first; i < min(first + per, n); ++i) put(i, run += value(i));
       __syncthreads();
     };
     const int ctas = (int)gridDim.x, me = (int)blockIdx.x;
-    if (!fits) {
+    if (!cuts) {
       if (threadIdx.x == 0) {
         const int items = tiles * columns;
         work.valid = tiles;
@@ -570,9 +654,16 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       };
       for (int q = (int)threadIdx.x; q < valid; q += kWinThreads) {
         const TileAt at = locate(valid - 1 - q);
-        WinPlan p;
-        plan_tile<PAGED>(a, at.seq, at.t, rows_per_cta, p);
-        upto[q] = p.steps + kItemCost;
+        const RowRange qr = row_range(a.q_starts, at.seq, a.Tq);
+        int lk;
+        if constexpr (PAGED) {
+          lk = paged_len(a.paged, paged_slot(a.paged, at.seq));
+        } else {
+          const RowRange kr = row_range(a.k_starts, at.seq, a.Tk);
+          lk = kr.b - kr.a;
+        }
+        const int lq = qr.b - qr.a, first = at.t * rows_per_cta;
+        upto[q] = union_keys(a.rule, lk - lq + first, lk - lq + min(first + rows_per_cta, lq) - 1, lk).steps + kItemCost;
       }
       __syncthreads();
       prefix(valid, [&](int i) { return upto[i]; }, [&](int i, long long x) { upto[i] = x; });
@@ -583,13 +674,19 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         return upto[q] - (q ? upto[q - 1] : 0);
       };
       // whole rounds; a thread per CTA (the launch has at most kWinThreads)
-      int rounds = 0;
+      int rounds = 0, my_q = (int)threadIdx.x / columns, my_column = (int)threadIdx.x % columns;
+      const int step_q = ctas / columns, step_column = ctas % columns;
       long long load = 0;
       for (;; ++rounds) {
-        const int first = rounds * ctas;
-        const long long next = (int)threadIdx.x < ctas && first + ctas <= items ? load + cost(first + (int)threadIdx.x) : 0;
-        if (!__syncthreads_and(first + ctas <= items && next <= share)) break;
+        const bool in = (rounds + 1) * ctas <= items;
+        const long long next = (int)threadIdx.x < ctas && in ? load + upto[my_q] - (my_q ? upto[my_q - 1] : 0) : 0;
+        if (!__syncthreads_and(in && next <= share)) break;
         load = next;
+        my_q += step_q;
+        if ((my_column += step_column) >= columns) {
+          my_column -= columns;
+          ++my_q;
+        }
       }
       const int dealt = rounds * ctas;  // first item of the list
       const int q0 = dealt / columns;
@@ -609,7 +706,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           const long long in = at - first * columns;
           w.item = lo * columns + (int)(in / worth);
           w.step = max((int)(in % worth) - kItemCost, 0);
-          const bool whole = !a.notes || steps < kCutFrom;  // the item may not be cut
+          const bool whole = steps < kCutFrom;  // the item may not be cut
           if (w.step > 0 && (whole ? 2 * w.step >= steps : steps - w.step < kLeastPiece)) {
             w.step = 0;
             ++w.item;
@@ -642,6 +739,13 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // last step of a piece that a tile takes (-1: none)
+  auto last_step = [](const WinPlan& p, int x) {
+    const StepRanges& r = p.tile[x];
+    int last = min(r.to, p.to) - 1;
+    if (last < max(r.from, p.from)) last = min(r.head, p.to) - 1;
+    return last < p.from ? -1 : last;
+  };
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWinCtrlRegs));
   if (warp == 0) {
     // plans the items and loads their tiles
@@ -655,15 +759,18 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     PieceNote* notes = reinterpret_cast<PieceNote*>(a.notes) + 2 * blockIdx.x;
     if (a.notes && lane < 2) notes[lane].state = 0;
     __syncwarp();
-    for (int k = 0;; ++k) {
-      WinPlan* pl = &plans[k & 1];
-      if (k > 1 && !wait(&plan_free[k & 1], (uint32_t)((k >> 1) & 1) ^ 1u)) break;
-      const bool round = k < rounds;
+    // the plan of the next item, as far as there is one; made while one is loaded
+    RingAt<3> next;
+    int made = 0;
+    auto make_plan = [&]() -> bool {
+      WinPlan* pl = &plans[next.slot];
+      if (!wait(&plan_free[next.slot], next.parity ^ 1u)) return false;
+      const bool round = made < rounds;
       if (round || w.item < stop.item || (w.item == stop.item && w.step < stop.step)) {
-        const int item = round ? (int)blockIdx.x + k * (int)gridDim.x : w.item, q = item / columns;
-        const int entry = round ? k : rounds + q - dealt_tile;
+        const int item = round ? (int)blockIdx.x + made * (int)gridDim.x : w.item, q = item / columns;
+        const int entry = round ? made : rounds + q - dealt_tile;
         TileAt at;
-        if (entry < kListed && tiles <= kMaxTiles)
+        if (a.notes && entry < kListed)
           at = work.tile[entry];
         else
           at = find_tile(a, work.valid - 1 - q, rows_per_cta);
@@ -689,17 +796,27 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             notes[slot] = n;
           }
           *pl = p;
-          cleared[k & 1] = 0;
+          cleared[next.slot] = 0;
         }
         if (!round) w = {w.item + 1, 0};
       } else if (lane == 0) {
         pl->to = -1;
       }
+      ++made;
       __syncwarp();
+      if (lane == 0) mbar_arrive(&plan_full[next.slot]);
+      next.next();
+      return true;
+    };
+    ok = make_plan();
+    for (RingAt<3> pr; ok; pr.next()) {
+      const WinPlan* pl = &plans[pr.slot];
       const int from = pl->from, to = pl->to, sn = pl->sn, w0 = pl->w0, kh = pl->kh;
-      if (lane == 0) mbar_arrive(&plan_full[k & 1]);
       if (to < 0) break;
-      if (from == to) continue;
+      if (from == to) {
+        ok = make_plan();
+        continue;
+      }
       if (!(ok = wait(q_empty, q_parity))) break;
       q_parity ^= 1u;
       if (lane == 0) mbar_arrive_expect_tx(q_full, 2 * kWinTile);
@@ -709,6 +826,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                     by_heads ? pl->head0 + (lane >> 1) : pl->head0, pl->row[lane >> 1]);
       __syncwarp();
       for (int i = 2 * from; i < 2 * to; ++i, at.next()) {
+        if (i == min(2 * from + 4, 2 * to - 1) && !(ok = make_plan())) break;  // the ring is full by now
         if (!(ok = wait(&empty[at.slot], at.parity ^ 1u))) break;
         const int n = i >> 1, j0 = (n < sn ? n : w0 + (n - sn)) * 128;
         const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
@@ -740,23 +858,29 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     RingAt<kWinSlots> at;
     RingAt<4> vo;
     bool ok = true;
-    for (int k = 0; ok; ++k) {
-      const WinPlan& pl = plans[k & 1];
-      if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
+    for (RingAt<3> pr; ok; pr.next()) {
+      const WinPlan& pl = plans[pr.slot];
+      if (!wait(&plan_full[pr.slot], pr.parity)) break;
       const int to = pl.to;
       if (to < 0) break;
       for (int i = pl.from; i < to; ++i) {
+        // K first: a slot's fills alternate between K and V, and a wait that skipped K's
+        // would take the fill before it for V's
+        if (!(ok = wait(&full[at.slot], at.parity))) break;
         at.next();
         if (!(ok = wait(&full[at.slot], at.parity))) break;
         if (pl.masked(i)) {
           uint4* v = reinterpret_cast<uint4*>(smem + kWinOffRing + at.slot * kWinTile);
-          uint32_t any = 0;
-#pragma unroll 8
+          uint32_t any[4] = {0, 0, 0, 0};  // 0, or NaN once an element was not finite
+#pragma unroll 16
           for (int x = 0; x < kWinTile / 16 / 32; ++x) {
             const uint4 w = v[x * 32 + lane];
-            any |= nonfinite2<BF16>(w.x) | nonfinite2<BF16>(w.y) | nonfinite2<BF16>(w.z) | nonfinite2<BF16>(w.w);
+            any[0] = zero_times2<BF16>(w.x, any[0]);
+            any[1] = zero_times2<BF16>(w.y, any[1]);
+            any[2] = zero_times2<BF16>(w.z, any[2]);
+            any[3] = zero_times2<BF16>(w.w, any[3]);
           }
-          if (__any_sync(0xffffffffu, any & 0x80008000u)) {
+          if (__any_sync(0xffffffffu, (any[0] | any[1] | any[2] | any[3]) & 0x7fff7fffu)) {
             const int j0 = pl.key_tile(i) * 128;
             for (int x = lane; x < kWinTile / 16; x += 32) {
               uint4 w = v[x];
@@ -771,7 +895,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
               }
               if (hit) {
                 v[x] = w;
-                if (j0 + (x / 8) % 128 < pl.lk) cleared[k & 1] = 1;  // 8 pieces per row and half
+                if (j0 + (x / 8) % 128 < pl.lk) cleared[pr.slot] = 1;  // 8 pieces per row and half
               }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -782,7 +906,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         vo.next();
         at.next();
       }
-      if (lane == 0) mbar_arrive(&plan_free[k & 1]);
+      if (lane == 0) mbar_arrive(&plan_free[pr.slot]);
     }
   } else if (warp < 4) {
     // MMA issuer of tile x: the whole warp walks the steps, one elected lane issues
@@ -805,15 +929,12 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     RingAt<4> vo;
     uint32_t q_parity = 0, o_parity = 1, step_parity = 0;
     bool ok = true;
-    for (int k = 0; ok; ++k) {
-      if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
-      const int from = plans[k & 1].from, to = plans[k & 1].to;
+    for (RingAt<3> pr; ok; pr.next()) {
+      if (!wait(&plan_full[pr.slot], pr.parity)) break;
+      const int from = plans[pr.slot].from, to = plans[pr.slot].to;
       if (to < 0) break;
-      const StepRanges r = plans[k & 1].tile[x];
-      // last step taken (-1: none)
-      int last = min(r.to, to) - 1;
-      if (last < max(r.from, from)) last = min(r.head, to) - 1;
-      if (last < from) last = -1;
+      const StepRanges r = plans[pr.slot].tile[x];
+      const int last = last_step(plans[pr.slot], x);
       if (to > from) {
         if (!(ok = wait(q_full, q_parity))) break;
         q_parity ^= 1u;
@@ -851,29 +972,29 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         issued = i < last && r.takes(i + 1);
         if (issued) {
           // the next S of the first 64 keys, over the columns that hold neither S nor P now
-          if (!(ok = wait(&full[at.slot], at.parity) && wait(&s_free[x], step_parity))) break;
+          if (!(ok = wait(&full[at.slot], at.parity) && tmem_wait(&s_free[x], step_parity, abort_flag))) break;
           tc_fence_after();
           if (elect_one()) issue_s(at.slot, 0, idesc_half);
           __syncwarp();
         }
         const uint64_t vdesc = sdesc_mnmajor_sw128(ring + vt.slot * kWinTile, kWinTile / 2);
-        if (first && !(ok = wait(&o_free[x], o_parity))) break;
-        if (!(ok = wait(&v_ok[vs.slot], vs.parity) && wait(&p_half[x], step_parity))) break;
+        if (first && !(ok = tmem_wait(&o_free[x], o_parity, abort_flag))) break;
+        if (!(ok = wait(&v_ok[vs.slot], vs.parity) && tmem_wait(&p_half[x], step_parity, abort_flag))) break;
         tc_fence_after();
         //TM0 i
         if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            mma_f16_ts(o_tmem, s_tmem + 64 + 8 * c, vdesc + (uint64_t)(128 * c), idesc_pv, first && c == 0 ? 0u : 1u);
+          for (int c = 4; c < 8; ++c)
+            mma_f16_ts(o_tmem, s_tmem + 64 + 8 * c, vdesc + (uint64_t)(128 * c), idesc_pv, first && c == 4 ? 0u : 1u);
         }
         __syncwarp();
         first = false;
-        if (!(ok = wait(&p_full[x], step_parity))) break;
+        if (!(ok = tmem_wait(&p_full[x], step_parity, abort_flag))) break;
         tc_fence_after();
         //TM1 i
         if (elect_one()) {
 #pragma unroll
-          for (int c = 4; c < 8; ++c)
+          for (int c = 0; c < 4; ++c)
             mma_f16_ts(o_tmem, s_tmem + 64 + 8 * c, vdesc + (uint64_t)(128 * c), idesc_pv, 1u);
           mma_commit(&empty[vt.slot]);
           if (issued) {
@@ -891,9 +1012,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       }
       if (!ok) break;
       if (last >= 0) o_parity ^= 1u;
-      if (lane == 0) mbar_arrive(&plan_free[k & 1]);
+      if (lane == 0) mbar_arrive(&plan_free[pr.slot]);
     }
-  } else {
+  } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWinSoftRegs));
     const int x = (warp - 4) >> 2, quad = warp & 3;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
@@ -903,11 +1024,11 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     // share one): otherwise both softmaxes run at the same time, and then both wait for
     // the tensor pipe at the same time.
     uint64_t *turn = &turns[x * 4 + quad], *other_turn = &turns[(x ^ 1) * 4 + quad];
-    uint32_t turn_parity = (uint32_t)(x ^ 1), step_parity = 0, o_parity = 0;
+    uint32_t turn_parity = (uint32_t)(x ^ 1), step_parity = 0, l_parity = 1;
     bool ok = true;
-    for (int k = 0; ok; ++k) {
-      const WinPlan& pl = plans[k & 1];
-      if (!wait(&plan_full[k & 1], (uint32_t)(k >> 1) & 1u)) break;
+    for (RingAt<3> pr; ok; pr.next()) {
+      const WinPlan& pl = plans[pr.slot];
+      if (!wait(&plan_full[pr.slot], pr.parity)) break;
       const int to = pl.to;
       if (to < 0) break;
       const StepRanges r = pl.tile[x];
@@ -916,95 +1037,117 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       int cnt = 0;
       for (int i = pl.from; i < to; ++i, turn_parity ^= 1u) {
         if (!r.takes(i)) {
-          if (!(ok = wait(turn, turn_parity))) break;
-          if (lane == 0) mbar_arrive(other_turn);
+          if (!(ok = tmem_wait(turn, turn_parity, abort_flag))) break;
+          tmem_arrive(other_turn);
           continue;
         }
         //TR0
-        if (!(ok = wait(&s_full[x], step_parity))) break;
+        if (!(ok = tmem_wait(&s_full[x], step_parity, abort_flag))) break;
         tc_fence_after();
         //TR1
-        ok = r.whole(i) ? win_softmax<BF16, false>(s_addr, o_addr, a.scale_log2, see, 0, cnt, m, l, &s_free[x],
-                                                   &p_half[x], turn, turn_parity, other_turn, abort_flag)
-                        : win_softmax<BF16, true>(s_addr, o_addr, a.scale_log2, see, pl.key_tile(i) * 128, cnt, m, l,
-                                                  &s_free[x], &p_half[x], turn, turn_parity, other_turn, abort_flag);
+        ok = win_softmax<BF16>(s_addr, o_addr, a.scale_log2, see, r.whole(i), pl.key_tile(i) * 128, cnt, m, l, &s_free[x],
+                               &p_half[x], turn, turn_parity, other_turn, abort_flag);
         if (!ok) break;
         //TR2
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        tmem_arrive(&p_full[x]);
         step_parity ^= 1u;
         ++cnt;
       }
       if (!ok) break;
-      const int rows = pl.rows[x] - quad * 32;  // valid rows of this warp
-      const int64_t row0 = pl.row[x] + quad * 32;
-      uint16_t* dst = a.out + row0 * a.out_stride + (int64_t)(by_heads ? pl.head0 + x : pl.head0) * 128;
-      const int part = pl.part;
-      float* sums = nullptr;  // this warp's rows of a piece: O [32][128]
-      if (part >= 0) {
-        float* piece = a.pieces + (int64_t)part * kPieceFloats;
-        sums = piece + (x * 128 + quad * 32) * 128;
-        *reinterpret_cast<float2*>(piece + 2 * 128 * 128 + (x * 128 + quad * 32 + lane) * 2) = make_float2(m, l);
-      }
+      if (pl.part >= 0)
+        *reinterpret_cast<float2*>(a.pieces + (int64_t)pl.part * kPieceFloats + 2 * 128 * 128 +
+                                   (x * 128 + quad * 32 + lane) * 2) = make_float2(m, l);
       if (cnt > 0) {
-        if (!(ok = wait(&o_full[x], o_parity))) break;
-        o_parity ^= 1u;
+        if (!(ok = wait(&l_free[x], l_parity))) break;
+        l_parity ^= 1u;
+        rest.l[x][quad * 32 + lane] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_full[x]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&plan_free[pr.slot]);
+    }
+  } else {
+    // the outputs of both tiles, a row per thread in tensor memory
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWinOutRegs));
+    const int quad = warp & 3;
+    uint32_t parity[2] = {0, 0};
+    bool ok = true;
+    for (RingAt<3> pr; ok; pr.next()) {
+      const WinPlan& pl = plans[pr.slot];
+      if (!wait(&plan_full[pr.slot], pr.parity)) break;
+      if (pl.to < 0) break;
+      const int part = pl.part;
+#pragma unroll 1
+      for (int x = 0; x < 2 && ok; ++x) {
+        const uint32_t o_addr = tmem + ((uint32_t)(quad * 32) << 16) + 256 + (uint32_t)(x * 128);
+        const int rows = pl.rows[x] - quad * 32;  // valid rows of this warp
+        const int64_t row0 = pl.row[x] + quad * 32;
+        uint16_t* dst = a.out + row0 * a.out_stride + (int64_t)(by_heads ? pl.head0 + x : pl.head0) * 128;
+        float* sums = part < 0 ? nullptr : a.pieces + (int64_t)part * kPieceFloats + (x * 128 + quad * 32) * 128;
+        if (last_step(pl, x) < 0) {
+          if (part < 0) {
+            for (int e = 0; e < min(rows, 32) * 16; e += 32) {
+              const int row = (e + lane) >> 4;
+              if (row < rows)
+                *reinterpret_cast<uint4*>(dst + row * a.out_stride + ((e + lane) & 15) * 8) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          continue;
+        }
+        if (!(ok = wait(&l_full[x], parity[x]))) break;
+        const float l = rest.l[x][quad * 32 + lane], inv = l == 0.f ? 0.f : 1.0f / l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_free[x]);
+        if (!(ok = tmem_wait(&o_full[x], parity[x], abort_flag))) break;
+        parity[x] ^= 1u;
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t o[64];
-          tmem_ld32(o_addr + half * 64, H3B_S32(o, 0));
-          tmem_ld32(o_addr + half * 64 + 32, H3B_S32(o, 32));
-          tmem_wait_ld_dep(H3B_S32(o, 0));
-          reg_barrier32(H3B_S32(o, 32));
-          if (half == 1) {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c, o);
+          tmem_wait_ld_dep(o);
+          if (c == 96) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[x]);
+            tmem_arrive(&o_free[x]);
           }
-          uint4 u[8];
           if (part >= 0) {
+            uint4 u[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            for (int e = 0; e < 8; ++e) u[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            transpose_pieces<8>(u);
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                u[e] = make_uint4(o[q * 32 + 4 * e], o[q * 32 + 4 * e + 1], o[q * 32 + 4 * e + 2], o[q * 32 + 4 * e + 3]);
-              transpose_pieces(u);
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(sums + ((lane & 24) + e) * 128 + c + (lane & 7) * 4) = u[e];
+          } else {
+            uint4 u[4];
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<uint4*>(sums + ((lane & 24) + e) * 128 + half * 64 + q * 32 + (lane & 7) * 4) = u[e];
+            for (int e = 0; e < 4; ++e) {
+              u[e].x = pack2<BF16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+              u[e].y = pack2<BF16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+              u[e].z = pack2<BF16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+              u[e].w = pack2<BF16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
             }
-            continue;
-          }
+            transpose_pieces<4>(u);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            u[e].x = pack2<BF16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-            u[e].y = pack2<BF16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-            u[e].z = pack2<BF16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-            u[e].w = pack2<BF16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
-          }
-          transpose_pieces(u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int row = (lane & 24) + e;
-            if (row < rows)
-              *reinterpret_cast<uint4*>(dst + row * a.out_stride + half * 64 + (lane & 7) * 8) = u[e];
+            for (int e = 0; e < 4; ++e) {
+              const int row = (lane & 28) + e;
+              if (row < rows) *reinterpret_cast<uint4*>(dst + row * a.out_stride + c + (lane & 3) * 8) = u[e];
+            }
           }
         }
-        if (cleared[k & 1]) {
+        if (cleared[pr.slot]) {
           __syncwarp();
-          if (lane < rows)
+          if (lane < rows) {
+            const VisibleKeys see = visible_keys(a.rule, pl.p0[x] + quad * 32 + lane, pl.lk);
             add_nonfinite<BF16, PAGED>(a, pl, see, dst + lane * a.out_stride, part >= 0 ? sums + lane * 128 : nullptr);
-        }
-      } else if (part < 0) {
-        for (int e = 0; e < min(rows, 32) * 16; e += 32) {
-          const int row = (e + lane) >> 4;
-          if (row < rows) *reinterpret_cast<uint4*>(dst + row * a.out_stride + ((e + lane) & 15) * 8) = make_uint4(0, 0, 0, 0);
+          }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&plan_free[k & 1]);
+      if (lane == 0) mbar_arrive(&plan_free[pr.slot]);
     }
   }
 
@@ -1080,7 +1223,7 @@ bool make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, uint64_t d1, ui
 int64_t window_most_steps(const WindowArgs& a, int rows) {
   const int64_t keys = a.paged.k ? (int64_t)a.paged.width * a.paged.page : a.Tk;
   const int64_t span = (int64_t)a.rule.window + rows + (a.rule.chunk > 1 ? 2 * (int64_t)a.rule.chunk : 0);
-  const int64_t window = span < keys ? span / 128 + 2 : keys / 128 + 1;
+  const int64_t window = span < keys ? (span + 126) / 128 + 1 : (keys + 127) / 128;
   return window + (a.rule.sinks + 127) / 128;
 }
 
@@ -1115,8 +1258,11 @@ int launch_window(WindowArgs a, cudaStream_t s, cudaError_t* err) {
   const int64_t tiles = (int64_t)a.Tq / rows + a.seqs;  // sum of ceil(len / rows) is at most this
   const int64_t items = tiles * (by_heads ? a.Hq / 2 : a.Hq);
   if (items > INT_MAX / 2) return 4;
-  // Pieces need room, a second launch and a pass over their sums: only where some item can
-  // be long enough to be cut (a bound from what the host knows).
+  // Cutting takes a plan of all items by every CTA, a second launch and a pass over the
+  // pieces, together about five steps' time; dealing whole items leaves half an item's
+  // steps unbalanced on average.  So: where some item can have kCutFrom steps (a bound from
+  // what the host knows).  11 prompts of about 500 tokens, window 1,024: 97 us whole,
+  // 107 us cut; a 720p frame over four frames and a prefix: 1,103 us whole, 979 us cut.
   const bool cuts = a.pieces && window_most_steps(a, rows) >= kCutFrom && tiles <= kMaxTiles;
   if (!cuts) a.notes = nullptr;
   const int sms = num_sms() < kWinThreads ? num_sms() : kWinThreads;
