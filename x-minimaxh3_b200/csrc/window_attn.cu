@@ -397,7 +397,7 @@ constexpr int kItemCost = 4;
 constexpr int kCutFrom = 8;
 constexpr int kLeastPiece = 3;
 constexpr int kPieceFloats = 2 * 128 * 130;  // O [2][128][128], then (m, l) [2][128]
-constexpr int kMaxTiles = kWinSlots * kWinTile / 12 - 16;  // prefix sums of tiles and sequences that fit the ring
+constexpr int kMaxTiles = kWinSlots * kWinTile / 16 - kWinThreads;  // sums of tiles and sequences that fit the ring
 
 struct PieceNote {  // [CTA][2]: slot 1 a piece with the item's first step, slot 0 any other
   int state;        // 0: none, 1: more pieces follow, 2: the last
@@ -407,7 +407,7 @@ __host__ __device__ inline int64_t window_notes_bytes(int ctas) { return (int64_
 
 __device__ __forceinline__ int tiles_of(const WindowArgs& a, int seq, int rows_per_cta) {
   const RowRange r = row_range(a.q_starts, seq, a.Tq);
-  return (r.b - r.a + rows_per_cta - 1) / rows_per_cta;
+  return (r.b - r.a + rows_per_cta - 1) >> (rows_per_cta == 128 ? 7 : 8);  // 128 or 256
 }
 // A tile's sequence (-1: past the last tile) and its number in it.
 struct TileAt {
@@ -471,6 +471,29 @@ __device__ __forceinline__ void plan_tile(const WindowArgs& a, int seq, int t, i
 struct WorkAt {
   int item, step;
 };
+// Inclusive prefix sums of x[0, n) in shared memory, by the whole block (in loops: the code
+// runs once, from a cold instruction cache).
+__device__ __forceinline__ void block_prefix(long long* x, int n, long long* scan) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (n + kWinThreads - 1) / kWinThreads, first = (int)threadIdx.x * per, last = min(first + per, n);
+  long long sum = 0;
+#pragma unroll 1
+  for (int i = first; i < last; ++i) sum += x[i];
+  long long incl = sum;
+#pragma unroll 1
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  long long run = incl - sum;
+#pragma unroll
+  for (int w = 0; w < kWinThreads / 32; ++w) run += w < warp ? scan[w] : 0;
+#pragma unroll 1
+  for (int i = first; i < last; ++i) x[i] = run += x[i];
+  __syncthreads();
+}
 // What a CTA does: `rounds` whole items, then from bounds[0] to bounds[1].
 constexpr int kListed = 48;
 struct WorkShare {
@@ -611,27 +634,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     // Where no item is cut, all are dealt whole, in rounds.
     const bool cuts = a.notes != nullptr;
     // Else costs of all tiles, as prefix sums in the ring's memory.
-    long long* upto = reinterpret_cast<long long*>(smem + kWinOffRing);  // [tiles] from the last tile, per column
-    int* seq_upto = reinterpret_cast<int*>(upto + tiles);   // [seqs]: tiles of 0..i
-    // inclusive prefix sums of n values over the block: value(i) -> put(i, sum)
-    auto prefix = [&](int n, auto value, auto put) {
-      const int per = (n + kWinThreads - 1) / kWinThreads, first = (int)threadIdx.x * per;
-      long long sum = 0;
-      for (int i = first; i < min(first + per, n); ++i) sum += value(i);
-      long long incl = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      if (lane == 31) scan[warp] = incl;
-      __syncthreads();
-      long long run = incl - sum;
-#pragma unroll
-      for (int w = 0; w < kWinThreads / 32; ++w) run += w < warp ? scan[w] : 0;
-      for (int i = first; i < min(first + per, n); ++i) put(i, run += value(i));
-      __syncthreads();
-    };
     const int ctas = (int)gridDim.x, me = (int)blockIdx.x;
     if (!cuts) {
       if (threadIdx.x == 0) {
@@ -641,17 +643,23 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         work.bounds[0] = work.bounds[1] = {items, 0};
       }
     } else {
-      prefix(a.seqs, [&](int i) { return (long long)tiles_of(a, i, rows_per_cta); },
-             [&](int i, long long x) { seq_upto[i] = (int)x; });
-      const int valid = min(seq_upto[a.seqs - 1], tiles);  // more only where the starts overlap
+      long long* lack = reinterpret_cast<long long*>(smem + kWinOffRing);  // [CTAs]: share without the rounds' items
+      long long* seq_upto = lack + kWinThreads;                            // [seqs]: tiles of sequences 0..i
+      long long* upto = seq_upto + a.seqs;  // [tiles] from the last tile: cost of an item of each, summed
+      for (int i = (int)threadIdx.x; i < a.seqs; i += kWinThreads) seq_upto[i] = tiles_of(a, i, rows_per_cta);
+      __syncthreads();
+      block_prefix(seq_upto, a.seqs, scan);
+      const int valid = (int)min(seq_upto[a.seqs - 1], (long long)tiles);  // more only where the starts overlap
       auto locate = [&](int tile) {
         int lo = 0, hi = a.seqs - 1;
+#pragma unroll 1
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
           if (seq_upto[mid] > tile) hi = mid; else lo = mid + 1;
         }
-        return TileAt{lo, tile - (lo ? seq_upto[lo - 1] : 0)};
+        return TileAt{lo, tile - (lo ? (int)seq_upto[lo - 1] : 0)};
       };
+#pragma unroll 1
       for (int q = (int)threadIdx.x; q < valid; q += kWinThreads) {
         const TileAt at = locate(valid - 1 - q);
         const RowRange qr = row_range(a.q_starts, at.seq, a.Tq);
@@ -666,20 +674,18 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         upto[q] = union_keys(a.rule, lk - lq + first, lk - lq + min(first + rows_per_cta, lq) - 1, lk).steps + kItemCost;
       }
       __syncthreads();
-      prefix(valid, [&](int i) { return upto[i]; }, [&](int i, long long x) { upto[i] = x; });
+      block_prefix(upto, valid, scan);
       const int items = valid * columns;
       const long long all = valid ? upto[valid - 1] * columns : 0, share = (all + ctas - 1) / ctas;
-      auto cost = [&](int item) {
-        const int q = item / columns;
-        return upto[q] - (q ? upto[q - 1] : 0);
-      };
+      auto cost = [&](int q) { return upto[q] - (q ? upto[q - 1] : 0); };
       // whole rounds; a thread per CTA (the launch has at most kWinThreads)
       int rounds = 0, my_q = (int)threadIdx.x / columns, my_column = (int)threadIdx.x % columns;
       const int step_q = ctas / columns, step_column = ctas % columns;
       long long load = 0;
+#pragma unroll 1
       for (;; ++rounds) {
         const bool in = (rounds + 1) * ctas <= items;
-        const long long next = (int)threadIdx.x < ctas && in ? load + upto[my_q] - (my_q ? upto[my_q - 1] : 0) : 0;
+        const long long next = (int)threadIdx.x < ctas && in ? load + cost(my_q) : 0;
         if (!__syncthreads_and(in && next <= share)) break;
         load = next;
         my_q += step_q;
@@ -688,22 +694,26 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           ++my_q;
         }
       }
-      const int dealt = rounds * ctas;  // first item of the list
-      const int q0 = dealt / columns;
-      const long long begin = dealt >= items ? all : (q0 ? upto[q0 - 1] : 0) * columns + (dealt - q0 * columns) * cost(dealt);
-      // what the CTAs before this one lack, and this one
-      auto place = [&](long long at, int which) {
+      if ((int)threadIdx.x < ctas) lack[threadIdx.x] = share - load;
+      __syncthreads();
+      block_prefix(lack, ctas, scan);
+      if (threadIdx.x < 2) {
+        // from after what the CTAs before this one lack, to after what it lacks itself
+        const int i = me - 1 + (int)threadIdx.x, dealt = rounds * ctas, q0 = dealt / columns;
+        const long long at = dealt >= items ? all
+                                            : (q0 ? upto[q0 - 1] : 0) * columns + (dealt - q0 * columns) * cost(q0) +
+                                                  (i < 0 ? 0 : lack[i]);
         WorkAt w{items, 0};
-        at += begin;
         if (at < all) {
           int lo = 0, hi = valid - 1;  // the first tile that ends beyond `at`
+#pragma unroll 1
           while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (upto[mid] * columns > at) hi = mid; else lo = mid + 1;
           }
-          const long long first = lo ? upto[lo - 1] : 0;
-          const int worth = (int)(upto[lo] - first), steps = worth - kItemCost;
-          const long long in = at - first * columns;
+          // items of a tile are worth less than 2^31 together (the launcher sees to it)
+          const unsigned worth = (unsigned)cost(lo), in = (unsigned)(at - (lo ? upto[lo - 1] : 0) * columns);
+          const int steps = (int)worth - kItemCost;
           w.item = lo * columns + (int)(in / worth);
           w.step = max((int)(in % worth) - kItemCost, 0);
           const bool whole = steps < kCutFrom;  // the item may not be cut
@@ -714,22 +724,15 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             w.step = 0;
           }
         }
-        work.bounds[which] = w;
-      };
-      prefix(ctas, [&](int i) { return share - load; },  // thread i holds load i
-             [&](int i, long long x) {
-               if (i == me) place(x, 1);
-               if (i == me - 1) place(x, 0);
-               if (me == 0 && i == 0) place(0, 0);
-             });
-      const int sk = work.bounds[0].item / columns;
-      for (int e = (int)threadIdx.x; e < kListed; e += kWinThreads) {
-        const int q = e < rounds ? (me + e * ctas) / columns : sk + e - rounds;
-        work.tile[e] = q < valid ? locate(valid - 1 - q) : TileAt{-1, 0};
-      }
-      if (threadIdx.x == 0) {
+        work.bounds[threadIdx.x] = w;
         work.valid = valid;
         work.rounds = rounds;
+      }
+      __syncthreads();
+      const int dealt_tile = work.bounds[0].item / columns;
+      for (int e = (int)threadIdx.x; e < kListed; e += kWinThreads) {
+        const int q = e < rounds ? (me + e * ctas) / columns : dealt_tile + e - rounds;
+        work.tile[e] = q < valid ? locate(valid - 1 - q) : TileAt{-1, 0};
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring's loads come next
@@ -759,25 +762,25 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     PieceNote* notes = reinterpret_cast<PieceNote*>(a.notes) + 2 * blockIdx.x;
     if (a.notes && lane < 2) notes[lane].state = 0;
     __syncwarp();
-    // the plan of the next item, as far as there is one; made while one is loaded
-    RingAt<3> next;
+    // An item's plan is made when the loads of the one before it are under way: they are
+    // two steps ahead.
     int made = 0;
-    auto make_plan = [&]() -> bool {
-      WinPlan* pl = &plans[next.slot];
-      if (!wait(&plan_free[next.slot], next.parity ^ 1u)) return false;
+    for (RingAt<3> pr; ok; pr.next(), ++made) {
+      WinPlan* pl = &plans[pr.slot];
+      if (!wait(&plan_free[pr.slot], pr.parity ^ 1u)) break;
       const bool round = made < rounds;
       if (round || w.item < stop.item || (w.item == stop.item && w.step < stop.step)) {
         const int item = round ? (int)blockIdx.x + made * (int)gridDim.x : w.item, q = item / columns;
         const int entry = round ? made : rounds + q - dealt_tile;
-        TileAt at;
+        TileAt at_tile;
         if (a.notes && entry < kListed)
-          at = work.tile[entry];
+          at_tile = work.tile[entry];
         else
-          at = find_tile(a, work.valid - 1 - q, rows_per_cta);
+          at_tile = find_tile(a, work.valid - 1 - q, rows_per_cta);
         if (lane == 0) {
           WinPlan p{};  // past the last tile: nothing to visit, no row to write
           p.part = -1;
-          if (at.seq >= 0) plan_tile<PAGED>(a, at.seq, at.t, rows_per_cta, p);
+          if (at_tile.seq >= 0) plan_tile<PAGED>(a, at_tile.seq, at_tile.t, rows_per_cta, p);
           p.head0 = (item - q * columns) * (by_heads ? 2 : 1);
           p.kh = p.head0 / (a.Hq / a.Hkv);
           p.from = round ? 0 : w.step;
@@ -796,27 +799,17 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             notes[slot] = n;
           }
           *pl = p;
-          cleared[next.slot] = 0;
+          cleared[pr.slot] = 0;
         }
         if (!round) w = {w.item + 1, 0};
       } else if (lane == 0) {
         pl->to = -1;
       }
-      ++made;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&plan_full[next.slot]);
-      next.next();
-      return true;
-    };
-    ok = make_plan();
-    for (RingAt<3> pr; ok; pr.next()) {
-      const WinPlan* pl = &plans[pr.slot];
       const int from = pl->from, to = pl->to, sn = pl->sn, w0 = pl->w0, kh = pl->kh;
+      if (lane == 0) mbar_arrive(&plan_full[pr.slot]);
       if (to < 0) break;
-      if (from == to) {
-        ok = make_plan();
-        continue;
-      }
+      if (from == to) continue;
       if (!(ok = wait(q_empty, q_parity))) break;
       q_parity ^= 1u;
       if (lane == 0) mbar_arrive_expect_tx(q_full, 2 * kWinTile);
@@ -826,7 +819,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                     by_heads ? pl->head0 + (lane >> 1) : pl->head0, pl->row[lane >> 1]);
       __syncwarp();
       for (int i = 2 * from; i < 2 * to; ++i, at.next()) {
-        if (i == min(2 * from + 4, 2 * to - 1) && !(ok = make_plan())) break;  // the ring is full by now
         if (!(ok = wait(&empty[at.slot], at.parity ^ 1u))) break;
         const int n = i >> 1, j0 = (n < sn ? n : w0 + (n - sn)) * 128;
         const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
@@ -1263,7 +1255,8 @@ int launch_window(WindowArgs a, cudaStream_t s, cudaError_t* err) {
   // steps unbalanced on average.  So: where some item can have kCutFrom steps (a bound from
   // what the host knows).  11 prompts of about 500 tokens, window 1,024: 97 us whole,
   // 107 us cut; a 720p frame over four frames and a prefix: 1,103 us whole, 979 us cut.
-  const bool cuts = a.pieces && window_most_steps(a, rows) >= kCutFrom && tiles <= kMaxTiles;
+  const int64_t most = window_most_steps(a, rows);
+  const bool cuts = a.pieces && most >= kCutFrom && tiles <= kMaxTiles && (most + kItemCost) * items / tiles < INT_MAX;
   if (!cuts) a.notes = nullptr;
   const int sms = num_sms() < kWinThreads ? num_sms() : kWinThreads;
   const int64_t ctas = !cuts && items < sms ? items : sms;
