@@ -818,28 +818,37 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         tma_load_3d(smem + lane * (kWinTile / 2), &tmQ, q_full, (lane & 1) * 64,
                     by_heads ? pl->head0 + (lane >> 1) : pl->head0, pl->row[lane >> 1]);
       __syncwarp();
+      // The slab (page, kv head) of this lane's copy for a step's tiles: a copy per page and
+      // half of the channels.  Pages that no row needs, or that the table does not have, are
+      // read as zeros from outside the pool.  K and V of a step share it, and the next
+      // step's is fetched while this one's copies are issued.
+      auto slab_of = [&](int n) -> int {
+        const int nowhere = (int)(a.paged.pages * a.Hkv), j = (n < sn ? n : w0 + (n - sn)) * 128 + (lane >> 1) * box;
+        const int col = j / box;
+        if (lane >= 256 / box || j >= pl->lk || col >= a.paged.width) return nowhere;
+        const int pg = a.paged.table[(int64_t)pl->slot * a.paged.width + col];
+        return pg >= 0 && pg < a.paged.pages ? pg * a.Hkv + kh : nowhere;
+      };
+      int slab = 0, next_slab = 0;
+      if constexpr (PAGED) slab = slab_of(from);
       for (int i = 2 * from; i < 2 * to; ++i, at.next()) {
+        const int n = i >> 1;
+        if constexpr (PAGED) {
+          if (!(i & 1) && n + 1 < to) next_slab = slab_of(n + 1);
+        }
         if (!(ok = wait(&empty[at.slot], at.parity ^ 1u))) break;
-        const int n = i >> 1, j0 = (n < sn ? n : w0 + (n - sn)) * 128;
         const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
         uint8_t* dst = smem + kWinOffRing + at.slot * kWinTile;
         uint64_t* bar = &full[at.slot];
         if (lane == 0) mbar_arrive_expect_tx(bar, kWinTile);
         __syncwarp();
         if constexpr (PAGED) {
-          // a copy per page and half of the channels; pages that no row needs, or that the
-          // table does not have, are read as zeros from outside the pool
-          if (lane < 256 / box) {
-            const int half = lane & 1, j = j0 + (lane >> 1) * box, col = j / box;
-            int64_t z = a.paged.pages * a.Hkv;
-            if (j < pl->lk && col < a.paged.width) {
-              const int pg = a.paged.table[(int64_t)pl->slot * a.paged.width + col];
-              if (pg >= 0 && pg < a.paged.pages) z = (int64_t)pg * a.Hkv + kh;
-            }
-            tma_load_3d(dst + half * (kWinTile / 2) + (lane >> 1) * box * 128, tm, bar, half * 64, 0, (int)z);
-          }
+          if (lane < 256 / box)
+            tma_load_3d(dst + (lane & 1) * (kWinTile / 2) + (lane >> 1) * box * 128, tm, bar, (lane & 1) * 64, 0, slab);
+          if (i & 1) slab = next_slab;
         } else if (lane < 2) {
-          tma_load_3d(dst + lane * (kWinTile / 2), tm, bar, lane * 64, kh, pl->k_row + j0);
+          tma_load_3d(dst + lane * (kWinTile / 2), tm, bar, lane * 64, kh,
+                      pl->k_row + (n < sn ? n : w0 + (n - sn)) * 128);
         }
         __syncwarp();
       }
