@@ -427,8 +427,10 @@ typedef struct h3b_page_cache {
  * sequence).  Query rows outside every sequence are not written.
  * workspace: NULL, or h3b_window_workspace_bytes() bytes, 16-byte aligned and not shared
  * by calls on different streams, with which long rows of keys are divided over the
- * multiprocessors (the results differ in the last bits of the fp32 sums). */
-int64_t h3b_window_workspace_bytes(void);
+ * multiprocessors (the results differ in the last bits of the fp32 sums).  0: the call
+ * has no use for one.  keys: Tk, or table_width * page_tokens of a cache. */
+int64_t h3b_window_workspace_bytes(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, int64_t window,
+                                   int64_t sinks, int64_t chunk);
 int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                          int64_t v_row_stride, int dtype, int64_t Tq, int64_t Tk, const int32_t* query_starts,
                          const int32_t* key_starts, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t window,
@@ -444,9 +446,9 @@ int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, i
 
 /* Attention of one new token per sequence, the last of table row slots[i] (NULL: row i),
  * over a 16-bit cache of the queries' type or an e4m3 cache.  q, out: rows [seqs,
- * Hq * 128]; seqs <= 4096.  workspace: h3b_decode_workspace_bytes() bytes, 16-byte
- * aligned, not shared by calls on different streams. */
-int64_t h3b_decode_workspace_bytes(void);
+ * Hq * 128]; seqs <= 4096.  workspace: h3b_decode_workspace_bytes() bytes (0 for few
+ * short sequences: NULL), 16-byte aligned, not shared by calls on different streams. */
+int64_t h3b_decode_workspace_bytes(int64_t seqs, int64_t Hq, const h3b_page_cache* cache);
 int h3b_decode_attention(const void* q, int64_t q_row_stride, int dtype, const int32_t* slots, int64_t seqs, int64_t Hq,
                          const h3b_page_cache* cache, int64_t layer, int64_t window, int64_t sinks, float sm_scale,
                          void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream);

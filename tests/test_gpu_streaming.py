@@ -666,3 +666,27 @@ def test_window_backend_follows_the_request():
     ref, spread = attend(q, k, v, see)
     assert_close(out, ref, spread, L, 6.0)
     assert torch.equal(WindowAttentionB200(tokens=50)(q, k, v), window_attention(q, k, v, window=50))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_streaming_example(e4m3):
+    """Frame by frame over the cache is the whole sequence at once; forked continuations end where they should."""
+    import importlib.util
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("streaming_example", os.path.join(root, "examples", "streaming.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    r = example.stream(frames=4, tokens=200, e4m3=e4m3)
+    # the same sums in another division: two roundings to bf16 apart at most, P's and the output's
+    assert ((r["frames"].float() - r["whole"].float()).abs() <= 2.0 ** -6 * (r["whole"].float().abs() + 1)).all()
+    assert torch.isfinite(r["decoded"].float()).all() and r["decoded"].abs().amax() > 0
+    cache = r["cache"]
+    assert cache.lens.tolist() == [0] + [r["total"] + 10] * 3
+    used = cache.refs > 0
+    n = int(used.sum())
+    assert used[:n].all() and not used[n:].any()
+    # shared pages carry three references, the last pages of each continuation are its own
+    full = r["total"] // 64
+    assert cache.refs[cache.table[1, :full].long()].tolist() == [3] * full

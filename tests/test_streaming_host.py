@@ -33,7 +33,7 @@ def _window(q=D, qs=512, k=D, ks=256, v=D, vs=256, dtype=2, tq=8, tk=8, sq=None,
     (-2, dict(dtype=3)), (-1, dict(window=-1)), (-1, dict(sinks=-1)), (-1, dict(chunk=0)), (-1, dict(qs=504)),
     (-1, dict(qs=516)), (-1, dict(os=128)), (-1, dict(ks=128)), (-1, dict(vs=260)), (-2, dict(q=ODD)), (-2, dict(v=ODD)),
     (-2, dict(tq=1 << 31)), (-1, dict(tk=-1)), (-1, dict(tq=-1)), (-1, dict(seqs=2)), (-1, dict(sq=D)), (-1, dict(seqs=0)),
-    (-1, dict(ws=D, wsb=100)), (-2, dict(ws=ODD, wsb=1 << 40)), (0, dict(tq=0, q=None)),
+    (-1, dict(ws=D, wsb=100, tk=9000, window=9000)), (-2, dict(ws=ODD, wsb=1 << 40)), (0, dict(tq=0, q=None)),
 ])
 def test_window_entry_refuses(status, kw):
     assert _window(**kw) == status
@@ -63,12 +63,25 @@ def _decode(q=D, dtype=2, seqs=2, hq=4, cache=None, ws=D, wsb=1 << 40, window=4)
 
 
 @pytest.mark.parametrize("status,kw", [
-    (-1, dict(q=None)), (-2, dict(seqs=5000)), (-1, dict(ws=None)), (-1, dict(wsb=8)), (-2, dict(ws=ODD)),
+    (-1, dict(q=None)), (-2, dict(seqs=5000)), (-1, dict(ws=None, seqs=4000)), (-1, dict(wsb=8, seqs=4000)), (-2, dict(ws=ODD)),
     (-2, dict(dtype=1)), (-1, dict(hq=3)), (-1, dict(window=-2)), (-1, dict(cache=_cache(dtype=3, k_scale=16))),
     (0, dict(seqs=0)),
 ])
 def test_decode_entry_refuses(status, kw):
     assert _decode(**kw) == status
+
+
+def test_workspace_sizes():
+    L = lib()
+    assert L.h3b_window_workspace_bytes(8, 1, 4, 2, 896, 1 << 30, 0, 1) == 0          # seven tiles: items stay whole
+    assert L.h3b_window_workspace_bytes(8, 1, 4, 2, 9000, 128, 0, 1) == 0             # the window keeps them short
+    assert L.h3b_window_workspace_bytes(8, 1, 4, 2, 9000, 128, 4000, 1) != 0          # first tokens make them long
+    for bad in ((-1, 1, 4, 2, 9, 9, 0, 1), (8, 0, 4, 2, 9, 9, 0, 1), (8, 1, 4, 3, 9, 9, 0, 1), (8, 1, 4, 2, 9, 9, 0, 0)):
+        assert L.h3b_window_workspace_bytes(*bad) == -1
+    assert L.h3b_decode_workspace_bytes(2, 3, _cache()) == -1
+    assert L.h3b_decode_workspace_bytes(2, 4, None) == -1
+    # few pairs of short sequences need none where there is a GPU; none is known here or there are 148 processors
+    assert L.h3b_decode_workspace_bytes(4000, 4, _cache()) > 0
 
 
 def test_page_entries_refuse():

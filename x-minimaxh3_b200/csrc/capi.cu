@@ -617,7 +617,11 @@ int window_status(int r, cudaError_t e, const char* what) {
 
 }  // namespace
 
-int64_t h3b_window_workspace_bytes(void) { return h3b::window_workspace_bytes(); }
+int64_t h3b_window_workspace_bytes(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, int64_t window,
+                                   int64_t sinks, int64_t chunk) {
+  if (Tq < 0 || seqs < 1 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || keys < 0 || window < 0 || sinks < 0 || chunk < 1) return -1;
+  return h3b::window_workspace_bytes(Tq, seqs, Hq, Hkv, keys, {clip(window), clip(sinks), clip(chunk)});
+}
 
 int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                          int64_t v_row_stride, int dtype, int64_t Tq, int64_t Tk, const int32_t* query_starts,
@@ -634,7 +638,7 @@ int h3b_window_attention(const void* q, int64_t q_row_stride, const void* k, int
   if (Tk > 0 && (k_row_stride < Hkv * 128 || k_row_stride % 8 || v_row_stride < Hkv * 128 || v_row_stride % 8))
     return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: bad K/V row stride");
   if (!aligned16(k) || !aligned16(v)) return fail(H3B_ERR_UNSUPPORTED, "window_attention: K and V must be 16-byte aligned");
-  if (workspace && workspace_bytes < h3b::window_workspace_bytes())
+  if (workspace && workspace_bytes < h3b_window_workspace_bytes(Tq, seqs, Hq, Hkv, Tk, window, sinks, chunk))
     return fail(H3B_ERR_INVALID_ARGUMENT, "window_attention: workspace too small");
   if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "window_attention: workspace must be 16-byte aligned");
   h3b::WindowArgs a{};
@@ -675,7 +679,8 @@ int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, i
   if (seqs < 1 || seqs > (1 << 24)) return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: bad sizes");
   if (!query_starts && seqs != 1)
     return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: several sequences need query_starts");
-  if (workspace && workspace_bytes < h3b::window_workspace_bytes())
+  if (workspace && workspace_bytes < h3b_window_workspace_bytes(Tq, seqs, Hq, cache->kv_heads,
+                                                                cache->table_width * cache->page_tokens, window, sinks, chunk))
     return fail(H3B_ERR_INVALID_ARGUMENT, "paged_window_attention: workspace too small");
   if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "paged_window_attention: workspace must be 16-byte aligned");
   h3b::WindowArgs a{};
@@ -696,7 +701,10 @@ int h3b_paged_window_attention(const void* q, int64_t q_row_stride, int dtype, i
   return window_status(r, e, "paged_window_attention");
 }
 
-int64_t h3b_decode_workspace_bytes(void) { return h3b::decode_workspace_bytes(); }
+int64_t h3b_decode_workspace_bytes(int64_t seqs, int64_t Hq, const h3b_page_cache* cache) {
+  if (!cache || cache->kv_heads <= 0 || Hq <= 0 || Hq % cache->kv_heads) return -1;
+  return h3b::decode_workspace_bytes(seqs, Hq, cache->kv_heads, cache->table_width * cache->page_tokens);
+}
 
 int h3b_decode_attention(const void* q, int64_t q_row_stride, int dtype, const int32_t* slots, int64_t seqs, int64_t Hq,
                          const h3b_page_cache* cache, int64_t layer, int64_t window, int64_t sinks, float sm_scale,
@@ -711,7 +719,8 @@ int h3b_decode_attention(const void* q, int64_t q_row_stride, int dtype, const i
     return fail(H3B_ERR_UNSUPPORTED, "decode_attention: the cache must hold the queries' type or e4m3");
   if (seqs > h3b::kDecodeMaxSeqs) return fail(H3B_ERR_UNSUPPORTED, "decode_attention: more than 4096 sequences in a call");
   if (seqs * Hq > INT_MAX) return fail(H3B_ERR_UNSUPPORTED, "decode_attention: too many heads");
-  if (!workspace || workspace_bytes < h3b::decode_workspace_bytes())
+  const int64_t need = h3b_decode_workspace_bytes(seqs, Hq, cache);
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(H3B_ERR_INVALID_ARGUMENT, "decode_attention: workspace too small");
   if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "decode_attention: workspace must be 16-byte aligned");
   h3b::DecodeArgs a{};

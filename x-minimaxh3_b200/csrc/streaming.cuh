@@ -108,10 +108,10 @@ struct WindowArgs {
   void* notes;      // of cut items and their pieces (set by the launcher; null: none is cut)
   float* pieces;
 };
-// bf16: bfloat16, else float16.  workspace: null, or window_workspace_bytes() with which
-// long items are cut.  0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err), 3 the
+// bf16: bfloat16, else float16.  workspace: null, or window_workspace_bytes() (0 where it
+// would not be used) with which long items are cut; keys: all, or what a table row names.  0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err), 3 the
 // kernel's register count is not the planned one, 4 too many tiles
-int64_t window_workspace_bytes();
+int64_t window_workspace_bytes(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, const WindowRule& r);
 int launch_window_attention(WindowArgs a, bool bf16, void* workspace, cudaStream_t s, cudaError_t* err);
 
 struct DecodeArgs {
@@ -129,7 +129,8 @@ struct DecodeArgs {
   int workers;
 };
 constexpr int kDecodeMaxSeqs = 4096;
-int64_t decode_workspace_bytes();
+// capacity: tokens that a table row can name
+int64_t decode_workspace_bytes(int64_t seqs, int64_t Hq, int64_t Hkv, int64_t capacity);
 // kind 0: bf16 cache, 1: fp16 cache, 2: E4M3 cache with bf16 q, 3: E4M3 cache with fp16 q
 cudaError_t launch_decode_attention(DecodeArgs a, int kind, cudaStream_t s);
 

@@ -1220,12 +1220,18 @@ bool make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, uint64_t d1, ui
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// most key tiles that any item can visit
-int64_t window_most_steps(const WindowArgs& a, int rows) {
-  const int64_t keys = a.paged.k ? (int64_t)a.paged.width * a.paged.page : a.Tk;
-  const int64_t span = (int64_t)a.rule.window + rows + (a.rule.chunk > 1 ? 2 * (int64_t)a.rule.chunk : 0);
-  const int64_t window = span < keys ? (span + 126) / 128 + 1 : (keys + 127) / 128;
-  return window + (a.rule.sinks + 127) / 128;
+// Whether items are cut.  Cutting takes a plan of all items by every CTA, a second launch
+// and a pass over the pieces, together about five steps' time; dealing whole items leaves
+// half an item's steps unbalanced on average.  So: where some item can have kCutFrom steps
+// (a bound from what the host knows).  A 720p frame over four frames and a prefix: 1,103 us
+// whole, 979 us cut; 11 prompts of about 500 tokens, window 1,024: 117 us whole, 108 cut.
+// keys: all of them, or what a table row can name.
+bool window_cuts(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, const WindowRule& r) {
+  const bool by_heads = (Hq / Hkv) % 2 == 0;
+  const int64_t rows = by_heads ? 128 : 256, columns = by_heads ? Hq / 2 : Hq, tiles = Tq / rows + seqs;
+  const int64_t span = (int64_t)r.window + rows + (r.chunk > 1 ? 2 * (int64_t)r.chunk : 0);
+  const int64_t most = (span < keys ? (span + 126) / 128 + 1 : (keys + 127) / 128) + (r.sinks + 127) / 128;
+  return most >= kCutFrom && tiles <= kMaxTiles && (most + kItemCost) * columns < INT_MAX;
 }
 
 template <bool BF16, bool PAGED>
@@ -1259,13 +1265,8 @@ int launch_window(WindowArgs a, cudaStream_t s, cudaError_t* err) {
   const int64_t tiles = (int64_t)a.Tq / rows + a.seqs;  // sum of ceil(len / rows) is at most this
   const int64_t items = tiles * (by_heads ? a.Hq / 2 : a.Hq);
   if (items > INT_MAX / 2) return 4;
-  // Cutting takes a plan of all items by every CTA, a second launch and a pass over the
-  // pieces, together about five steps' time; dealing whole items leaves half an item's
-  // steps unbalanced on average.  So: where some item can have kCutFrom steps (a bound from
-  // what the host knows).  11 prompts of about 500 tokens, window 1,024: 97 us whole,
-  // 107 us cut; a 720p frame over four frames and a prefix: 1,103 us whole, 979 us cut.
-  const int64_t most = window_most_steps(a, rows);
-  const bool cuts = a.pieces && most >= kCutFrom && tiles <= kMaxTiles && (most + kItemCost) * items / tiles < INT_MAX;
+  const bool cuts = a.pieces && window_cuts(a.Tq, a.seqs, a.Hq, a.Hkv,
+                                           PAGED ? (int64_t)a.paged.width * a.paged.page : a.Tk, a.rule);
   if (!cuts) a.notes = nullptr;
   const int sms = num_sms() < kWinThreads ? num_sms() : kWinThreads;
   const int64_t ctas = !cuts && items < sms ? items : sms;
@@ -1277,7 +1278,8 @@ int launch_window(WindowArgs a, cudaStream_t s, cudaError_t* err) {
 
 }  // namespace
 
-int64_t window_workspace_bytes() {
+int64_t window_workspace_bytes(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, const WindowRule& r) {
+  if (!window_cuts(Tq, seqs, Hq, Hkv, keys, r)) return 0;
   const int sms = num_sms();
   return window_notes_bytes(sms) + (int64_t)sms * 2 * kPieceFloats * 4;
 }

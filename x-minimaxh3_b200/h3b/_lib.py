@@ -113,14 +113,14 @@ _SIGNATURES = {
     "h3b_bitmap_to_lut": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
     "h3b_attention": [c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
                       c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p],
-    "h3b_window_workspace_bytes": [],
+    "h3b_window_workspace_bytes": [c_int64] * 8,
     "h3b_window_attention": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p,
                              c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
                              c_int64, c_void_p, c_int64, c_void_p],
     "h3b_paged_window_attention": [c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, _cache_p,
                                    c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_int64,
                                    c_void_p],
-    "h3b_decode_workspace_bytes": [],
+    "h3b_decode_workspace_bytes": [c_int64, c_int64, _cache_p],
     "h3b_decode_attention": [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, _cache_p, c_int64, c_int64, c_int64,
                              c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p],
     "h3b_pages_workspace_bytes": [c_int64, c_int64],

@@ -27,7 +27,6 @@ import torch
 from . import context as _context
 from ._lib import check, lib
 from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _ptr, _stream, _token_rows
-from .ops import _cuda
 
 UNLIMITED = 1 << 30
 
@@ -67,9 +66,9 @@ def _workspace(workspace: torch.Tensor | None, need: int, q: torch.Tensor) -> to
     return workspace
 
 
-def _window_workspace(workspace: torch.Tensor | None, q: torch.Tensor) -> tuple[torch.Tensor, int]:
-    need = lib().h3b_window_workspace_bytes()
-    return _workspace(workspace, need, q), need
+def _window_workspace(workspace, q, seqs, kv_heads, keys, rule) -> tuple[torch.Tensor | None, int]:
+    need = lib().h3b_window_workspace_bytes(q.shape[0], seqs, q.shape[1], kv_heads, keys, *rule)
+    return (_workspace(workspace, need, q), need) if need > 0 else (None, 0)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
@@ -81,7 +80,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     query_starts / key_starts: int32 [sequences + 1] first rows of each sequence of a
     ragged batch (from 0 to Tq / Tk); None: one sequence.  workspace: uint8, reused by
     calls on one stream."""
-    _cuda("window_attention", q, k, v)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise RuntimeError("window_attention runs only on CUDA tensors (the B200 library has no CPU path)")
     q, k, v = _token_rows(q, None, "q"), _token_rows(k, None, "k"), _token_rows(v, None, "v")
     if k.shape != v.shape or not q.dtype is k.dtype is v.dtype:
         raise ValueError("k and v must have one shape, and q their type")
@@ -97,7 +97,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         if seqs < 1:
             raise ValueError("query_starts needs at least two entries")
     out = _output(out, q)
-    workspace, size = _window_workspace(workspace, q)
+    workspace, size = _window_workspace(workspace, q, seqs, k.shape[1], k.shape[0], (window, sinks, chunk))
     check(lib().h3b_window_attention(_ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), DTYPE_CODES[q.dtype],
                                      q.shape[0], k.shape[0], _ptr(query_starts), _ptr(key_starts), seqs, q.shape[1],
                                      k.shape[1], window, sinks, chunk, _scale(scale), _ptr(out), out.stride(0),
@@ -106,9 +106,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
 
 
 def _cached_queries(q: torch.Tensor, cache: PagedKVCache, layer: int, what: str) -> torch.Tensor:
-    _cuda(what, q)
+    if not q.is_cuda:
+        raise RuntimeError(f"{what} runs only on CUDA tensors (the B200 library has no CPU path)")
     q = _token_rows(q, None, "q")
-    if q.shape[1] == 0 or q.shape[1] % cache.k.shape[2]:
+    heads = q.shape[1]
+    if heads == 0 or heads % cache.kv_heads:
         raise ValueError("the query heads must be a multiple of the kv heads")
     if not 0 <= layer < cache.k.shape[0]:
         raise ValueError(f"the cache has no layer {layer}")
@@ -133,7 +135,8 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
     elif seqs > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
     out = _output(out, q)
-    workspace, size = _window_workspace(workspace, q)
+    workspace, size = _window_workspace(workspace, q, seqs, cache.kv_heads, cache.table.shape[1] * cache.page_tokens,
+                                        (window, sinks, chunk))
     check(lib().h3b_paged_window_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], q.shape[0], _ptr(query_starts),
                                            _ptr(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
                                            _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), size, _stream(q)),
@@ -155,8 +158,9 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
         _index(slots, "slots", n)
     elif n > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
-    need = lib().h3b_decode_workspace_bytes()
-    workspace = _workspace(workspace, need, q)
+    need = lib().h3b_decode_workspace_bytes(n, q.shape[1], cache._ref)
+    if need:
+        workspace = _workspace(workspace, need, q)
     out = _output(out, q)
     check(lib().h3b_decode_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], _ptr(slots), n, q.shape[1], cache._ref,
                                      layer, window, sinks, _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), need,
