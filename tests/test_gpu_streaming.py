@@ -351,14 +351,17 @@ def test_paged_window_unseen_pages_are_not_needed():
 @pytest.mark.parametrize("page", [16, 64, 128])
 @pytest.mark.parametrize("dtype,store", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
                                          (torch.bfloat16, "e4m3"), (torch.float16, "e4m3")], ids=str)
-@pytest.mark.parametrize("heads", [(1, 1), (8, 2), (5, 5), (24, 2), (32, 2), (20, 1), (16, 2)], ids=str)
-def test_decode_attention(page, dtype, store, heads):
+@pytest.mark.parametrize("heads", [(1, 1), (8, 2), (5, 5), (24, 2), (32, 2), (20, 1), (16, 2), (3, 1), (14, 2)], ids=str)
+@pytest.mark.parametrize("room", [0, 20000])
+def test_decode_attention(page, dtype, store, heads, room):
+    """room: tokens that the table could name beyond the lengths; with much of it, and with many pairs, the
+    chunks of all sequences are dealt out over the grid, else a cluster serves each pair."""
     from h3b import decode_attention
 
     hq, hkv = heads
     g = _gen(page + hq)
     lens = [1, 15, 16, 17, 0, 130, 1000, 333, 64, 2500]
-    cache = _cache(g, lens, page, hkv, store, layers=2)
+    cache = _cache(g, lens, page, hkv, store, layers=2, extra=room)
     slots = [9, 0, 3, 4, 2, 8, 1, 7, 5, 6]
     q = _rand(g, len(slots), hq, D, dtype=dtype, scale=1.5)
     host = HostCache(cache)
@@ -386,6 +389,27 @@ def test_decode_one_long_sequence(store):
     work = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
     assert torch.equal(decode_attention(q, cache, workspace=work), out)
     assert torch.equal(decode_attention(q, cache, workspace=work), out)
+
+
+@pytest.mark.parametrize("store", [torch.bfloat16, "e4m3"], ids=str)
+@pytest.mark.parametrize("heads", [(3, 1), (14, 2), (24, 8), (16, 1)], ids=str)
+def test_decode_many_short_sequences(store, heads):
+    """More pairs than warps have parts: most are one warp's, some are joined, some are empty."""
+    from h3b import decode_attention
+
+    hq, hkv = heads
+    g = _gen(hq)
+    rng = np.random.RandomState(hq)
+    lens = [int(x) for x in rng.choice([0, 1, 7, 16, 40, 130, 400, 1500], 310)]
+    cache = _cache(g, lens, 16, hkv, store)
+    q = _rand(g, len(lens), hq, D, dtype=torch.bfloat16, scale=1.5)
+    out = decode_attention(q, cache, window=700, sinks=9)
+    host = HostCache(cache)
+    for i, n in enumerate(lens):
+        k, v = host.rows(i)
+        see = visible(1, n, 700, 9, 1, "cuda") if n else torch.zeros(1, 0, dtype=torch.bool, device="cuda")
+        ref, spread = attend(q[i:i + 1], k, v, see)
+        assert_close(out[i:i + 1], ref, spread, n, 14.0, f"sequence {i} of {n}")
 
 
 def test_decode_extreme_queries_of_an_8_bit_cache():

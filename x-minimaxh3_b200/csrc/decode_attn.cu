@@ -466,6 +466,7 @@ __global__ void __launch_bounds__(kDecodeThreads, MINB) decode_kernel(DecodeArgs
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = t * 8 + 2 * c + e;
+          if (r0 + r >= group) continue;
 #pragma unroll
           for (int i = 0; i < 8; i += 2)
             *reinterpret_cast<float4*>(rows + r * 128 + tile_channel<FP8>(i)) =
@@ -563,96 +564,85 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDecodeThread
 }
 
 // Joins the partial sums of a (kv head, row group): out = sum_p 2^(m_p - M) O_p /
-// sum_p 2^(m_p - M) l_p.  A block per pair, its warps shared out over the rows and over
-// the parts of a row, four channels per lane; the order of the sums is that of the keys
-// for a given split.  Pairs that one warp finished are left alone; pairs without any
-// visible key give 0.
-constexpr int kJoinThreads = 512;
+// sum_p 2^(m_p - M) l_p.  A block per pair, its warps shared out over the rows and, where
+// there are more of them, over the parts of a row; four channels per lane.  Pairs that one
+// warp finished are left alone; pairs without any visible key give 0.  Blocks of 128
+// threads where there are many pairs, of 512 where few pairs have many parts each.
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(DecodeArgs a) {
-  __shared__ float4 acc_s[kJoinThreads];
-  __shared__ float2 stat_s[kJoinThreads / 32];
+__global__ void __launch_bounds__(512) decode_join_kernel(DecodeArgs a) {
+  __shared__ float4 acc_s[512];
+  __shared__ float2 stat_s[16];
   const int group = a.Hq / a.Hkv, groups = (group + NT * 8 - 1) / (NT * 8), heads = a.Hkv * groups;
   const int b = blockIdx.x / heads, hp = blockIdx.x % heads;
   const int kh = hp / groups, first = (hp % groups) * NT * 8, rows = min(group - first, NT * 8);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int splits = (kJoinThreads / 32) / rows, r = warp % rows, split = warp / rows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int splits = max(warps / rows, 1), split = warp / rows;
   chain_next();
   chain_wait();
   const int64_t* prefix = reinterpret_cast<const int64_t*>(a.partial);
-  const int64_t share = prefix[kDecodeMaxSeqs + 1], before = prefix[b];
-  const int64_t n = prefix[b + 1] - before;
-  uint16_t* dst = a.out + b * a.out_stride + ((int64_t)kh * group + first + r) * 128 + lane * 4;
-  if (n == 0) {
-    if (split == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
-    return;
-  }
+  const int64_t share = prefix[kDecodeMaxSeqs + 1], before = prefix[b], n = prefix[b + 1] - before;
   const int64_t s0 = before * heads + hp * n, s1 = s0 + n;
-  const int64_t w0 = s0 / share, w1 = (s1 - 1) / share;
-  if (w0 == w1) return;
+  const int64_t w0 = n ? s0 / share : 0, w1 = n ? (s1 - 1) / share : 0;
+  if ((n && w0 == w1) || (splits == 1 && split > 0)) return;
   const int parts = (int)(w1 - w0 + 1);
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (split < splits) {
-    // only the first part can lie in its worker's second slot: a later worker begins in the pair
-    const int head_slot = w0 * share >= s0 ? 0 : 1;
-    for (int p0 = split; p0 < parts; p0 += 8 * splits) {
-      float2 st[8];
-      float4 x[8];
+  // only the first part can lie in its worker's second slot: a later worker begins in the pair
+  const int head_slot = n && w0 * share < s0 ? 1 : 0;
+  for (int r = warp % rows; r < rows; r += warps) {  // once, unless there are more rows than warps
+    uint16_t* dst = a.out + b * a.out_stride + ((int64_t)kh * group + first + r) * 128 + lane * 4;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (split < splits && n) {
+      for (int p0 = split; p0 < parts; p0 += 4 * splits) {
+        float2 st[4];
+        float4 x[4];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int p = p0 + u * splits;
-        const bool in = p < parts;
-        const int64_t w = w0 + (in ? p : 0);
-        const int slot = p == 0 ? head_slot : 0;
-        st[u] = in ? *reinterpret_cast<const float2*>(partial_stats<NT>(a.partial, a.workers, w, slot) + r * 2)
-                   : make_float2(-INFINITY, 0.f);
-        x[u] = in ? *reinterpret_cast<const float4*>(partial_rows<NT>(a.partial, w, slot) + r * 128 + lane * 4)
-                  : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float mx = m;
+        for (int u = 0; u < 4; ++u) {
+          const int p = p0 + u * splits;
+          const bool in = p < parts;
+          const int64_t w = w0 + (in ? p : 0);
+          const int slot = p == 0 ? head_slot : 0;
+          st[u] = in ? *reinterpret_cast<const float2*>(partial_stats<NT>(a.partial, a.workers, w, slot) + r * 2)
+                     : make_float2(-INFINITY, 0.f);
+          x[u] = in ? *reinterpret_cast<const float4*>(partial_rows<NT>(a.partial, w, slot) + r * 128 + lane * 4)
+                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float mx = m;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) mx = fmaxf(mx, st[u].x);
-      const float base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base);
-      m = mx;
-      l *= keep;
-      acc.x *= keep;
-      acc.y *= keep;
-      acc.z *= keep;
-      acc.w *= keep;
+        for (int u = 0; u < 4; ++u) mx = fmaxf(mx, st[u].x);
+        const float base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base);
+        m = mx;
+        l *= keep;
+        acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float w = exp2f(st[u].x - base);
-        l = fmaf(w, st[u].y, l);
-        acc.x = fmaf(w, x[u].x, acc.x);
-        acc.y = fmaf(w, x[u].y, acc.y);
-        acc.z = fmaf(w, x[u].z, acc.z);
-        acc.w = fmaf(w, x[u].w, acc.w);
+        for (int u = 0; u < 4; ++u) {
+          const float w = exp2f(st[u].x - base);
+          l = fmaf(w, st[u].y, l);
+          acc = make_float4(fmaf(w, x[u].x, acc.x), fmaf(w, x[u].y, acc.y), fmaf(w, x[u].z, acc.z), fmaf(w, x[u].w, acc.w));
+        }
       }
     }
+    if (splits > 1) {  // then rows <= warps / 2, and every warp passes here once
+      acc_s[threadIdx.x] = acc;
+      if (lane == 0) stat_s[warp] = make_float2(m, l);
+      __syncthreads();
+      if (split > 0) return;
+      const float own = m;
+      for (int i = 1; i < splits; ++i) m = fmaxf(m, stat_s[r + i * rows].x);
+      const float base = m == -INFINITY ? 0.f : m, keep = exp2f(own - base);
+      l *= keep;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+      for (int i = 1; i < splits; ++i) {
+        const float2 st = stat_s[r + i * rows];
+        const float4 x = acc_s[(r + i * rows) * 32 + lane];
+        const float w = exp2f(st.x - base);
+        l = fmaf(w, st.y, l);
+        acc = make_float4(fmaf(w, x.x, acc.x), fmaf(w, x.y, acc.y), fmaf(w, x.z, acc.z), fmaf(w, x.w, acc.w));
+      }
+    }
+    const float inv = (l == 0.f ? 0.f : 1.f / l) * (a.v_scale ? a.v_scale[kh] : 1.f);
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
   }
-  acc_s[threadIdx.x] = acc;
-  if (lane == 0) stat_s[warp] = make_float2(m, l);
-  __syncthreads();
-  if (split > 0) return;
-  float mx = -INFINITY;
-  for (int i = 0; i < splits; ++i) mx = fmaxf(mx, stat_s[r + i * rows].x);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float total = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < splits; ++i) {
-    const float2 st = stat_s[r + i * rows];
-    const float4 x = acc_s[(r + i * rows) * 32 + lane];
-    const float w = exp2f(st.x - base);
-    total = fmaf(w, st.y, total);
-    acc.x = fmaf(w, x.x, acc.x);
-    acc.y = fmaf(w, x.y, acc.y);
-    acc.z = fmaf(w, x.z, acc.z);
-    acc.w = fmaf(w, x.w, acc.w);
-  }
-  const float inv = (total == 0.f ? 0.f : 1.f / total) * (a.v_scale ? a.v_scale[kh] : 1.f);
-  *reinterpret_cast<uint2*>(dst) =
-      make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
 }
 
 constexpr int kMinBlocks = 4;  // most blocks an SM runs in any variant (sizes the workspace)
@@ -688,7 +678,8 @@ cudaError_t launch_decode(DecodeArgs a, cudaStream_t s) {
   const size_t smem = (size_t)(a.seqs + 1) * 8;
   const cudaError_t e = launch_chained(decode_kernel<BF16, FP8, NT, MINB>, blocks, kDecodeThreads, smem, s, a);
   if (e != cudaSuccess) return e;
-  return launch_chained(decode_join_kernel<BF16, NT>, a.seqs * heads, kJoinThreads, 0, s, a);
+  const int64_t pairs = a.seqs * heads;
+  return launch_chained(decode_join_kernel<BF16, NT>, pairs, pairs >= 2 * sms ? 128 : 512, 0, s, a);
 }
 
 }  // namespace
