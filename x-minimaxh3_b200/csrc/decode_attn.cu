@@ -111,242 +111,242 @@ __device__ __forceinline__ void decode_chunks(const DecodeArgs& a, int b, int sl
                                               const ChunkList& cl, int kh, int r0, int c0, int c1, float (&o)[NT][8][4],
                                               float (&m)[NT][2], float (&l)[NT][2]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, group = a.Hq / a.Hkv;
-      // Q of head r0 + 8 t + g: the channels this thread's K loads bring
-      uint32_t qf[NT][8][2];
-      float sc[NT][2];
-  #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int r = r0 + t * 8 + g;
-        const uint16_t* qp = a.q + b * a.q_stride + ((int64_t)kh * group + r) * 128;
-        uint4 w[4];
-  #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // 16-bit: channels 32 i + 8 c + 0..7; E4M3: 64 (i / 2) + 16 c + 8 (i % 2) + 0..7
-          const int d = FP8 ? (i >> 1) * 64 + c * 16 + (i & 1) * 8 : i * 32 + c * 8;
-          w[i] = r < group ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
-        }
-        float up = 1.f;
-        if constexpr (FP8 && BF16) {
-          // bf16 q -> fp16 under a power of two: the head's largest |q| comes to [1, 2)
-          float mx = 0.f;
-  #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-  #pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(ws[e])), fabsf(bf16_hi(ws[e]))));
-          }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const int ex = (int)(__float_as_uint(mx) >> 23) - 127;  // of a normal, finite maximum
-          float down = 1.f;
-          if (mx > 0.f && ex > -126 && ex < 127) {
-            up = __uint_as_float((uint32_t)(ex + 127) << 23);
-            down = __uint_as_float((uint32_t)(127 - ex) << 23);
-          }
-  #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t* ws = reinterpret_cast<uint32_t*>(&w[i]);
-  #pragma unroll
-            for (int e = 0; e < 4; ++e) ws[e] = pack16<false>(bf16_lo(ws[e]) * down, bf16_hi(ws[e]) * down);
-          }
-        }
-  #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qf[t][2 * i][0] = w[i].x;
-          qf[t][2 * i][1] = w[i].y;
-          qf[t][2 * i + 1][0] = w[i].z;
-          qf[t][2 * i + 1][1] = w[i].w;
-        }
-        const float s = a.scale_log2 * (FP8 ? a.k_scale[kh] : 1.f);
-        // the score columns of this thread are heads 2c and 2c + 1 of the tile
-        sc[t][0] = s * __shfl_sync(0xffffffffu, up, 8 * c);
-        sc[t][1] = s * __shfl_sync(0xffffffffu, up, 8 * c + 4);
+  // Q of head r0 + 8 t + g: the channels this thread's K loads bring
+  uint32_t qf[NT][8][2];
+  float sc[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + t * 8 + g;
+    const uint16_t* qp = a.q + b * a.q_stride + ((int64_t)kh * group + r) * 128;
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // 16-bit: channels 32 i + 8 c + 0..7; E4M3: 64 (i / 2) + 16 c + 8 (i % 2) + 0..7
+      const int d = FP8 ? (i >> 1) * 64 + c * 16 + (i & 1) * 8 : i * 32 + c * 8;
+      w[i] = r < group ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
+    }
+    float up = 1.f;
+    if constexpr (FP8 && BF16) {
+      // bf16 q -> fp16 under a power of two: the head's largest |q| comes to [1, 2)
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(ws[e])), fabsf(bf16_hi(ws[e]))));
       }
-
-  #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-  #pragma unroll
-        for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
-        m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.f;
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const int ex = (int)(__float_as_uint(mx) >> 23) - 127;  // of a normal, finite maximum
+      float down = 1.f;
+      if (mx > 0.f && ex > -126 && ex < 127) {
+        up = __uint_as_float((uint32_t)(ex + 127) << 23);
+        down = __uint_as_float((uint32_t)(127 - ex) << 23);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* ws = reinterpret_cast<uint32_t*>(&w[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ws[e] = pack16<false>(bf16_lo(ws[e]) * down, bf16_hi(ws[e]) * down);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      qf[t][2 * i][0] = w[i].x;
+      qf[t][2 * i][1] = w[i].y;
+      qf[t][2 * i + 1][0] = w[i].z;
+      qf[t][2 * i + 1][1] = w[i].w;
+    }
+    const float s = a.scale_log2 * (FP8 ? a.k_scale[kh] : 1.f);
+    // the score columns of this thread are heads 2c and 2c + 1 of the tile
+    sc[t][0] = s * __shfl_sync(0xffffffffu, up, 8 * c);
+    sc[t][1] = s * __shfl_sync(0xffffffffu, up, 8 * c + 4);
+  }
 
-      constexpr int kEB = FP8 ? 1 : 2;  // bytes per element
-      constexpr int kKL = FP8 ? 2 : 4;  // 16-byte loads of a key row per thread
-      constexpr int kVL = FP8 ? 1 : 2;
-      constexpr int CH = FP8 ? 2 : 1;   // chunks of a step: 8 KB of K and V under way per warp either way
-      uint4 kr[CH][2][kKL], vr[CH][4][kVL];
-      int pgs = 0, pbase = c0 - 64;
-      auto chunk_of = [&](int ord) { return ord < cl.first_n ? ord : ord - cl.first_n + cl.win; };
-      // byte offset of key row 0 of chunk ordinal `ord`; page numbers come 32 chunks at a
-      // time (an ordinal past the piece stands for its last)
-      auto offset_of = [&](int ord) -> int64_t {
-        if (ord - pbase >= 32) {
-          pbase = ord;
-          const int o2 = min(ord + lane, c1 - 1);
-          pgs = (int)paged_page(a.paged, slot, chunk_of(o2) * kChunk / a.paged.page);
-        }
-        const int64_t pg = __shfl_sync(0xffffffffu, pgs, ord - pbase);
-        const int j = chunk_of(min(ord, c1 - 1)) * kChunk;
-        return ((pg * a.Hkv + kh) * a.paged.page + (j & (a.paged.page - 1))) * (int64_t)(128 * kEB);
-      };
-      auto load_k = [&](const int64_t (&off)[CH]) {
-  #pragma unroll
-        for (int u = 0; u < CH; ++u) {
-          const uint8_t* p = static_cast<const uint8_t*>(a.paged.k) + off[u] + g * (128 * kEB) + c * 16;
-  #pragma unroll
-          for (int i = 0; i < kKL; ++i) {
-            kr[u][0][i] = ld_stream(p + i * 64);
-            kr[u][1][i] = ld_stream(p + i * 64 + 8 * 128 * kEB);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+  }
+
+  constexpr int kEB = FP8 ? 1 : 2;  // bytes per element
+  constexpr int kKL = FP8 ? 2 : 4;  // 16-byte loads of a key row per thread
+  constexpr int kVL = FP8 ? 1 : 2;
+  constexpr int CH = FP8 ? 2 : 1;   // chunks of a step: 8 KB of K and V under way per warp either way
+  uint4 kr[CH][2][kKL], vr[CH][4][kVL];
+  int pgs = 0, pbase = c0 - 64;
+  auto chunk_of = [&](int ord) { return ord < cl.first_n ? ord : ord - cl.first_n + cl.win; };
+  // byte offset of key row 0 of chunk ordinal `ord`; page numbers come 32 chunks at a
+  // time (an ordinal past the piece stands for its last)
+  auto offset_of = [&](int ord) -> int64_t {
+    if (ord - pbase >= 32) {
+      pbase = ord;
+      const int o2 = min(ord + lane, c1 - 1);
+      pgs = (int)paged_page(a.paged, slot, chunk_of(o2) * kChunk / a.paged.page);
+    }
+    const int64_t pg = __shfl_sync(0xffffffffu, pgs, ord - pbase);
+    const int j = chunk_of(min(ord, c1 - 1)) * kChunk;
+    return ((pg * a.Hkv + kh) * a.paged.page + (j & (a.paged.page - 1))) * (int64_t)(128 * kEB);
+  };
+  auto load_k = [&](const int64_t (&off)[CH]) {
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.paged.k) + off[u] + g * (128 * kEB) + c * 16;
+#pragma unroll
+      for (int i = 0; i < kKL; ++i) {
+        kr[u][0][i] = ld_stream(p + i * 64);
+        kr[u][1][i] = ld_stream(p + i * 64 + 8 * 128 * kEB);
+      }
+    }
+  };
+  auto load_v = [&](const int64_t (&off)[CH]) {
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.paged.v) + off[u] + 2 * c * (128 * kEB) + g * 16;
+#pragma unroll
+      for (int i = 0; i < kVL; ++i) {
+        vr[u][0][i] = ld_stream(p + i * 128);
+        vr[u][1][i] = ld_stream(p + i * 128 + 128 * kEB);
+        vr[u][2][i] = ld_stream(p + i * 128 + 8 * 128 * kEB);
+        vr[u][3][i] = ld_stream(p + i * 128 + 9 * 128 * kEB);
+      }
+    }
+  };
+  int64_t off[CH];
+#pragma unroll
+  for (int u = 0; u < CH; ++u) off[u] = offset_of(c0 + u);
+  load_k(off);
+  load_v(off);
+  for (int ord = c0; ord < c1; ord += CH) {
+    float s[CH][NT][4];
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float(&st)[4] = s[u][t];
+        st[0] = st[1] = st[2] = st[3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kKL; ++i) {
+          const uint4 &x = kr[u][0][i], &y = kr[u][1][i];
+          if constexpr (FP8) {
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mma16816<false>(st, widen_lo(xs[e]), widen_lo(ys[e]), widen_hi(xs[e]), widen_hi(ys[e]),
+                              qf[t][4 * i + e][0], qf[t][4 * i + e][1]);
+          } else {
+            mma16816<BF16>(st, x.x, y.x, x.y, y.y, qf[t][2 * i][0], qf[t][2 * i][1]);
+            mma16816<BF16>(st, x.z, y.z, x.w, y.w, qf[t][2 * i + 1][0], qf[t][2 * i + 1][1]);
           }
         }
-      };
-      auto load_v = [&](const int64_t (&off)[CH]) {
-  #pragma unroll
-        for (int u = 0; u < CH; ++u) {
-          const uint8_t* p = static_cast<const uint8_t*>(a.paged.v) + off[u] + 2 * c * (128 * kEB) + g * 16;
-  #pragma unroll
-          for (int i = 0; i < kVL; ++i) {
-            vr[u][0][i] = ld_stream(p + i * 128);
-            vr[u][1][i] = ld_stream(p + i * 128 + 128 * kEB);
-            vr[u][2][i] = ld_stream(p + i * 128 + 8 * 128 * kEB);
-            vr[u][3][i] = ld_stream(p + i * 128 + 9 * 128 * kEB);
-          }
-        }
-      };
-      int64_t off[CH];
-  #pragma unroll
-      for (int u = 0; u < CH; ++u) off[u] = offset_of(c0 + u);
+      }
+    }
+    const bool more = ord + CH < c1;
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < CH; ++u) off[u] = offset_of(ord + CH + u);
       load_k(off);
-      load_v(off);
-      for (int ord = c0; ord < c1; ord += CH) {
-        float s[CH][NT][4];
-  #pragma unroll
-        for (int u = 0; u < CH; ++u) {
-  #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float(&st)[4] = s[u][t];
-            st[0] = st[1] = st[2] = st[3] = 0.f;
-  #pragma unroll
-            for (int i = 0; i < kKL; ++i) {
-              const uint4 &x = kr[u][0][i], &y = kr[u][1][i];
-              if constexpr (FP8) {
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-  #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  mma16816<false>(st, widen_lo(xs[e]), widen_lo(ys[e]), widen_hi(xs[e]), widen_hi(ys[e]),
-                                  qf[t][4 * i + e][0], qf[t][4 * i + e][1]);
-              } else {
-                mma16816<BF16>(st, x.x, y.x, x.y, y.y, qf[t][2 * i][0], qf[t][2 * i][1]);
-                mma16816<BF16>(st, x.z, y.z, x.w, y.w, qf[t][2 * i + 1][0], qf[t][2 * i + 1][1]);
-              }
-            }
+    }
+    uint32_t hide[CH];  // bit 0: key j0 + g of the chunk is invisible, bit 1: key j0 + g + 8
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int j0 = chunk_of(ord + u) * kChunk;
+      const bool past = ord + u >= c1;
+      hide[u] = 0;
+      if (past || !(j0 + kChunk <= see.end && (j0 >= see.lo || j0 + kChunk <= see.sinks))) {
+        auto seen = [&](int j) { return !past && j < see.end && (j >= see.lo || j < see.sinks); };
+        hide[u] = (seen(j0 + g) ? 0u : 1u) | (seen(j0 + g + 8) ? 0u : 2u);
+        // what lies in invisible rows (stale or never written) must not meet P = 0
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (!seen(j0 + 2 * c + (kk & 1) + (kk >> 1) * 8)) {
+#pragma unroll
+            for (int i = 0; i < kVL; ++i) vr[u][kk][i] = make_uint4(0, 0, 0, 0);
           }
         }
-        const bool more = ord + CH < c1;
-        if (more) {
-  #pragma unroll
-          for (int u = 0; u < CH; ++u) off[u] = offset_of(ord + CH + u);
-          load_k(off);
-        }
-        uint32_t hide[CH];  // bit 0: key j0 + g of the chunk is invisible, bit 1: key j0 + g + 8
-  #pragma unroll
-        for (int u = 0; u < CH; ++u) {
-          const int j0 = chunk_of(ord + u) * kChunk;
-          const bool past = ord + u >= c1;
-          hide[u] = 0;
-          if (past || !(j0 + kChunk <= see.end && (j0 >= see.lo || j0 + kChunk <= see.sinks))) {
-            auto seen = [&](int j) { return !past && j < see.end && (j >= see.lo || j < see.sinks); };
-            hide[u] = (seen(j0 + g) ? 0u : 1u) | (seen(j0 + g + 8) ? 0u : 2u);
-            // what lies in invisible rows (stale or never written) must not meet P = 0
-  #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (!seen(j0 + 2 * c + (kk & 1) + (kk >> 1) * 8)) {
-  #pragma unroll
-                for (int i = 0; i < kVL; ++i) vr[u][kk][i] = make_uint4(0, 0, 0, 0);
-              }
-            }
-          }
-        }
-        uint32_t pb[CH][NT][2];
-  #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float x[CH][4];
-          float mx0 = -INFINITY, mx1 = -INFINITY;
-  #pragma unroll
-          for (int u = 0; u < CH; ++u) {
-  #pragma unroll
-            for (int e = 0; e < 4; ++e) x[u][e] = (hide[u] >> (e >> 1)) & 1u ? -INFINITY : s[u][t][e] * sc[t][e & 1];
-            mx0 = fmaxf(mx0, fmaxf(x[u][0], x[u][2]));
-            mx1 = fmaxf(mx1, fmaxf(x[u][1], x[u][3]));
-          }
-  #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
-          }
-          const float n0 = fmaxf(m[t][0], mx0), n1 = fmaxf(m[t][1], mx1);
-          if (__any_sync(0xffffffffu, n0 != m[t][0] || n1 != m[t][1])) {
-            const float a0 = n0 == m[t][0] ? 1.f : exp2_fast(m[t][0] - n0);
-            const float a1 = n1 == m[t][1] ? 1.f : exp2_fast(m[t][1] - n1);
-            m[t][0] = n0;
-            m[t][1] = n1;
-            l[t][0] *= a0;
-            l[t][1] *= a1;
-  #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              o[t][i][0] *= a0;
-              o[t][i][1] *= a1;
-              o[t][i][2] *= a0;
-              o[t][i][3] *= a1;
-            }
-          }
-          // a maximum of -inf (nothing seen yet) subtracts as 0: exp2(-inf) = 0
-          const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;
-  #pragma unroll
-          for (int u = 0; u < CH; ++u) {
-            const float p0 = exp2_fast(x[u][0] - f0), p1 = exp2_fast(x[u][1] - f1);
-            const float p2 = exp2_fast(x[u][2] - f0), p3 = exp2_fast(x[u][3] - f1);
-            l[t][0] += p0 + p2;
-            l[t][1] += p1 + p3;
-            // P rounds to the 16-bit type of the V product; its sum stays in fp32
-            pb[u][t][0] = transpose8x8(pack16<BF16 && !FP8>(p0, p1));
-            pb[u][t][1] = transpose8x8(pack16<BF16 && !FP8>(p2, p3));
-          }
-        }
-  #pragma unroll
-        for (int u = 0; u < CH; ++u) {
-  #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t w[4];
-  #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if constexpr (FP8) {
-                const uint4& v = vr[u][kk][0];
-                const uint32_t word = (i >> 1) == 0 ? v.x : (i >> 1) == 1 ? v.y : (i >> 1) == 2 ? v.z : v.w;
-                w[kk] = (i & 1) ? widen_hi(word) : widen_lo(word);
-              } else {
-                const uint4& v = vr[u][kk][i >> 2];
-                w[kk] = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
-              }
-            }
-            const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);
-            const uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
-  #pragma unroll
-            for (int t = 0; t < NT; ++t) mma16816<BF16 && !FP8>(o[t][i], a0, a1, a2, a3, pb[u][t][0], pb[u][t][1]);
-          }
-        }
-        if (more) load_v(off);
       }
+    }
+    uint32_t pb[CH][NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[CH][4];
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[u][e] = (hide[u] >> (e >> 1)) & 1u ? -INFINITY : s[u][t][e] * sc[t][e & 1];
+        mx0 = fmaxf(mx0, fmaxf(x[u][0], x[u][2]));
+        mx1 = fmaxf(mx1, fmaxf(x[u][1], x[u][3]));
+      }
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+      }
+      const float n0 = fmaxf(m[t][0], mx0), n1 = fmaxf(m[t][1], mx1);
+      if (__any_sync(0xffffffffu, n0 != m[t][0] || n1 != m[t][1])) {
+        const float a0 = n0 == m[t][0] ? 1.f : exp2_fast(m[t][0] - n0);
+        const float a1 = n1 == m[t][1] ? 1.f : exp2_fast(m[t][1] - n1);
+        m[t][0] = n0;
+        m[t][1] = n1;
+        l[t][0] *= a0;
+        l[t][1] *= a1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[t][i][0] *= a0;
+          o[t][i][1] *= a1;
+          o[t][i][2] *= a0;
+          o[t][i][3] *= a1;
+        }
+      }
+      // a maximum of -inf (nothing seen yet) subtracts as 0: exp2(-inf) = 0
+      const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const float p0 = exp2_fast(x[u][0] - f0), p1 = exp2_fast(x[u][1] - f1);
+        const float p2 = exp2_fast(x[u][2] - f0), p3 = exp2_fast(x[u][3] - f1);
+        l[t][0] += p0 + p2;
+        l[t][1] += p1 + p3;
+        // P rounds to the 16-bit type of the V product; its sum stays in fp32
+        pb[u][t][0] = transpose8x8(pack16<BF16 && !FP8>(p0, p1));
+        pb[u][t][1] = transpose8x8(pack16<BF16 && !FP8>(p2, p3));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if constexpr (FP8) {
+            const uint4& v = vr[u][kk][0];
+            const uint32_t word = (i >> 1) == 0 ? v.x : (i >> 1) == 1 ? v.y : (i >> 1) == 2 ? v.z : v.w;
+            w[kk] = (i & 1) ? widen_hi(word) : widen_lo(word);
+          } else {
+            const uint4& v = vr[u][kk][i >> 2];
+            w[kk] = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+          }
+        }
+        const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);
+        const uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816<BF16 && !FP8>(o[t][i], a0, a1, a2, a3, pb[u][t][0], pb[u][t][1]);
+      }
+    }
+    if (more) load_v(off);
+  }
 
-  #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-  #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          l[t][0] += __shfl_xor_sync(0xffffffffu, l[t][0], d);
-          l[t][1] += __shfl_xor_sync(0xffffffffu, l[t][1], d);
-        }
-      }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      l[t][0] += __shfl_xor_sync(0xffffffffu, l[t][0], d);
+      l[t][1] += __shfl_xor_sync(0xffffffffu, l[t][1], d);
+    }
+  }
 }
 // first channel of accumulator tile i of a thread: elements 0 / 1 are it, 2 / 3 the next
 template <bool FP8>
@@ -645,7 +645,6 @@ __global__ void __launch_bounds__(512) decode_join_kernel(DecodeArgs a) {
   }
 }
 
-constexpr int kMinBlocks = 4;  // most blocks an SM runs in any variant (sizes the workspace)
 int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -687,8 +686,8 @@ cudaError_t launch_decode(DecodeArgs a, cudaStream_t s) {
 int64_t decode_workspace_bytes(int64_t seqs, int64_t Hq, int64_t Hkv, int64_t capacity) {
   const int sms = sm_count();
   if (decode_by_clusters(seqs, Hq, Hkv, capacity)) return 0;
-  // NT = 1 at kMinBlocks blocks per SM and NT = 2 at half of that need the same
-  return kDecodeHeader + (int64_t)sms * kMinBlocks * (kDecodeThreads / 32) * 2 * 8 * (128 + 2) * 4;
+  // two pieces per warp; two blocks per SM with 16 rows a piece (more than three with 8)
+  return kDecodeHeader + (int64_t)sms * 2 * (kDecodeThreads / 32) * 2 * 16 * (128 + 2) * 4;
 }
 
 cudaError_t launch_decode_attention(DecodeArgs a, int kind, cudaStream_t s) {

@@ -3,9 +3,9 @@
 // compacting and copying.
 //
 // The tables are small and their changes have to be seen as one step, so one block
-// plans each change (validates all of it first: a call that cannot be done changes
-// nothing and sets the sticky status word); the rows themselves, which are bound by
-// memory bandwidth, are moved by full grids that follow in the stream.
+// checks each change first (a call that cannot be done changes nothing and sets the
+// sticky status word) and plans it; the rows themselves, which are bound by memory
+// bandwidth, and long table changes are moved by full grids that follow in the stream.
 // Pages are handed out lowest index first, so every result is a function of the calls.
 #include "streaming.cuh"
 
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool
     const int j = u / pieces, x = u - j * pieces, h = x >> 3, d = (x & 7) * 16;
     const uint4* ks = reinterpret_cast<const uint4*>(w.k + (tok0 + j) * w.k_stride + h * 128 + d);
     const uint4* vs = reinterpret_cast<const uint4*>(w.v + (tok0 + j) * w.v_stride + h * 128 + d);
-    const uint4 k0 = __ldg(ks), k1 = __ldg(ks + 1), v0 = __ldg(vs), v1 = __ldg(vs + 1);
+    const uint4 k0 = __ldcs(ks), k1 = __ldcs(ks + 1), v0 = __ldcs(vs), v1 = __ldcs(vs + 1);  // read once
     const int64_t at = place[j], o = base + at + h * head_step + d;
     if (at < 0) continue;
     if constexpr (FP8) {
@@ -349,10 +349,9 @@ __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const int32_t* src, const int32_t* dst, int n,
-                                                            bool apply) {
+__global__ void __launch_bounds__(kPlanThreads) fork_check_kernel(PageTables t, const int32_t* src,
+                                                                  const int32_t* dst, int n) {
   extern __shared__ uint32_t seen[];
-  __shared__ int red[kPlanWarps], ends[kPlanThreads];
   __shared__ int fault;
   const int tid = threadIdx.x;
   if (tid == 0) fault = kPagesOk;
@@ -377,22 +376,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const 
     if (tid == 0) *t.status = fault;
     return;
   }
-  if (!apply) return;
-  for (int base = 0; base < n; base += kPlanThreads) {
-    const int i = base + tid;
-    const int len = i < n ? t.lens[src[i]] : 0;
-    block_expand(
-        min(pages_of(max(len, 0), t.page), t.width), red, ends,
-        [&](int owner, int x) { return t.table[(int64_t)src[base + owner] * t.width + x]; },
-        [&](int owner, int x, int pg) {
-          t.table[(int64_t)dst[base + owner] * t.width + x] = pg;
-          if (pg >= 0 && pg < t.pages) atomicAdd(&t.refs[pg], 1);
-        });
-    if (i < n) t.lens[dst[i]] = len;
-  }
 }
-
-// The same without the checks, a block per pair.
+// A block per pair; does nothing where the check refused the call.
 __global__ void __launch_bounds__(128) fork_rows_kernel(PageTables t, const int32_t* src, const int32_t* dst) {
   chain_next();
   chain_wait();
@@ -408,10 +393,9 @@ __global__ void __launch_bounds__(128) fork_rows_kernel(PageTables t, const int3
 }
 
 // keep[i] tokens of slots[i] stay (null: none); the pages behind them lose a reference.
-__global__ void __launch_bounds__(kPlanThreads) truncate_kernel(PageTables t, const int32_t* slots, const int32_t* keep,
-                                                                int n, bool apply) {
+__global__ void __launch_bounds__(kPlanThreads) truncate_check_kernel(PageTables t, const int32_t* slots,
+                                                                      const int32_t* keep, int n) {
   extern __shared__ uint32_t seen[];
-  __shared__ int red[kPlanWarps], ends[kPlanThreads], from[kPlanThreads];
   const int tid = threadIdx.x;
   chain_next();
   chain_wait();
@@ -429,27 +413,8 @@ __global__ void __launch_bounds__(kPlanThreads) truncate_kernel(PageTables t, co
     if (tid == 0) *t.status = kPagesBadCount;
     return;
   }
-  if (!apply) return;
-  for (int base = 0; base < n; base += kPlanThreads) {
-    const int i = base + tid;
-    int left = 0, drop = 0;
-    if (i < n) {
-      left = keep ? keep[i] : 0;
-      from[tid] = pages_of(left, t.page);
-      drop = min(pages_of(max(t.lens[slots[i]], 0), t.page), t.width) - from[tid];
-    }
-    block_expand(
-        max(drop, 0), red, ends,
-        [&](int owner, int x) { return t.table[(int64_t)slots[base + owner] * t.width + from[owner] + x]; },
-        [&](int owner, int x, int pg) {
-          t.table[(int64_t)slots[base + owner] * t.width + from[owner] + x] = -1;
-          if (pg >= 0 && pg < t.pages) atomicSub(&t.refs[pg], 1);
-        });
-    if (i < n) t.lens[slots[i]] = left;
-  }
 }
-
-// The same without the checks, a block per slot.
+// A block per slot; does nothing where the check refused the call.
 __global__ void __launch_bounds__(128) truncate_rows_kernel(PageTables t, const int32_t* slots, const int32_t* keep) {
   chain_next();
   chain_wait();
@@ -577,7 +542,7 @@ __global__ void __launch_bounds__(256) move_kernel(PagePools pool, int pages, in
     const int64_t n16 = bytes / 16;
     int64_t x = threadIdx.x;
     for (; x + 3 * 256 < n16; x += 4 * 256) {
-      const uint4 a = from[x], b = from[x + 256], c = from[x + 512], e = from[x + 768];
+      const uint4 a = __ldcs(from + x), b = __ldcs(from + x + 256), c = __ldcs(from + x + 512), e = __ldcs(from + x + 768);
       to[x] = a;
       to[x + 256] = b;
       to[x + 512] = c;
@@ -620,22 +585,19 @@ cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t 
   return launch_chained(kern, copies + (w.tokens + per - 1) / per, 256, 0, s, t, p, layer, w, ws, (int)copies, (int)per);
 }
 
-// Above this many table entries that a call may touch, a second launch with a block per
-// sequence changes them: one multiprocessor makes about a scattered reference update per
-// clock.  (fork + append + free of 128 sequences of 94 pages: 52 us in one launch each, 32 us in
-// two; appending and dropping a token of 200 sequences, 13 us in one, 14 us in two.)
-constexpr int64_t kOneBlockEntries = 16384;
+// One block checks a fork or a truncation, a grid with a block per sequence then changes the
+// tables: one multiprocessor alone makes about a scattered reference update per clock.
+// (fork + free, in two kernels each against one block each: 16 sequences of 60 pages 6.8
+// against 10.2 us, 512 of 60 pages 8.0 against 39 us, 200 of one page 7.0 against 9.4 us.)
 cudaError_t launch_pages_fork(const PageTables& t, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
-  const bool one = (int64_t)n * t.width <= kOneBlockEntries;
-  const cudaError_t e = launch_chained(fork_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n, one);
-  if (e != cudaSuccess || one) return e;
+  const cudaError_t e = launch_chained(fork_check_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n);
+  if (e != cudaSuccess) return e;
   return launch_chained(fork_rows_kernel, n, 128, 0, s, t, src, dst);
 }
 cudaError_t launch_pages_truncate(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
                                   cudaStream_t s) {
-  const bool one = (int64_t)n * t.width <= kOneBlockEntries;
-  const cudaError_t e = launch_chained(truncate_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n, one);
-  if (e != cudaSuccess || one) return e;
+  const cudaError_t e = launch_chained(truncate_check_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n);
+  if (e != cudaSuccess) return e;
   return launch_chained(truncate_rows_kernel, n, 128, 0, s, t, slots, keep);
 }
 cudaError_t launch_pages_compact(const PageTables& t, const PagePools& p, int32_t* ws, cudaStream_t s) {

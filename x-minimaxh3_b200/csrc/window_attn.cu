@@ -307,9 +307,7 @@ __device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, fl
   // nothing seen so far: subtract 0, so that the -inf of unseen keys gives 0
   const float off = m == -__int_as_float(0x7f800000) ? 0.f : -m;
   const float2 c2 = make_float2(c, c), o2 = make_float2(off, off);
-  //TR3
   if (!tmem_wait(turn, turn_parity, abort_flag)) return false;
-  //TR4
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll 1
   for (int g = 1; g >= 0; --g) {
@@ -324,7 +322,6 @@ __device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, fl
     if (g == 0) {
       __syncwarp();
       tmem_arrive(other_turn);
-      //TR5
     }
     uint32_t p[32];
 #pragma unroll
@@ -982,7 +979,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         if (first && !(ok = tmem_wait(&o_free[x], o_parity, abort_flag))) break;
         if (!(ok = wait(&v_ok[vs.slot], vs.parity) && tmem_wait(&p_half[x], step_parity, abort_flag))) break;
         tc_fence_after();
-        //TM0 i
         if (elect_one()) {
 #pragma unroll
           for (int c = 4; c < 8; ++c)
@@ -992,7 +988,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         first = false;
         if (!(ok = tmem_wait(&p_full[x], step_parity, abort_flag))) break;
         tc_fence_after();
-        //TM1 i
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -1008,7 +1003,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           }
         }
         __syncwarp();
-        //TM2 i
         step_parity ^= 1u;
       }
       if (!ok) break;
@@ -1042,14 +1036,11 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           tmem_arrive(other_turn);
           continue;
         }
-        //TR0
         if (!(ok = tmem_wait(&s_full[x], step_parity, abort_flag))) break;
         tc_fence_after();
-        //TR1
         ok = win_softmax<BF16>(s_addr, o_addr, a.scale_log2, see, r.whole(i), pl.key_tile(i) * 128, cnt, m, l, &s_free[x],
                                &p_half[x], turn, turn_parity, other_turn, abort_flag);
         if (!ok) break;
-        //TR2
         __syncwarp();
         tmem_arrive(&p_full[x]);
         step_parity ^= 1u;
