@@ -138,12 +138,13 @@ __device__ __forceinline__ uint32_t zero_times2(uint32_t w, uint32_t sum) {
   return r;
 }
 
-// The 128-key tiles that rows [p0, p1] of a tile see: [0, sn) and [w0, w1), sn <= w0.
+// The 128-key tiles that rows [p0, p1] see: [0, sn) and [w0, w1), sn <= w0.
 struct TileKeys {
   int sn, w0, w1;
   int end, lo, sinks;  // what every row sees: keys below `sinks`, and [lo, end)
+  __device__ int steps() const { return sn + w1 - w0; }
 };
-__device__ TileKeys tile_keys(const WindowRule& r, int p0, int p1, int lk) {
+__device__ __forceinline__ TileKeys tile_keys(const WindowRule& r, int p0, int p1, int lk) {
   TileKeys t{0, 0, 0, 0, 0, 0};
   if (p1 < 0) return t;
   const VisibleKeys a = visible_keys(r, p0 < 0 ? 0 : p0, lk), b = visible_keys(r, p1, lk);
@@ -168,18 +169,6 @@ struct StepRanges {
   __device__ bool takes(int i) const { return i < head || (i >= from && i < to); }
   __device__ bool whole(int i) const { return i < whole_head || (i >= whole_from && i < whole_to); }
 };
-// The key tiles that rows [p0, p1] see, in the order of the steps: [0, sn), then w0 and on.
-struct UnionKeys {
-  int sn, w0, steps;
-};
-__device__ __forceinline__ UnionKeys union_keys(const WindowRule& r, int p0, int p1, int lk) {
-  if (p1 < 0) return {0, 0, 0};
-  const VisibleKeys a = visible_keys(r, p0 < 0 ? 0 : p0, lk), b = visible_keys(r, p1, lk);
-  const int sn = (b.sinks + 127) / 128;
-  if (a.lo >= b.end) return {sn, sn, sn};
-  const int w0 = max(a.lo / 128, sn);
-  return {sn, w0, sn + max((b.end + 127) / 128, w0) - w0};
-}
 struct WinPlan {
   StepRanges tile[2];
   int row[2], rows[2];  // first row (of q) and valid rows of each tile
@@ -394,7 +383,7 @@ constexpr int kItemCost = 4;
 constexpr int kCutFrom = 8;
 constexpr int kLeastPiece = 3;
 constexpr int kPieceFloats = 2 * 128 * 130;  // O [2][128][128], then (m, l) [2][128]
-constexpr int kMaxTiles = kWinSlots * kWinTile / 16 - kWinThreads;  // sums of tiles and sequences that fit the ring
+constexpr int kMaxTiles = kWinSlots * kWinTile / 24 - kWinThreads;  // whose sums and sequences fit the ring
 
 struct PieceNote {  // [CTA][2]: slot 1 a piece with the item's first step, slot 0 any other
   int state;        // 0: none, 1: more pieces follow, 2: the last
@@ -431,37 +420,48 @@ __device__ TileAt find_tile(const WindowArgs& a, int t, int rows_per_cta) {
   return {-1, 0};
 }
 
-// Everything about a tile's item but its column: rows, key tiles, steps.
+// Everything about a tile's item but its column and its piece, by the whole warp: lanes 0
+// and 1 find the keys of tiles A and B, lane 2 those of both, all in one run through the
+// code (it runs once, from a cold instruction cache).  at.seq < 0, past the last tile:
+// nothing to visit, no row to write.  Returns the number of steps.
 template <bool PAGED>
-__device__ __forceinline__ void plan_tile(const WindowArgs& a, int seq, int t, int rows_per_cta, WinPlan& p) {
-  const bool by_heads = rows_per_cta == 128;  // tiles A, B: two heads of a group; else two row tiles
-  const RowRange qr = row_range(a.q_starts, seq, a.Tq);
-  if constexpr (PAGED) {
-    p.slot = paged_slot(a.paged, seq);
-    p.lk = paged_len(a.paged, p.slot);
-    p.k_row = 0;
-  } else {
-    const RowRange kr = row_range(a.k_starts, seq, a.Tk);
-    p.slot = 0;
-    p.lk = kr.b - kr.a;
-    p.k_row = kr.a;
+__device__ __forceinline__ int plan_tile(const WindowArgs& a, TileAt at, int rows_per_cta, WinPlan* p) {
+  const int lane = threadIdx.x & 31;
+  RowRange qr{0, 0};
+  int slot = 0, lk = 0, k_row = 0;
+  if (at.seq >= 0) {
+    qr = row_range(a.q_starts, at.seq, a.Tq);
+    if constexpr (PAGED) {
+      slot = paged_slot(a.paged, at.seq);
+      lk = paged_len(a.paged, slot);
+    } else {
+      const RowRange kr = row_range(a.k_starts, at.seq, a.Tk);
+      lk = kr.b - kr.a;
+      k_row = kr.a;
+    }
   }
   const int lq = qr.b - qr.a;
-  const int first = t * rows_per_cta;
-  const UnionKeys u = union_keys(a.rule, p.lk - lq + first, p.lk - lq + min(first + rows_per_cta, lq) - 1, p.lk);
-  p.sn = u.sn;
-  p.w0 = u.w0;
-  p.steps = u.steps;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int from = first + (by_heads ? 0 : x * 128);
-    p.row[x] = qr.a + from;
-    p.rows[x] = max(0, min(128, lq - from));
-    p.p0[x] = p.lk - lq + from;
-    const TileKeys keys =
-        p.rows[x] > 0 ? tile_keys(a.rule, p.p0[x], p.p0[x] + p.rows[x] - 1, p.lk) : TileKeys{0, 0, 0, 0, 0, 0};
-    p.tile[x] = step_ranges(keys, p.sn, p.w0);
+  // tiles A, B: two heads of a group at the same 128 rows; else two row tiles
+  const int from = at.t * rows_per_cta + (lane == 1 && rows_per_cta != 128 ? 128 : 0);
+  const int rows = max(0, min(lane == 2 ? rows_per_cta : 128, lq - from)), p0 = lk - lq + from;
+  const TileKeys keys = rows > 0 ? tile_keys(a.rule, p0, p0 + rows - 1, lk) : TileKeys{0, 0, 0, 0, 0, 0};
+  const int sn = __shfl_sync(0xffffffffu, keys.sn, 2), w0 = __shfl_sync(0xffffffffu, keys.w0, 2);
+  const int steps = __shfl_sync(0xffffffffu, keys.steps(), 2);
+  if (lane < 2) {
+    p->row[lane] = qr.a + from;
+    p->rows[lane] = rows;
+    p->p0[lane] = p0;
+    p->tile[lane] = step_ranges(keys, sn, w0);
   }
+  if (lane == 0) {
+    p->sn = sn;
+    p->w0 = w0;
+    p->steps = steps;
+    p->lk = lk;
+    p->k_row = k_row;
+    p->slot = slot;
+  }
+  return steps;
 }
 
 // A place in the list that is dealt out: an item and a step of it.
@@ -643,10 +643,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       long long* lack = reinterpret_cast<long long*>(smem + kWinOffRing);  // [CTAs]: share without the rounds' items
       long long* seq_upto = lack + kWinThreads;                            // [seqs]: tiles of sequences 0..i
       long long* upto = seq_upto + a.seqs;  // [tiles] from the last tile: cost of an item of each, summed
-      for (int i = (int)threadIdx.x; i < a.seqs; i += kWinThreads) seq_upto[i] = tiles_of(a, i, rows_per_cta);
-      __syncthreads();
-      block_prefix(seq_upto, a.seqs, scan);
-      const int valid = (int)min(seq_upto[a.seqs - 1], (long long)tiles);  // more only where the starts overlap
+      int2* seq_len = reinterpret_cast<int2*>(upto + tiles);  // [seqs]: rows and keys
       auto locate = [&](int tile) {
         int lo = 0, hi = a.seqs - 1;
 #pragma unroll 1
@@ -656,44 +653,66 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         }
         return TileAt{lo, tile - (lo ? (int)seq_upto[lo - 1] : 0)};
       };
-#pragma unroll 1
-      for (int q = (int)threadIdx.x; q < valid; q += kWinThreads) {
-        const TileAt at = locate(valid - 1 - q);
-        const RowRange qr = row_range(a.q_starts, at.seq, a.Tq);
-        int lk;
-        if constexpr (PAGED) {
-          lk = paged_len(a.paged, paged_slot(a.paged, at.seq));
-        } else {
-          const RowRange kr = row_range(a.k_starts, at.seq, a.Tk);
-          lk = kr.b - kr.a;
-        }
-        const int lq = qr.b - qr.a, first = at.t * rows_per_cta;
-        upto[q] = union_keys(a.rule, lk - lq + first, lk - lq + min(first + rows_per_cta, lq) - 1, lk).steps + kItemCost;
-      }
-      __syncthreads();
-      block_prefix(upto, valid, scan);
-      const int items = valid * columns;
-      const long long all = valid ? upto[valid - 1] * columns : 0, share = (all + ctas - 1) / ctas;
       auto cost = [&](int q) { return upto[q] - (q ? upto[q - 1] : 0); };
-      // whole rounds; a thread per CTA (the launch has at most kWinThreads)
-      int rounds = 0, my_q = (int)threadIdx.x / columns, my_column = (int)threadIdx.x % columns;
-      const int step_q = ctas / columns, step_column = ctas % columns;
-      long long load = 0;
+      int valid = 0, items = 0, rounds = 0;
+      long long all = 0, share = 0;
+      // a loop: one copy of the prefix sums, which run from a cold instruction cache
 #pragma unroll 1
-      for (;; ++rounds) {
-        const bool in = (rounds + 1) * ctas <= items;
-        const long long next = (int)threadIdx.x < ctas && in ? load + cost(my_q) : 0;
-        if (!__syncthreads_and(in && next <= share)) break;
-        load = next;
-        my_q += step_q;
-        if ((my_column += step_column) >= columns) {
-          my_column -= columns;
-          ++my_q;
+      for (int stage = 0; stage < 3; ++stage) {
+        long long* sums;
+        int n;
+        if (stage == 0) {
+          sums = seq_upto;
+          n = a.seqs;
+          for (int i = (int)threadIdx.x; i < n; i += kWinThreads) {
+            int lk;
+            if constexpr (PAGED) {
+              lk = paged_len(a.paged, paged_slot(a.paged, i));
+            } else {
+              const RowRange kr = row_range(a.k_starts, i, a.Tk);
+              lk = kr.b - kr.a;
+            }
+            const RowRange qr = row_range(a.q_starts, i, a.Tq);
+            seq_len[i] = make_int2(qr.b - qr.a, lk);
+            seq_upto[i] = (qr.b - qr.a + rows_per_cta - 1) >> (by_heads ? 7 : 8);  // 128 or 256
+          }
+        } else if (stage == 1) {
+          sums = upto;
+          n = valid = (int)min(seq_upto[a.seqs - 1], (long long)tiles);  // more only where the starts overlap
+#pragma unroll 1
+          for (int q = (int)threadIdx.x; q < n; q += kWinThreads) {
+            const TileAt at = locate(n - 1 - q);
+            const int2 len = seq_len[at.seq];
+            const int first = at.t * rows_per_cta, rows = min(rows_per_cta, len.x - first), p0 = len.y - len.x + first;
+            upto[q] = tile_keys(a.rule, p0, p0 + rows - 1, len.y).steps() + kItemCost;
+          }
+        } else {
+          sums = lack;
+          n = ctas;
+          items = valid * columns;
+          all = valid ? upto[valid - 1] * columns : 0;
+          share = (all + ctas - 1) / ctas;
+          // whole rounds; a thread per CTA (the launch has at most kWinThreads)
+          int my_q = (int)threadIdx.x / columns, my_column = (int)threadIdx.x % columns;
+          const int step_q = ctas / columns, step_column = ctas % columns;
+          long long load = 0;
+#pragma unroll 1
+          for (;; ++rounds) {
+            const bool in = (rounds + 1) * ctas <= items;
+            const long long next = (int)threadIdx.x < ctas && in ? load + cost(my_q) : 0;
+            if (!__syncthreads_and(in && next <= share)) break;
+            load = next;
+            my_q += step_q;
+            if ((my_column += step_column) >= columns) {
+              my_column -= columns;
+              ++my_q;
+            }
+          }
+          if ((int)threadIdx.x < ctas) lack[threadIdx.x] = share - load;
         }
+        __syncthreads();
+        block_prefix(sums, n, scan);
       }
-      if ((int)threadIdx.x < ctas) lack[threadIdx.x] = share - load;
-      __syncthreads();
-      block_prefix(lack, ctas, scan);
       if (threadIdx.x < 2) {
         // from after what the CTAs before this one lack, to after what it lacks itself
         const int i = me - 1 + (int)threadIdx.x, dealt = rounds * ctas, q0 = dealt / columns;
@@ -774,29 +793,25 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           at_tile = work.tile[entry];
         else
           at_tile = find_tile(a, work.valid - 1 - q, rows_per_cta);
+        const int steps = plan_tile<PAGED>(a, at_tile, rows_per_cta, pl);
+        const int from = round ? 0 : w.step, to = !round && item == stop.item ? stop.step : steps;
+        const bool cut = from > 0 || to < steps;
+        const int slot = from == 0 ? 1 : 0, head0 = (item - q * columns) * (by_heads ? 2 : 1);
         if (lane == 0) {
-          WinPlan p{};  // past the last tile: nothing to visit, no row to write
-          p.part = -1;
-          if (at_tile.seq >= 0) plan_tile<PAGED>(a, at_tile.seq, at_tile.t, rows_per_cta, p);
-          p.head0 = (item - q * columns) * (by_heads ? 2 : 1);
-          p.kh = p.head0 / (a.Hq / a.Hkv);
-          p.from = round ? 0 : w.step;
-          p.to = !round && item == stop.item ? stop.step : p.steps;
-          if (p.from > 0 || p.to < p.steps) {
-            const int slot = p.from == 0 ? 1 : 0;
-            p.part = 2 * blockIdx.x + slot;
-            PieceNote n;
-            n.state = p.to == p.steps ? 2 : 1;
-            for (int x = 0; x < 2; ++x) {
-              n.row[x] = p.row[x];
-              n.rows[x] = p.rows[x];
-            }
-            n.head0 = p.head0;
-            n.pad[0] = n.pad[1] = 0;
-            notes[slot] = n;
-          }
-          *pl = p;
+          pl->head0 = head0;
+          pl->kh = head0 / (a.Hq / a.Hkv);
+          pl->from = from;
+          pl->to = to;
+          pl->part = cut ? 2 * (int)blockIdx.x + slot : -1;
           cleared[pr.slot] = 0;
+          if (cut) {
+            notes[slot].state = to == steps ? 2 : 1;
+            notes[slot].head0 = head0;
+          }
+        }
+        if (lane < 2 && cut) {
+          notes[slot].row[lane] = pl->row[lane];
+          notes[slot].rows[lane] = pl->rows[lane];
         }
         if (!round) w = {w.item + 1, 0};
       } else if (lane == 0) {
