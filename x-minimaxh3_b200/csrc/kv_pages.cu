@@ -3,9 +3,9 @@
 // compacting and copying.
 //
 // The tables are small and their changes have to be seen as one step, so one block
-// checks each change first (a call that cannot be done changes nothing and sets the
-// sticky status word) and plans it; the rows themselves, which are bound by memory
-// bandwidth, and long table changes are moved by full grids that follow in the stream.
+// plans each change (validates all of it first: a call that cannot be done changes
+// nothing and sets the sticky status word); the rows themselves, which are bound by
+// memory bandwidth, are moved by full grids that follow in the stream.
 // Pages are handed out lowest index first, so every result is a function of the calls.
 #include "streaming.cuh"
 
@@ -108,6 +108,9 @@ __host__ __device__ __forceinline__ ExtendPlan extend_plan(int32_t* ws, int n) {
           ws + 4 + 5 * (int64_t)n};
 }
 
+// Bound by the latency of its dependent loads (status, slots, lengths, tables, counts): about
+// half of the 12 us of a token's append to 200 sequences and its truncation.  One block,
+// because the pages of a sequence depend on what all before it ask for.
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t, const int32_t* slots, int n,
                                                                    const int32_t* starts, int32_t* ws) {
   extern __shared__ uint32_t seen[];
@@ -308,7 +311,8 @@ __device__ __forceinline__ int64_t row_place(const PageTables& t, const PageWrit
   return ((int64_t)pg * Hkv * t.page + pos % t.page) * 128;
 }
 // A block writes `per` (1..8) tokens: their places are looked up side by side first, then
-// all their rows are under way together.
+// all their rows are under way together.  Bound by memory: 32,600 tokens of 8 kv heads into
+// an E4M3 cache, with the plan before it, 53 us (3.8 TB/s; 58 us with four tokens a block).
 template <bool FP8, bool BF16>
 __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w,
                                                     const int32_t* ws, int copy_blocks, int per) {
@@ -349,9 +353,10 @@ __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) fork_check_kernel(PageTables t, const int32_t* src,
-                                                                  const int32_t* dst, int n) {
+__global__ void __launch_bounds__(kPlanThreads) fork_kernel(PageTables t, const int32_t* src, const int32_t* dst, int n,
+                                                            bool apply) {
   extern __shared__ uint32_t seen[];
+  __shared__ int red[kPlanWarps], ends[kPlanThreads];
   __shared__ int fault;
   const int tid = threadIdx.x;
   if (tid == 0) fault = kPagesOk;
@@ -376,8 +381,22 @@ __global__ void __launch_bounds__(kPlanThreads) fork_check_kernel(PageTables t, 
     if (tid == 0) *t.status = fault;
     return;
   }
+  if (!apply) return;
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + tid;
+    const int len = i < n ? t.lens[src[i]] : 0;
+    block_expand(
+        min(pages_of(max(len, 0), t.page), t.width), red, ends,
+        [&](int owner, int x) { return t.table[(int64_t)src[base + owner] * t.width + x]; },
+        [&](int owner, int x, int pg) {
+          t.table[(int64_t)dst[base + owner] * t.width + x] = pg;
+          if (pg >= 0 && pg < t.pages) atomicAdd(&t.refs[pg], 1);
+        });
+    if (i < n) t.lens[dst[i]] = len;
+  }
 }
-// A block per pair; does nothing where the check refused the call.
+
+// The same without the checks, a block per pair.
 __global__ void __launch_bounds__(128) fork_rows_kernel(PageTables t, const int32_t* src, const int32_t* dst) {
   chain_next();
   chain_wait();
@@ -393,9 +412,10 @@ __global__ void __launch_bounds__(128) fork_rows_kernel(PageTables t, const int3
 }
 
 // keep[i] tokens of slots[i] stay (null: none); the pages behind them lose a reference.
-__global__ void __launch_bounds__(kPlanThreads) truncate_check_kernel(PageTables t, const int32_t* slots,
-                                                                      const int32_t* keep, int n) {
+__global__ void __launch_bounds__(kPlanThreads) truncate_kernel(PageTables t, const int32_t* slots, const int32_t* keep,
+                                                                int n, bool apply) {
   extern __shared__ uint32_t seen[];
+  __shared__ int red[kPlanWarps], ends[kPlanThreads], from[kPlanThreads];
   const int tid = threadIdx.x;
   chain_next();
   chain_wait();
@@ -413,8 +433,27 @@ __global__ void __launch_bounds__(kPlanThreads) truncate_check_kernel(PageTables
     if (tid == 0) *t.status = kPagesBadCount;
     return;
   }
+  if (!apply) return;
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + tid;
+    int left = 0, drop = 0;
+    if (i < n) {
+      left = keep ? keep[i] : 0;
+      from[tid] = pages_of(left, t.page);
+      drop = min(pages_of(max(t.lens[slots[i]], 0), t.page), t.width) - from[tid];
+    }
+    block_expand(
+        max(drop, 0), red, ends,
+        [&](int owner, int x) { return t.table[(int64_t)slots[base + owner] * t.width + from[owner] + x]; },
+        [&](int owner, int x, int pg) {
+          t.table[(int64_t)slots[base + owner] * t.width + from[owner] + x] = -1;
+          if (pg >= 0 && pg < t.pages) atomicSub(&t.refs[pg], 1);
+        });
+    if (i < n) t.lens[slots[i]] = left;
+  }
 }
-// A block per slot; does nothing where the check refused the call.
+
+// The same without the checks, a block per slot.
 __global__ void __launch_bounds__(128) truncate_rows_kernel(PageTables t, const int32_t* slots, const int32_t* keep) {
   chain_next();
   chain_wait();
@@ -521,7 +560,8 @@ __global__ void __launch_bounds__(256) compact_table_kernel(PageTables t, const 
     if (pg >= used && pg < t.pages) t.table[i] = p.to[pg];
   }
 }
-// Whole pages, K and V of every layer: a block per (move, layer, K/V).  count: device
+// Whole pages, K and V of every layer: a block per (move, layer, K/V).  Bound by memory: 1.07
+// GB moved in 364 us with the plan, 5.9 TB/s of reads and writes.  count: device
 // value (compact) or null (n moves, whose pages are checked here).
 __global__ void __launch_bounds__(256) move_kernel(PagePools pool, int pages, int64_t bytes, const int32_t* src,
                                                    const int32_t* dst, const int32_t* count, int n, int32_t* status) {
@@ -585,19 +625,24 @@ cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t 
   return launch_chained(kern, copies + (w.tokens + per - 1) / per, 256, 0, s, t, p, layer, w, ws, (int)copies, (int)per);
 }
 
-// One block checks a fork or a truncation, a grid with a block per sequence then changes the
-// tables: one multiprocessor alone makes about a scattered reference update per clock.
-// (fork + free, in two kernels each against one block each: 16 sequences of 60 pages 6.8
-// against 10.2 us, 512 of 60 pages 8.0 against 39 us, 200 of one page 7.0 against 9.4 us.)
+// One block that checks a call also changes the tables where it can touch few entries; else
+// a second launch with a block per sequence does: one multiprocessor makes about a scattered
+// reference update per clock, a launch costs the host 2 to 3 us.  (fork + free, on the device
+// in one launch each / in two: 16 sequences of 60 pages 10.2 / 6.8 us, 128 of 94 pages 19.5 /
+// 6.9 us, 512 of 60 pages 39 / 8.0 us.)  A truncation mostly drops a few tokens (a pass that
+// appends a token to 200 sequences and drops it, launched from the host: 21.6 / 24.2 us).
+constexpr int64_t kOneBlockEntries = 4096, kOneBlockKept = 16384;
 cudaError_t launch_pages_fork(const PageTables& t, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
-  const cudaError_t e = launch_chained(fork_check_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n);
-  if (e != cudaSuccess) return e;
+  const bool one = (int64_t)n * t.width <= kOneBlockEntries;
+  const cudaError_t e = launch_chained(fork_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, src, dst, n, one);
+  if (e != cudaSuccess || one) return e;
   return launch_chained(fork_rows_kernel, n, 128, 0, s, t, src, dst);
 }
 cudaError_t launch_pages_truncate(const PageTables& t, const int32_t* slots, const int32_t* keep, int n,
                                   cudaStream_t s) {
-  const cudaError_t e = launch_chained(truncate_check_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n);
-  if (e != cudaSuccess) return e;
+  const bool one = (int64_t)n * t.width <= (keep ? kOneBlockKept : kOneBlockEntries);
+  const cudaError_t e = launch_chained(truncate_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, keep, n, one);
+  if (e != cudaSuccess || one) return e;
   return launch_chained(truncate_rows_kernel, n, 128, 0, s, t, slots, keep);
 }
 cudaError_t launch_pages_compact(const PageTables& t, const PagePools& p, int32_t* ws, cudaStream_t s) {
