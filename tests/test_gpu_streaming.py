@@ -133,6 +133,28 @@ def test_window_few_rows_over_many_keys(case, dtype):
     assert torch.equal(window_attention(q, k, v, **kw), out)
 
 
+@pytest.mark.parametrize("n", [6000, 6150, 6400])
+def test_window_thousands_of_sequences(n):
+    """Sequences of a few tokens, on both sides of the number whose plan fits shared memory."""
+    from h3b import window_attention
+
+    rng = np.random.RandomState(n)
+    lens = rng.choice([0, 1, 2, 3], n)
+    keys = lens + 1
+    g = _gen(n)
+    q = _rand(g, int(lens.sum()), 2, D, dtype=torch.bfloat16, scale=1.5)
+    k, v = (_rand(g, int(keys.sum()), 1, D, dtype=torch.bfloat16) for _ in range(2))
+    out = window_attention(q, k, v, query_starts=_starts(lens.tolist()), key_starts=_starts(keys.tolist()))
+    a = b = 0
+    for i in range(0, n, 100):
+        see = torch.block_diag(*[visible(int(lq), int(lk), None, 0, 1).float()
+                                 for lq, lk in zip(lens[i:i + 100], keys[i:i + 100])]).bool().cuda()
+        rows, cols = see.shape
+        ref, spread = attend(q[a:a + rows], k[b:b + cols], v[b:b + cols], see)
+        assert_close(out[a:a + rows], ref, spread, 4, 6.0, f"sequences from {i}")
+        a, b = a + rows, b + cols
+
+
 def test_window_cut_items_keep_unseen_rows_apart():
     """Non-finite V and K rows inside and outside what the rows of cut items see."""
     from h3b import window_attention

@@ -51,7 +51,7 @@ constexpr int kWinSlots = 5;
 constexpr int kWinTile = 128 * 128 * 2;  // bytes of a 128 x 128 16-bit tile
 constexpr int kWinOffRing = 2 * kWinTile;
 constexpr int kWinOffRest = kWinOffRing + kWinSlots * kWinTile;
-constexpr int kWinSmem = kWinOffRest + 3072;  // all of a block's 227 KB
+constexpr int kWinSmem = kWinOffRest + 3 * 1024;  // all of a block's 227 KB
 // Register split (setmaxnreg): every thread starts with kWinRegs, the control and output
 // warpgroups drop to kWinCtrlRegs and kWinOutRegs, each softmax warpgroup rises to
 // kWinSoftRegs; the shares may not exceed the launch's total, or the rise would wait
