@@ -659,6 +659,24 @@ def test_e4m3_write_rounds_and_saturates(dtype):
         assert torch.equal(got.float()[~nan], want.float()[~nan])
 
 
+@pytest.mark.parametrize("scale", [3e-39, 7e-31, 1.1e-30, 0.013, 0.25, 9e29, 3e30, 5e37])
+def test_e4m3_write_divides_exactly_at_any_scale(scale):
+    """Scales whose reciprocal is usable and scales whose is not: the codes are those of the fp32 quotient."""
+    cache = _nan_cache(16, 2, 1, 40, 1, 640, torch.float8_e4m3fn)
+    cache.k_scale.fill_(scale)
+    cache.v_scale.fill_(scale * 0.5)
+    g = _gen(31)
+    rows = (torch.randn(601, 2, D, device="cuda", generator=g).double() * scale * 20).float().to(torch.bfloat16)
+    cache.append(_i32([0]), rows, rows, starts=_i32([0, 601]))
+    cache.check()
+    pages = cache.table[0, :-(-601 // 16)].long()
+    for pool, by in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        got = pool[0, pages].permute(0, 2, 1, 3).reshape(-1, 2, D)[:601]
+        # the quotient in 64 bits, rounded to 32 and then to 8: the fp32 quotient is correctly rounded
+        want = (rows.double() / by[0, 0].double()).float().clamp(-448, 448).to(torch.float8_e4m3fn)
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
 def test_cache_step_in_a_cuda_graph():
     """Append and decode captured once and replayed: the tables grow on the device."""
     from h3b import decode_attention
