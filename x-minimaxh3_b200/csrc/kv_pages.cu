@@ -111,7 +111,7 @@ __host__ __device__ __forceinline__ ExtendPlan extend_plan(int32_t* ws, int n) {
 }
 
 // Bound by the latency of its dependent loads (status, slots, lengths, tables, counts): about
-// half of the 12 us of a token's append to 200 sequences and its truncation.  One block,
+// half of the 11 us of a token's append to 200 sequences and its truncation.  One block,
 // because the pages of a sequence depend on what all before it ask for.
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t, const int32_t* slots, int n,
                                                                    const int32_t* starts, int32_t* ws) {
@@ -327,8 +327,8 @@ __device__ __forceinline__ int64_t row_place(const PageTables& t, const PageWrit
 }
 // A block writes `per` (1..8) tokens: their places are looked up side by side first, then
 // all their rows are under way together.  Bound by memory: 32,600 tokens of 8 kv heads into
-// an E4M3 cache, with the plan before it, 46 us (4.4 TB/s), half of the issue slots taken by
-// the conversion.
+// an E4M3 cache, with the plan before it, 50 us (4.0 TB/s; 46 where L2 holds some of the
+// rows), half of the issue slots taken by the conversion.
 template <bool FP8, bool BF16>
 __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w,
                                                     const int32_t* ws, int copy_blocks, int per) {
