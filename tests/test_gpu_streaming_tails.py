@@ -1,0 +1,76 @@
+"""Long tails of small softmax weights under one dominant key (GPU).
+
+The dominant key has V = 0, so the output is what the tail leaves: weights that get lost in
+the rounding of P, but not in its sum, show in full."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from streaming_util import D, UNIT  # noqa: E402
+
+
+def _tail(n, octaves, v):
+    """Key 0 with a score of 0 and V 0, n - 1 keys `octaves` powers of two below with V = v."""
+    w = 2.0 ** -octaves * (n - 1)
+    return v * w / (1 + w)
+
+
+def _close(out, ref, dtype, p_unit):
+    """The output's rounding, that of the weights (all equal, so it does not average out) and 2e-4 for
+    the exponential and the fp32 scores and sums, all relative to the output."""
+    rel = ((out.double() - ref).abs() / ref).amax()
+    assert rel <= (UNIT[dtype] + p_unit + 2e-4) * 1.01, f"relative error {float(rel):.2e}"
+
+
+def _cache(store, heads, page, pages, slots, n, v):
+    """Every slot reads the same pages: key 0 with 8 in channel 0 and V 0, the others 0 with V = v."""
+    from h3b import PagedKVCache
+
+    dtype = torch.float8_e4m3fn if store == "e4m3" else store
+    ones = lambda: torch.ones(1, heads, device="cuda")  # noqa: E731
+    scale = dict(k_scale=ones(), v_scale=ones()) if store == "e4m3" else {}
+    cache = PagedKVCache.create(1, pages, page, heads, slots, pages * page, dtype, **scale)
+    k = torch.zeros(cache.k.shape, device="cuda")
+    k[0, 0, :, 0, 0] = 8
+    cache.k.copy_(k.to(dtype))
+    k.fill_(v)[0, 0, :, 0] = 0
+    cache.v.copy_(k.to(dtype))
+    cache.table.copy_(torch.arange(pages, device="cuda", dtype=torch.int32).expand(slots, -1))
+    cache.lens.fill_(n)
+    cache.refs.fill_(slots)
+    return cache
+
+
+def _query(rows, heads, dtype):
+    q = torch.zeros(rows, heads, D, device="cuda", dtype=dtype)
+    q[..., 0] = 8
+    return q
+
+
+@pytest.mark.parametrize("store,dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                         ("e4m3", torch.bfloat16), ("e4m3", torch.float16)], ids=str)
+@pytest.mark.parametrize("octaves", [20.6, 23.4, 25.2, 26.0])
+@pytest.mark.parametrize("group", [1, 12])
+def test_decode_keeps_a_long_tail(store, dtype, octaves, group):
+    """As many pairs as warps, so that one warp has the dominant key and thousands of the others."""
+    from h3b import decode_attention
+
+    n, kv, slots = 32768, 8, 250
+    cache = _cache(store, kv, 128, n // 128, slots, n, 1.0)
+    out = decode_attention(_query(slots, kv * group, dtype), cache, scale=octaves * math.log(2) / 64)
+    p_unit = UNIT[torch.bfloat16 if store is torch.bfloat16 else torch.float16]
+    _close(out, _tail(n, octaves, 1.0), dtype, p_unit)
+
+
+@pytest.mark.parametrize("store,dtype", [(torch.float16, torch.float16), ("e4m3", torch.bfloat16)], ids=str)
+def test_decode_of_one_short_sequence_keeps_a_tail(store, dtype):
+    """One chunk of 16 keys in a table that the cluster launch takes."""
+    from h3b import decode_attention
+
+    cache = _cache(store, 1, 16, 1, 1, 16, 384.0)
+    out = decode_attention(_query(1, 1, dtype), cache, scale=20.6 * math.log(2) / 64)
+    _close(out, _tail(16, 20.6, 384.0), dtype, UNIT[torch.float16])

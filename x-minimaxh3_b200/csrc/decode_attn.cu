@@ -17,11 +17,16 @@
 //   S^T = K . Q^T   m16n8k16, M = 16 keys, N = 8 heads of the group.  The products'
 //                   order over the 128 channels is free, so each thread loads 16
 //                   contiguous bytes of its key rows and the matching ones of Q.
-//   P^T             exp2 of S^T under the running maximum; the accumulator layout of
-//                   S^T becomes the B operand by one 8 x 8 transpose per 8 keys
+//   P^T             exp2 of S^T under the running maximum, rounded to the 16-bit type of the
+//                   V product (its sum is not: one more rounding of the weights, relative
+//                   2^-9 in bf16 and 2^-12 in fp16, that tensor cores ask for); the accumulator
+//                   layout of S^T becomes the B operand by one 8 x 8 transpose per 8 keys
 //   O^T += V^T . P^T  M = 16 channels, N = 8 heads, K = 16 keys: the A operand pairs
 //                   two keys of one channel, one byte permute per register
-// E4M3 caches are widened to fp16 (exact) with q in fp16 under a power of two per head.
+// E4M3 caches are widened to fp16 (exact), with a bf16 q in fp16 under a power of two per head
+// that brings its largest channel to [1, 2).  Channels of 2^-17 and more are exact then; smaller
+// ones round to multiples of 2^-24, an error of the size that an fp32 sum with the largest
+// channel's product has anyway (only where that channel's keys are 0 it would not).
 #include "streaming.cuh"
 
 namespace h3b {
@@ -30,6 +35,13 @@ namespace {
 
 constexpr int kDecodeThreads = 128;
 constexpr int kChunk = 16;
+// P = 2^(x - m) times 2^kHalfUp where it rounds to fp16 (16-bit fp16 caches, and E4M3 ones,
+// whose V widens to fp16): its peak is then 2^15, below fp16's largest value, and a weight
+// keeps fp16's 11 bits down to 2^-29 of the largest (without the factor to 2^-14, and none
+// below 2^-25: 32,768 keys 23.4 octaves below a first token came out 32 % too heavy).  The
+// row sum has the same factor, so it leaves in O / l, and every piece has it, so the joins
+// need not know.  bf16 has fp32's exponents and needs none.
+constexpr float kHalfUp = 15.f;
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -307,7 +319,8 @@ __device__ __forceinline__ void decode_chunks(const DecodeArgs& a, int b, int sl
         }
       }
       // a maximum of -inf (nothing seen yet) subtracts as 0: exp2(-inf) = 0
-      const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;
+      constexpr float up = BF16 && !FP8 ? 0.f : kHalfUp;
+      const float f0 = n0 == -INFINITY ? 0.f : n0 - up, f1 = n1 == -INFINITY ? 0.f : n1 - up;
 #pragma unroll
       for (int u = 0; u < CH; ++u) {
         const float p0 = exp2_fast(x[u][0] - f0), p1 = exp2_fast(x[u][1] - f1);
