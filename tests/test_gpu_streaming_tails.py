@@ -74,3 +74,53 @@ def test_decode_of_one_short_sequence_keeps_a_tail(store, dtype):
     cache = _cache(store, 1, 16, 1, 1, 16, 384.0)
     out = decode_attention(_query(1, 1, dtype), cache, scale=20.6 * math.log(2) / 64)
     _close(out, _tail(16, 20.6, 384.0), dtype, UNIT[torch.float16])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("octaves", [20.6, 23.4, 25.2, 26.0])
+@pytest.mark.parametrize("n", [100, 800])
+def test_window_keeps_a_tail(dtype, octaves, n):
+    """Few keys, with a V that keeps the output in fp16's range."""
+    from h3b import window_attention
+
+    k = torch.zeros(n, 1, D, device="cuda", dtype=dtype)
+    k[0, 0, 0] = 8
+    v = torch.full((n, 1, D), 30000.0, device="cuda", dtype=dtype)
+    ref = _tail(n, octaves, float(v[0, 0, 0]))
+    v[0] = 0
+    out = window_attention(_query(1, 1, dtype), k, v, scale=octaves * math.log(2) / 64)
+    _close(out, ref, dtype, UNIT[dtype])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("octaves", [23.4, 26.0])
+@pytest.mark.parametrize("slots", [1, 64])
+def test_paged_window_keeps_a_long_tail(dtype, octaves, slots):
+    """One sequence, whose keys are divided over the multiprocessors, and more than there are of those."""
+    from h3b import paged_window_attention
+
+    n, kv = 32768, 4
+    cache = _cache(dtype, kv, 128, n // 128, slots, n, 1.0)
+    starts = torch.arange(slots + 1, device="cuda", dtype=torch.int32)
+    out = paged_window_attention(_query(slots, kv, dtype), cache, query_starts=starts, scale=octaves * math.log(2) / 64)
+    _close(out, _tail(n, octaves, 1.0), dtype, UNIT[dtype])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_window_maximum_that_creeps_up(dtype):
+    """Tiles whose maxima rise by less, about and more than the running maximum tolerates: the weights
+    before and after each move keep their proportions."""
+    from h3b import window_attention
+
+    n = 1280  # ten tiles
+    for octaves in (0.7, 2.9, 3.1, 7.9, 8.1, 20.0):
+        k = torch.zeros(n, 1, D, device="cuda", dtype=dtype)
+        rise = (torch.arange(n, device="cuda") // 128).double()
+        k[:, 0, 0] = rise.to(dtype)  # whole numbers up to 9
+        v = torch.randn(n, 1, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).to(dtype)
+        out = window_attention(_query(1, 1, dtype), k, v, scale=octaves * math.log(2) / 8)
+        w = torch.exp2((rise - rise.max()) * octaves)
+        w /= w.sum()
+        ref, spread = (w @ v[:, 0].double()), (w @ v[:, 0].double().abs())
+        u = UNIT[dtype]
+        assert ((out[0, 0].double() - ref).abs() <= u * ref.abs() + (u + 2e-4) * spread * 1.01).all(), octaves

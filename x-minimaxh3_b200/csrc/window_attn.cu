@@ -9,9 +9,9 @@
 // then those of the window -- in one pass with the running maximum and sum:
 //   S = Q . K^T     tcgen05 kind::f16, fp32 in tensor memory
 //   P = 2^(S c - m) the running maximum m moves only when a tile exceeds it by more than
-//                   kWinTau, so P <= 2^kWinTau and O is rarely rescaled; P is rounded to
-//                   the inputs' 16-bit type over S's own tensor-memory columns, its row
-//                   sum is taken before the rounding, in fp32
+//                   win_tau, so P <= 2^win_tau and O is rarely rescaled; P is rounded to the
+//                   inputs' 16-bit type, which the matrix product asks for, over S's own
+//                   tensor-memory columns; its row sum is taken before that, in fp32
 //   O += P . V      A = P from tensor memory, B = V as it lies (rows of channels, the
 //                   MN-major form), so V needs no transposition
 //
@@ -61,7 +61,14 @@ constexpr int kWinCtrlRegs = 104;
 constexpr int kWinOutRegs = 104;
 constexpr int kWinSoftRegs = 152;
 static_assert(128 * (kWinCtrlRegs + kWinOutRegs + 2 * kWinSoftRegs) <= kWinThreads * kWinRegs, "register split too large");
-constexpr float kWinTau = 8.0f;
+// How far P may pass 2^0 before the maximum moves, and a factor 2^win_up of P that leaves in
+// O / l (the pieces of cut items all have it).  fp16: P stays below 2^15, fp16's largest power
+// of two, and a weight keeps 11 bits down to 2^-26 of the largest; without the factor down to
+// 2^-14, and none below 2^-25 (800 keys 20.6 octaves below a first token: 4.2 % off).
+template <bool BF16>
+constexpr float win_tau = BF16 ? 8.0f : 3.0f;
+template <bool BF16>
+constexpr float win_up = BF16 ? 0.0f : 15.0f - win_tau<BF16>;
 
 // D(tmem) (+)= A(tmem) * B(smem), 16-bit x 16-bit -> fp32
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
@@ -284,7 +291,7 @@ __device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, fl
   tmax *= c;
   // a score of +inf or NaN: the row's result is not a number, whatever the rest does
   if (!(tmax < __int_as_float(0x7f800000))) l = __int_as_float(0x7fffffff);
-  const float m_new = tmax > m + kWinTau || m == -__int_as_float(0x7f800000) ? tmax : m;
+  const float m_new = tmax > m + win_tau<BF16> || m == -__int_as_float(0x7f800000) ? tmax : m;
   if (__any_sync(0xffffffffu, m_new != m)) {
     const float alpha = m_new == m ? 1.f : ex2(m - m_new);
     m = m_new;
@@ -303,7 +310,7 @@ __device__ __forceinline__ bool win_softmax(uint32_t s_addr, uint32_t o_addr, fl
     }
   }
   // nothing seen so far: subtract 0, so that the -inf of unseen keys gives 0
-  const float off = m == -__int_as_float(0x7f800000) ? 0.f : -m;
+  const float off = m == -__int_as_float(0x7f800000) ? 0.f : win_up<BF16> - m;
   const float2 c2 = make_float2(c, c), o2 = make_float2(off, off);
   if (!tmem_wait(turn, turn_parity, abort_flag)) return false;
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
