@@ -419,7 +419,7 @@ typedef struct h3b_page_cache {
 #define H3B_PAGES_BAD_SLOT 3  /* a slot outside the table, or named twice */
 #define H3B_PAGES_OCCUPIED 4  /* fork into a slot that holds tokens */
 #define H3B_PAGES_BAD_COUNT 5 /* token counts negative, unordered or beyond the length */
-#define H3B_PAGES_BAD_PAGE 6  /* a page outside the pool */
+#define H3B_PAGES_BAD_PAGE 6  /* a page outside the pool, or copied to twice, or both from and to */
 
 /* Window attention over contiguous K/V.  q, out: rows [Tq, Hq * 128] with their strides;
  * k, v: rows [Tk, Hkv * 128].  query_starts / key_starts: device int32 [seqs + 1], the
@@ -487,7 +487,7 @@ int h3b_pages_truncate(const h3b_page_cache* cache, const int32_t* slots, const 
  * h3b_pages_workspace_bytes(0, pages) bytes. */
 int h3b_pages_compact(const h3b_page_cache* cache, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Pages src[i] over pages dst[i] in every layer; no page both source and target.  The
+/* Pages src[i] over pages dst[i] (distinct, none of them a source) in every layer.  The
  * tables stay as they are. */
 int h3b_pages_copy(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
 

@@ -576,22 +576,53 @@ __global__ void __launch_bounds__(256) compact_table_kernel(PageTables t, const 
     if (pg >= used && pg < t.pages) t.table[i] = p.to[pg];
   }
 }
-// Whole pages, K and V of every layer: a block per (move, layer, K/V).  Bound by memory: 1.07
-// GB moved in 364 us with the plan, 5.9 TB/s of reads and writes.  count: device
-// value (compact) or null (n moves, whose pages are checked here).
-__global__ void __launch_bounds__(256) move_kernel(PagePools pool, int pages, int64_t bytes, const int32_t* src,
-                                                   const int32_t* dst, const int32_t* count, int n, int32_t* status) {
+// A copy of pages: all of them in the pool, none copied to twice, none copied from and to.
+// The targets are marked in shared memory, kCheckPages pages of the pool at a time.
+constexpr int kCheckPages = 1 << 18;
+__global__ void __launch_bounds__(kPlanThreads) copy_check_kernel(const int32_t* src, const int32_t* dst, int n, int pages,
+                                                                  int32_t* status) {
+  extern __shared__ uint32_t target[];
+  const int tid = threadIdx.x;
   chain_next();
   chain_wait();
+  if (*status != kPagesOk) return;
+  bool bad = false;
+  for (int lo = 0; lo < pages; lo += kCheckPages) {
+    const int some = min(pages - lo, kCheckPages);
+    for (int i = tid; i < (some + 31) / 32; i += kPlanThreads) target[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kPlanThreads) {
+      const int d = dst[i];
+      if (d < 0 || d >= pages)
+        bad = true;
+      else if (d >= lo && d - lo < some)
+        bad |= (atomicOr(&target[(d - lo) >> 5], 1u << (d & 31)) >> (d & 31)) & 1u;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPlanThreads) {
+      const int s = src[i];
+      if (s < 0 || s >= pages)
+        bad = true;
+      else if (s >= lo && s - lo < some)
+        bad |= (target[(s - lo) >> 5] >> (s & 31)) & 1u;
+    }
+    __syncthreads();
+  }
+  if (__syncthreads_or(bad) && tid == 0) *status = kPagesBadPage;
+}
+// Whole pages, K and V of every layer: a block per (move, layer, K/V).  Bound by memory: 1.07
+// GB moved in 364 us with the plan, 5.9 TB/s of reads and writes.  count: device value
+// (compact), or null: n moves that copy_check_kernel let pass (status 0).
+__global__ void __launch_bounds__(256) move_kernel(PagePools pool, int pages, int64_t bytes, const int32_t* src,
+                                                   const int32_t* dst, const int32_t* count, int n, const int32_t* status) {
+  chain_next();
+  chain_wait();
+  if (!count && *status != kPagesOk) return;
   const int64_t units = (int64_t)(count ? *count : n) * pool.layers * 2;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t layer = u / 2 % pool.layers;
     const int i = (int)(u / 2 / pool.layers);
     const int s = src[i], d = dst[i];
-    if (s < 0 || s >= pages || d < 0 || d >= pages) {
-      if (status && threadIdx.x == 0) *status = kPagesBadPage;
-      continue;
-    }
     uint8_t* base = u & 1 ? pool.v : pool.k;
     const uint4* from = reinterpret_cast<const uint4*>(base + (layer * pages + s) * bytes);
     uint4* to = reinterpret_cast<uint4*>(base + (layer * pages + d) * bytes);
@@ -673,6 +704,9 @@ cudaError_t launch_pages_compact(const PageTables& t, const PagePools& p, int32_
 }
 cudaError_t launch_pages_copy(const PagePools& p, int pages, int page, const int32_t* src, const int32_t* dst, int n,
                               int32_t* status, cudaStream_t s) {
+  const cudaError_t e = launch_chained(copy_check_kernel, 1, kPlanThreads, seen_bytes(pages < kCheckPages ? pages : kCheckPages),
+                                       s, src, dst, n, pages, status);
+  if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)n * p.layers * 2;
   return launch_chained(move_kernel, units < kFullGrid ? units : kFullGrid, 256, 0, s, p, pages,
                         (int64_t)p.Hkv * page * 128 * p.elem, src, dst, nullptr, n, status);

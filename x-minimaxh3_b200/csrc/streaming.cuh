@@ -143,7 +143,7 @@ enum PageStatus : int {
   kPagesBadSlot = 3,     // a slot outside the table, or named twice in one call
   kPagesOccupied = 4,    // fork into a slot that holds tokens
   kPagesBadCount = 5,    // token counts that are negative, not ordered or beyond the length
-  kPagesBadPage = 6,     // a page outside the pool
+  kPagesBadPage = 6,     // a page outside the pool; in a copy, a target named twice or also a source
 };
 struct PageTables {
   int32_t* table;

@@ -35,7 +35,7 @@ STATUS_TEXT = {
     3: "a slot lies outside the table or was named twice",
     4: "fork into a slot that holds tokens",
     5: "token counts are negative, unordered or beyond the length",
-    6: "a page lies outside the pool",
+    6: "a page lies outside the pool, or was copied to twice, or both from and to",
 }
 
 
@@ -200,7 +200,7 @@ class PagedKVCache:
         check(lib().h3b_pages_compact(self._ref, _ptr(ws), ws.numel(), _stream(self.k)), "pages_compact")
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """Pages src[i] over pages dst[i] in every layer (no page may be both); the tables stay."""
+        """Pages src[i] over the distinct pages dst[i] in every layer (no page may be both); the tables stay."""
         n = _index(src, "src").numel()
         check(lib().h3b_pages_copy(self._ref, _ptr(src), _ptr(_index(dst, "dst", n)), n, _stream(self.k)), "pages_copy")
 
