@@ -60,17 +60,31 @@ def _index(t: torch.Tensor, what: str, n: int | None = None) -> torch.Tensor:
     return t
 
 
-def _token_rows(x: torch.Tensor, heads: int | None, what: str) -> torch.Tensor:
-    """[T, H, 128] fp16 / bf16 with contiguous heads (any row stride that keeps 16-byte alignment)."""
+def _row_step(x: torch.Tensor) -> int:
+    """Elements from one of x's rows [T, H, 128] to the next, if the kernels take them as they lie:
+    contiguous heads, 16-byte aligned rows apart from each other; else 0.  Strides of dimensions of one
+    entry, which may be anything, do not count."""
+    row, head, channel = x.stride()
+    tokens, heads, _ = x.shape
+    if channel != 1 or (head != HEAD_DIM and heads != 1) or x.data_ptr() % 16:
+        return 0
+    if tokens <= 1:
+        return heads * HEAD_DIM
+    return row if row % 8 == 0 and row >= heads * HEAD_DIM else 0
+
+
+def _token_rows(x: torch.Tensor, heads: int | None, what: str) -> tuple[torch.Tensor, int]:
+    """[T, H, 128] fp16 / bf16 rows and the step between them; copied where they do not lie right."""
     shape = x.shape
     if len(shape) != 3 or shape[2] != HEAD_DIM or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {HEAD_DIM}]")
     if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
         raise ValueError(f"{what} must be bfloat16 or float16")
-    row, head, channel = x.stride()
-    if channel != 1 or head != HEAD_DIM or row % 8 or row < shape[1] * HEAD_DIM or x.data_ptr() % 16:
-        x = x.contiguous()
-    return x
+    step = _row_step(x)
+    if not step:
+        # not contiguous(), which returns rows at an odd address, and any single row, as they are
+        x, step = x.clone(memory_format=torch.contiguous_format), shape[1] * HEAD_DIM
+    return x, step
 
 
 @dataclass
@@ -157,7 +171,8 @@ class PagedKVCache:
         n = _index(slots, "slots").shape[0]
         if starts is not None:
             _index(starts, "starts", n + 1)
-        k, v = _token_rows(k, self.kv_heads, "k"), _token_rows(v, self.kv_heads, "v")
+        k, k_step = _token_rows(k, self.kv_heads, "k")
+        v, v_step = _token_rows(v, self.kv_heads, "v")
         if not (k.is_cuda and v.is_cuda):
             raise RuntimeError("PagedKVCache takes only CUDA tensors (the B200 library has no CPU path)")
         if k.shape != v.shape or k.dtype is not v.dtype:
@@ -166,8 +181,8 @@ class PagedKVCache:
             raise ValueError("without starts there is one token for each slot")
         if self.k.dtype is not k.dtype and self.k.dtype is not torch.float8_e4m3fn:
             raise ValueError(f"a {self.k.dtype} cache does not take {k.dtype} rows")
-        args = (self._ref, int(layer), slots.data_ptr(), n, _ptr(starts), k.data_ptr(), k.stride(0), v.data_ptr(),
-                v.stride(0), DTYPE_CODES[k.dtype], k.shape[0])
+        args = (self._ref, int(layer), slots.data_ptr(), n, _ptr(starts), k.data_ptr(), k_step, v.data_ptr(),
+                v_step, DTYPE_CODES[k.dtype], k.shape[0])
         if ws is not None:
             args += (ws.data_ptr(), ws.shape[0])
         check(entry(*args, _stream(self.k)), what)

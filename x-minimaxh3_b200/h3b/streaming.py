@@ -26,7 +26,7 @@ import torch
 
 from . import context as _context
 from ._lib import check, lib
-from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _ptr, _stream, _token_rows
+from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _ptr, _row_step, _stream, _token_rows
 
 UNLIMITED = 1 << 30
 
@@ -39,15 +39,15 @@ def _rule(window: int | None, sinks: int, chunk: int) -> tuple[int, int, int]:
     return window, sinks, chunk
 
 
-def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+def _output(out: torch.Tensor | None, q: torch.Tensor) -> tuple[torch.Tensor, int]:
     if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
+        return torch.empty_like(q, memory_format=torch.contiguous_format), q.shape[1] * HEAD_DIM
     if out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda:
         raise ValueError("out must have q's shape and type")
-    st = out.stride()
-    if st[2] != 1 or st[1] != HEAD_DIM or st[0] % 8 or st[0] < q.shape[1] * HEAD_DIM or out.data_ptr() % 16:
+    step = _row_step(out)
+    if not step:
         raise ValueError("out must have contiguous heads and 16-byte aligned rows")
-    return out
+    return out, step
 
 
 def _scale(scale: float | None) -> float:
@@ -82,7 +82,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     calls on one stream."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError("window_attention runs only on CUDA tensors (the B200 library has no CPU path)")
-    q, k, v = _token_rows(q, None, "q"), _token_rows(k, None, "k"), _token_rows(v, None, "v")
+    (q, q_step), (k, k_step), (v, v_step) = (_token_rows(q, None, "q"), _token_rows(k, None, "k"),
+                                             _token_rows(v, None, "v"))
     if k.shape != v.shape or not q.dtype is k.dtype is v.dtype:
         raise ValueError("k and v must have one shape, and q their type")
     if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
@@ -96,25 +97,25 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         _index(key_starts, "key_starts", seqs + 1)
         if seqs < 1:
             raise ValueError("query_starts needs at least two entries")
-    out = _output(out, q)
+    out, out_step = _output(out, q)
     workspace, size = _window_workspace(workspace, q, seqs, k.shape[1], k.shape[0], (window, sinks, chunk))
-    check(lib().h3b_window_attention(_ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), DTYPE_CODES[q.dtype],
-                                     q.shape[0], k.shape[0], _ptr(query_starts), _ptr(key_starts), seqs, q.shape[1],
-                                     k.shape[1], window, sinks, chunk, _scale(scale), _ptr(out), out.stride(0),
-                                     _ptr(workspace), size, _stream(q)), "window_attention")
+    check(lib().h3b_window_attention(_ptr(q), q_step, _ptr(k), k_step, _ptr(v), v_step,
+                                     DTYPE_CODES[q.dtype], q.shape[0], k.shape[0], _ptr(query_starts), _ptr(key_starts),
+                                     seqs, q.shape[1], k.shape[1], window, sinks, chunk, _scale(scale), _ptr(out),
+                                     out_step, _ptr(workspace), size, _stream(q)), "window_attention")
     return out
 
 
-def _cached_queries(q: torch.Tensor, cache: PagedKVCache, layer: int, what: str) -> torch.Tensor:
+def _cached_queries(q: torch.Tensor, cache: PagedKVCache, layer: int, what: str) -> tuple[torch.Tensor, int]:
     if not q.is_cuda:
         raise RuntimeError(f"{what} runs only on CUDA tensors (the B200 library has no CPU path)")
-    q = _token_rows(q, None, "q")
+    q, step = _token_rows(q, None, "q")
     heads = q.shape[1]
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError("the query heads must be a multiple of the kv heads")
     if not 0 <= layer < cache.k.shape[0]:
         raise ValueError(f"the cache has no layer {layer}")
-    return q
+    return q, step
 
 
 def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor | None = None, *,
@@ -123,7 +124,7 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
                            workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q [Tq, Hq, 128]: the last tokens of the cache's sequences `slots` (int32; None: slot 0, 1, ...),
     already appended.  query_starts: int32 [sequences + 1]; None: one sequence."""
-    q = _cached_queries(q, cache, layer, "paged_window_attention")
+    q, q_step = _cached_queries(q, cache, layer, "paged_window_attention")
     if cache.k.dtype != q.dtype:
         raise ValueError(f"a {cache.k.dtype} cache does not serve {q.dtype} queries of several tokens")
     window, sinks, chunk = _rule(window, sinks, chunk)
@@ -134,12 +135,12 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
         _index(slots, "slots", seqs)
     elif seqs > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
-    out = _output(out, q)
+    out, out_step = _output(out, q)
     workspace, size = _window_workspace(workspace, q, seqs, cache.kv_heads, cache.table.shape[1] * cache.page_tokens,
                                         (window, sinks, chunk))
-    check(lib().h3b_paged_window_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], q.shape[0], _ptr(query_starts),
+    check(lib().h3b_paged_window_attention(_ptr(q), q_step, DTYPE_CODES[q.dtype], q.shape[0], _ptr(query_starts),
                                            _ptr(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
-                                           _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), size, _stream(q)),
+                                           _scale(scale), _ptr(out), out_step, _ptr(workspace), size, _stream(q)),
           "paged_window_attention")
     return out
 
@@ -149,7 +150,7 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
                      out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q [n, Hq, 128]: the last token of each of the cache's sequences `slots` (int32 [n]; None: slots
     0..n-1), already appended -> [n, Hq, 128].  workspace: uint8, reused by calls on one stream."""
-    q = _cached_queries(q, cache, layer, "decode_attention")
+    q, q_step = _cached_queries(q, cache, layer, "decode_attention")
     if cache.k.dtype not in (q.dtype, torch.float8_e4m3fn):
         raise ValueError(f"a {cache.k.dtype} cache does not serve {q.dtype} queries")
     window, sinks, _ = _rule(window, sinks, 1)
@@ -161,9 +162,9 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
     need = lib().h3b_decode_workspace_bytes(n, q.shape[1], cache._ref)
     if need:
         workspace = _workspace(workspace, need, q)
-    out = _output(out, q)
-    check(lib().h3b_decode_attention(_ptr(q), q.stride(0), DTYPE_CODES[q.dtype], _ptr(slots), n, q.shape[1], cache._ref,
-                                     layer, window, sinks, _scale(scale), _ptr(out), out.stride(0), _ptr(workspace), need,
+    out, out_step = _output(out, q)
+    check(lib().h3b_decode_attention(_ptr(q), q_step, DTYPE_CODES[q.dtype], _ptr(slots), n, q.shape[1], cache._ref,
+                                     layer, window, sinks, _scale(scale), _ptr(out), out_step, _ptr(workspace), need,
                                      _stream(q)), "decode_attention")
     return out
 
