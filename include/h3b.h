@@ -418,7 +418,7 @@ typedef struct h3b_page_cache {
 #define H3B_PAGES_TOO_LONG 2  /* a sequence would outgrow its row of the table */
 #define H3B_PAGES_BAD_SLOT 3  /* a slot outside the table, or named twice */
 #define H3B_PAGES_OCCUPIED 4  /* fork into a slot that holds tokens */
-#define H3B_PAGES_BAD_COUNT 5 /* token counts negative, unordered or beyond the length */
+#define H3B_PAGES_BAD_COUNT 5 /* token counts negative, unordered or beyond the length or the rows */
 #define H3B_PAGES_BAD_PAGE 6  /* a page outside the pool, or copied to twice, or both from and to */
 
 /* Window attention over contiguous K/V.  q, out: rows [Tq, Hq * 128] with their strides;
@@ -469,7 +469,8 @@ int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* s
                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
                     int64_t tokens, void* stream);
 
-/* h3b_pages_extend, then h3b_pages_write into `layer`, in two launches. */
+/* h3b_pages_extend, then h3b_pages_write into `layer`, in two launches.  Starts that reach
+ * past the rows (starts[n] > tokens) are refused; rows outside every sequence are not used. */
 int h3b_pages_append(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
                      const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
                      int64_t tokens, void* workspace, int64_t workspace_bytes, void* stream);

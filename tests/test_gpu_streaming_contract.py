@@ -86,3 +86,46 @@ def test_page_copies_of_a_pool_of_many_pages():
     cache.check()
     want[0, dst.long()] = want[0, src.long()]
     assert torch.equal(cache.k.view(torch.uint8), want) and torch.equal(cache.v.view(torch.uint8), want)
+
+
+# ------------------------------------------------------------------------------ append
+
+@pytest.mark.parametrize("slots,starts", [([2], [0, 9]), ([2, 3], [0, 2, 5]), ([2, 3], [0, 5, 5]), ([2], [-1, 2]),
+                                          ([4, 2, 3], [-4, 0, 2, 4])], ids=str)
+def test_appends_of_more_tokens_than_rows_are_refused(slots, starts):
+    """Four rows come with the call; lengths would grow over rows that are never written."""
+    from h3b import H3BError
+
+    cache, host = _filled()
+    cache.append(_i32(slots), _rows(4), _rows(4), _i32(starts))
+    host.assert_equal(cache)
+    with pytest.raises(H3BError, match="beyond the length or the rows"):
+        cache.check()
+
+
+def test_appends_may_leave_rows_unused():
+    """A buffer of more rows than the starts name, as a captured graph has, and rows before the first."""
+    for starts in ([0, 1, 3], [2, 3, 4], [1, 1, 1]):
+        cache, host = _filled()
+        k, v = _rows(4, seed=5), _rows(4, seed=6)
+        cache.append(_i32([2, 0]), k, v, _i32(starts))
+        counts = [starts[1] - starts[0], starts[2] - starts[1]]
+        host.extend([2, 0], counts)
+        host.write([2, 0], counts, k[starts[0]:], v[starts[0]:])
+        cache.check()
+        host.assert_equal(cache, str(starts))
+
+
+def test_an_append_behind_a_page_that_is_gone_is_refused():
+    """A table whose partly filled last page is no page of the pool: the rows would have no place."""
+    from h3b import H3BError
+
+    for page in (-1, 8, 1 << 28):
+        for call in (lambda c: c.append(_i32([2, 0]), _rows(2), _rows(2)), lambda c: c.extend(_i32([2, 0]))):
+            cache, host = _filled()
+            cache.table[0, 1] = page
+            host.table[0, 1] = page
+            call(cache)
+            host.assert_equal(cache)
+            with pytest.raises(H3BError, match="outside the pool"):
+                cache.check()

@@ -754,7 +754,7 @@ int h3b_pages_extend(const h3b_page_cache* cache, const int32_t* slots, int64_t 
   if (!workspace || workspace_bytes < h3b::pages_workspace_bytes(n, cache->pages))
     return fail(H3B_ERR_INVALID_ARGUMENT, "pages_extend: workspace too small");
   return cuda_status(h3b::launch_pages_extend(page_tables(cache), page_pools(cache), slots, (int)n, starts,
-                                              static_cast<int32_t*>(workspace), true, st(stream)), "pages_extend");
+                                              -1, static_cast<int32_t*>(workspace), st(stream)), "pages_extend");
 }
 
 }  // extern "C"
@@ -820,7 +820,7 @@ int h3b_pages_append(const h3b_page_cache* cache, int64_t layer, const int32_t* 
   if (!workspace || workspace_bytes < h3b::pages_workspace_bytes(n, cache->pages))
     return fail(H3B_ERR_INVALID_ARGUMENT, "pages_append: workspace too small");
   int32_t* ws = static_cast<int32_t*>(workspace);
-  const cudaError_t e = h3b::launch_pages_extend(page_tables(cache), page_pools(cache), slots, (int)n, starts, ws, false,
+  const cudaError_t e = h3b::launch_pages_extend(page_tables(cache), page_pools(cache), slots, (int)n, starts, tokens, ws,
                                                  st(stream));
   if (e != cudaSuccess) return cuda_status(e, "pages_append");
   return cuda_status(h3b::launch_pages_write(page_tables(cache), page_pools(cache), layer, w, ws, st(stream)),

@@ -113,8 +113,9 @@ __host__ __device__ __forceinline__ ExtendPlan extend_plan(int32_t* ws, int n) {
 // Bound by the latency of its dependent loads (status, slots, lengths, tables, counts): about
 // half of the 11 us of a token's append to 200 sequences and its truncation.  One block,
 // because the pages of a sequence depend on what all before it ask for.
+// tokens: rows that come with the call (append), or -1: starts may not reach past them.
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t, const int32_t* slots, int n,
-                                                                   const int32_t* starts, int32_t* ws) {
+                                                                   const int32_t* starts, int64_t tokens, int32_t* ws) {
   extern __shared__ uint32_t seen[];
   __shared__ int red[kPlanWarps], ends[kPlanThreads], col[kPlanThreads], first_of[kPlanThreads];
   __shared__ int copies, fault;
@@ -138,6 +139,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t,
   }
   // pages asked for by each sequence, and where its share of them begins
   int carry = 0, error = 0, my_asked = 0, my_first = 0;
+  if (starts && tokens >= 0 && tid == 0 && (starts[0] < 0 || starts[n] > tokens)) error = kPagesBadCount;
   for (int base = 0; base < n; base += kPlanThreads) {
     const int i = base + tid;
     int asked = 0;
@@ -153,7 +155,10 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t,
         asked = pages_of(len + (int)count, t.page) - have;
         if (len % t.page && count > 0) {
           const int last = t.table[(int64_t)slot * t.width + have - 1];
-          if (last >= 0 && last < t.pages && t.refs[last] > 1) ++asked;
+          if (last < 0 || last >= t.pages)
+            error = kPagesBadPage;
+          else if (t.refs[last] > 1)
+            ++asked;
         }
       }
     }
@@ -651,9 +656,10 @@ int64_t pages_workspace_bytes(int64_t n, int64_t pages) {
 constexpr int kFullGrid = 1184;  // eight blocks for each of 148 multiprocessors
 
 cudaError_t launch_pages_extend(const PageTables& t, const PagePools& p, const int32_t* slots, int n,
-                                const int32_t* starts, int32_t* ws, bool copy, cudaStream_t s) {
-  const cudaError_t e = launch_chained(extend_plan_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, n, starts, ws);
-  if (e != cudaSuccess || !copy) return e;
+                                const int32_t* starts, int64_t tokens, int32_t* ws, cudaStream_t s) {
+  const cudaError_t e =
+      launch_chained(extend_plan_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, slots, n, starts, tokens, ws);
+  if (e != cudaSuccess || tokens >= 0) return e;
   const int64_t most = ((int64_t)n * p.layers * 2 * p.Hkv + 7) / 8;
   return launch_chained(extend_copy_kernel, most < kFullGrid ? most : kFullGrid, 256, 0, s, p, t.pages, t.page, n, ws);
 }

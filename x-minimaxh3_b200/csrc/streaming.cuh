@@ -161,9 +161,10 @@ struct PagePools {
 };
 constexpr int kPagesMaxRows = 1 << 18;
 int64_t pages_workspace_bytes(int64_t n, int64_t pages);
-// copy: whether to make the planned copies too (launch_pages_write can)
+// tokens: -1, or the rows that launch_pages_write will take next, which then makes the
+// planned copies too
 cudaError_t launch_pages_extend(const PageTables& t, const PagePools& p, const int32_t* slots, int n,
-                                const int32_t* starts, int32_t* ws, bool copy, cudaStream_t s);
+                                const int32_t* starts, int64_t tokens, int32_t* ws, cudaStream_t s);
 struct PageWriteArgs {
   const uint16_t* k;
   int64_t k_stride;

@@ -34,7 +34,7 @@ STATUS_TEXT = {
     2: "a sequence would outgrow its row of the table",
     3: "a slot lies outside the table or was named twice",
     4: "fork into a slot that holds tokens",
-    5: "token counts are negative, unordered or beyond the length",
+    5: "token counts are negative, unordered or beyond the length or the rows",
     6: "a page lies outside the pool, or was copied to twice, or both from and to",
 }
 
@@ -189,7 +189,8 @@ class PagedKVCache:
 
     def append(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | None = None,
                layer: int = 0) -> None:
-        """extend, then write into `layer` (the other layers' rows are the caller's to write)."""
+        """extend, then write into `layer` (the other layers' rows are the caller's to write).  Rows outside
+        every sequence are not used; starts that reach past the rows are refused."""
         self._rows_into(lib().h3b_pages_append, "pages_append", slots, k, v, starts, layer,
                         self._workspace(slots.shape[0]))
 
