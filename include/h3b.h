@@ -463,8 +463,9 @@ int h3b_pages_extend(const h3b_page_cache* cache, const int32_t* slots, int64_t 
                      void* workspace, int64_t workspace_bytes, void* stream);
 
 /* K/V rows [tokens, kv_heads * 128] (fp16 or bf16, row strides) into the last
- * starts[i + 1] - starts[i] tokens (NULL: one) of each slot, in one layer.  An e4m3
- * pool holds x / scale, rounded to nearest even, saturated at +-448. */
+ * starts[i + 1] - starts[i] tokens (NULL: one) of each of the n distinct slots, in one
+ * layer; refused as a whole where a slot, its length, the rows or the pages do not fit.
+ * An e4m3 pool holds x / scale, rounded to nearest even, saturated at +-448. */
 int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
                     int64_t tokens, void* stream);

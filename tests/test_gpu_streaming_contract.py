@@ -129,3 +129,98 @@ def test_an_append_behind_a_page_that_is_gone_is_refused():
             host.assert_equal(cache)
             with pytest.raises(H3BError, match="outside the pool"):
                 cache.check()
+
+
+# ------------------------------------------------------------------------------ write
+
+@pytest.mark.parametrize("slots,starts,why", [
+    ([6], [0, 2], "a slot lies outside"), ([-1], [0, 2], "a slot lies outside"), ([0, 7], [0, 2, 4], "a slot lies outside"),
+    ([0, 0], [0, 1, 2], "named twice"), ([2], [0, 1], "beyond the length"), ([0], [0, 21], "beyond the length"),
+    ([1, 0], [0, 30, 51], "beyond the length"), ([0, 1], [0, 20, 51], "beyond the length"), ([0, 1], [0, 2, 1], "unordered"),
+    ([0], [-1, 2], "negative"), ([0], None, None), ([2], None, "beyond the length"), ([0, 1], [0, 20, 50], None),
+    ([0, 2, 1], [3, 9, 9, 12], None),
+], ids=str)
+def test_writes_are_done_whole_or_not_at_all(slots, starts, why):
+    from h3b import H3BError
+
+    cache, host = _filled()
+    rows = len(slots) if starts is None else 50
+    k, v = _rows(rows, seed=7), _rows(rows, seed=8)
+    cache.write(_i32(slots), k, v, None if starts is None else _i32(starts))
+    if why is None:
+        first = 0 if starts is None else starts[0]
+        host.write(slots, [1] if starts is None else [b - a for a, b in zip(starts, starts[1:])], k[first:], v[first:])
+        cache.check()
+    else:
+        with pytest.raises(H3BError, match=why):
+            cache.check()
+    host.assert_equal(cache)
+
+
+def test_writes_into_pages_that_are_gone_are_refused():
+    """Also where the page lies among the many that a long write fills."""
+    from h3b import H3BError, PagedKVCache
+
+    cache = PagedKVCache.create(1, 3200, 16, 1, 1100, 16 * 2100)
+    slots = list(range(1099, -1, -1))
+    counts = [16 * 2000 - 3] + [1] * 1023 + [2] * 76
+    at = [0]
+    for n in counts:
+        at.append(at[-1] + n)
+    k = _rows(at[-1], heads=1)
+    cache.extend(_i32(slots[:1024]), _i32(at[:1025]))
+    cache.extend(_i32(slots[1024:]), _i32(at[1024:]))
+    cache.check()
+    want = cache.k.clone()
+    for slot, col in ((1099, 1234), (3, 0)):
+        page = int(cache.table[slot, col])
+        for gone in (-1, 3200):
+            cache.table[slot, col] = gone
+            cache.write(_i32(slots), k, k, _i32(at))
+            with pytest.raises(H3BError, match="outside the pool"):
+                cache.check()
+            assert torch.equal(cache.k.view(torch.int16), want.view(torch.int16))
+        cache.table[slot, col] = page
+    cache.write(_i32(slots), k, k, _i32(at))
+    cache.check()
+    got = cache.k[0, cache.table[1099, :2000].long()].reshape(-1, 1, D)[: at[1]]
+    assert torch.equal(got, k[: at[1]])
+    assert torch.equal(cache.k[0, cache.table[3, 0].long(), 0, :2], k[at[1096]:at[1097], 0])
+
+
+@pytest.mark.parametrize("slots,tokens", [(8192, 512), (8192, 513), (8193, 500), (600, 100)], ids=str)
+def test_writes_around_what_each_block_checks_itself(slots, tokens):
+    """Ragged writes on both sides of the sizes at which a launch of its own checks the call."""
+    from h3b import H3BError, PagedKVCache
+
+    cache = PagedKVCache.create(1, 1400, 16, 1, slots, 1024)
+    n = 600 if slots == 600 else 17
+    order = torch.randperm(slots, generator=torch.Generator().manual_seed(slots))[:n].tolist()
+    counts = [0] * n
+    for i in range(n):
+        counts[i] = tokens // n + (i < tokens % n)
+    counts[0], counts[5] = counts[0] + counts[5], 0
+    at = [0]
+    for c in counts:
+        at.append(at[-1] + c)
+    assert at[-1] == tokens
+    cache.extend(_i32(order), _i32(at))
+    cache.check()
+    host = HostCache(cache)
+    k, v = _rows(tokens, heads=1, seed=3), _rows(tokens, heads=1, seed=4)
+    for bad_slots, bad_at, why in ((order[:-1] + order[:1], at, "named twice"), (order[:-1] + [slots], at, "outside the table"),
+                                   (order[5:6] + order[1:5] + order[:1] + order[6:], at, "beyond the length")):
+        cache.write(_i32(bad_slots), k, v, _i32(bad_at))
+        with pytest.raises(H3BError, match=why):
+            cache.check()
+    page = int(cache.table[order[0], 0])
+    cache.table[order[0], 0] = 1400
+    cache.write(_i32(order), k, v, _i32(at))
+    with pytest.raises(H3BError, match="outside the pool"):
+        cache.check()
+    cache.table[order[0], 0] = page
+    host.assert_equal(cache)
+    cache.write(_i32(order), k, v, _i32(at))
+    host.write(order, counts, k, v)
+    cache.check()
+    host.assert_equal(cache)

@@ -73,12 +73,13 @@ __device__ __forceinline__ void block_expand(int count, int* red, int* ends, L l
 // Every slot named by slots[0, n) lies in the table and is named once.  seen: a bit per
 // row, zeroed here.  Returns false to every thread if not.  mine: the thread's slots[tid],
 // loaded by the caller (n > tid).
+template <int THREADS = kPlanThreads>
 __device__ bool slots_valid(const int32_t* slots, int n, int rows, uint32_t* seen, int mine) {
-  for (int i = threadIdx.x; i < (rows + 31) / 32; i += kPlanThreads) seen[i] = 0;
+  for (int i = threadIdx.x; i < (rows + 31) / 32; i += THREADS) seen[i] = 0;
   __syncthreads();
   bool bad = false;
-  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-    const int s = i < kPlanThreads ? mine : slots[i];
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const int s = i < THREADS ? mine : slots[i];
     if (s < 0 || s >= rows)
       bad = true;
     else
@@ -309,7 +310,74 @@ __device__ __forceinline__ uint4 to_e4m3x16(const uint4& a, const uint4& b, floa
   return make_uint4(to_e4m3x4(widen4<BF16>(a.x, a.y), scale, rb), to_e4m3x4(widen4<BF16>(a.z, a.w), scale, rb),
                     to_e4m3x4(widen4<BF16>(b.x, b.y), scale, rb), to_e4m3x4(widen4<BF16>(b.z, b.w), scale, rb));
 }
-// Element offset in a layer's pool of kv head 0 of row `tok` of the new rows; -1: nowhere.
+// A write by itself (an append's plan has seen to it): the slots are distinct ones of the
+// table, each holds as many tokens as it gets rows, the rows are there, and so are the pages.
+__device__ __forceinline__ int64_t write_count(const PageWriteArgs& w, int i) {
+  return w.starts ? (int64_t)w.starts[i + 1] - w.starts[i] : 1;
+}
+// The status for all but the pages, to every thread.
+template <int THREADS>
+__device__ __forceinline__ int write_fault(const PageTables& t, const PageWriteArgs& w, uint32_t* seen) {
+  if (!slots_valid<THREADS>(w.slots, w.n, t.rows, seen, (int)threadIdx.x < w.n ? w.slots[threadIdx.x] : 0))
+    return kPagesBadSlot;
+  bool bad = w.starts && (w.starts[0] < 0 || w.starts[w.n] > w.tokens);
+  for (int i = threadIdx.x; i < w.n; i += THREADS) {
+    const int64_t count = write_count(w, i), len = t.lens[w.slots[i]];
+    bad |= count < 0 || count > len || len > (int64_t)t.width * t.page;
+  }
+  return __syncthreads_or(bad) ? kPagesBadCount : kPagesOk;
+}
+__global__ void __launch_bounds__(kPlanThreads) write_check_kernel(PageTables t, PageWriteArgs w) {
+  extern __shared__ uint32_t seen[];
+  __shared__ int red[kPlanWarps], ends[kPlanThreads], col[kPlanThreads];
+  const int tid = threadIdx.x;
+  chain_next();
+  chain_wait();
+  if (*t.status != kPagesOk) return;
+  int fault = write_fault<kPlanThreads>(t, w, seen);
+  if (!fault) {
+    bool bad = false;
+    for (int base = 0; base < w.n; base += kPlanThreads) {
+      const int i = base + tid;
+      int pages = 0;
+      if (i < w.n) {
+        const int len = t.lens[w.slots[i]], count = (int)write_count(w, i);
+        col[tid] = (len - count) / t.page;
+        pages = count ? pages_of(len, t.page) - col[tid] : 0;
+      }
+      block_expand(
+          pages, red, ends,
+          [&](int owner, int x) { return t.table[(int64_t)w.slots[base + owner] * t.width + col[owner] + x]; },
+          [&](int, int, int page) { bad |= page < 0 || page >= t.pages; });
+    }
+    if (__syncthreads_or(bad)) fault = kPagesBadPage;
+  }
+  if (fault && tid == 0) *t.status = fault;
+}
+// The same by each block of a small write, so that it needs no launch of its own: 200 tokens
+// into one layer 9.9 us from the host, with write_check_kernel before it 13.7 us.  All blocks
+// come to the same answer, whether or not one of them has already reported it.
+constexpr int kOwnCheckTokens = 512, kOwnCheckRows = 8192;
+__device__ __forceinline__ bool write_fits(const PageTables& t, const PageWriteArgs& w, uint32_t* seen) {
+  int fault = write_fault<256>(t, w, seen);
+  if (!fault) {
+    bool bad = false;
+    for (int i = threadIdx.x; i < w.n; i += 256) {
+      const int slot = w.slots[i], len = t.lens[slot], count = (int)write_count(w, i);
+      const int end = count ? pages_of(len, t.page) : 0;
+      for (int col = (len - count) / t.page; col < end; ++col) {
+        const int page = t.table[(int64_t)slot * t.width + col];
+        bad |= page < 0 || page >= t.pages;
+      }
+    }
+    if (__syncthreads_or(bad)) fault = kPagesBadPage;
+  }
+  if (fault && blockIdx.x == 0 && threadIdx.x == 0 && *t.status == kPagesOk) *t.status = fault;
+  return !fault;
+}
+
+// Element offset in a layer's pool of kv head 0 of row `tok` of the new rows; -1: of no
+// sequence.  (All else was checked before, by the plan, write_check_kernel or write_fits.)
 __device__ __forceinline__ int64_t row_place(const PageTables& t, const PageWriteArgs& w, int Hkv, int64_t tok) {
   int i = (int)tok, back = 1;  // the token is the back-th last of sequence i
   if (w.starts) {
@@ -334,12 +402,17 @@ __device__ __forceinline__ int64_t row_place(const PageTables& t, const PageWrit
 // all their rows are under way together.  Bound by memory: 32,600 tokens of 8 kv heads into
 // an E4M3 cache, with the plan before it, 50 us (4.0 TB/s; 46 where L2 holds some of the
 // rows), half of the issue slots taken by the conversion.
-template <bool FP8, bool BF16>
+// CHECK: the call is one that its blocks check; else it was checked before.
+template <bool FP8, bool BF16, bool CHECK>
 __global__ void __launch_bounds__(256) write_kernel(PageTables t, PagePools pool, int64_t layer, PageWriteArgs w,
                                                     const int32_t* ws, int copy_blocks, int per) {
   __shared__ int64_t place[8];
   chain_next();
   chain_wait();
+  if constexpr (CHECK) {
+    __shared__ uint32_t seen[kOwnCheckRows / 32];
+    if (!write_fits(t, w, seen)) return;
+  }
   if ((int)blockIdx.x < copy_blocks) {  // rows of other places of the same pages
     copy_shared_rows(pool, t.pages, t.page, w.n, ws, (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5),
                      (int64_t)copy_blocks * 8);
@@ -671,7 +744,14 @@ cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t 
     copies = ((int64_t)w.n * p.layers * 2 * p.Hkv + 7) / 8;
     if (copies > kFullGrid / 2) copies = kFullGrid / 2;
   }
-  auto kern = p.elem == 2 ? write_kernel<false, true> : w.src_bf16 ? write_kernel<true, true> : write_kernel<true, false>;
+  const bool own_check = !ws && w.tokens <= kOwnCheckTokens && w.n <= kOwnCheckTokens && t.rows <= kOwnCheckRows;
+  if (!ws && !own_check) {
+    const cudaError_t e = launch_chained(write_check_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, w);
+    if (e != cudaSuccess) return e;
+  }
+  auto kern = p.elem == 2    ? (own_check ? write_kernel<false, true, true> : write_kernel<false, true, false>)
+              : w.src_bf16 ? (own_check ? write_kernel<true, true, true> : write_kernel<true, true, false>)
+                           : (own_check ? write_kernel<true, false, true> : write_kernel<true, false, false>);
   // two blocks for each multiprocessor first, then up to 8 tokens a block
   int64_t per = w.tokens / (kFullGrid / 4);
   per = per < 1 ? 1 : per > 8 ? 8 : per;

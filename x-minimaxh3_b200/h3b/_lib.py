@@ -168,7 +168,7 @@ def lib():
 
 # kernels each entry launches (for the benchmark's launch count); default 1
 _KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2, "decode_attention": 2, "pages_extend": 2, "pages_append": 2,
-                     "pages_compact": 3, "pages_copy": 2}
+                     "pages_compact": 3, "pages_copy": 2, "pages_write": 2}
 _launches = 0
 
 

@@ -164,7 +164,8 @@ class PagedKVCache:
 
     def write(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | None = None,
               layer: int = 0) -> None:
-        """K/V rows [tokens, kv heads, 128] into the last tokens of each slot, as `extend` made room for them."""
+        """K/V rows [tokens, kv heads, 128] into the last tokens of each of the distinct slots, as `extend` made
+        room for them."""
         self._rows_into(lib().h3b_pages_write, "pages_write", slots, k, v, starts, layer)
 
     def _rows_into(self, entry, what, slots, k, v, starts, layer, ws=None) -> None:
