@@ -394,7 +394,8 @@ __device__ __noinline__ void add_nonfinite(const WindowArgs& a, const WinPlan& p
 // each CTA what it lacks.  A boundary that falls into an item there cuts it, unless the
 // item is short (kCutFrom) or the piece would be (kLeastPiece): then it moves to the
 // item's nearer end.  The pieces of a cut item leave their sums, and window_join_kernel
-// puts them together.
+// puts them together.  Where no item is cut (window_cuts) all are dealt whole, tiles from the
+// first on.
 constexpr int kItemCost = 4;
 constexpr int kCutFrom = 8;
 constexpr int kLeastPiece = 3;
@@ -415,25 +416,51 @@ __device__ __forceinline__ int tiles_of(const WindowArgs& a, int seq, int rows_p
 struct TileAt {
   int seq, t;
 };
-// Tile t of all, found by the whole warp.
-__device__ TileAt find_tile(const WindowArgs& a, int t, int rows_per_cta) {
+// Where a warp looked for a tile last (in shared memory: few calls need it): the 32 sequences
+// from `base`, and the tiles before them.
+struct SeqsAt {
+  long long before;
+  int base;
+};
+// Tile t of all, found by the whole warp from where it looked last: a CTA's tiles follow each
+// other, and a search from the first sequence for each took the square of their number (65,536
+// sequences of a token 153 ms).
+__device__ __forceinline__ TileAt find_tile(const WindowArgs& a, int t, int rows_per_cta, SeqsAt* last) {
   const int lane = threadIdx.x & 31;
-  for (int base = 0; base < a.seqs; base += 32) {
-    const int n = base + lane < a.seqs ? tiles_of(a, base + lane, rows_per_cta) : 0;
+  SeqsAt at = *last;
+  TileAt found{-1, 0};
+  for (;;) {
+    const bool back = t < at.before && at.base > 0;
+    if (back) at.base -= 32;
+    else if (at.base >= a.seqs) break;
+    const int n = at.base + lane < a.seqs ? tiles_of(a, at.base + lane, rows_per_cta) : 0;
     int x = n;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, t < x);
+    const int all = __shfl_sync(0xffffffffu, x, 31);
+    if (back) at.before -= all;
+    if (at.base == 0) at.before = 0;
+    if (t < at.before) continue;
+    const unsigned hit = __ballot_sync(0xffffffffu, t - at.before < x);
     if (hit) {
       const int w = __ffs(hit) - 1;
-      return {base + w, t - __shfl_sync(0xffffffffu, x - n, w)};
+      found = {at.base + w, t - (int)at.before - __shfl_sync(0xffffffffu, x - n, w)};
+      break;
     }
-    t -= __shfl_sync(0xffffffffu, x, 31);
+    at.before += all;
+    at.base += 32;
   }
-  return {-1, 0};
+  if (lane == 0) *last = at;
+  return found;
+}
+// The same out of the way of the planner's code: the paged kernel is faster with it there, the
+// other one with it in place (six follow-ups of 90 tokens: 75.3 / 77.2 us, 8,192 tokens:
+// 422 / 415 us; neither call comes here).
+__device__ __noinline__ TileAt find_tile_apart(const WindowArgs& a, int t, int rows_per_cta, SeqsAt* last) {
+  return find_tile(a, t, rows_per_cta, last);
 }
 
 // Everything about a tile's item but its column and its piece, by the whole warp: lanes 0
@@ -572,6 +599,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     WorkShare work;
     long long scan[kWinThreads / 32];
     float l[2][128];  // row sums of the item that warps 12..15 write
+    SeqsAt seqs_at;
   };
   static_assert(sizeof(Rest) <= kWinSmem - kWinOffRest, "shared memory");
   Rest& rest = *reinterpret_cast<Rest*>(smem + kWinOffRest);
@@ -638,6 +666,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     for (int s = 0; s < 8; ++s) mbar_init(&turns[s], 1);
     *abort_flag = 0;
     cleared[0] = cleared[1] = cleared[2] = 0;
+    rest.seqs_at = {0, 0};
     fence_mbar_init();
   }
   chain_next();
@@ -805,10 +834,11 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         const int item = round ? (int)blockIdx.x + made * (int)gridDim.x : w.item, q = item / columns;
         const int entry = round ? made : rounds + q - dealt_tile;
         TileAt at_tile;
-        if (a.notes && entry < kListed)
+        if (__builtin_expect(a.notes && entry < kListed, 1))
           at_tile = work.tile[entry];
         else
-          at_tile = find_tile(a, work.valid - 1 - q, rows_per_cta);
+          at_tile = (PAGED ? find_tile_apart : find_tile)(a, a.notes ? work.valid - 1 - q : q, rows_per_cta,
+                                                          &rest.seqs_at);
         const int steps = plan_tile<PAGED>(a, at_tile, rows_per_cta, pl);
         const int from = round ? 0 : w.step, to = !round && item == stop.item ? stop.step : steps;
         const bool cut = from > 0 || to < steps;
