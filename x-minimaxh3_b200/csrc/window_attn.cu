@@ -590,10 +590,12 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // the swizzled tiles and the room behind them count on it
     if (threadIdx.x == 0) record_status(H3B_STATUS_ATTN_TIMEOUT);
+    chain_wait();
+    if (a.notes && threadIdx.x < 2) reinterpret_cast<PieceNote*>(a.notes)[2 * blockIdx.x + threadIdx.x].state = 0;
     return;
   }
   struct Rest {
-    uint64_t bars[46];
+    uint64_t bars[48];
     uint32_t words[8];
     WinPlan plans[3];
     WorkShare work;
@@ -623,13 +625,21 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   uint64_t* plan_free = plan_full + 3;  // 3
   uint64_t* l_full = plan_free + 3;     // 2: row sums of an item written
   uint64_t* l_free = l_full + 2;        // 2: and read
+  uint64_t* drained = l_free + 2;       // 2: the products of a tile's issuer are all done
   uint32_t* tmem_slot = rest.words;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* cleared = abort_flag + 1;  // [3]: some seen V row of the item was cleared
+  volatile int* late_flag = cleared + 3;   // the last waits, which go on after abort_flag, gave up
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool by_heads = rows_per_cta == 128;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait_warp(bar, parity, abort_flag, H3B_STATUS_ATTN_TIMEOUT);
+  };
+  // A CTA that has given up still may not leave, or free its tensor memory, before its copies
+  // and products in flight have landed: each warp that starts them waits at its end (at once
+  // over where all went well).
+  auto wait_landed = [&](uint64_t* bar, uint32_t parity) {
+    mbar_wait_warp(bar, parity, late_flag, H3B_STATUS_ATTN_TIMEOUT);
   };
 
   if (warp == 0) {
@@ -658,13 +668,14 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       mbar_init(&o_free[x], 4);
       mbar_init(&l_full[x], 4);
       mbar_init(&l_free[x], 4);
+      mbar_init(&drained[x], 1);
     }
     for (int s = 0; s < 3; ++s) {
       mbar_init(&plan_full[s], 1);
       mbar_init(&plan_free[s], 15);  // all warps but the planning one
     }
     for (int s = 0; s < 8; ++s) mbar_init(&turns[s], 1);
-    *abort_flag = 0;
+    *abort_flag = *late_flag = 0;
     cleared[0] = cleared[1] = cleared[2] = 0;
     rest.seqs_at = {0, 0};
     fence_mbar_init();
@@ -912,6 +923,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       }
       if (!ok) break;
     }
+    // of each slot the last fill, of the slots from at.slot on that of the round before
+    wait_landed(q_full, q_parity);
+    for (int s = 0; s < kWinSlots; ++s) wait_landed(&full[s], s < at.slot ? at.parity : at.parity ^ 1u);
   } else if (warp == 1) {
     // V tiles, in order: those that are masked somewhere lose their non-finite elements
     RingAt<kWinSlots> at;
@@ -1070,6 +1084,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       if (last >= 0) o_parity ^= 1u;
       if (lane == 0) mbar_arrive(&plan_free[pr.slot]);
     }
+    if (elect_one()) mma_commit(&drained[x]);
+    __syncwarp();
+    wait_landed(&drained[x], 0);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWinSoftRegs));
     const int x = (warp - 4) >> 2, quad = warp & 3;
