@@ -40,21 +40,25 @@ STATUS_TEXT = {
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_gpu = torch._C._cuda_getDevice
 
 
-def _stream(t: torch.Tensor) -> int:
-    """The current stream of the tensor's device, as the C entries take it (a token's worth of
-    calls is short enough for the stream object's construction to count)."""
-    return _raw_stream(t.get_device())
+def _stream(gpu: int) -> int:
+    """The current stream of the GPU that a call's tensors are on, as the C entries take it (a token's worth
+    of calls is short enough for the stream object's construction to count).  The library launches on the
+    current GPU, which has to be that one: a kernel of another would reach into memory that is not its own."""
+    if _current_gpu() != gpu:
+        raise RuntimeError(f"the tensors are on cuda:{gpu}, the current device is cuda:{_current_gpu()}")
+    return _raw_stream(gpu)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _index(t: torch.Tensor, what: str, n: int | None = None) -> torch.Tensor:
-    if t.dtype is not torch.int32 or t.ndim != 1 or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 CUDA vector")
+def _index(t: torch.Tensor, what: str, gpu: int, n: int | None = None) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.ndim != 1 or t.get_device() != gpu or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 CUDA vector on the other tensors' GPU")
     if n is not None and t.shape[0] != n:
         raise ValueError(f"{what} must have {n} entries")
     return t
@@ -105,8 +109,12 @@ class PagedKVCache:
     def __post_init__(self) -> None:
         k, v, t, lens, refs, status = self.k, self.v, self.table, self.lens, self.refs, self.status
         shape, dtype = k.shape, k.dtype
-        if not (k.is_cuda and v.is_cuda and t.is_cuda and lens.is_cuda and refs.is_cuda and status.is_cuda):
+        if not k.is_cuda:
             raise RuntimeError("PagedKVCache runs only on CUDA tensors (the B200 library has no CPU path)")
+        self._gpu = gpu = k.get_device()
+        if not (v.get_device() == gpu == t.get_device() == lens.get_device() and refs.get_device() == gpu
+                and status.get_device() == gpu):
+            raise ValueError("cache tensors must be on one GPU")
         if len(shape) != 5 or shape[4] != HEAD_DIM or shape != v.shape or dtype is not v.dtype:
             raise ValueError("k and v must be [layers, pages, kv heads, page tokens, 128] of one type")
         if dtype not in DTYPE_CODES:
@@ -126,8 +134,8 @@ class PagedKVCache:
         if dtype is torch.float8_e4m3fn:
             for x in (self.k_scale, self.v_scale):
                 if (x is None or x.dtype is not torch.float32 or x.shape != (layers, heads) or not x.is_contiguous()
-                        or not x.is_cuda):
-                    raise ValueError("an e4m3 cache needs float32 k_scale and v_scale [layers, kv heads]")
+                        or x.get_device() != gpu):
+                    raise ValueError("an e4m3 cache needs float32 k_scale and v_scale [layers, kv heads] on its GPU")
             k_scale, v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
         self.page_tokens, self.kv_heads = page, heads
         self._ref = ctypes.byref(PageCacheStruct(
@@ -155,12 +163,12 @@ class PagedKVCache:
     def extend(self, slots: torch.Tensor, starts: torch.Tensor | None = None) -> None:
         """Room for starts[i + 1] - starts[i] more tokens (None: one) of each of the distinct slots,
         in every layer; a shared, partly filled last page is copied first."""
-        n = _index(slots, "slots").numel()
+        n = _index(slots, "slots", self._gpu).numel()
         if starts is not None:
-            _index(starts, "starts", n + 1)
+            _index(starts, "starts", self._gpu, n + 1)
         ws = self._workspace(n)
-        check(lib().h3b_pages_extend(self._ref, _ptr(slots), n, _ptr(starts), _ptr(ws), ws.numel(), _stream(self.k)),
-              "pages_extend")
+        check(lib().h3b_pages_extend(self._ref, _ptr(slots), n, _ptr(starts), _ptr(ws), ws.numel(),
+                                     _stream(self._gpu)), "pages_extend")
 
     def write(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | None = None,
               layer: int = 0) -> None:
@@ -169,13 +177,13 @@ class PagedKVCache:
         self._rows_into(lib().h3b_pages_write, "pages_write", slots, k, v, starts, layer)
 
     def _rows_into(self, entry, what, slots, k, v, starts, layer, ws=None) -> None:
-        n = _index(slots, "slots").shape[0]
+        n = _index(slots, "slots", self._gpu).shape[0]
         if starts is not None:
-            _index(starts, "starts", n + 1)
+            _index(starts, "starts", self._gpu, n + 1)
         k, k_step = _token_rows(k, self.kv_heads, "k")
         v, v_step = _token_rows(v, self.kv_heads, "v")
-        if not (k.is_cuda and v.is_cuda):
-            raise RuntimeError("PagedKVCache takes only CUDA tensors (the B200 library has no CPU path)")
+        if not k.get_device() == v.get_device() == self._gpu:
+            raise RuntimeError("PagedKVCache takes only CUDA tensors on its GPU (the B200 library has no CPU path)")
         if k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError("k and v must have one shape and type")
         if starts is None and k.shape[0] != n:
@@ -186,7 +194,7 @@ class PagedKVCache:
                 v_step, DTYPE_CODES[k.dtype], k.shape[0])
         if ws is not None:
             args += (ws.data_ptr(), ws.shape[0])
-        check(entry(*args, _stream(self.k)), what)
+        check(entry(*args, _stream(self._gpu)), what)
 
     def append(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | None = None,
                layer: int = 0) -> None:
@@ -197,29 +205,31 @@ class PagedKVCache:
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Empty slots dst[i] become sequences that share the pages of src[i]."""
-        n = _index(src, "src").numel()
-        check(lib().h3b_pages_fork(self._ref, _ptr(src), _ptr(_index(dst, "dst", n)), n, _stream(self.k)), "pages_fork")
+        n = _index(src, "src", self._gpu).numel()
+        check(lib().h3b_pages_fork(self._ref, _ptr(src), _ptr(_index(dst, "dst", self._gpu, n)), n,
+                                   _stream(self._gpu)), "pages_fork")
 
     def truncate(self, slots: torch.Tensor, keep: torch.Tensor) -> None:
         """Each of the distinct slots keeps its first keep[i] tokens."""
-        n = _index(slots, "slots").numel()
-        check(lib().h3b_pages_truncate(self._ref, _ptr(slots), _ptr(_index(keep, "keep", n)), n, _stream(self.k)),
-              "pages_truncate")
+        n = _index(slots, "slots", self._gpu).numel()
+        check(lib().h3b_pages_truncate(self._ref, _ptr(slots), _ptr(_index(keep, "keep", self._gpu, n)), n,
+                                       _stream(self._gpu)), "pages_truncate")
 
     def free(self, slots: torch.Tensor) -> None:
         """The distinct slots become empty; pages that no other sequence shares are free again."""
-        n = _index(slots, "slots").numel()
-        check(lib().h3b_pages_truncate(self._ref, _ptr(slots), None, n, _stream(self.k)), "pages_truncate")
+        n = _index(slots, "slots", self._gpu).numel()
+        check(lib().h3b_pages_truncate(self._ref, _ptr(slots), None, n, _stream(self._gpu)), "pages_truncate")
 
     def compact(self) -> None:
         """Pages in use move to the front of the pool."""
         ws = self._workspace(0)
-        check(lib().h3b_pages_compact(self._ref, _ptr(ws), ws.numel(), _stream(self.k)), "pages_compact")
+        check(lib().h3b_pages_compact(self._ref, _ptr(ws), ws.numel(), _stream(self._gpu)), "pages_compact")
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Pages src[i] over the distinct pages dst[i] in every layer (no page may be both); the tables stay."""
-        n = _index(src, "src").numel()
-        check(lib().h3b_pages_copy(self._ref, _ptr(src), _ptr(_index(dst, "dst", n)), n, _stream(self.k)), "pages_copy")
+        n = _index(src, "src", self._gpu).numel()
+        check(lib().h3b_pages_copy(self._ref, _ptr(src), _ptr(_index(dst, "dst", self._gpu, n)), n,
+                                   _stream(self._gpu)), "pages_copy")
 
     def check(self) -> None:
         """Wait for the stream; raise, and clear the status word, if a call could not be done."""

@@ -42,8 +42,8 @@ def _rule(window: int | None, sinks: int, chunk: int) -> tuple[int, int, int]:
 def _output(out: torch.Tensor | None, q: torch.Tensor) -> tuple[torch.Tensor, int]:
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format), q.shape[1] * HEAD_DIM
-    if out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda:
-        raise ValueError("out must have q's shape and type")
+    if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device():
+        raise ValueError("out must have q's shape and type, on its GPU")
     step = _row_step(out)
     if not step:
         raise ValueError("out must have contiguous heads and 16-byte aligned rows")
@@ -61,8 +61,9 @@ def _scale(scale: float | None) -> float:
 def _workspace(workspace: torch.Tensor | None, need: int, q: torch.Tensor) -> torch.Tensor:
     if workspace is None:
         return q.new_empty(need, dtype=torch.uint8)
-    if workspace.numel() * workspace.element_size() < need or not workspace.is_cuda or not workspace.is_contiguous():
-        raise ValueError(f"the workspace must have {need} contiguous bytes on the device")
+    if (workspace.numel() * workspace.element_size() < need or workspace.get_device() != q.get_device()
+            or not workspace.is_contiguous()):
+        raise ValueError(f"the workspace must have {need} contiguous bytes on the queries' GPU")
     return workspace
 
 
@@ -82,6 +83,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     calls on one stream."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError("window_attention runs only on CUDA tensors (the B200 library has no CPU path)")
+    gpu = q.get_device()
+    if not k.get_device() == v.get_device() == gpu:
+        raise ValueError("q, k and v must be on one GPU")
     (q, q_step), (k, k_step), (v, v_step) = (_token_rows(q, None, "q"), _token_rows(k, None, "k"),
                                              _token_rows(v, None, "v"))
     if k.shape != v.shape or not q.dtype is k.dtype is v.dtype:
@@ -93,8 +97,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     if (query_starts is None) != (key_starts is None):
         raise ValueError("query_starts and key_starts come together")
     if query_starts is not None:
-        seqs = _index(query_starts, "query_starts").numel() - 1
-        _index(key_starts, "key_starts", seqs + 1)
+        seqs = _index(query_starts, "query_starts", gpu).numel() - 1
+        _index(key_starts, "key_starts", gpu, seqs + 1)
         if seqs < 1:
             raise ValueError("query_starts needs at least two entries")
     out, out_step = _output(out, q)
@@ -102,13 +106,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     check(lib().h3b_window_attention(_ptr(q), q_step, _ptr(k), k_step, _ptr(v), v_step,
                                      DTYPE_CODES[q.dtype], q.shape[0], k.shape[0], _ptr(query_starts), _ptr(key_starts),
                                      seqs, q.shape[1], k.shape[1], window, sinks, chunk, _scale(scale), _ptr(out),
-                                     out_step, _ptr(workspace), size, _stream(q)), "window_attention")
+                                     out_step, _ptr(workspace), size, _stream(gpu)), "window_attention")
     return out
 
 
 def _cached_queries(q: torch.Tensor, cache: PagedKVCache, layer: int, what: str) -> tuple[torch.Tensor, int]:
     if not q.is_cuda:
         raise RuntimeError(f"{what} runs only on CUDA tensors (the B200 library has no CPU path)")
+    if q.get_device() != cache._gpu:
+        raise ValueError("q must be on the cache's GPU")
     q, step = _token_rows(q, None, "q")
     heads = q.shape[1]
     if heads == 0 or heads % cache.kv_heads:
@@ -128,11 +134,11 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
     if cache.k.dtype != q.dtype:
         raise ValueError(f"a {cache.k.dtype} cache does not serve {q.dtype} queries of several tokens")
     window, sinks, chunk = _rule(window, sinks, chunk)
-    seqs = 1 if query_starts is None else _index(query_starts, "query_starts").numel() - 1
+    seqs = 1 if query_starts is None else _index(query_starts, "query_starts", cache._gpu).numel() - 1
     if seqs < 1:
         raise ValueError("query_starts needs at least two entries")
     if slots is not None:
-        _index(slots, "slots", seqs)
+        _index(slots, "slots", cache._gpu, seqs)
     elif seqs > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
     out, out_step = _output(out, q)
@@ -140,8 +146,8 @@ def paged_window_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Te
                                         (window, sinks, chunk))
     check(lib().h3b_paged_window_attention(_ptr(q), q_step, DTYPE_CODES[q.dtype], q.shape[0], _ptr(query_starts),
                                            _ptr(slots), seqs, q.shape[1], cache._ref, layer, window, sinks, chunk,
-                                           _scale(scale), _ptr(out), out_step, _ptr(workspace), size, _stream(q)),
-          "paged_window_attention")
+                                           _scale(scale), _ptr(out), out_step, _ptr(workspace), size,
+                                           _stream(cache._gpu)), "paged_window_attention")
     return out
 
 
@@ -156,7 +162,7 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
     window, sinks, _ = _rule(window, sinks, 1)
     n = q.shape[0]
     if slots is not None:
-        _index(slots, "slots", n)
+        _index(slots, "slots", cache._gpu, n)
     elif n > cache.table.shape[0]:
         raise ValueError("more sequences than the cache has slots")
     need = lib().h3b_decode_workspace_bytes(n, q.shape[1], cache._ref)
@@ -165,7 +171,7 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor |
     out, out_step = _output(out, q)
     check(lib().h3b_decode_attention(_ptr(q), q_step, DTYPE_CODES[q.dtype], _ptr(slots), n, q.shape[1], cache._ref,
                                      layer, window, sinks, _scale(scale), _ptr(out), out_step, _ptr(workspace), need,
-                                     _stream(q)), "decode_attention")
+                                     _stream(cache._gpu)), "decode_attention")
     return out
 
 
