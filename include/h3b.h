@@ -392,6 +392,9 @@ int h3b_attention(const void* q, const void* q_scale, int q_gran, int q_block, i
  * fp16 or bf16 (dtype 1 or 2) rows of heads of 128 channels, fp32 softmax and sums;
  * sm_scale positive and finite. */
 
+/* Kernels that the entries of this section have launched in this process. */
+int64_t h3b_chained_launches(void);
+
 /* A paged K/V cache: pools [layers, pages, kv_heads, page_tokens, 128] that share one
  * page table.  dtype: 1 fp16, 2 bf16, 3 e4m3 with k_scale / v_scale f32 [layers,
  * kv_heads] (value = code * scale).  table int32 [table_rows, table_width]: the pages of

@@ -617,6 +617,8 @@ int window_status(int r, cudaError_t e, const char* what) {
 
 }  // namespace
 
+int64_t h3b_chained_launches(void) { return h3b::chained_launches.load(std::memory_order_relaxed); }
+
 int64_t h3b_window_workspace_bytes(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, int64_t window,
                                    int64_t sinks, int64_t chunk) {
   if (Tq < 0 || seqs < 1 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || keys < 0 || window < 0 || sinks < 0 || chunk < 1) return -1;

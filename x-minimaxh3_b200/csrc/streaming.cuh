@@ -2,6 +2,8 @@
 // streaming-attention kernels (window_attn.cu, decode_attn.cu, kv_pages.cu).
 #pragma once
 
+#include <atomic>
+
 #include "h3b_common.cuh"
 
 namespace h3b {
@@ -12,6 +14,9 @@ namespace h3b {
 // global memory; chain_next lets the kernel after it start that early in turn.
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// How many have been launched (in a captured graph: once, when it was captured): an entry
+// takes one, two or three, as the sizes ask for.
+inline std::atomic<int64_t> chained_launches{0};
 template <typename... P, typename... A>
 cudaError_t launch_chained(void (*kernel)(P...), int64_t grid, int threads, size_t smem, cudaStream_t s, A... args) {
   cudaLaunchAttribute attr;
@@ -24,7 +29,9 @@ cudaError_t launch_chained(void (*kernel)(P...), int64_t grid, int threads, size
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  if (e == cudaSuccess) chained_launches.fetch_add(1, std::memory_order_relaxed);
+  return e;
 }
 
 // Which keys a query sees: key j of a sequence with lk keys is visible to the query at

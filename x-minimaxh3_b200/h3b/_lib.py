@@ -113,6 +113,7 @@ _SIGNATURES = {
     "h3b_bitmap_to_lut": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
     "h3b_attention": [c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
                       c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p],
+    "h3b_chained_launches": [],
     "h3b_window_workspace_bytes": [c_int64] * 8,
     "h3b_window_attention": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p,
                              c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
@@ -136,8 +137,8 @@ _SIGNATURES = {
 }
 _RESTYPES = {"h3b_version": ctypes.c_char_p, "h3b_last_error": ctypes.c_char_p,
              "h3b_key_mean_workspace_bytes": c_int64, "h3b_decode_workspace_bytes": c_int64,
-             "h3b_window_workspace_bytes": c_int64,
-             "h3b_pages_workspace_bytes": c_int64}
+             "h3b_window_workspace_bytes": c_int64, "h3b_pages_workspace_bytes": c_int64,
+             "h3b_chained_launches": c_int64}
 
 EXPORTED = tuple(_SIGNATURES)
 
@@ -166,19 +167,27 @@ def lib():
     return _lib
 
 
-# kernels each entry launches (for the benchmark's launch count); default 1
-_KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2, "decode_attention": 2, "pages_extend": 2, "pages_append": 2,
-                     "pages_compact": 3, "pages_copy": 2, "pages_write": 2}
+# kernels each entry launches (for the benchmark's launch count); default 1.  The streaming
+# entries launch as many as the sizes ask for, which the library counts itself.
+_KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2}
+_KERNELS_PER_CALL |= dict.fromkeys(
+    ("window_attention", "paged_window_attention", "decode_attention", "pages_extend", "pages_write", "pages_append",
+     "pages_fork", "pages_truncate", "pages_compact", "pages_copy"), 0)
 _launches = 0
+_chained_before = 0
+
+
+def _chained() -> int:
+    return 0 if _lib is None else _lib.h3b_chained_launches()
 
 
 def reset_launch_count() -> None:
-    global _launches
-    _launches = 0
+    global _launches, _chained_before
+    _launches, _chained_before = 0, _chained()
 
 
 def launch_count() -> int:
-    return _launches
+    return _launches + _chained() - _chained_before
 
 
 def check(status: int, what: str) -> None:
