@@ -124,3 +124,30 @@ def test_window_maximum_that_creeps_up(dtype):
         ref, spread = (w @ v[:, 0].double()), (w @ v[:, 0].double().abs())
         u = UNIT[dtype]
         assert ((out[0, 0].double() - ref).abs() <= u * ref.abs() + (u + 2e-4) * spread * 1.01).all(), octaves
+
+
+def test_decode_of_queries_with_channels_far_apart():
+    """bf16 queries over an E4M3 cache whose channels span 2^42: a channel errs by at most 2^-25 of the
+    head's power of two (fp16's subnormal step), a score by 128 of those times the largest key."""
+    from h3b import decode_attention
+    from streaming_util import HostCache, attend, visible
+
+    g = torch.Generator(device="cuda").manual_seed(11)
+    heads, n = 6, 1000
+    cache = _cache("e4m3", 1, 16, 63, 1, n, 1.0)
+    for pool in (cache.k, cache.v):
+        pool.copy_(torch.randn(pool.shape, device="cuda", generator=g).to(pool.dtype))
+    size = 2.0 ** -(torch.arange(D, device="cuda") / 3)
+    sign = torch.randint(0, 2, (1, heads, D), device="cuda", generator=g) * 2 - 1
+    factor = 2.0 ** torch.tensor([-30, -10, 0, 3, 20, 60], device="cuda").view(1, heads, 1)
+    order = torch.stack([torch.randperm(D, device="cuda", generator=g) for _ in range(heads)])
+    q = (size[order][None] * sign * factor).to(torch.bfloat16)
+    k, v = HostCache(cache).rows(0)
+    for h in range(heads):
+        scale = float(0.7 / factor[0, h, 0])
+        out = decode_attention(q, cache, scale=scale)[:, h]
+        ref, spread = attend(q[:, h:h + 1], k, v, visible(1, n, None, 0, 1, "cuda"), scale)
+        score = scale * 128 * 2.0 ** -25 * float(factor[0, h, 0]) * float(k.abs().max())
+        u = UNIT[torch.bfloat16]
+        err = (out.double() - ref[:, 0]).abs()
+        assert (err <= u * ref[:, 0].abs() + (u + 2e-4 + 2 * score) * spread[:, 0] * 1.01).all(), h
