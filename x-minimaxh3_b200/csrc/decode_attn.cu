@@ -9,9 +9,9 @@
 // several warps is joined by a second kernel from fp32 partial sums with their softmax
 // statistics.  Few short sequences are bound by latency and take one launch of clusters.
 //
-// Measured, 32 heads of 8 kv heads: 2 sequences of 150,000 bf16 tokens 181 us, 6.4 TB/s of
-// K and V; 96 ragged sequences of about 3,500 E4M3 tokens 108 us, 5.5 TB/s; one of 701
-// tokens 6.5 us.
+// Measured, 32 heads of 8 kv heads: 2 sequences of 150,000 bf16 tokens 182 us, 6.3 TB/s of
+// K and V; 96 ragged sequences of about 3,500 E4M3 tokens 110 us, 5.4 TB/s; one of 701
+// tokens 6.3 us on the device.
 //
 // A warp keeps its chunk in registers, without shared memory:
 //   S^T = K . Q^T   m16n8k16, M = 16 keys, N = 8 heads of the group.  The products'
@@ -671,8 +671,10 @@ int sm_count() {
   return n;
 }
 
-// One wave of clusters (two CTAs per multiprocessor) and at most eight chunks a warp:
-// decode of one 701-token sequence, 32/8 heads: 6.5 us, by the list of all chunks 10.8 us.
+// One wave of clusters (two CTAs per multiprocessor) and at most eight chunks a warp.
+// capacity: the tokens that a table row can name, for the host does not know the lengths.
+// Decode of one 701-token sequence, 32/8 heads, on the device: 6.3 us in a table of 720
+// tokens, and 10.5 us by the list of all chunks, as in a table of 32,768.
 bool decode_by_clusters(int64_t seqs, int64_t Hq, int64_t Hkv, int64_t capacity) {
   const int64_t group = Hq / Hkv, rows = group > 8 ? 16 : 8;
   const int64_t pairs = seqs * Hkv * ((group + rows - 1) / rows);

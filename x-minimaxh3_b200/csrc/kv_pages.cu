@@ -112,7 +112,7 @@ __host__ __device__ __forceinline__ ExtendPlan extend_plan(int32_t* ws, int n) {
 }
 
 // Bound by the latency of its dependent loads (status, slots, lengths, tables, counts): about
-// half of the 11 us of a token's append to 200 sequences and its truncation.  One block,
+// half of the 10.5 us of a token's append to 200 sequences and its truncation.  One block,
 // because the pages of a sequence depend on what all before it ask for.
 // tokens: rows that come with the call (append), or -1: starts may not reach past them.
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PageTables t, const int32_t* slots, int n,
@@ -400,7 +400,7 @@ __device__ __forceinline__ int64_t row_place(const PageTables& t, const PageWrit
 }
 // A block writes `per` (1..8) tokens: their places are looked up side by side first, then
 // all their rows are under way together.  Bound by memory: 32,600 tokens of 8 kv heads into
-// an E4M3 cache, with the plan before it, 50 us (4.0 TB/s; 46 where L2 holds some of the
+// an E4M3 cache, with the plan before it, 51 us (3.9 TB/s; 47 where L2 holds some of the
 // rows), half of the issue slots taken by the conversion.
 // CHECK: the call is one that its blocks check; else it was checked before.
 template <bool FP8, bool BF16, bool CHECK>
@@ -763,7 +763,9 @@ cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t 
 // reference update per clock, a launch costs the host 2 to 3 us.  (fork + free, on the device
 // in one launch each / in two: 16 sequences of 60 pages 10.2 / 6.8 us, 128 of 94 pages 19.5 /
 // 6.9 us, 512 of 60 pages 39 / 8.0 us.)  A truncation mostly drops a few tokens (a pass that
-// appends a token to 200 sequences and drops it, launched from the host: 21.6 / 24.2 us).
+// appends a token to 200 sequences and drops it, launched from the host: 17.1 / 19.2 us).  What
+// is compared are the entries of the table's rows, which the host knows: in a table of 32,768
+// tokens that pass takes the second launch.
 constexpr int64_t kOneBlockEntries = 4096, kOneBlockKept = 16384;
 cudaError_t launch_pages_fork(const PageTables& t, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
   const bool one = (int64_t)n * t.width <= kOneBlockEntries;

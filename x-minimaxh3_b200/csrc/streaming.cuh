@@ -115,10 +115,11 @@ struct WindowArgs {
   void* notes;      // of cut items and their pieces (set by the launcher; null: none is cut)
   float* pieces;
 };
-// bf16: bfloat16, else float16.  workspace: null, or window_workspace_bytes() (0 where it
-// would not be used) with which long items are cut; keys: all, or what a table row names.  0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err), 3 the
-// kernel's register count is not the planned one, 4 too many tiles
+// keys: all, or what a table row can name.  0 where no workspace would be used
 int64_t window_workspace_bytes(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, const WindowRule& r);
+// bf16: bfloat16, else float16.  workspace: null, or window_workspace_bytes() with which long
+// items are cut.  Returns 0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err), 3 the
+// kernel's register count is not the planned one, 4 too many tiles
 int launch_window_attention(WindowArgs a, bool bf16, void* workspace, cudaStream_t s, cudaError_t* err);
 
 struct DecodeArgs {

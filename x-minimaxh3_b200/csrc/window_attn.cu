@@ -29,13 +29,14 @@
 // Tensor memory: S_A 0..127, S_B 128..255, O_A 256..383, O_B 384..511, P over S + 64.
 //
 // Bound by the chain of a step (S -> maximum -> P -> PV -> the next S), which two tiles hide
-// in part: of the 470 us, 245 to 283 are left without exponentials and products.  More tiles do not
-// fit tensor memory; more code per step (unrolled columns, a second softmax warpgroup,
-// wider output loops) measured slower, the instruction cache being short of it.
-// Measured, bf16, 32 heads: 8,192 tokens, 8 kv heads, window 4,096: 445 to 470 us, 880 to
-// 930 TFLOP/s (the lower under the power limit); a frame of 3,600 tokens over four frames
-// and a prefix of 509, paged: 985 us, 890 TFLOP/s; 11 ragged prompts of about 500 tokens:
-// 94 us, 430 TFLOP/s; six follow-ups of 90 tokens over 2,900 cached ones: 79 us.
+// in part: the tensor pipe and the exponential unit are each busy half of the time.  More
+// tiles do not fit tensor memory; more code per step (unrolled columns, a second softmax
+// warpgroup, wider output loops) measured slower, the instruction cache being short of it.
+// Measured, bf16, 32 heads: 8,192 tokens, 8 kv heads, window 4,096: 417 to 475 us, 870 to
+// 990 TFLOP/s (the lower under the power limit); a frame of 3,600 tokens over four frames
+// and a prefix of 509, paged: 870 to 1,000 us, 880 to 1,010 TFLOP/s; 11 ragged prompts of
+// about 500 tokens, fp16: 96 us, 422 TFLOP/s; six follow-ups of 90 tokens over 2,900 cached
+// ones: 80 us.
 #include <atomic>
 #include <climits>
 
@@ -220,7 +221,8 @@ __device__ __forceinline__ uint32_t key_bits(int base, int a, int b) {
 
 // 32 scores -> P = 2^(s c - m), and their sum.  All through ex2.approx: under the power
 // cap a polynomial on the FMA pipe for a share of them only adds instructions (8,192 x 32
-// heads, window 4,096: none 485 us, one in eight 494, one in four 492, one in two 533).
+// heads, window 4,096, in an earlier form of the kernel: none 485 us, one in eight 494, one in
+// four 492, one in two 533).
 __device__ __forceinline__ void win_exp32(uint32_t* s, float2 c2, float2 o2, float2& acc0, float2& acc1) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
@@ -248,8 +250,8 @@ __device__ __forceinline__ void win_load64(uint32_t s_addr, uint32_t (&s)[64]) {
 // One key tile for one query row, in two passes over the scores: the maximum, then P.
 // Both are loops over halves of 64 keys, not unrolled: the softmax warps of both tiles run
 // through this code every step, and with all 128 columns unrolled (and masked tiles apart)
-// it did not stay in the instruction cache (11 prompts of about 500 tokens: 148 us with
-// masked tiles apart, 134 us as one, 116 us as loops).
+// it did not stay in the instruction cache (11 prompts of about 500 tokens, in an earlier form
+// of the kernel: 148 us with masked tiles apart, 134 us as one, 116 us as loops).
 // The upper half goes first: its P lies over its own scores, and the lower half's columns
 // are free for the next S as soon as they are read.
 // cnt: tiles that the row's query tile has taken before (their PV is complete: it was
@@ -1292,9 +1294,12 @@ bool make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, uint64_t d1, ui
 // Whether items are cut.  Cutting takes a plan of all items by every CTA, a second launch
 // and a pass over the pieces, together about five steps' time; dealing whole items leaves
 // half an item's steps unbalanced on average.  So: where some item can have kCutFrom steps
-// (a bound from what the host knows).  A 720p frame over four frames and a prefix: 1,103 us
-// whole, 979 us cut; 11 prompts of about 500 tokens, window 1,024: 117 us whole, 108 cut.
-// keys: all of them, or what a table row can name.
+// (a bound from what the host knows).  keys: all of them, or what a table row can name.
+// Whole / cut: a 720p frame over four frames and a prefix 1,017 / 950 us; 11 prompts of about
+// 500 tokens, window 1,024, 107 / 95; six follow-ups of 90 tokens 77 / 80; one causal prompt
+// of 32 heads: 1,024 tokens 26 / 35, 2,048 tokens 60 / 65, 8,192 tokens, window 4,096, 420 /
+// 458 in short runs and 456 / 465 under the power limit; of 8 heads: 2,048 tokens 41 / 40.
+// Where whole items fill the multiprocessors evenly by themselves the rule loses by that much.
 bool window_cuts(int64_t Tq, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t keys, const WindowRule& r) {
   const bool by_heads = (Hq / Hkv) % 2 == 0;
   const int64_t rows = by_heads ? 128 : 256, columns = by_heads ? Hq / 2 : Hq, tiles = Tq / rows + seqs;

@@ -16,6 +16,10 @@ p = Lk - Lq + i sees key j when j <= last(p) and (last(p) - j < window or j < si
 last(p) = p, or with chunk > 1 the end of p's chunk (a latent frame sees itself whole),
 chunks counted from the end of the `sinks` first tokens, which form one of their own.
 A query that sees nothing gives 0.
+
+Scores, softmax and sums are fp32.  The weights are rounded to the queries' type for the V
+product (over an e4m3 cache: to fp16, as bf16 queries are, under a power of two per head); their
+sum is not.
 """
 
 from __future__ import annotations
@@ -181,7 +185,10 @@ class WindowAttentionB200:
     The request's protected prefix stays visible (sinks) and its video layout sets the
     chunk: every latent frame sees itself, the prefix and the `frames` - 1 frames before
     it (all of them when `frames` is None).  Without a layout attention is causal with a
-    window of `tokens` (None: unlimited)."""
+    window of `tokens` (None: unlimited).
+
+    It is called with a chunk's rows; the long-sequence protocol of the whole-sequence
+    backends (resolve_long_sequence_backend and what follows) is not its form."""
 
     approximate = True
 
