@@ -224,3 +224,20 @@ def test_writes_around_what_each_block_checks_itself(slots, tokens):
     host.write(order, counts, k, v)
     cache.check()
     host.assert_equal(cache)
+
+
+def test_writes_and_appends_without_rows():
+    """No row comes with the call: starts that name none are done, others are refused."""
+    from h3b import H3BError
+
+    none = _rows(0)
+    for call in (lambda c, *a: c.write(*a), lambda c, *a: c.append(*a)):
+        cache, host = _filled()
+        call(cache, _i32([1, 0]), none, none, _i32([0, 0, 0]))
+        cache.check()
+        host.assert_equal(cache)
+        for starts in ([0, 0, 3], [0, 2, 2], [-1, 0, 0]):
+            call(cache, _i32([1, 0]), none, none, _i32(starts))
+            with pytest.raises(H3BError, match="beyond the length or the rows"):
+                cache.check()
+            host.assert_equal(cache)

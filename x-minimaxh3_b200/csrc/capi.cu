@@ -804,7 +804,7 @@ extern "C" {
 int h3b_pages_write(const h3b_page_cache* cache, int64_t layer, const int32_t* slots, int64_t n, const int32_t* starts,
                     const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int dtype,
                     int64_t tokens, void* stream) {
-  if (n == 0 || tokens == 0) return ok();
+  if (n == 0 || (tokens == 0 && !starts)) return ok();
   h3b::PageWriteArgs w;
   const int r = write_args(cache, layer, slots, n, starts, k, k_row_stride, v, v_row_stride, dtype, tokens, "pages_write", &w);
   if (r) return r;

@@ -744,10 +744,10 @@ cudaError_t launch_pages_write(const PageTables& t, const PagePools& p, int64_t 
     copies = ((int64_t)w.n * p.layers * 2 * p.Hkv + 7) / 8;
     if (copies > kFullGrid / 2) copies = kFullGrid / 2;
   }
-  const bool own_check = !ws && w.tokens <= kOwnCheckTokens && w.n <= kOwnCheckTokens && t.rows <= kOwnCheckRows;
+  const bool own_check = !ws && w.tokens > 0 && w.tokens <= kOwnCheckTokens && w.n <= kOwnCheckTokens && t.rows <= kOwnCheckRows;
   if (!ws && !own_check) {
     const cudaError_t e = launch_chained(write_check_kernel, 1, kPlanThreads, seen_bytes(t.rows), s, t, w);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || w.tokens == 0) return e;  // without rows the starts may name none
   }
   auto kern = p.elem == 2    ? (own_check ? write_kernel<false, true, true> : write_kernel<false, true, false>)
               : w.src_bf16 ? (own_check ? write_kernel<true, true, true> : write_kernel<true, true, false>)
