@@ -1317,8 +1317,9 @@ int launch_window(WindowArgs a, cudaStream_t s, cudaError_t* err) {
     if (!make_rows_tmap(&tk, a.paged.k, BF16, page, slabs, 256, page * 256, (uint32_t)page, 1)) return 1;
     if (!make_rows_tmap(&tv, a.paged.v, BF16, page, slabs, 256, page * 256, (uint32_t)page, 1)) return 1;
   } else {
-    if (!make_rows_tmap(&tk, a.k, BF16, (uint64_t)a.Hkv, (uint64_t)a.Tk, 256, (uint64_t)a.k_stride * 2, 1, 128)) return 1;
-    if (!make_rows_tmap(&tv, a.v, BF16, (uint64_t)a.Hkv, (uint64_t)a.Tk, 256, (uint64_t)a.v_stride * 2, 1, 128)) return 1;
+    const uint64_t rows = (uint64_t)(a.Tk ? a.Tk : a.Tq);  // no keys: the map of Q (see launch_window_attention)
+    if (!make_rows_tmap(&tk, a.k, BF16, (uint64_t)a.Hkv, rows, 256, (uint64_t)a.k_stride * 2, 1, 128)) return 1;
+    if (!make_rows_tmap(&tv, a.v, BF16, (uint64_t)a.Hkv, rows, 256, (uint64_t)a.v_stride * 2, 1, 128)) return 1;
   }
   auto kern = window_kernel<BF16, PAGED>;
   // the kernel's attributes are checked and set once per device
@@ -1362,6 +1363,11 @@ int launch_window_attention(WindowArgs a, bool bf16, void* workspace, cudaStream
   a.notes = workspace;
   a.pieces = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + window_notes_bytes(num_sms())) : nullptr;
   if (!a.paged.k && a.Tk == 0) {  // no key anywhere
+    if (a.q_starts) {  // rows of no sequence stay: the kernel visits no key, and needs maps that can be made
+      a.k = a.v = a.q;
+      a.k_stride = a.v_stride = a.q_stride;
+      return bf16 ? launch_window<true, false>(a, s, err) : launch_window<false, false>(a, s, err);
+    }
     *err = cudaMemset2DAsync(a.out, (size_t)a.out_stride * 2, 0, (size_t)a.Hq * 256, (size_t)a.Tq, s);
     return *err == cudaSuccess ? 0 : 2;
   }
