@@ -390,7 +390,7 @@ int h3b_attention(const void* q, const void* q_scale, int q_gran, int q_block, i
  * the end of the `sinks` first tokens (the packed prefix), which form one of their own.
  * A query that sees no key gives 0.  Query head h reads kv head h / (Hq / Hkv).
  * fp16 or bf16 (dtype 1 or 2) rows of heads of 128 channels, fp32 softmax and sums;
- * sm_scale positive and finite.  The weights of the V product are rounded to the 16-bit
+ * sm_scale positive and finite, times log2(e) too.  The weights of the V product are rounded to the 16-bit
  * type (over an e4m3 cache: to fp16, as are bf16 queries under a power of two per head that
  * brings the largest channel to [1, 2)); their sum is not. */
 

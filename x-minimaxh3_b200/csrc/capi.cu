@@ -1,6 +1,7 @@
 // capi.cu -- the extern "C" boundary of libh3b.so (declared in include/h3b.h).
 // Validates arguments, launches on the caller's stream, converts every failure
 // into an int status plus a per-thread message; nothing throws out of here.
+#include <cfloat>
 #include <climits>
 #include <cstdio>
 #include <cstring>
@@ -599,8 +600,8 @@ int check_rows(const void* q, int64_t q_stride, int dtype, int64_t rows, int64_t
   if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, w + ": dtype must be fp16 or bf16");
   if (window < 0 || sinks < 0 || chunk < 1)
     return fail(H3B_ERR_INVALID_ARGUMENT, w + ": need window >= 0, sinks >= 0 and chunk >= 1");
-  if (!(sm_scale > 0.f) || sm_scale > 3e38f)
-    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": the softmax scale must be positive and finite");
+  if (!(sm_scale > 0.f) || sm_scale * 1.4426950408889634f > FLT_MAX)  // the kernels' scores are powers of two
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": the softmax scale must be positive and finite, times log2(e) too");
   if (rows > (1 << 30) || Hq > 65535) return fail(H3B_ERR_UNSUPPORTED, w + ": too many rows or heads");
   if (q_stride < Hq * 128 || q_stride % 8 || out_stride < Hq * 128 || out_stride % 8)
     return fail(H3B_ERR_INVALID_ARGUMENT, w + ": bad row stride");

@@ -33,6 +33,7 @@ from ._lib import check, lib
 from .cache import DTYPE_CODES, HEAD_DIM, PagedKVCache, _index, _ptr, _row_step, _stream, _token_rows
 
 UNLIMITED = 1 << 30
+MAX_SCALE = torch.finfo(torch.float32).max * math.log(2)  # the kernels' scores are powers of two
 
 
 def _rule(window: int | None, sinks: int, chunk: int) -> tuple[int, int, int]:
@@ -57,8 +58,8 @@ def _output(out: torch.Tensor | None, q: torch.Tensor) -> tuple[torch.Tensor, in
 def _scale(scale: float | None) -> float:
     if scale is None:
         return 1.0 / math.sqrt(HEAD_DIM)
-    if not 0.0 < float(scale) < math.inf:
-        raise ValueError("the softmax scale must be positive and finite")
+    if not 0.0 < float(scale) < MAX_SCALE:
+        raise ValueError("the softmax scale must be positive and finite, times log2(e) too")
     return float(scale)
 
 
