@@ -498,6 +498,64 @@ int h3b_pages_compact(const h3b_page_cache* cache, void* workspace, int64_t work
  * tables stay as they are. */
 int h3b_pages_copy(const h3b_page_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
 
+/* ---------------------------------------------------------------- microscaled 4-bit floats
+ * Rows of E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) with a scale per block:
+ *   H3B_MXFP4: blocks of 32 columns, E8M0 scales (2^(byte - 127)); no row scale
+ *   H3B_NVFP4: blocks of 16 columns, E4M3 scales, and a float32 scale per row
+ * value = element * block scale * row scale.
+ * codes: [rows, ceil(cols / 32) * 16] bytes, column 2i in the low nibble of byte i, zero
+ * codes behind the last column.  scales: tiles of 128 rows x 4 blocks in 512 bytes,
+ * [ceil(rows / 128), ceil(cols / (4 * block)), 512]; row r of a tile has its four bytes at
+ * (r % 32) * 16 + (r / 32) * 4; zero bytes behind the last block.  The bytes of rows
+ * behind the last one are not used.  row_scales: [rows], or NULL for 1.  codes and scales
+ * are 16-byte aligned. */
+#define H3B_MXFP4 1
+#define H3B_NVFP4 2
+typedef struct h3b_fp4_rows {
+  void* codes;
+  void* scales;
+  float* row_scales;
+  int64_t rows, cols;
+  int format;
+} h3b_fp4_rows;
+
+/* fp16 / bf16 rows x [out->rows, out->cols] to 4-bit floats; cols <= 32768.
+ * MXFP4: a block's scale is 2^(floor(log2(absmax)) - 2).  NVFP4: the row's scale is the
+ * least 2^e, e >= -126, with absmax <= 2688 * 2^e (1 for a row of zeros), a block's
+ * e4m3(absmax / 6 / 2^e).  Elements are rounded to the nearest, ties to the even code,
+ * and saturate at 6.  A block with an infinity or a NaN gets the scale NaN. */
+int h3b_fp4_quantize(const void* x, int dtype, int64_t x_row_stride, const h3b_fp4_rows* out, void* stream);
+
+/* The values that `rows` stand for, rounded to fp16 / bf16, into out [rows, cols]. */
+int h3b_fp4_dequantize(const h3b_fp4_rows* rows, void* out, int dtype, int64_t out_row_stride, void* stream);
+
+/* out[m, n] = sum over k of x[m, k] * w[n, k], times the row scales of x and w, + bias[n]
+ * (float32 [w->rows] or NULL), rounded to fp16 / bf16; fp32 sums, the same ones every time.
+ * x and w have one format and one number of columns. */
+int h3b_fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
+                 int64_t out_row_stride, void* stream);
+
+/* h3b_fp4_quantize of x [rows, w->cols] into the workspace, then h3b_fp4_gemm; the output
+ * has x's type.  workspace: h3b_fp4_linear_workspace_bytes() bytes, 16-byte aligned, not
+ * shared by calls on different streams. */
+int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, int64_t cols, int format);
+int h3b_fp4_linear(const void* x, int dtype, int64_t rows, int64_t x_row_stride, const h3b_fp4_rows* w,
+                   const float* bias, void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* h = x + residual (rounded to their type and written to sum; residual NULL: h = x, sum not
+ * written), y = h / sqrt(mean(h^2) + eps) * weight in float32, and y quantised: to int8 rows
+ * q [rows, cols] with scales [rows] (absmax / 127; a row with an infinity or a NaN gets that
+ * as its scale), or to 4-bit floats as h3b_fp4_quantize does.  x, residual, weight [cols] and
+ * sum are fp16 or bf16; sum may be x or residual itself, and must not overlap them
+ * otherwise.  cols <= 32768. */
+int h3b_add_rms_norm_int8(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                          void* sum, int64_t sum_row_stride, const void* weight, int dtype, int64_t rows,
+                          int64_t cols, float eps, void* q, float* scales, void* stream);
+int h3b_add_rms_norm_fp4(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                         void* sum, int64_t sum_row_stride, const void* weight, int dtype, float eps,
+                         const h3b_fp4_rows* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,139 @@
+"""Host side of the 4-bit operators: what is refused before a launch (no GPU needed)."""
+
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+import fp4_util as U
+import h3b
+from h3b._lib import Fp4RowsStruct, lib
+
+A = 4096  # an address that no call below reads: each is refused before a launch
+
+
+def _rows(codes=A, scales=A, row_scales=None, rows=4, cols=64, fmt=1):
+    return ctypes.byref(Fp4RowsStruct(codes, scales, row_scales, rows, cols, fmt))
+
+
+def _refused(status, code, text):
+    assert status == code, lib().h3b_last_error()
+    assert text in lib().h3b_last_error().decode()
+
+
+def test_quantize_refuses_before_a_launch():
+    f = lib().h3b_fp4_quantize
+    _refused(f(A, 2, 64, None, None), -1, "null")
+    _refused(f(None, 2, 64, _rows(), None), -1, "null")
+    _refused(f(A, 2, 64, _rows(codes=None), None), -1, "null")
+    _refused(f(A, 2, 64, _rows(codes=A + 4), None), -2, "aligned")
+    _refused(f(A, 2, 64, _rows(scales=A + 8), None), -2, "aligned")
+    _refused(f(A + 1, 2, 64, _rows(), None), -2, "aligned")
+    _refused(f(A, 0, 64, _rows(), None), -2, "dtype")
+    _refused(f(A, 2, 63, _rows(), None), -1, "stride")
+    _refused(f(A, 2, 64, _rows(fmt=3), None), -1, "format")
+    _refused(f(A, 2, 64, _rows(fmt=2), None), -1, "row scales")
+    _refused(f(A, 2, 64, _rows(cols=0), None), -1, "sizes")
+    _refused(f(A, 2, 64, _rows(rows=-1), None), -1, "sizes")
+    _refused(f(A, 2, 40000, _rows(cols=32769), None), -2, "32768")
+    assert f(None, 2, 64, _rows(codes=None, scales=None, rows=0), None) == 0
+
+
+def test_dequantize_and_gemm_refuse_before_a_launch():
+    f = lib().h3b_fp4_dequantize
+    _refused(f(_rows(), None, 2, 64, None), -1, "null")
+    _refused(f(_rows(), A, 0, 64, None), -2, "dtype")
+    _refused(f(_rows(), A, 2, 10, None), -1, "stride")
+    assert f(_rows(rows=0), None, 2, 64, None) == 0
+    f = lib().h3b_fp4_gemm
+    _refused(f(_rows(), _rows(fmt=2), None, A, 2, 64, None), -1, "one format")
+    _refused(f(_rows(), _rows(cols=32), None, A, 2, 64, None), -1, "columns")
+    _refused(f(_rows(), _rows(rows=65), None, A, 2, 64, None), -1, "stride")
+    _refused(f(_rows(), _rows(), None, None, 2, 64, None), -1, "null")
+    _refused(f(_rows(), _rows(), None, A, 0, 64, None), -2, "dtype")
+    _refused(f(_rows(rows=1 << 30), _rows(rows=1 << 30), None, A, 2, 1 << 30, None), -2, "tiles")
+    assert f(_rows(rows=0), _rows(), None, None, 2, 64, None) == 0
+    assert f(_rows(), _rows(rows=0), None, None, 2, 64, None) == 0
+
+
+def test_linear_refuses_before_a_launch():
+    f, need = lib().h3b_fp4_linear, lib().h3b_fp4_linear_workspace_bytes(4, 64, 1)
+    assert need == 4 * 32 + 512
+    assert lib().h3b_fp4_linear_workspace_bytes(200, 100, 2) == 200 * 64 + 2 * 2 * 512 + 800
+    assert lib().h3b_fp4_linear_workspace_bytes(4, 64, 3) == -1
+    assert lib().h3b_fp4_linear_workspace_bytes(4, 32769, 1) == -1
+    _refused(f(A, 2, 4, 64, _rows(), None, A, 4, A, need - 1, None), -1, "workspace")
+    _refused(f(A, 2, 4, 64, _rows(), None, A, 4, None, 0, None), -1, "workspace")
+    _refused(f(A, 2, 4, 64, _rows(), None, A, 4, A + 8, need, None), -2, "aligned")
+    _refused(f(A, 2, 4, 64, None, None, A, 4, A, need, None), -1, "null")
+    _refused(f(A, 2, 4, 60, _rows(), None, A, 4, A, need, None), -1, "stride")
+    _refused(f(A, 2, 4, 64, _rows(), None, A, 3, A, need, None), -1, "stride")
+    _refused(f(A, 2, -4, 64, _rows(), None, A, 4, A, need, None), -1, "sizes")
+    _refused(f(A, 2, 4, 40000, _rows(cols=32769), None, A, 4, A, 1 << 30, None), -2, "32768")
+    assert f(None, 2, 0, 64, _rows(), None, None, 4, None, 0, None) == 0
+
+
+def test_norm_refuses_before_a_launch():
+    f = lib().h3b_add_rms_norm_int8
+    ok = dict(x=A, xs=64, r=A, rs=64, s=A, ss=64, w=A, dt=2, m=4, k=64, eps=1e-5, q=A, sc=A)
+
+    def call(**changed):
+        a = ok | changed
+        return f(*(a[n] for n in ("x", "xs", "r", "rs", "s", "ss", "w", "dt", "m", "k", "eps", "q", "sc")), None)
+    for name in ("x", "s", "w", "q", "sc"):
+        _refused(call(**{name: None}), -1, "null")
+    for name in ("xs", "rs", "ss"):
+        _refused(call(**{name: 63}), -1, "stride")
+    _refused(call(dt=0), -2, "dtype")
+    _refused(call(eps=-1.0), -1, "eps")
+    _refused(call(eps=float("nan")), -1, "eps")
+    _refused(call(eps=float("inf")), -1, "eps")
+    _refused(call(k=0), -1, "sizes")
+    _refused(call(k=32769, xs=40000, rs=40000, ss=40000), -2, "32768")
+    _refused(call(q=A + 4), -2, "aligned")
+    assert call(m=0) == 0
+    f4 = lib().h3b_add_rms_norm_fp4
+    _refused(f4(A, 64, A, 64, A, 64, A, 2, 1e-5, None, None), -1, "null")
+    _refused(f4(A, 64, A, 64, None, 64, A, 2, 1e-5, _rows(), None), -1, "null")
+    _refused(f4(A, 64, A, 64, A, 64, A, 2, 1e-5, _rows(fmt=2), None), -1, "row scales")
+    assert f4(A, 64, A, 64, A, 64, A, 2, 1e-5, _rows(rows=0), None) == 0
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    for call in (lambda: h3b.quantize_fp4(x), lambda: h3b.add_rms_norm_quantize(x, x, x[0]),
+                 lambda: h3b.Fp4Linear.from_weight(x),
+                 lambda: h3b.Fp4Rows(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), 64,
+                                     "mxfp4")):
+        with pytest.raises(RuntimeError, match="only (on )?CUDA tensors"):
+            call()
+
+
+def test_the_64_bit_form_on_known_values():
+    """Elements, ties and scales worked out by hand."""
+    x = torch.zeros(1, 32, dtype=torch.float64)
+    x[0, :10] = torch.tensor([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.3, 7.9])
+    code, byte, _ = U.quantize(x, "mxfp4")
+    assert byte.item() == 127  # 2^(floor(log2 7.9) - 2) = 1
+    assert code[0, 0, :10].tolist() == [6, 0, 2, 2, 4, 4, 6, 6, 9, 7]
+    x = torch.zeros(1, 16, dtype=torch.float64)
+    x[0, :3] = torch.tensor([6.0, 3.0, -1.0])
+    code, byte, e = U.quantize(x, "nvfp4")
+    assert e.item() == -8  # 6 <= 2688 * 2^-8 = 10.5, and not 2688 * 2^-9
+    assert U.scale_values(byte, "nvfp4").item() == 256.0
+    assert code[0, 0, :3].tolist() == [7, 5, 10]
+
+
+def test_no_read_only_loads_in_chained_kernels():
+    """These kernels start while the one before them runs, and wait for it: what it writes may not come through
+    the read-only path."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "x-minimaxh3_b200", "csrc")
+    for name in ("fp4_rows.cu", "fp4_gemm.cu", "fp4.cuh"):
+        code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+        assert not re.search(r"ld\.global(\.\w+)*\.nc|__ldg\b|__restrict__", code), name
+        assert code.count("chain_wait();") >= code.count("__global__")
+    rows = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, "fp4_rows.cu")).read())
+    # a product may read its weight before it waits, so the rows' kernels let it start only behind their own wait
+    assert len(re.findall(r"chain_wait\(\);\s*chain_next\(\);", rows)) == rows.count("__global__")

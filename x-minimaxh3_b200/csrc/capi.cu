@@ -7,6 +7,7 @@
 #include <cstring>
 #include <string>
 
+#include "fp4.cuh"
 #include "h3b_kernels.cuh"
 #include "streaming.cuh"
 
@@ -866,6 +867,202 @@ int h3b_pages_copy(const h3b_page_cache* cache, const int32_t* src, const int32_
   if (n < 0 || n > cache->pages) return fail(H3B_ERR_INVALID_ARGUMENT, "pages_copy: more pairs than pages");
   return cuda_status(h3b::launch_pages_copy(page_pools(cache), (int)cache->pages, (int)cache->page_tokens, src, dst, (int)n,
                                             cache->status, st(stream)), "pages_copy");
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_fp4(const h3b_fp4_rows* r, const char* what) {
+  const std::string w(what);
+  if (!r) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null pointer");
+  if (r->format != H3B_MXFP4 && r->format != H3B_NVFP4)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": format must be H3B_MXFP4 or H3B_NVFP4");
+  if (r->rows < 0 || r->cols < 1) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": bad sizes");
+  if (r->rows > (1 << 30) || r->cols > (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, w + ": sizes beyond 2^30");
+  if (r->rows > 0 && (!r->codes || !r->scales)) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null pointer");
+  if (!aligned16(r->codes) || !aligned16(r->scales))
+    return fail(H3B_ERR_UNSUPPORTED, w + ": codes and scales must be 16-byte aligned");
+  return H3B_OK;
+}
+h3b::Fp4RowsView fp4_view(const h3b_fp4_rows* r) {
+  return {static_cast<const uint8_t*>(r->codes), static_cast<const uint8_t*>(r->scales), r->row_scales, r->rows,
+          (int)r->cols};
+}
+int check_half_rows(const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride, const char* what) {
+  const std::string w(what);
+  if (dtype != 1 && dtype != 2) return fail(H3B_ERR_UNSUPPORTED, w + ": dtype must be fp16 or bf16");
+  if (rows > 0 && !p) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": null pointer");
+  if (rows > 1 && stride < cols) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": bad row stride");
+  if (reinterpret_cast<uintptr_t>(p) % 2) return fail(H3B_ERR_UNSUPPORTED, w + ": rows must be 2-byte aligned");
+  return H3B_OK;
+}
+// what the row kernels write: 4-bit rows of at most kFp4MaxRowCols columns
+int check_fp4_output(const h3b_fp4_rows* r, const char* what) {
+  const int e = check_fp4(r, what);
+  if (e) return e;
+  const std::string w(what);
+  if (r->cols > h3b::kFp4MaxRowCols) return fail(H3B_ERR_UNSUPPORTED, w + ": more than 32768 columns");
+  if (r->rows > 0 && r->format == H3B_NVFP4 && !r->row_scales)
+    return fail(H3B_ERR_INVALID_ARGUMENT, w + ": NVFP4 rows need row scales");
+  return H3B_OK;
+}
+int norm_args(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, void* sum,
+              int64_t sum_row_stride, const void* weight, int dtype, int64_t rows, int64_t cols, float eps,
+              const char* what, h3b::Fp4RowArgs* a) {
+  const std::string w(what);
+  if (rows < 0 || cols < 1) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": bad sizes");
+  if (rows > (1 << 30) || cols > h3b::kFp4MaxRowCols) return fail(H3B_ERR_UNSUPPORTED, w + ": more than 32768 columns");
+  if (!(eps >= 0.f) || eps > FLT_MAX) return fail(H3B_ERR_INVALID_ARGUMENT, w + ": eps must be finite and not negative");
+  int e = check_half_rows(x, dtype, rows, cols, x_row_stride, what);
+  if (!e) e = check_half_rows(weight, dtype, 1, cols, cols, what);
+  if (!e && residual) e = check_half_rows(residual, dtype, rows, cols, residual_row_stride, what);
+  if (!e && residual) e = check_half_rows(sum, dtype, rows, cols, sum_row_stride, what);
+  if (e) return e;
+  *a = {};
+  a->x = static_cast<const uint16_t*>(x);
+  a->x_stride = x_row_stride;
+  a->rows = rows;
+  a->K = (int)cols;
+  a->res = static_cast<const uint16_t*>(residual);
+  a->res_stride = residual_row_stride;
+  a->sum = static_cast<uint16_t*>(sum);
+  a->sum_stride = sum_row_stride;
+  a->norm_w = static_cast<const uint16_t*>(weight);
+  a->eps = eps;
+  return H3B_OK;
+}
+void set_fp4_output(const h3b_fp4_rows* r, h3b::Fp4RowArgs* a) {
+  a->codes = static_cast<uint8_t*>(r->codes);
+  a->blocks = static_cast<uint8_t*>(r->scales);
+  a->row_scales = r->format == H3B_NVFP4 ? r->row_scales : nullptr;
+}
+int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+
+int fp4_quantize(const void* x, int dtype, int64_t x_row_stride, const h3b_fp4_rows* out, void* stream, const char* what) {
+  h3b::Fp4RowArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.x_stride = x_row_stride;
+  a.rows = out->rows;
+  a.K = (int)out->cols;
+  set_fp4_output(out, &a);
+  return cuda_status(h3b::launch_fp4_rows(a, out->format, dtype == 2, st(stream)), what);
+}
+int fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
+             int64_t out_row_stride, int behind_rows, void* stream, const char* what) {
+  h3b::Fp4GemmArgs a{};
+  a.M = (int)x->rows;
+  a.N = (int)w->rows;
+  a.K = (int)x->cols;
+  a.bias = bias;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride = out_row_stride;
+  a.bf16 = out_dtype == 2;
+  a.behind_rows = behind_rows;
+  cudaError_t e = cudaSuccess;
+  const int r = h3b::launch_fp4_gemm(fp4_view(x), fp4_view(w), a, x->format, st(stream), &e);
+  if (r == 1) return fail(H3B_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed");
+  return cuda_status(e, what);
+}
+// what a product checks of its weight, bias and output
+int check_fp4_product(int64_t M, const h3b_fp4_rows* w, const void* out, int out_dtype, int64_t out_row_stride,
+                      const char* what) {
+  const int e = check_fp4(w, what);
+  if (e) return e;
+  if (((M + 127) / 128) * ((w->rows + 127) / 128) > (1 << 27))
+    return fail(H3B_ERR_UNSUPPORTED, std::string(what) + ": too many output tiles");
+  return check_half_rows(w->rows > 0 ? out : nullptr, out_dtype, w->rows > 0 ? M : 0, w->rows, out_row_stride, what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int h3b_fp4_quantize(const void* x, int dtype, int64_t x_row_stride, const h3b_fp4_rows* out, void* stream) {
+  int e = check_fp4_output(out, "fp4_quantize");
+  if (!e) e = check_half_rows(x, dtype, out->rows, out->cols, x_row_stride, "fp4_quantize");
+  if (e) return e;
+  if (out->rows == 0) return ok();
+  return fp4_quantize(x, dtype, x_row_stride, out, stream, "fp4_quantize");
+}
+
+int h3b_fp4_dequantize(const h3b_fp4_rows* rows, void* out, int dtype, int64_t out_row_stride, void* stream) {
+  int e = check_fp4(rows, "fp4_dequantize");
+  if (!e) e = check_half_rows(out, dtype, rows->rows, rows->cols, out_row_stride, "fp4_dequantize");
+  if (e) return e;
+  if (rows->rows == 0) return ok();
+  if ((rows->cols + 15) / 16 * rows->rows > ((int64_t)INT_MAX << 8))
+    return fail(H3B_ERR_UNSUPPORTED, "fp4_dequantize: too many elements");
+  return cuda_status(h3b::launch_fp4_dequantize(fp4_view(rows), rows->format, static_cast<uint16_t*>(out),
+                                                out_row_stride, dtype == 2, st(stream)), "fp4_dequantize");
+}
+
+int h3b_fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
+                 int64_t out_row_stride, void* stream) {
+  int e = check_fp4(x, "fp4_gemm");
+  if (!e) e = check_fp4_product(x->rows, w, out, out_dtype, out_row_stride, "fp4_gemm");
+  if (e) return e;
+  if (x->format != w->format || x->cols != w->cols)
+    return fail(H3B_ERR_INVALID_ARGUMENT, "fp4_gemm: x and w must have one format and one number of columns");
+  if (x->rows == 0 || w->rows == 0) return ok();
+  return fp4_gemm(x, w, bias, out, out_dtype, out_row_stride, 0, stream, "fp4_gemm");
+}
+
+int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, int64_t cols, int format) {
+  if (rows < 0 || cols < 1 || rows > (1 << 30) || cols > h3b::kFp4MaxRowCols || (format != H3B_MXFP4 && format != H3B_NVFP4))
+    return -1;
+  return align16(rows * h3b::fp4_pitch(cols)) + h3b::fp4_scale_bytes(rows, cols, format) +
+         (format == H3B_NVFP4 ? align16(4 * rows) : 0);
+}
+
+int h3b_fp4_linear(const void* x, int dtype, int64_t rows, int64_t x_row_stride, const h3b_fp4_rows* w,
+                   const float* bias, void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
+  if (rows < 0 || rows > (1 << 30)) return fail(H3B_ERR_INVALID_ARGUMENT, "fp4_linear: bad sizes");
+  int e = check_fp4_product(rows, w, out, dtype, out_row_stride, "fp4_linear");
+  if (!e) e = check_half_rows(x, dtype, rows, w->cols, x_row_stride, "fp4_linear");
+  if (e) return e;
+  if (w->cols > h3b::kFp4MaxRowCols) return fail(H3B_ERR_UNSUPPORTED, "fp4_linear: more than 32768 columns");
+  if (rows == 0 || w->rows == 0) return ok();
+  if (!workspace || workspace_bytes < h3b_fp4_linear_workspace_bytes(rows, w->cols, w->format))
+    return fail(H3B_ERR_INVALID_ARGUMENT, "fp4_linear: workspace too small");
+  if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "fp4_linear: workspace must be 16-byte aligned");
+  char* at = static_cast<char*>(workspace);
+  h3b_fp4_rows q{at, at + align16(rows * h3b::fp4_pitch(w->cols)), nullptr, rows, w->cols, w->format};
+  if (w->format == H3B_NVFP4)
+    q.row_scales = reinterpret_cast<float*>(static_cast<char*>(q.scales) + h3b::fp4_scale_bytes(rows, w->cols, w->format));
+  e = fp4_quantize(x, dtype, x_row_stride, &q, stream, "fp4_linear");
+  if (e) return e;
+  return fp4_gemm(&q, w, bias, out, dtype, out_row_stride, 1, stream, "fp4_linear");
+}
+
+int h3b_add_rms_norm_int8(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                          void* sum, int64_t sum_row_stride, const void* weight, int dtype, int64_t rows,
+                          int64_t cols, float eps, void* q, float* scales, void* stream) {
+  h3b::Fp4RowArgs a;
+  const int e = norm_args(x, x_row_stride, residual, residual_row_stride, sum, sum_row_stride, weight, dtype, rows, cols,
+                          eps, "add_rms_norm_int8", &a);
+  if (e) return e;
+  if (rows == 0) return ok();
+  if (!q || !scales) return fail(H3B_ERR_INVALID_ARGUMENT, "add_rms_norm_int8: null pointer");
+  if (!aligned16(q)) return fail(H3B_ERR_UNSUPPORTED, "add_rms_norm_int8: q must be 16-byte aligned");
+  a.codes = static_cast<uint8_t*>(q);
+  a.row_scales = scales;
+  return cuda_status(h3b::launch_fp4_rows(a, 0, dtype == 2, st(stream)), "add_rms_norm_int8");
+}
+
+int h3b_add_rms_norm_fp4(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                         void* sum, int64_t sum_row_stride, const void* weight, int dtype, float eps,
+                         const h3b_fp4_rows* out, void* stream) {
+  int e = check_fp4_output(out, "add_rms_norm_fp4");
+  if (e) return e;
+  h3b::Fp4RowArgs a;
+  e = norm_args(x, x_row_stride, residual, residual_row_stride, sum, sum_row_stride, weight, dtype, out->rows, out->cols,
+                eps, "add_rms_norm_fp4", &a);
+  if (e) return e;
+  if (out->rows == 0) return ok();
+  set_fp4_output(out, &a);
+  return cuda_status(h3b::launch_fp4_rows(a, out->format, dtype == 2, st(stream)), "add_rms_norm_fp4");
 }
 
 }  // extern "C"

@@ -62,7 +62,21 @@ class PageCacheStruct(ctypes.Structure):
     ]
 
 
+class Fp4RowsStruct(ctypes.Structure):
+    """h3b_fp4_rows (include/h3b.h)."""
+
+    _fields_ = [
+        ("codes", c_void_p),
+        ("scales", c_void_p),
+        ("row_scales", c_void_p),
+        ("rows", c_int64),
+        ("cols", c_int64),
+        ("format", c_int),
+    ]
+
+
 _cache_p = ctypes.POINTER(PageCacheStruct)
+_fp4_p = ctypes.POINTER(Fp4RowsStruct)
 
 # name -> argtypes (all return int status unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -134,11 +148,21 @@ _SIGNATURES = {
     "h3b_pages_truncate": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
     "h3b_pages_compact": [_cache_p, c_void_p, c_int64, c_void_p],
     "h3b_pages_copy": [_cache_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "h3b_fp4_quantize": [c_void_p, c_int, c_int64, _fp4_p, c_void_p],
+    "h3b_fp4_dequantize": [_fp4_p, c_void_p, c_int, c_int64, c_void_p],
+    "h3b_fp4_gemm": [_fp4_p, _fp4_p, c_void_p, c_void_p, c_int, c_int64, c_void_p],
+    "h3b_fp4_linear_workspace_bytes": [c_int64, c_int64, c_int],
+    "h3b_fp4_linear": [c_void_p, c_int, c_int64, c_int64, _fp4_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                       c_void_p],
+    "h3b_add_rms_norm_int8": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64,
+                              c_int64, c_float, c_void_p, c_void_p, c_void_p],
+    "h3b_add_rms_norm_fp4": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, _fp4_p,
+                             c_void_p],
 }
 _RESTYPES = {"h3b_version": ctypes.c_char_p, "h3b_last_error": ctypes.c_char_p,
              "h3b_key_mean_workspace_bytes": c_int64, "h3b_decode_workspace_bytes": c_int64,
              "h3b_window_workspace_bytes": c_int64, "h3b_pages_workspace_bytes": c_int64,
-             "h3b_chained_launches": c_int64}
+             "h3b_chained_launches": c_int64, "h3b_fp4_linear_workspace_bytes": c_int64}
 
 EXPORTED = tuple(_SIGNATURES)
 
@@ -168,11 +192,12 @@ def lib():
 
 
 # kernels each entry launches (for the benchmark's launch count); default 1.  The streaming
-# entries launch as many as the sizes ask for, which the library counts itself.
+# and 4-bit entries launch as many as the sizes ask for, which the library counts itself.
 _KERNELS_PER_CALL = {"value_fp8": 3, "key_mean": 2, "key_mean_no_alloc": 2}
 _KERNELS_PER_CALL |= dict.fromkeys(
     ("window_attention", "paged_window_attention", "decode_attention", "pages_extend", "pages_write", "pages_append",
-     "pages_fork", "pages_truncate", "pages_compact", "pages_copy"), 0)
+     "pages_fork", "pages_truncate", "pages_compact", "pages_copy", "fp4_quantize", "fp4_dequantize", "fp4_gemm",
+     "fp4_linear", "add_rms_norm_int8", "add_rms_norm_fp4"), 0)
 _launches = 0
 _chained_before = 0
 
