@@ -59,14 +59,16 @@ def test_dequantize_and_gemm_refuse_before_a_launch():
 
 
 def test_linear_refuses_before_a_launch():
-    f, need = lib().h3b_fp4_linear, lib().h3b_fp4_linear_workspace_bytes(4, 64, 1)
-    assert need == 4 * 32 + 512
-    assert lib().h3b_fp4_linear_workspace_bytes(200, 100, 2) == 200 * 64 + 2 * 2 * 512 + 800
-    assert lib().h3b_fp4_linear_workspace_bytes(4, 64, 3) == -1
-    assert lib().h3b_fp4_linear_workspace_bytes(4, 32769, 1) == -1
-    _refused(f(A, 2, 4, 64, _rows(), None, A, 4, A, need - 1, None), -1, "workspace")
-    _refused(f(A, 2, 4, 64, _rows(), None, A, 4, None, 0, None), -1, "workspace")
-    _refused(f(A, 2, 4, 64, _rows(), None, A, 4, A + 8, need, None), -2, "aligned")
+    f, size = lib().h3b_fp4_linear, lib().h3b_fp4_linear_workspace_bytes
+    need = size(40, _rows())
+    assert need == 40 * 32 + 512
+    assert size(200, _rows(cols=100, fmt=2, row_scales=A)) == 200 * 64 + 2 * 2 * 512 + 800
+    assert size(4, _rows(fmt=3)) == -1 and size(4, _rows(cols=32769)) == -1 and size(-1, _rows()) == -1
+    assert size(4, None) == -1 and size(0, _rows()) == 0 and size(4, _rows(rows=0)) == 0
+    assert size(4, _rows()) == 0  # few rows are quantised by the product itself
+    _refused(f(A, 2, 40, 64, _rows(), None, A, 4, A, need - 1, None), -1, "workspace")
+    _refused(f(A, 2, 40, 64, _rows(), None, A, 4, None, 0, None), -1, "workspace")
+    _refused(f(A, 2, 40, 64, _rows(), None, A, 4, A + 8, need, None), -2, "aligned")
     _refused(f(A, 2, 4, 64, None, None, A, 4, A, need, None), -1, "null")
     _refused(f(A, 2, 4, 60, _rows(), None, A, 4, A, need, None), -1, "stride")
     _refused(f(A, 2, 4, 64, _rows(), None, A, 3, A, need, None), -1, "stride")

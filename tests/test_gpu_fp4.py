@@ -192,7 +192,8 @@ def test_products_whose_sums_are_exact(h3b, fmt, dtype, m, n, k):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (7, 1003, 1044), (48, 520, 16384), (333, 384, 2048), (1111, 1003, 1056),
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (1, 12288, 4096), (7, 1003, 1044), (16, 333, 4100), (2, 70, 24),
+                                   (11, 8192, 16384), (3, 40000, 8192), (48, 520, 16384), (333, 384, 2048), (1111, 1003, 1056),
                                    (2300, 2050, 700)])
 def test_linear_against_the_definition(h3b, fmt, dtype, m, n, k):
     x, w = _rows(m, k, dtype, seed=m, spread=0.7), _rows(n, k, torch.bfloat16, seed=n, spread=0.3) / 64
@@ -307,11 +308,12 @@ def test_linear_takes_leading_dimensions_and_no_rows(h3b, fmt):
     assert torch.equal(layer.forward_prequantized(layer.quantize(x)), want)
     empty = h3b.Fp4Linear(h3b.quantize_fp4(_rows(96, 80, torch.bfloat16)[:0], fmt))
     assert empty(x).shape == (12, 0)
-    need = h3b.lib().h3b_fp4_linear_workspace_bytes(12, 80, h3b.fp4.FORMATS[fmt])
+    x = x.repeat(10, 1)
+    need = h3b.lib().h3b_fp4_linear_workspace_bytes(120, layer.weight._ref)
     ws = torch.full((need + 64,), 0x5A, device="cuda", dtype=torch.uint8)
-    out = torch.empty(12, 96, device="cuda", dtype=torch.bfloat16)
+    out = torch.empty(120, 96, device="cuda", dtype=torch.bfloat16)
     assert h3b.fp4_linear(x, layer.weight, layer.bias, out=out, workspace=ws) is out
-    assert torch.equal(out, want) and (ws[need:] == 0x5A).all()
+    assert torch.equal(out, want.repeat(10, 1)) and (ws[need:] == 0x5A).all()
 
 
 @pytest.mark.parametrize("m", [1, 40, 2300])
@@ -380,8 +382,8 @@ def test_refusals_on_the_gpu(h3b):
         lambda: h3b.fp4_linear_prequantized(q, q, out=torch.empty(1, 4, device="cuda", dtype=torch.bfloat16).expand(4, 4)),
         lambda: h3b.fp4_linear(x[:, :32], q),
         lambda: h3b.fp4_linear(x.float(), q),
-        lambda: h3b.fp4_linear(x, q, workspace=torch.empty(16, device="cuda", dtype=torch.uint8)),
-        lambda: h3b.fp4_linear(x, q, workspace=torch.empty(1 << 16, device="cuda", dtype=torch.uint8)[1:]),
+        lambda: h3b.fp4_linear(x.repeat(10, 1), q, workspace=torch.empty(16, device="cuda", dtype=torch.uint8)),
+        lambda: h3b.fp4_linear(x.repeat(10, 1), q, workspace=torch.empty(1 << 16, device="cuda", dtype=torch.uint8)[1:]),
         lambda: h3b.fp4_linear(x, q, torch.zeros(4)),
         lambda: h3b.Fp4Rows(q.codes, q.scales, 65, "mxfp4"),
         lambda: h3b.Fp4Rows(q.codes, q.scales, 64, "nvfp4x"),

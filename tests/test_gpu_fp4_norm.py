@@ -219,8 +219,10 @@ def test_launches_are_counted(h3b):
     layer = h3b.Fp4Linear.from_weight(x.repeat(40, 1))
     reset_launch_count()
     layer(x)
-    assert launch_count() == 2
+    assert launch_count() == 1  # few rows are quantised by the product
     h3b.add_rms_norm_quantize(x, r, w)
-    assert launch_count() == 3
+    assert launch_count() == 2
     layer.forward_prequantized(layer.quantize(x))
-    assert launch_count() == 5
+    assert launch_count() == 4
+    layer(x.repeat(40, 1))
+    assert launch_count() == 6

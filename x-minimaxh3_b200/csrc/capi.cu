@@ -948,21 +948,29 @@ int fp4_quantize(const void* x, int dtype, int64_t x_row_stride, const h3b_fp4_r
   set_fp4_output(out, &a);
   return cuda_status(h3b::launch_fp4_rows(a, out->format, dtype == 2, st(stream)), what);
 }
-int fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
-             int64_t out_row_stride, int behind_rows, void* stream, const char* what) {
+h3b::Fp4GemmArgs gemm_args(int64_t rows, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
+                           int64_t out_row_stride) {
   h3b::Fp4GemmArgs a{};
-  a.M = (int)x->rows;
+  a.M = (int)rows;
   a.N = (int)w->rows;
-  a.K = (int)x->cols;
+  a.K = (int)w->cols;
   a.bias = bias;
   a.out = static_cast<uint16_t*>(out);
   a.out_stride = out_row_stride;
   a.bf16 = out_dtype == 2;
+  return a;
+}
+int gemm_status(int r, cudaError_t e, const char* what) {
+  if (r == 1) return fail(H3B_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed");
+  return cuda_status(e, what);
+}
+int fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
+             int64_t out_row_stride, int behind_rows, void* stream, const char* what) {
+  h3b::Fp4GemmArgs a = gemm_args(x->rows, w, bias, out, out_dtype, out_row_stride);
   a.behind_rows = behind_rows;
   cudaError_t e = cudaSuccess;
   const int r = h3b::launch_fp4_gemm(fp4_view(x), fp4_view(w), a, x->format, st(stream), &e);
-  if (r == 1) return fail(H3B_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed");
-  return cuda_status(e, what);
+  return gemm_status(r, e, what);
 }
 // what a product checks of its weight, bias and output
 int check_fp4_product(int64_t M, const h3b_fp4_rows* w, const void* out, int out_dtype, int64_t out_row_stride,
@@ -991,7 +999,7 @@ int h3b_fp4_dequantize(const h3b_fp4_rows* rows, void* out, int dtype, int64_t o
   if (!e) e = check_half_rows(out, dtype, rows->rows, rows->cols, out_row_stride, "fp4_dequantize");
   if (e) return e;
   if (rows->rows == 0) return ok();
-  if ((rows->cols + 15) / 16 * rows->rows > ((int64_t)INT_MAX << 8))
+  if ((rows->cols + 511) / 512 * rows->rows > ((int64_t)INT_MAX << 3))
     return fail(H3B_ERR_UNSUPPORTED, "fp4_dequantize: too many elements");
   return cuda_status(h3b::launch_fp4_dequantize(fp4_view(rows), rows->format, static_cast<uint16_t*>(out),
                                                 out_row_stride, dtype == 2, st(stream)), "fp4_dequantize");
@@ -1008,11 +1016,13 @@ int h3b_fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias
   return fp4_gemm(x, w, bias, out, out_dtype, out_row_stride, 0, stream, "fp4_gemm");
 }
 
-int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, int64_t cols, int format) {
-  if (rows < 0 || cols < 1 || rows > (1 << 30) || cols > h3b::kFp4MaxRowCols || (format != H3B_MXFP4 && format != H3B_NVFP4))
+int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, const h3b_fp4_rows* w) {
+  if (!w || rows < 0 || rows > (1 << 30) || w->rows < 0 || w->rows > (1 << 30) || w->cols < 1 ||
+      w->cols > h3b::kFp4MaxRowCols || (w->format != H3B_MXFP4 && w->format != H3B_NVFP4))
     return -1;
-  return align16(rows * h3b::fp4_pitch(cols)) + h3b::fp4_scale_bytes(rows, cols, format) +
-         (format == H3B_NVFP4 ? align16(4 * rows) : 0);
+  if (rows == 0 || w->rows == 0 || h3b::fp4_takes_rows16(rows, w->rows, w->cols)) return 0;
+  return rows * h3b::fp4_pitch(w->cols) + h3b::fp4_scale_bytes(rows, w->cols, w->format) +
+         (w->format == H3B_NVFP4 ? align16(4 * rows) : 0);
 }
 
 int h3b_fp4_linear(const void* x, int dtype, int64_t rows, int64_t x_row_stride, const h3b_fp4_rows* w,
@@ -1024,11 +1034,18 @@ int h3b_fp4_linear(const void* x, int dtype, int64_t rows, int64_t x_row_stride,
   if (e) return e;
   if (w->cols > h3b::kFp4MaxRowCols) return fail(H3B_ERR_UNSUPPORTED, "fp4_linear: more than 32768 columns");
   if (rows == 0 || w->rows == 0) return ok();
-  if (!workspace || workspace_bytes < h3b_fp4_linear_workspace_bytes(rows, w->cols, w->format))
-    return fail(H3B_ERR_INVALID_ARGUMENT, "fp4_linear: workspace too small");
+  const int64_t need = h3b_fp4_linear_workspace_bytes(rows, w);
+  if (need == 0) {
+    h3b::Fp4GemmArgs a = gemm_args(rows, w, bias, out, dtype, out_row_stride);
+    cudaError_t err = cudaSuccess;
+    const int r = h3b::launch_fp4_gemm_rows16(static_cast<const uint16_t*>(x), x_row_stride, fp4_view(w), a, w->format,
+                                              st(stream), &err);
+    return gemm_status(r, err, "fp4_linear");
+  }
+  if (!workspace || workspace_bytes < need) return fail(H3B_ERR_INVALID_ARGUMENT, "fp4_linear: workspace too small");
   if (!aligned16(workspace)) return fail(H3B_ERR_UNSUPPORTED, "fp4_linear: workspace must be 16-byte aligned");
   char* at = static_cast<char*>(workspace);
-  h3b_fp4_rows q{at, at + align16(rows * h3b::fp4_pitch(w->cols)), nullptr, rows, w->cols, w->format};
+  h3b_fp4_rows q{at, at + rows * h3b::fp4_pitch(w->cols), nullptr, rows, w->cols, w->format};
   if (w->format == H3B_NVFP4)
     q.row_scales = reinterpret_cast<float*>(static_cast<char*>(q.scales) + h3b::fp4_scale_bytes(rows, w->cols, w->format));
   e = fp4_quantize(x, dtype, x_row_stride, &q, stream, "fp4_linear");

@@ -72,10 +72,19 @@ struct Fp4GemmArgs {
   int64_t out_stride;
   int bf16;
   int behind_rows;  // launched right behind the kernel that quantises x, after which w does not change
+  // 16-bit rows that the product quantises itself (launch_fp4_gemm_rows16)
+  const uint16_t* x16;
+  int64_t x16_stride;
+  int x16_vec;  // they allow 16-byte accesses
 };
 // 0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err)
 int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, int format, cudaStream_t s,
                     cudaError_t* err);
+
+// Whether a linear of these sizes quantises its 16-bit rows inside the product, and that product
+bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K);
+int launch_fp4_gemm_rows16(const uint16_t* x, int64_t x_stride, const Fp4RowsView& w, Fp4GemmArgs a, int format,
+                           cudaStream_t s, cudaError_t* err);
 
 template <bool BF16>
 __device__ __forceinline__ float half_to_f32(uint16_t b) {
@@ -89,5 +98,75 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
   return (uint32_t)f32_to_half_bits<BF16>(lo) | ((uint32_t)f32_to_half_bits<BF16>(hi) << 16);
 }
+
+// ------------------------------------------------------------------ a chunk of 16 columns to codes
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// two floats -> E2M1 codes, to nearest even, saturating; lo in bits 0..3
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float e4m3_to_f32(uint32_t code) {
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)code));
+  return __half2float(__ushort_as_half((uint16_t)(h2 & 0xffffu)));
+}
+__device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
+  return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7FC00000u : b << 23);
+}
+
+// The 16 codes (w) and the block's scale byte of a chunk v, of which the block's absmax has the
+// bits `top`; inv_r: 1 / row scale.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t quantize16(const float (&v)[16], uint32_t top, float inv_r, uint32_t (&w)[2]) {
+  const bool bad = top >= kInfBits;
+  uint32_t byte;
+  w[0] = w[1] = 0u;
+  if constexpr (FORMAT == kMxfp4) {
+    byte = bad ? 255u : (uint32_t)max((int)(top >> 23) - 2, 0);
+    const float inv = __uint_as_float((254u - byte) << 23);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) w[j >> 3] |= e2m1x2(__fmul_rn(v[j], inv), __fmul_rn(v[j + 1], inv)) << (4 * (j & 7));
+  } else {
+    byte = bad ? 0x7Fu : (uint32_t)f32x2_to_e4m3x2(__fdiv_rn(__fmul_rn(__uint_as_float(top), inv_r), 6.0f), 0.0f) & 0xffu;
+    const float s = e4m3_to_f32(byte);
+    const float rs = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;  // under a scale of zero: zeros, with their signs
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      // the remainder of -0 is 0 and would make the quotient 0: the sign is x's
+      const float q0 = copysignf(div_rn_by(__fmul_rn(v[j], inv_r), s, rs), v[j]);
+      const float q1 = copysignf(div_rn_by(__fmul_rn(v[j + 1], inv_r), s, rs), v[j + 1]);
+      w[j >> 3] |= e2m1x2(q0, q1) << (4 * (j & 7));
+    }
+  }
+  if (bad) w[0] = w[1] = 0u;
+  return byte;
+}
+__device__ __forceinline__ uint32_t absmax16(const float (&v)[16]) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  return top;
+}
+// The exponent of an nvfp4 row's scale from its absmax's bits: least e with absmax <= 2688 * 2^e =
+// 1.3125 * 2^(11 + e), at least -126; 0 for a row of zeros.
+__device__ __forceinline__ int row_exponent(uint32_t top) {
+  return top ? max((int)(top >> 23) - 138 + ((top & 0x7FFFFFu) > 0x280000u ? 1 : 0), -126) : 0;
+}
+__device__ __forceinline__ float exp2_bits(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+// Four blocks' scale bytes to a word, in all lanes that share it: those of four lanes with a
+// chunk each (nvfp4) or of four pairs of lanes (mxfp4).
+template <int FORMAT>
+struct ScaleWord {
+  static constexpr int kLanes = FORMAT == kMxfp4 ? 8 : 4;
+  __device__ __forceinline__ static uint32_t of(uint32_t byte, int lane) {
+    uint32_t word = byte << (8 * ((lane / (kLanes / 4)) & 3));
+#pragma unroll
+    for (int o = kLanes / 4; o < kLanes; o *= 2) word |= __shfl_xor_sync(0xffffffffu, word, o);
+    return word;
+  }
+};
 
 }  // namespace h3b

@@ -55,12 +55,18 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t sdesc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
 
+// A sum to its output value; xs and ws are 1 where there are no row scales
+__device__ __forceinline__ float fp4_finish(float sum, float xs, float ws, float bias, const Fp4GemmArgs& a) {
+  const float v = __fmul_rn(__fmul_rn(sum, xs), ws);
+  return a.bias ? __fadd_rn(v, bias) : v;
+}
+
 // One thread: the scale copies and products of one K step into accumulator d.  BANDS: 128-row
-// bands of scales of the B operand.
+// bands of scales of the B operand, whose first row's scales lie in column column_b of theirs.
 template <int FORMAT, int CTAS, int M, int N, int BANDS>
 __device__ __forceinline__ void fp4_step(uint32_t d, uint32_t smem_a, uint32_t smem_b, uint32_t smem_sa,
-                                         uint32_t smem_sb, uint32_t tmem_sa, uint32_t tmem_sb, int products,
-                                         bool first) {
+                                         uint32_t smem_sb, uint32_t tmem_sa, uint32_t tmem_sb, uint32_t column_b,
+                                         int products, bool first) {
   constexpr int kTiles = FORMAT == kMxfp4 ? 2 : 4;  // scale tiles per band and step
 #pragma unroll
   for (int g = 0; g < kTiles; ++g) {
@@ -77,53 +83,62 @@ __device__ __forceinline__ void fp4_step(uint32_t d, uint32_t smem_a, uint32_t s
     const uint32_t byte = FORMAT == kMxfp4 ? 2u * (uint32_t)(k & 1) : 0u;
     const uint32_t g = FORMAT == kMxfp4 ? (uint32_t)(k >> 1) : (uint32_t)k;
     mma_fp4<FORMAT, CTAS>(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_fp4(M, N, FORMAT == kMxfp4, byte),
-                          tmem_sa + 4u * g, tmem_sb + 4u * BANDS * g, first && k == 0 ? 0u : 1u);
+                          tmem_sa + 4u * g, tmem_sb + 4u * BANDS * g + column_b, first && k == 0 ? 0u : 1u);
   }
 }
 
 // ------------------------------------------------------------------ few rows: a split over K
 // A tile is 128 rows of the weight (the products' M) x TOK rows of x (their N), so that one
-// token costs the reading of the weight and hardly more.  The cluster's CTAs take equal parts
+// token costs the reading of the weight and hardly more.  The CTAs of a cluster take equal parts
 // of K; each puts its sums into its shared memory, and every CTA adds up and writes out a part
-// of the tile's tokens, from all CTAs in their order (the same sums every time).  Two CTAs fit
-// an SM.  Launched behind the quantisation of x, the first weight tiles are on their way
-// before that has ended.
+// of the tile's tokens, from all CTAs in their order (the same sums every time).  Without a
+// split the sums go out as they come from tensor memory.  Two CTAs fit an SM.
 //   warp 0: TMA, warp 1: tensor memory and products, warps 2-5: sums; all: the joining
-template <int FORMAT, int TOK>
+// Behind the quantisation of x in the stream, the first weight tiles are on their way before
+// that has ended.  ROWS16: x is 16-bit, at most 16 rows, and warps 2-5 of each CTA quantise
+// its part of K themselves (for nvfp4 the cluster's CTAs tell each other their rows' absmax).
+template <int FORMAT, int TOK, bool ROWS16>
 struct SplitCfg {
+  static_assert(!ROWS16 || TOK == 16, "rows are quantised here for a tile of 16");
   static constexpr int kScaleBytes = FORMAT == kMxfp4 ? 1024 : 2048;  // of a band and step
   static constexpr int kWBytes = 128 * kF4Step;
   static constexpr int kXBytes = TOK * kF4Step;
-  static constexpr int kStageBytes = kWBytes + kXBytes + 2 * kScaleBytes;
-  static constexpr int kStages = TOK == 128 ? 3 : TOK == 64 ? 3 : 4;
-  static constexpr int kTotal = kStages * kStageBytes + 1024;
+  static constexpr int kXStep = kXBytes + kScaleBytes;
+  static constexpr int kStageBytes = kWBytes + kScaleBytes + (ROWS16 ? 0 : kXStep);
+  static constexpr int kStages = TOK == 128 ? 3 : 4;
   static constexpr int kAccCols = TOK < 32 ? 32 : TOK;
   static constexpr int kTmemCols = kAccCols + 64 <= 128 ? 128 : 256;  // and two slots of 16 + 16 columns of scales
-  static_assert(kStageBytes % 1024 == 0, "swizzled tiles start at multiples of 1024");
+  static_assert(kStageBytes % 1024 == 0 && kXStep % 1024 == 0, "swizzled tiles start at multiples of 1024");
   static_assert(128 * TOK * 4 <= kStages * kStageBytes, "the sums take the stages' place");
+  static constexpr int smem_bytes(int steps) { return kStages * kStageBytes + (ROWS16 ? steps * kXStep : 0) + 1024; }
 };
 constexpr int kSplitThreads = 192;
+constexpr int kRows16Steps = 8;  // K steps of a CTA that quantises x: what fits twice on an SM
 
-template <int FORMAT, int TOK>
+template <int FORMAT, int TOK, bool ROWS16, bool BF16>
 __global__ void __launch_bounds__(kSplitThreads)
-    fp4_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                     const __grid_constant__ CUtensorMap tm_sw, const __grid_constant__ CUtensorMap tm_sx,
+    fp4_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sw,
+                     const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_sx,
                      Fp4GemmArgs a, int split) {
-  using C = SplitCfg<FORMAT, TOK>;
+  using C = SplitCfg<FORMAT, TOK, ROWS16>;
   constexpr int kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kStages], empty[kStages], done;
+  __shared__ uint64_t full[kStages], empty[kStages], done, x_ready;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, late_flag;
+  __shared__ uint32_t row_top[16];
+  __shared__ float row_scale[16];
+  __shared__ __align__(16) uint16_t stages[ROWS16 ? 4 : 1][ROWS16 ? 512 : 8];
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
   const int num_n = (a.N + 127) / 128;
   const int tile = blockIdx.x / split;
   const int n0 = tile % num_n * 128, m0 = tile / num_n * TOK;
   const int num_k = (a.K + 255) / 256;
   const int kb0 = (int)((int64_t)num_k * rank / split), steps = (int)((int64_t)num_k * (rank + 1) / split) - kb0;
+  uint8_t* x_area = smem + kStages * C::kStageBytes;  // ROWS16: [steps] codes and scales
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -131,9 +146,11 @@ __global__ void __launch_bounds__(kSplitThreads)
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, 1);
+    mbar_init(&x_ready, 128);
     abort_flag = late_flag = 0;
     fence_mbar_init();
   }
+  if (ROWS16 && threadIdx.x < 16) row_top[threadIdx.x] = 0u;
   if (warp == 1) {
     tmem_alloc(&tmem_slot, C::kTmemCols);
     tmem_relinquish();
@@ -149,13 +166,14 @@ __global__ void __launch_bounds__(kSplitThreads)
       uint8_t* at = smem + i % kStages * C::kStageBytes;
       mbar_arrive_expect_tx(&full[i % kStages], C::kStageBytes);
       tma_load_2d(at, &tm_w, &full[i % kStages], (kb0 + i) * kF4Step, n0);
-      tma_load_2d(at + C::kWBytes + C::kXBytes, &tm_sw, &full[i % kStages], (kb0 + i) * (C::kScaleBytes / 8), n0 >> 7);
+      tma_load_2d(at + C::kWBytes, &tm_sw, &full[i % kStages], (kb0 + i) * (C::kScaleBytes / 8), n0 >> 7);
     };
     auto load_x = [&](int i) {
-      uint8_t* at = smem + i % kStages * C::kStageBytes;
-      tma_load_2d(at + C::kWBytes, &tm_x, &full[i % kStages], (kb0 + i) * kF4Step, m0);
-      tma_load_2d(at + C::kWBytes + C::kXBytes + C::kScaleBytes, &tm_sx, &full[i % kStages],
-                  (kb0 + i) * (C::kScaleBytes / 8), m0 >> 7);
+      if constexpr (!ROWS16) {
+        uint8_t* at = smem + i % kStages * C::kStageBytes + C::kWBytes + C::kScaleBytes;
+        tma_load_2d(at, &tm_x, &full[i % kStages], (kb0 + i) * kF4Step, m0);
+        tma_load_2d(at + C::kXBytes, &tm_sx, &full[i % kStages], (kb0 + i) * (C::kScaleBytes / 8), m0 >> 7);
+      }
     };
     const int ahead = steps < kStages ? steps : kStages;
     if (!a.behind_rows) chain_wait();
@@ -163,9 +181,10 @@ __global__ void __launch_bounds__(kSplitThreads)
       for (int i = 0; i < ahead; ++i) load_w(i);
     __syncwarp();
     if (a.behind_rows) chain_wait();
-    if (elect_one())
+    if (!ROWS16 && elect_one())
       for (int i = 0; i < ahead; ++i) load_x(i);
     __syncwarp();
+    if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
     int fills = ahead;
     for (; fills < steps; ++fills) {
       if (!mbar_wait_warp(&empty[fills % kStages], (fills / kStages - 1) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
@@ -179,8 +198,10 @@ __global__ void __launch_bounds__(kSplitThreads)
     for (int i = fills > kStages ? fills - kStages : 0; i < fills; ++i)
       mbar_wait_warp(&full[i % kStages], (i / kStages) & 1, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
   } else if (warp == 1) {
-    const uint32_t smem0 = smem_u32(smem);
-    for (int i = 0; i < steps; ++i) {
+    const uint32_t smem0 = smem_u32(smem), x0 = smem_u32(x_area);
+    if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
+    const bool ready = !ROWS16 || mbar_wait_warp(&x_ready, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
+    for (int i = 0; ready && i < steps; ++i) {
       if (!mbar_wait_warp(&full[i % kStages], (i / kStages) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
       // the scale slot of this step: read by the products of the step before last
       if (i >= 2 && !mbar_wait_warp(&empty[(i - 2) % kStages], ((i - 2) / kStages) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT))
@@ -188,10 +209,12 @@ __global__ void __launch_bounds__(kSplitThreads)
       tc_fence_after();
       if (elect_one()) {
         const uint32_t at = smem0 + (uint32_t)(i % kStages * C::kStageBytes);
+        const uint32_t x = ROWS16 ? x0 + (uint32_t)(i * C::kXStep) : at + C::kWBytes + C::kScaleBytes;
         const uint32_t ts = tmem + C::kAccCols + 32u * (uint32_t)(i & 1);
         const int products = (a.K - (kb0 + i) * 256 + 63) / 64;
-        fp4_step<FORMAT, 1, 128, TOK, 1>(tmem, at, at + C::kWBytes, at + C::kWBytes + C::kXBytes,
-                                         at + C::kWBytes + C::kXBytes + C::kScaleBytes, ts, ts + 16, products, i == 0);
+        // rows m0 .. of their 128-row band: 32 to a column of the scales in tensor memory
+        fp4_step<FORMAT, 1, 128, TOK, 1>(tmem, at, x, at + C::kWBytes, x + C::kXBytes, ts, ts + 16,
+                                         (uint32_t)(m0 >> 5) & 3u, products, i == 0);
         mma_commit(&empty[i % kStages]);
       }
       __syncwarp();
@@ -201,63 +224,127 @@ __global__ void __launch_bounds__(kSplitThreads)
     mbar_wait_warp(&done, 0, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
     chain_wait();
   } else {
-    const int row = (warp & 3) * 32 + (threadIdx.x & 31);
     chain_wait();
+    if constexpr (ROWS16) {
+      // a warp takes 32 chunks of 16 columns of a row at a time
+      const uint16_t* x = a.x16 + kb0 * 256;
+      const int K = a.K - kb0 * 256, segs = (steps + 1) / 2, items = a.M * segs;
+      const bool vec = a.x16_vec;
+      uint16_t* stage = stages[warp - 2];
+      float v[16];
+      auto load = [&](int item) {
+        const uint16_t* row = x + (int64_t)(item / segs) * a.x16_stride;
+        const int c = item % segs * 32 + lane;
+        if (vec) load16<BF16, true>(row, c, K, stage, v);
+        else load16<BF16, false>(row, c, K, stage, v);
+      };
+      if constexpr (FORMAT == kNvfp4) {
+        for (int item = warp - 2; item < items; item += 4) {
+          load(item);
+          uint32_t top = absmax16(v);
+          if (top >= kInfBits) top = 0u;
+          top = __reduce_max_sync(0xffffffffu, top);
+          if (lane == 0) atomicMax(&row_top[item / segs], top);
+        }
+        cluster_sync_all();
+      }
+      for (int item = warp - 2; item < items; item += 4) {
+        const int r = item / segs, c = item % segs * 32 + lane;
+        if (FORMAT == kMxfp4 || items > 4) load(item);  // else it is there from above
+        float inv_r = 1.0f;
+        if constexpr (FORMAT == kNvfp4) {
+          uint32_t top = 0u;
+          if (lane < split)
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(top) : "r"(mapa_shared(smem_u32(&row_top[r]), (uint32_t)lane)));
+          const int e = row_exponent(__reduce_max_sync(0xffffffffu, top));
+          inv_r = exp2_bits(-e);
+          if (lane == 0) row_scale[r] = exp2_bits(e);
+        }
+        uint32_t top = absmax16(v), w[2];
+        if (FORMAT == kMxfp4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        const uint32_t word = ScaleWord<FORMAT>::of(quantize16<FORMAT>(v, top, inv_r, w), lane);
+        constexpr int kLanes = ScaleWord<FORMAT>::kLanes;
+        if (c < steps * 16) {
+          uint8_t* at = x_area + (c >> 4) * C::kXStep;
+          // 16-byte pieces of a 128-byte row are swizzled by the row, as a TMA copy would leave them
+          *reinterpret_cast<uint2*>(at + r * 128 + (((((c & 15) >> 1) ^ r) & 7) << 4) + (c & 1) * 8) = make_uint2(w[0], w[1]);
+          if ((lane & (kLanes - 1)) == 0)
+            *reinterpret_cast<uint32_t*>(at + C::kXBytes + (c & 15) / kLanes * 512 + r * 16) = word;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&x_ready);
+    }
+    const int quad = warp & 3, row = quad * 32 + lane, toks = min(TOK, a.M - m0);
     if (mbar_wait_warp(&done, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) {
       tc_fence_after();
       float* sums = reinterpret_cast<float*>(smem);  // [TOK][128]
+      const int n = n0 + row;
+      const float ws = a.ws && n < a.N ? a.ws[n] : 1.0f, bias = a.bias && n < a.N ? a.bias[n] : 0.0f;
 #pragma unroll 1
-      for (int c = 0; c < TOK; c += 16) {
+      for (int c = 0; c < toks; c += 16) {
         uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, r);
+        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, r);
         tmem_wait_ld();
         reg_barrier16(r);
+        if (split > 1) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + row] = __uint_as_float(r[j]);
+          for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + row] = __uint_as_float(r[j]);
+        } else if (n < a.N) {
+          uint16_t* dst = a.out + (int64_t)(m0 + c) * a.out_stride + n;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (c + j >= toks) break;
+            const float xs = ROWS16 ? (FORMAT == kNvfp4 ? row_scale[c + j] : 1.0f) : a.xs ? a.xs[m0 + c + j] : 1.0f;
+            dst[j * a.out_stride] = f32_to_half_bits<BF16>(fp4_finish(__uint_as_float(r[j]), xs, ws, bias, a));
+          }
+        }
+        __syncwarp();
       }
     }
     tc_fence_before();
   }
-  cluster_sync_all();
-
-  const int t0 = TOK * rank / split, t1 = min(TOK * (rank + 1) / split, a.M - m0);
-  const uint32_t sums0 = smem_u32(smem);
-  const bool wide = (a.out_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
-  for (int i = (int)threadIdx.x; i < (t1 - t0) * 32; i += kSplitThreads) {
-    const int tok = t0 + (i >> 5), c = (i & 31) * 4, n = n0 + c;
-    if (n >= a.N) continue;
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int r = 0; r < split; ++r) {
-      float4 p;
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
-                   : "r"(mapa_shared(sums0 + (uint32_t)(tok * 512 + c * 4), (uint32_t)r)));
-      y[0] = __fadd_rn(y[0], p.x);
-      y[1] = __fadd_rn(y[1], p.y);
-      y[2] = __fadd_rn(y[2], p.z);
-      y[3] = __fadd_rn(y[3], p.w);
-    }
-    const float xs = a.xs ? a.xs[m0 + tok] : 1.0f;
-    uint16_t h[4];
+  if (split > 1) {
+    cluster_sync_all();
+    const int t0 = TOK * rank / split, t1 = min(TOK * (rank + 1) / split, a.M - m0);
+    const uint32_t sums0 = smem_u32(smem);
+    const bool wide = (a.out_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
+    for (int i = (int)threadIdx.x; i < (t1 - t0) * 32; i += kSplitThreads) {
+      const int tok = t0 + (i >> 5), c = (i & 31) * 4, n = n0 + c;
+      if (n >= a.N) continue;
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int r = 0; r < split; ++r) {
+        float4 p;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
+                     : "r"(mapa_shared(sums0 + (uint32_t)(tok * 512 + c * 4), (uint32_t)r)));
+        y[0] = __fadd_rn(y[0], p.x);
+        y[1] = __fadd_rn(y[1], p.y);
+        y[2] = __fadd_rn(y[2], p.z);
+        y[3] = __fadd_rn(y[3], p.w);
+      }
+      const float xs = ROWS16 ? (FORMAT == kNvfp4 ? row_scale[tok] : 1.0f) : a.xs ? a.xs[m0 + tok] : 1.0f;
+      uint16_t h[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int nn = min(n + j, a.N - 1);
-      float v = __fmul_rn(y[j], xs);
-      if (a.ws) v = __fmul_rn(v, a.ws[nn]);
-      if (a.bias) v = __fadd_rn(v, a.bias[nn]);
-      h[j] = a.bf16 ? f32_to_half_bits<true>(v) : f32_to_half_bits<false>(v);
-    }
-    uint16_t* dst = a.out + (int64_t)(m0 + tok) * a.out_stride + n;
-    if (wide && n + 4 <= a.N) {
-      *reinterpret_cast<uint2*>(dst) =
-          make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
-    } else {
+      for (int j = 0; j < 4; ++j) {
+        const int nn = min(n + j, a.N - 1);
+        h[j] = f32_to_half_bits<BF16>(fp4_finish(y[j], xs, a.ws ? a.ws[nn] : 1.0f, a.bias ? a.bias[nn] : 0.0f, a));
+      }
+      uint16_t* dst = a.out + (int64_t)(m0 + tok) * a.out_stride + n;
+      if (wide && n + 4 <= a.N) {
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) dst[j] = h[j];
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) dst[j] = h[j];
+      }
     }
+    cluster_sync_all();  // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
   }
-  cluster_sync_all();  // no CTA leaves while another reads its sums
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
@@ -416,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
             const uint32_t at = smem0 + stage * C::kStageBytes;
             const uint32_t ts = tmem + kPairFp4Scales + 48u * (it & 1);
             fp4_step<FORMAT, 2, 256, 256, 2>(d, at, at + 128 * kF4Step, at + 2 * 128 * kF4Step,
-                                             at + 2 * 128 * kF4Step + C::kScaleBytes, ts, ts + 16,
+                                             at + 2 * 128 * kF4Step + C::kScaleBytes, ts, ts + 16, 0u,
                                              (a.K - kb * 256 + 63) / 64, kb == 0);
             mma_commit_pair(&empty[stage], 0x3);
           }
@@ -516,17 +603,36 @@ static bool make_fp4_maps(const Fp4RowsView& v, int format, int box_rows, int bo
                       words * 8, format == kMxfp4 ? 128 : 256, (uint32_t)box_bands, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int FORMAT, int TOK>
-static int launch_split(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, cudaStream_t s,
-                        cudaError_t* err) {
-  CUtensorMap tx, tw, tsx, tsw;
-  if (!make_fp4_maps(x, FORMAT, TOK, 1, &tx, &tsx) || !make_fp4_maps(w, FORMAT, 128, 1, &tw, &tsw)) return 1;
-  const int64_t tiles = (int64_t)((a.N + 127) / 128) * ((a.M + TOK - 1) / TOK);
-  const int num_k = (a.K + 255) / 256;
+#ifdef FORCE
+#include <cstdlib>
+static int env(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+#endif
+// How a product of few rows is divided: TOK and the CTAs along K
+struct SplitPlan {
+  int tok, split;
+};
+static SplitPlan plan_split(int M, int N, int K) {
+#ifdef FORCE
+  if (env("H3B_TOK", 0)) return {env("H3B_TOK", 0), env("H3B_SPLIT", 1)};
+#endif
+  const int tok = M <= 16 ? 16 : M <= 64 ? 64 : 128, num_k = (K + 255) / 256;
+  const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + tok - 1) / tok);
   int split = 1;
   while (split < 8 && 2 * split <= num_k && tiles * 2 * split <= 2 * num_sms()) split *= 2;
-  *err = launch_fp4(fp4_split_kernel<FORMAT, TOK>, tiles * split, split, kSplitThreads, SplitCfg<FORMAT, TOK>::kTotal, s,
-                    tw, tx, tsw, tsx, a, split);
+  return {tok, split};
+}
+template <int FORMAT, int TOK, bool ROWS16>
+static int launch_split(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, int split, cudaStream_t s,
+                        cudaError_t* err) {
+  CUtensorMap tx, tw, tsx, tsw;
+  if (!make_fp4_maps(w, FORMAT, 128, 1, &tw, &tsw)) return 1;
+  if (ROWS16) tx = tw, tsx = tsw;  // not used
+  else if (!make_fp4_maps(x, FORMAT, TOK, 1, &tx, &tsx)) return 1;
+  const int64_t tiles = (int64_t)((a.N + 127) / 128) * ((a.M + TOK - 1) / TOK);
+  const int steps = ((a.K + 255) / 256 + split - 1) / split;
+  *err = launch_fp4(a.bf16 ? fp4_split_kernel<FORMAT, TOK, ROWS16, true> : fp4_split_kernel<FORMAT, TOK, ROWS16, false>,
+                    tiles * split, split, kSplitThreads, SplitCfg<FORMAT, TOK, ROWS16>::smem_bytes(steps), s, tw, tsw, tx,
+                    tsx, a, split);
   return *err == cudaSuccess ? 0 : 2;
 }
 template <int FORMAT>
@@ -540,14 +646,20 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
                     kPairFp4Threads, PairFp4Cfg<FORMAT>::kTotal, s, tx, tw, tsx, tsw, a);
   return *err == cudaSuccess ? 0 : 2;
 }
+static bool uses_pair(int M, int N) {
+#ifdef FORCE
+  if (env("H3B_PAIR", -1) >= 0) return env("H3B_PAIR", 0);
+#endif
+  return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= num_sms() / 2;
+}
 template <int FORMAT>
 static int launch_gemm_of(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, cudaStream_t s,
                           cudaError_t* err) {
-  const int64_t pair_tiles = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
-  if (pair_tiles >= num_sms() / 2) return launch_pair<FORMAT>(x, w, a, s, err);
-  return a.M <= 16   ? launch_split<FORMAT, 16>(x, w, a, s, err)
-         : a.M <= 64 ? launch_split<FORMAT, 64>(x, w, a, s, err)
-                     : launch_split<FORMAT, 128>(x, w, a, s, err);
+  if (uses_pair(a.M, a.N)) return launch_pair<FORMAT>(x, w, a, s, err);
+  const SplitPlan p = plan_split(a.M, a.N, a.K);
+  return p.tok == 16   ? launch_split<FORMAT, 16, false>(x, w, a, p.split, s, err)
+         : p.tok == 64 ? launch_split<FORMAT, 64, false>(x, w, a, p.split, s, err)
+                       : launch_split<FORMAT, 128, false>(x, w, a, p.split, s, err);
 }
 
 int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, int format, cudaStream_t s,
@@ -555,6 +667,22 @@ int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, i
   a.xs = x.row_scales;
   a.ws = w.row_scales;
   return format == kMxfp4 ? launch_gemm_of<kMxfp4>(x, w, a, s, err) : launch_gemm_of<kNvfp4>(x, w, a, s, err);
+}
+
+bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K) {
+  if (M > 16 || uses_pair((int)M, (int)N)) return false;
+  const SplitPlan p = plan_split((int)M, (int)N, (int)K);
+  return p.tok == 16 && (K + 255) / 256 <= (int64_t)kRows16Steps * p.split;
+}
+int launch_fp4_gemm_rows16(const uint16_t* x, int64_t x_stride, const Fp4RowsView& w, Fp4GemmArgs a, int format,
+                           cudaStream_t s, cudaError_t* err) {
+  a.ws = w.row_scales;
+  a.x16 = x;
+  a.x16_stride = x_stride;
+  a.x16_vec = a.K % 16 == 0 && rows16(x, a.M > 1 ? x_stride : 0);
+  const int split = plan_split(a.M, a.N, a.K).split;
+  return format == kMxfp4 ? launch_split<kMxfp4, 16, true>({}, w, a, split, s, err)
+                          : launch_split<kNvfp4, 16, true>({}, w, a, split, s, err);
 }
 
 }  // namespace h3b

@@ -22,23 +22,6 @@
 
 namespace h3b {
 
-constexpr uint32_t kInfBits = 0x7F800000u;
-
-// two floats -> E2M1 codes, to nearest even, saturating; lo in bits 0..3
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float e4m3_to_f32(uint32_t code) {
-  uint32_t h2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)code));
-  return __half2float(__ushort_as_half((uint16_t)(h2 & 0xffffu)));
-}
-__device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
-  return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7FC00000u : b << 23);
-}
-
 // max of non-negative floats' bits over the row's threads (a warp, or the block)
 template <bool BLOCK>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
@@ -63,39 +46,95 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
-// 16 columns from column c0 on, zeros beyond K.  VEC: all pointers and strides allow 16-byte
-// accesses and K is a multiple of 16.
+// 16 columns from chunk c (of 16 columns) on, zeros beyond K; neighbouring lanes of a warp ask for
+// neighbouring chunks.  VEC: all pointers and strides allow 16-byte accesses and K is a multiple
+// of 16.  Otherwise the warp moves its 512 columns together, through `stage`, in words or 16-bit
+// pieces as the row's address allows (a lane's own 16 pieces would be 32 bytes apart from its
+// neighbours': 3,607 rows of 1,044 columns to nvfp4 and back took 34 us that way).
 template <bool BF16, bool VEC>
-__device__ __forceinline__ void load16(const uint16_t* row, int c0, int K, float (&v)[16]) {
+__device__ __forceinline__ void load16(const uint16_t* row, int c, int K, uint16_t* stage, float (&v)[16]) {
+  uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
   if constexpr (VEC) {
-    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-    const bool live = c0 < K;
-    const uint4 a = live ? *reinterpret_cast<const uint4*>(row + c0) : z;
-    const uint4 b = live ? *reinterpret_cast<const uint4*>(row + c0 + 8) : z;
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[2 * i] = half_to_f32<BF16>((uint16_t)(w[i] & 0xffffu));
-      v[2 * i + 1] = half_to_f32<BF16>((uint16_t)(w[i] >> 16));
+    if (c * 16 < K) {
+      a = *reinterpret_cast<const uint4*>(row + c * 16);
+      b = *reinterpret_cast<const uint4*>(row + c * 16 + 8);
     }
   } else {
+    const int lane = threadIdx.x & 31, base = (c - lane) * 16, n = K - base;
+    const uint16_t* src = row + base;
+    if ((reinterpret_cast<uintptr_t>(row) & 3) == 0) {
+      uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c0 + i < K ? half_to_f32<BF16>(row[c0 + i]) : 0.0f;
+      for (int j = 0; j < 8; ++j) {
+        const int at = j * 64 + lane * 2;
+        w[j] = at + 1 < n ? *reinterpret_cast<const uint32_t*>(src + at) : at < n ? (uint32_t)src[at] : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) reinterpret_cast<uint32_t*>(stage)[j * 32 + lane] = w[j];
+    } else {
+      uint16_t h[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) h[j] = j * 32 + lane < n ? src[j * 32 + lane] : (uint16_t)0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) stage[j * 32 + lane] = h[j];
+    }
+    __syncwarp();
+    a = *reinterpret_cast<const uint4*>(stage + lane * 16);
+    b = *reinterpret_cast<const uint4*>(stage + lane * 16 + 8);
+    __syncwarp();
+  }
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = half_to_f32<BF16>((uint16_t)(w[i] & 0xffffu));
+    v[2 * i + 1] = half_to_f32<BF16>((uint16_t)(w[i] >> 16));
   }
 }
 template <bool BF16, bool VEC>
-__device__ __forceinline__ void store16(uint16_t* row, int c0, int K, const float (&v)[16]) {
+__device__ __forceinline__ void store16(uint16_t* row, int c, int K, uint16_t* stage, const float (&v)[16]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_halves<BF16>(v[2 * i], v[2 * i + 1]);
+  const uint4 a = make_uint4(w[0], w[1], w[2], w[3]), b = make_uint4(w[4], w[5], w[6], w[7]);
   if constexpr (VEC) {
-    if (c0 >= K) return;
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack_halves<BF16>(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4*>(row + c0) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(row + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    if (c * 16 < K) {
+      *reinterpret_cast<uint4*>(row + c * 16) = a;
+      *reinterpret_cast<uint4*>(row + c * 16 + 8) = b;
+    }
   } else {
+    const int lane = threadIdx.x & 31, base = (c - lane) * 16, n = K - base;
+    *reinterpret_cast<uint4*>(stage + lane * 16) = a;
+    *reinterpret_cast<uint4*>(stage + lane * 16 + 8) = b;
+    __syncwarp();
+    uint16_t* dst = row + base;
+    if ((reinterpret_cast<uintptr_t>(row) & 3) == 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (c0 + i < K) row[c0 + i] = f32_to_half_bits<BF16>(v[i]);
+      for (int j = 0; j < 8; ++j) {
+        const int at = j * 64 + lane * 2;
+        if (at + 1 < n) *reinterpret_cast<uint32_t*>(dst + at) = reinterpret_cast<const uint32_t*>(stage)[j * 32 + lane];
+        else if (at < n) dst[at] = stage[at];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j * 32 + lane < n) dst[j * 32 + lane] = stage[j * 32 + lane];
+    }
+    __syncwarp();
+  }
+}
+// 16 int8 codes of chunk c (w: four to a word) into a row of K bytes
+template <bool VEC>
+__device__ __forceinline__ void store16_bytes(uint8_t* row, int c, int K, uint8_t* stage, const uint32_t (&w)[4]) {
+  if constexpr (VEC) {
+    if (c * 16 < K) *reinterpret_cast<uint4*>(row + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    const int lane = threadIdx.x & 31, base = (c - lane) * 16, n = K - base;
+    *reinterpret_cast<uint4*>(stage + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j * 32 + lane < n) row[base + j * 32 + lane] = stage[j * 32 + lane];
+    __syncwarp();
   }
 }
 
@@ -103,28 +142,31 @@ __device__ __forceinline__ void store16(uint16_t* row, int c0, int K, const floa
 template <int FORMAT, bool BF16, bool NORM, bool VEC, bool BLOCK, int CH>
 __global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
   __shared__ uint32_t red[2][32];
+  __shared__ __align__(16) uint16_t stages[VEC ? 1 : 16][VEC ? 8 : 512];
   chain_wait();
   chain_next();  // behind the wait: a product that follows may read its weight before it waits
-  const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & 31);
+  const int lane = threadIdx.x & 31;
+  const int t = BLOCK ? (int)threadIdx.x : lane;
   const int step = BLOCK ? (int)blockDim.x : 32;
   const int64_t row = BLOCK ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (row >= a.rows) return;  // whole warps of a warp-per-row block
+  uint16_t* stage = stages[VEC ? 0 : threadIdx.x >> 5];
   float v[CH][16];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) load16<BF16, VEC>(a.x + row * a.x_stride, (t + i * step) * 16, a.K, v[i]);
+  for (int i = 0; i < CH; ++i) load16<BF16, VEC>(a.x + row * a.x_stride, t + i * step, a.K, stage, v[i]);
 
   if constexpr (NORM) {
     if (a.res) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         float r[16];
-        load16<BF16, VEC>(a.res + row * a.res_stride, (t + i * step) * 16, a.K, r);
+        load16<BF16, VEC>(a.res + row * a.res_stride, t + i * step, a.K, stage, r);
 #pragma unroll
         // the sum as it is stored: what a later layer reads is what is normed here
         for (int j = 0; j < 16; ++j) v[i][j] = half_to_f32<BF16>(f32_to_half_bits<BF16>(__fadd_rn(v[i][j], r[j])));
       }
 #pragma unroll
-      for (int i = 0; i < CH; ++i) store16<BF16, VEC>(a.sum + row * a.sum_stride, (t + i * step) * 16, a.K, v[i]);
+      for (int i = 0; i < CH; ++i) store16<BF16, VEC>(a.sum + row * a.sum_stride, t + i * step, a.K, stage, v[i]);
     }
     float ss = 0.0f;
 #pragma unroll
@@ -135,25 +177,21 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
     const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.K), a.eps)));
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
+      const int c = t + i * step;
       float w[16];
-      load16<BF16, VEC>(a.norm_w, (t + i * step) * 16, a.K, w);
+      load16<BF16, VEC>(a.norm_w, c, a.K, stage, w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[i][j] = __fmul_rn(__fmul_rn(v[i][j], inv), w[j]);
+      for (int j = 0; j < 16; ++j) {
+        v[i][j] = __fmul_rn(__fmul_rn(v[i][j], inv), w[j]);
+        if (!(VEC ? c * 16 < a.K : c * 16 + j < a.K)) v[i][j] = 0.0f;  // beyond K inv may have made a zero NaN
+      }
     }
-    // beyond K: zeros times inv (finite or NaN) times a weight of zero
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if ((t + i * step) * 16 + j >= a.K) v[i][j] = 0.0f;
   }
 
   uint32_t top[CH];  // absmax bits of each block (of 16 columns for int8)
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    top[i] = 0u;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) top[i] = max(top[i], __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+    top[i] = absmax16(v[i]);
     if (FORMAT == kMxfp4) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
   }
 
@@ -166,103 +204,76 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
     if (t == 0) a.row_scales[row] = scale;
     const bool some = m < kInfBits && scale >= FLT_MIN;  // a row below that is zeros
     const float rs = some ? __fdiv_rn(1.0f, scale) : 0.0f;
-    uint8_t* dst = a.codes + row * (int64_t)a.K;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c0 = (t + i * step) * 16;
       uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float q = some ? div_rn_by(v[i][j], scale, rs) : 0.0f;  // at most 127 and an fp32 rounding
         w[j >> 2] |= ((uint32_t)__float2int_rn(q) & 0xffu) << (8 * (j & 3));
       }
-      if constexpr (VEC) {
-        if (c0 < a.K) *reinterpret_cast<uint4*>(dst + c0) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + j < a.K) dst[c0 + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-      }
+      store16_bytes<VEC>(a.codes + row * (int64_t)a.K, t + i * step, a.K, reinterpret_cast<uint8_t*>(stage), w);
     }
-    return;
-  }
-
-  const int64_t pitch = fp4_pitch(a.K);
-  const int groups = (int)fp4_groups(a.K, FORMAT);
-  uint8_t* dst = a.codes + row * pitch;
-  uint8_t* word0 = a.blocks + (row >> 7) * groups * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
-  float inv_r = 1.0f;
-  if constexpr (FORMAT == kNvfp4) {
-    uint32_t m = 0u;
+  } else {
+    const int64_t pitch = fp4_pitch(a.K);
+    const int groups = (int)fp4_groups(a.K, FORMAT);
+    uint8_t* dst = a.codes + row * pitch;
+    uint8_t* word0 = a.blocks + (row >> 7) * groups * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+    float inv_r = 1.0f;
+    if constexpr (FORMAT == kNvfp4) {
+      uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) m = max(m, top[i] < kInfBits ? top[i] : 0u);
-    m = row_max<BLOCK>(m, red[1]);
-    // least e with absmax <= 2688 * 2^e = 1.3125 * 2^(11 + e), at least -126
-    const int e = m ? max((int)(m >> 23) - 138 + ((m & 0x7FFFFFu) > 0x280000u ? 1 : 0), -126) : 0;
-    inv_r = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (t == 0) a.row_scales[row] = __uint_as_float((uint32_t)(127 + e) << 23);
-  }
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const int c = t + i * step;
-    const bool bad = top[i] >= kInfBits;
-    uint32_t byte, w[2] = {0u, 0u};
-    if constexpr (FORMAT == kMxfp4) {
-      byte = bad ? 255u : (uint32_t)max((int)(top[i] >> 23) - 2, 0);
-      const float inv = __uint_as_float((254u - byte) << 23);
-#pragma unroll
-      for (int j = 0; j < 16; j += 2)
-        w[j >> 3] |= e2m1x2(__fmul_rn(v[i][j], inv), __fmul_rn(v[i][j + 1], inv)) << (4 * (j & 7));
-    } else {
-      byte = bad ? 0x7Fu : (uint32_t)f32x2_to_e4m3x2(__fdiv_rn(__fmul_rn(__uint_as_float(top[i]), inv_r), 6.0f), 0.0f) & 0xffu;
-      const float s = e4m3_to_f32(byte);
-      const float rs = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;  // under a scale of zero: zeros, with their signs
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        // the remainder of -0 is 0 and would make the quotient 0: the sign is x's
-        const float q0 = copysignf(div_rn_by(__fmul_rn(v[i][j], inv_r), s, rs), v[i][j]);
-        const float q1 = copysignf(div_rn_by(__fmul_rn(v[i][j + 1], inv_r), s, rs), v[i][j + 1]);
-        w[j >> 3] |= e2m1x2(q0, q1) << (4 * (j & 7));
-      }
+      for (int i = 0; i < CH; ++i) m = max(m, top[i] < kInfBits ? top[i] : 0u);
+      const int e = row_exponent(row_max<BLOCK>(m, red[1]));
+      inv_r = exp2_bits(-e);
+      if (t == 0) a.row_scales[row] = exp2_bits(e);
     }
-    if (bad) w[0] = w[1] = 0u;
-    if (c * 8 < pitch) *reinterpret_cast<uint2*>(dst + c * 8) = make_uint2(w[0], w[1]);
-    // four blocks' scales to a word: those of four lanes, or of four pairs
-    constexpr int kLanes = FORMAT == kMxfp4 ? 8 : 4, kPer = kLanes / 4;
-    uint32_t word = byte << (8 * ((t / kPer) & 3));
 #pragma unroll
-    for (int o = kPer; o < kLanes; o *= 2) word |= __shfl_xor_sync(0xffffffffu, word, o);
-    if ((t & (kLanes - 1)) == 0 && c / kLanes < groups)
-      *reinterpret_cast<uint32_t*>(word0 + (int64_t)(c / kLanes) * 512) = word;
+    for (int i = 0; i < CH; ++i) {
+      const int c = t + i * step;
+      uint32_t w[2];
+      const uint32_t byte = quantize16<FORMAT>(v[i], top[i], inv_r, w);
+      if (c * 8 < pitch) *reinterpret_cast<uint2*>(dst + c * 8) = make_uint2(w[0], w[1]);
+      const uint32_t word = ScaleWord<FORMAT>::of(byte, lane);
+      constexpr int kLanes = ScaleWord<FORMAT>::kLanes;
+      if ((lane & (kLanes - 1)) == 0 && c / kLanes < groups)
+        *reinterpret_cast<uint32_t*>(word0 + (int64_t)(c / kLanes) * 512) = word;
+    }
   }
 }
 
-// Codes and scales to 16-bit values: a thread takes 16 columns.  value = code * block scale * row scale
+// Codes and scales to 16-bit values: a warp takes 512 columns of a row, a thread 16.
+// value = code * block scale * row scale
 template <int FORMAT, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint16_t* out, int64_t out_stride,
-                                                             int chunks, int64_t total) {
+                                                             uint32_t parts, int64_t total) {
+  __shared__ __align__(16) uint16_t stages[VEC ? 1 : 8][VEC ? 8 : 512];
   chain_wait();
   chain_next();
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (at >= total) return;
-  const int64_t row = at / chunks;
-  const int c = (int)(at - row * chunks);
-  const uint2 q = *reinterpret_cast<const uint2*>(a.codes + row * fp4_pitch(a.K) + c * 8);
-  const int b = c * 16 / fp4_block(FORMAT);
-  const uint32_t byte = a.blocks[((row >> 7) * fp4_groups(a.K, FORMAT) + (b >> 2)) * 512 + (row & 31) * 16 +
-                                 ((row >> 5) & 3) * 4 + (b & 3)];
-  const float s = FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte);
-  const float r = a.row_scales ? a.row_scales[row] : 1.0f;
-  float v[16];
+  const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)at / parts) : at / parts;
+  const int c = (int)(at - row * parts) * 32 + lane;
+  const bool live = c * 16 < a.K;
+  float v[16] = {};
+  if (live) {
+    const uint2 q = *reinterpret_cast<const uint2*>(a.codes + row * fp4_pitch(a.K) + c * 8);
+    const int b = c * 16 / fp4_block(FORMAT);
+    const uint32_t byte = a.blocks[((row >> 7) * fp4_groups(a.K, FORMAT) + (b >> 2)) * 512 + (row & 31) * 16 +
+                                   ((row >> 5) & 3) * 4 + (b & 3)];
+    const float s = FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte);
+    const float r = a.row_scales ? a.row_scales[row] : 1.0f;
 #pragma unroll
-  for (int j = 0; j < 16; j += 2) {
-    const uint32_t pair = ((j < 8 ? q.x : q.y) >> (4 * (j & 7))) & 0xffu;
-    uint32_t h2;
-    asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h2) : "r"(pair));
-    v[j] = __fmul_rn(__fmul_rn(__half2float(__ushort_as_half((uint16_t)(h2 & 0xffffu))), s), r);
-    v[j + 1] = __fmul_rn(__fmul_rn(__half2float(__ushort_as_half((uint16_t)(h2 >> 16))), s), r);
+    for (int j = 0; j < 16; j += 2) {
+      const uint32_t pair = ((j < 8 ? q.x : q.y) >> (4 * (j & 7))) & 0xffu;
+      uint32_t h2;
+      asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h2) : "r"(pair));
+      v[j] = __fmul_rn(__fmul_rn(__half2float(__ushort_as_half((uint16_t)(h2 & 0xffffu))), s), r);
+      v[j + 1] = __fmul_rn(__fmul_rn(__half2float(__ushort_as_half((uint16_t)(h2 >> 16))), s), r);
+    }
   }
-  store16<BF16, VEC>(out + row * out_stride, c * 16, a.K, v);
+  store16<BF16, VEC>(out + row * out_stride, c, a.K, stages[VEC ? 0 : threadIdx.x >> 5], v);
 }
 
 // ------------------------------------------------------------------ host side
@@ -304,14 +315,14 @@ cudaError_t launch_fp4_rows(const Fp4RowArgs& a, int format, bool bf16, cudaStre
 
 template <int FORMAT>
 static cudaError_t launch_dequantize(const Fp4RowsView& a, uint16_t* out, int64_t stride, bool bf16, cudaStream_t s) {
-  const int chunks = (a.K + 15) / 16;
-  const int64_t total = a.rows * chunks, grid = (total + 255) / 256;
+  const uint32_t parts = (uint32_t)((a.K + 511) / 512);
+  const int64_t total = a.rows * parts, grid = (total + 7) / 8;
   const bool vec = a.K % 16 == 0 && rows16(out, stride);
   if (bf16)
-    return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, true, true>, grid, 256, 0, s, a, out, stride, chunks, total)
-               : launch_chained(fp4_dequantize_kernel<FORMAT, true, false>, grid, 256, 0, s, a, out, stride, chunks, total);
-  return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, false, true>, grid, 256, 0, s, a, out, stride, chunks, total)
-             : launch_chained(fp4_dequantize_kernel<FORMAT, false, false>, grid, 256, 0, s, a, out, stride, chunks, total);
+    return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, true, true>, grid, 256, 0, s, a, out, stride, parts, total)
+               : launch_chained(fp4_dequantize_kernel<FORMAT, true, false>, grid, 256, 0, s, a, out, stride, parts, total);
+  return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, false, true>, grid, 256, 0, s, a, out, stride, parts, total)
+             : launch_chained(fp4_dequantize_kernel<FORMAT, false, false>, grid, 256, 0, s, a, out, stride, parts, total);
 }
 cudaError_t launch_fp4_dequantize(const Fp4RowsView& a, int format, uint16_t* out, int64_t out_stride, bool bf16,
                                   cudaStream_t s) {

@@ -151,7 +151,7 @@ _SIGNATURES = {
     "h3b_fp4_quantize": [c_void_p, c_int, c_int64, _fp4_p, c_void_p],
     "h3b_fp4_dequantize": [_fp4_p, c_void_p, c_int, c_int64, c_void_p],
     "h3b_fp4_gemm": [_fp4_p, _fp4_p, c_void_p, c_void_p, c_int, c_int64, c_void_p],
-    "h3b_fp4_linear_workspace_bytes": [c_int64, c_int64, c_int],
+    "h3b_fp4_linear_workspace_bytes": [c_int64, _fp4_p],
     "h3b_fp4_linear": [c_void_p, c_int, c_int64, c_int64, _fp4_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
                        c_void_p],
     "h3b_add_rms_norm_int8": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64,

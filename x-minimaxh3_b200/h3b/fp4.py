@@ -25,7 +25,7 @@ same codes everywhere.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+import math
 
 import torch
 
@@ -36,6 +36,7 @@ FORMATS = {"mxfp4": 1, "nvfp4": 2}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 MAX_ROW = 32768  # columns of a row that is quantised here
 _DTYPES = {torch.float16: 1, torch.bfloat16: 2}
+_FLOAT_MAX = torch.finfo(torch.float32).max
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
@@ -46,61 +47,97 @@ def _format(name: str) -> int:
         raise ValueError(f"unknown 4-bit format {name!r} (expected one of {sorted(FORMATS)})") from None
 
 
-@dataclass
+def _scale_tiles(rows: int, cols: int, format: str) -> tuple[int, int]:
+    group = 4 * BLOCK[format]
+    return (rows + 127) // 128, (cols + group - 1) // group
+
+
 class Fp4Rows:
-    """Rows of 4-bit floats (h3b_fp4_rows).  The tensors must not be replaced by others.
+    """Rows of 4-bit floats (h3b_fp4_rows).
 
-    codes: two columns to a byte, the even one in the low nibble; rows end at a multiple of 32 columns.
-    scales: block scales in tiles of 128 rows x 4 blocks, the order in which the products read them
-    (`from_blocks` and `blocks` convert from and to [rows, blocks])."""
+    codes: uint8 [rows, ceil(cols / 32) * 16], two columns to a byte, the even one in the low nibble.
+    scales: uint8 [ceil(rows / 128), ceil(cols / (4 * block)), 512], block scales in tiles of 128 rows x 4
+    blocks, the order in which the products read them (`from_blocks` and `blocks` convert from and to
+    [rows, blocks]).  row_scales: f32 [rows], or None for 1."""
 
-    codes: torch.Tensor              # uint8 [rows, ceil(cols / 32) * 16]
-    scales: torch.Tensor             # uint8 [ceil(rows / 128), ceil(cols / (4 * block)), 512]
-    cols: int
-    format: str
-    row_scales: torch.Tensor | None = None  # f32 [rows]; None: 1
+    __slots__ = ("rows", "cols", "format", "_gpu", "_ref", "_buffer", "_codes", "_scales", "_row_scales")
 
-    def __post_init__(self) -> None:
-        codes, scales, row_scales = self.codes, self.scales, self.row_scales
-        code = _format(self.format)
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int, format: str,
+                 row_scales: torch.Tensor | None = None) -> None:
+        code = _format(format)
         if not codes.is_cuda:
             raise RuntimeError("Fp4Rows takes only CUDA tensors (the B200 library has no CPU path)")
-        self._gpu = gpu = codes.get_device()
-        if codes.ndim != 2 or self.cols < 1:
+        gpu = codes.get_device()
+        if codes.ndim != 2 or cols < 1:
             raise ValueError("codes must be [rows, bytes] of at least one column")
         rows = codes.shape[0]
-        group = 4 * BLOCK[self.format]
-        if codes.shape[1] != (self.cols + 31) // 32 * 16:
-            raise ValueError(f"{self.cols} columns take {(self.cols + 31) // 32 * 16} bytes of codes per row")
-        if scales.shape != ((rows + 127) // 128, (self.cols + group - 1) // group, 512):
+        if codes.shape[1] != (cols + 31) // 32 * 16:
+            raise ValueError(f"{cols} columns take {(cols + 31) // 32 * 16} bytes of codes per row")
+        if scales.shape != (*_scale_tiles(rows, cols, format), 512):
             raise ValueError("scales must be [ceil(rows / 128), ceil(cols / (4 * block)), 512]")
         if not codes.dtype is scales.dtype is torch.uint8 or not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("codes and scales must be contiguous uint8")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise ValueError("codes and scales must be 16-byte aligned")
         if row_scales is not None and (row_scales.dtype is not torch.float32 or row_scales.shape != (rows,)
                                        or not row_scales.is_contiguous() or row_scales.get_device() != gpu):
             raise ValueError("row_scales must be a contiguous float32 vector with an entry for each row, on the codes' GPU")
         if scales.get_device() != gpu:
             raise ValueError("codes and scales must be on one GPU")
-        self._ref = ctypes.byref(Fp4RowsStruct(codes.data_ptr(), scales.data_ptr(), _ptr(row_scales), rows, self.cols,
-                                               code))
+        self.rows, self.cols, self.format, self._gpu = rows, cols, format, gpu
+        self._buffer, self._codes, self._scales, self._row_scales = None, codes, scales, row_scales
+        self._ref = ctypes.byref(Fp4RowsStruct(codes.data_ptr(), scales.data_ptr(), _ptr(row_scales), rows, cols, code))
+
+    @classmethod
+    def _room(cls, rows: int, cols: int, format: str, like: torch.Tensor) -> Fp4Rows:
+        """Room for rows that a kernel writes, in one buffer on `like`'s GPU: a decoded token's calls are short
+        enough for each tensor's making to count, so the parts become tensors where they are asked for."""
+        self = object.__new__(cls)
+        code = FORMATS[format]
+        bands, groups = _scale_tiles(rows, cols, format)
+        size = rows * ((cols + 31) // 32 * 16)
+        end = size + bands * groups * 512
+        self._buffer = buffer = like.new_empty(end + (4 * rows if code == 2 else 0), dtype=torch.uint8)
+        at = buffer.data_ptr()
+        self.rows, self.cols, self.format, self._gpu = rows, cols, format, like.get_device()
+        self._codes = self._scales = self._row_scales = None
+        self._ref = ctypes.byref(Fp4RowsStruct(at, at + size, at + end if code == 2 else None, rows, cols, code))
+        return self
+
+    def _parts(self) -> None:
+        bands, groups = _scale_tiles(self.rows, self.cols, self.format)
+        pitch = (self.cols + 31) // 32 * 16
+        size = self.rows * pitch
+        end = size + bands * groups * 512
+        self._codes = self._buffer[:size].view(self.rows, pitch)
+        self._scales = self._buffer[size:end].view(bands, groups, 512)
+        if self.format == "nvfp4":
+            self._row_scales = self._buffer[end:].view(torch.float32)
 
     @property
-    def rows(self) -> int:
-        return self.codes.shape[0]
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._parts()
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._codes is None:
+            self._parts()
+        return self._scales
+
+    @property
+    def row_scales(self) -> torch.Tensor | None:
+        if self._codes is None:
+            self._parts()
+        return self._row_scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._buffer is None else self._buffer).device
 
-    @classmethod
-    def empty(cls, rows: int, cols: int, format: str, device="cuda", row_scales: bool | None = None) -> Fp4Rows:
-        """Room for rows; with row scales by default where the format has them."""
-        _format(format)
-        group = 4 * BLOCK[format]
-        codes = torch.empty((rows, (cols + 31) // 32 * 16), device=device, dtype=torch.uint8)
-        scales = torch.empty(((rows + 127) // 128, (cols + group - 1) // group, 512), device=device, dtype=torch.uint8)
-        with_rows = format == "nvfp4" if row_scales is None else row_scales
-        return cls(codes, scales, cols, format, torch.empty(rows, device=device, dtype=torch.float32) if with_rows else None)
+    def _new(self, shape: tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
+        return (self._codes if self._buffer is None else self._buffer).new_empty(shape, dtype=dtype)
 
     @classmethod
     def from_blocks(cls, codes: torch.Tensor, block_scales: torch.Tensor, format: str,
@@ -133,29 +170,32 @@ def _half_rows(x: torch.Tensor, what: str) -> torch.Tensor:
     """[..., K] as fp16 / bf16 rows [M, K] of unit column stride; copied where they do not lie so."""
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} must be bfloat16 or float16")
-    if x.ndim == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError(f"{what} must have at least one column")
-    if x.ndim != 2:
-        x = x.reshape(x.numel() // x.shape[-1], x.shape[-1])
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    if len(shape) != 2:
+        x = x.reshape(math.prod(shape[:-1]), shape[-1])
+    if not x.is_contiguous() and (x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()
     return x
 
 
 def _row_step(x: torch.Tensor) -> int:
     """Elements between x's rows (of a single row, whose stride may be anything, its length)."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    rows, cols = x.shape
+    return x.stride(0) if rows > 1 else cols
 
 
-def _cuda(name: str, *tensors: torch.Tensor | None) -> int:
+def _gpu_of(x: torch.Tensor, name: str) -> int:
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} runs only on CUDA tensors (the B200 library has no CPU path)")
+    return x.get_device()
+
+
+def _on(gpu: int, *tensors: torch.Tensor | None) -> None:
     for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise RuntimeError(f"{name} runs only on CUDA tensors (the B200 library has no CPU path)")
-    gpu = tensors[0].get_device()
-    for t in tensors[1:]:
         if t is not None and t.get_device() != gpu:
             raise ValueError("all tensors must be on one GPU")
-    return gpu
 
 
 def _row_length(cols: int) -> None:
@@ -165,32 +205,35 @@ def _row_length(cols: int) -> None:
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4") -> Fp4Rows:
     """Rows x [..., K] (bf16 or fp16) to 4-bit floats [M, K]."""
-    gpu = _cuda("quantize_fp4", x)
+    gpu = _gpu_of(x, "quantize_fp4")
     _format(format)
     x = _half_rows(x, "x")
-    _row_length(x.shape[1])
-    out = Fp4Rows.empty(x.shape[0], x.shape[1], format, x.device)
-    check(lib().h3b_fp4_quantize(_ptr(x), _DTYPES[x.dtype], _row_step(x), out._ref, _stream(gpu)), "fp4_quantize")
+    m, k = x.shape
+    _row_length(k)
+    out = Fp4Rows._room(m, k, format, x)
+    check(lib().h3b_fp4_quantize(x.data_ptr(), _DTYPES[x.dtype], _row_step(x), out._ref, _stream(gpu)), "fp4_quantize")
     return out
 
 
-def _rows_out(out: torch.Tensor | None, like: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
-    if out is None:
-        return torch.empty((rows, cols), device=like.device, dtype=dtype)
-    if out.shape != (rows, cols) or out.dtype is not dtype or out.get_device() != like.get_device():
+def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, gpu: int) -> int:
+    """The step between the rows of a caller's output."""
+    if out.shape != (rows, cols) or out.dtype is not dtype or out.get_device() != gpu:
         raise ValueError(f"out must be {dtype} [{rows}, {cols}] on the operands' GPU")
     if cols > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < cols:
         raise ValueError("out must have unit column stride and rows apart from each other")
-    return out
+    return _row_step(out)
 
 
 def dequantize_fp4(rows: Fp4Rows, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values that 4-bit rows stand for, [M, K]."""
     if dtype not in _DTYPES:
         raise ValueError("dequantize_fp4 writes bfloat16 or float16")
-    out = _rows_out(out, rows.codes, rows.rows, rows.cols, dtype)
-    check(lib().h3b_fp4_dequantize(rows._ref, _ptr(out), _DTYPES[dtype], _row_step(out), _stream(rows._gpu)),
-          "fp4_dequantize")
+    step = rows.cols
+    if out is None:
+        out = rows._new((rows.rows, rows.cols), dtype)
+    else:
+        step = _check_out(out, rows.rows, rows.cols, dtype, rows._gpu)
+    check(lib().h3b_fp4_dequantize(rows._ref, out.data_ptr(), _DTYPES[dtype], step, _stream(rows._gpu)), "fp4_dequantize")
     return out
 
 
@@ -199,8 +242,9 @@ def _bias(bias: torch.Tensor | None, n: int, gpu: int) -> torch.Tensor | None:
         return None
     if bias.numel() != n:
         raise ValueError("bias does not match the weight's output rows")
-    if bias.get_device() != gpu:
-        raise ValueError("all tensors must be on one GPU")
+    _on(gpu, bias)
+    if bias.dtype is torch.float32 and bias.is_contiguous():
+        return bias
     return bias.to(torch.float32).reshape(-1).contiguous()
 
 
@@ -216,10 +260,14 @@ def fp4_linear_prequantized(xq: Fp4Rows, weight: Fp4Rows, bias: torch.Tensor | N
         raise ValueError(f"Input and weight inner dimensions must match, got {xq.cols} and {weight.cols}")
     if out_dtype not in _DTYPES:
         raise ValueError("fp4_linear writes bfloat16 or float16")
-    bias = _bias(bias, weight.rows, gpu)
-    out = _rows_out(out, xq.codes, xq.rows, weight.rows, out_dtype)
-    check(lib().h3b_fp4_gemm(xq._ref, weight._ref, _ptr(bias), _ptr(out), _DTYPES[out_dtype], _row_step(out),
-                             _stream(gpu)), "fp4_gemm")
+    step = n = weight.rows
+    bias = _bias(bias, n, gpu)
+    if out is None:
+        out = xq._new((xq.rows, n), out_dtype)
+    else:
+        step = _check_out(out, xq.rows, n, out_dtype, gpu)
+    check(lib().h3b_fp4_gemm(xq._ref, weight._ref, _ptr(bias), out.data_ptr(), _DTYPES[out_dtype], step, _stream(gpu)),
+          "fp4_gemm")
     return out
 
 
@@ -228,28 +276,34 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
     """x [..., K] (bf16 or fp16), quantised to the weight's format, times weight [N, K]^T, + bias -> x's type [..., N].
 
     out: rows [M, N] that receive the result.  workspace: uint8, reused by calls on one stream."""
-    gpu = _cuda("fp4_linear", x)
+    gpu = _gpu_of(x, "fp4_linear")
     if weight._gpu != gpu:
         raise ValueError("all tensors must be on one GPU")
-    if x.ndim == 0 or x.shape[-1] != weight.cols:
-        raise ValueError(f"Input and weight inner dimensions must match, got {x.shape[-1] if x.ndim else 0} and "
-                         f"{weight.cols}")
-    lead = x.shape[:-1]
+    shape, k, n = x.shape, weight.cols, weight.rows
+    if not shape or shape[-1] != k:
+        raise ValueError(f"Input and weight inner dimensions must match, got {shape[-1] if shape else 0} and {k}")
     x = _half_rows(x, "x")
-    _row_length(weight.cols)
-    m = x.shape[0]
-    bias = _bias(bias, weight.rows, gpu)
+    _row_length(k)
+    m, step = x.shape[0], n
+    bias = _bias(bias, n, gpu)
     given = out is not None
-    out = _rows_out(out, x, m, weight.rows, x.dtype)
-    need = lib().h3b_fp4_linear_workspace_bytes(m, weight.cols, FORMATS[weight.format])
-    if workspace is None:
-        workspace = torch.empty(need, device=x.device, dtype=torch.uint8)
-    elif (workspace.numel() * workspace.element_size() < need or workspace.get_device() != gpu
-          or not workspace.is_contiguous() or workspace.data_ptr() % 16):
-        raise ValueError(f"the workspace must have {need} contiguous, 16-byte aligned bytes on the operands' GPU")
-    check(lib().h3b_fp4_linear(_ptr(x), _DTYPES[x.dtype], m, _row_step(x), weight._ref, _ptr(bias), _ptr(out),
-                               _row_step(out), _ptr(workspace), need, _stream(gpu)), "fp4_linear")
-    return out if given or len(lead) == 1 else out.view(*lead, weight.rows)
+    if given:
+        step = _check_out(out, m, n, x.dtype, gpu)
+    else:
+        out = x.new_empty((m, n))
+    library = lib()
+    need = library.h3b_fp4_linear_workspace_bytes(m, weight._ref)
+    at = None
+    if need:
+        if workspace is None:
+            workspace = x.new_empty(need, dtype=torch.uint8)
+        elif (workspace.numel() * workspace.element_size() < need or workspace.get_device() != gpu
+              or not workspace.is_contiguous() or workspace.data_ptr() % 16):
+            raise ValueError(f"the workspace must have {need} contiguous, 16-byte aligned bytes on the operands' GPU")
+        at = workspace.data_ptr()
+    check(library.h3b_fp4_linear(x.data_ptr(), _DTYPES[x.dtype], m, _row_step(x), weight._ref, _ptr(bias),
+                                 out.data_ptr(), step, at, need, _stream(gpu)), "fp4_linear")
+    return out if given or len(shape) == 2 else out.view(*shape[:-1], n)
 
 
 def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *, eps: float = 1e-5,
@@ -260,43 +314,45 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
     themselves may, and no other tensor that overlaps them).  Without a residual h is x, and nothing is
     written to it.  to "int8": (codes int8 [M, K], scales f32 [M, 1] = absmax / 127), as
     ops.int8_linear_prequantized takes them; "mxfp4" or "nvfp4": Fp4Rows, as fp4_linear_prequantized does."""
-    gpu = _cuda("add_rms_norm_quantize", x, residual, weight, out)
-    if to != "int8":
+    gpu = _gpu_of(x, "add_rms_norm_quantize")
+    int8 = to == "int8"
+    if not int8:
         _format(to)
-    shape = x.shape
-    if weight.dtype is not x.dtype or weight.ndim != 1 or x.ndim == 0 or weight.shape[0] != shape[-1]:
+    shape, dtype = x.shape, x.dtype
+    if weight.dtype is not dtype or not shape or weight.shape != shape[-1:]:
         raise ValueError("weight must be a vector of x's type with an entry for each column")
-    if not 0.0 <= eps <= torch.finfo(torch.float32).max:
+    if not 0.0 <= eps <= _FLOAT_MAX:
         raise ValueError("eps must be finite and not negative")
     if residual is None and out is not None:
         raise ValueError("without a residual there is no sum to write")
+    _on(gpu, residual, weight, out)
     rows = _half_rows(x, "x")
     m, k = rows.shape
     _row_length(k)
-    weight = weight.contiguous()
-    res = None
-    h = x
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    h, res, res_step, sum_at, sum_step = x, None, 0, None, 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype is not x.dtype:
+        if residual.shape != shape or residual.dtype is not dtype:
             raise ValueError("residual must have x's shape and type")
         res = _half_rows(residual, "residual")
+        res_step = _row_step(res)
         if out is None:
-            out = torch.empty(shape, device=x.device, dtype=x.dtype)
-        elif out.shape != shape or out.dtype is not x.dtype:
-            raise ValueError("out must have x's shape and type")
-        h, out = out, out.view(m, k)  # refused by view() where the rows do not lie in one step
-        if k > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < k:
-            raise ValueError("out must have unit column stride and rows apart from each other")
-    args = (_ptr(rows), _row_step(rows), _ptr(res), 0 if res is None else _row_step(res), _ptr(out),
-            0 if out is None else _row_step(out), _ptr(weight), _DTYPES[x.dtype])
-    if to == "int8":
-        q = torch.empty((m, k), device=x.device, dtype=torch.int8)
-        scales = torch.empty((m, 1), device=x.device, dtype=torch.float32)
-        check(lib().h3b_add_rms_norm_int8(*args, m, k, float(eps), _ptr(q), _ptr(scales), _stream(gpu)),
+            h = x.new_empty(shape)
+            sum_at, sum_step = h.data_ptr(), k
+        else:
+            if out.shape != shape:
+                raise ValueError("out must have x's shape")
+            h = out
+            sum_at, sum_step = out.data_ptr(), _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
+    args = (rows.data_ptr(), _row_step(rows), _ptr(res), res_step, sum_at, sum_step, weight.data_ptr(), _DTYPES[dtype])
+    if int8:
+        q, scales = x.new_empty((m, k), dtype=torch.int8), x.new_empty((m, 1), dtype=torch.float32)
+        check(lib().h3b_add_rms_norm_int8(*args, m, k, eps, q.data_ptr(), scales.data_ptr(), _stream(gpu)),
               "add_rms_norm_int8")
         return h, (q, scales)
-    quantised = Fp4Rows.empty(m, k, to, x.device)
-    check(lib().h3b_add_rms_norm_fp4(*args, float(eps), quantised._ref, _stream(gpu)), "add_rms_norm_fp4")
+    quantised = Fp4Rows._room(m, k, to, x)
+    check(lib().h3b_add_rms_norm_fp4(*args, eps, quantised._ref, _stream(gpu)), "add_rms_norm_fp4")
     return h, quantised
 
 
