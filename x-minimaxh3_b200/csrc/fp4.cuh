@@ -76,6 +76,7 @@ struct Fp4GemmArgs {
   const uint16_t* x16;
   int64_t x16_stride;
   int x16_vec;  // they allow 16-byte accesses
+  int out_tma;  // set by the launcher: the output rows go out by TMA
 };
 // 0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err)
 int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, int format, cudaStream_t s,

@@ -15,6 +15,9 @@ namespace h3b {
 
 constexpr int kF4Step = 128;  // bytes of codes per row and K step
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // Shared-memory matrix descriptor without swizzle for a tile of block scales: 32 rows of 16
 // bytes, 8-row pieces of 128 bytes one after the other (SBO).
 __device__ __forceinline__ uint64_t sdesc_scales(uint32_t smem_addr) {
@@ -61,12 +64,9 @@ __device__ __forceinline__ float fp4_finish(float sum, float xs, float ws, float
   return a.bias ? __fadd_rn(v, bias) : v;
 }
 
-// One thread: the scale copies and products of one K step into accumulator d.  BANDS: 128-row
-// bands of scales of the B operand, whose first row's scales lie in column column_b of theirs.
-template <int FORMAT, int CTAS, int M, int N, int BANDS>
-__device__ __forceinline__ void fp4_step(uint32_t d, uint32_t smem_a, uint32_t smem_b, uint32_t smem_sa,
-                                         uint32_t smem_sb, uint32_t tmem_sa, uint32_t tmem_sb, uint32_t column_b,
-                                         int products, bool first) {
+// One thread: the scale copies of one K step.  BANDS: 128-row bands of scales of the B operand.
+template <int FORMAT, int CTAS, int BANDS>
+__device__ __forceinline__ void fp4_step_scales(uint32_t smem_sa, uint32_t smem_sb, uint32_t tmem_sa, uint32_t tmem_sb) {
   constexpr int kTiles = FORMAT == kMxfp4 ? 2 : 4;  // scale tiles per band and step
 #pragma unroll
   for (int g = 0; g < kTiles; ++g) {
@@ -76,24 +76,50 @@ __device__ __forceinline__ void fp4_step(uint32_t d, uint32_t smem_a, uint32_t s
       copy_scales<CTAS>(tmem_sb + (uint32_t)(4 * (BANDS * g + b)),
                         sdesc_scales(smem_sb + (uint32_t)(512 * (kTiles * b + g))));
   }
+}
+// One thread: the products of one K step into accumulator d; tmem_sb: the column of B's scales
+// in which those of its first row lie.
+template <int FORMAT, int CTAS, int M, int N, int BANDS>
+__device__ __forceinline__ void fp4_step_products(uint32_t d, uint32_t smem_a, uint32_t smem_b, uint32_t tmem_sa,
+                                                  uint32_t tmem_sb, int products, bool first) {
   const uint64_t da = sdesc_kmajor_sw128(smem_a), db = sdesc_kmajor_sw128(smem_b);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if (k >= products) break;
+    if (k > 0 && k >= products) break;
     const uint32_t byte = FORMAT == kMxfp4 ? 2u * (uint32_t)(k & 1) : 0u;
     const uint32_t g = FORMAT == kMxfp4 ? (uint32_t)(k >> 1) : (uint32_t)k;
     mma_fp4<FORMAT, CTAS>(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_fp4(M, N, FORMAT == kMxfp4, byte),
-                          tmem_sa + 4u * g, tmem_sb + 4u * BANDS * g + column_b, first && k == 0 ? 0u : 1u);
+                          tmem_sa + 4u * g, tmem_sb + 4u * BANDS * g, first && k == 0 ? 0u : 1u);
   }
 }
+// Non-blocking look at a barrier.  The warps that issue products look at the next step's barriers
+// before they issue this step's: a wait costs about 100 cycles even where it is over, and a step
+// of the 256 x 256 tiles has 512 in all.
+__device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// A place in a ring of n stages: the next fill's stage and the parity of its barrier
+struct RingPlace {
+  uint32_t stage = 0, parity = 0;
+  __device__ __forceinline__ void next(uint32_t n) {
+    if (++stage == n) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+};
 
 // ------------------------------------------------------------------ few rows: a split over K
 // A tile is 128 rows of the weight (the products' M) x TOK rows of x (their N), so that one
-// token costs the reading of the weight and hardly more.  The CTAs of a cluster take equal parts
-// of K; each puts its sums into its shared memory, and every CTA adds up and writes out a part
-// of the tile's tokens, from all CTAs in their order (the same sums every time).  Without a
-// split the sums go out as they come from tensor memory.  Two CTAs fit an SM.
-//   warp 0: TMA, warp 1: tensor memory and products, warps 2-5: sums; all: the joining
+// token costs the reading of the weight and hardly more.  The CTAs of a cluster (1, 2, 4 or 8)
+// take equal parts of K; each sends its sums to the CTAs that own their columns (equal shares of
+// the tile's 128), which add them in the CTAs' order (the same sums every time) and write them.
+// Without a split the sums go out as they come from tensor memory.
+//   warp 0: TMA, warp 1: tensor memory, scale copies and products, warps 2-5: sums
 // Behind the quantisation of x in the stream, the first weight tiles are on their way before
 // that has ended.  ROWS16: x is 16-bit, at most 16 rows, and warps 2-5 of each CTA quantise
 // its part of K themselves (for nvfp4 the cluster's CTAs tell each other their rows' absmax).
@@ -105,31 +131,51 @@ struct SplitCfg {
   static constexpr int kXBytes = TOK * kF4Step;
   static constexpr int kXStep = kXBytes + kScaleBytes;
   static constexpr int kStageBytes = kWBytes + kScaleBytes + (ROWS16 ? 0 : kXStep);
-  static constexpr int kStages = TOK == 128 ? 3 : 4;
-  static constexpr int kAccCols = TOK < 32 ? 32 : TOK;
-  static constexpr int kTmemCols = kAccCols + 64 <= 128 ? 128 : 256;  // and two slots of 16 + 16 columns of scales
   static_assert(kStageBytes % 1024 == 0 && kXStep % 1024 == 0, "swizzled tiles start at multiples of 1024");
-  static_assert(128 * TOK * 4 <= kStages * kStageBytes, "the sums take the stages' place");
-  static constexpr int smem_bytes(int steps) { return kStages * kStageBytes + (ROWS16 ? steps * kXStep : 0) + 1024; }
+  static constexpr int kAccCols = TOK < 32 ? 32 : TOK;
+  static constexpr int kSlotCols = kScaleBytes / 64;  // both operands' scales of a step: 16 or 32 columns
+  static constexpr int kSlots = 4;
+  static constexpr int kTmemCols = 256;
+  static_assert(kAccCols + kSlots * kSlotCols <= kTmemCols, "");
+  // what a CTA needs beside its stages
+  static constexpr int rest_bytes(int steps, int split) {
+    return (ROWS16 ? steps * kXStep : 0) + (split > 1 ? TOK * 512 : 0) + 1024;
+  }
 };
-constexpr int kSplitThreads = 192;
-constexpr int kRows16Steps = 8;  // K steps of a CTA that quantises x: what fits twice on an SM
+constexpr int kSplitThreads = 192, kSplitMaxStages = 8;
+constexpr int kRows16Steps = 8;  // K steps of a CTA that quantises x
+
+// bounded wait for an mbarrier whose arrivals release what other CTAs of the cluster wrote here
+__device__ __forceinline__ bool mbar_wait_sent(uint64_t* bar, volatile int* abort_flag) {
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t n = 0;; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)) : "memory");
+    if (ok) return true;
+    if (n >= kWaitMaxTries || (n > 64 && globaltimer_ns() - t0 > kWaitLimitNs)) {
+      *abort_flag = 1;
+      record_status(H3B_STATUS_GEMM_TIMEOUT);
+      return false;
+    }
+  }
+}
 
 template <int FORMAT, int TOK, bool ROWS16, bool BF16>
 __global__ void __launch_bounds__(kSplitThreads)
     fp4_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sw,
                      const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_sx,
-                     Fp4GemmArgs a, int split) {
+                     Fp4GemmArgs a, int split, int num_stages) {
   using C = SplitCfg<FORMAT, TOK, ROWS16>;
-  constexpr int kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kStages], empty[kStages], done, x_ready;
+  __shared__ uint64_t full[kSplitMaxStages], empty[kSplitMaxStages], done, x_ready, sent;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, late_flag;
   __shared__ uint32_t row_top[16];
   __shared__ float row_scale[16];
-  __shared__ __align__(16) uint16_t stages[ROWS16 ? 4 : 1][ROWS16 ? 512 : 8];
+  __shared__ __align__(16) uint16_t pieces[ROWS16 ? 4 : 1][ROWS16 ? 512 : 8];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
@@ -138,91 +184,121 @@ __global__ void __launch_bounds__(kSplitThreads)
   const int n0 = tile % num_n * 128, m0 = tile / num_n * TOK;
   const int num_k = (a.K + 255) / 256;
   const int kb0 = (int)((int64_t)num_k * rank / split), steps = (int)((int64_t)num_k * (rank + 1) / split) - kb0;
-  uint8_t* x_area = smem + kStages * C::kStageBytes;  // ROWS16: [steps] codes and scales
+  const uint32_t stages = (uint32_t)num_stages;
+  const int share = 128 / split;                     // columns of the tile that this CTA adds up
+  uint8_t* x_area = smem + stages * C::kStageBytes;  // ROWS16: [steps] codes and scales
+  // [split][TOK][share], at the same place in all CTAs of the cluster
+  float* sums = reinterpret_cast<float*>(x_area + (ROWS16 ? (num_k + split - 1) / split * C::kXStep : 0));
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  RingPlace fill;
+  int fills = 0;
+  auto load_w = [&]() {
+    uint8_t* at = smem + fill.stage * C::kStageBytes;
+    uint64_t* bar = &full[fill.stage];
+    mbar_arrive_expect_tx(bar, C::kStageBytes);
+    tma_load_2d(at, &tm_w, bar, (kb0 + fills) * kF4Step, n0);
+    tma_load_2d(at + C::kWBytes, &tm_sw, bar, (kb0 + fills) * (C::kScaleBytes / 8), n0 >> 7);
+  };
+  auto load_x = [&](int i, uint32_t stage) {
+    if constexpr (!ROWS16) {
+      uint8_t* at = smem + stage * C::kStageBytes + C::kWBytes + C::kScaleBytes;
+      tma_load_2d(at, &tm_x, &full[stage], (kb0 + i) * kF4Step, m0);
+      tma_load_2d(at + C::kXBytes, &tm_sx, &full[stage], (kb0 + i) * (C::kScaleBytes / 8), m0 >> 7);
     }
-    mbar_init(&done, 1);
-    mbar_init(&x_ready, 128);
-    abort_flag = late_flag = 0;
-    fence_mbar_init();
-  }
-  if (ROWS16 && threadIdx.x < 16) row_top[threadIdx.x] = 0u;
-  if (warp == 1) {
+  };
+  if (warp == 0) {
+    // the first loads start before tensor memory is there: nobody else looks at their barriers yet
+    if (lane == 0) {
+      for (uint32_t s = 0; s < stages; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(&done, 1);
+      mbar_init(&x_ready, 128);
+      mbar_init(&sent, (uint32_t)(128 / min(32, share)));
+      abort_flag = late_flag = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    if (!a.behind_rows) chain_wait();
+    const int ahead = min(steps, num_stages);
+    for (; fills < ahead; ++fills) {
+      if (elect_one()) load_w();
+      __syncwarp();
+      fill.next(stages);
+    }
+    if (a.behind_rows) chain_wait();
+    if (!ROWS16 && elect_one())
+      for (int i = 0; i < ahead; ++i) load_x(i, (uint32_t)i);
+    __syncwarp();
+  } else if (warp == 1) {
     tmem_alloc(&tmem_slot, C::kTmemCols);
     tmem_relinquish();
+  } else if (ROWS16 && threadIdx.x < 80) {
+    row_top[threadIdx.x - 64] = 0u;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   chain_next();
+  if (split > 1) cluster_arrive();  // and wait before anything of another CTA is touched
   const uint32_t tmem = tmem_slot;
 
   if (warp == 0) {
-    auto load_w = [&](int i) {
-      uint8_t* at = smem + i % kStages * C::kStageBytes;
-      mbar_arrive_expect_tx(&full[i % kStages], C::kStageBytes);
-      tma_load_2d(at, &tm_w, &full[i % kStages], (kb0 + i) * kF4Step, n0);
-      tma_load_2d(at + C::kWBytes, &tm_sw, &full[i % kStages], (kb0 + i) * (C::kScaleBytes / 8), n0 >> 7);
-    };
-    auto load_x = [&](int i) {
-      if constexpr (!ROWS16) {
-        uint8_t* at = smem + i % kStages * C::kStageBytes + C::kWBytes + C::kScaleBytes;
-        tma_load_2d(at, &tm_x, &full[i % kStages], (kb0 + i) * kF4Step, m0);
-        tma_load_2d(at + C::kXBytes, &tm_sx, &full[i % kStages], (kb0 + i) * (C::kScaleBytes / 8), m0 >> 7);
-      }
-    };
-    const int ahead = steps < kStages ? steps : kStages;
-    if (!a.behind_rows) chain_wait();
-    if (elect_one())
-      for (int i = 0; i < ahead; ++i) load_w(i);
-    __syncwarp();
-    if (a.behind_rows) chain_wait();
-    if (!ROWS16 && elect_one())
-      for (int i = 0; i < ahead; ++i) load_x(i);
-    __syncwarp();
-    if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
-    int fills = ahead;
+    if (split > 1) cluster_wait();
+    if (ROWS16 && FORMAT == kNvfp4 && split > 1) cluster_sync_all();
+    RingPlace freed;
     for (; fills < steps; ++fills) {
-      if (!mbar_wait_warp(&empty[fills % kStages], (fills / kStages - 1) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
+      if (!mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
+      freed.next(stages);
       if (elect_one()) {
-        load_w(fills);
-        load_x(fills);
+        load_w();
+        load_x(fills, fill.stage);
       }
       __syncwarp();
+      fill.next(stages);
     }
-    // every copy that was started has landed before the CTA may leave
-    for (int i = fills > kStages ? fills - kStages : 0; i < fills; ++i)
-      mbar_wait_warp(&full[i % kStages], (i / kStages) & 1, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
+    // every copy that was started has landed before the CTA may leave: of each slot the last fill
+    for (uint32_t s = 0; s < stages; ++s)
+      mbar_wait_warp(&full[s], s < fill.stage ? fill.parity : fill.parity ^ 1u, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
   } else if (warp == 1) {
     const uint32_t smem0 = smem_u32(smem), x0 = smem_u32(x_area);
-    if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
+    if (split > 1) cluster_wait();
+    if (ROWS16 && FORMAT == kNvfp4 && split > 1) cluster_sync_all();
     const bool ready = !ROWS16 || mbar_wait_warp(&x_ready, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
+    RingPlace at, freed;
+    // the slot of scales of step i: read by the products of step i - kSlots
+    auto wants_slot = [&](int i) { return i >= C::kSlots && num_stages > C::kSlots; };
+    auto peek = [&](int i) {
+      const bool slot = lane == 1 && wants_slot(i);
+      return mbar_peek(slot ? &empty[freed.stage] : &full[at.stage], slot ? freed.parity : at.parity);
+    };
+    bool seen = peek(0);
     for (int i = 0; ready && i < steps; ++i) {
-      if (!mbar_wait_warp(&full[i % kStages], (i / kStages) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
-      // the scale slot of this step: read by the products of the step before last
-      if (i >= 2 && !mbar_wait_warp(&empty[(i - 2) % kStages], ((i - 2) / kStages) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT))
+      if (!__all_sync(0xffffffffu, seen) &&
+          (!mbar_wait_warp(&full[at.stage], at.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
+           (wants_slot(i) && !mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT))))
         break;
       tc_fence_after();
+      const uint32_t w = smem0 + at.stage * C::kStageBytes;
+      const uint32_t x = ROWS16 ? x0 + (uint32_t)(i * C::kXStep) : w + C::kWBytes + C::kScaleBytes;
+      const uint32_t ts = tmem + C::kAccCols + (uint32_t)(C::kSlotCols * (i & (C::kSlots - 1)));
+      uint64_t* used = &empty[at.stage];
+      if (wants_slot(i)) freed.next(stages);
+      at.next(stages);
+      seen = peek(i + 1);
       if (elect_one()) {
-        const uint32_t at = smem0 + (uint32_t)(i % kStages * C::kStageBytes);
-        const uint32_t x = ROWS16 ? x0 + (uint32_t)(i * C::kXStep) : at + C::kWBytes + C::kScaleBytes;
-        const uint32_t ts = tmem + C::kAccCols + 32u * (uint32_t)(i & 1);
-        const int products = (a.K - (kb0 + i) * 256 + 63) / 64;
-        // rows m0 .. of their 128-row band: 32 to a column of the scales in tensor memory
-        fp4_step<FORMAT, 1, 128, TOK, 1>(tmem, at, x, at + C::kWBytes, x + C::kXBytes, ts, ts + 16,
-                                         (uint32_t)(m0 >> 5) & 3u, products, i == 0);
-        mma_commit(&empty[i % kStages]);
+        fp4_step_scales<FORMAT, 1, 1>(w + C::kWBytes, x + C::kXBytes, ts, ts + C::kSlotCols / 2);
+        // rows m0 .. of their 128-row band: 32 to a column of the scales
+        fp4_step_products<FORMAT, 1, 128, TOK, 1>(tmem, w, x, ts, ts + C::kSlotCols / 2 + ((uint32_t)(m0 >> 5) & 3u),
+                                                  (a.K - (kb0 + i) * 256 + 63) / 64, i == 0);
+        mma_commit(used);
       }
       __syncwarp();
     }
     if (elect_one()) mma_commit(&done);
     __syncwarp();
     mbar_wait_warp(&done, 0, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
-    chain_wait();
   } else {
     chain_wait();
     if constexpr (ROWS16) {
@@ -230,13 +306,13 @@ __global__ void __launch_bounds__(kSplitThreads)
       const uint16_t* x = a.x16 + kb0 * 256;
       const int K = a.K - kb0 * 256, segs = (steps + 1) / 2, items = a.M * segs;
       const bool vec = a.x16_vec;
-      uint16_t* stage = stages[warp - 2];
+      uint16_t* piece = pieces[warp - 2];
       float v[16];
       auto load = [&](int item) {
         const uint16_t* row = x + (int64_t)(item / segs) * a.x16_stride;
         const int c = item % segs * 32 + lane;
-        if (vec) load16<BF16, true>(row, c, K, stage, v);
-        else load16<BF16, false>(row, c, K, stage, v);
+        if (vec) load16<BF16, true>(row, c, K, piece, v);
+        else load16<BF16, false>(row, c, K, piece, v);
       };
       if constexpr (FORMAT == kNvfp4) {
         for (int item = warp - 2; item < items; item += 4) {
@@ -246,7 +322,12 @@ __global__ void __launch_bounds__(kSplitThreads)
           top = __reduce_max_sync(0xffffffffu, top);
           if (lane == 0) atomicMax(&row_top[item / segs], top);
         }
-        cluster_sync_all();
+        if (split > 1) {
+          cluster_wait();
+          cluster_sync_all();
+        } else {
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
       }
       for (int item = warp - 2; item < items; item += 4) {
         const int r = item / segs, c = item % segs * 32 + lane;
@@ -255,7 +336,8 @@ __global__ void __launch_bounds__(kSplitThreads)
         if constexpr (FORMAT == kNvfp4) {
           uint32_t top = 0u;
           if (lane < split)
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(top) : "r"(mapa_shared(smem_u32(&row_top[r]), (uint32_t)lane)));
+            asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                         : "=r"(top) : "r"(mapa_shared(smem_u32(&row_top[r]), (uint32_t)lane)) : "memory");
           const int e = row_exponent(__reduce_max_sync(0xffffffffu, top));
           inv_r = exp2_bits(-e);
           if (lane == 0) row_scale[r] = exp2_bits(e);
@@ -274,23 +356,23 @@ __global__ void __launch_bounds__(kSplitThreads)
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&x_ready);
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // row_scale is read by all four warps
     }
+    if (split > 1 && !(ROWS16 && FORMAT == kNvfp4)) cluster_wait();
     const int quad = warp & 3, row = quad * 32 + lane, toks = min(TOK, a.M - m0);
-    if (mbar_wait_warp(&done, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) {
-      tc_fence_after();
-      float* sums = reinterpret_cast<float*>(smem);  // [TOK][128]
+    const bool summed = mbar_wait_warp(&done, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
+    tc_fence_after();
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
+    if (split == 1) {
       const int n = n0 + row;
       const float ws = a.ws && n < a.N ? a.ws[n] : 1.0f, bias = a.bias && n < a.N ? a.bias[n] : 0.0f;
 #pragma unroll 1
-      for (int c = 0; c < toks; c += 16) {
+      for (int c = 0; summed && c < toks; c += 16) {
         uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, r);
+        tmem_ld16(taddr + (uint32_t)c, r);
         tmem_wait_ld();
         reg_barrier16(r);
-        if (split > 1) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + row] = __uint_as_float(r[j]);
-        } else if (n < a.N) {
+        if (n < a.N) {
           uint16_t* dst = a.out + (int64_t)(m0 + c) * a.out_stride + n;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
@@ -301,50 +383,52 @@ __global__ void __launch_bounds__(kSplitThreads)
         }
         __syncwarp();
       }
+    } else {
+      const uint32_t owner = (uint32_t)(row / share);
+      const uint32_t to = mapa_shared(smem_u32(sums + rank * TOK * share + row % share), owner);
+#pragma unroll 1
+      for (int c = 0; summed && c < toks; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + (uint32_t)c, r);
+        tmem_wait_ld();
+        reg_barrier16(r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c + j < toks)
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (uint32_t)((c + j) * share * 4)), "r"(r[j]) : "memory");
+      }
+      __syncwarp();
+      if (summed && row % min(32, share) == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                     ::"r"(mapa_shared(smem_u32(&sent), owner)) : "memory");
+      // also where this CTA has given up: the others' sums must find it here
+      const bool got = mbar_wait_sent(&sent, &abort_flag);
+      const int pairs = share / 2;
+      for (int i = (int)threadIdx.x - 64; got && i < toks * pairs; i += 128) {
+        const int tok = i / pairs, c = i % pairs * 2, n = n0 + rank * share + c;
+        float y0 = 0.f, y1 = 0.f;
+        for (int r = 0; r < split; ++r) {
+          const float2 p = *reinterpret_cast<const float2*>(sums + (r * TOK + tok) * share + c);
+          y0 = __fadd_rn(y0, p.x);
+          y1 = __fadd_rn(y1, p.y);
+        }
+        if (n >= a.N) continue;
+        const int n1 = min(n + 1, a.N - 1);
+        const float xs = ROWS16 ? (FORMAT == kNvfp4 ? row_scale[tok] : 1.0f) : a.xs ? a.xs[m0 + tok] : 1.0f;
+        const uint16_t h0 = f32_to_half_bits<BF16>(fp4_finish(y0, xs, a.ws ? a.ws[n] : 1.0f, a.bias ? a.bias[n] : 0.0f, a));
+        const uint16_t h1 = f32_to_half_bits<BF16>(fp4_finish(y1, xs, a.ws ? a.ws[n1] : 1.0f, a.bias ? a.bias[n1] : 0.0f, a));
+        uint16_t* dst = a.out + (int64_t)(m0 + tok) * a.out_stride + n;
+        if (n1 > n && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+          *reinterpret_cast<uint32_t*>(dst) = (uint32_t)h0 | ((uint32_t)h1 << 16);
+        } else {
+          dst[0] = h0;
+          if (n1 > n) dst[1] = h1;
+        }
+      }
     }
     tc_fence_before();
   }
-  if (split > 1) {
-    cluster_sync_all();
-    const int t0 = TOK * rank / split, t1 = min(TOK * (rank + 1) / split, a.M - m0);
-    const uint32_t sums0 = smem_u32(smem);
-    const bool wide = (a.out_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
-    for (int i = (int)threadIdx.x; i < (t1 - t0) * 32; i += kSplitThreads) {
-      const int tok = t0 + (i >> 5), c = (i & 31) * 4, n = n0 + c;
-      if (n >= a.N) continue;
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int r = 0; r < split; ++r) {
-        float4 p;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
-                     : "r"(mapa_shared(sums0 + (uint32_t)(tok * 512 + c * 4), (uint32_t)r)));
-        y[0] = __fadd_rn(y[0], p.x);
-        y[1] = __fadd_rn(y[1], p.y);
-        y[2] = __fadd_rn(y[2], p.z);
-        y[3] = __fadd_rn(y[3], p.w);
-      }
-      const float xs = ROWS16 ? (FORMAT == kNvfp4 ? row_scale[tok] : 1.0f) : a.xs ? a.xs[m0 + tok] : 1.0f;
-      uint16_t h[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int nn = min(n + j, a.N - 1);
-        h[j] = f32_to_half_bits<BF16>(fp4_finish(y[j], xs, a.ws ? a.ws[nn] : 1.0f, a.bias ? a.bias[nn] : 0.0f, a));
-      }
-      uint16_t* dst = a.out + (int64_t)(m0 + tok) * a.out_stride + n;
-      if (wide && n + 4 <= a.N) {
-        *reinterpret_cast<uint2*>(dst) =
-            make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < a.N) dst[j] = h[j];
-      }
-    }
-    cluster_sync_all();  // no CTA leaves while another reads its sums
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
@@ -354,57 +438,113 @@ __global__ void __launch_bounds__(kSplitThreads)
 // ------------------------------------------------------------------ many rows: 256 x 256 tiles on two SMs
 // A cluster of two CTAs computes 256 x 256 tiles (rows of x are the products' M): each CTA
 // loads 128 rows of x and 128 of the weight, and the even CTA's products read both.  Its
-// tensor memory holds 256 accumulator columns twice, overlapping by 96 columns ([0, 256) and
-// [160, 416)), and two slots of scales (48 columns each).  The epilogue of a tile first takes
-// what lies in the overlap into registers and lets the next tile's products begin.
-//   warp 0: TMA, warp 1: tensor memory and (even CTA) products, warps 4-11: epilogue, two per
-//   lane quadrant
+// tensor memory holds 256 accumulator columns twice, overlapping ([0, 256) and [kSecond,
+// kSecond + 256)), and behind them slots of scales.  The epilogue of a tile first takes what
+// lies in the overlap into registers and lets the next tile's products begin; its output
+// goes through shared memory in pieces of 32 rows x 64 columns, by TMA (16-byte stores of a
+// thread per row took the same shared-memory cycles that the products read with: 8,192 x
+// 12,288 x 4,096 180 us).
+//   warp 0: TMA, warp 1: tensor memory and (even CTA) scale copies and products, warps 4-11:
+//   epilogue, two per lane quadrant
 template <int FORMAT>
 struct PairFp4Cfg {
   static constexpr int kScaleBytes = FORMAT == kMxfp4 ? 1024 : 2048;  // of a band and step
   static constexpr int kStageBytes = 2 * 128 * kF4Step + 3 * kScaleBytes;
-  static constexpr int kStages = FORMAT == kMxfp4 ? 6 : 5;
-  static constexpr int kTotal = kStages * kStageBytes + 1024;
+  static constexpr int kStages = 5;
+  static constexpr int kOutBytes = 8 * 4096;
+  static constexpr int kTotal = kStages * kStageBytes + kOutBytes + 1024;
   static_assert(kStageBytes % 1024 == 0, "swizzled tiles start at multiples of 1024");
+  // Scale copies run ahead of the products by kSlots - 1 steps at most.  With 2 slots the copy
+  // for a step starts when the products of the step before it do and comes too late (9,472 x
+  // 2,048 x 16,384 mxfp4: 124 us, with 3 104 us, with 4 the same).
+  static constexpr int kSlots = 3;
+  static constexpr int kSlotCols = 3 * kScaleBytes / 128;  // 24 or 48 columns
+  static constexpr int kSecond = FORMAT == kMxfp4 ? 160 : 96;
+  static constexpr int kScales = kSecond + 256;
+  static_assert(kScales + kSlots * kSlotCols <= 512, "");
 };
 constexpr int kPairFp4Threads = 384;
-constexpr int kPairFp4Second = 160, kPairFp4Scales = 416;  // tensor-memory columns
 
+// 32 columns from n0 on of a row's sums: scales and bias, to 16 bits, two to a word
 template <bool BF16>
-__device__ __forceinline__ void fp4_store_chunk(const uint32_t (&r)[32], int m, int n0, const Fp4GemmArgs& a, float xs,
-                                                bool vec) {
-  uint16_t* dst = a.out + (int64_t)m * a.out_stride + n0;
+__device__ __forceinline__ void fp4_pack_chunk(const uint32_t (&r)[32], uint32_t (&h)[16], int n0, float xs, bool vec,
+                                               const Fp4GemmArgs& a) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
+    const int n = n0 + 8 * q;
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(__uint_as_float(r[8 * q + j]), xs);
-    const int n = n0 + 8 * q;
-    if (vec && n + 8 <= a.N) {
+    if (a.ws || a.bias) {
+      float w[8], b[8];
+      if (vec && n + 8 <= a.N) {
+        if (a.ws) {
+          const float4 p = *reinterpret_cast<const float4*>(a.ws + n), s = *reinterpret_cast<const float4*>(a.ws + n + 4);
+          w[0] = p.x, w[1] = p.y, w[2] = p.z, w[3] = p.w, w[4] = s.x, w[5] = s.y, w[6] = s.z, w[7] = s.w;
+        }
+        if (a.bias) {
+          const float4 p = *reinterpret_cast<const float4*>(a.bias + n), s = *reinterpret_cast<const float4*>(a.bias + n + 4);
+          b[0] = p.x, b[1] = p.y, b[2] = p.z, b[3] = p.w, b[4] = s.x, b[5] = s.y, b[6] = s.z, b[7] = s.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          w[j] = a.ws && n + j < a.N ? a.ws[n + j] : 1.0f;
+          b[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
+        }
+      }
       if (a.ws) {
-        const float4 w0 = *reinterpret_cast<const float4*>(a.ws + n), w1 = *reinterpret_cast<const float4*>(a.ws + n + 4);
-        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(y[j], w[j]);
       }
       if (a.bias) {
-        const float4 b0 = *reinterpret_cast<const float4*>(a.bias + n), b1 = *reinterpret_cast<const float4*>(a.bias + n + 4);
-        const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = __fadd_rn(y[j], b[j]);
       }
-      *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(pack_halves<BF16>(y[0], y[1]), pack_halves<BF16>(y[2], y[3]),
-                                                          pack_halves<BF16>(y[4], y[5]), pack_halves<BF16>(y[6], y[7]));
-    } else {
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (n + j >= a.N) continue;
-        float v = y[j];
-        if (a.ws) v = __fmul_rn(v, a.ws[n + j]);
-        if (a.bias) v = __fadd_rn(v, a.bias[n + j]);
-        dst[8 * q + j] = f32_to_half_bits<BF16>(v);
+    for (int j = 0; j < 4; ++j) h[4 * q + j] = pack_halves<BF16>(y[2 * j], y[2 * j + 1]);
+  }
+}
+// A warp's 32 x 64 piece of the output through its 4 KB of shared memory (rows of 128 bytes,
+// 16-byte pieces swizzled by the row, as TMA reads them): this lane's row is m = m0 + lane, its
+// columns from n0 on are lo and hi.
+__device__ __forceinline__ void fp4_put_piece(const CUtensorMap* tm_out, uint8_t* buf, const uint32_t (&lo)[16],
+                                              const uint32_t (&hi)[16], int m0, int n0, const Fp4GemmArgs& a) {
+  const int lane = threadIdx.x & 31;
+  if (a.out_tma) {  // the piece before has been read
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+        make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
+    *reinterpret_cast<uint4*>(buf + lane * 128 + (((q + 4) ^ (lane & 7)) << 4)) =
+        make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
+  }
+  if (a.out_tma) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0 && m0 < a.M && n0 < a.N) {  // rows and columns beyond are not written
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                   ::"l"(reinterpret_cast<uint64_t>(tm_out)), "r"(smem_u32(buf)), "r"(n0), "r"(m0) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  } else {  // rows that TMA does not take: each by the whole warp, a lane for two columns
+    __syncwarp();
+    const int n = n0 + 2 * lane;
+    for (int r = 0; r < 32 && m0 + r < a.M; ++r) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+      uint16_t* dst = a.out + (int64_t)(m0 + r) * a.out_stride + n;
+      if (n + 1 < a.N && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+        *reinterpret_cast<uint32_t*>(dst) = w;
+      } else {
+        if (n < a.N) dst[0] = (uint16_t)(w & 0xffffu);
+        if (n + 1 < a.N) dst[1] = (uint16_t)(w >> 16);
       }
     }
+    __syncwarp();
   }
 }
 
@@ -412,9 +552,9 @@ template <int FORMAT, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
     fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                     const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ CUtensorMap tm_sw,
-                    Fp4GemmArgs a) {
+                    const __grid_constant__ CUtensorMap tm_out, Fp4GemmArgs a) {
   using C = PairFp4Cfg<FORMAT>;
-  constexpr int kStages = C::kStages;
+  constexpr uint32_t kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kStages], empty[kStages], tfull, tempty, drained;
@@ -429,7 +569,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
   const int num_k = (a.K + 255) / 256;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (uint32_t s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
     }
@@ -453,16 +593,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
   const uint32_t tempty0 = mapa_shared(smem_u32(&tempty), 0);
 
   if (warp == 0) {
-    int stage = 0;
-    uint32_t phase = 0;
+    RingPlace fill;
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
       const int mb = t / num_n, nb = t % num_n;
       for (int kb = 0; kb < num_k; ++kb) {
-        if (!mbar_wait_warp(&empty[stage], phase ^ 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) { ok = false; break; }
+        if (!mbar_wait_warp(&empty[fill.stage], fill.parity ^ 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) { ok = false; break; }
         if (elect_one()) {
-          uint8_t* at = smem + stage * C::kStageBytes;
-          const uint32_t fb = full0 + (uint32_t)(stage * 8);
+          uint8_t* at = smem + fill.stage * C::kStageBytes;
+          const uint32_t fb = full0 + fill.stage * 8;
           mbar_arrive_expect_tx_cluster(fb, C::kStageBytes);
           tma_load_2d_pair(at, &tm_x, fb, kb * kF4Step, mb * 256 + (int)rank * 128);
           tma_load_2d_pair(at + 128 * kF4Step, &tm_w, fb, kb * kF4Step, nb * 256 + (int)rank * 128);
@@ -472,40 +611,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
           tma_load_2d_pair(at + C::kScaleBytes, &tm_sw, fb, kb * (C::kScaleBytes / 8), nb * 2);
         }
         __syncwarp();
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        fill.next(kStages);
       }
     }
     // Both CTAs' copies are counted by the even CTA's barriers; the odd one waits for it at the
-    // end.  Of each slot the last fill: slots before `stage` in this round, the others before.
+    // end.  Of each slot the last fill: slots before the next one in this round, the others before.
     if (rank == 0)
-      for (int s = 0; s < kStages; ++s)
-        mbar_wait_warp(&full[s], s < stage ? phase : phase ^ 1u, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
+      for (uint32_t s = 0; s < kStages; ++s)
+        mbar_wait_warp(&full[s], s < fill.stage ? fill.parity : fill.parity ^ 1u, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t smem0 = smem_u32(smem);
-      uint32_t it = 0;  // K steps so far
-      uint32_t tile = 0;
+      RingPlace at, freed;
+      uint32_t it = 0, slot = 0, tile = 0;  // K steps so far, the next one's slot of scales, tiles so far
       bool ok = true;
+      // the slot of a step's scales is read by the products kSlots steps before
+      auto peek = [&]() {
+        const bool two = lane == 1 && it >= C::kSlots;
+        return mbar_peek(two ? &empty[freed.stage] : &full[at.stage], two ? freed.parity : at.parity);
+      };
+      bool seen = peek();
       for (int t = pair; ok && t < tiles; t += pairs, ++tile) {
         if (tile > 0 && !mbar_wait_warp(&tempty, (tile - 1) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + (tile & 1 ? (uint32_t)kPairFp4Second : 0u);
-        for (int kb = 0; kb < num_k; ++kb, ++it) {
-          const uint32_t stage = it % kStages;
-          if (!mbar_wait_warp(&full[stage], (it / kStages) & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
-              (it >= 2 && !mbar_wait_warp(&empty[(it - 2) % kStages], ((it - 2) / kStages) & 1, &abort_flag,
-                                          H3B_STATUS_GEMM_TIMEOUT))) {
+        const uint32_t d = tmem + (tile & 1 ? (uint32_t)C::kSecond : 0u);
+        int products = (a.K + 63) / 64;
+        for (int kb = 0; kb < num_k; ++kb, products -= 4) {
+          if (!__all_sync(0xffffffffu, seen) &&
+              (!mbar_wait_warp(&full[at.stage], at.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
+               (it >= C::kSlots && !mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)))) {
             ok = false;
             break;
           }
           tc_fence_after();
+          const uint32_t x = smem0 + at.stage * C::kStageBytes;
+          const uint32_t sx = x + 2 * 128 * kF4Step;
+          const uint32_t ts = tmem + C::kScales + C::kSlotCols * slot;
+          uint64_t* used = &empty[at.stage];
+          if (it >= C::kSlots) freed.next(kStages);
+          at.next(kStages);
+          slot = slot == C::kSlots - 1 ? 0u : slot + 1;
+          ++it;
+          seen = peek();
           if (elect_one()) {
-            const uint32_t at = smem0 + stage * C::kStageBytes;
-            const uint32_t ts = tmem + kPairFp4Scales + 48u * (it & 1);
-            fp4_step<FORMAT, 2, 256, 256, 2>(d, at, at + 128 * kF4Step, at + 2 * 128 * kF4Step,
-                                             at + 2 * 128 * kF4Step + C::kScaleBytes, ts, ts + 16, 0u,
-                                             (a.K - kb * 256 + 63) / 64, kb == 0);
-            mma_commit_pair(&empty[stage], 0x3);
+            fp4_step_scales<FORMAT, 2, 2>(sx, sx + C::kScaleBytes, ts, ts + C::kSlotCols / 3);
+            fp4_step_products<FORMAT, 2, 256, 256, 2>(d, x, x + 128 * kF4Step, ts, ts + C::kSlotCols / 3, products, kb == 0);
+            mma_commit_pair(used, 0x3);
           }
           __syncwarp();
         }
@@ -518,44 +668,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
     }
   } else if (warp >= 4) {
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    const bool vec = (a.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
-                     (reinterpret_cast<uintptr_t>(a.ws) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(a.ws) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
+    uint8_t* buf = smem + kStages * C::kStageBytes + (warp - 4) * 4096;
     uint32_t tile = 0;
     for (int t = pair; t < tiles; t += pairs, ++tile) {
       const int mb = t / num_n, nb = t % num_n;
+      const int m_warp = mb * 256 + (int)rank * 128 + quad * 32, m = m_warp + lane;
+      const float xs = a.xs && m < a.M ? a.xs[m] : 1.0f;
       if (!mbar_wait_warp(&tfull, tile & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
       tc_fence_after();
-      const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane;
-      const float xs = a.xs && m < a.M ? a.xs[m] : 1.0f;
       const bool odd = tile & 1;
-      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (odd ? (uint32_t)kPairFp4Second : 0u);
-      // this warp's four chunks of 32 columns; in the overlap lie 5, 6, 7 of the even tiles
-      // and 0, 1, 2 of the odd ones, and they come first
-      const int order = odd ? (half ? 0x6572 : 0x4310) : (half ? 0x3247 : 0x1065);
-      uint32_t r0[32], r1[32];
-      tmem_ld32(taddr + 32u * (uint32_t)(order & 15), r0);
-      tmem_ld32(taddr + 32u * (uint32_t)((order >> 4) & 15), r1);
+      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (odd ? (uint32_t)C::kSecond : 0u);
+      // This warp's two 64-column pieces.  The overlap is the end of the even tiles and the start
+      // of the odd ones, 96 (mxfp4) or 160 columns: the first pieces of the two warps of a lane
+      // quadrant cover 128 of them, and for nvfp4 `half` 1 takes 32 columns of its second one along.
+      const int first = odd ? half : 3 - half, second = odd ? (half ? 2 : 3) : half;
+      const int n0 = nb * 256;
+      uint32_t r0[32], r1[32], r2[32], h0[16], h1[16];
+      const int early = odd ? 2 * second : 2 * second + 1, late = odd ? 2 * second + 1 : 2 * second;  // chunks of 32
+      tmem_ld32(taddr + 64u * (uint32_t)first, r0);
+      tmem_ld32(taddr + 64u * (uint32_t)first + 32u, r1);
+      if (FORMAT == kNvfp4) tmem_ld32(taddr + 32u * (uint32_t)early, r2);
       tmem_wait_ld_dep(r0);
       reg_barrier32(r1);
+      if (FORMAT == kNvfp4) reg_barrier32(r2);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0);
-      const int n0 = nb * 256;
-      if (m < a.M) {
-        fp4_store_chunk<BF16>(r0, m, n0 + 32 * (order & 15), a, xs, vec);
-        fp4_store_chunk<BF16>(r1, m, n0 + 32 * ((order >> 4) & 15), a, xs, vec);
-      }
-      __syncwarp();
-      tmem_ld32(taddr + 32u * (uint32_t)((order >> 8) & 15), r0);
-      tmem_ld32(taddr + 32u * (uint32_t)((order >> 12) & 15), r1);
+      fp4_pack_chunk<BF16>(r0, h0, n0 + 64 * first, xs, vec, a);
+      fp4_pack_chunk<BF16>(r1, h1, n0 + 64 * first + 32, xs, vec, a);
+      fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * first, a);
+      if (FORMAT != kNvfp4) tmem_ld32(taddr + 32u * (uint32_t)early, r2);
+      tmem_ld32(taddr + 32u * (uint32_t)late, r0);
       tmem_wait_ld_dep(r0);
-      reg_barrier32(r1);
-      if (m < a.M) {
-        fp4_store_chunk<BF16>(r0, m, n0 + 32 * ((order >> 8) & 15), a, xs, vec);
-        fp4_store_chunk<BF16>(r1, m, n0 + 32 * ((order >> 12) & 15), a, xs, vec);
-      }
-      __syncwarp();
+      reg_barrier32(r2);
+      fp4_pack_chunk<BF16>(r2, h0, n0 + 32 * early, xs, vec, a);
+      fp4_pack_chunk<BF16>(r0, h1, n0 + 32 * late, xs, vec, a);
+      if (odd) fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * second, a);
+      else fp4_put_piece(&tm_out, buf, h1, h0, m_warp, n0 + 64 * second, a);
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // written before the block leaves
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -607,7 +760,7 @@ static bool make_fp4_maps(const Fp4RowsView& v, int format, int box_rows, int bo
 #include <cstdlib>
 static int env(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
 #endif
-// How a product of few rows is divided: TOK and the CTAs along K
+// How a product of few rows is divided: rows of x per tile and CTAs along K
 struct SplitPlan {
   int tok, split;
 };
@@ -618,21 +771,27 @@ static SplitPlan plan_split(int M, int N, int K) {
   const int tok = M <= 16 ? 16 : M <= 64 ? 64 : 128, num_k = (K + 255) / 256;
   const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + tok - 1) / tok);
   int split = 1;
-  while (split < 8 && 2 * split <= num_k && tiles * 2 * split <= 2 * num_sms()) split *= 2;
+  while (split < 8 && 2 * split <= num_k && tiles * 2 * split <= num_sms()) split *= 2;
   return {tok, split};
 }
 template <int FORMAT, int TOK, bool ROWS16>
 static int launch_split(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, int split, cudaStream_t s,
                         cudaError_t* err) {
+  using C = SplitCfg<FORMAT, TOK, ROWS16>;
   CUtensorMap tx, tw, tsx, tsw;
   if (!make_fp4_maps(w, FORMAT, 128, 1, &tw, &tsw)) return 1;
   if (ROWS16) tx = tw, tsx = tsw;  // not used
   else if (!make_fp4_maps(x, FORMAT, TOK, 1, &tx, &tsx)) return 1;
-  const int64_t tiles = (int64_t)((a.N + 127) / 128) * ((a.M + TOK - 1) / TOK);
-  const int steps = ((a.K + 255) / 256 + split - 1) / split;
+  const int64_t grid = (int64_t)((a.N + 127) / 128) * ((a.M + TOK - 1) / TOK) * split;
+  const int steps = ((a.K + 255) / 256 + split - 1) / split, rest = C::rest_bytes(steps, split);
+  // as many stages as one CTA per SM has room for, or two where there are more CTAs than SMs
+  const int room = grid > num_sms() ? 112 * 1024 : 224 * 1024;
+  int stages = (room - rest) / C::kStageBytes;
+  stages = stages < 2 ? 2 : stages > kSplitMaxStages ? kSplitMaxStages : stages;
+  if (stages > steps) stages = steps;
   *err = launch_fp4(a.bf16 ? fp4_split_kernel<FORMAT, TOK, ROWS16, true> : fp4_split_kernel<FORMAT, TOK, ROWS16, false>,
-                    tiles * split, split, kSplitThreads, SplitCfg<FORMAT, TOK, ROWS16>::smem_bytes(steps), s, tw, tsw, tx,
-                    tsx, a, split);
+                    grid, split, kSplitThreads, (size_t)(stages * C::kStageBytes + rest), s, tw, tsw, tx, tsx, a, split,
+                    stages);
   return *err == cudaSuccess ? 0 : 2;
 }
 template <int FORMAT>
@@ -640,10 +799,18 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
                        cudaError_t* err) {
   CUtensorMap tx, tw, tsx, tsw;
   if (!make_fp4_maps(x, FORMAT, 128, 1, &tx, &tsx) || !make_fp4_maps(w, FORMAT, 128, 2, &tw, &tsw)) return 1;
+  // output rows that TMA takes: 16-byte aligned, and so are the steps between them
+  CUtensorMap to = tx;
+  Fp4GemmArgs b = a;
+  b.out_tma = (a.M == 1 || a.out_stride % 8 == 0) && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  if (b.out_tma && !make_tmap_2d(&to, a.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.N, (uint64_t)a.M,
+                                 (uint64_t)(a.M == 1 ? (a.N + 7) / 8 * 8 : a.out_stride) * 2, 64, 32,
+                                 CU_TENSOR_MAP_SWIZZLE_128B))
+    return 1;
   const int64_t tiles = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
   const int64_t pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
   *err = launch_fp4(a.bf16 ? fp4_pair_kernel<FORMAT, true> : fp4_pair_kernel<FORMAT, false>, 2 * pairs, 0,
-                    kPairFp4Threads, PairFp4Cfg<FORMAT>::kTotal, s, tx, tw, tsx, tsw, a);
+                    kPairFp4Threads, PairFp4Cfg<FORMAT>::kTotal, s, tx, tw, tsx, tsw, to, b);
   return *err == cudaSuccess ? 0 : 2;
 }
 static bool uses_pair(int M, int N) {
