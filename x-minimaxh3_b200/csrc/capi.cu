@@ -1020,7 +1020,7 @@ int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, const h3b_fp4_rows* w) {
   if (!w || rows < 0 || rows > (1 << 30) || w->rows < 0 || w->rows > (1 << 30) || w->cols < 1 ||
       w->cols > h3b::kFp4MaxRowCols || (w->format != H3B_MXFP4 && w->format != H3B_NVFP4))
     return -1;
-  if (rows == 0 || w->rows == 0 || h3b::fp4_takes_rows16(rows, w->rows, w->cols)) return 0;
+  if (rows == 0 || w->rows == 0 || h3b::fp4_takes_rows16(rows, w->rows, w->cols, w->format)) return 0;
   return rows * h3b::fp4_pitch(w->cols) + h3b::fp4_scale_bytes(rows, w->cols, w->format) +
          (w->format == H3B_NVFP4 ? align16(4 * rows) : 0);
 }

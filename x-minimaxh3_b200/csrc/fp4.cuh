@@ -75,7 +75,8 @@ struct Fp4GemmArgs {
   // 16-bit rows that the product quantises itself (launch_fp4_gemm_rows16)
   const uint16_t* x16;
   int64_t x16_stride;
-  int x16_vec;  // they allow 16-byte accesses
+  int x16_vec;       // they allow 16-byte accesses
+  int x16_log_segs;  // pieces of 512 columns that a CTA takes of a row, as a power of two
   int out_tma;  // set by the launcher: the output rows go out by TMA
 };
 // 0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err)
@@ -83,7 +84,7 @@ int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, i
                     cudaError_t* err);
 
 // Whether a linear of these sizes quantises its 16-bit rows inside the product, and that product
-bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K);
+bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K, int format);
 int launch_fp4_gemm_rows16(const uint16_t* x, int64_t x_stride, const Fp4RowsView& w, Fp4GemmArgs a, int format,
                            cudaStream_t s, cudaError_t* err);
 
@@ -97,7 +98,10 @@ __device__ __forceinline__ uint16_t f32_to_half_bits(float f) {
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
-  return (uint32_t)f32_to_half_bits<BF16>(lo) | ((uint32_t)f32_to_half_bits<BF16>(hi) << 16);
+  uint32_t r;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 // ------------------------------------------------------------------ a chunk of 16 columns to codes

@@ -6,8 +6,8 @@
 // A K step is 256 columns: 128 bytes of codes per row (one 128-byte swizzle row, four
 // products of 64 columns) and, per 128 rows, four (nvfp4) or two (mxfp4) 512-byte tiles of
 // block scales.  Codes and scales come by TMA into a ring of stages; the scales go on into
-// tensor memory by tcgen05.cp, into one of two slots: the copy into a slot waits for the
-// products of the step before last, which read it.
+// tensor memory by tcgen05.cp, into one of a few slots: the copy into a slot waits for the
+// products that read it last, and the products of a step for its copies.
 #include "fp4.cuh"
 #include "h3b_kernels.cuh"
 
@@ -18,15 +18,18 @@ constexpr int kF4Step = 128;  // bytes of codes per row and K step
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Shared-memory matrix descriptor without swizzle for a tile of block scales: 32 rows of 16
-// bytes, 8-row pieces of 128 bytes one after the other (SBO).
-__device__ __forceinline__ uint64_t sdesc_scales(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(128 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  return d;
+// Shared-memory matrix descriptors, of which the high word is constant and the low one the address
+// in units of 16 bytes and a flag: what a step needs comes by additions to it.
+__device__ __forceinline__ uint32_t sdesc_low(uint32_t smem_addr) { return ((smem_addr & 0x3FFFF) >> 4) | (1u << 16); }
+// K-major in the 128-byte swizzle: 8-row atoms of 1,024 bytes (SBO)
+__device__ __forceinline__ uint64_t sdesc_codes(uint32_t low) {
+  constexpr uint32_t high = (1024 >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)high << 32) | low;
+}
+// A tile of block scales, without swizzle: 32 rows of 16 bytes, 8-row pieces of 128 bytes (SBO)
+__device__ __forceinline__ uint64_t sdesc_scales(uint32_t low) {
+  constexpr uint32_t high = (128 >> 4) | (1u << 14);
+  return ((uint64_t)high << 32) | low;
 }
 // Instruction descriptor of the block-scaled 4-bit kinds: bits 4-5 / 29-30 first byte of the
 // scale word of B / A, 7-9 / 10-11 E2M1 operands (1), 17-22 N>>3, 23 E8M0 scales, 24-28 M>>4.
@@ -68,13 +71,13 @@ __device__ __forceinline__ float fp4_finish(float sum, float xs, float ws, float
 template <int FORMAT, int CTAS, int BANDS>
 __device__ __forceinline__ void fp4_step_scales(uint32_t smem_sa, uint32_t smem_sb, uint32_t tmem_sa, uint32_t tmem_sb) {
   constexpr int kTiles = FORMAT == kMxfp4 ? 2 : 4;  // scale tiles per band and step
+  const uint32_t la = sdesc_low(smem_sa), lb = sdesc_low(smem_sb);
 #pragma unroll
   for (int g = 0; g < kTiles; ++g) {
-    copy_scales<CTAS>(tmem_sa + (uint32_t)(4 * g), sdesc_scales(smem_sa + (uint32_t)(512 * g)));
+    copy_scales<CTAS>(tmem_sa + (uint32_t)(4 * g), sdesc_scales(la + 32u * g));
 #pragma unroll
     for (int b = 0; b < BANDS; ++b)
-      copy_scales<CTAS>(tmem_sb + (uint32_t)(4 * (BANDS * g + b)),
-                        sdesc_scales(smem_sb + (uint32_t)(512 * (kTiles * b + g))));
+      copy_scales<CTAS>(tmem_sb + (uint32_t)(4 * (BANDS * g + b)), sdesc_scales(lb + 32u * (kTiles * b + g)));
   }
 }
 // One thread: the products of one K step into accumulator d; tmem_sb: the column of B's scales
@@ -82,19 +85,20 @@ __device__ __forceinline__ void fp4_step_scales(uint32_t smem_sa, uint32_t smem_
 template <int FORMAT, int CTAS, int M, int N, int BANDS>
 __device__ __forceinline__ void fp4_step_products(uint32_t d, uint32_t smem_a, uint32_t smem_b, uint32_t tmem_sa,
                                                   uint32_t tmem_sb, int products, bool first) {
-  const uint64_t da = sdesc_kmajor_sw128(smem_a), db = sdesc_kmajor_sw128(smem_b);
+  const uint32_t la = sdesc_low(smem_a), lb = sdesc_low(smem_b);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (k > 0 && k >= products) break;
     const uint32_t byte = FORMAT == kMxfp4 ? 2u * (uint32_t)(k & 1) : 0u;
     const uint32_t g = FORMAT == kMxfp4 ? (uint32_t)(k >> 1) : (uint32_t)k;
-    mma_fp4<FORMAT, CTAS>(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_fp4(M, N, FORMAT == kMxfp4, byte),
+    mma_fp4<FORMAT, CTAS>(d, sdesc_codes(la + 2u * k), sdesc_codes(lb + 2u * k), idesc_fp4(M, N, FORMAT == kMxfp4, byte),
                           tmem_sa + 4u * g, tmem_sb + 4u * BANDS * g, first && k == 0 ? 0u : 1u);
   }
 }
-// Non-blocking look at a barrier.  The warps that issue products look at the next step's barriers
-// before they issue this step's: a wait costs about 100 cycles even where it is over, and a step
-// of the 256 x 256 tiles has 512 in all.
+// Non-blocking look at a barrier.  The warps that issue scale copies and products look at the next
+// step's barriers, a lane at each, before they issue this step's: a wait costs about 100 cycles
+// even where it is over, a scale copy 20 to 30, and a step of the 256 x 256 tiles has 512 in all
+// (9,472 x 2,048 x 16,384 mxfp4 with plain waits 124 us, so 104 us).
 __device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -119,9 +123,9 @@ struct RingPlace {
 // take equal parts of K; each sends its sums to the CTAs that own their columns (equal shares of
 // the tile's 128), which add them in the CTAs' order (the same sums every time) and write them.
 // Without a split the sums go out as they come from tensor memory.
-//   warp 0: TMA, warp 1: tensor memory, scale copies and products, warps 2-5: sums
+//   warp 0: TMA, warp 1: tensor memory and products, warp 2: scale copies, warps 3-6: sums
 // Behind the quantisation of x in the stream, the first weight tiles are on their way before
-// that has ended.  ROWS16: x is 16-bit, at most 16 rows, and warps 2-5 of each CTA quantise
+// that has ended.  ROWS16: x is 16-bit, at most 16 rows, and warps 3-6 of each CTA quantise
 // its part of K themselves (for nvfp4 the cluster's CTAs tell each other their rows' absmax).
 template <int FORMAT, int TOK, bool ROWS16>
 struct SplitCfg {
@@ -142,8 +146,12 @@ struct SplitCfg {
     return (ROWS16 ? steps * kXStep : 0) + (split > 1 ? TOK * 512 : 0) + 1024;
   }
 };
-constexpr int kSplitThreads = 192, kSplitMaxStages = 8;
-constexpr int kRows16Steps = 8;  // K steps of a CTA that quantises x
+constexpr int kSplitThreads = 224, kSplitMaxStages = 8;
+constexpr int kRows16Steps = 16;  // K steps of a CTA that quantises x
+// Pieces of 512 columns of x that one of its four warps holds.  More rows take longer here than in a
+// kernel of their own in front (4,096 -> 4,096, nvfp4: 4 rows 7.2 us in one launch and 6.2 in two, 8 rows
+// 8.4 and 6.1; mxfp4: 8 rows 5.8 and 5.7); a call in one launch costs the host 10 us, one in two 14.
+constexpr int rows16_items(int format) { return format == kMxfp4 ? 4 : 2; }
 
 // bounded wait for an mbarrier whose arrivals release what other CTAs of the cluster wrote here
 __device__ __forceinline__ bool mbar_wait_sent(uint64_t* bar, volatile int* abort_flag) {
@@ -166,93 +174,89 @@ template <int FORMAT, int TOK, bool ROWS16, bool BF16>
 __global__ void __launch_bounds__(kSplitThreads)
     fp4_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sw,
                      const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_sx,
-                     Fp4GemmArgs a, int split, int num_stages) {
+                     Fp4GemmArgs a, int log_split, int num_stages) {
   using C = SplitCfg<FORMAT, TOK, ROWS16>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kSplitMaxStages], empty[kSplitMaxStages], done, x_ready, sent;
+  __shared__ uint64_t full[kSplitMaxStages], empty[kSplitMaxStages], scaled[C::kSlots], done, copied, x_ready, sent;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, late_flag;
   __shared__ uint32_t row_top[16];
-  __shared__ float row_scale[16];
+  __shared__ float row_scale[TOK];
   __shared__ __align__(16) uint16_t pieces[ROWS16 ? 4 : 1][ROWS16 ? 512 : 8];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
-  const int num_n = (a.N + 127) / 128;
-  const int tile = blockIdx.x / split;
-  const int n0 = tile % num_n * 128, m0 = tile / num_n * TOK;
+  const int split = 1 << log_split, rank = (int)blockIdx.x & (split - 1);
+  const int n0 = ((int)blockIdx.x >> log_split) * 128, m0 = (int)blockIdx.y * TOK;
   const int num_k = (a.K + 255) / 256;
-  const int kb0 = (int)((int64_t)num_k * rank / split), steps = (int)((int64_t)num_k * (rank + 1) / split) - kb0;
+  const int kb0 = (num_k * rank) >> log_split, steps = ((num_k * (rank + 1)) >> log_split) - kb0;
   const uint32_t stages = (uint32_t)num_stages;
-  const int share = 128 / split;                     // columns of the tile that this CTA adds up
-  uint8_t* x_area = smem + stages * C::kStageBytes;  // ROWS16: [steps] codes and scales
+  const int log_share = 7 - log_split, share = 1 << log_share;  // columns of the tile that this CTA adds up
+  uint8_t* x_area = smem + stages * C::kStageBytes;             // ROWS16: [steps] codes and scales
   // [split][TOK][share], at the same place in all CTAs of the cluster
-  float* sums = reinterpret_cast<float*>(x_area + (ROWS16 ? (num_k + split - 1) / split * C::kXStep : 0));
+  float* sums = reinterpret_cast<float*>(x_area + (ROWS16 ? ((num_k + split - 1) >> log_split) * C::kXStep : 0));
 
-  RingPlace fill;
-  int fills = 0;
-  auto load_w = [&]() {
-    uint8_t* at = smem + fill.stage * C::kStageBytes;
-    uint64_t* bar = &full[fill.stage];
-    mbar_arrive_expect_tx(bar, C::kStageBytes);
-    tma_load_2d(at, &tm_w, bar, (kb0 + fills) * kF4Step, n0);
-    tma_load_2d(at + C::kWBytes, &tm_sw, bar, (kb0 + fills) * (C::kScaleBytes / 8), n0 >> 7);
-  };
-  auto load_x = [&](int i, uint32_t stage) {
-    if constexpr (!ROWS16) {
-      uint8_t* at = smem + stage * C::kStageBytes + C::kWBytes + C::kScaleBytes;
-      tma_load_2d(at, &tm_x, &full[stage], (kb0 + i) * kF4Step, m0);
-      tma_load_2d(at + C::kXBytes, &tm_sx, &full[stage], (kb0 + i) * (C::kScaleBytes / 8), m0 >> 7);
-    }
-  };
   if (warp == 0) {
-    // the first loads start before tensor memory is there: nobody else looks at their barriers yet
-    if (lane == 0) {
-      for (uint32_t s = 0; s < stages; ++s) {
-        mbar_init(&full[s], 1);
-        mbar_init(&empty[s], 1);
-      }
+    if (lane < kSplitMaxStages) {
+      mbar_init(&full[lane], 1);
+      mbar_init(&empty[lane], 1);
+    } else if (lane < kSplitMaxStages + C::kSlots) {
+      mbar_init(&scaled[lane - kSplitMaxStages], 1);
+    } else if (lane == 31) {
       mbar_init(&done, 1);
+      mbar_init(&copied, 1);
       mbar_init(&x_ready, 128);
       mbar_init(&sent, (uint32_t)(128 / min(32, share)));
       abort_flag = late_flag = 0;
-      fence_mbar_init();
     }
+    fence_mbar_init();
     __syncwarp();
-    if (!a.behind_rows) chain_wait();
+    asm volatile("bar.arrive 1, %0;" ::"n"(kSplitThreads) : "memory");
+    // the first loads start before tensor memory is there
+    RingPlace fill, freed;
+    auto load_w = [&](int i, uint32_t stage) {
+      uint8_t* at = smem + stage * C::kStageBytes;
+      mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+      tma_load_2d(at, &tm_w, &full[stage], (kb0 + i) * kF4Step, n0);
+      tma_load_2d(at + C::kWBytes, &tm_sw, &full[stage], (kb0 + i) * (C::kScaleBytes / 8), n0 >> 7);
+    };
+    auto load_x = [&](int i, uint32_t stage) {
+      if constexpr (!ROWS16) {
+        uint8_t* at = smem + stage * C::kStageBytes + C::kWBytes + C::kScaleBytes;
+        tma_load_2d(at, &tm_x, &full[stage], (kb0 + i) * kF4Step, m0);
+        tma_load_2d(at + C::kXBytes, &tm_sx, &full[stage], (kb0 + i) * (C::kScaleBytes / 8), m0 >> 7);
+      }
+    };
     const int ahead = min(steps, num_stages);
-    for (; fills < ahead; ++fills) {
-      if (elect_one()) load_w();
+    if (a.behind_rows) {
+      if (elect_one())
+        for (int i = 0; i < ahead; ++i) load_w(i, (uint32_t)i);
       __syncwarp();
-      fill.next(stages);
+      chain_wait();
+      if (elect_one())
+        for (int i = 0; i < ahead; ++i) load_x(i, (uint32_t)i);
+    } else {
+      chain_wait();
+      if (elect_one())
+        for (int i = 0; i < ahead; ++i) {
+          load_w(i, (uint32_t)i);
+          load_x(i, (uint32_t)i);
+        }
     }
-    if (a.behind_rows) chain_wait();
-    if (!ROWS16 && elect_one())
-      for (int i = 0; i < ahead; ++i) load_x(i, (uint32_t)i);
     __syncwarp();
-  } else if (warp == 1) {
-    tmem_alloc(&tmem_slot, C::kTmemCols);
-    tmem_relinquish();
-  } else if (ROWS16 && threadIdx.x < 80) {
-    row_top[threadIdx.x - 64] = 0u;
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  chain_next();
-  if (split > 1) cluster_arrive();  // and wait before anything of another CTA is touched
-  const uint32_t tmem = tmem_slot;
-
-  if (warp == 0) {
-    if (split > 1) cluster_wait();
-    if (ROWS16 && FORMAT == kNvfp4 && split > 1) cluster_sync_all();
-    RingPlace freed;
+    chain_next();
+    if (split > 1) {
+      cluster_arrive();
+      cluster_wait();
+      if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
+    }
+    int fills = ahead;
+    for (int i = 0; i < ahead; ++i) fill.next(stages);
     for (; fills < steps; ++fills) {
       if (!mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
       freed.next(stages);
       if (elect_one()) {
-        load_w();
+        load_w(fills, fill.stage);
         load_x(fills, fill.stage);
       }
       __syncwarp();
@@ -261,34 +265,48 @@ __global__ void __launch_bounds__(kSplitThreads)
     // every copy that was started has landed before the CTA may leave: of each slot the last fill
     for (uint32_t s = 0; s < stages; ++s)
       mbar_wait_warp(&full[s], s < fill.stage ? fill.parity : fill.parity ^ 1u, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
-  } else if (warp == 1) {
+  } else {
+    if (warp == 1) {
+      tmem_alloc(&tmem_slot, C::kTmemCols);
+      tmem_relinquish();
+    } else if (ROWS16 && threadIdx.x >= 96 && threadIdx.x < 112) {
+      row_top[threadIdx.x - 96] = 0u;
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 1, %0;" ::"n"(kSplitThreads) : "memory");
+    tc_fence_after();
+    chain_next();
+    if (split > 1) cluster_arrive();  // and wait before anything of another CTA is touched
+  }
+  const uint32_t tmem = tmem_slot;  // warp 0 does not use it
+
+  if (warp == 1) {
+    if (split > 1) {
+      cluster_wait();
+      if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
+    }
+    // products: a step's operands are there, and its scales in tensor memory
     const uint32_t smem0 = smem_u32(smem), x0 = smem_u32(x_area);
-    if (split > 1) cluster_wait();
-    if (ROWS16 && FORMAT == kNvfp4 && split > 1) cluster_sync_all();
-    const bool ready = !ROWS16 || mbar_wait_warp(&x_ready, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
-    RingPlace at, freed;
-    // the slot of scales of step i: read by the products of step i - kSlots
-    auto wants_slot = [&](int i) { return i >= C::kSlots && num_stages > C::kSlots; };
-    auto peek = [&](int i) {
-      const bool slot = lane == 1 && wants_slot(i);
-      return mbar_peek(slot ? &empty[freed.stage] : &full[at.stage], slot ? freed.parity : at.parity);
+    RingPlace at, scales;
+    auto peek = [&]() {
+      return lane == 1 ? mbar_peek(&full[at.stage], at.parity) : mbar_peek(&scaled[scales.stage], scales.parity);
     };
-    bool seen = peek(0);
+    bool seen = peek();
+    const bool ready = !ROWS16 || mbar_wait_warp(&x_ready, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
     for (int i = 0; ready && i < steps; ++i) {
       if (!__all_sync(0xffffffffu, seen) &&
-          (!mbar_wait_warp(&full[at.stage], at.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
-           (wants_slot(i) && !mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT))))
+          (!mbar_wait_warp(&scaled[scales.stage], scales.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
+           !mbar_wait_warp(&full[at.stage], at.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)))
         break;
       tc_fence_after();
       const uint32_t w = smem0 + at.stage * C::kStageBytes;
       const uint32_t x = ROWS16 ? x0 + (uint32_t)(i * C::kXStep) : w + C::kWBytes + C::kScaleBytes;
-      const uint32_t ts = tmem + C::kAccCols + (uint32_t)(C::kSlotCols * (i & (C::kSlots - 1)));
+      const uint32_t ts = tmem + C::kAccCols + C::kSlotCols * scales.stage;
       uint64_t* used = &empty[at.stage];
-      if (wants_slot(i)) freed.next(stages);
       at.next(stages);
-      seen = peek(i + 1);
+      scales.next(C::kSlots);
+      seen = peek();
       if (elect_one()) {
-        fp4_step_scales<FORMAT, 1, 1>(w + C::kWBytes, x + C::kXBytes, ts, ts + C::kSlotCols / 2);
         // rows m0 .. of their 128-row band: 32 to a column of the scales
         fp4_step_products<FORMAT, 1, 128, TOK, 1>(tmem, w, x, ts, ts + C::kSlotCols / 2 + ((uint32_t)(m0 >> 5) & 3u),
                                                   (a.K - (kb0 + i) * 256 + 63) / 64, i == 0);
@@ -299,40 +317,93 @@ __global__ void __launch_bounds__(kSplitThreads)
     if (elect_one()) mma_commit(&done);
     __syncwarp();
     mbar_wait_warp(&done, 0, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
-  } else {
+  } else if (warp == 2) {
+    if (split > 1) {
+      cluster_wait();
+      if (ROWS16 && FORMAT == kNvfp4) cluster_sync_all();
+    }
+    // scale copies: into the slot that the products kSlots steps before have read
+    const uint32_t smem0 = smem_u32(smem), x0 = smem_u32(x_area);
+    const bool ready = !ROWS16 || mbar_wait_warp(&x_ready, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
+    RingPlace at, freed, scales;
+    int i = 0;
+    // With as many stages as slots or fewer, a stage that is full says that its slot was read; with
+    // more, the slot's barrier is asked, which cannot have moved on by more than one phase.
+    auto asks = [&]() { return i >= C::kSlots && num_stages > C::kSlots; };
+    auto peek = [&]() {
+      const bool slot = lane == 1 && asks();
+      return mbar_peek(slot ? &empty[freed.stage] : &full[at.stage], slot ? freed.parity : at.parity);
+    };
+    bool seen = peek();
+    while (ready && i < steps) {
+      if (!__all_sync(0xffffffffu, seen) &&
+          (!mbar_wait_warp(&full[at.stage], at.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
+           (asks() && !mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT))))
+        break;
+      tc_fence_after();
+      const uint32_t w = smem0 + at.stage * C::kStageBytes;
+      const uint32_t x = ROWS16 ? x0 + (uint32_t)(i * C::kXStep) : w + C::kWBytes + C::kScaleBytes;
+      const uint32_t ts = tmem + C::kAccCols + C::kSlotCols * scales.stage;
+      uint64_t* there = &scaled[scales.stage];
+      if (asks()) freed.next(stages);
+      at.next(stages);
+      scales.next(C::kSlots);
+      ++i;
+      seen = peek();
+      if (elect_one()) {
+        fp4_step_scales<FORMAT, 1, 1>(w + C::kWBytes, x + C::kXBytes, ts, ts + C::kSlotCols / 2);
+        mma_commit(there);
+      }
+      __syncwarp();
+    }
+    if (elect_one()) mma_commit(&copied);
+    __syncwarp();
+    mbar_wait_warp(&copied, 0, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
+  } else if (warp > 2) {
+    const int tid = (int)threadIdx.x - 96;
     chain_wait();
+    const int toks = min(TOK, a.M - m0);
     if constexpr (ROWS16) {
-      // a warp takes 32 chunks of 16 columns of a row at a time
+      // A warp takes 32 chunks of 16 columns of a row at a time, and keeps them between the passes.
       const uint16_t* x = a.x16 + kb0 * 256;
-      const int K = a.K - kb0 * 256, segs = (steps + 1) / 2, items = a.M * segs;
-      const bool vec = a.x16_vec;
-      uint16_t* piece = pieces[warp - 2];
-      float v[16];
-      auto load = [&](int item) {
-        const uint16_t* row = x + (int64_t)(item / segs) * a.x16_stride;
-        const int c = item % segs * 32 + lane;
-        if (vec) load16<BF16, true>(row, c, K, piece, v);
-        else load16<BF16, false>(row, c, K, piece, v);
-      };
+      const int K = a.K - kb0 * 256, log_segs = a.x16_log_segs, items = a.M << log_segs;
+      constexpr int kItems = rows16_items(FORMAT);
+      uint4 raw[kItems][2];
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        const int item = warp - 3 + 4 * j;
+        if (item >= items) break;
+        const uint16_t* row = x + (int64_t)(item >> log_segs) * a.x16_stride;
+        const int c = (item & ((1 << log_segs) - 1)) * 32 + lane;
+        if (a.x16_vec) load16_raw<true>(row, c, K, pieces[warp - 3], raw[j][0], raw[j][1]);
+        else load16_raw<false>(row, c, K, pieces[warp - 3], raw[j][0], raw[j][1]);
+      }
       if constexpr (FORMAT == kNvfp4) {
-        for (int item = warp - 2; item < items; item += 4) {
-          load(item);
+#pragma unroll
+        for (int j = 0; j < kItems; ++j) {
+          const int item = warp - 3 + 4 * j;
+          if (item >= items) break;
+          float v[16];
+          unpack16<BF16>(raw[j][0], raw[j][1], v);
           uint32_t top = absmax16(v);
           if (top >= kInfBits) top = 0u;
           top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0) atomicMax(&row_top[item / segs], top);
+          if (lane == 0) atomicMax(&row_top[item >> log_segs], top);
         }
         if (split > 1) {
           cluster_wait();
           cluster_sync_all();
         } else {
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 2, 128;" ::: "memory");
         }
       }
-      for (int item = warp - 2; item < items; item += 4) {
-        const int r = item / segs, c = item % segs * 32 + lane;
-        if (FORMAT == kMxfp4 || items > 4) load(item);  // else it is there from above
-        float inv_r = 1.0f;
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        const int item = warp - 3 + 4 * j;
+        if (item >= items) break;
+        const int r = item >> log_segs, c = (item & ((1 << log_segs) - 1)) * 32 + lane;
+        float v[16], inv_r = 1.0f;
+        unpack16<BF16>(raw[j][0], raw[j][1], v);
         if constexpr (FORMAT == kNvfp4) {
           uint32_t top = 0u;
           if (lane < split)
@@ -354,18 +425,24 @@ __global__ void __launch_bounds__(kSplitThreads)
             *reinterpret_cast<uint32_t*>(at + C::kXBytes + (c & 15) / kLanes * 512 + r * 16) = word;
         }
       }
+      if (FORMAT == kMxfp4 && tid < 16) row_scale[tid] = 1.0f;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&x_ready);
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // row_scale is read by all four warps
+    } else {
+      for (int i = tid; i < toks; i += 128) row_scale[i] = a.xs ? a.xs[m0 + i] : 1.0f;
     }
+    // what the output needs beside the sums is fetched before they are there
+    const int quad = warp & 3, row = quad * 32 + lane;
+    const int n = split == 1 ? n0 + row : n0 + rank * share + ((2 * tid) & (share - 1));
+    const int n1 = min(n + 1, a.N - 1);
+    const float ws0 = a.ws && n < a.N ? a.ws[n] : 1.0f, bias0 = a.bias && n < a.N ? a.bias[n] : 0.0f;
+    const float ws1 = a.ws && n < a.N ? a.ws[n1] : 1.0f, bias1 = a.bias && n < a.N ? a.bias[n1] : 0.0f;
+    asm volatile("bar.sync 2, 128;" ::: "memory");  // row_scale
     if (split > 1 && !(ROWS16 && FORMAT == kNvfp4)) cluster_wait();
-    const int quad = warp & 3, row = quad * 32 + lane, toks = min(TOK, a.M - m0);
     const bool summed = mbar_wait_warp(&done, 0, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
     tc_fence_after();
     const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
     if (split == 1) {
-      const int n = n0 + row;
-      const float ws = a.ws && n < a.N ? a.ws[n] : 1.0f, bias = a.bias && n < a.N ? a.bias[n] : 0.0f;
 #pragma unroll 1
       for (int c = 0; summed && c < toks; c += 16) {
         uint32_t r[16];
@@ -377,15 +454,14 @@ __global__ void __launch_bounds__(kSplitThreads)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             if (c + j >= toks) break;
-            const float xs = ROWS16 ? (FORMAT == kNvfp4 ? row_scale[c + j] : 1.0f) : a.xs ? a.xs[m0 + c + j] : 1.0f;
-            dst[j * a.out_stride] = f32_to_half_bits<BF16>(fp4_finish(__uint_as_float(r[j]), xs, ws, bias, a));
+            dst[j * a.out_stride] = f32_to_half_bits<BF16>(fp4_finish(__uint_as_float(r[j]), row_scale[c + j], ws0, bias0, a));
           }
         }
         __syncwarp();
       }
     } else {
-      const uint32_t owner = (uint32_t)(row / share);
-      const uint32_t to = mapa_shared(smem_u32(sums + rank * TOK * share + row % share), owner);
+      const uint32_t owner = (uint32_t)(row >> log_share);
+      const uint32_t to = mapa_shared(smem_u32(sums + ((rank * TOK) << log_share) + (row & (share - 1))), owner);
 #pragma unroll 1
       for (int c = 0; summed && c < toks; c += 16) {
         uint32_t r[16];
@@ -395,28 +471,31 @@ __global__ void __launch_bounds__(kSplitThreads)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (c + j < toks)
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (uint32_t)((c + j) * share * 4)), "r"(r[j]) : "memory");
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (uint32_t)(((c + j) << log_share) * 4)), "r"(r[j]) : "memory");
       }
       __syncwarp();
-      if (summed && row % min(32, share) == 0)
+      if (summed && (row & (min(32, share) - 1)) == 0)
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
                      ::"r"(mapa_shared(smem_u32(&sent), owner)) : "memory");
       // also where this CTA has given up: the others' sums must find it here
       const bool got = mbar_wait_sent(&sent, &abort_flag);
-      const int pairs = share / 2;
-      for (int i = (int)threadIdx.x - 64; got && i < toks * pairs; i += 128) {
-        const int tok = i / pairs, c = i % pairs * 2, n = n0 + rank * share + c;
+      const float* mine = sums + ((2 * tid) & (share - 1));
+      const int log_pairs = log_share - 1;
+      for (int tok = tid >> log_pairs; got && tok < toks; tok += 128 >> log_pairs) {
+        float2 p[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < split) p[r] = *reinterpret_cast<const float2*>(mine + ((r * TOK + tok) << log_share));
         float y0 = 0.f, y1 = 0.f;
-        for (int r = 0; r < split; ++r) {
-          const float2 p = *reinterpret_cast<const float2*>(sums + (r * TOK + tok) * share + c);
-          y0 = __fadd_rn(y0, p.x);
-          y1 = __fadd_rn(y1, p.y);
-        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < split) {
+            y0 = __fadd_rn(y0, p[r].x);
+            y1 = __fadd_rn(y1, p[r].y);
+          }
         if (n >= a.N) continue;
-        const int n1 = min(n + 1, a.N - 1);
-        const float xs = ROWS16 ? (FORMAT == kNvfp4 ? row_scale[tok] : 1.0f) : a.xs ? a.xs[m0 + tok] : 1.0f;
-        const uint16_t h0 = f32_to_half_bits<BF16>(fp4_finish(y0, xs, a.ws ? a.ws[n] : 1.0f, a.bias ? a.bias[n] : 0.0f, a));
-        const uint16_t h1 = f32_to_half_bits<BF16>(fp4_finish(y1, xs, a.ws ? a.ws[n1] : 1.0f, a.bias ? a.bias[n1] : 0.0f, a));
+        const uint16_t h0 = f32_to_half_bits<BF16>(fp4_finish(y0, row_scale[tok], ws0, bias0, a));
+        const uint16_t h1 = f32_to_half_bits<BF16>(fp4_finish(y1, row_scale[tok], ws1, bias1, a));
         uint16_t* dst = a.out + (int64_t)(m0 + tok) * a.out_stride + n;
         if (n1 > n && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
           *reinterpret_cast<uint32_t*>(dst) = (uint32_t)h0 | ((uint32_t)h1 << 16);
@@ -444,8 +523,9 @@ __global__ void __launch_bounds__(kSplitThreads)
 // goes through shared memory in pieces of 32 rows x 64 columns, by TMA (16-byte stores of a
 // thread per row took the same shared-memory cycles that the products read with: 8,192 x
 // 12,288 x 4,096 180 us).
-//   warp 0: TMA, warp 1: tensor memory and (even CTA) scale copies and products, warps 4-11:
-//   epilogue, two per lane quadrant
+//   warp 0: TMA, warp 1: tensor memory and (even CTA) scale copies and products (a warp of its own
+//   for the copies made it slower: they wait in the tensor pipe behind the products issued before
+//   them, and what follows would wait for their barrier), warps 4-11: epilogue, two per lane quadrant
 template <int FORMAT>
 struct PairFp4Cfg {
   static constexpr int kScaleBytes = FORMAT == kMxfp4 ? 1024 : 2048;  // of a band and step
@@ -465,45 +545,32 @@ struct PairFp4Cfg {
 };
 constexpr int kPairFp4Threads = 384;
 
-// 32 columns from n0 on of a row's sums: scales and bias, to 16 bits, two to a word
+// 32 columns of a row's sums: scales and bias (of these columns, in shared memory), to 16 bits, two
+// to a word
 template <bool BF16>
-__device__ __forceinline__ void fp4_pack_chunk(const uint32_t (&r)[32], uint32_t (&h)[16], int n0, float xs, bool vec,
-                                               const Fp4GemmArgs& a) {
+__device__ __forceinline__ void fp4_pack_chunk(const uint32_t (&r)[32], uint32_t (&h)[16], float xs, const float* ws,
+                                               const float* bias, const Fp4GemmArgs& a) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int n = n0 + 8 * q;
-    float y[8];
+  for (int q = 0; q < 8; ++q) {
+    float y[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(__uint_as_float(r[8 * q + j]), xs);
-    if (a.ws || a.bias) {
-      float w[8], b[8];
-      if (vec && n + 8 <= a.N) {
-        if (a.ws) {
-          const float4 p = *reinterpret_cast<const float4*>(a.ws + n), s = *reinterpret_cast<const float4*>(a.ws + n + 4);
-          w[0] = p.x, w[1] = p.y, w[2] = p.z, w[3] = p.w, w[4] = s.x, w[5] = s.y, w[6] = s.z, w[7] = s.w;
-        }
-        if (a.bias) {
-          const float4 p = *reinterpret_cast<const float4*>(a.bias + n), s = *reinterpret_cast<const float4*>(a.bias + n + 4);
-          b[0] = p.x, b[1] = p.y, b[2] = p.z, b[3] = p.w, b[4] = s.x, b[5] = s.y, b[6] = s.z, b[7] = s.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          w[j] = a.ws && n + j < a.N ? a.ws[n + j] : 1.0f;
-          b[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
-        }
-      }
-      if (a.ws) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(y[j], w[j]);
-      }
-      if (a.bias) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = __fadd_rn(y[j], b[j]);
-      }
+    for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(__uint_as_float(r[4 * q + j]), xs);
+    if (a.ws) {
+      const float4 w = *reinterpret_cast<const float4*>(ws + 4 * q);
+      y[0] = __fmul_rn(y[0], w.x);
+      y[1] = __fmul_rn(y[1], w.y);
+      y[2] = __fmul_rn(y[2], w.z);
+      y[3] = __fmul_rn(y[3], w.w);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[4 * q + j] = pack_halves<BF16>(y[2 * j], y[2 * j + 1]);
+    if (a.bias) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + 4 * q);
+      y[0] = __fadd_rn(y[0], b.x);
+      y[1] = __fadd_rn(y[1], b.y);
+      y[2] = __fadd_rn(y[2], b.z);
+      y[3] = __fadd_rn(y[3], b.w);
+    }
+    h[2 * q] = pack_halves<BF16>(y[0], y[1]);
+    h[2 * q + 1] = pack_halves<BF16>(y[2], y[3]);
   }
 }
 // A warp's 32 x 64 piece of the output through its 4 KB of shared memory (rows of 128 bytes,
@@ -560,6 +627,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
   __shared__ uint64_t full[kStages], empty[kStages], tfull, tempty, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, late_flag;
+  __shared__ __align__(16) float col_ws[256], col_bias[256];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -622,13 +690,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t smem0 = smem_u32(smem);
-      RingPlace at, freed;
-      uint32_t it = 0, slot = 0, tile = 0;  // K steps so far, the next one's slot of scales, tiles so far
+      RingPlace at, freed, scales;
+      uint32_t it = 0, tile = 0;  // K steps so far (up to the slots' number), tiles so far
       bool ok = true;
-      // the slot of a step's scales is read by the products kSlots steps before
+      // a step's operands are there, and the products kSlots steps before have read its slot of scales
       auto peek = [&]() {
-        const bool two = lane == 1 && it >= C::kSlots;
-        return mbar_peek(two ? &empty[freed.stage] : &full[at.stage], two ? freed.parity : at.parity);
+        const bool slot = lane == 1 && it == C::kSlots;
+        return mbar_peek(slot ? &empty[freed.stage] : &full[at.stage], slot ? freed.parity : at.parity);
       };
       bool seen = peek();
       for (int t = pair; ok && t < tiles; t += pairs, ++tile) {
@@ -638,19 +706,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
         for (int kb = 0; kb < num_k; ++kb, products -= 4) {
           if (!__all_sync(0xffffffffu, seen) &&
               (!mbar_wait_warp(&full[at.stage], at.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT) ||
-               (it >= C::kSlots && !mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)))) {
+               (it == C::kSlots && !mbar_wait_warp(&empty[freed.stage], freed.parity, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)))) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t x = smem0 + at.stage * C::kStageBytes;
           const uint32_t sx = x + 2 * 128 * kF4Step;
-          const uint32_t ts = tmem + C::kScales + C::kSlotCols * slot;
+          const uint32_t ts = tmem + C::kScales + C::kSlotCols * scales.stage;
           uint64_t* used = &empty[at.stage];
-          if (it >= C::kSlots) freed.next(kStages);
+          if (it == C::kSlots) freed.next(kStages);
+          else ++it;
           at.next(kStages);
-          slot = slot == C::kSlots - 1 ? 0u : slot + 1;
-          ++it;
+          scales.next(C::kSlots);
           seen = peek();
           if (elect_one()) {
             fp4_step_scales<FORMAT, 2, 2>(sx, sx + C::kScaleBytes, ts, ts + C::kSlotCols / 3);
@@ -668,14 +736,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
     }
   } else if (warp >= 4) {
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    const bool vec = (reinterpret_cast<uintptr_t>(a.ws) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
     uint8_t* buf = smem + kStages * C::kStageBytes + (warp - 4) * 4096;
     uint32_t tile = 0;
+    bool live = true;
     for (int t = pair; t < tiles; t += pairs, ++tile) {
       const int mb = t / num_n, nb = t % num_n;
       const int m_warp = mb * 256 + (int)rank * 128 + quad * 32, m = m_warp + lane;
       const float xs = a.xs && m < a.M ? a.xs[m] : 1.0f;
-      if (!mbar_wait_warp(&tfull, tile & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) break;
+      if (a.ws || a.bias) {  // the tile's columns' scales and bias, while its products run
+        const int i = (int)threadIdx.x - 128, n = nb * 256 + i;
+        const float w = a.ws && n < a.N ? a.ws[n] : 0.0f, b = a.bias && n < a.N ? a.bias[n] : 0.0f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // all warps are done with the last tile's
+        col_ws[i] = w;
+        col_bias[i] = b;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      // a warp that has given up goes on through the tiles, since the others meet it at the barriers above
+      live = live && mbar_wait_warp(&tfull, tile & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
+      if (!live) continue;
       tc_fence_after();
       const bool odd = tile & 1;
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (odd ? (uint32_t)C::kSecond : 0u);
@@ -695,15 +773,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0);
-      fp4_pack_chunk<BF16>(r0, h0, n0 + 64 * first, xs, vec, a);
-      fp4_pack_chunk<BF16>(r1, h1, n0 + 64 * first + 32, xs, vec, a);
+      fp4_pack_chunk<BF16>(r0, h0, xs, col_ws + 64 * first, col_bias + 64 * first, a);
+      fp4_pack_chunk<BF16>(r1, h1, xs, col_ws + 64 * first + 32, col_bias + 64 * first + 32, a);
       fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * first, a);
       if (FORMAT != kNvfp4) tmem_ld32(taddr + 32u * (uint32_t)early, r2);
       tmem_ld32(taddr + 32u * (uint32_t)late, r0);
       tmem_wait_ld_dep(r0);
       reg_barrier32(r2);
-      fp4_pack_chunk<BF16>(r2, h0, n0 + 32 * early, xs, vec, a);
-      fp4_pack_chunk<BF16>(r0, h1, n0 + 32 * late, xs, vec, a);
+      fp4_pack_chunk<BF16>(r2, h0, xs, col_ws + 32 * early, col_bias + 32 * early, a);
+      fp4_pack_chunk<BF16>(r0, h1, xs, col_ws + 32 * late, col_bias + 32 * late, a);
       if (odd) fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * second, a);
       else fp4_put_piece(&tm_out, buf, h1, h0, m_warp, n0 + 64 * second, a);
     }
@@ -723,7 +801,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
 
 // Launch in a cluster of `ctas` (0: as the kernel declares), starting while the kernel before ends
 template <typename... P, typename... A>
-static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int ctas, int threads, size_t smem, cudaStream_t s,
+static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int64_t grid_y, int ctas, int threads, size_t smem, cudaStream_t s,
                               const A&... args) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
@@ -734,7 +812,7 @@ static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int ctas, int 
   attr[1].val.clusterDim.x = (unsigned)ctas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)grid_y);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -762,36 +840,55 @@ static int env(const char* n, int d) { const char* v = getenv(n); return v ? ato
 #endif
 // How a product of few rows is divided: rows of x per tile and CTAs along K
 struct SplitPlan {
-  int tok, split;
+  int tok, log_split;
 };
 static SplitPlan plan_split(int M, int N, int K) {
 #ifdef FORCE
-  if (env("H3B_TOK", 0)) return {env("H3B_TOK", 0), env("H3B_SPLIT", 1)};
+  if (env("H3B_TOK", 0)) return {env("H3B_TOK", 0), __builtin_ctz(env("H3B_SPLIT", 1))};
 #endif
-  const int tok = M <= 16 ? 16 : M <= 64 ? 64 : 128, num_k = (K + 255) / 256;
-  const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + tok - 1) / tok);
-  int split = 1;
-  while (split < 8 && 2 * split <= num_k && tiles * 2 * split <= num_sms()) split *= 2;
-  return {tok, split};
+  const int num_k = (K + 255) / 256, sms = num_sms();
+  const int64_t tiles_n = (N + 127) / 128;
+  // tiles of 64 rows as long as most of them run at once (128 rows, 4,096 -> 4,096: 8.0 us, with
+  // tiles of 128 10.2; 1,024 rows: 23 and 17 us)
+  const int tok = M <= 16 ? 16 : 2 * tiles_n * ((M + 63) / 64) <= 3 * sms ? 64 : 128;
+  const int64_t tiles = tiles_n * ((M + tok - 1) / tok);
+  // K steps that the busiest SM takes, and what adding up costs in steps (48 rows, 16,384 -> 4,096:
+  // one part 20.5 us, four 12.8; 128 rows, 4,096 -> 4,096: one part 8.0 us, two 10.7)
+  const int joining = tok == 16 ? 2 : tok == 64 ? 12 : 24;
+  SplitPlan best{tok, 0};
+  int64_t least = INT64_MAX;
+  for (int l = 0; l <= 3 && 1 << l <= num_k; ++l) {
+    const int64_t cost = ((tiles << l) + sms - 1) / sms * ((num_k + (1 << l) - 1) >> l) + (l ? joining : 0);
+    if (cost < least) {
+      least = cost;
+      best.log_split = l;
+    }
+  }
+  return best;
 }
 template <int FORMAT, int TOK, bool ROWS16>
-static int launch_split(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, int split, cudaStream_t s,
+static int launch_split(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, int log_split, cudaStream_t s,
                         cudaError_t* err) {
   using C = SplitCfg<FORMAT, TOK, ROWS16>;
   CUtensorMap tx, tw, tsx, tsw;
   if (!make_fp4_maps(w, FORMAT, 128, 1, &tw, &tsw)) return 1;
   if (ROWS16) tx = tw, tsx = tsw;  // not used
   else if (!make_fp4_maps(x, FORMAT, TOK, 1, &tx, &tsx)) return 1;
-  const int64_t grid = (int64_t)((a.N + 127) / 128) * ((a.M + TOK - 1) / TOK) * split;
+  const int split = 1 << log_split;
+  const int64_t grid = (int64_t)((a.N + 127) / 128) * split, grid_y = (a.M + TOK - 1) / TOK;
   const int steps = ((a.K + 255) / 256 + split - 1) / split, rest = C::rest_bytes(steps, split);
-  // as many stages as one CTA per SM has room for, or two where there are more CTAs than SMs
-  const int room = grid > num_sms() ? 112 * 1024 : 224 * 1024;
+  // As many stages as one CTA per SM has room for, or two where there are more CTAs than SMs.  Never
+  // so little shared memory that three fit: tensor memory is for two, and a third one that waited for
+  // it could keep the clusters of the other two, or the kernel before, waiting.
+  const int room = (grid * grid_y > num_sms() ? 106 : 220) * 1024;
   int stages = (room - rest) / C::kStageBytes;
   stages = stages < 2 ? 2 : stages > kSplitMaxStages ? kSplitMaxStages : stages;
   if (stages > steps) stages = steps;
+  int smem = stages * C::kStageBytes + rest;
+  if (smem < 80 * 1024) smem = 80 * 1024;
   *err = launch_fp4(a.bf16 ? fp4_split_kernel<FORMAT, TOK, ROWS16, true> : fp4_split_kernel<FORMAT, TOK, ROWS16, false>,
-                    grid, split, kSplitThreads, (size_t)(stages * C::kStageBytes + rest), s, tw, tsw, tx, tsx, a, split,
-                    stages);
+                    grid, grid_y, split, kSplitThreads, (size_t)smem, s, tw, tsw, tx, tsx, a,
+                    log_split, stages);
   return *err == cudaSuccess ? 0 : 2;
 }
 template <int FORMAT>
@@ -809,7 +906,7 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
     return 1;
   const int64_t tiles = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
   const int64_t pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
-  *err = launch_fp4(a.bf16 ? fp4_pair_kernel<FORMAT, true> : fp4_pair_kernel<FORMAT, false>, 2 * pairs, 0,
+  *err = launch_fp4(a.bf16 ? fp4_pair_kernel<FORMAT, true> : fp4_pair_kernel<FORMAT, false>, 2 * pairs, 1, 0,
                     kPairFp4Threads, PairFp4Cfg<FORMAT>::kTotal, s, tx, tw, tsx, tsw, to, b);
   return *err == cudaSuccess ? 0 : 2;
 }
@@ -817,16 +914,18 @@ static bool uses_pair(int M, int N) {
 #ifdef FORCE
   if (env("H3B_PAIR", -1) >= 0) return env("H3B_PAIR", 0);
 #endif
-  return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= num_sms() / 2;
+  // from about half as many tiles as there are pairs of SMs on (1,024 rows, 4,096 -> 4,096, 64 tiles:
+  // 15.8 us and 17.4 by the other kernel; 333 rows, 32 tiles: 11.1 and 10.3)
+  return M > 128 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) > num_sms() / 4;
 }
 template <int FORMAT>
 static int launch_gemm_of(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4GemmArgs& a, cudaStream_t s,
                           cudaError_t* err) {
   if (uses_pair(a.M, a.N)) return launch_pair<FORMAT>(x, w, a, s, err);
   const SplitPlan p = plan_split(a.M, a.N, a.K);
-  return p.tok == 16   ? launch_split<FORMAT, 16, false>(x, w, a, p.split, s, err)
-         : p.tok == 64 ? launch_split<FORMAT, 64, false>(x, w, a, p.split, s, err)
-                       : launch_split<FORMAT, 128, false>(x, w, a, p.split, s, err);
+  return p.tok == 16   ? launch_split<FORMAT, 16, false>(x, w, a, p.log_split, s, err)
+         : p.tok == 64 ? launch_split<FORMAT, 64, false>(x, w, a, p.log_split, s, err)
+                       : launch_split<FORMAT, 128, false>(x, w, a, p.log_split, s, err);
 }
 
 int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, int format, cudaStream_t s,
@@ -836,10 +935,17 @@ int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, i
   return format == kMxfp4 ? launch_gemm_of<kMxfp4>(x, w, a, s, err) : launch_gemm_of<kNvfp4>(x, w, a, s, err);
 }
 
-bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K) {
+// K steps of a CTA, and the pieces of 512 columns that they make of a row, as a power of two
+static int64_t rows16_steps(int64_t K, int log_split) { return ((K + 255) / 256 + (1 << log_split) - 1) >> log_split; }
+static int rows16_log_segs(int64_t steps) { return steps <= 2 ? 0 : steps <= 4 ? 1 : steps <= 8 ? 2 : 3; }
+bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K, int format) {
   if (M > 16 || uses_pair((int)M, (int)N)) return false;
+#ifdef FORCE
+  if (env("H3B_NOFUSE", 0)) return false;
+#endif
   const SplitPlan p = plan_split((int)M, (int)N, (int)K);
-  return p.tok == 16 && (K + 255) / 256 <= (int64_t)kRows16Steps * p.split;
+  const int64_t steps = rows16_steps(K, p.log_split);
+  return p.tok == 16 && steps <= kRows16Steps && M << rows16_log_segs(steps) <= 4 * rows16_items(format);
 }
 int launch_fp4_gemm_rows16(const uint16_t* x, int64_t x_stride, const Fp4RowsView& w, Fp4GemmArgs a, int format,
                            cudaStream_t s, cudaError_t* err) {
@@ -847,9 +953,10 @@ int launch_fp4_gemm_rows16(const uint16_t* x, int64_t x_stride, const Fp4RowsVie
   a.x16 = x;
   a.x16_stride = x_stride;
   a.x16_vec = a.K % 16 == 0 && rows16(x, a.M > 1 ? x_stride : 0);
-  const int split = plan_split(a.M, a.N, a.K).split;
-  return format == kMxfp4 ? launch_split<kMxfp4, 16, true>({}, w, a, split, s, err)
-                          : launch_split<kNvfp4, 16, true>({}, w, a, split, s, err);
+  const int log_split = plan_split(a.M, a.N, a.K).log_split;
+  a.x16_log_segs = rows16_log_segs(rows16_steps(a.K, log_split));
+  return format == kMxfp4 ? launch_split<kMxfp4, 16, true>({}, w, a, log_split, s, err)
+                          : launch_split<kNvfp4, 16, true>({}, w, a, log_split, s, err);
 }
 
 }  // namespace h3b

@@ -51,9 +51,9 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // of 16.  Otherwise the warp moves its 512 columns together, through `stage`, in words or 16-bit
 // pieces as the row's address allows (a lane's own 16 pieces would be 32 bytes apart from its
 // neighbours': 3,607 rows of 1,044 columns to nvfp4 and back took 34 us that way).
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void load16(const uint16_t* row, int c, int K, uint16_t* stage, float (&v)[16]) {
-  uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+template <bool VEC>
+__device__ __forceinline__ void load16_raw(const uint16_t* row, int c, int K, uint16_t* stage, uint4& a, uint4& b) {
+  a = b = make_uint4(0u, 0u, 0u, 0u);
   if constexpr (VEC) {
     if (c * 16 < K) {
       a = *reinterpret_cast<const uint4*>(row + c * 16);
@@ -83,12 +83,21 @@ __device__ __forceinline__ void load16(const uint16_t* row, int c, int K, uint16
     b = *reinterpret_cast<const uint4*>(stage + lane * 16 + 8);
     __syncwarp();
   }
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float (&v)[16]) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     v[2 * i] = half_to_f32<BF16>((uint16_t)(w[i] & 0xffffu));
     v[2 * i + 1] = half_to_f32<BF16>((uint16_t)(w[i] >> 16));
   }
+}
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void load16(const uint16_t* row, int c, int K, uint16_t* stage, float (&v)[16]) {
+  uint4 a, b;
+  load16_raw<VEC>(row, c, K, stage, a, b);
+  unpack16<BF16>(a, b, v);
 }
 template <bool BF16, bool VEC>
 __device__ __forceinline__ void store16(uint16_t* row, int c, int K, uint16_t* stage, const float (&v)[16]) {
