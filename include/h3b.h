@@ -536,7 +536,7 @@ int h3b_fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias
                  int64_t out_row_stride, void* stream);
 
 /* h3b_fp4_quantize of x [rows, w->cols] into the workspace, then h3b_fp4_gemm; the output
- * has x's type.  workspace: h3b_fp4_linear_workspace_bytes() bytes (0 for few rows, which
+ * has x's type and must not overlap x.  workspace: h3b_fp4_linear_workspace_bytes() bytes (0 for few rows, which
  * the product quantises itself: NULL), 16-byte aligned, not shared by calls on different
  * streams.  The same values either way. */
 int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, const h3b_fp4_rows* w);

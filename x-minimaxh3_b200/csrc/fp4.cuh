@@ -13,6 +13,7 @@
 #pragma once
 
 #include "h3b_common.cuh"
+#include "h3b_packed.cuh"
 #include "streaming.cuh"
 
 namespace h3b {
@@ -125,35 +126,39 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
 // The 16 codes (w) and the block's scale byte of a chunk v, of which the block's absmax has the
 // bits `top`; inv_r: 1 / row scale.
 template <int FORMAT>
-__device__ __forceinline__ uint32_t quantize16(const float (&v)[16], uint32_t top, float inv_r, uint32_t (&w)[2]) {
+__device__ __forceinline__ uint32_t quantize16(const float2 (&v)[8], uint32_t top, float inv_r, uint32_t (&w)[2]) {
   const bool bad = top >= kInfBits;
   uint32_t byte;
   w[0] = w[1] = 0u;
   if constexpr (FORMAT == kMxfp4) {
     byte = bad ? 255u : (uint32_t)max((int)(top >> 23) - 2, 0);
-    const float inv = __uint_as_float((254u - byte) << 23);
+    const float2 inv = splat2(__uint_as_float((254u - byte) << 23));
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) w[j >> 3] |= e2m1x2(__fmul_rn(v[j], inv), __fmul_rn(v[j + 1], inv)) << (4 * (j & 7));
+    for (int j = 0; j < 8; ++j) {
+      const float2 q = mul2(v[j], inv);
+      w[j >> 2] |= e2m1x2(q.x, q.y) << (8 * (j & 3));
+    }
   } else {
     byte = bad ? 0x7Fu : (uint32_t)f32x2_to_e4m3x2(__fdiv_rn(__fmul_rn(__uint_as_float(top), inv_r), 6.0f), 0.0f) & 0xffu;
     const float s = e4m3_to_f32(byte);
-    const float rs = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;  // under a scale of zero: zeros, with their signs
+    const float2 s2 = splat2(s), r2 = splat2(inv_r);
+    const float2 rs2 = splat2(s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f);  // under a scale of zero: zeros, with their signs
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) {
+    for (int j = 0; j < 8; ++j) {
       // the remainder of -0 is 0 and would make the quotient 0: the sign is x's
-      const float q0 = copysignf(div_rn_by(__fmul_rn(v[j], inv_r), s, rs), v[j]);
-      const float q1 = copysignf(div_rn_by(__fmul_rn(v[j + 1], inv_r), s, rs), v[j + 1]);
-      w[j >> 3] |= e2m1x2(q0, q1) << (4 * (j & 7));
+      const float2 q = div2_rn_by(mul2(v[j], r2), s2, rs2);
+      w[j >> 2] |= e2m1x2(copysignf(q.x, v[j].x), copysignf(q.y, v[j].y)) << (8 * (j & 3));
     }
   }
   if (bad) w[0] = w[1] = 0u;
   return byte;
 }
-__device__ __forceinline__ uint32_t absmax16(const float (&v)[16]) {
-  uint32_t top = 0u;
+// bits of the largest magnitude; above infinity's where there is a NaN
+__device__ __forceinline__ uint32_t absmax16(const float2 (&v)[8]) {
+  float m = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-  return top;
+  for (int j = 0; j < 8; ++j) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[j].x), "f"(v[j].y));
+  return __float_as_uint(m) & 0x7FFFFFFFu;
 }
 // The exponent of an nvfp4 row's scale from its absmax's bits: least e with absmax <= 2688 * 2^e =
 // 1.3125 * 2^(11 + e), at least -126; 0 for a row of zeros.

@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kSplitThreads)
         for (int j = 0; j < kItems; ++j) {
           const int item = warp - 3 + 4 * j;
           if (item >= items) break;
-          float v[16];
+          float2 v[8];
           unpack16<BF16>(raw[j][0], raw[j][1], v);
           uint32_t top = absmax16(v);
           if (top >= kInfBits) top = 0u;
@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(kSplitThreads)
         const int item = warp - 3 + 4 * j;
         if (item >= items) break;
         const int r = item >> log_segs, c = (item & ((1 << log_segs) - 1)) * 32 + lane;
-        float v[16], inv_r = 1.0f;
+        float2 v[8];
+        float inv_r = 1.0f;
         unpack16<BF16>(raw[j][0], raw[j][1], v);
         if constexpr (FORMAT == kNvfp4) {
           uint32_t top = 0u;
@@ -654,7 +655,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers are initialised; all 512 columns were taken, so both bases are 0
   tc_fence_after();
-  chain_next();
+  // The kernel after this one is not let in early: where its blocks came onto SMs whose pair was done
+  // first, a norm and its product took 197 us instead of 187 (8,192 rows, 4,096 -> 12,288, mxfp4).
   chain_wait();
   const uint32_t tmem = tmem_slot;
   const uint32_t full0 = mapa_shared(smem_u32(full), 0);
@@ -834,18 +836,11 @@ static bool make_fp4_maps(const Fp4RowsView& v, int format, int box_rows, int bo
                       words * 8, format == kMxfp4 ? 128 : 256, (uint32_t)box_bands, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-#ifdef FORCE
-#include <cstdlib>
-static int env(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#endif
 // How a product of few rows is divided: rows of x per tile and CTAs along K
 struct SplitPlan {
   int tok, log_split;
 };
 static SplitPlan plan_split(int M, int N, int K) {
-#ifdef FORCE
-  if (env("H3B_TOK", 0)) return {env("H3B_TOK", 0), __builtin_ctz(env("H3B_SPLIT", 1))};
-#endif
   const int num_k = (K + 255) / 256, sms = num_sms();
   const int64_t tiles_n = (N + 127) / 128;
   // tiles of 64 rows as long as most of them run at once (128 rows, 4,096 -> 4,096: 8.0 us, with
@@ -858,6 +853,7 @@ static SplitPlan plan_split(int M, int N, int K) {
   SplitPlan best{tok, 0};
   int64_t least = INT64_MAX;
   for (int l = 0; l <= 3 && 1 << l <= num_k; ++l) {
+    if (l && tiles << l > 2 * sms) break;  // more than run at once
     const int64_t cost = ((tiles << l) + sms - 1) / sms * ((num_k + (1 << l) - 1) >> l) + (l ? joining : 0);
     if (cost < least) {
       least = cost;
@@ -899,10 +895,9 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
   // output rows that TMA takes: 16-byte aligned, and so are the steps between them
   CUtensorMap to = tx;
   Fp4GemmArgs b = a;
-  b.out_tma = (a.M == 1 || a.out_stride % 8 == 0) && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  b.out_tma = a.out_stride % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
   if (b.out_tma && !make_tmap_2d(&to, a.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.N, (uint64_t)a.M,
-                                 (uint64_t)(a.M == 1 ? (a.N + 7) / 8 * 8 : a.out_stride) * 2, 64, 32,
-                                 CU_TENSOR_MAP_SWIZZLE_128B))
+                                 (uint64_t)a.out_stride * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
     return 1;
   const int64_t tiles = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
   const int64_t pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
@@ -911,9 +906,6 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
   return *err == cudaSuccess ? 0 : 2;
 }
 static bool uses_pair(int M, int N) {
-#ifdef FORCE
-  if (env("H3B_PAIR", -1) >= 0) return env("H3B_PAIR", 0);
-#endif
   // from about half as many tiles as there are pairs of SMs on (1,024 rows, 4,096 -> 4,096, 64 tiles:
   // 15.8 us and 17.4 by the other kernel; 333 rows, 32 tiles: 11.1 and 10.3)
   return M > 128 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) > num_sms() / 4;
@@ -940,9 +932,6 @@ static int64_t rows16_steps(int64_t K, int log_split) { return ((K + 255) / 256 
 static int rows16_log_segs(int64_t steps) { return steps <= 2 ? 0 : steps <= 4 ? 1 : steps <= 8 ? 2 : 3; }
 bool fp4_takes_rows16(int64_t M, int64_t N, int64_t K, int format) {
   if (M > 16 || uses_pair((int)M, (int)N)) return false;
-#ifdef FORCE
-  if (env("H3B_NOFUSE", 0)) return false;
-#endif
   const SplitPlan p = plan_split((int)M, (int)N, (int)K);
   const int64_t steps = rows16_steps(K, p.log_split);
   return p.tok == 16 && steps <= kRows16Steps && M << rows16_log_segs(steps) <= 4 * rows16_items(format);

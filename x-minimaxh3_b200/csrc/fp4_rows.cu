@@ -85,25 +85,27 @@ __device__ __forceinline__ void load16_raw(const uint16_t* row, int c, int K, ui
   }
 }
 template <bool BF16>
-__device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float (&v)[16]) {
+__device__ __forceinline__ float2 unpack_halves(uint32_t w) {
+  if constexpr (BF16) return unpack_bf16x2(w);
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float2 (&v)[8]) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[2 * i] = half_to_f32<BF16>((uint16_t)(w[i] & 0xffffu));
-    v[2 * i + 1] = half_to_f32<BF16>((uint16_t)(w[i] >> 16));
-  }
+  for (int i = 0; i < 8; ++i) v[i] = unpack_halves<BF16>(w[i]);
 }
 template <bool BF16, bool VEC>
-__device__ __forceinline__ void load16(const uint16_t* row, int c, int K, uint16_t* stage, float (&v)[16]) {
+__device__ __forceinline__ void load16(const uint16_t* row, int c, int K, uint16_t* stage, float2 (&v)[8]) {
   uint4 a, b;
   load16_raw<VEC>(row, c, K, stage, a, b);
   unpack16<BF16>(a, b, v);
 }
 template <bool BF16, bool VEC>
-__device__ __forceinline__ void store16(uint16_t* row, int c, int K, uint16_t* stage, const float (&v)[16]) {
+__device__ __forceinline__ void store16(uint16_t* row, int c, int K, uint16_t* stage, const float2 (&v)[8]) {
   uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = pack_halves<BF16>(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < 8; ++i) w[i] = pack_halves<BF16>(v[i].x, v[i].y);
   const uint4 a = make_uint4(w[0], w[1], w[2], w[3]), b = make_uint4(w[4], w[5], w[6], w[7]);
   if constexpr (VEC) {
     if (c * 16 < K) {
@@ -149,7 +151,7 @@ __device__ __forceinline__ void store16_bytes(uint8_t* row, int c, int K, uint8_
 
 // FORMAT 0: int8.  BLOCK: a row per block, else per warp.  CH chunks per thread.
 template <int FORMAT, bool BF16, bool NORM, bool VEC, bool BLOCK, int CH>
-__global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
+__global__ void __launch_bounds__(512, CH <= 2 ? 2 : 1) fp4_rows_kernel(Fp4RowArgs a) {
   __shared__ uint32_t red[2][32];
   __shared__ __align__(16) uint16_t stages[VEC ? 1 : 16][VEC ? 8 : 512];
   chain_wait();
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
   const int64_t row = BLOCK ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (row >= a.rows) return;  // whole warps of a warp-per-row block
   uint16_t* stage = stages[VEC ? 0 : threadIdx.x >> 5];
-  float v[CH][16];
+  float2 v[CH][8];
 #pragma unroll
   for (int i = 0; i < CH; ++i) load16<BF16, VEC>(a.x + row * a.x_stride, t + i * step, a.K, stage, v[i]);
 
@@ -168,31 +170,36 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
     if (a.res) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        float r[16];
+        float2 r[8];
         load16<BF16, VEC>(a.res + row * a.res_stride, t + i * step, a.K, stage, r);
 #pragma unroll
-        // the sum as it is stored: what a later layer reads is what is normed here
-        for (int j = 0; j < 16; ++j) v[i][j] = half_to_f32<BF16>(f32_to_half_bits<BF16>(__fadd_rn(v[i][j], r[j])));
+        for (int j = 0; j < 8; ++j) {  // the sum as it is stored: what a later layer reads is what is normed here
+          const float2 h = add2(v[i][j], r[j]);
+          v[i][j] = unpack_halves<BF16>(pack_halves<BF16>(h.x, h.y));
+        }
       }
 #pragma unroll
       for (int i = 0; i < CH; ++i) store16<BF16, VEC>(a.sum + row * a.sum_stride, t + i * step, a.K, stage, v[i]);
     }
-    float ss = 0.0f;
+    float2 ss2 = splat2(0.0f);
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+      for (int j = 0; j < 8; ++j) ss2 = fma2(v[i][j], v[i][j], ss2);
+    float ss = __fadd_rn(ss2.x, ss2.y);
     ss = row_sum<BLOCK>(ss, reinterpret_cast<float*>(red[0]));
     const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.K), a.eps)));
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = t + i * step;
-      float w[16];
+      float2 w[8];
       load16<BF16, VEC>(a.norm_w, c, a.K, stage, w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        v[i][j] = __fmul_rn(__fmul_rn(v[i][j], inv), w[j]);
-        if (!(VEC ? c * 16 < a.K : c * 16 + j < a.K)) v[i][j] = 0.0f;  // beyond K inv may have made a zero NaN
+      for (int j = 0; j < 8; ++j) {
+        v[i][j] = mul2(mul2(v[i][j], splat2(inv)), w[j]);
+        // beyond K inv may have made a zero NaN
+        if (!(VEC ? c * 16 < a.K : c * 16 + 2 * j < a.K)) v[i][j].x = 0.0f;
+        if (!(VEC ? c * 16 < a.K : c * 16 + 2 * j + 1 < a.K)) v[i][j].y = 0.0f;
       }
     }
   }
@@ -217,9 +224,11 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(Fp4RowArgs a) {
     for (int i = 0; i < CH; ++i) {
       uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float q = some ? div_rn_by(v[i][j], scale, rs) : 0.0f;  // at most 127 and an fp32 rounding
-        w[j >> 2] |= ((uint32_t)__float2int_rn(q) & 0xffu) << (8 * (j & 3));
+      for (int j = 0; j < 8; ++j) {
+        // at most 127 and an fp32 rounding; rounded by adding 1.5 * 2^23, whose low byte is then the code
+        const float2 q = some ? div2_rn_by(v[i][j], splat2(scale), splat2(rs)) : splat2(0.0f);
+        const float2 n = add2(q, splat2(12582912.0f));
+        w[j >> 1] |= (__byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040) & 0xffffu) << (16 * (j & 1));
       }
       store16_bytes<VEC>(a.codes + row * (int64_t)a.K, t + i * step, a.K, reinterpret_cast<uint8_t*>(stage), w);
     }
@@ -265,7 +274,7 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint
   const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)at / parts) : at / parts;
   const int c = (int)(at - row * parts) * 32 + lane;
   const bool live = c * 16 < a.K;
-  float v[16] = {};
+  float2 v[8] = {};
   if (live) {
     const uint2 q = *reinterpret_cast<const uint2*>(a.codes + row * fp4_pitch(a.K) + c * 8);
     const int b = c * 16 / fp4_block(FORMAT);
@@ -274,18 +283,19 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint
     const float s = FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte);
     const float r = a.row_scales ? a.row_scales[row] : 1.0f;
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const uint32_t pair = ((j < 8 ? q.x : q.y) >> (4 * (j & 7))) & 0xffu;
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t pair = ((j < 4 ? q.x : q.y) >> (8 * (j & 3))) & 0xffu;
       uint32_t h2;
       asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h2) : "r"(pair));
-      v[j] = __fmul_rn(__fmul_rn(__half2float(__ushort_as_half((uint16_t)(h2 & 0xffffu))), s), r);
-      v[j + 1] = __fmul_rn(__fmul_rn(__half2float(__ushort_as_half((uint16_t)(h2 >> 16))), s), r);
+      v[j] = mul2(mul2(unpack_halves<false>(h2), splat2(s)), splat2(r));
     }
   }
   store16<BF16, VEC>(out + row * out_stride, c, a.K, stages[VEC ? 0 : threadIdx.x >> 5], v);
 }
 
 // ------------------------------------------------------------------ host side
+
+int num_sms();
 
 static bool rows16(const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
 
@@ -298,7 +308,10 @@ static cudaError_t launch_rows(const Fp4RowArgs& a, cudaStream_t s) {
     return chunks <= 32 ? launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, false, 1>, grid, 256, 0, s, a)
                         : launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, false, 2>, grid, 256, 0, s, a);
   }
-  const int ch = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
+  // Two chunks a thread where there are rows for all SMs: fewer warps meet for a row's sum (8,192 x 4,096
+  // normed into nvfp4 49.1 -> 42.9 us, from 16-bit rows 24.6 -> 21.9); one for a few rows (1 x 4,096 into
+  // INT8 2.8 us, with two 3.2).
+  const int ch = chunks > 1024 ? 4 : chunks > 512 || a.rows >= 4 * num_sms() ? 2 : 1;
   const int threads = ((chunks + ch - 1) / ch + 31) / 32 * 32;
   return ch == 1   ? launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, true, 1>, a.rows, threads, 0, s, a)
          : ch == 2 ? launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, true, 2>, a.rows, threads, 0, s, a)

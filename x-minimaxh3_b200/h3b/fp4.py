@@ -166,24 +166,32 @@ class Fp4Rows:
         return b[: self.rows, : -(-self.cols // BLOCK[self.format])].contiguous()
 
 
-def _half_rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """[..., K] as fp16 / bf16 rows [M, K] of unit column stride; copied where they do not lie so."""
+def _half_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
+    """[..., K] as fp16 / bf16 rows of unit column stride (copied where they do not lie so): the tensor, the number
+    of rows, K and the elements between rows (of a single row, whose stride may be anything, its length)."""
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} must be bfloat16 or float16")
     shape = x.shape
     if not shape or shape[-1] == 0:
         raise ValueError(f"{what} must have at least one column")
+    k = shape[-1]
+    if x.is_contiguous():
+        return x, (shape[0] if len(shape) == 2 else math.prod(shape[:-1])), k, k
     if len(shape) != 2:
-        x = x.reshape(math.prod(shape[:-1]), shape[-1])
-    if not x.is_contiguous() and (x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.reshape(math.prod(shape[:-1]), k)
+    if k > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < k:
         x = x.contiguous()
-    return x
+    return x, x.shape[0], k, x.stride(0) if x.shape[0] > 1 else k
 
 
-def _row_step(x: torch.Tensor) -> int:
-    """Elements between x's rows (of a single row, whose stride may be anything, its length)."""
-    rows, cols = x.shape
-    return x.stride(0) if rows > 1 else cols
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from a's first to its last element and that of b have bytes in common."""
+    spans = []
+    for t in (a, b):
+        if t.numel() == 0:
+            return False
+        spans.append((t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()))
+    return spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]
 
 
 def _gpu_of(x: torch.Tensor, name: str) -> int:
@@ -207,11 +215,10 @@ def quantize_fp4(x: torch.Tensor, format: str = "nvfp4") -> Fp4Rows:
     """Rows x [..., K] (bf16 or fp16) to 4-bit floats [M, K]."""
     gpu = _gpu_of(x, "quantize_fp4")
     _format(format)
-    x = _half_rows(x, "x")
-    m, k = x.shape
+    x, m, k, step = _half_rows(x, "x")
     _row_length(k)
     out = Fp4Rows._room(m, k, format, x)
-    check(lib().h3b_fp4_quantize(x.data_ptr(), _DTYPES[x.dtype], _row_step(x), out._ref, _stream(gpu)), "fp4_quantize")
+    check(lib().h3b_fp4_quantize(x.data_ptr(), _DTYPES[x.dtype], step, out._ref, _stream(gpu)), "fp4_quantize")
     return out
 
 
@@ -219,9 +226,11 @@ def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, gpu:
     """The step between the rows of a caller's output."""
     if out.shape != (rows, cols) or out.dtype is not dtype or out.get_device() != gpu:
         raise ValueError(f"out must be {dtype} [{rows}, {cols}] on the operands' GPU")
+    if out.is_contiguous():
+        return cols
     if cols > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < cols:
         raise ValueError("out must have unit column stride and rows apart from each other")
-    return _row_step(out)
+    return out.stride(0) if rows > 1 else cols
 
 
 def dequantize_fp4(rows: Fp4Rows, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -275,20 +284,22 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] (bf16 or fp16), quantised to the weight's format, times weight [N, K]^T, + bias -> x's type [..., N].
 
-    out: rows [M, N] that receive the result.  workspace: uint8, reused by calls on one stream."""
+    out: rows [M, N] that receive the result, apart from x.  workspace: uint8, reused by calls on one stream."""
     gpu = _gpu_of(x, "fp4_linear")
     if weight._gpu != gpu:
         raise ValueError("all tensors must be on one GPU")
     shape, k, n = x.shape, weight.cols, weight.rows
     if not shape or shape[-1] != k:
         raise ValueError(f"Input and weight inner dimensions must match, got {shape[-1] if shape else 0} and {k}")
-    x = _half_rows(x, "x")
+    x, m, k, x_step = _half_rows(x, "x")
     _row_length(k)
-    m, step = x.shape[0], n
+    step = n
     bias = _bias(bias, n, gpu)
     given = out is not None
     if given:
         step = _check_out(out, m, n, x.dtype, gpu)
+        if _overlap(out, x):
+            raise ValueError("out must not overlap x")
     else:
         out = x.new_empty((m, n))
     library = lib()
@@ -301,7 +312,7 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
               or not workspace.is_contiguous() or workspace.data_ptr() % 16):
             raise ValueError(f"the workspace must have {need} contiguous, 16-byte aligned bytes on the operands' GPU")
         at = workspace.data_ptr()
-    check(library.h3b_fp4_linear(x.data_ptr(), _DTYPES[x.dtype], m, _row_step(x), weight._ref, _ptr(bias),
+    check(library.h3b_fp4_linear(x.data_ptr(), _DTYPES[x.dtype], m, x_step, weight._ref, _ptr(bias),
                                  out.data_ptr(), step, at, need, _stream(gpu)), "fp4_linear")
     return out if given or len(shape) == 2 else out.view(*shape[:-1], n)
 
@@ -318,34 +329,39 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
     int8 = to == "int8"
     if not int8:
         _format(to)
-    shape, dtype = x.shape, x.dtype
-    if weight.dtype is not dtype or not shape or weight.shape != shape[-1:]:
+    rows, m, k, step = _half_rows(x, "x")
+    _row_length(k)
+    dtype = x.dtype
+    if weight.dtype is not dtype or weight.ndim != 1 or weight.shape[0] != k:
         raise ValueError("weight must be a vector of x's type with an entry for each column")
     if not 0.0 <= eps <= _FLOAT_MAX:
         raise ValueError("eps must be finite and not negative")
-    if residual is None and out is not None:
-        raise ValueError("without a residual there is no sum to write")
-    _on(gpu, residual, weight, out)
-    rows = _half_rows(x, "x")
-    m, k = rows.shape
-    _row_length(k)
+    if weight.get_device() != gpu:
+        raise ValueError("all tensors must be on one GPU")
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    h, res, res_step, sum_at, sum_step = x, None, 0, None, 0
+    h, res, res_at, res_step, sum_at, sum_step = x, None, None, 0, None, 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype is not dtype:
-            raise ValueError("residual must have x's shape and type")
-        res = _half_rows(residual, "residual")
-        res_step = _row_step(res)
+        shape = x.shape
+        if residual.shape != shape or residual.dtype is not dtype or residual.get_device() != gpu:
+            raise ValueError("residual must have x's shape and type, on its GPU")
+        res, _, _, res_step = _half_rows(residual, "residual")
+        res_at, sum_step = res.data_ptr(), k
         if out is None:
             h = x.new_empty(shape)
-            sum_at, sum_step = h.data_ptr(), k
         else:
-            if out.shape != shape:
-                raise ValueError("out must have x's shape")
+            if out.shape != shape or out.dtype is not dtype or out.get_device() != gpu:
+                raise ValueError("out must have x's shape and type, on its GPU")
             h = out
-            sum_at, sum_step = out.data_ptr(), _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
-    args = (rows.data_ptr(), _row_step(rows), _ptr(res), res_step, sum_at, sum_step, weight.data_ptr(), _DTYPES[dtype])
+            for t in (x, residual, weight):
+                if _overlap(out, t) and (out.data_ptr() != t.data_ptr() or out.shape != t.shape or out.stride() != t.stride()):
+                    raise ValueError("out may be x or residual, and must not overlap them or the weight otherwise")
+            if not out.is_contiguous():
+                sum_step = _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
+        sum_at = h.data_ptr()
+    elif out is not None:
+        raise ValueError("without a residual there is no sum to write")
+    args = (rows.data_ptr(), step, res_at, res_step, sum_at, sum_step, weight.data_ptr(), _DTYPES[dtype])
     if int8:
         q, scales = x.new_empty((m, k), dtype=torch.int8), x.new_empty((m, 1), dtype=torch.float32)
         check(lib().h3b_add_rms_norm_int8(*args, m, k, eps, q.data_ptr(), scales.data_ptr(), _stream(gpu)),
