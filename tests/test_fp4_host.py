@@ -3,6 +3,7 @@
 import ctypes
 import os
 import re
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -111,6 +112,55 @@ def test_host_tensors_are_refused():
                                      "mxfp4")):
         with pytest.raises(RuntimeError, match="only (on )?CUDA tensors"):
             call()
+
+
+def _on(gpu, shape, dtype=torch.bfloat16):
+    x = torch.zeros(shape, dtype=dtype)
+    return SimpleNamespace(get_device=lambda: gpu, is_cuda=gpu >= 0, shape=x.shape, ndim=x.ndim, dtype=dtype,
+                           stride=x.stride, data_ptr=lambda: 4096, is_contiguous=lambda: True, numel=x.numel,
+                           element_size=x.element_size, new_empty=x.new_empty)
+
+
+def _rows_on(gpu, other=None):
+    u8 = torch.uint8
+    return h3b.Fp4Rows(_on(gpu, (4, 32), u8), _on(gpu if other is None else other, (1, 1, 512), u8), 64, "nvfp4",
+                       _on(gpu, (4,), torch.float32))
+
+
+@pytest.mark.parametrize("gpu", [1, -1])  # -1: not a GPU's
+def test_tensors_of_another_gpu_are_refused(gpu):
+    x, w, norm = _on(0, (2, 64)), _rows_on(0), _on(0, (64,))
+    other = _on(gpu, (2, 64))
+    for call in (lambda: _rows_on(0, gpu), lambda: h3b.fp4_linear(other, w), lambda: h3b.fp4_linear(x, w, _on(gpu, (4,))),
+                 lambda: h3b.fp4_linear(x, w, out=_on(gpu, (2, 4))),
+                 lambda: h3b.fp4_linear_prequantized(w, w, _on(gpu, (4,))),
+                 lambda: h3b.fp4_linear_prequantized(w, w, out=_on(gpu, (4, 4))),
+                 lambda: h3b.dequantize_fp4(w, out=_on(gpu, (4, 64))),
+                 lambda: h3b.add_rms_norm_quantize(x, other, norm), lambda: h3b.add_rms_norm_quantize(other, x, norm),
+                 lambda: h3b.add_rms_norm_quantize(x, x, _on(gpu, (64,))),
+                 lambda: h3b.add_rms_norm_quantize(x, x, norm, out=other)):
+        with pytest.raises((ValueError, RuntimeError), match="GPU|CUDA"):
+            call()
+    if gpu == 1:
+        with pytest.raises(ValueError, match="one GPU"):
+            h3b.fp4_linear_prequantized(w, _rows_on(1))
+
+
+def test_calls_on_another_gpu_than_the_current_one_are_refused(monkeypatch):
+    from h3b import cache
+    monkeypatch.setattr(cache, "_current_gpu", lambda: 1)
+    w = _rows_on(0)
+    for call in (lambda: h3b.fp4_linear_prequantized(w, w, out=_on(0, (4, 4))),
+                 lambda: h3b.dequantize_fp4(w, out=_on(0, (4, 64)))):
+        with pytest.raises(RuntimeError, match="the current device is cuda:1"):
+            call()
+
+
+def test_overlaps_are_found():
+    from h3b.fp4 import _overlap
+    x = torch.zeros(10, 8)
+    assert _overlap(x, x) and _overlap(x[2:4], x[3:]) and _overlap(x[:, :2], x[:, 4:])  # spans, not elements
+    assert not _overlap(x[:2], x[2:]) and not _overlap(x, torch.zeros(3)) and not _overlap(x[:0], x)
 
 
 def test_the_64_bit_form_on_known_values():

@@ -173,7 +173,8 @@ def test_blocks_from_elsewhere(h3b, fmt):
 
 SMALL = [(1, 1, 1), (1, 128, 64), (2, 7, 31), (3, 129, 32), (15, 64, 65), (16, 130, 256), (17, 127, 257), (33, 1003, 96),
          (64, 256, 1056), (65, 128, 100), (128, 384, 512), (129, 100, 4096), (257, 65, 2080), (300, 1003, 1041),
-         (1, 4096, 4096), (8, 512, 16384), (5, 12288, 320), (16, 40000, 64)]
+         (1, 4096, 4096), (8, 512, 16384), (5, 12288, 320), (16, 40000, 64), (5, 30000, 4160), (100, 30000, 1100),
+         (60, 30000, 1100), (300, 4500, 1100), (1, 24000, 260), (40, 300, 5000)]
 LARGE = [(2300, 2050, 32), (2304, 2304, 257), (2301, 2051, 1056), (256, 18950, 100), (19000, 250, 640), (1300, 4096, 4096)]
 
 
@@ -316,6 +317,52 @@ def test_linear_takes_leading_dimensions_and_no_rows(h3b, fmt):
     assert torch.equal(out, want.repeat(10, 1)) and (ws[need:] == 0x5A).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 8, 9, 16, 17])
+@pytest.mark.parametrize("n,k", [(96, 200), (4096, 1024), (300, 4096), (12288, 4096)])
+def test_few_rows_of_any_step_and_address(h3b, fmt, m, n, k):
+    """The product that quantises its rows itself, and the one behind a kernel that does, give what the two
+    calls give; infinities and NaN in x stay in their rows."""
+    base = _rows(m + 1, k + 24, torch.bfloat16, seed=m, spread=1.0)
+    w = h3b.quantize_fp4(_rows(n, k, torch.bfloat16, seed=n, spread=0.3), fmt)
+    bias = torch.randn(n, device="cuda")
+    for x in (base[1:, 8: k + 8], base[1:, 1: k + 1], base[:m, : k].contiguous(), base[1:, 2: k + 2]):
+        want = h3b.fp4_linear_prequantized(h3b.quantize_fp4(x, fmt), w, bias)
+        assert torch.equal(h3b.fp4_linear(x, w, bias), want)
+    x = base[1:, :k].clone()
+    x[m // 2, k // 3], x[0, k - 1] = float("nan"), float("inf")
+    got, want = h3b.fp4_linear(x, w), h3b.fp4_linear_prequantized(h3b.quantize_fp4(x, fmt), w)
+    lost = torch.zeros(m, device="cuda", dtype=torch.bool)
+    lost[m // 2] = lost[0] = True
+    assert torch.equal(torch.isnan(got).all(1), lost) and torch.equal(got[~lost], want[~lost])
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+@pytest.mark.parametrize("m", [40, 700])
+def test_graphs_that_share_a_workspace(h3b, m):
+    """Two captured calls with one workspace, replayed one after the other on a stream, in either order."""
+    k, n = 1024, 768
+    w = [h3b.quantize_fp4(_rows(n, k, torch.bfloat16, seed=s, spread=0.3), "nvfp4") for s in (1, 2)]
+    x = [_rows(m, k, torch.bfloat16, seed=s) for s in (3, 4)]
+    ws = torch.empty(h3b.lib().h3b_fp4_linear_workspace_bytes(m, w[0]._ref), device="cuda", dtype=torch.uint8)
+    graphs, outs = [], []
+    for i in range(2):
+        h3b.fp4_linear(x[i], w[i], workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(h3b.fp4_linear(x[i], w[i], workspace=ws))
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (1, 1, 0)):
+        for i in range(2):
+            x[i].copy_(torch.randn(m, k, device="cuda"))
+        want = [h3b.fp4_linear(x[i], w[i]) for i in range(2)]
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i]) for i in set(order))
+
+
 @pytest.mark.parametrize("m", [1, 40, 2300])
 def test_same_sums_every_time(h3b, m):
     x = _rows(m, 2048, torch.bfloat16, seed=8)
@@ -385,6 +432,7 @@ def test_refusals_on_the_gpu(h3b):
         lambda: h3b.fp4_linear(x.repeat(10, 1), q, workspace=torch.empty(16, device="cuda", dtype=torch.uint8)),
         lambda: h3b.fp4_linear(x.repeat(10, 1), q, workspace=torch.empty(1 << 16, device="cuda", dtype=torch.uint8)[1:]),
         lambda: h3b.fp4_linear(x, q, torch.zeros(4)),
+        lambda: h3b.fp4_linear(x, q, out=x[:, :4]),
         lambda: h3b.Fp4Rows(q.codes, q.scales, 65, "mxfp4"),
         lambda: h3b.Fp4Rows(q.codes, q.scales, 64, "nvfp4x"),
         lambda: h3b.Fp4Rows(q.codes, q.scales[:, :, :256], 64, "mxfp4"),

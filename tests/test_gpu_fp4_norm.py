@@ -146,6 +146,7 @@ def test_rows_of_zeros_and_of_no_number(h3b):
 
 def test_refusals(h3b):
     x, r, w = _inputs(4, 64, torch.bfloat16)
+    both = torch.zeros(5, 64, device="cuda", dtype=torch.bfloat16)
     for call in (lambda: h3b.add_rms_norm_quantize(x, r, w, to="int4"),
                  lambda: h3b.add_rms_norm_quantize(x, r[:3], w),
                  lambda: h3b.add_rms_norm_quantize(x, r.half(), w),
@@ -156,6 +157,8 @@ def test_refusals(h3b):
                  lambda: h3b.add_rms_norm_quantize(x, r, w, eps=float("nan")),
                  lambda: h3b.add_rms_norm_quantize(x, None, w, out=r),
                  lambda: h3b.add_rms_norm_quantize(x, r, w, out=r[:, :32]),
+                 lambda: h3b.add_rms_norm_quantize(both[:4], r, w, out=both[1:]),
+                 lambda: h3b.add_rms_norm_quantize(x, both[:4], w, out=both[1:]),
                  lambda: h3b.add_rms_norm_quantize(x, r, w, out=torch.empty(64, 4, device="cuda", dtype=torch.bfloat16).T)):
         with pytest.raises(ValueError):
             call()
