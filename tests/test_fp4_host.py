@@ -157,10 +157,13 @@ def test_calls_on_another_gpu_than_the_current_one_are_refused(monkeypatch):
 
 
 def test_overlaps_are_found():
-    from h3b.fp4 import _overlap
-    x = torch.zeros(10, 8)
-    assert _overlap(x, x) and _overlap(x[2:4], x[3:]) and _overlap(x[:, :2], x[:, 4:])  # spans, not elements
-    assert not _overlap(x[:2], x[2:]) and not _overlap(x, torch.zeros(3)) and not _overlap(x[:0], x)
+    from h3b.fp4 import _meet
+    rows = lambda at, step, cols, n=3: [set(range(at + 2 * step * r, at + 2 * (step * r + cols))) for r in range(n)]
+    for a, b in (((100, 8, 8), (100, 8, 8)), ((100, 8, 8), (146, 8, 8)), ((100, 8, 8), (148, 8, 8)), ((148, 8, 8), (100, 8, 8)),
+                 ((100, 8, 8), (52, 8, 8)), ((100, 8, 8), (54, 8, 8)), ((100, 0, 8), (116, 8, 8)), ((100, 0, 8), (114, 8, 8))):
+        spans = [range(min(min(r) for r in rows(*t)), max(max(r) for r in rows(*t)) + 1) for t in (a, b)]
+        want = spans[0].start < spans[1].stop and spans[1].start < spans[0].stop
+        assert _meet(*a, *b, 3) == want, (a, b)
 
 
 def test_the_64_bit_form_on_known_values():

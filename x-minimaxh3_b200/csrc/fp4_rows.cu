@@ -260,8 +260,16 @@ __global__ void __launch_bounds__(512, CH <= 2 ? 2 : 1) fp4_rows_kernel(Fp4RowAr
   }
 }
 
-// Codes and scales to 16-bit values: a warp takes 512 columns of a row, a thread 16.
-// value = code * block scale * row scale
+// A code pair to its two elements
+__device__ __forceinline__ float2 elements_of(uint32_t pair) {
+  uint32_t h2;
+  asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h2) : "r"(pair));
+  return unpack_halves<false>(h2);
+}
+// Codes and scales to 16-bit values: value = code * block scale * row scale.  A warp takes 1,024
+// columns of a row, a thread eight at a time (16 bytes of output, so that a warp's store is 512
+// bytes in a row: 16,384 x 4,096 with 16 columns a thread 33 us), or, where rows do not allow
+// that, 512 columns through shared memory.
 template <int FORMAT, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint16_t* out, int64_t out_stride,
                                                              uint32_t parts, int64_t total) {
@@ -272,25 +280,47 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (at >= total) return;
   const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)at / parts) : at / parts;
-  const int c = (int)(at - row * parts) * 32 + lane;
-  const bool live = c * 16 < a.K;
-  float2 v[8] = {};
-  if (live) {
-    const uint2 q = *reinterpret_cast<const uint2*>(a.codes + row * fp4_pitch(a.K) + c * 8);
-    const int b = c * 16 / fp4_block(FORMAT);
-    const uint32_t byte = a.blocks[((row >> 7) * fp4_groups(a.K, FORMAT) + (b >> 2)) * 512 + (row & 31) * 16 +
-                                   ((row >> 5) & 3) * 4 + (b & 3)];
-    const float s = FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte);
-    const float r = a.row_scales ? a.row_scales[row] : 1.0f;
+  const int part = (int)(at - row * parts);
+  const uint8_t* codes = a.codes + row * fp4_pitch(a.K);
+  const uint8_t* blocks = a.blocks + (row >> 7) * fp4_groups(a.K, FORMAT) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+  auto scale_byte = [&](int column) -> uint32_t {
+    const int b = column / fp4_block(FORMAT);
+    return blocks[(int64_t)(b >> 2) * 512 + (b & 3)];
+  };
+  const float2 r = splat2(a.row_scales ? a.row_scales[row] : 1.0f);
+  if constexpr (VEC) {
+    uint32_t q[4], byte[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t pair = ((j < 4 ? q.x : q.y) >> (8 * (j & 3))) & 0xffu;
-      uint32_t h2;
-      asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h2) : "r"(pair));
-      v[j] = mul2(mul2(unpack_halves<false>(h2), splat2(s)), splat2(r));
+    for (int i = 0; i < 4; ++i) {
+      const int c = part * 1024 + i * 256 + lane * 8;
+      q[i] = c < a.K ? *reinterpret_cast<const uint32_t*>(codes + c / 2) : 0u;
+      byte[i] = c < a.K ? scale_byte(c) : 0u;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = part * 1024 + i * 256 + lane * 8;
+      const float2 s = splat2(FORMAT == kMxfp4 ? e8m0_to_f32(byte[i]) : e4m3_to_f32(byte[i]));
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = mul2(mul2(elements_of((q[i] >> (8 * j)) & 0xffu), s), r);
+        w[j] = pack_halves<BF16>(v.x, v.y);
+      }
+      if (c < a.K) *reinterpret_cast<uint4*>(out + row * out_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+    const int c = part * 32 + lane;
+    float2 v[8] = {};
+    if (c * 16 < a.K) {
+      const uint2 q = *reinterpret_cast<const uint2*>(codes + c * 8);
+      const uint32_t byte = scale_byte(c * 16);
+      const float2 s = splat2(FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = mul2(mul2(elements_of(((j < 4 ? q.x : q.y) >> (8 * (j & 3))) & 0xffu), s), r);
+    }
+    store16<BF16, VEC>(out + row * out_stride, c, a.K, stages[threadIdx.x >> 5], v);
   }
-  store16<BF16, VEC>(out + row * out_stride, c, a.K, stages[VEC ? 0 : threadIdx.x >> 5], v);
 }
 
 // ------------------------------------------------------------------ host side
@@ -337,9 +367,9 @@ cudaError_t launch_fp4_rows(const Fp4RowArgs& a, int format, bool bf16, cudaStre
 
 template <int FORMAT>
 static cudaError_t launch_dequantize(const Fp4RowsView& a, uint16_t* out, int64_t stride, bool bf16, cudaStream_t s) {
-  const uint32_t parts = (uint32_t)((a.K + 511) / 512);
-  const int64_t total = a.rows * parts, grid = (total + 7) / 8;
   const bool vec = a.K % 16 == 0 && rows16(out, stride);
+  const uint32_t parts = (uint32_t)(vec ? (a.K + 1023) / 1024 : (a.K + 511) / 512);
+  const int64_t total = a.rows * parts, grid = (total + 7) / 8;
   if (bf16)
     return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, true, true>, grid, 256, 0, s, a, out, stride, parts, total)
                : launch_chained(fp4_dequantize_kernel<FORMAT, true, false>, grid, 256, 0, s, a, out, stride, parts, total);

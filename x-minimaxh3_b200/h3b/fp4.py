@@ -184,14 +184,10 @@ def _half_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]
     return x, x.shape[0], k, x.stride(0) if x.shape[0] > 1 else k
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory from a's first to its last element and that of b have bytes in common."""
-    spans = []
-    for t in (a, b):
-        if t.numel() == 0:
-            return False
-        spans.append((t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()))
-    return spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]
+def _meet(a: int, a_step: int, a_cols: int, b: int, b_step: int, b_cols: int, rows: int) -> bool:
+    """Whether the memory of 16-bit rows at address a and that of rows at b, from the first to the last element,
+    have bytes in common."""
+    return a < b + 2 * ((rows - 1) * b_step + b_cols) and b < a + 2 * ((rows - 1) * a_step + a_cols)
 
 
 def _gpu_of(x: torch.Tensor, name: str) -> int:
@@ -298,7 +294,7 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
     given = out is not None
     if given:
         step = _check_out(out, m, n, x.dtype, gpu)
-        if _overlap(out, x):
+        if m and n and _meet(out.data_ptr(), step, n, x.data_ptr(), x_step, k, m):
             raise ValueError("out must not overlap x")
     else:
         out = x.new_empty((m, n))
@@ -345,7 +341,7 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
         shape = x.shape
         if residual.shape != shape or residual.dtype is not dtype or residual.get_device() != gpu:
             raise ValueError("residual must have x's shape and type, on its GPU")
-        res, _, _, res_step = _half_rows(residual, "residual")
+        res, res_step = (residual, k) if residual.is_contiguous() else _half_rows(residual, "residual")[::3]
         res_at, sum_step = res.data_ptr(), k
         if out is None:
             h = x.new_empty(shape)
@@ -353,12 +349,13 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
             if out.shape != shape or out.dtype is not dtype or out.get_device() != gpu:
                 raise ValueError("out must have x's shape and type, on its GPU")
             h = out
-            for t in (x, residual, weight):
-                if _overlap(out, t) and (out.data_ptr() != t.data_ptr() or out.shape != t.shape or out.stride() != t.stride()):
-                    raise ValueError("out may be x or residual, and must not overlap them or the weight otherwise")
             if not out.is_contiguous():
                 sum_step = _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
         sum_at = h.data_ptr()
+        if out is not None and m:
+            for at, at_step in ((rows.data_ptr(), step), (res_at, res_step), (weight.data_ptr(), 0)):
+                if _meet(sum_at, sum_step, k, at, at_step, k, m) and (at != sum_at or at_step != sum_step):
+                    raise ValueError("out may be x or residual, and must not overlap them or the weight otherwise")
     elif out is not None:
         raise ValueError("without a residual there is no sum to write")
     args = (rows.data_ptr(), step, res_at, res_step, sum_at, sum_step, weight.data_ptr(), _DTYPES[dtype])
