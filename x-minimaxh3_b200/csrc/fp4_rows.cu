@@ -338,10 +338,12 @@ static cudaError_t launch_rows(const Fp4RowArgs& a, cudaStream_t s) {
     return chunks <= 32 ? launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, false, 1>, grid, 256, 0, s, a)
                         : launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, false, 2>, grid, 256, 0, s, a);
   }
-  // Two chunks a thread where there are rows for all SMs: fewer warps meet for a row's sum (8,192 x 4,096
-  // normed into nvfp4 49.1 -> 42.9 us, from 16-bit rows 24.6 -> 21.9); one for a few rows (1 x 4,096 into
-  // INT8 2.8 us, with two 3.2).
-  const int ch = chunks > 1024 ? 4 : chunks > 512 || a.rows >= 4 * num_sms() ? 2 : 1;
+  // Two chunks a thread in long rows where there are some for all SMs: fewer warps meet for a row's
+  // sum (4,000 x 4,096 normed into nvfp4 27.0 -> 21.6 us, from 16-bit rows 13.5 -> 10.7); one for a
+  // few rows (1 x 4,096 into INT8 2.8 us, with two 3.2) and short ones (3,607 x 1,044 into nvfp4 6.2,
+  // with two 7.4).
+  const bool two = a.rows >= 4 * num_sms() && chunks >= (VEC ? 128 : 256);
+  const int ch = chunks > 1024 ? 4 : chunks > 512 || two ? 2 : 1;
   const int threads = ((chunks + ch - 1) / ch + 31) / 32 * 32;
   return ch == 1   ? launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, true, 1>, a.rows, threads, 0, s, a)
          : ch == 2 ? launch_chained(fp4_rows_kernel<FORMAT, BF16, NORM, VEC, true, 2>, a.rows, threads, 0, s, a)
