@@ -32,9 +32,10 @@ def _inputs(m, k, dtype, seed=0):
 
 
 def _normed(h, w, eps):
-    """RMSNorm(h) * w in fp64, and a bound on the relative error of a kernel's fp32 value: each partial sum of
-    squares is off by at most 2^-24 of itself per addition, at most 16 per chunk, 3 for a thread's chunks and 10 in the
-    tree (half of it is left after the root), the quotient, sum, root, reciprocal and two products by one each."""
+    """RMSNorm(h) * w in fp64, and a bound on the relative error of a kernel's fp32 value, in units of 2^-24: a
+    thread's squares are added one after the other, at most 64 of them, then in a tree of 10 levels (half of a sum's
+    error is left after the root); quotient, sum and products are off by one unit at most, and a root and reciprocal of
+    two units of 2^-23 take up what threads of fewer squares leave (the longest chain is 33)."""
     h = h.double()
     y = h / torch.sqrt((h * h).mean(1, keepdim=True) + eps) * w.double()
     return y, ((64 + 10 + 2) / 2 + 6) * 2.0 ** -24

@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(512, CH <= 2 ? 2 : 1) fp4_rows_kernel(Fp4RowAr
       for (int j = 0; j < 8; ++j) ss2 = fma2(v[i][j], v[i][j], ss2);
     float ss = __fadd_rn(ss2.x, ss2.y);
     ss = row_sum<BLOCK>(ss, reinterpret_cast<float*>(red[0]));
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.K), a.eps)));
+    const float inv = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.K), a.eps));  // within 2 ulp, and common to the row
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = t + i * step;
