@@ -78,7 +78,8 @@ struct Fp4GemmArgs {
   int64_t x16_stride;
   int x16_vec;       // they allow 16-byte accesses
   int x16_log_segs;  // pieces of 512 columns that a CTA takes of a row, as a power of two
-  int out_tma;  // set by the launcher: the output rows go out by TMA
+  // set by the launcher: the output rows go out by TMA; tiles of columns that are gone through at a time
+  int out_tma, group;
 };
 // 0 ok, 1 tensor-map encoding failed, 2 CUDA error (*err)
 int launch_fp4_gemm(const Fp4RowsView& x, const Fp4RowsView& w, Fp4GemmArgs a, int format, cudaStream_t s,

@@ -631,15 +631,13 @@ __device__ __forceinline__ void fp4_put_piece(const CUtensorMap* tm_out, uint8_t
   }
 }
 
-// Tile t of a product: eight tiles of columns at a time, all tiles of rows for them, so that the tiles
-// that run at once share the operands of about as many rows as columns (one row of tiles after the
-// other, 8,192 x 12,288 x 4,096 takes 151 us)
+// Tile t of a product: `group` tiles of columns at a time, and for them all tiles of rows
 struct TilePlace {
   int m, n;
 };
-__device__ __forceinline__ TilePlace tile_place(int t, int num_m, int num_n) {
-  const int group = t / (8 * num_m), in = t - group * 8 * num_m, width = min(8, num_n - 8 * group);
-  return {in / width, 8 * group + in % width};
+__device__ __forceinline__ TilePlace tile_place(int t, int num_m, int num_n, int group) {
+  const int g = t / (group * num_m), in = t - g * group * num_m, width = min(group, num_n - group * g);
+  return {in / width, group * g + in % width};
 }
 
 template <int FORMAT, bool BF16>
@@ -692,7 +690,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
     RingPlace fill;
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
-      const auto [mb, nb] = tile_place(t, num_m, num_n);
+      const auto [mb, nb] = tile_place(t, num_m, num_n, a.group);
       for (int kb = 0; kb < num_k; ++kb) {
         if (!mbar_wait_warp(&empty[fill.stage], fill.parity ^ 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT)) { ok = false; break; }
         if (elect_one()) {
@@ -769,7 +767,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
     uint32_t tile = 0;
     bool live = true;
     for (int t = pair; t < tiles; t += pairs, ++tile) {
-      const auto [mb, nb] = tile_place(t, num_m, num_n);
+      const auto [mb, nb] = tile_place(t, num_m, num_n, a.group);
       const int m_warp = mb * 256 + (int)rank * 128 + quad * 32, m = m_warp + lane;
       const float xs = a.xs && m < a.M ? a.xs[m] : 1.0f;
       if (a.ws || a.bias) {  // the tile's columns' scales and bias, while its products run
@@ -927,7 +925,11 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
   if (b.out_tma && !make_tmap_2d(&to, a.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.N, (uint64_t)a.M,
                                  (uint64_t)a.out_stride * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
     return 1;
-  const int64_t tiles = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
+  // Eight tiles of columns at a time, so that the weight is read once and x again for each eight; all of
+  // them where x is the longer operand and the weight stays in L2 (4,096 x 16,384 x 16,384 nvfp4 396 us,
+  // with all columns 490; 16,384 x 4,096 x 16,384 mxfp4 368 and 359).
+  const int64_t num_n = (a.N + 255) / 256, tiles = (int64_t)((a.M + 255) / 256) * num_n;
+  b.group = a.M >= a.N && (int64_t)a.N * fp4_pitch(a.K) <= 48 << 20 ? (int)num_n : 8;
   const int64_t pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
   *err = launch_fp4(a.bf16 ? fp4_pair_kernel<FORMAT, true> : fp4_pair_kernel<FORMAT, false>, 2 * pairs, 1, 0,
                     kPairFp4Threads, PairFp4Cfg<FORMAT>::kTotal, s, tx, tw, tsx, tsw, to, b);
