@@ -156,14 +156,41 @@ def test_calls_on_another_gpu_than_the_current_one_are_refused(monkeypatch):
             call()
 
 
-def test_overlaps_are_found():
-    from h3b.fp4 import _meet
-    rows = lambda at, step, cols, n=3: [set(range(at + 2 * step * r, at + 2 * (step * r + cols))) for r in range(n)]
-    for a, b in (((100, 8, 8), (100, 8, 8)), ((100, 8, 8), (146, 8, 8)), ((100, 8, 8), (148, 8, 8)), ((148, 8, 8), (100, 8, 8)),
-                 ((100, 8, 8), (52, 8, 8)), ((100, 8, 8), (54, 8, 8)), ((100, 0, 8), (116, 8, 8)), ((100, 0, 8), (114, 8, 8))):
-        spans = [range(min(min(r) for r in rows(*t)), max(max(r) for r in rows(*t)) + 1) for t in (a, b)]
-        want = spans[0].start < spans[1].stop and spans[1].start < spans[0].stop
-        assert _meet(*a, *b, 3) == want, (a, b)
+def _at(address, shape, step=None):
+    t = _on(0, shape)
+    t.data_ptr = lambda: address
+    if step is not None and step != shape[-1]:
+        t.stride, t.is_contiguous = (lambda d: (step, 1)[d]), lambda: False
+    return t
+
+
+class _Reached(Exception):
+    pass
+
+
+@pytest.mark.parametrize("at,step,met", [
+    (4096, 64, True), (4096 + 3 * 128, 64, True), (4096 + 4 * 128, 64, False), (4096 - 4 * 128, 64, False),
+    (4096 - 4 * 128 + 2, 64, True), (4096, 72, True), (4096 - 3 * 144 - 128, 72, False), (4096 - 3 * 144 - 126, 72, True)])
+def test_outputs_that_overlap_an_input_are_refused(monkeypatch, at, step, met):
+    """Rows of 64 columns, four of x at 4,096; what is not refused reaches the library."""
+    from h3b import cache, fp4
+
+    def reached():
+        raise _Reached
+    square = h3b.Fp4Rows(_on(0, (64, 32), torch.uint8), _on(0, (1, 1, 512), torch.uint8), 64, "nvfp4")
+    monkeypatch.setattr(cache, "_current_gpu", lambda: 0)
+    monkeypatch.setattr(fp4, "lib", reached)
+    x, out, far = _at(4096, (4, 64)), _at(at, (4, 64), step), _at(1 << 20, (4, 64))
+    with pytest.raises(ValueError if met else _Reached, match="overlap" if met else None):
+        h3b.fp4_linear(x, square, out=out)
+    norm = _at(1 << 21, (64,))
+    same = at == 4096 and step == 64
+    for a, b in ((x, far), (far, x)):
+        with pytest.raises(ValueError if met and not same else _Reached, match="overlap" if met and not same else None):
+            h3b.add_rms_norm_quantize(a, b, norm, out=out)
+    if same:
+        with pytest.raises(ValueError, match="overlap"):
+            h3b.add_rms_norm_quantize(far, far, _at(4096 + 64, (64,)), out=out)
 
 
 def test_the_64_bit_form_on_known_values():

@@ -472,7 +472,8 @@ __global__ void __launch_bounds__(kSplitThreads)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (c + j < toks)
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (uint32_t)(((c + j) << log_share) * 4)), "r"(r[j]) : "memory");
+            asm volatile("st.shared::cluster.b32 [%0], %1;"
+                         ::"r"(to + (uint32_t)(((c + j) << log_share) * 4)), "r"(r[j]) : "memory");
       }
       __syncwarp();
       if (summed && (row & (min(32, share) - 1)) == 0)
@@ -829,8 +830,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
 
 // Launch in a cluster of `ctas` (0: as the kernel declares), starting while the kernel before ends
 template <typename... P, typename... A>
-static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int64_t grid_y, int ctas, int threads, size_t smem, cudaStream_t s,
-                              const A&... args) {
+static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int64_t grid_y, int ctas, int threads, size_t smem,
+                              cudaStream_t s, const A&... args) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];

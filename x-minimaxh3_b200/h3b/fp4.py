@@ -184,12 +184,6 @@ def _half_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]
     return x, x.shape[0], k, x.stride(0) if x.shape[0] > 1 else k
 
 
-def _meet(a: int, a_step: int, a_cols: int, b: int, b_step: int, b_cols: int, rows: int) -> bool:
-    """Whether the memory of 16-bit rows at address a and that of rows at b, from the first to the last element,
-    have bytes in common."""
-    return a < b + 2 * ((rows - 1) * b_step + b_cols) and b < a + 2 * ((rows - 1) * a_step + a_cols)
-
-
 def _gpu_of(x: torch.Tensor, name: str) -> int:
     if not x.is_cuda:
         raise RuntimeError(f"{name} runs only on CUDA tensors (the B200 library has no CPU path)")
@@ -294,7 +288,8 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
     given = out is not None
     if given:
         step = _check_out(out, m, n, x.dtype, gpu)
-        if m and n and _meet(out.data_ptr(), step, n, x.data_ptr(), x_step, k, m):
+        at, x_at = out.data_ptr(), x.data_ptr()
+        if m and n and at < x_at + 2 * ((m - 1) * x_step + k) and x_at < at + 2 * ((m - 1) * step + n):
             raise ValueError("out must not overlap x")
     else:
         out = x.new_empty((m, n))
@@ -336,29 +331,33 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
         raise ValueError("all tensors must be on one GPU")
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    h, res, res_at, res_step, sum_at, sum_step = x, None, None, 0, None, 0
+    at, w_at = rows.data_ptr(), weight.data_ptr()
+    h, res_at, res_step, sum_at, sum_step = x, None, 0, None, 0
     if residual is not None:
         shape = x.shape
         if residual.shape != shape or residual.dtype is not dtype or residual.get_device() != gpu:
             raise ValueError("residual must have x's shape and type, on its GPU")
-        res, res_step = (residual, k) if residual.is_contiguous() else _half_rows(residual, "residual")[::3]
+        if residual.is_contiguous():
+            res, res_step = residual, k
+        else:
+            res, _, _, res_step = _half_rows(residual, "residual")
         res_at, sum_step = res.data_ptr(), k
         if out is None:
             h = x.new_empty(shape)
+            sum_at = h.data_ptr()
         else:
             if out.shape != shape or out.dtype is not dtype or out.get_device() != gpu:
                 raise ValueError("out must have x's shape and type, on its GPU")
-            h = out
+            h, sum_at = out, out.data_ptr()
             if not out.is_contiguous():
                 sum_step = _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
-        sum_at = h.data_ptr()
-        if out is not None and m:
-            for at, at_step in ((rows.data_ptr(), step), (res_at, res_step), (weight.data_ptr(), 0)):
-                if _meet(sum_at, sum_step, k, at, at_step, k, m) and (at != sum_at or at_step != sum_step):
+            end = sum_at + 2 * ((m - 1) * sum_step + k)
+            for i, i_step in ((at, step), (res_at, res_step), (w_at, 0)):
+                if i < end and sum_at < i + 2 * ((m - 1) * i_step + k) and (i != sum_at or i_step != sum_step) and m:
                     raise ValueError("out may be x or residual, and must not overlap them or the weight otherwise")
     elif out is not None:
         raise ValueError("without a residual there is no sum to write")
-    args = (rows.data_ptr(), step, res_at, res_step, sum_at, sum_step, weight.data_ptr(), _DTYPES[dtype])
+    args = (at, step, res_at, res_step, sum_at, sum_step, w_at, _DTYPES[dtype])
     if int8:
         q, scales = x.new_empty((m, k), dtype=torch.int8), x.new_empty((m, 1), dtype=torch.float32)
         check(lib().h3b_add_rms_norm_int8(*args, m, k, eps, q.data_ptr(), scales.data_ptr(), _stream(gpu)),
