@@ -175,7 +175,8 @@ SMALL = [(1, 1, 1), (1, 128, 64), (2, 7, 31), (3, 129, 32), (15, 64, 65), (16, 1
          (64, 256, 1056), (65, 128, 100), (128, 384, 512), (129, 100, 4096), (257, 65, 2080), (300, 1003, 1041),
          (1, 4096, 4096), (8, 512, 16384), (5, 12288, 320), (16, 40000, 64), (5, 30000, 4160), (100, 30000, 1100),
          (60, 30000, 1100), (300, 4500, 1100), (1, 24000, 260), (40, 300, 5000)]
-LARGE = [(2300, 2050, 32), (2304, 2304, 257), (2301, 2051, 1056), (256, 18950, 100), (19000, 250, 640), (1300, 4096, 4096)]
+LARGE = [(2300, 2050, 32), (10000, 8, 96), (10001, 1, 300), (9900, 72, 64), (2304, 2304, 257),
+         (2301, 2051, 1056), (256, 18950, 100), (19000, 250, 640), (1300, 4096, 4096)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
