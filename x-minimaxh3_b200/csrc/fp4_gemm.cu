@@ -61,9 +61,16 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t sdesc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
 
+// A sum times its row scales.  Of two scales on the same side of 1 the first takes the sum no further
+// than both do, and they follow each other; where one is below 1 and the other is not, their product
+// lies between them and comes first, so that nothing leaves fp32's range on the way to a value in it.
+__device__ __forceinline__ float fp4_scaled(float sum, float xs, float ws) {
+  const bool apart = (fabsf(xs) < 1.0f) != (fabsf(ws) < 1.0f);
+  return __fmul_rn(__fmul_rn(sum, apart ? __fmul_rn(xs, ws) : xs), apart ? 1.0f : ws);
+}
 // A sum to its output value; xs and ws are 1 where there are no row scales
 __device__ __forceinline__ float fp4_finish(float sum, float xs, float ws, float bias, const Fp4GemmArgs& a) {
-  const float v = __fmul_rn(__fmul_rn(sum, xs), ws);
+  const float v = fp4_scaled(sum, xs, ws);
   return a.bias ? __fadd_rn(v, bias) : v;
 }
 
@@ -548,12 +555,23 @@ struct PairFp4Cfg {
 constexpr int kPairFp4Threads = 384;
 
 // 32 columns of a row's sums to 16 bits, two to a word; columns: their scales and biases, four of
-// each in turn, in shared memory, or null where there are none
+// each in turn, in shared memory, or null where there are none.  apart: some row's scale of this warp
+// may lie on the other side of 1 than some column's (fp4_scaled); else the two follow each other.
 template <bool BF16>
 __device__ __forceinline__ void fp4_pack_chunk(const uint32_t (&r)[32], uint32_t (&h)[16], float xs,
-                                               const float4* columns) {
+                                               const float4* columns, bool apart) {
   const float2 x2 = splat2(xs);
-  if (columns) {
+  if (apart) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 w = columns[2 * q], b = columns[2 * q + 1];
+      float z[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] = fp4_scaled(__uint_as_float(r[4 * q + j]), xs, (&w.x)[j]);
+      h[2 * q] = pack_halves<BF16>(__fadd_rn(z[0], b.x), __fadd_rn(z[1], b.y));
+      h[2 * q + 1] = pack_halves<BF16>(__fadd_rn(z[2], b.z), __fadd_rn(z[3], b.w));
+    }
+  } else if (columns) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const float4 w = columns[2 * q], b = columns[2 * q + 1];
@@ -771,6 +789,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
       const auto [mb, nb] = tile_place(t, num_m, num_n, a.group);
       const int m_warp = mb * 256 + (int)rank * 128 + quad * 32, m = m_warp + lane;
       const float xs = a.xs && m < a.M ? a.xs[m] : 1.0f;
+      bool apart = false;
       if (a.ws || a.bias) {  // the tile's columns' scales and bias, while its products run
         const int i = (int)threadIdx.x - 128, n = nb * 256 + i;
         // where there are none, 1 and -0, which change no sum
@@ -778,7 +797,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
         asm volatile("bar.sync 1, 256;" ::: "memory");  // all warps are done with the last tile's
         columns[i >> 2 << 1][i & 3] = w;
         columns[(i >> 2 << 1) + 1][i & 3] = b;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        // how many of the columns' scales are below 1: where none or all are, and this warp's rows' likewise,
+        // the scales need no order of their own
+        uint32_t below;
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.popc.u32 %0, 1, 256, p;\n\t}"
+                     : "=r"(below) : "r"(n < a.N && fabsf(w) < 1.0f ? 1u : 0u) : "memory");
+        const bool row_below = fabsf(xs) < 1.0f;
+        const bool alike = m >= a.M || (row_below ? below == (uint32_t)min(256, a.N - nb * 256) : below == 0u);
+        apart = a.xs && a.ws && !__all_sync(0xffffffffu, alike);
       }
       // a warp that has given up goes on through the tiles, since the others meet it at the barriers above
       live = live && mbar_wait_warp(&tfull, tile & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
@@ -802,15 +828,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0);
-      fp4_pack_chunk<BF16>(r0, h0, xs, cols ? cols + (64 * first) / 2 : nullptr);
-      fp4_pack_chunk<BF16>(r1, h1, xs, cols ? cols + (64 * first + 32) / 2 : nullptr);
+      fp4_pack_chunk<BF16>(r0, h0, xs, cols ? cols + (64 * first) / 2 : nullptr, apart);
+      fp4_pack_chunk<BF16>(r1, h1, xs, cols ? cols + (64 * first + 32) / 2 : nullptr, apart);
       fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * first, a);
       if (FORMAT != kNvfp4) tmem_ld32(taddr + 32u * (uint32_t)early, r2);
       tmem_ld32(taddr + 32u * (uint32_t)late, r0);
       tmem_wait_ld_dep(r0);
       reg_barrier32(r2);
-      fp4_pack_chunk<BF16>(r2, h0, xs, cols ? cols + (32 * early) / 2 : nullptr);
-      fp4_pack_chunk<BF16>(r0, h1, xs, cols ? cols + (32 * late) / 2 : nullptr);
+      fp4_pack_chunk<BF16>(r2, h0, xs, cols ? cols + (32 * early) / 2 : nullptr, apart);
+      fp4_pack_chunk<BF16>(r0, h1, xs, cols ? cols + (32 * late) / 2 : nullptr, apart);
       if (odd) fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * second, a);
       else fp4_put_piece(&tm_out, buf, h1, h0, m_warp, n0 + 64 * second, a);
     }
