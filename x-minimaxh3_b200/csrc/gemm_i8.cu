@@ -792,21 +792,33 @@ EncodeTiledFn get_encode_tiled() {
   return fn;
 }
 
+// A tensor map of `rank` dimensions.  Encoding is a driver call and needs a current context, which a host thread
+// has only once a runtime call of its own has bound the device's: where it fails, that is done, and it is tried again.
+bool encode_tiled(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+                  const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
+  const cuuint32_t steps[3] = {1, 1, 1};
+  EncodeTiledFn fn = get_encode_tiled();
+  if (!fn) return false;
+  auto encode = [&]() {
+    return fn(m, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode()) return true;
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode();
+}
+
 // 2-D byte tensor [rows, cols] with row stride `stride` bytes; box [box_rows, box_cols]
 // with 128-byte swizzle (box_cols * elem must be <= 128).
 bool make_tmap_2d(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t cols,
                   uint64_t rows, uint64_t stride_bytes, uint32_t box_cols, uint32_t box_rows,
                   CUtensorMapSwizzle sw) {
-  EncodeTiledFn fn = get_encode_tiled();
-  if (!fn) return false;
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {stride_bytes};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {stride_bytes};
+  const cuuint32_t box[2] = {box_cols, box_rows};
   (void)elem_bytes;
-  CUresult r = fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode_tiled(m, dt, 2, base, dims, strides, box, sw);
 }
 
 int num_sms() {

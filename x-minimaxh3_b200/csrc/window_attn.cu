@@ -1283,12 +1283,8 @@ bool make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, uint64_t d1, ui
   const cuuint64_t dims[3] = {128, d1, d2};
   const cuuint64_t strides[2] = {stride1, stride2};
   const cuuint32_t box[3] = {64, box1, box2};
-  const cuuint32_t steps[3] = {1, 1, 1};
-  EncodeTiledFn encode = get_encode_tiled();
-  return encode && encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                                const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides,
+                      box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Whether items are cut.  Cutting takes a plan of all items by every CTA, a second launch
