@@ -1,4 +1,4 @@
-"""Calls from host threads: a thread's first one (B200)."""
+"""Calls from host threads: a thread's first one, and one operator from two threads, each on a stream of its own (B200)."""
 
 import threading
 
@@ -17,6 +17,33 @@ def h3b():
     yield h3b
     torch.cuda.synchronize()
     assert h3b.device_status(0) == 0
+
+
+def _at_once(calls, times):
+    """Each call `times` times in a thread of its own; their last results."""
+    errors, last = [], [None] * len(calls)
+    start = threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                torch.zeros(1, device="cuda")
+                start.wait()
+                for _ in range(times):
+                    last[i] = calls[i]()
+                    if errors:
+                        return
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 - told to the thread that asserts
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[0]
+    return last
 
 
 def _first_calls(h3b):
@@ -53,3 +80,28 @@ def test_first_call_of_a_thread(h3b, name):
     torch.cuda.synchronize()
     assert isinstance(got[0], torch.Tensor), got[0]
     assert torch.equal(got[0], want)
+
+
+def _check(calls, times):
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    for got, w in zip(_at_once(calls, times), want):
+        pairs = zip(got, w) if isinstance(w, tuple) else [(got, w)]
+        assert all(torch.equal(a, b) for a, b in pairs)
+
+
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+@pytest.mark.parametrize("m,wide,narrow", [(1, (12288, 4096), (512, 4096)), (24, (4096, 4096), (20000, 256)),
+                                           (100, (2048, 8192), (256, 512))])
+def test_4_bit_linears_of_unequal_size(h3b, fmt, m, wide, narrow):
+    """Calls whose kernels take unequal amounts of shared memory."""
+    calls = []
+    for n, k in (wide, narrow):
+        g = torch.Generator(device="cuda").manual_seed(n)
+        x = torch.randn(m, k, device="cuda", generator=g).bfloat16()
+        w = h3b.quantize_fp4(torch.randn(n, k, device="cuda", generator=g).bfloat16(), fmt)
+        out = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+        need = h3b.lib().h3b_fp4_linear_workspace_bytes(m, w._ref)
+        ws = torch.empty(max(need, 16), device="cuda", dtype=torch.uint8)
+        calls.append(lambda x=x, w=w, out=out, ws=ws: h3b.fp4_linear(x, w, out=out, workspace=ws))
+    _check(calls, 3000)

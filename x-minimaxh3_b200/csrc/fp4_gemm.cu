@@ -8,6 +8,8 @@
 // block scales.  Codes and scales come by TMA into a ring of stages; the scales go on into
 // tensor memory by tcgen05.cp, into one of a few slots: the copy into a slot waits for the
 // products that read it last, and the products of a step for its copies.
+#include <type_traits>
+
 #include "fp4.cuh"
 #include "h3b_kernels.cuh"
 
@@ -154,6 +156,7 @@ struct SplitCfg {
   }
 };
 constexpr int kSplitThreads = 224, kSplitMaxStages = 8;
+constexpr int kSplitMost = 220 * 1024;  // dynamic shared memory of a CTA
 constexpr int kRows16Steps = 16;  // K steps of a CTA that quantises x
 // Pieces of 512 columns of x that one of its four warps holds.  More rows take longer here than in a
 // kernel of their own in front (4,096 -> 4,096, nvfp4: 4 rows 7.2 us in one launch and 6.2 in two, 8 rows
@@ -854,11 +857,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
 
 // ------------------------------------------------------------------ host side
 
-// Launch in a cluster of `ctas` (0: as the kernel declares), starting while the kernel before ends
-template <typename... P, typename... A>
-static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int64_t grid_y, int ctas, int threads, size_t smem,
-                              cudaStream_t s, const A&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+// Launch in a cluster of `ctas` (0: as the kernel declares), starting while the kernel before ends; with
+// `smem` bytes of shared memory, kMost in the kernel's largest call
+template <auto Kernel, int kMost, typename... A>
+static cudaError_t launch_fp4(int64_t grid, int64_t grid_y, int ctas, int threads, size_t smem, cudaStream_t s,
+                              const A&... args) {
+  cudaError_t e = allow_shared_memory<Kernel, kMost>();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -873,7 +877,7 @@ static cudaError_t launch_fp4(void (*kernel)(P...), int64_t grid, int64_t grid_y
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = ctas ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  e = cudaLaunchKernelEx(&cfg, Kernel, args...);
   if (e == cudaSuccess) chained_launches.fetch_add(1, std::memory_order_relaxed);
   return e;
 }
@@ -929,15 +933,18 @@ static int launch_split(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gem
   // As many stages as one CTA per SM has room for, or two where there are more CTAs than SMs.  Never
   // so little shared memory that three fit: tensor memory is for two, and a third one that waited for
   // it could keep the clusters of the other two, or the kernel before, waiting.
-  const int room = (grid * grid_y > num_sms() ? 106 : 220) * 1024;
+  const int room = grid * grid_y > num_sms() ? 106 * 1024 : kSplitMost;
+  static_assert(C::rest_bytes(kRows16Steps, 8) + 2 * C::kStageBytes <= kSplitMost, "two stages always fit");
   int stages = (room - rest) / C::kStageBytes;
   stages = stages < 2 ? 2 : stages > kSplitMaxStages ? kSplitMaxStages : stages;
   if (stages > steps) stages = steps;
   int smem = stages * C::kStageBytes + rest;
   if (smem < 80 * 1024) smem = 80 * 1024;
-  *err = launch_fp4(a.bf16 ? fp4_split_kernel<FORMAT, TOK, ROWS16, true> : fp4_split_kernel<FORMAT, TOK, ROWS16, false>,
-                    grid, grid_y, split, kSplitThreads, (size_t)smem, s, tw, tsw, tx, tsx, a,
-                    log_split, stages);
+  auto launch = [&](auto bf16) {
+    return launch_fp4<fp4_split_kernel<FORMAT, TOK, ROWS16, decltype(bf16)::value>, kSplitMost>(
+        grid, grid_y, split, kSplitThreads, (size_t)smem, s, tw, tsw, tx, tsx, a, log_split, stages);
+  };
+  *err = a.bf16 ? launch(std::true_type{}) : launch(std::false_type{});
   return *err == cudaSuccess ? 0 : 2;
 }
 template <int FORMAT>
@@ -958,8 +965,12 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
   const int64_t num_n = (a.N + 255) / 256, tiles = (int64_t)((a.M + 255) / 256) * num_n;
   b.group = a.M >= a.N && (int64_t)a.N * fp4_pitch(a.K) <= 48 << 20 ? (int)num_n : 8;
   const int64_t pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
-  *err = launch_fp4(a.bf16 ? fp4_pair_kernel<FORMAT, true> : fp4_pair_kernel<FORMAT, false>, 2 * pairs, 1, 0,
-                    kPairFp4Threads, PairFp4Cfg<FORMAT>::kTotal, s, tx, tw, tsx, tsw, to, b);
+  constexpr int kTotal = PairFp4Cfg<FORMAT>::kTotal;
+  auto launch = [&](auto bf16) {
+    return launch_fp4<fp4_pair_kernel<FORMAT, decltype(bf16)::value>, kTotal>(2 * pairs, 1, 0, kPairFp4Threads, kTotal, s,
+                                                                              tx, tw, tsx, tsw, to, b);
+  };
+  *err = a.bf16 ? launch(std::true_type{}) : launch(std::false_type{});
   return *err == cudaSuccess ? 0 : 2;
 }
 static bool uses_pair(int M, int N) {

@@ -2,9 +2,27 @@
 // kernel translation units and the C ABI (capi.cu).
 #pragma once
 
+#include <atomic>
+
 #include "h3b_common.cuh"
 
 namespace h3b {
+
+// Lets Kernel's launches ask for up to kBytes of dynamic shared memory, once per device.  The limit
+// belongs to the kernel, not to a call: one that set it to its own size could do so between another
+// host thread's setting and launch, which would then be refused.
+template <auto Kernel, int kBytes>
+cudaError_t allow_shared_memory() {
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 struct QuantArgs {
   const uint16_t* x;          // bf16 [rows, x_stride]
