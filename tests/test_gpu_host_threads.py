@@ -105,3 +105,33 @@ def test_4_bit_linears_of_unequal_size(h3b, fmt, m, wide, narrow):
         ws = torch.empty(max(need, 16), device="cuda", dtype=torch.uint8)
         calls.append(lambda x=x, w=w, out=out, ws=ws: h3b.fp4_linear(x, w, out=out, workspace=ws))
     _check(calls, 3000)
+
+
+def _entry(h3b, name, *args):
+    """A C entry as its own call: hardly any of a thread's time is spent outside it."""
+    from h3b._lib import check
+    entry, stream = getattr(h3b.lib(), name), lambda: torch.cuda.current_stream().cuda_stream
+    return lambda: check(entry(*args, stream()), name)
+
+
+def test_row_quantisers_of_unequal_width(h3b):
+    calls, results = [], []
+    for k in (16384, 12288):
+        x = torch.randn(2, k, device="cuda").bfloat16()
+        q, s = torch.empty(2, k, device="cuda", dtype=torch.int8), torch.empty(2, 1, device="cuda")
+        call = _entry(h3b, "h3b_quantize_int8_rowwise", x.data_ptr(), 2, k, k, q.data_ptr(), s.data_ptr())
+        calls.append(lambda call=call, keep=x, out=(q, s): (call(), out)[1])
+    _check(calls, 20000)
+
+
+def test_block_masks_of_unequal_length(h3b):
+    from h3b import attention as A
+    calls = []
+    for blocks in (2000, 10):
+        g = torch.Generator(device="cuda").manual_seed(blocks)
+        pooled = lambda n: torch.randn(1, n, 128, device="cuda", generator=g).bfloat16()
+        same = lambda n: torch.ones(1, n, device="cuda", dtype=torch.uint8)
+        q = A.PreparedBlocks(pooled(2), same(2), None, None, 256, 128, 256)
+        k = A.PreparedBlocks(pooled(blocks), same(blocks), None, None, 64 * blocks, 64, 64 * blocks)
+        calls.append(lambda q=q, k=k: A.block_mask(q, k, A.MaskConfig("topk", 0.3)))
+    _check(calls, 10000)

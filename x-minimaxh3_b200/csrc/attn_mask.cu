@@ -366,16 +366,16 @@ __global__ void __launch_bounds__(128) bitmap_to_lut_kernel(const uint32_t* __re
   if (lane == 0) valid[row] = n;
 }
 
-static size_t mask_smem_bytes(int64_t Kb, int rows) {
+static constexpr size_t mask_smem_bytes(int64_t Kb, int rows) {
   return rows * 128 * sizeof(float) + rows * 256 * sizeof(uint32_t) + rows * 256 * sizeof(unsigned long long) +
          rows * (size_t)Kb * sizeof(uint16_t);
 }
 
-template <int ROWS>
+// kMost: the most key blocks of a call
+template <int ROWS, int kMost>
 static cudaError_t launch_block_mask_rows(const MaskArgs& a, int64_t H, cudaStream_t s) {
   const size_t smem = mask_smem_bytes(a.Kb, ROWS);
-  cudaError_t e =
-      cudaFuncSetAttribute(block_mask_kernel<ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_shared_memory<block_mask_kernel<ROWS>, (int)mask_smem_bytes(kMost, ROWS)>();
   if (e != cudaSuccess) return e;
   dim3 grid((unsigned)((a.Qb + ROWS - 1) / ROWS), (unsigned)H);
   block_mask_kernel<ROWS><<<grid, kMaskThreads, smem, s>>>(a);
@@ -383,7 +383,7 @@ static cudaError_t launch_block_mask_rows(const MaskArgs& a, int64_t H, cudaStre
 }
 
 cudaError_t launch_block_mask(const MaskArgs& a, int64_t H, cudaStream_t s) {
-  return a.Kb <= 8192 ? launch_block_mask_rows<8>(a, H, s) : launch_block_mask_rows<4>(a, H, s);
+  return a.Kb <= 8192 ? launch_block_mask_rows<8, 8192>(a, H, s) : launch_block_mask_rows<4, 16384>(a, H, s);
 }
 
 cudaError_t launch_bitmap_to_lut(const void* bm, int64_t rows, int64_t Kb, void* lut, void* valid, cudaStream_t s) {

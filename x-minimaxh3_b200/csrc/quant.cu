@@ -337,17 +337,17 @@ int quant_threads_for(int K) {
   return ((T + 31) / 32) * 32;
 }
 
+static constexpr size_t quant_smem_bytes(int T) { return (size_t)(T / 16) * 16 * 17 * sizeof(float2); }
+
 template <int MODE, int ACT, bool RMS>
 static cudaError_t launch_q(const QuantArgs& a, int64_t rows, cudaStream_t s) {
   const int T = quant_threads_for(a.K);
-  const size_t smem = (size_t)(T / 16) * 16 * 17 * sizeof(float2);
+  const size_t smem = quant_smem_bytes(T);
   auto k = quant_rows_kernel<MODE, ACT, RMS>;
-  if (smem > 48 * 1024) {
-    cudaError_t e0 = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e0 != cudaSuccess) return e0;
-  }
+  cudaError_t e = allow_shared_memory<quant_rows_kernel<MODE, ACT, RMS>, (int)quant_smem_bytes(512)>();
+  if (e != cudaSuccess) return e;
   int per_sm = 0;
-  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, T, smem);
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, T, smem);
   if (e != cudaSuccess) return e;
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
