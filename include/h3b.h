@@ -547,7 +547,7 @@ int h3b_fp4_linear(const void* x, int dtype, int64_t rows, int64_t x_row_stride,
 /* h = x + residual (rounded to their type and written to sum; residual NULL: h = x, sum not
  * written), y = h / sqrt(mean(h^2) + eps) * weight in float32, and y quantised: to int8 rows
  * q [rows, cols] with scales [rows] (absmax / 127; a row with an infinity or a NaN gets that
- * as its scale), or to 4-bit floats as h3b_fp4_quantize does.  x, residual, weight [cols] and
+ * as its scale, and zero codes, as rows whose scale is 0 do), or to 4-bit floats as h3b_fp4_quantize does.  x, residual, weight [cols] and
  * sum are fp16 or bf16; sum may be x or residual itself, and must not overlap them
  * otherwise.  cols <= 32768. */
 int h3b_add_rms_norm_int8(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,

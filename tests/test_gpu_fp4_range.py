@@ -112,3 +112,35 @@ def test_long_sums_of_scales_with_mantissas(h3b, dtype, m, n, k):
     assert (a.abs() @ b.abs().T).max().item() * 256 < 2 ** 24
     want = (a @ b.T).to(torch.float32).to(dtype)
     assert torch.equal(h3b.fp4_linear_prequantized(*rows, out_dtype=dtype), want)
+
+
+# ------------------------------------------------------------------------------------ the norm's INT8 rows
+
+
+@pytest.mark.parametrize("k", [40, 1024, 4096])
+def test_int8_rows_whose_scale_is_subnormal(h3b, k):
+    """Rows whose absmax / 127 is below fp32's normal numbers have codes like any others.  y is off by half of
+    2^-149 in each of two roundings besides what the norm's tests count, and so is the scale."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(12, k, device="cuda", generator=g).bfloat16()
+    sign = torch.sign(torch.randn(k, device="cuda", generator=g))
+    for e in (-125, -128, -131, -133):
+        w = (sign * 2.0 ** e).bfloat16()
+        h, (q, s) = h3b.add_rms_norm_quantize(x, None, w)
+        y = x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-5) * w.double()
+        off, step = 44 * 2.0 ** -24, 2.0 ** -149
+        top = y.abs().amax(1, keepdim=True)
+        assert (s > 0).all() and (s < 2.0 ** -126).any()
+        assert ((s.double() * 127 - top).abs() <= (off + 2.0 ** -23) * top + 64 * step).all()
+        ratio = y / s.double()
+        want = ratio.clamp(-127, 127)
+        assert ((q.double() - want).abs() <= 0.5 + 127 * (off + 2.0 ** -23) + 2 * step / s.double()).all()
+    # rows on either side of the border in one call, and one of zeros
+    x[3] = 0
+    x[5:, k // 2:] = 0
+    w = torch.full((k,), 1.0, device="cuda").bfloat16()
+    w[: k // 2] = 2.0 ** -130
+    x[0, : k // 2] = 0
+    x[1, k // 2:] = 0
+    h, (q, s) = h3b.add_rms_norm_quantize(x, None, w)
+    assert s[0] > 1e-3 and q[0].any() and 0 < s[1] < 2.0 ** -126 and q[1].abs().max() >= 126 and s[3] == 0 and not q[3].any()

@@ -216,9 +216,24 @@ __global__ void __launch_bounds__(512, CH <= 2 ? 2 : 1) fp4_rows_kernel(Fp4RowAr
 #pragma unroll
     for (int i = 0; i < CH; ++i) m = max(m, top[i]);
     m = row_max<BLOCK>(m, red[1]);
-    const float scale = __fdiv_rn(__uint_as_float(m), 127.0f);  // NaN and infinity stay
+    float scale = __fdiv_rn(__uint_as_float(m), 127.0f);  // NaN and infinity stay
     if (t == 0) a.row_scales[row] = scale;
-    const bool some = m < kInfBits && scale >= FLT_MIN;  // a row below that is zeros
+    if (scale > 0.0f && scale < FLT_MIN) {
+      // The reciprocal of a subnormal scale may be infinite: row and scale times 2^64.  The scale's own rounding
+      // may have taken it so far below absmax / 127 that values go beyond 127 of them.
+      const float up = exp2_bits(64);
+      scale = __fmul_rn(scale, up);
+      const float most = __fmul_rn(scale, 127.0f);
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[i][j] = mul2(v[i][j], splat2(up));
+          v[i][j].x = fminf(fmaxf(v[i][j].x, -most), most);
+          v[i][j].y = fminf(fmaxf(v[i][j].y, -most), most);
+        }
+    }
+    const bool some = m < kInfBits && scale > 0.0f;
     const float rs = some ? __fdiv_rn(1.0f, scale) : 0.0f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
