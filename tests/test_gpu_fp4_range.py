@@ -93,6 +93,20 @@ def test_few_scales_apart_among_others(h3b, dtype):
     assert inside[:70, :300].all()
 
 
+def test_dequantised_rows_under_far_scales(h3b):
+    """A block scale that a row scale brings back into the range."""
+    for bytes_, e in (((254, 253, 200), -60), ((254, 253, 200), -127), ((0, 1, 60), 60), ((0, 1, 60), 100), ((120, 127, 130), 0)):
+        codes = torch.arange(256, device="cuda").to(torch.uint8).repeat(3).view(3, 256)
+        scales = torch.tensor(bytes_, device="cuda", dtype=torch.uint8)[:, None].expand(3, 16)
+        for factor in (1.0, -1.0):
+            q = h3b.Fp4Rows.from_blocks(codes, scales, "mxfp4", torch.full((3,), factor * 2.0 ** e, device="cuda"))
+            want = U.values(q)
+            got = h3b.dequantize_fp4(q)
+            inside = want.abs() <= torch.finfo(torch.bfloat16).max
+            assert torch.equal(got[inside].double(), want[inside].bfloat16().double()) and not got[~inside].isfinite().any()
+            assert not got.isnan().any()
+
+
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (2, 700, 16384), (11, 520, 16384), (48, 520, 16384), (100, 4100, 4096),
                                    (333, 700, 16384), (2300, 2050, 4096), (1300, 2050, 16384)])

@@ -284,8 +284,10 @@ __device__ __forceinline__ float2 elements_of(uint32_t pair) {
 // Codes and scales to 16-bit values: value = code * block scale * row scale.  A warp takes 1,024
 // columns of a row, a thread eight at a time (16 bytes of output, so that a warp's store is 512
 // bytes in a row: 16,384 x 4,096 with 16 columns a thread 33 us), or, where rows do not allow
-// that, 512 columns through shared memory.
-template <int FORMAT, bool BF16, bool VEC>
+// that, 512 columns through shared memory.  ROW: there are row scales.  Of mxfp4, one below 1 goes onto
+// the block's first, which is a power of two, since the largest of those times an element of 4 or 6
+// leaves fp32's range.
+template <int FORMAT, bool ROW, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint16_t* out, int64_t out_stride,
                                                              uint32_t parts, int64_t total) {
   __shared__ __align__(16) uint16_t stages[VEC ? 1 : 8][VEC ? 8 : 512];
@@ -302,7 +304,16 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint
     const int b = column / fp4_block(FORMAT);
     return blocks[(int64_t)(b >> 2) * 512 + (b & 3)];
   };
-  const float2 r = splat2(a.row_scales ? a.row_scales[row] : 1.0f);
+  const float r = ROW ? a.row_scales[row] : 1.0f;
+  const bool first = ROW && FORMAT == kMxfp4 && fabsf(r) < 1.0f;
+  auto scale_of = [&](uint32_t byte) {
+    const float s = FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte);
+    return splat2(first ? __fmul_rn(s, r) : s);
+  };
+  auto value_of = [&](uint32_t pair, float2 s) {
+    const float2 v = mul2(elements_of(pair), s);
+    return ROW ? mul2(v, splat2(first ? 1.0f : r)) : v;
+  };
   if constexpr (VEC) {
     uint32_t q[4], byte[4];
 #pragma unroll
@@ -314,11 +325,11 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int c = part * 1024 + i * 256 + lane * 8;
-      const float2 s = splat2(FORMAT == kMxfp4 ? e8m0_to_f32(byte[i]) : e4m3_to_f32(byte[i]));
+      const float2 s = scale_of(byte[i]);
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 v = mul2(mul2(elements_of((q[i] >> (8 * j)) & 0xffu), s), r);
+        const float2 v = value_of((q[i] >> (8 * j)) & 0xffu, s);
         w[j] = pack_halves<BF16>(v.x, v.y);
       }
       if (c < a.K) *reinterpret_cast<uint4*>(out + row * out_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -328,11 +339,9 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(Fp4RowsView a, uint
     float2 v[8] = {};
     if (c * 16 < a.K) {
       const uint2 q = *reinterpret_cast<const uint2*>(codes + c * 8);
-      const uint32_t byte = scale_byte(c * 16);
-      const float2 s = splat2(FORMAT == kMxfp4 ? e8m0_to_f32(byte) : e4m3_to_f32(byte));
+      const float2 s = scale_of(scale_byte(c * 16));
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = mul2(mul2(elements_of(((j < 4 ? q.x : q.y) >> (8 * (j & 3))) & 0xffu), s), r);
+      for (int j = 0; j < 8; ++j) v[j] = value_of(((j < 4 ? q.x : q.y) >> (8 * (j & 3))) & 0xffu, s);
     }
     store16<BF16, VEC>(out + row * out_stride, c, a.K, stages[threadIdx.x >> 5], v);
   }
@@ -382,21 +391,24 @@ cudaError_t launch_fp4_rows(const Fp4RowArgs& a, int format, bool bf16, cudaStre
                              : launch_rows_as<kNvfp4, true>(a, bf16, s);
 }
 
-template <int FORMAT>
-static cudaError_t launch_dequantize(const Fp4RowsView& a, uint16_t* out, int64_t stride, bool bf16, cudaStream_t s) {
+template <int FORMAT, bool ROW, bool BF16>
+static cudaError_t launch_dequantize(const Fp4RowsView& a, uint16_t* out, int64_t stride, cudaStream_t s) {
   const bool vec = a.K % 16 == 0 && rows16(out, stride);
   const uint32_t parts = (uint32_t)(vec ? (a.K + 1023) / 1024 : (a.K + 511) / 512);
   const int64_t total = a.rows * parts, grid = (total + 7) / 8;
-  if (bf16)
-    return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, true, true>, grid, 256, 0, s, a, out, stride, parts, total)
-               : launch_chained(fp4_dequantize_kernel<FORMAT, true, false>, grid, 256, 0, s, a, out, stride, parts, total);
-  return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, false, true>, grid, 256, 0, s, a, out, stride, parts, total)
-             : launch_chained(fp4_dequantize_kernel<FORMAT, false, false>, grid, 256, 0, s, a, out, stride, parts, total);
+  return vec ? launch_chained(fp4_dequantize_kernel<FORMAT, ROW, BF16, true>, grid, 256, 0, s, a, out, stride, parts, total)
+             : launch_chained(fp4_dequantize_kernel<FORMAT, ROW, BF16, false>, grid, 256, 0, s, a, out, stride, parts, total);
+}
+template <int FORMAT>
+static cudaError_t launch_dequantize_as(const Fp4RowsView& a, uint16_t* out, int64_t stride, bool bf16, cudaStream_t s) {
+  if (a.row_scales)
+    return bf16 ? launch_dequantize<FORMAT, true, true>(a, out, stride, s) : launch_dequantize<FORMAT, true, false>(a, out, stride, s);
+  return bf16 ? launch_dequantize<FORMAT, false, true>(a, out, stride, s) : launch_dequantize<FORMAT, false, false>(a, out, stride, s);
 }
 cudaError_t launch_fp4_dequantize(const Fp4RowsView& a, int format, uint16_t* out, int64_t out_stride, bool bf16,
                                   cudaStream_t s) {
-  return format == kMxfp4 ? launch_dequantize<kMxfp4>(a, out, out_stride, bf16, s)
-                          : launch_dequantize<kNvfp4>(a, out, out_stride, bf16, s);
+  return format == kMxfp4 ? launch_dequantize_as<kMxfp4>(a, out, out_stride, bf16, s)
+                          : launch_dequantize_as<kNvfp4>(a, out, out_stride, bf16, s);
 }
 
 }  // namespace h3b
