@@ -524,6 +524,13 @@ __global__ void __launch_bounds__(kSplitThreads)
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }
+  __syncwarp();
+  // A CTA that gave up leaves last: the others' sums may still be on their way into its shared memory.
+  // Those that have all sums leave at once, and the barrier counts them.
+  if (split > 1 && abort_flag) {
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 // ------------------------------------------------------------------ many rows: 256 x 256 tiles on two SMs
