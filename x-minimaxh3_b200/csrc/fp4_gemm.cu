@@ -737,11 +737,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
         fill.next(kStages);
       }
     }
-    // Both CTAs' copies are counted by the even CTA's barriers; the odd one waits for it at the
-    // end.  Of each slot the last fill: slots before the next one in this round, the others before.
-    if (rank == 0)
-      for (uint32_t s = 0; s < kStages; ++s)
-        mbar_wait_warp(&full[s], s < fill.stage ? fill.parity : fill.parity ^ 1u, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
+    // Copies have landed before the CTAs leave.  Both CTAs' are counted by the even CTA's barriers, up to its
+    // own last fill, and the odd CTA's by their use, of which its barriers are told: the even one may have
+    // given up before them.  Of each slot the last fill: slots before the next one in this round, the others before.
+    uint64_t* landed = rank == 0 ? full : empty;
+    for (uint32_t s = 0; s < kStages; ++s)
+      mbar_wait_warp(&landed[s], s < fill.stage ? fill.parity : fill.parity ^ 1u, &late_flag, H3B_STATUS_GEMM_TIMEOUT);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t smem0 = smem_u32(smem);
