@@ -158,3 +158,24 @@ def test_int8_rows_whose_scale_is_subnormal(h3b, k):
     x[1, k // 2:] = 0
     h, (q, s) = h3b.add_rms_norm_quantize(x, None, w)
     assert s[0] > 1e-3 and q[0].any() and 0 < s[1] < 2.0 ** -126 and q[1].abs().max() >= 126 and s[3] == 0 and not q[3].any()
+
+
+# ------------------------------------------------------------------------------------ outputs beside inputs
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 700])
+def test_inputs_and_outputs_in_the_columns_of_one_buffer(h3b, m):
+    k = n = 384
+    for gap in (0, 8, 3):
+        buffer = torch.randn(m, 2 * k + gap, device="cuda", generator=torch.Generator(device="cuda").manual_seed(m)).bfloat16()
+        x, out = buffer[:, :k], buffer[:, k + gap:]
+        first, kept = x.clone(), buffer[:, k: k + gap].clone()
+        weight = h3b.quantize_fp4(torch.randn(n, k, device="cuda").bfloat16(), "nvfp4")
+        want = h3b.fp4_linear(first, weight)
+        h3b.fp4_linear(x, weight, out=out)
+        assert torch.equal(out, want) and torch.equal(x, first) and torch.equal(buffer[:, k: k + gap], kept)
+        residual, norm = torch.randn(m, k, device="cuda").bfloat16(), torch.randn(k, device="cuda").bfloat16()
+        total, (q, s) = h3b.add_rms_norm_quantize(first, residual, norm)
+        h, (q2, s2) = h3b.add_rms_norm_quantize(x, residual, norm, out=out)
+        assert h is out and torch.equal(out, total) and torch.equal(q, q2) and torch.equal(s, s2) and torch.equal(x, first)
+        assert torch.equal(buffer[:, k: k + gap], kept)

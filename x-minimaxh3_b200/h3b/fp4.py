@@ -184,6 +184,23 @@ def _half_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]
     return x, x.shape[0], k, x.stride(0) if x.shape[0] > 1 else k
 
 
+def _meet(a: tuple[int, int, int, int], b: tuple[int, int, int, int]) -> bool:
+    """Whether two pieces of memory (address, rows, bytes of a row, bytes between rows) share any.  Of pieces that reach
+    into each other only those of one step are looked at more closely: their rows may lie beside each other, as
+    column ranges of one buffer do."""
+    (a_at, a_rows, a_row, a_step), (b_at, b_rows, b_row, b_step) = a, b
+    if not (a_rows and b_rows) or a_at + (a_rows - 1) * a_step + a_row <= b_at or b_at + (b_rows - 1) * b_step + b_row <= a_at:
+        return False
+    if a_rows == 1:
+        a_step = b_step
+    elif b_rows == 1:
+        b_step = a_step
+    if a_rows == b_rows == 1 or a_step != b_step:
+        return True
+    beside = (b_at - a_at) % a_step
+    return beside < a_row or beside + b_row > a_step
+
+
 def _gpu_of(x: torch.Tensor, name: str) -> int:
     if not x.is_cuda:
         raise RuntimeError(f"{name} runs only on CUDA tensors (the B200 library has no CPU path)")
@@ -289,7 +306,8 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
     if given:
         step = _check_out(out, m, n, x.dtype, gpu)
         at, x_at = out.data_ptr(), x.data_ptr()
-        if m and n and at < x_at + 2 * ((m - 1) * x_step + k) and x_at < at + 2 * ((m - 1) * step + n):
+        if (m and n and at < x_at + 2 * ((m - 1) * x_step + k) and x_at < at + 2 * ((m - 1) * step + n)
+                and _meet((at, m, 2 * n, 2 * step), (x_at, m, 2 * k, 2 * x_step))):
             raise ValueError("out must not overlap x")
     else:
         out = x.new_empty((m, n))
@@ -352,8 +370,9 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
             if not out.is_contiguous():
                 sum_step = _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
             end = sum_at + 2 * ((m - 1) * sum_step + k)
-            for i, i_step in ((at, step), (res_at, res_step), (w_at, 0)):
-                if i < end and sum_at < i + 2 * ((m - 1) * i_step + k) and (i != sum_at or i_step != sum_step) and m:
+            for i, i_rows, i_step in ((at, m, step), (res_at, m, res_step), (w_at, 1, 0)):
+                if (i < end and sum_at < i + 2 * ((m - 1) * i_step + k) and (i != sum_at or i_step != sum_step) and m
+                        and _meet((sum_at, m, 2 * k, 2 * sum_step), (i, i_rows, 2 * k, 2 * i_step))):
                     raise ValueError("out may be x or residual, and must not overlap them or the weight otherwise")
     elif out is not None:
         raise ValueError("without a residual there is no sum to write")
