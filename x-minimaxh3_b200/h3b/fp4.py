@@ -60,7 +60,7 @@ class Fp4Rows:
     blocks, the order in which the products read them (`from_blocks` and `blocks` convert from and to
     [rows, blocks]).  row_scales: f32 [rows], or None for 1."""
 
-    __slots__ = ("rows", "cols", "format", "_gpu", "_ref", "_buffer", "_codes", "_scales", "_row_scales")
+    __slots__ = ("rows", "cols", "format", "_gpu", "_ref", "_buffer", "_codes", "_scales", "_row_scales", "_from", "_to")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int, format: str,
                  row_scales: torch.Tensor | None = None) -> None:
@@ -87,6 +87,8 @@ class Fp4Rows:
         self.rows, self.cols, self.format, self._gpu = rows, cols, format, gpu
         self._buffer, self._codes, self._scales, self._row_scales = None, codes, scales, row_scales
         self._ref = ctypes.byref(Fp4RowsStruct(codes.data_ptr(), scales.data_ptr(), _ptr(row_scales), rows, cols, code))
+        pieces = self._pieces()
+        self._from, self._to = min((p[0] for p in pieces), default=0), max((p[0] + p[2] for p in pieces), default=0)
 
     @classmethod
     def _room(cls, rows: int, cols: int, format: str, like: torch.Tensor) -> Fp4Rows:
@@ -97,12 +99,22 @@ class Fp4Rows:
         bands, groups = _scale_tiles(rows, cols, format)
         size = rows * ((cols + 31) // 32 * 16)
         end = size + bands * groups * 512
-        self._buffer = buffer = like.new_empty(end + (4 * rows if code == 2 else 0), dtype=torch.uint8)
-        at = buffer.data_ptr()
+        whole = end + (4 * rows if code == 2 else 0)
+        self._buffer = buffer = like.new_empty(whole, dtype=torch.uint8)
+        self._from = at = buffer.data_ptr()
+        self._to = at + whole
         self.rows, self.cols, self.format, self._gpu = rows, cols, format, like.get_device()
         self._codes = self._scales = self._row_scales = None
         self._ref = ctypes.byref(Fp4RowsStruct(at, at + size, at + end if code == 2 else None, rows, cols, code))
         return self
+
+    def _pieces(self) -> list[tuple[int, int, int, int]]:
+        """The memory it lies in (see _meet), between _from and _to."""
+        r = self._ref._obj
+        bands, groups = _scale_tiles(self.rows, self.cols, self.format)
+        sizes = ((r.codes, self.rows * ((self.cols + 31) // 32 * 16)), (r.scales, bands * groups * 512),
+                 (r.row_scales, 4 * self.rows))
+        return [(at, 1, size, size) for at, size in sizes if at and size]
 
     def _parts(self) -> None:
         bands, groups = _scale_tiles(self.rows, self.cols, self.format)
@@ -189,7 +201,9 @@ def _meet(a: tuple[int, int, int, int], b: tuple[int, int, int, int]) -> bool:
     into each other only those of one step are looked at more closely: their rows may lie beside each other, as
     column ranges of one buffer do."""
     (a_at, a_rows, a_row, a_step), (b_at, b_rows, b_row, b_step) = a, b
-    if not (a_rows and b_rows) or a_at + (a_rows - 1) * a_step + a_row <= b_at or b_at + (b_rows - 1) * b_step + b_row <= a_at:
+    if not (a_rows and a_row and b_rows and b_row):
+        return False
+    if a_at + (a_rows - 1) * a_step + a_row <= b_at or b_at + (b_rows - 1) * b_step + b_row <= a_at:
         return False
     if a_rows == 1:
         a_step = b_step
@@ -199,6 +213,23 @@ def _meet(a: tuple[int, int, int, int], b: tuple[int, int, int, int]) -> bool:
         return True
     beside = (b_at - a_at) % a_step
     return beside < a_row or beside + b_row > a_step
+
+
+def _refuse_overlap(what: str, piece: tuple[int, int, int, int], quantised, others=()) -> None:
+    """Refuses a piece of memory that a call writes and that shares any with what it reads."""
+    at, rows, row, step = piece
+    end = at + (rows - 1) * step + row
+    for q in quantised:
+        if at < q._to and q._from < end and any(_meet(piece, p) for p in q._pieces()):
+            raise ValueError(f"{what} must not overlap the call's 4-bit rows")
+    for p in others:
+        if _meet(piece, p):
+            raise ValueError(f"{what} must not overlap what the call reads or writes besides")
+
+
+def _vector(t: torch.Tensor | None) -> tuple[tuple[int, int, int, int], ...]:
+    """A contiguous float32 vector as a piece of memory, if there is one."""
+    return () if t is None else ((t.data_ptr(), 1, 4 * t.numel(), 0),)
 
 
 def _gpu_of(x: torch.Tensor, name: str) -> int:
@@ -245,11 +276,15 @@ def dequantize_fp4(rows: Fp4Rows, dtype: torch.dtype = torch.bfloat16, out: torc
     if dtype not in _DTYPES:
         raise ValueError("dequantize_fp4 writes bfloat16 or float16")
     step = rows.cols
-    if out is None:
+    given = out is not None
+    if not given:
         out = rows._new((rows.rows, rows.cols), dtype)
     else:
         step = _check_out(out, rows.rows, rows.cols, dtype, rows._gpu)
-    check(lib().h3b_fp4_dequantize(rows._ref, out.data_ptr(), _DTYPES[dtype], step, _stream(rows._gpu)), "fp4_dequantize")
+    stream = _stream(rows._gpu)
+    if given:
+        _refuse_overlap("out", (out.data_ptr(), rows.rows, 2 * rows.cols, 2 * step), (rows,))
+    check(lib().h3b_fp4_dequantize(rows._ref, out.data_ptr(), _DTYPES[dtype], step, stream), "fp4_dequantize")
     return out
 
 
@@ -278,12 +313,15 @@ def fp4_linear_prequantized(xq: Fp4Rows, weight: Fp4Rows, bias: torch.Tensor | N
         raise ValueError("fp4_linear writes bfloat16 or float16")
     step = n = weight.rows
     bias = _bias(bias, n, gpu)
-    if out is None:
+    given = out is not None
+    if not given:
         out = xq._new((xq.rows, n), out_dtype)
     else:
         step = _check_out(out, xq.rows, n, out_dtype, gpu)
-    check(lib().h3b_fp4_gemm(xq._ref, weight._ref, _ptr(bias), out.data_ptr(), _DTYPES[out_dtype], step, _stream(gpu)),
-          "fp4_gemm")
+    stream = _stream(gpu)
+    if given:
+        _refuse_overlap("out", (out.data_ptr(), xq.rows, 2 * n, 2 * step), (xq, weight), _vector(bias))
+    check(lib().h3b_fp4_gemm(xq._ref, weight._ref, _ptr(bias), out.data_ptr(), _DTYPES[out_dtype], step, stream), "fp4_gemm")
     return out
 
 
@@ -291,7 +329,8 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] (bf16 or fp16), quantised to the weight's format, times weight [N, K]^T, + bias -> x's type [..., N].
 
-    out: rows [M, N] that receive the result, apart from x.  workspace: uint8, reused by calls on one stream."""
+    out: rows [M, N] that receive the result.  workspace: uint8, reused by calls on one stream.  Neither may share
+    memory with the call's other tensors."""
     gpu = _gpu_of(x, "fp4_linear")
     if weight._gpu != gpu:
         raise ValueError("all tensors must be on one GPU")
@@ -312,17 +351,23 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
     else:
         out = x.new_empty((m, n))
     library = lib()
+    if given:
+        _refuse_overlap("out", (at, m, 2 * n, 2 * step), (weight,), _vector(bias))
     need = library.h3b_fp4_linear_workspace_bytes(m, weight._ref)
-    at = None
+    ws_at = None
     if need:
-        if workspace is None:
+        shared = workspace is not None
+        if not shared:
             workspace = x.new_empty(need, dtype=torch.uint8)
         elif (workspace.numel() * workspace.element_size() < need or workspace.get_device() != gpu
               or not workspace.is_contiguous() or workspace.data_ptr() % 16):
             raise ValueError(f"the workspace must have {need} contiguous, 16-byte aligned bytes on the operands' GPU")
-        at = workspace.data_ptr()
+        ws_at = workspace.data_ptr()
+        if shared:
+            _refuse_overlap("the workspace", (ws_at, 1, need, 0), (weight,),
+                            ((x.data_ptr(), m, 2 * k, 2 * x_step), (out.data_ptr(), m, 2 * n, 2 * step), *_vector(bias)))
     check(library.h3b_fp4_linear(x.data_ptr(), _DTYPES[x.dtype], m, x_step, weight._ref, _ptr(bias),
-                                 out.data_ptr(), step, at, need, _stream(gpu)), "fp4_linear")
+                                 out.data_ptr(), step, ws_at, need, _stream(gpu)), "fp4_linear")
     return out if given or len(shape) == 2 else out.view(*shape[:-1], n)
 
 
