@@ -118,3 +118,16 @@ def test_outputs_and_workspaces_on_anything_else_are_refused(monkeypatch):
 def test_rows_without_any_memory():
     empty = h3b.Fp4Rows(_at(0, (0, 32), torch.uint8), _at(0, (0, 1, 512), torch.uint8), 64, "nvfp4")
     assert empty._pieces() == [] and not fp4._meet((0, 4, 8, 8), (0, 0, 8, 8)) and not fp4._meet((0, 4, 0, 8), (0, 1, 8, 8))
+
+
+def test_sums_into_part_of_a_batchs_rows_are_refused(monkeypatch):
+    """[batch, 3 of 5 rows, columns]: these rows have no one step.  All of the batch's rows, in part of their columns, do."""
+    monkeypatch.setattr(cache, "_current_gpu", lambda: 0)
+    monkeypatch.setattr(fp4, "lib", _reached)
+    x, residual, weight = _at(4096, (2, 3, 64)), _at(1 << 20, (2, 3, 64)), _at(1 << 21, (64,))
+    for buffer, met in ((torch.zeros(2, 5, 64, dtype=torch.bfloat16)[:, :3], True), (torch.zeros(2, 3, 80, dtype=torch.bfloat16)[..., :64], False)):
+        def rows(t, at=1 << 22):
+            return SimpleNamespace(get_device=lambda: 0, shape=t.shape, ndim=t.ndim, dtype=t.dtype, stride=t.stride,
+                                   data_ptr=lambda: at, is_contiguous=t.is_contiguous, view=lambda *s: rows(t.view(*s)))
+        with pytest.raises(ValueError if met else H._Reached, match="one step" if met else None):
+            h3b.add_rms_norm_quantize(x, residual, weight, out=rows(buffer))

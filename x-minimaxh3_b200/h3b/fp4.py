@@ -375,10 +375,11 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
                           to: str = "int8", out: torch.Tensor | None = None):
     """(h, quantised RMSNorm(h) * weight) of h = x + residual; x, residual [..., K], weight [K], one 16-bit type.
 
-    h is rounded to that type, and normed as it is stored, in fp32; `out` receives it (x or residual
-    themselves may, and no other tensor that overlaps them).  Without a residual h is x, and nothing is
-    written to it.  to "int8": (codes int8 [M, K], scales f32 [M, 1] = absmax / 127), as
-    ops.int8_linear_prequantized takes them; "mxfp4" or "nvfp4": Fp4Rows, as fp4_linear_prequantized does."""
+    h is rounded to that type, and normed as it is stored, in fp32; `out`, whose rows lie at one step from
+    each other, receives it (x or residual themselves may, and no other tensor that overlaps them).  Without
+    a residual h is x, and nothing is written to it.  to "int8": (codes int8 [M, K], scales f32 [M, 1] =
+    absmax / 127), as ops.int8_linear_prequantized takes them; "mxfp4" or "nvfp4": Fp4Rows, as
+    fp4_linear_prequantized does."""
     gpu = _gpu_of(x, "add_rms_norm_quantize")
     int8 = to == "int8"
     if not int8:
@@ -413,7 +414,11 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight
                 raise ValueError("out must have x's shape and type, on its GPU")
             h, sum_at = out, out.data_ptr()
             if not out.is_contiguous():
-                sum_step = _check_out(out if len(shape) == 2 else out.view(m, k), m, k, dtype, gpu)
+                try:
+                    flat = out if len(shape) == 2 else out.view(m, k)
+                except RuntimeError:  # a part of a batch's rows, say
+                    raise ValueError("out's rows must lie at one step from each other") from None
+                sum_step = _check_out(flat, m, k, dtype, gpu)
             end = sum_at + 2 * ((m - 1) * sum_step + k)
             for i, i_rows, i_step in ((at, m, step), (res_at, m, res_step), (w_at, 1, 0)):
                 if (i < end and sum_at < i + 2 * ((m - 1) * i_step + k) and (i != sum_at or i_step != sum_step) and m
