@@ -1,0 +1,23 @@
+"""Fp4Rows' own layout work, on host tensors (no GPU needed)."""
+
+import pytest
+import torch
+
+import h3b
+
+from_blocks = h3b.Fp4Rows.from_blocks.__func__
+
+
+@pytest.mark.parametrize("format,block", [("mxfp4", 32), ("nvfp4", 16)])
+@pytest.mark.parametrize("rows,cols", [(0, 64), (0, 4096), (1, 32), (130, 96), (3, 0), (0, 0)])
+def test_rows_from_elsewhere_of_any_number(format, block, rows, cols):
+    """What the constructor is given.  Rows without columns reach it too, which refuses them."""
+    codes = torch.arange(rows * (cols // 2)).to(torch.uint8).view(rows, cols // 2)
+    blocks = -(-cols // block)
+    scales = torch.arange(rows * blocks).to(torch.uint8).view(rows, blocks)
+    got, tiles, n, *_ = from_blocks(lambda *a: a, codes, scales, format)
+    assert n == cols and got.shape == (rows, -(-cols // 32) * 16) and torch.equal(got[:, : cols // 2], codes)
+    assert tiles.shape == (-(-rows // 128), -(-blocks // 4), 512)
+    for r in range(0, rows, 7):
+        for b in range(blocks):
+            assert tiles[r // 128, b // 4, (r % 32) * 16 + (r % 128 // 32) * 4 + b % 4] == scales[r, b]

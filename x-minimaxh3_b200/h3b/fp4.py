@@ -167,7 +167,7 @@ class Fp4Rows:
             raise ValueError("codes and scales must be on one GPU")
         pad = torch.nn.functional.pad
         b = pad(block_scales.contiguous().view(torch.uint8), (0, -blocks % 4, 0, -rows % 128))
-        b = b.view(b.shape[0] // 128, 4, 32, -1, 4).permute(0, 3, 2, 1, 4)  # band, group, row % 32, row / 32, block
+        b = b.view(b.shape[0] // 128, 4, 32, b.shape[1] // 4, 4).permute(0, 3, 2, 1, 4)  # band, group, row % 32, row / 32, block
         return cls(pad(codes, (0, -codes.shape[1] % 16)).contiguous(), b.reshape(b.shape[0], b.shape[1], 512), cols, format,
                    None if row_scales is None else row_scales.to(torch.float32).reshape(-1).contiguous())
 
