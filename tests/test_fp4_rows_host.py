@@ -21,3 +21,29 @@ def test_rows_from_elsewhere_of_any_number(format, block, rows, cols):
     for r in range(0, rows, 7):
         for b in range(blocks):
             assert tiles[r // 128, b // 4, (r % 32) * 16 + (r % 128 // 32) * 4 + b % 4] == scales[r, b]
+
+
+@pytest.mark.parametrize("format", ("mxfp4", "nvfp4"))
+def test_parts_asked_for_by_two_threads(format):
+    """The parts become tensors where they are first asked for.  While one thread makes them, another asks for them
+    between any two steps of the first."""
+    rows = h3b.Fp4Rows._room(5, 64, format, torch.empty(0, dtype=torch.bfloat16))
+    buffer, other = rows._buffer, []
+
+    class Watched:
+        """The buffer; each part that is cut from it lets the other thread ask for all of them first."""
+        def __getitem__(self, part):
+            if len(other) < 3:
+                other.append(None)
+                rows._buffer, found = buffer, rows._codes is not None
+                other[-1] = (rows.codes, rows.scales, rows.row_scales)
+                if not found:  # nothing was there: what the other thread made is taken away again
+                    rows._codes = rows._scales = rows._row_scales = None
+                rows._buffer = self
+            return buffer[part]
+    rows._buffer = Watched()
+    assert rows.codes.shape == (5, 32)
+    assert other
+    for codes, scales, row_scales in other:
+        assert codes.shape == (5, 32) and scales is not None and scales.shape[-1] == 512
+        assert (row_scales is None) == (format == "mxfp4")

@@ -121,10 +121,10 @@ class Fp4Rows:
         pitch = (self.cols + 31) // 32 * 16
         size = self.rows * pitch
         end = size + bands * groups * 512
-        self._codes = self._buffer[:size].view(self.rows, pitch)
-        self._scales = self._buffer[size:end].view(bands, groups, 512)
         if self.format == "nvfp4":
             self._row_scales = self._buffer[end:].view(torch.float32)
+        self._scales = self._buffer[size:end].view(bands, groups, 512)
+        self._codes = self._buffer[:size].view(self.rows, pitch)  # last: another thread takes it as a sign that all are there
 
     @property
     def codes(self) -> torch.Tensor:
