@@ -4,6 +4,8 @@ import pytest
 import torch
 
 import h3b
+import test_fp4_host as H
+from h3b import cache, fp4
 
 from_blocks = h3b.Fp4Rows.from_blocks.__func__
 
@@ -47,3 +49,14 @@ def test_parts_asked_for_by_two_threads(format):
     for codes, scales, row_scales in other:
         assert codes.shape == (5, 32) and scales is not None and scales.shape[-1] == 512
         assert (row_scales is None) == (format == "mxfp4")
+
+
+def test_more_rows_than_a_call_takes_reach_the_refusal(monkeypatch):
+    """2^30 + 1 rows of one column: no workspace is made for them, and the library's own words are the answer."""
+    monkeypatch.setattr(cache, "_current_gpu", lambda: 0)
+    monkeypatch.setattr(cache, "_raw_stream", lambda gpu: 0)
+    weight = h3b.Fp4Rows(H._on(0, (4, 16), torch.uint8), H._on(0, (1, 1, 512), torch.uint8), 1, "mxfp4")
+    x = H._on(0, (2, 1))
+    x.shape, x.new_empty = torch.Size(((1 << 30) + 1, 1)), lambda shape, **k: H._on(0, (2, 4)) if isinstance(shape, tuple) else torch.empty(shape)
+    with pytest.raises(h3b.H3BError, match="bad sizes"):
+        fp4.fp4_linear(x, weight)

@@ -355,7 +355,7 @@ def fp4_linear(x: torch.Tensor, weight: Fp4Rows, bias: torch.Tensor | None = Non
         _refuse_overlap("out", (at, m, 2 * n, 2 * step), (weight,), _vector(bias))
     need = library.h3b_fp4_linear_workspace_bytes(m, weight._ref)
     ws_at = None
-    if need:
+    if need > 0:  # below 0: sizes that the call refuses
         shared = workspace is not None
         if not shared:
             workspace = x.new_empty(need, dtype=torch.uint8)
