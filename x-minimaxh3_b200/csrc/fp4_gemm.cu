@@ -162,7 +162,8 @@ constexpr int kSplitMost = 220 * 1024;  // dynamic shared memory of a CTA
 constexpr int kRows16Steps = 16;  // K steps of a CTA that quantises x
 // Pieces of 512 columns of x that one of its four warps holds.  More rows take longer here than in a
 // kernel of their own in front (4,096 -> 4,096, nvfp4: 4 rows 7.2 us in one launch and 6.2 in two, 8 rows
-// 8.4 and 6.1; mxfp4: 8 rows 5.8 and 5.7); a call in one launch costs the host 10 us, one in two 14.
+// 8.4 and 6.1; mxfp4: 8 rows 5.8 and 5.7); a call in one launch costs the host 10 us, one in two 14.  The limits
+// go by the call from the host: in a captured graph, nvfp4 rows near them would take less time in two launches.
 constexpr int rows16_items(int format) { return format == kMxfp4 ? 4 : 2; }
 
 // bounded wait for an mbarrier whose arrivals release what other CTAs of the cluster wrote here
@@ -452,7 +453,8 @@ __global__ void __launch_bounds__(kSplitThreads)
     const float ws1 = a.ws && n < a.N ? a.ws[n1] : 1.0f, bias1 = a.bias && n < a.N ? a.bias[n1] : 0.0f;
     asm volatile("bar.sync 2, 128;" ::: "memory");  // row_scale
     // Whether some row's and some column's scale of this warp lie on different sides of 1: found here, while the
-    // products run, since the order for it takes each sum longer (1,111 x 1,003 x 1,056 nvfp4 7.2 us, so 6.5).
+    // products run, since the order for it takes each sum longer (333 rows, 4,096 -> 4,096: mxfp4 12.4 us with it
+    // for all sums, so 11.7, nvfp4 14.6 and 14.0).
     bool apart = a.ws && (ROWS16 ? FORMAT == kNvfp4 : a.xs != nullptr);
     if (apart) {
       const bool below0 = fabsf(ws0) < 1.0f, below1 = fabsf(ws1) < 1.0f;
@@ -589,13 +591,14 @@ struct PairFp4Cfg {
 constexpr int kPairFp4Threads = 384;
 
 // 32 columns of a row's sums to 16 bits, two to a word; columns: their scales and biases, four of
-// each in turn, in shared memory, or null where there are none.  apart: some row's scale of this warp
-// may lie on the other side of 1 than some column's (fp4_scaled); else the two follow each other.
-template <bool BF16>
+// each in turn, in shared memory, or null where there are none.  BOTH: there are row scales on both
+// sides (nvfp4; mxfp4 rows of a caller's), and with `apart` some row's of this warp may lie on the other
+// side of 1 than some column's (fp4_scaled); else the two follow each other.
+template <bool BOTH, bool BF16>
 __device__ __forceinline__ void fp4_pack_chunk(const uint32_t (&r)[32], uint32_t (&h)[16], float xs,
                                                const float4* columns, bool apart) {
   const float2 x2 = splat2(xs);
-  if (apart) {
+  if (BOTH && __builtin_expect(apart, 0)) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const float4 w = columns[2 * q], b = columns[2 * q + 1];
@@ -693,7 +696,7 @@ __device__ __forceinline__ TilePlace tile_place(int t, int num_m, int num_n, int
   return {in / width, group * g + in % width};
 }
 
-template <int FORMAT, bool BF16>
+template <int FORMAT, bool BOTH, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
     fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                     const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ CUtensorMap tm_sw,
@@ -832,14 +835,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
         asm volatile("bar.sync 1, 256;" ::: "memory");  // all warps are done with the last tile's
         columns[i >> 2 << 1][i & 3] = w;
         columns[(i >> 2 << 1) + 1][i & 3] = b;
-        // how many of the columns' scales are below 1: where none or all are, and this warp's rows' likewise,
-        // the scales need no order of their own
-        uint32_t below;
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.popc.u32 %0, 1, 256, p;\n\t}"
-                     : "=r"(below) : "r"(n < a.N && fabsf(w) < 1.0f ? 1u : 0u) : "memory");
-        const bool row_below = fabsf(xs) < 1.0f;
-        const bool alike = m >= a.M || (row_below ? below == (uint32_t)min(256, a.N - nb * 256) : below == 0u);
-        apart = a.xs && a.ws && !__all_sync(0xffffffffu, alike);
+        if constexpr (BOTH) {
+          // How many of the columns' scales are below 1: where none or all are, and this warp's rows' likewise, they
+          // need no order.  (One code for all cases took 3,600 rows, 4,096 -> 16,384 nvfp4 126.3 us, so 123.7,
+          // and 122.5 to 124.5 with no order at all.)
+          uint32_t below;
+          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.popc.u32 %0, 1, 256, p;\n\t}"
+                       : "=r"(below) : "r"(n < a.N && fabsf(w) < 1.0f ? 1u : 0u) : "memory");
+          const bool row_below = fabsf(xs) < 1.0f;
+          const bool alike = m >= a.M || (row_below ? below == (uint32_t)min(256, a.N - nb * 256) : below == 0u);
+          apart = !__all_sync(0xffffffffu, alike);
+        } else {
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
       }
       // a warp that has given up goes on through the tiles, since the others meet it at the barriers above
       live = live && mbar_wait_warp(&tfull, tile & 1, &abort_flag, H3B_STATUS_GEMM_TIMEOUT);
@@ -863,15 +871,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairFp4Threads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0);
-      fp4_pack_chunk<BF16>(r0, h0, xs, cols ? cols + (64 * first) / 2 : nullptr, apart);
-      fp4_pack_chunk<BF16>(r1, h1, xs, cols ? cols + (64 * first + 32) / 2 : nullptr, apart);
+      fp4_pack_chunk<BOTH, BF16>(r0, h0, xs, cols ? cols + (64 * first) / 2 : nullptr, apart);
+      fp4_pack_chunk<BOTH, BF16>(r1, h1, xs, cols ? cols + (64 * first + 32) / 2 : nullptr, apart);
       fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * first, a);
       if (FORMAT != kNvfp4) tmem_ld32(taddr + 32u * (uint32_t)early, r2);
       tmem_ld32(taddr + 32u * (uint32_t)late, r0);
       tmem_wait_ld_dep(r0);
       reg_barrier32(r2);
-      fp4_pack_chunk<BF16>(r2, h0, xs, cols ? cols + (32 * early) / 2 : nullptr, apart);
-      fp4_pack_chunk<BF16>(r0, h1, xs, cols ? cols + (32 * late) / 2 : nullptr, apart);
+      fp4_pack_chunk<BOTH, BF16>(r2, h0, xs, cols ? cols + (32 * early) / 2 : nullptr, apart);
+      fp4_pack_chunk<BOTH, BF16>(r0, h1, xs, cols ? cols + (32 * late) / 2 : nullptr, apart);
       if (odd) fp4_put_piece(&tm_out, buf, h0, h1, m_warp, n0 + 64 * second, a);
       else fp4_put_piece(&tm_out, buf, h1, h0, m_warp, n0 + 64 * second, a);
     }
@@ -998,11 +1006,14 @@ static int launch_pair(const Fp4RowsView& x, const Fp4RowsView& w, const Fp4Gemm
   b.group = a.M >= a.N && (int64_t)a.N * fp4_pitch(a.K) <= 48 << 20 ? (int)num_n : 8;
   const int64_t pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
   constexpr int kTotal = PairFp4Cfg<FORMAT>::kTotal;
-  auto launch = [&](auto bf16) {
-    return launch_fp4<fp4_pair_kernel<FORMAT, decltype(bf16)::value>, kTotal>(2 * pairs, 1, 0, kPairFp4Threads, kTotal, s,
-                                                                              tx, tw, tsx, tsw, to, b);
+  auto launch = [&](auto both, auto bf16) {
+    return launch_fp4<fp4_pair_kernel<FORMAT, decltype(both)::value, decltype(bf16)::value>, kTotal>(
+        2 * pairs, 1, 0, kPairFp4Threads, kTotal, s, tx, tw, tsx, tsw, to, b);
   };
-  *err = a.bf16 ? launch(std::true_type{}) : launch(std::false_type{});
+  auto launch_as = [&](auto both) { return a.bf16 ? launch(both, std::true_type{}) : launch(both, std::false_type{}); };
+  // The order of two scales in an instance of its own (9,472 x 2,048 x 4,096 mxfp4, where there are none, with a cold
+  // instruction cache: 34.6 us, with the code for both 36.9)
+  *err = a.xs && a.ws ? launch_as(std::true_type{}) : launch_as(std::false_type{});
   return *err == cudaSuccess ? 0 : 2;
 }
 static bool uses_pair(int M, int N) {
