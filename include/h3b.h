@@ -500,9 +500,11 @@ int h3b_pages_copy(const h3b_page_cache* cache, const int32_t* src, const int32_
 
 /* ---------------------------------------------------------------- microscaled 4-bit floats
  * Rows of E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) with a scale per block:
- *   H3B_MXFP4: blocks of 32 columns, E8M0 scales (2^(byte - 127)); no row scale
- *   H3B_NVFP4: blocks of 16 columns, E4M3 scales, and a float32 scale per row
- * value = element * block scale * row scale.
+ *   H3B_MXFP4: blocks of 32 columns, E8M0 scales (2^(byte - 127))
+ *   H3B_NVFP4: blocks of 16 columns, E4M3 scales
+ * and, for rows of either format that have one, a float32 scale per row (the entries below
+ * write one for each NVFP4 row and none for MXFP4):
+ *   value = element * block scale * row scale.
  * codes: [rows, ceil(cols / 32) * 16] bytes, column 2i in the low nibble of byte i, zero
  * codes behind the last column.  scales: tiles of 128 rows x 4 blocks in 512 bytes,
  * [ceil(rows / 128), ceil(cols / (4 * block)), 512]; row r of a tile has its four bytes at
@@ -531,14 +533,17 @@ int h3b_fp4_dequantize(const h3b_fp4_rows* rows, void* out, int dtype, int64_t o
 
 /* out[m, n] = sum over k of x[m, k] * w[n, k], times the row scales of x and w, + bias[n]
  * (float32 [w->rows] or NULL), rounded to fp16 / bf16; fp32 sums, the same ones every time.
+ * A sum within fp32's range takes its row scales without leaving it on the way to a result
+ * within it.  out must not overlap anything that is read.
  * x and w have one format and one number of columns. */
 int h3b_fp4_gemm(const h3b_fp4_rows* x, const h3b_fp4_rows* w, const float* bias, void* out, int out_dtype,
                  int64_t out_row_stride, void* stream);
 
 /* h3b_fp4_quantize of x [rows, w->cols] into the workspace, then h3b_fp4_gemm; the output
- * has x's type and must not overlap x.  workspace: h3b_fp4_linear_workspace_bytes() bytes (0 for few rows, which
+ * has x's type.  workspace: h3b_fp4_linear_workspace_bytes() bytes (0 for few rows, which
  * the product quantises itself: NULL), 16-byte aligned, not shared by calls on different
- * streams.  The same values either way. */
+ * streams.  out and the workspace must not overlap each other or anything that is read.
+ * The same values either way. */
 int64_t h3b_fp4_linear_workspace_bytes(int64_t rows, const h3b_fp4_rows* w);
 int h3b_fp4_linear(const void* x, int dtype, int64_t rows, int64_t x_row_stride, const h3b_fp4_rows* w,
                    const float* bias, void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes,

@@ -18,8 +18,10 @@ Elements are E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign.  Two formats:
              row, the least (e >= -126) with the row's absmax <= 2688 r
 
 An element is the nearest to x / scale, ties to the even code, and 6 at most.  A block with an
-infinity or a NaN becomes NaN.  Every step is exact or rounded once, so the same rows give the
-same codes everywhere.
+infinity or a NaN becomes NaN.  Every step of quantize_fp4 is exact or rounded once, so the same
+rows give the same codes everywhere.  The norm in front of add_rms_norm_quantize's codes is fp32: the
+order in which its squares are added goes by the row's length and address and by the number of rows,
+and where their sum is beyond fp32's range, the normed row is 0.
 """
 
 from __future__ import annotations
@@ -55,10 +57,11 @@ def _scale_tiles(rows: int, cols: int, format: str) -> tuple[int, int]:
 class Fp4Rows:
     """Rows of 4-bit floats (h3b_fp4_rows).
 
-    codes: uint8 [rows, ceil(cols / 32) * 16], two columns to a byte, the even one in the low nibble.
+    codes: uint8 [rows, ceil(cols / 32) * 16], two columns to a byte, the even one in the low nibble; zero codes
+    behind the last column, and zero scales behind the last block.
     scales: uint8 [ceil(rows / 128), ceil(cols / (4 * block)), 512], block scales in tiles of 128 rows x 4
     blocks, the order in which the products read them (`from_blocks` and `blocks` convert from and to
-    [rows, blocks]).  row_scales: f32 [rows], or None for 1."""
+    [rows, blocks]).  row_scales: f32 [rows], or None for 1; quantize_fp4 makes some for nvfp4."""
 
     __slots__ = ("rows", "cols", "format", "_gpu", "_ref", "_buffer", "_codes", "_scales", "_row_scales", "_from", "_to")
 
